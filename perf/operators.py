@@ -160,7 +160,7 @@ def _pages(case, lens, g):
 
 
 def _quantize(x, G, bits):
-    """x [..., D] -> codes (4 bits: two a byte, the even element low), scale and minimum a group of G."""
+    """x [..., D] -> codes (4 bits: two a byte, the even element low) and [..., D / G, 2], a group's scale and minimum."""
     levels = float(2 ** bits - 1)
     v = x.reshape(*x.shape[:-1], -1, G)
     lo, hi = v.amin(-1), v.amax(-1)
@@ -168,7 +168,7 @@ def _quantize(x, G, bits):
     s = scale.float().unsqueeze(-1)
     q = torch.where(s > 0, torch.round((v - least.float().unsqueeze(-1)) / torch.where(s > 0, s, 1.0)), 0.0).clamp(0, levels).to(torch.uint8)
     q = q.reshape(x.shape)
-    return (q[..., 0::2] | (q[..., 1::2] << 4)) if bits == 4 else q, scale, least
+    return (q[..., 0::2] | (q[..., 1::2] << 4)) if bits == 4 else q, torch.stack((scale, least), -1)
 
 
 def _pool(case, n_pages, g, filled):
@@ -183,7 +183,7 @@ def _pool(case, n_pages, g, filled):
             n = min(step, n_pages - p)
             x = torch.randn((n, *shape[1:]), generator=g, device="cuda") + mean if filled else torch.zeros((n, *shape[1:]), device="cuda")
             parts.append((x.to(torch.bfloat16),) if case["bits"] == 16 else _quantize(x, case["G"], case["bits"]))
-        for key, t in zip(("", "_scale", "_min"), zip(*parts)):
+        for key, t in zip(("", "_sm"), zip(*parts)):
             pool[name + key] = torch.cat(t)
     return pool
 
@@ -254,9 +254,9 @@ def _values(st, name, page, at):
         return codes.float()
     if st["bits"] == 4:
         codes = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)
-    scale, least = st[name + "_scale"][page, :, at].float(), st[name + "_min"][page, :, at].float()
+    sm = st[name + "_sm"][page, :, at].float()
     x = codes.reshape(*codes.shape[:-1], -1, st["G"]).float()
-    return (x * scale.unsqueeze(-1) + least.unsqueeze(-1)).flatten(-2)
+    return (x * sm[..., :1] + sm[..., 1:]).flatten(-2)
 
 
 def _plain_read(st):
@@ -268,10 +268,7 @@ def _store(st, name, page, at, x):
     if st["bits"] == 16:
         st[name][page, :, at] = x.to(torch.bfloat16)
         return
-    q, scale, least = _quantize(x, st["G"], st["bits"])
-    st[name][page, :, at] = q
-    st[name + "_scale"][page, :, at] = scale
-    st[name + "_min"][page, :, at] = least
+    st[name][page, :, at], st[name + "_sm"][page, :, at] = _quantize(x, st["G"], st["bits"])
 
 
 def _plain_write(st):
@@ -322,7 +319,7 @@ def run(st):
         return _plain_read(st) if st["kind"] == "read" else _plain_attend(st)
     from strixite_b200 import kernels as K
     if "cache" not in st:  # the handle and the workspace that a program keeps
-        st["cache"] = K.KvCache(st["k"], st["v"], st["bits"], st.get("k_scale"), st.get("k_min"), st.get("v_scale"), st.get("v_min"), st["G"])
+        st["cache"] = K.KvCache(st["k"], st["v"], st["bits"], st["G"], st.get("k_sm"), st.get("v_sm"))
         if st["kind"] == "attend":
             st["ws"] = torch.zeros(K.attn_decode_workspace_bytes(st["cache"], st["n_q"], st["max_q"]), dtype=torch.uint8, device="cuda")
     if st["kind"] == "attend":
@@ -353,9 +350,8 @@ def _wide(st, name, rows_page, rows_at):
         x[..., 1::2] = (c // 16).double()
     else:
         x.copy_(c)
-    s = st[name + "_scale"][rows_page][torch.arange(len(rows_at)), :, rows_at].double()
-    m = st[name + "_min"][rows_page][torch.arange(len(rows_at)), :, rows_at].double()
-    return x * s.repeat_interleave(G, -1) + m.repeat_interleave(G, -1)
+    sm = st[name + "_sm"][rows_page][torch.arange(len(rows_at)), :, rows_at].double()
+    return x * sm[..., 0].repeat_interleave(G, -1) + sm[..., 1].repeat_interleave(G, -1)
 
 
 def _as_kept(x, G, bits):
