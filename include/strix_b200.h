@@ -506,6 +506,62 @@ int sxb_strixw_qview(const SxbStrixw *f, const char *name, int64_t N, int64_t K,
  * NULL) = the shared expert's view, or all zero when the file keeps it elsewhere. */
 int sxb_strixw_expert_views(const SxbStrixw *f, const char *name, int64_t E, SxbQView *routed, SxbQView *shared, int *bits);
 
+/* ---- Attention over a paged, quantized key-value cache ------------------------------------------------------- */
+
+/* No counterpart among the reference's launchers mirrored here (its own attention kernels are another design).  A pool of pages; a
+ * cache row is one token's key or value in one head: D elements, BF16 (bits = 16), or codes of 8 or 4 bits along D in groups of
+ * G with a scale and a min each, as in SxbQView (low nibble = even element; element = code * scale + min, both BF16).  A
+ * group's scale and min stand side by side in one 32-bit word, the scale in its lower half.
+ * Row number of (page, head, token in page) = page * page_stride + head * head_stride + token * row_stride: a row's codes start at
+ * number * D * bits / 8 bytes, its words of scales at number * D / G.  [n_pages, n_kv, page, D] has the strides n_kv * page, page, 1.
+ * D = 64, 128 or 256; G = 32, 64 or 128, at most D; page = a power of two of 8..4096; all four arrays 16-byte aligned.
+ * Token p of a sequence lies in page pages[seq * pages_ld + p / page].  A page may stand in several tables (a shared prefix). */
+typedef struct SxbKvCache {
+    void *k, *v;
+    uint32_t *k_sm, *v_sm; /* NULL for BF16 */
+    int64_t n_pages, n_kv, page, D, G;
+    int64_t page_stride, head_stride, row_stride; /* in rows */
+    int bits;
+} SxbKvCache;
+
+/* The step between the projections and the attention.  qkv [T, ld >= (n_q + 2 n_kv) D], BF16 or FP32 (act): per token the query
+ * heads, the key heads, the value heads.  Queries and keys: x / sqrt(mean(x^2) + eps) * norm weight [D] (FP32; NULL: no norm), then
+ * the first rot elements turned by pos * inv_freq[i] (FP32 [rot / 2]; the product in FP64): pairs (i, i + rot / 2), or (2i, 2i + 1)
+ * if interleaved; rot = 0: none, else a multiple of 16.  Queries to q_out [T, q_ld >= n_q D] BF16; keys and values of token t to
+ * position pos[t] of sequence seq[t]: rounded once to BF16, or quantized from the FP32 values as sxb_quantize does (a group that
+ * holds a NaN or an infinity reads back as NaN).  seq[t] < 0: a padding row, nothing of it is written.  A position or page out of
+ * range: err = {1, token, pos}, the token's queries NaN, nothing written to the cache.  No (seq, pos) twice in one call.
+ * Rows of qkv and q_out 16-byte aligned. */
+int sxb_attn_qkv_write(const void *qkv, int64_t ld, int act, int64_t T, int64_t n_q, const float *q_norm, const float *k_norm,
+                       float eps, const float *inv_freq, int64_t rot, int interleaved, const int32_t *seq, const int32_t *pos,
+                       const int32_t *pages, int64_t pages_ld, int64_t n_cols, int64_t n_seq, const SxbKvCache *cache, void *q_out,
+                       int64_t q_ld, uint32_t *err, sxb_stream_t stream);
+/* Rows of the cache back: k_out, v_out [T, n_kv, D], BF16 or FP32 (out_act) = code * scale + min in FP32, rounded once.
+ * seq, pos and err as above: seq[t] < 0 leaves the rows as they are, a bad place gives NaN. */
+int sxb_kv_read(const SxbKvCache *cache, const int32_t *seq, const int32_t *pos, const int32_t *pages, int64_t pages_ld,
+                int64_t n_cols, int64_t n_seq, int64_t T, void *k_out, void *v_out, int out_act, uint32_t *err, sxb_stream_t stream);
+/* Attention of the new tokens of B sequences over their pages.  q [T, q_ld] BF16 (n_q heads of D, as sxb_attn_qkv_write leaves them);
+ * sequence b has the rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]) and kv_len[b] keys, the new tokens' own included: its row
+ * i of n stands at position p = kv_len[b] - n + i and sees the keys j <= p, with window > 0 only j > p - window.  Query head h
+ * reads key head h / (n_q / n_kv).  Scores scale * q . k, with softcap > 0 softcap * tanh(score / softcap).
+ * out [T, out_ld] BF16 = softmax(scores) . V, lse [T, n_q] FP32 (or NULL) = log of the sum of exp(score); a row that sees no key
+ * (or none with a score above -inf): 0 and -inf.  Rows outside every sequence are left as they are.  Scores, statistics and
+ * sums are FP32; weights are rounded to BF16 (BF16 cache) or, times a group's scale, to F16 for the product with V.
+ * max_q: a sequence's largest count of new tokens, which picks the kernel (a sequence with more is handled, in several passes over
+ * its keys).  Made for a token and its drafts; long chunks of queries are right but no match for a prefill kernel.
+ * ws: sxb_attn_decode_workspace_bytes, device, 16-byte aligned, zeroed once before its first use; every call leaves what it needs
+ * of it zeroed.  Calls that share a workspace must be ordered (one stream, or events); the sizes depend on the device.
+ * Data errors (err = {1, sequence, value}): a page id out of range makes the keys on that page NaN; kv_len outside
+ * 0 .. n_cols * page makes the sequence's rows NaN; a q_start that falls or leaves 0..T skips the sequence. */
+size_t sxb_attn_decode_workspace_bytes(int64_t n_q, int64_t n_kv, int64_t D, int bits, int64_t max_q);
+int sxb_attn_decode(const void *q, int64_t q_ld, int64_t T, int64_t n_q, const SxbKvCache *cache, const int32_t *pages,
+                    int64_t pages_ld, int64_t n_cols, const int32_t *q_start, const int32_t *kv_len, int64_t B, int64_t max_q,
+                    float scale, float softcap, int64_t window, void *out, int64_t out_ld, float *lse, void *ws, size_t ws_bytes,
+                    uint32_t *err, sxb_stream_t stream);
+/* The error words of the three (a blocking 12-byte copy, as sxb_check_router_error) / already on the host. */
+int sxb_check_attn_error(const uint32_t *err, const char *what);
+int sxb_report_attn_error(const uint32_t e[3], const char *what);
+
 /* ---- Quantizers on the device ------------------------------------------------------------------------------- */
 
 /* formats/q4.hpp:32 quantize_q4 / formats/q8.hpp:32 quantize_q8, for weights already on the device: w [N, K] FP32 ->

@@ -26,6 +26,13 @@ class SxbMoeSharedAdd(C.Structure):
     _fields_ = [("s", vp), ("gate_logit", vp), ("gate_ld", i64), ("gate_index", u32), ("err", vp)]
 
 
+class SxbKvCache(C.Structure):
+    """A paged key-value cache (include/strix_b200.h), field for field."""
+
+    _fields_ = [("k", vp), ("v", vp), ("k_sm", vp), ("v_sm", vp), ("n_pages", i64), ("n_kv", i64), ("page", i64), ("D", i64), ("G", i64),
+                ("page_stride", i64), ("head_stride", i64), ("row_stride", i64), ("bits", C.c_int)]
+
+
 class SxbStrixwTensor(C.Structure):
     """formats/strixw.hpp:37-48 StrixwTensor, flattened (include/strix_b200.h)."""
 
@@ -48,6 +55,7 @@ class SxbMoeLayerArgs(C.Structure):
 
 QV = C.POINTER(SxbQView)
 SA = C.POINTER(SxbMoeSharedAdd)
+KV = C.POINTER(SxbKvCache)
 
 # name -> (restype, argtypes); mirrors include/strix_b200.h declaration by declaration.
 SIGNATURES = {
@@ -123,6 +131,14 @@ SIGNATURES = {
     "sxb_hc_mix_up_wmma_q8": (C.c_int, [vp, QV, vp, vp, vp, i64, i64, i64, vp, vp, sz, C.c_int, vp]),
     "sxb_moe_route_small": (C.c_int, [vp, i64, i64, i64, i64, i64, i64, vp, vp, vp, sz, vp, vp, vp]),
 }
+SIGNATURES.update({
+    "sxb_attn_qkv_write": (C.c_int, [vp, i64, C.c_int, i64, i64, vp, vp, C.c_float, vp, i64, C.c_int, vp, vp, vp, i64, i64, i64, KV, vp, i64, vp, vp]),
+    "sxb_kv_read": (C.c_int, [KV, vp, vp, vp, i64, i64, i64, i64, vp, vp, C.c_int, vp, vp]),
+    "sxb_attn_decode_workspace_bytes": (sz, [i64, i64, i64, C.c_int, i64]),
+    "sxb_attn_decode": (C.c_int, [vp, i64, i64, i64, KV, vp, i64, i64, vp, vp, i64, i64, C.c_float, C.c_float, i64, vp, i64, vp, vp, sz, vp, vp]),
+    "sxb_check_attn_error": (C.c_int, [vp, cp]),
+    "sxb_report_attn_error": (C.c_int, [C.POINTER(u32), cp]),
+})
 for _b in ("q4", "q8"):
     SIGNATURES[f"sxb_linear_{_b}_experts_gather"] = (C.c_int, [vp, QV, i64, vp, i64, i64, vp, C.c_int, vp, vp])
     SIGNATURES[f"sxb_linear_{_b}_experts_gather_swiglu"] = (C.c_int, [vp, QV, i64, vp, i64, i64, vp, C.c_int, vp, vp])

@@ -1,0 +1,370 @@
+// The cache side of a decode step's attention: queries and keys normed per head and rotated by their position, keys and values into their pages
+// (sxb_attn_qkv_write), and rows of the cache back (sxb_kv_read).
+//
+//   x' = x / sqrt(mean(x^2) + eps) * w,   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = pos * inv_freq[i]
+//
+// One pass: a warp has a head of a token in registers (D / 32 neighbouring elements a lane), the norm's sum, the rotation's partner and a group's
+// extremes go by shuffles.  All FP32, but for the angle: pos * inv_freq loses 2^-24 of a number of turns that grows with the position (a hundred thousand
+// tokens: 6e-3 of a radian), so product and reduction are FP64, once a token and angle, into shared memory for all of its heads.
+// The same formulas as sxb_quantize's make the codes (formats/q4.cpp:44-88), from the FP32 values: nothing is rounded on the way.
+
+#include "attn.cuh"
+
+namespace sxb {
+namespace {
+
+constexpr int kWriteWarps = 8, kWriteThreads = 32 * kWriteWarps;
+constexpr int64_t kMaxTokens = 1ll << 24;
+
+struct WriteArgs {
+    const void *qkv;
+    int64_t ld;
+    int n_q, n_kv, rot, interleaved;
+    const float *q_norm, *k_norm, *inv_freq;
+    float eps;
+    const int32_t *seq, *pos, *pages;
+    int64_t pages_ld;
+    int n_seq, n_cols, G, heads_per_cta;
+    KvView c;
+    uint16_t *q_out;
+    int64_t q_ld;
+    uint32_t *err;
+};
+
+// N neighbouring elements (4 to 32 bytes, aligned to them) as FP32, and back.
+template <int BYTES> struct Words { uint32_t w[BYTES / 4]; };
+template <int BYTES> __device__ inline Words<BYTES> load_words(const void *p) {
+    Words<BYTES> r;
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4 *>(r.w)[i] = reinterpret_cast<const uint4 *>(p)[i];
+    } else if constexpr (BYTES == 8) {
+        *reinterpret_cast<uint2 *>(r.w) = *reinterpret_cast<const uint2 *>(p);
+    } else {
+        r.w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+    return r;
+}
+template <int BYTES> __device__ inline void store_words(void *p, const Words<BYTES> &r) {
+    if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(r.w)[i];
+    } else if constexpr (BYTES == 8) {
+        *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(r.w);
+    } else {
+        *reinterpret_cast<uint32_t *>(p) = r.w[0];
+    }
+}
+template <typename T, int N> __device__ inline void load_run(const T *p, float (&v)[N]) {
+    const auto r = load_words<N * (int)sizeof(T)>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(r.w[i]);
+        else v[i] = __uint_as_float(i & 1 ? r.w[i / 2] & 0xffff0000u : r.w[i / 2] << 16);
+    }
+}
+template <int N> __device__ inline void store_bf16_run(uint16_t *p, const float (&v)[N]) {
+    Words<2 * N> r;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) r.w[i] = (uint32_t)f32_to_bf16_bits(v[2 * i]) | (uint32_t)f32_to_bf16_bits(v[2 * i + 1]) << 16;
+    store_words<2 * N>(p, r);
+}
+
+// A head's elements into a cache row.  BITS 16: rounded to BF16.  Otherwise a group's lanes find its extremes; a group that holds a NaN or an infinity
+// has no code that stands for it and reads back as NaN throughout.
+template <int D, int BITS>
+__device__ inline void store_row(uint8_t *rows, uint32_t *sm, int64_t row, const float (&v)[D / 32], int lane, int G) {
+    constexpr int N = D / 32;
+    if constexpr (BITS == 16) {
+        store_bf16_run(reinterpret_cast<uint16_t *>(rows) + row * D + lane * N, v);
+    } else {
+        constexpr float kLevels = BITS == 4 ? 15.f : 255.f;
+        const int lanes = G / N;  // of a group: a power of two, 4 to 32 (G = 128 at D = 64 is refused)
+        float lo = v[0], hi = v[0];
+        bool bad = !isfinite(v[0]);
+#pragma unroll
+        for (int i = 1; i < N; ++i) lo = fminf(lo, v[i]), hi = fmaxf(hi, v[i]), bad = bad || !isfinite(v[i]);
+        for (int off = 1; off < lanes; off <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+            bad = __shfl_xor_sync(0xffffffffu, (int)bad, off) || bad;
+        }
+        const uint32_t s_bits = bad ? 0x7fc0u : f32_to_bf16_bits(__fdiv_rn(__fsub_rn(hi, lo), kLevels)), m_bits = bad ? 0x7fc0u : f32_to_bf16_bits(lo);
+        const float s = bf16_bits_to_f32((uint16_t)s_bits), m = bf16_bits_to_f32((uint16_t)m_bits);
+        if (lane % lanes == 0) sm[row * (D / G) + lane / lanes] = s_bits | m_bits << 16;
+        uint32_t packed[(N * BITS + 31) / 32] = {};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            uint32_t code = 0;
+            if (s > 0.f) code = (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v[i], m), s)), 0.f), kLevels);
+            packed[i * BITS / 32] |= code << (i * BITS % 32);
+        }
+        constexpr int kLaneBytes = N * BITS / 8;  // 1 to 8
+        uint8_t *dst = rows + row * (D * BITS / 8) + lane * kLaneBytes;
+        if constexpr (kLaneBytes >= 4) store_words<kLaneBytes>(dst, *reinterpret_cast<const Words<kLaneBytes> *>(packed));
+        else if constexpr (kLaneBytes == 2) *reinterpret_cast<uint16_t *>(dst) = (uint16_t)packed[0];
+        else *dst = (uint8_t)packed[0];
+    }
+}
+
+// Cache row of (sequence, position), or why there is none: 0 = found, 1 = a row to leave alone, 2 = bad.
+struct Place {
+    int page, at, state;
+};
+__device__ inline Place find_place(int seq, int pos, const int32_t *pages, int64_t pages_ld, int n_seq, int n_cols, const KvView &c) {
+    Place p{0, 0, 0};
+    if (seq < 0) {
+        p.state = 1;
+    } else if (seq >= n_seq || pos < 0 || (pos >> c.page_shift) >= n_cols) {
+        p.state = 2;
+    } else {
+        p.page = pages[seq * pages_ld + (pos >> c.page_shift)];
+        p.at = pos & ((1 << c.page_shift) - 1);
+        if ((unsigned)p.page >= (unsigned)c.n_pages) p.state = 2;
+    }
+    return p;
+}
+
+template <typename T, int D, int BITS>
+__global__ void __launch_bounds__(kWriteThreads) qkv_write_kernel(const __grid_constant__ WriteArgs a) {
+    __shared__ float2 turn[D / 2];  // cos, sin of the token's angles
+    behind_grid();
+    constexpr int N = D / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t t = blockIdx.x;
+    const int seq = a.seq[t], pos = a.pos[t];
+    const Place place = find_place(seq, pos, a.pages, a.pages_ld, a.n_seq, a.n_cols, a.c);
+    if (place.state == 1) return;
+    const int half = a.rot / 2;
+    if ((int)threadIdx.x < half) {
+        // the angle less whole turns: what is left of 2^31 * inv_freq in FP64 is good to 2^-22 of a radian, of 2^20 * 1 to 2^-33
+        const double angle = (double)pos * (double)a.inv_freq[threadIdx.x];
+        const double turns = rint(angle * 0.15915494309189533577);
+        float s, c;
+        sincosf((float)fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, angle)), &s, &c);
+        turn[threadIdx.x] = make_float2(c, s);
+    }
+    __syncthreads();
+    const int heads = a.n_q + 2 * a.n_kv, first = blockIdx.y * a.heads_per_cta, last = min(heads, first + a.heads_per_cta);
+    if (place.state == 2 && threadIdx.x == 0 && first == 0) raise_error(a.err, (uint32_t)t, (uint32_t)pos);
+    for (int h = first + warp; h < last; h += kWriteWarps) {
+        const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
+        float v[N];
+        load_run<T, N>(static_cast<const T *>(a.qkv) + t * a.ld + (int64_t)h * D + lane * N, v);
+        if (is_q || is_k) {
+            const float *w = is_q ? a.q_norm : a.k_norm;
+            if (w != nullptr) {
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum = fmaf(v[i], v[i], sum);
+#pragma unroll
+                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                const float inv = 1.0f / sqrtf(sum * (1.0f / D) + a.eps);
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = v[i] * inv * w[lane * N + i];
+            }
+            if (a.rot != 0) {
+                const bool turned = lane * N < a.rot;
+                if (a.interleaved) {
+                    if (turned) {
+#pragma unroll
+                        for (int i = 0; i < N; i += 2) {
+                            const float2 cs = turn[(lane * N + i) / 2];
+                            const float x = v[i], y = v[i + 1];
+                            v[i] = x * cs.x - y * cs.y, v[i + 1] = y * cs.x + x * cs.y;
+                        }
+                    }
+                } else {
+                    const int off = half / N;  // lanes to the partner: half is a multiple of 8 >= N
+                    const bool low = lane < off;
+                    const int from = turned ? (low ? lane + off : lane - off) : lane;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float other = __shfl_sync(0xffffffffu, v[i], from);
+                        if (turned) {
+                            const float2 cs = turn[low ? lane * N + i : lane * N + i - half];
+                            v[i] = low ? v[i] * cs.x - other * cs.y : v[i] * cs.x + other * cs.y;
+                        }
+                    }
+                }
+            }
+        }
+        if (is_q) {
+            if (place.state == 2) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = qnan_f32();
+            }
+            store_bf16_run(a.q_out + t * a.q_ld + (int64_t)h * D + lane * N, v);
+        } else if (place.state == 0) {
+            const int kv = is_k ? h - a.n_q : h - a.n_q - a.n_kv;
+            store_row<D, BITS>(is_k ? a.c.k : a.c.v, is_k ? a.c.k_sm : a.c.v_sm, kv_row(a.c, place.page, kv, place.at), v, lane, a.G);
+        }
+    }
+}
+
+struct ReadArgs {
+    const int32_t *seq, *pos, *pages;
+    int64_t pages_ld, items;
+    int n_seq, n_cols, G;
+    KvView c;
+    void *k_out, *v_out;
+    uint32_t *err;
+};
+
+// Eight elements a thread: neighbouring threads have neighbouring runs of a row.
+template <typename T, int D, int BITS>
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ ReadArgs a) {
+    behind_grid();
+    constexpr int kRuns = D / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.items; i += (int64_t)gridDim.x * 256) {
+        const int run = (int)(i % kRuns);
+        const int64_t row = i / kRuns, t = row / (2 * a.c.n_kv);
+        const int h = (int)(row - t * 2 * a.c.n_kv);
+        const bool is_k = h < a.c.n_kv;
+        const int head = is_k ? h : h - a.c.n_kv;
+        const Place place = find_place(a.seq[t], a.pos[t], a.pages, a.pages_ld, a.n_seq, a.n_cols, a.c);
+        if (place.state == 1) continue;
+        float v[8];
+        if (place.state == 2) {
+            if (h == 0 && run == 0) raise_error(a.err, (uint32_t)t, (uint32_t)a.pos[t]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = qnan_f32();
+        } else {
+            const int64_t from = kv_row(a.c, place.page, head, place.at);
+            const uint8_t *p = (is_k ? a.c.k : a.c.v) + from * (D * BITS / 8) + run * BITS;
+            if constexpr (BITS == 16) {
+                load_run(reinterpret_cast<const uint16_t *>(p), v);
+            } else {
+                const auto w = load_words<BITS>(p);
+                const uint32_t sm = (is_k ? a.c.k_sm : a.c.v_sm)[from * (D / a.G) + run * 8 / a.G];
+                const float s = __uint_as_float(sm << 16), m = __uint_as_float(sm & 0xffff0000u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = fmaf((float)((w.w[e * BITS / 32] >> (e * BITS % 32)) & ((1u << BITS) - 1)), s, m);
+            }
+        }
+        T *to = static_cast<T *>(is_k ? a.k_out : a.v_out) + ((t * a.c.n_kv + head) * D + run * 8);
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            store_bf16_run(to, v);
+        }
+    }
+}
+
+template <typename T>
+cudaError_t launch_write(const WriteArgs &a, int D, int bits, dim3 grid, cudaStream_t st) {
+#define SXB_W(DD, BB) \
+    if (D == DD && bits == BB) return launch_behind(qkv_write_kernel<T, DD, BB>, grid, kWriteThreads, 0, st, 1, a)
+    SXB_W(64, 16); SXB_W(64, 8); SXB_W(64, 4);
+    SXB_W(128, 16); SXB_W(128, 8); SXB_W(128, 4);
+    SXB_W(256, 16); SXB_W(256, 8); SXB_W(256, 4);
+#undef SXB_W
+    return cudaErrorInvalidValue;
+}
+template <typename T>
+cudaError_t launch_read(const ReadArgs &a, int D, int bits, unsigned grid, cudaStream_t st) {
+#define SXB_R(DD, BB) \
+    if (D == DD && bits == BB) return launch_behind(kv_read_kernel<T, DD, BB>, grid, 256, 0, st, 1, a)
+    SXB_R(64, 16); SXB_R(64, 8); SXB_R(64, 4);
+    SXB_R(128, 16); SXB_R(128, 8); SXB_R(128, 4);
+    SXB_R(256, 16); SXB_R(256, 8); SXB_R(256, 4);
+#undef SXB_R
+    return cudaErrorInvalidValue;
+}
+
+int check_places(const char *fn, const int32_t *seq, const int32_t *pos, const int32_t *pages, int64_t pages_ld, int64_t n_cols, int64_t n_seq, int64_t T,
+                 const SxbKvCache *c, const uint32_t *err) {
+    SXB_CHECK(seq != nullptr && pos != nullptr && pages != nullptr && err != nullptr, fn, ": null pointer (seq=", (const void *)seq, ", pos=",
+              (const void *)pos, ", pages=", (const void *)pages, ", err=", (const void *)err, ")");
+    SXB_CHECK(T >= 1 && T <= kMaxTokens, fn, ": T = ", T, " tokens, expected 1..2^24");
+    SXB_CHECK(n_seq >= 1 && n_seq <= (1 << 20), fn, ": n_seq = ", n_seq, ", expected 1..2^20");
+    SXB_CHECK(n_cols >= 1 && pages_ld >= n_cols, fn, ": page table of ", n_cols, " columns with a stride of ", pages_ld);
+    SXB_CHECK(n_cols <= ((1ll << 31) - 1024) / c->page, fn, ": ", n_cols, " pages of ", c->page, " tokens a sequence, positions end below 2^31 - 1024");
+    return SXB_OK;
+}
+
+}  // namespace
+
+int kv_view(const char *fn, const SxbKvCache *c, KvView *out) {
+    SXB_CHECK(c != nullptr, fn, ": null cache");
+    SXB_CHECK(c->bits == 16 || c->bits == 8 || c->bits == 4, fn, ": cache of ", c->bits, " bits unsupported (16 = BF16, 8 or 4)");
+    SXB_CHECK(c->D == 64 || c->D == 128 || c->D == 256, fn, ": heads of ", c->D, " elements unsupported (64, 128 or 256)");
+    SXB_CHECK(c->k != nullptr && c->v != nullptr, fn, ": null pointer (cache k=", c->k, ", v=", c->v, ")");
+    SXB_CHECK(aligned16(c->k) && aligned16(c->v), fn, ": cache k and v must be 16-byte aligned");
+    if (c->bits != 16) {
+        SXB_CHECK((c->G == 32 || c->G == 64 || c->G == 128) && c->G <= c->D, fn, ": group size ", c->G, " unsupported (32, 64 or 128, at most D = ", c->D, ")");
+        SXB_CHECK(c->k_sm != nullptr && c->v_sm != nullptr, fn, ": null pointer (cache k_sm=", (const void *)c->k_sm, ", v_sm=", (const void *)c->v_sm, ")");
+        SXB_CHECK(aligned16(c->k_sm) && aligned16(c->v_sm), fn, ": cache k_sm and v_sm must be 16-byte aligned");
+    }
+    SXB_CHECK(c->n_pages >= 1 && c->n_pages < (1ll << 31), fn, ": n_pages = ", c->n_pages, ", expected 1..2^31 - 1");
+    SXB_CHECK(c->n_kv >= 1 && c->n_kv <= 1024, fn, ": n_kv = ", c->n_kv, " heads, expected 1..1024");
+    SXB_CHECK(is_pow2(c->page) && c->page >= 8 && c->page <= 4096, fn, ": pages of ", c->page, " tokens, expected a power of two of 8..4096");
+    SXB_CHECK(c->page_stride >= 1 && c->head_stride >= 1 && c->row_stride >= 1 && c->page_stride < (1ll << 32) && c->head_stride < (1ll << 32) &&
+                  c->row_stride < (1ll << 32),
+              fn, ": strides of ", c->page_stride, " / ", c->head_stride, " / ", c->row_stride, " rows (page / head / token), expected 1..2^32 - 1");
+    *out = KvView{static_cast<uint8_t *>(c->k), static_cast<uint8_t *>(c->v), c->k_sm, c->v_sm, c->page_stride, c->head_stride, c->row_stride,
+                  (int)c->n_pages, __builtin_ctzll((unsigned long long)c->page), (int)c->n_kv};
+    return SXB_OK;
+}
+
+}  // namespace sxb
+
+using namespace sxb;
+
+extern "C" int sxb_attn_qkv_write(const void *qkv, int64_t ld, int act, int64_t T, int64_t n_q, const float *q_norm, const float *k_norm, float eps,
+                                  const float *inv_freq, int64_t rot, int interleaved, const int32_t *seq, const int32_t *pos, const int32_t *pages,
+                                  int64_t pages_ld, int64_t n_cols, int64_t n_seq, const SxbKvCache *cache, void *q_out, int64_t q_ld, uint32_t *err,
+                                  sxb_stream_t stream) {
+    const char *fn = "attn_qkv_write";
+    WriteArgs a{};
+    if (int rc = kv_view(fn, cache, &a.c)) return rc;
+    if (int rc = check_places(fn, seq, pos, pages, pages_ld, n_cols, n_seq, T, cache, err)) return rc;
+    SXB_CHECK(qkv != nullptr && q_out != nullptr, fn, ": null pointer (qkv=", qkv, ", q_out=", q_out, ")");
+    SXB_CHECK(act_ok(act), fn, ": unsupported activation dtype ", act);
+    SXB_CHECK(n_q >= 1 && n_q <= 1024, fn, ": n_q = ", n_q, " heads, expected 1..1024");
+    const int64_t D = cache->D, heads = n_q + 2 * cache->n_kv, es = act_bytes(act);
+    SXB_CHECK(ld >= heads * D && ld <= (1ll << 32) && q_ld >= n_q * D && q_ld <= (1ll << 32), fn, ": row strides ", ld, " and ", q_ld, ", rows have ",
+              heads * D, " and ", n_q * D, " elements");
+    SXB_CHECK(aligned16(qkv) && aligned16(q_out) && ld * es % 16 == 0 && q_ld % 8 == 0, fn, ": rows of qkv and q_out must be 16-byte aligned");
+    SXB_CHECK(apart(qkv, ((T - 1) * ld + heads * D) * es, q_out, ((T - 1) * q_ld + n_q * D) * 2), fn, ": q_out [", q_out, "] overlaps qkv [", qkv, "]");
+    SXB_CHECK(inv_freq != nullptr || rot == 0, fn, ": rot = ", rot, " without inv_freq");
+    SXB_CHECK(rot >= 0 && rot <= D && rot % 16 == 0, fn, ": rot = ", rot, ", expected a multiple of 16 of 0..", D);
+    SXB_CHECK((q_norm == nullptr && k_norm == nullptr) || (eps > 0.f && eps < 1e30f), fn, ": eps must be finite and positive");
+    a.qkv = qkv, a.ld = ld, a.n_q = (int)n_q, a.n_kv = (int)cache->n_kv, a.rot = (int)rot, a.interleaved = interleaved != 0;
+    a.q_norm = q_norm, a.k_norm = k_norm, a.inv_freq = inv_freq, a.eps = eps;
+    a.seq = seq, a.pos = pos, a.pages = pages, a.pages_ld = pages_ld, a.n_seq = (int)n_seq, a.n_cols = (int)n_cols;
+    a.G = (int)(cache->bits == 16 ? D : cache->G), a.q_out = static_cast<uint16_t *>(q_out), a.q_ld = q_ld, a.err = err;
+    // few tokens: a head a warp, so that the SMs share them; many: a CTA has all heads of its token and its angles are computed once
+    const int64_t whole = (heads + kWriteWarps - 1) / kWriteWarps;
+    const int64_t parts = std::min(whole, std::max<int64_t>(1, 4 * (int64_t)sm_count() / T));
+    a.heads_per_cta = (int)((whole + parts - 1) / parts) * kWriteWarps;
+    const dim3 grid((unsigned)T, (unsigned)((heads + a.heads_per_cta - 1) / a.heads_per_cta));
+    auto st = static_cast<cudaStream_t>(stream);
+    if (act == SXB_ACT_F32) launch_write<float>(a, (int)D, cache->bits, grid, st);
+    else launch_write<uint16_t>(a, (int)D, cache->bits, grid, st);
+    SXB_CHECK_LAUNCH(fn, " ", act_name(act), " T=", T, " n_q=", n_q, " n_kv=", cache->n_kv, " D=", D, " bits=", cache->bits);
+    return SXB_OK;
+}
+
+extern "C" int sxb_kv_read(const SxbKvCache *cache, const int32_t *seq, const int32_t *pos, const int32_t *pages, int64_t pages_ld, int64_t n_cols,
+                           int64_t n_seq, int64_t T, void *k_out, void *v_out, int out_act, uint32_t *err, sxb_stream_t stream) {
+    const char *fn = "kv_read";
+    ReadArgs a{};
+    if (int rc = kv_view(fn, cache, &a.c)) return rc;
+    if (int rc = check_places(fn, seq, pos, pages, pages_ld, n_cols, n_seq, T, cache, err)) return rc;
+    SXB_CHECK(k_out != nullptr && v_out != nullptr, fn, ": null pointer (k_out=", k_out, ", v_out=", v_out, ")");
+    SXB_CHECK(act_ok(out_act), fn, ": unsupported output dtype ", out_act);
+    SXB_CHECK(aligned16(k_out) && aligned16(v_out), fn, ": k_out and v_out must be 16-byte aligned");
+    const int64_t D = cache->D, bytes = T * cache->n_kv * D * act_bytes(out_act);
+    SXB_CHECK(apart(k_out, bytes, v_out, bytes), fn, ": v_out [", v_out, "] overlaps k_out [", k_out, "]");
+    a.seq = seq, a.pos = pos, a.pages = pages, a.pages_ld = pages_ld, a.n_seq = (int)n_seq, a.n_cols = (int)n_cols;
+    a.G = (int)(cache->bits == 16 ? D : cache->G), a.k_out = k_out, a.v_out = v_out, a.err = err;
+    a.items = T * 2 * cache->n_kv * (D / 8);
+    const unsigned grid = (unsigned)std::min<int64_t>((a.items + 255) / 256, (int64_t)sm_count() * 32);
+    auto st = static_cast<cudaStream_t>(stream);
+    if (out_act == SXB_ACT_F32) launch_read<float>(a, (int)D, cache->bits, grid, st);
+    else launch_read<uint16_t>(a, (int)D, cache->bits, grid, st);
+    SXB_CHECK_LAUNCH(fn, " ", act_name(out_act), " T=", T, " n_kv=", cache->n_kv, " D=", D, " bits=", cache->bits);
+    return SXB_OK;
+}

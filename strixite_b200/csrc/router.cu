@@ -200,6 +200,19 @@ int sxb_check_expert_error(const uint32_t *err, const char *what) {
     return sxb_report_expert_error(e, what);
 }
 
+int sxb_report_attn_error(const uint32_t e[3], const char *what) {
+    if (e[0] == 0) return SXB_OK;
+    last_error() = cat(what, ": page, position, length or row range out of range at token or sequence ", e[1], " (", (int32_t)e[2],
+                       "); the affected outputs are NaN");
+    return SXB_ERR_DATA;
+}
+
+int sxb_check_attn_error(const uint32_t *err, const char *what) {
+    uint32_t e[3];
+    if (int rc = read_err_words(err, e, "check_attn_error", what)) return rc;
+    return sxb_report_attn_error(e, what);
+}
+
 static int shared_add_impl(const char *fn, void *y, const void *s, const float *gate_logit, int64_t gate_ld, int64_t M,
                            int64_t N, uint32_t gate_index, void *x, const float *w_in, int64_t H, bool inject, int act,
                            uint32_t *err, sxb_stream_t stream) {

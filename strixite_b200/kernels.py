@@ -439,6 +439,157 @@ def quantize(w: torch.Tensor, G: int, bits: int, err: Optional[torch.Tensor] = N
     return QDeviceView(q, scale, minv, N, K, G, bits)
 
 
+# ---- attention over a paged key-value cache (no counterpart among the launchers mirrored above) -------------------
+
+def _on(dev, what: str, **tensors):
+    """Refuses what the kernels would take for something else: {name: (tensor, dtypes)} on another device than the cache's, of another type, or
+    not contiguous along its last dimension."""
+    for name, (t, dtypes) in tensors.items():
+        if t is None:
+            continue
+        if t.device != dev or t.dtype not in dtypes or (t.dim() and t.stride(-1) != 1 and t.shape[-1] != 1):
+            raise Error(1, f"{what}: {name} is {t.dtype} on {t.device} with strides {tuple(t.stride())}, expected {' or '.join(map(str, dtypes))} on {dev}, "
+                           "its last dimension contiguous")
+
+
+_I32, _F32, _ROWS = (torch.int32,), (torch.float32,), (torch.bfloat16, torch.float32)
+_BF16 = (torch.bfloat16,)
+
+
+class KvCache:
+    """A pool of pages of keys and values (SxbKvCache).  k, v: BF16 [n_pages, n_kv, page, D] (bits 16), or uint8 codes of that shape (8) or
+    [n_pages, n_kv, page, D / 2] (4) with k_sm, v_sm [n_pages, n_kv, page, D / G, 2] BF16, a group's scale and min.  The first three
+    dimensions may have any strides, the same ones (in rows) for all: a transposed view of [n_pages, page, n_kv, D] is fine."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, bits: int, G: int = 0, k_sm: Optional[torch.Tensor] = None, v_sm: Optional[torch.Tensor] = None):
+        if bits not in (16, 8, 4):
+            raise Error(1, f"KvCache: {bits} bits unsupported (16 = BF16, 8 or 4)")
+        if k.dim() != 4 or v.shape != k.shape:
+            raise Error(1, f"KvCache: k {tuple(k.shape)} and v {tuple(v.shape)}, expected the same [n_pages, n_kv, page, D]")
+        if not k.is_cuda:
+            raise Error(1, "KvCache: the cache must live on a CUDA device (no CPU path exists)")
+        self.n_pages, self.n_kv, self.page = k.shape[:3]
+        self.D = k.shape[3] * (2 if bits == 4 else 1)
+        self.bits, self.G, self.device = bits, (self.D if bits == 16 else G), k.device
+        codes = _BF16 if bits == 16 else (torch.uint8,)
+        _on(k.device, "KvCache", k=(k, codes), v=(v, codes))
+        parts = [(k, k.shape[3]), (v, k.shape[3])]
+        if bits != 16:
+            if G not in (32, 64, 128) or G > self.D:
+                raise Error(1, f"KvCache: group size {G} unsupported (32, 64 or 128, at most D = {self.D})")
+            groups = self.D // G
+            for name, t in (("k_sm", k_sm), ("v_sm", v_sm)):
+                if t is None or tuple(t.shape) != (*k.shape[:3], groups, 2) or t.stride(3) != 2:
+                    raise Error(1, f"KvCache: {name} is {None if t is None else tuple(t.shape)}, expected {(*k.shape[:3], groups, 2)}, a row's groups contiguous")
+            _on(k.device, "KvCache", k_sm=(k_sm, _BF16), v_sm=(v_sm, _BF16))
+            parts += [(k_sm, 2 * groups), (v_sm, 2 * groups)]
+        elif k_sm is not None or v_sm is not None:
+            raise Error(1, "KvCache: a BF16 cache has no scales")
+        rows = None
+        for t, n in parts:
+            # a dimension of one has no stride to speak of
+            here = tuple(t.stride(i) / n if t.shape[i] > 1 else 1 for i in range(3))
+            if any(r != int(r) or r < 1 for r in here) or (rows is not None and here != rows):
+                raise Error(1, f"KvCache: strides {tuple(t.stride())} are not whole rows of {n}, or not those of k")
+            rows = here
+        self.k, self.v, self.k_sm, self.v_sm = k, v, k_sm, v_sm
+        self._c = _lib.SxbKvCache(k.data_ptr(), v.data_ptr(), _ptr(k_sm), _ptr(v_sm), self.n_pages, self.n_kv, self.page, self.D, self.G,
+                                  *[int(r) for r in rows], bits)
+        self._by_ref = C.byref(self._c)
+
+    @classmethod
+    def empty(cls, n_pages: int, n_kv: int, page: int, D: int, bits: int, G: int = 64, device="cuda") -> "KvCache":
+        """A pool of zeros."""
+        def zeros(*shape, dtype):
+            return torch.zeros((n_pages, n_kv, page, *shape), dtype=dtype, device=device)
+        if bits == 16:
+            return cls(zeros(D, dtype=torch.bfloat16), zeros(D, dtype=torch.bfloat16), 16)
+        n = D // 2 if bits == 4 else D
+        return cls(zeros(n, dtype=torch.uint8), zeros(n, dtype=torch.uint8), bits, G, zeros(D // G, 2, dtype=torch.bfloat16),
+                   zeros(D // G, 2, dtype=torch.bfloat16))
+
+    def bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_sm, self.v_sm) if t is not None)
+
+
+def _places(what: str, cache: KvCache, seq, pos, pages, err, T: int):
+    _on(cache.device, what, seq=(seq, _I32), pos=(pos, _I32), pages=(pages, _I32), err=(err, (torch.int32, torch.uint32)))
+    if pages.dim() != 2 or seq.shape != (T,) or pos.shape != (T,):
+        raise Error(1, f"{what}: pages {tuple(pages.shape)}, seq {tuple(seq.shape)}, pos {tuple(pos.shape)}, expected [n_seq, n_cols] and [{T}] twice")
+
+
+def _here(cache: KvCache, what: str):
+    if cache.device.index != torch.cuda.current_device():
+        raise Error(1, f"{what}: the cache lives on {cache.device}, the current device is {torch.cuda.current_device()}")
+
+
+def attn_qkv_write(qkv, cache: KvCache, seq, pos, pages, q_out, err, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None, interleaved=False, stream=None):
+    """sxb_attn_qkv_write: qkv [T, (n_q + 2 n_kv) D] BF16 or FP32 -> queries normed and rotated into q_out [T, n_q D] BF16, keys and values into the
+    cache at position pos [T] of sequence seq [T] (int32; seq < 0: a padding row), pages [n_seq, n_cols] int32.  q_norm, k_norm [D] FP32 or None;
+    inv_freq [rot / 2] FP32 or None.  err: 3 or more zeroed int32."""
+    what = "attn_qkv_write"
+    T, D = qkv.shape[0], cache.D
+    _here(cache, what)
+    _places(what, cache, seq, pos, pages, err, T)
+    _on(cache.device, what, qkv=(qkv, _ROWS), q_out=(q_out, _BF16), q_norm=(q_norm, _F32), k_norm=(k_norm, _F32), inv_freq=(inv_freq, _F32))
+    n_q, rest = divmod(qkv.shape[1] - 2 * cache.n_kv * D, D)
+    if rest or n_q < 1 or tuple(q_out.shape) != (T, n_q * D) or any(w is not None and w.shape != (D,) for w in (q_norm, k_norm)):
+        raise Error(1, f"{what}: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)} or a norm weight does not fit {cache.n_kv} key heads of {D}")
+    _check(_lib.load().sxb_attn_qkv_write(_ptr(qkv), qkv.stride(0) if T > 1 else qkv.shape[1], 0 if qkv.dtype == torch.float32 else 1, T, n_q, _ptr(q_norm), _ptr(k_norm),
+                                          eps, _ptr(inv_freq), 0 if inv_freq is None else 2 * inv_freq.numel(), int(bool(interleaved)), _ptr(seq),
+                                          _ptr(pos), _ptr(pages), pages.stride(0) if pages.shape[0] > 1 else pages.shape[1], pages.shape[1], pages.shape[0], cache._by_ref, _ptr(q_out),
+                                          q_out.stride(0) if T > 1 else q_out.shape[1], _ptr(err), _stream(stream)))
+
+
+def kv_read(cache: KvCache, seq, pos, pages, k_out, v_out, err, stream=None):
+    """sxb_kv_read: positions pos [T] of sequences seq [T] of the cache -> k_out, v_out [T, n_kv, D], BF16 or FP32."""
+    what = "kv_read"
+    T = seq.shape[0]
+    _here(cache, what)
+    _places(what, cache, seq, pos, pages, err, T)
+    _on(cache.device, what, k_out=(k_out, _ROWS), v_out=(v_out, (k_out.dtype,)))
+    for t in (k_out, v_out):
+        if tuple(t.shape) != (T, cache.n_kv, cache.D) or not t.is_contiguous():
+            raise Error(1, f"{what}: outputs {tuple(k_out.shape)} and {tuple(v_out.shape)}, expected contiguous {(T, cache.n_kv, cache.D)}")
+    _check(_lib.load().sxb_kv_read(cache._by_ref, _ptr(seq), _ptr(pos), _ptr(pages), pages.stride(0) if pages.shape[0] > 1 else pages.shape[1], pages.shape[1], pages.shape[0], T, _ptr(k_out),
+                                   _ptr(v_out), 0 if k_out.dtype == torch.float32 else 1, _ptr(err), _stream(stream)))
+
+
+def attn_decode_workspace_bytes(cache: KvCache, n_q: int, max_q: int) -> int:
+    """Bytes of workspace that attn_decode needs on the current device; zeroed once before its first use."""
+    n = _lib.load().sxb_attn_decode_workspace_bytes(n_q, cache.n_kv, cache.D, cache.bits, max_q)
+    if n == 0:
+        _check(1)
+    return n
+
+
+def attn_decode(q, cache: KvCache, pages, q_start, kv_len, max_q, out, ws, err, scale=None, softcap=0.0, window=0, lse=None, stream=None):
+    """sxb_attn_decode: q [T, n_q D] BF16, rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]) the new tokens of sequence b, kv_len [B] int32 its
+    keys, their own included -> out [T, n_q D] BF16, lse [T, n_q] FP32.  scale: None = D ** -0.5; softcap, window: 0 = none.  max_q: a
+    sequence's largest count of new tokens."""
+    what = "attn_decode"
+    T, B, D = q.shape[0], kv_len.shape[0], cache.D
+    _here(cache, what)
+    _on(cache.device, what, q=(q, _BF16), out=(out, _BF16), pages=(pages, _I32), q_start=(q_start, _I32), kv_len=(kv_len, _I32), lse=(lse, _F32),
+        err=(err, (torch.int32, torch.uint32)), ws=(ws, (ws.dtype,)))
+    n_q, rest = divmod(q.shape[1], D)
+    if rest or out.shape != q.shape or pages.dim() != 2 or pages.shape[0] < B or q_start.shape != (B + 1,) or \
+            (lse is not None and (tuple(lse.shape) != (T, n_q) or not lse.is_contiguous())):
+        raise Error(1, f"{what}: q {tuple(q.shape)}, out {tuple(out.shape)}, pages {tuple(pages.shape)}, q_start {tuple(q_start.shape)}, kv_len "
+                       f"{tuple(kv_len.shape)} or lse do not fit heads of {D}")
+    _check(_lib.load().sxb_attn_decode(_ptr(q), q.stride(0) if T > 1 else q.shape[1], T, n_q, cache._by_ref, _ptr(pages), pages.stride(0) if pages.shape[0] > 1 else pages.shape[1], pages.shape[1], _ptr(q_start), _ptr(kv_len), B,
+                                       max_q, D ** -0.5 if scale is None else scale, softcap, window, _ptr(out), out.stride(0) if T > 1 else out.shape[1], _ptr(lse), _ptr(ws),
+                                       ws.numel() * ws.element_size(), _ptr(err), _stream(stream)))
+
+
+def check_attn_error(err, what: str):
+    _check(_lib.load().sxb_check_attn_error(_ptr(err), what.encode()))
+
+
+def report_attn_error(e, what: str):
+    _check(_lib.load().sxb_report_attn_error((C.c_uint32 * 3)(*[int(v) for v in e]), what.encode()))
+
+
 # ---- the whole block as one call ------------------------------------------------------------------------------
 
 def _layer_args(x, logits, y, gate_up, down, E, A, ids, coef, ws, ws_bytes, h, partial, router_err, expert_err, xs, math, E_total,

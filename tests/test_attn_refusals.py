@@ -1,0 +1,128 @@
+"""CPU tests of what the attention entry points refuse before any launch."""
+import ctypes as C
+
+import pytest
+
+
+def cache(**kw):
+    from strixite_b200 import _lib
+    c = dict(k=1 << 20, v=2 << 20, k_sm=3 << 20, v_sm=4 << 20, n_pages=10, n_kv=2, page=16, D=128, G=64, page_stride=32, head_stride=16, row_stride=1, bits=8)
+    c.update(kw)
+    return _lib.SxbKvCache(*[c[f[0]] for f in _lib.SxbKvCache._fields_])
+
+
+BAD_CACHES = [
+    (dict(bits=5), "5 bits unsupported"), (dict(D=96), "heads of 96"), (dict(k=0), "null pointer"), (dict(v=(2 << 20) + 8), "16-byte aligned"),
+    (dict(G=48), "group size 48"), (dict(D=64, G=128), "group size 128"), (dict(k_sm=0), "null pointer"), (dict(v_sm=(4 << 20) + 4), "16-byte aligned"),
+    (dict(n_pages=0), "n_pages = 0"), (dict(n_kv=0), "n_kv = 0"), (dict(page=24), "pages of 24"), (dict(page=4), "pages of 4"), (dict(page=8192), "pages of 8192"),
+    (dict(page_stride=0), "strides of 0"), (dict(row_stride=-1), "strides of"), (dict(head_stride=1 << 40), "strides of"),
+]
+
+
+def write(lib, c=None, **kw):
+    a = dict(qkv=5 << 20, ld=8 * 128, act=1, T=4, n_q=4, q_norm=6 << 20, k_norm=6 << 20, eps=1e-6, inv=7 << 20, rot=128, inter=0, seq=8 << 20, pos=8 << 20,
+             pages=9 << 20, pages_ld=5, n_cols=5, n_seq=2, cache=C.byref(c or cache()), q_out=10 << 20, q_ld=512, err=11 << 20, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.sxb_attn_qkv_write(*a.values()), lib.sxb_last_error().decode()
+
+
+def attend(lib, c=None, **kw):
+    a = dict(q=5 << 20, q_ld=512, T=4, n_q=4, cache=C.byref(c or cache()), pages=9 << 20, pages_ld=5, n_cols=5, q_start=8 << 20, kv_len=8 << 20, B=2, max_q=2,
+             scale=0.1, cap=0.0, window=0, out=10 << 20, out_ld=512, lse=None, ws=12 << 20, ws_bytes=1 << 30, err=11 << 20, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.sxb_attn_decode(*a.values()), lib.sxb_last_error().decode()
+
+
+def read(lib, c=None, **kw):
+    a = dict(cache=C.byref(c or cache()), seq=8 << 20, pos=8 << 20, pages=9 << 20, pages_ld=5, n_cols=5, n_seq=2, T=4, k=5 << 20, v=10 << 20, act=1, err=11 << 20, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.sxb_kv_read(*a.values()), lib.sxb_last_error().decode()
+
+
+@pytest.mark.parametrize("entry", [write, attend, read])
+@pytest.mark.parametrize("kw,message", BAD_CACHES)
+def test_bad_caches(lib, entry, kw, message):
+    rc, said = entry(lib, cache(**kw))
+    assert rc == 1 and message in said, said
+
+
+@pytest.mark.parametrize("entry", [write, attend, read])
+def test_null_cache_and_tables(lib, entry):
+    for kw, message in ((dict(cache=None), "null cache"), (dict(pages=0), "null pointer"), (dict(err=0), "null pointer"), (dict(T=0), "T = 0"), (dict(n_cols=0), "0 columns"),
+                        (dict(pages_ld=4), "stride of 4"), (dict(n_cols=1 << 27, pages_ld=1 << 27), "positions end below")):
+        rc, said = entry(lib, **kw)
+        assert rc == 1 and message in said, (kw, said)
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(qkv=0), "null pointer"), (dict(q_out=0), "null pointer"), (dict(seq=0), "null pointer"), (dict(act=2), "activation dtype 2"), (dict(n_q=0), "n_q = 0"),
+    (dict(ld=1023), "row strides"), (dict(ld=1028), "16-byte aligned"), (dict(q_ld=516), "16-byte aligned"), (dict(q_out=(10 << 20) + 8), "16-byte aligned"),
+    (dict(q_out=(5 << 20) + 512), "overlaps"), (dict(inv=None), "without inv_freq"), (dict(rot=24), "rot = 24"), (dict(rot=144), "rot = 144"), (dict(rot=-16), "rot = -16"),
+    (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(n_seq=0), "n_seq = 0"), (dict(T=(1 << 24) + 1), "T = "),
+])
+def test_write_refusals(lib, kw, message):
+    rc, said = write(lib, **kw)
+    assert rc == 1 and message in said, said
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(q=0), "null pointer"), (dict(ws=0), "null pointer"), (dict(q_start=0), "null pointer"), (dict(n_q=3), "n_q = 3"), (dict(n_q=1), "n_q = 1"), (dict(B=0), "B = 0"),
+    (dict(max_q=0), "max_q = 0"), (dict(q_ld=511), "row strides"), (dict(out_ld=516), "row strides"), (dict(q=(5 << 20) + 2), "16-byte aligned"),
+    (dict(ws=(12 << 20) + 4), "16-byte aligned"), (dict(out=(5 << 20) + 64), "overlaps"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(cap=-1.0), "softcap"), (dict(window=-1), "window = -1"), (dict(window=1 << 31), "window"), (dict(ws_bytes=16), "workspace of 16 bytes, needs"),
+])
+def test_attend_refusals(lib, kw, message):
+    if "ws_bytes" in kw:
+        pytest.importorskip("torch")
+    rc, said = attend(lib, **kw)
+    assert rc == 1 and message in said, said
+
+
+@pytest.mark.parametrize("kw,message", [(dict(k=0), "null pointer"), (dict(act=3), "output dtype 3"), (dict(v=(10 << 20) + 2), "16-byte aligned"), (dict(v=5 << 20), "overlaps")])
+def test_read_refusals(lib, kw, message):
+    rc, said = read(lib, **kw)
+    assert rc == 1 and message in said, said
+
+
+def test_workspace_refusals(lib):
+    for bad in ((0, 1, 128, 16, 1), (3, 2, 128, 16, 1), (4, 2, 96, 16, 1), (4, 2, 128, 6, 1), (4, 2, 128, 8, 0), (2048, 2, 128, 8, 1)):
+        assert lib.sxb_attn_decode_workspace_bytes(*bad) == 0
+        assert "attn_decode_workspace_bytes" in lib.sxb_last_error().decode()
+
+
+def test_cache_struct_matches_the_header(tmp_path):
+    import pathlib
+    import subprocess
+    from strixite_b200 import _lib
+    root = pathlib.Path(__file__).resolve().parent.parent
+    names = [f[0] for f in _lib.SxbKvCache._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "strix_b200.h"\nint main(void) {\n    printf("sizeof %zu\\n", sizeof(SxbKvCache));\n'
+                   + "".join(f'    printf("{n} %zu\\n", offsetof(SxbKvCache, {n}));\n' for n in names) + "    return 0;\n}\n")
+    subprocess.run(["gcc", "-std=c99", f"-I{root / 'include'}", str(src), "-o", str(tmp_path / "layout")], check=True)
+    out = dict(line.split() for line in subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.splitlines())
+    assert int(out["sizeof"]) == C.sizeof(_lib.SxbKvCache)
+    for n in names:
+        assert int(out[n]) == getattr(_lib.SxbKvCache, n).offset, n
+
+
+def test_python_refuses_what_lives_nowhere_or_fits_nothing(lib):
+    import torch
+    from strixite_b200 import kernels as K
+    z = torch.zeros
+    with pytest.raises(K.Error, match="must live on a CUDA device"):
+        K.KvCache(z(2, 1, 16, 64, dtype=torch.bfloat16), z(2, 1, 16, 64, dtype=torch.bfloat16), 16)
+    with pytest.raises(K.Error, match="7 bits"):
+        K.KvCache(z(2, 1, 16, 64), z(2, 1, 16, 64), 7)
+    with pytest.raises(K.Error, match="expected the same"):
+        K.KvCache(z(2, 1, 16, 64), z(2, 1, 16, 32), 16)
+
+
+def test_report_attn_error(lib):
+    from strixite_b200 import kernels as K
+    K.report_attn_error([0, 0, 0], "step")
+    with pytest.raises(K.Error, match=r"step: page, position, length or row range out of range at token or sequence 7 \(-1\)"):
+        K.report_attn_error([1, 7, 0xFFFFFFFF], "step")

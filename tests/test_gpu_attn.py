@@ -1,0 +1,510 @@
+"""GPU tests of the attention operators over a paged key-value cache against their definition in 64 bits (attn_plain.py)."""
+import numpy as np
+import pytest
+import torch
+
+import attn_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+
+def K():
+    from strixite_b200 import kernels
+    return kernels
+
+
+def filled(cache, seed):
+    """N(0, 1) with a mean a channel in every row of the cache, quantized by the library's own quantizer where it is."""
+    g = torch.Generator(device=cache.device)
+    g.manual_seed(seed)
+    for name in ("k", "v"):
+        shape = (cache.n_pages, cache.n_kv, cache.page, cache.D)
+        x = torch.randn(shape, generator=g, device=cache.device) + 0.5 * torch.randn(cache.D, generator=g, device=cache.device)
+        if cache.bits == 16:
+            getattr(cache, name).copy_(x)
+        else:
+            w = K().quantize(x.reshape(-1, cache.D).contiguous(), cache.G, cache.bits)
+            getattr(cache, name).copy_(w.q.view(getattr(cache, name).shape))
+            sm = torch.stack((w.scale, w.minv), -1).view(torch.bfloat16)
+            getattr(cache, name + "_sm").copy_(sm.view(getattr(cache, name + "_sm").shape))
+    return cache
+
+
+def tables(lens, page, n_pages, seed, device):
+    """Pages scattered over the pool; entries behind a sequence's end name no page."""
+    rng = np.random.default_rng(seed)
+    wide = max(1, max(-(-max(n, 0) // page) for n in lens)) + 1
+    t = np.full((len(lens), wide), 0x7ffffff, dtype=np.int32)
+    ids = rng.permutation(n_pages)
+    at = 0
+    for b, n in enumerate(lens):
+        need = -(-max(n, 0) // page)
+        t[b, :need] = ids[at:at + need]
+        at += need
+    assert at <= n_pages
+    return torch.from_numpy(t).to(device)
+
+
+class Batch:
+    """A batch of sequences over a filled cache: new[b] new tokens of lens[b] keys."""
+
+    def __init__(self, device, D, bits, G, n_kv, group, lens, new, page=16, seed=0, max_q=None, spare=3):
+        self.lens, self.new = lens, new
+        n_pages = sum(-(-max(n, 0) // page) for n in lens) + spare
+        self.cache = filled(K().KvCache.empty(n_pages, n_kv, page, D, bits, G, device), seed)
+        self.pages = tables(lens, page, n_pages, seed, device)
+        self.T, self.n_q = sum(new), n_kv * group
+        g = torch.Generator(device=device)
+        g.manual_seed(seed + 1)
+        self.q = (1.5 * torch.randn((self.T, self.n_q * D), generator=g, device=device)).to(torch.bfloat16)
+        self.q_start = torch.tensor(np.concatenate(([0], np.cumsum(new))), dtype=torch.int32, device=device)
+        self.kv_len = torch.tensor(lens, dtype=torch.int32, device=device)
+        self.max_q = max(new) if max_q is None else max_q
+        self.out = torch.full_like(self.q, float("nan"))
+        self.lse = torch.full((self.T, self.n_q), float("nan"), device=device)
+        self.err = torch.zeros(4, dtype=torch.int32, device=device)
+        self.ws = torch.zeros(K().attn_decode_workspace_bytes(self.cache, self.n_q, self.max_q), dtype=torch.uint8, device=device)
+
+    def run(self, **kw):
+        kw.setdefault("lse", self.lse)
+        K().attn_decode(self.q, self.cache, self.pages, self.q_start, self.kv_len, self.max_q, self.out, self.ws, self.err, **kw)
+
+    def check(self, scale=None, softcap=0.0, window=0):
+        torch.cuda.synchronize()
+        assert int(self.err[0]) == 0
+        D = self.cache.D
+        want, lse, tol, lse_tol = plain.attend(self.q, self.cache, self.pages, self.q_start, self.kv_len, D ** -0.5 if scale is None else scale, softcap, window)
+        got = plain.f64(self.out).reshape(want.shape)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        far = np.nan_to_num(np.abs(got - want) - tol, nan=0.0)
+        assert far.max() <= 0, (far.max(), np.unravel_index(far.argmax(), far.shape))
+        got = plain.f64(self.lse)
+        assert np.array_equal(np.isneginf(got), np.isneginf(lse))
+        with np.errstate(invalid="ignore"):
+            far = np.nan_to_num(np.abs(got - lse) - lse_tol, nan=0.0)
+        assert far.max() <= 0, (far.max(), np.unravel_index(far.argmax(), far.shape))
+
+
+# Every form of the kernel: sizes, codes, groups, and the rows of a tile by the query heads a key head.
+FORMS = [(D, bits, G) for D in (64, 128, 256) for bits, groups in ((16, (0,)), (8, (32, 64, 128)), (4, (32, 64, 128))) for G in groups if G <= D]
+
+
+@pytest.mark.parametrize("group,new", [(4, 1), (1, 1), (3, 7), (8, 8), (5, 13)], ids=["rows4", "rows1", "rows21", "rows64", "rows65"])
+@pytest.mark.parametrize("D,bits,G", FORMS)
+def test_attend_against_the_definition(cuda, D, bits, G, group, new):
+    """Lengths around the tiles' ends, a row that sees one key, rows that see none, sequences of uneven counts of new tokens."""
+    lens = [1, new, 63, 64, 65, 128, 129, 0, 700, max(1, new - 2)]
+    news = [1, new, new, 1, max(1, new - 1), new, 1, 1, new, new]
+    b = Batch(cuda, D, bits, G, 2, group, lens, news, page=16, seed=D + bits + G + group)
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("page", [8, 32, 128, 1024])
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_attend_pages(cuda, bits, G, page):
+    b = Batch(cuda, 128, bits, G, 2, 4, [1300, 5, 257], [1, 2, 1], page=page, seed=page)
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("window", [1, 5, 64, 100, 5000])
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_attend_window_and_cap(cuda, bits, G, window):
+    b = Batch(cuda, 128, bits, G, 2, 4, [1000, 64, 3, 130, 2], [3, 2, 3, 1, 4], seed=window)
+    b.run(window=window, softcap=20.0, scale=0.3)
+    b.check(window=window, softcap=20.0, scale=0.3)
+
+
+@pytest.mark.parametrize("B", [1, 127, 128, 129, 300])
+def test_attend_many_sequences(cuda, B):
+    """More sequences than a CTA has threads: the list's place is found by several rounds."""
+    rng = np.random.default_rng(B)
+    lens = [int(n) for n in rng.integers(0, 90, B)]
+    b = Batch(cuda, 64, 16, 0, 1, 4, lens, [int(n) for n in rng.integers(0, 3, B - 1)] + [1], seed=B)
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_attend_long_cache_is_split_and_joined(cuda, bits, G):
+    b = Batch(cuda, 128, bits, G, 1, 8, [30011, 17], [1, 1], page=64, seed=5)
+    b.run()
+    b.check()
+    first = b.out.clone(), b.lse.clone()
+    for _ in range(3):  # the join adds in the list's order, whoever comes last
+        b.out.fill_(7.0), b.lse.fill_(7.0)
+        b.run()
+        assert torch.equal(b.out, first[0]) and torch.equal(b.lse, first[1])
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 32)])
+def test_attend_more_new_tokens_than_told(cuda, bits, G):
+    """max_q picks the kernel; a sequence with more rows takes several passes."""
+    b = Batch(cuda, 64, bits, G, 2, 2, [90, 200, 300], [33, 1, 150], max_q=1, seed=3)
+    b.run()
+    b.check()
+
+
+def test_attend_leaves_other_rows_and_columns(cuda):
+    """Rows before, between and behind the sequences and what lies beside a strided output stay as they were."""
+    b = Batch(cuda, 64, 16, 0, 2, 2, [40, 20, 33], [2, 1, 1], seed=8)
+    T, wide = 9, b.n_q * 64
+    q = torch.randn((T, wide + 64), device=cuda).to(torch.bfloat16)[:, :wide]
+    out = torch.full((T, wide + 8), 3.0, device=cuda, dtype=torch.bfloat16)
+    lse = torch.full((T, b.n_q), 3.0, device=cuda)
+    starts = torch.tensor([1, 3, 3, 4], dtype=torch.int32, device=cuda)  # rows 1-2, none, row 3
+    K().attn_decode(q, b.cache, b.pages, starts, b.kv_len, 2, out[:, :wide], b.ws, b.err, lse=lse)
+    torch.cuda.synchronize()
+    want, want_lse, tol, _ = plain.attend(q, b.cache, b.pages, starts, b.kv_len, 64 ** -0.5)
+    got = plain.f64(out[:, :wide]).reshape(want.shape)
+    assert (np.abs(got[1:4] - want[1:4]) <= tol[1:4]).all()
+    for t in (0, 4, 5, 6, 7, 8):
+        assert (out[t] == 3.0).all() and (lse[t] == 3.0).all()
+    assert (out[:, wide:] == 3.0).all()
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_attend_other_strides(cuda, bits, G):
+    """A pool kept token by token ([n_pages, page, n_kv, D]), keys and values in one tensor, gives the same bits as the plain one."""
+    b = Batch(cuda, 128, bits, G, 2, 4, [500, 77], [2, 1], seed=9)
+    b.run()
+    c = b.cache
+    def moved(k, v):
+        both = torch.empty((c.n_pages, 2, c.page, c.n_kv, *k.shape[3:]), dtype=k.dtype, device=cuda)
+        both[:, 0].copy_(k.transpose(1, 2))
+        both[:, 1].copy_(v.transpose(1, 2))
+        return both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    k, v = moved(c.k, c.v)
+    sm = moved(c.k_sm, c.v_sm) if bits != 16 else (None, None)
+    other = K().KvCache(k, v, bits, G, *sm)
+    out = torch.empty_like(b.out)
+    K().attn_decode(b.q, other, b.pages, b.q_start, b.kv_len, b.max_q, out, b.ws, b.err)
+    assert torch.equal(out, b.out)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_attend_what_is_not_finite_reaches_only_rows_that_see_it(cuda, bad):
+    """A NaN or an infinity in the newest key and value (BF16), rows of three drafts: only the last row sees it; junk behind the sequences' ends."""
+    for where in ("k", "v"):
+        b = Batch(cuda, 128, 16, 0, 2, 4, [70, 300], [3, 3], seed=11)
+        for s, n in enumerate(b.lens):
+            getattr(b.cache, where)[int(b.pages[s, (n - 1) // 16]), :, (n - 1) % 16, 5] = bad
+            for at in range(n % 16, 16):  # the last page's rest
+                getattr(b.cache, where)[int(b.pages[s, (n - 1) // 16]), :, at] = float("nan")
+        b.run()
+        torch.cuda.synchronize()
+        want, lse, tol, _ = plain.attend(b.q, b.cache, b.pages, b.q_start, b.kv_len, 128 ** -0.5)
+        got = plain.f64(b.out).reshape(want.shape)
+        rows = [0, 1, 3, 4]
+        assert np.isfinite(got[rows]).all() and (np.abs(got[rows] - want[rows]) <= tol[rows]).all()
+        if where == "v":  # the channel alone
+            assert np.array_equal(np.isfinite(got[[2, 5]]), np.isfinite(want[[2, 5]])) and not np.isfinite(got[[2, 5], :, 5]).any()
+        elif bad != bad:
+            assert np.isnan(got[[2, 5]]).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attend_scales_that_are_none_reach_only_rows_that_see_them(cuda, bits):
+    for where in ("k_sm", "v_sm"):
+        b = Batch(cuda, 128, bits, 32, 2, 4, [70, 300], [3, 3], seed=12)
+        for s, n in enumerate(b.lens):
+            getattr(b.cache, where)[int(b.pages[s, (n - 1) // 16]), :, (n - 1) % 16, 1] = float("nan")
+            getattr(b.cache, where)[int(b.pages[s, (n - 1) // 16]), :, n % 16:] = float("nan")
+        b.run()
+        torch.cuda.synchronize()
+        want, lse, tol, _ = plain.attend(b.q, b.cache, b.pages, b.q_start, b.kv_len, 128 ** -0.5)
+        got = plain.f64(b.out).reshape(want.shape)
+        rows = [0, 1, 3, 4]
+        assert np.isfinite(got[rows]).all() and (np.abs(got[rows] - want[rows]) <= tol[rows]).all()
+        assert np.array_equal(np.isnan(got[[2, 5]]), np.isnan(want[[2, 5]]))
+
+
+@pytest.mark.parametrize("size", [2.0 ** -60, 2.0 ** -20, 1.0, 2.0 ** 20, 2.0 ** 60])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attend_values_and_queries_of_any_size(cuda, bits, size):
+    """F16 operands' range is no limit: values (hence scales) and queries far outside of it, later values larger than earlier ones and smaller."""
+    for grows in (1.0, 2.0 ** 20, 2.0 ** -20):
+        b = Batch(cuda, 128, bits, 64, 1, 4, [400], [1], seed=13)
+        b.cache.v_sm.mul_(size)
+        b.cache.v_sm[b.pages[0, 10:20].long()] *= grows
+        b.q.mul_(1.0 / size)
+        b.cache.k_sm.mul_(size)
+        b.run()
+        b.check()
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64)])
+def test_attend_bad_pages_lengths_and_rows(cuda, bits, G):
+    """What the host cannot see is refused by the kernel: NaN for the rows that it concerns, the rest right, the error words set."""
+    b = Batch(cuda, 64, bits, G, 2, 2, [100, 90, 80, 60, 50], [1, 2, 1, 1, 1], seed=14)
+    clean = b.pages.clone(), b.kv_len.clone(), b.q_start.clone()
+    want, lse, tol, _ = plain.attend(b.q, b.cache, b.pages, b.q_start, b.kv_len, 64 ** -0.5)
+    b.pages[0, 2] = b.cache.n_pages
+    b.pages[1, 5] = -3                    # keys 80..89: both rows see them
+    b.kv_len[2] = b.pages.shape[1] * 16 + 1
+    b.kv_len[3] = -1
+    b.run()
+    torch.cuda.synchronize()
+    got = plain.f64(b.out).reshape(want.shape)
+    assert np.isnan(got[:5]).all() and torch.isnan(b.lse[:5]).all()
+    assert (np.abs(got[5] - want[5]) <= tol[5]).all()
+    assert int(b.err[0]) == 1
+    with pytest.raises(K().Error, match="batch: page, position, length"):
+        K().check_attn_error(b.err, "batch")
+    b.err.zero_()
+    b.pages, b.kv_len, b.q_start = clean[0], clean[1], clean[2].clone()
+    b.q_start[2] = b.T + 5  # sequences 1 and 2 have no rows to speak of
+    b.out.fill_(3.0)
+    b.run()
+    torch.cuda.synchronize()
+    got = plain.f64(b.out).reshape(want.shape)
+    assert (got[1:4] == 3.0).all() and int(b.err[0]) == 1
+    for t in (0, 4, 5):
+        assert (np.abs(got[t] - want[t]) <= tol[t]).all()
+
+
+def test_attend_captured_and_replayed_with_other_lengths(cuda):
+    """A graph follows the lengths, tables and rows that it finds; two graphs that share a workspace run one behind the other."""
+    b = Batch(cuda, 128, 8, 64, 2, 4, [1000, 300], [1, 2], seed=15)
+    b.run()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            b.run()
+    for lens in ([1000, 300], [17, 2], [640, 0], [1, 299]):
+        b.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        for graph in graphs:
+            b.out.fill_(float("nan"))
+            graph.replay()
+            b.check()
+
+
+def test_attend_on_another_stream(cuda):
+    b = Batch(cuda, 128, 16, 0, 2, 4, [3000], [1], seed=16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    b.run(stream=side)
+    side.synchronize()
+    b.check()
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_offsets_beyond_32_bits(cuda, bits, G):
+    """Pages at the end of a pool whose codes, and whose rows' words, lie more than 2^32 bytes behind its start."""
+    D, n_kv, page = 128, 8, 64
+    n_pages = (9 << 30) // (n_kv * page * D * bits // 8)
+    k = torch.empty((n_pages, n_kv, page, D // 2 if bits == 4 else D), dtype=torch.bfloat16 if bits == 16 else torch.uint8, device=cuda)
+    v = torch.empty_like(k)
+    sm = [torch.empty((n_pages, n_kv, page, D // G, 2), dtype=torch.bfloat16, device=cuda) for _ in range(2)] if bits != 16 else [None, None]
+    cache = K().KvCache(k, v, bits, G, *sm)
+    T = 150
+    pages = torch.arange(n_pages - 3, n_pages, dtype=torch.int32, device=cuda).view(1, 3)
+    seq, pos = torch.zeros(T, dtype=torch.int32, device=cuda), torch.arange(T, dtype=torch.int32, device=cuda)
+    qkv = torch.randn((T, (8 + 2 * n_kv) * D), device=cuda).to(torch.bfloat16)
+    q = torch.empty((T, 8 * D), dtype=torch.bfloat16, device=cuda)
+    err = torch.zeros(4, dtype=torch.int32, device=cuda)
+    K().attn_qkv_write(qkv, cache, seq, pos, pages, q, err)
+    ko, vo = (torch.empty((T, n_kv, D), dtype=torch.float32, device=cuda) for _ in range(2))
+    K().kv_read(cache, seq, pos, pages, ko, vo, err)
+    x = qkv.float().view(T, 8 + 2 * n_kv, D)
+    step = 0.0 if bits == 16 else 8.0 / (2 ** bits - 1)
+    assert (ko - x[:, 8:16]).abs().max() <= step and (vo - x[:, 16:]).abs().max() <= step
+    out, ws = torch.empty_like(q[:1]), torch.zeros(K().attn_decode_workspace_bytes(cache, 8, 1), dtype=torch.uint8, device=cuda)
+    starts, lens = torch.tensor([0, 1], dtype=torch.int32, device=cuda), torch.tensor([T], dtype=torch.int32, device=cuda)
+    K().attn_decode(q[:1], cache, pages, starts, lens, 1, out, ws, err)
+    want, _, tol, _ = plain.attend(q[:1], cache, pages, starts, lens, D ** -0.5)
+    assert (np.abs(plain.f64(out).reshape(want.shape) - want) <= tol).all() and int(err[0]) == 0
+
+
+# ---- writing and reading -----------------------------------------------------------------------------------------------------------
+
+class Rows:
+    """T tokens of B sequences, their places scattered, and what is to be written there."""
+
+    def __init__(self, device, T, B, n_q, n_kv, D, bits, G, page=16, f32=False, far=0, seed=0, norm=True):
+        g = torch.Generator(device=device)
+        g.manual_seed(seed)
+        self.T, self.n_q, self.D = T, n_q, D
+        counts = [T // B + (b < T % B) for b in range(B)]
+        self.lens = [far + 3 * b + n for b, n in enumerate(counts)]
+        n_pages = sum(-(-n // page) for n in self.lens) + 2
+        self.cache = filled(K().KvCache.empty(n_pages, n_kv, page, D, bits, G, device), seed + 7)
+        self.pages = tables(self.lens, page, n_pages, seed, device)
+        order = np.random.default_rng(seed).permutation(T)
+        seq = np.concatenate([np.full(n, b) for b, n in enumerate(counts)])[order]
+        pos = np.concatenate([np.arange(n) + self.lens[b] - n for b, n in enumerate(counts)])[order]
+        self.seq, self.pos = (torch.from_numpy(v.astype(np.int32)).to(device) for v in (seq, pos))
+        x = torch.randn((T, (n_q + 2 * n_kv) * D), generator=g, device=device) * 1.7
+        self.qkv = x if f32 else x.to(torch.bfloat16)
+        self.q_norm, self.k_norm = ((1 + 0.2 * torch.randn(D, generator=g, device=device)) if norm else None for _ in range(2))
+        self.q_out = torch.full((T, n_q * D), float("nan"), dtype=torch.bfloat16, device=device)
+        self.err = torch.zeros(4, dtype=torch.int32, device=device)
+
+    def inv_freq(self, rot):
+        return (1e6 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)).float().to(self.qkv.device) if rot else None
+
+    def read(self, dtype=torch.float32):
+        k, v = (torch.full((self.T, self.cache.n_kv, self.D), float("nan"), dtype=dtype, device=self.qkv.device) for _ in range(2))
+        K().kv_read(self.cache, self.seq, self.pos, self.pages, k, v, self.err)
+        return k, v
+
+
+@pytest.mark.parametrize("T,B,n_q,n_kv,f32", [(1, 1, 8, 2, False), (37, 5, 3, 1, True), (300, 2, 4, 4, False), (1500, 3, 2, 1, True)])
+@pytest.mark.parametrize("rot,interleaved", [("D", False), (32, True), (16, False), (0, False)])
+@pytest.mark.parametrize("D,bits,G", [f for f in FORMS if f[2] in (0, 32, f[0])])
+def test_write_and_read_against_the_definition(cuda, D, bits, G, rot, interleaved, T, B, n_q, n_kv, f32):
+    r = Rows(cuda, T, B, n_q, n_kv, D, bits, G, f32=f32, seed=T + D + bits)
+    rot = D if rot == "D" else rot
+    before = [t.clone() for t in (r.cache.k, r.cache.v)]
+    inv = r.inv_freq(rot)
+    K().attn_qkv_write(r.qkv, r.cache, r.seq, r.pos, r.pages, r.q_out, r.err, q_norm=r.q_norm, k_norm=r.k_norm, eps=1e-5, inv_freq=inv, interleaved=interleaved)
+    k, v = r.read()
+    torch.cuda.synchronize()
+    assert int(r.err[0]) == 0
+    x = plain.f64(r.qkv).reshape(T, n_q + 2 * n_kv, D)
+    pos = r.pos.cpu().numpy()
+    q, q_size = plain.norm_rotate(x[:, :n_q], r.q_norm, 1e-5, pos, inv, interleaved)
+    kk, k_size = plain.norm_rotate(x[:, n_q:n_q + n_kv], r.k_norm, 1e-5, pos, inv, interleaved)
+    vv = x[:, n_q + n_kv:]
+    # FP32: the norm's sum (D / 32 + 5 roundings, halved by the root), root, division, two products, the turn's two products and sum: under 2^-20
+    assert (np.abs(plain.f64(r.q_out).reshape(q.shape) - q) <= plain.BF16 * np.abs(q) + 2.0 ** -20 * q_size).all()
+    page, at = r.pages.cpu().numpy()[r.seq.cpu().numpy(), pos // 16], pos % 16
+    if bits == 16:
+        assert (np.abs(plain.f64(k) - kk) <= plain.BF16 * np.abs(kk) + 2.0 ** -20 * k_size).all()
+        assert np.array_equal(plain.f64(v), plain.f64(r.qkv.view(T, -1, D)[:, n_q + n_kv:].to(torch.bfloat16)))
+    else:
+        # V is not touched before it is quantized: the library's quantizer gives the same codes, bit for bit
+        w = K().quantize(r.qkv.float().view(T, -1, D)[:, n_q + n_kv:].reshape(-1, D).contiguous(), G, bits)
+        codes = torch.stack([r.cache.v[int(p), :, int(a)] for p, a in zip(page, at)])
+        assert torch.equal(codes.reshape(w.q.shape), w.q)
+        sm = torch.stack([r.cache.v_sm[int(p), :, int(a)] for p, a in zip(page, at)]).view(torch.int16)
+        assert torch.equal(sm[..., 0].reshape(w.scale.shape), w.scale) and torch.equal(sm[..., 1].reshape(w.minv.shape), w.minv)
+        # what is read is code * scale + min, one rounding
+        for which, got in (("k", k), ("v", v)):
+            for h in range(n_kv):
+                y, _, _ = plain.values(r.cache, which, page.astype(np.int64), h, at)
+                assert (np.abs(plain.f64(got)[:, h] - y) <= 2.0 ** -23 * np.abs(y)).all()
+        # K: half a step of the group's range, the scale's and the min's rounding to BF16 (at the far end the scale's counts `levels` times, and codes
+        # beyond the last are cut off), and FP32 on the way
+        groups = kk.reshape(T, n_kv, -1, G)
+        lo, hi = groups.min(-1, keepdims=True), groups.max(-1, keepdims=True)
+        tol = 0.51 * (hi - lo) / (2 ** bits - 1) + 2 * plain.BF16 * (np.abs(lo) + np.abs(hi - lo)) + 2.0 ** -19 * k_size.reshape(groups.shape)
+        assert (np.abs(plain.f64(k).reshape(groups.shape) - groups) <= tol).all()
+    # nothing but the tokens' rows
+    for name, old in zip(("k", "v"), before):
+        new = getattr(r.cache, name).clone()
+        p, a = torch.from_numpy(page.astype(np.int64)).to(cuda), torch.from_numpy(at.astype(np.int64)).to(cuda)
+        new[p, :, a] = old[p, :, a]
+        assert torch.equal(new.view(torch.uint8), old.view(torch.uint8))
+
+
+def test_write_far_positions(cuda):
+    """The angle of a position near 2^31: FP32 would lose whole turns."""
+    r = Rows(cuda, 1, 1, 4, 1, 128, 16, 0, page=4096, norm=False)
+    r.pages = torch.zeros((1, (1 << 19) - 1), dtype=torch.int32, device=cuda)
+    inv = r.inv_freq(128)
+    for pos in (0, 1, 123457, 1 << 24, (1 << 31) - 4097):
+        r.pos.fill_(pos)
+        K().attn_qkv_write(r.qkv, r.cache, r.seq, r.pos, r.pages, r.q_out, r.err, inv_freq=inv)
+        q, size = plain.norm_rotate(plain.f64(r.qkv).reshape(1, 6, 128)[:, :4], None, 0, np.array([pos]), inv, False)
+        assert (np.abs(plain.f64(r.q_out).reshape(q.shape) - q) <= plain.BF16 * np.abs(q) + 2.0 ** -20 * size).all(), pos
+    assert int(r.err[0]) == 0
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_write_and_read_padding_and_bad_places(cuda, bits, G):
+    """Padding rows stay as they are everywhere; a bad place gives NaN, writes nothing to the cache and sets the error words."""
+    r = Rows(cuda, 6, 2, 2, 1, 128, bits, G, seed=4)
+    r.q_out.fill_(3.0)
+    seq, pos = r.seq.clone(), r.pos.clone()
+    r.seq[1] = -1
+    K().attn_qkv_write(r.qkv, r.cache, r.seq, r.pos, r.pages, r.q_out, r.err)
+    k, v = r.read()
+    torch.cuda.synchronize()
+    assert int(r.err[0]) == 0 and (r.q_out[1] == 3.0).all() and torch.isfinite(r.q_out[[0, 2, 3, 4, 5]]).all()
+    assert torch.isnan(k[1]).all() and torch.isnan(v[1]).all() and torch.isfinite(k[[0, 2, 3, 4, 5]]).all()
+    old = r.cache.k.clone(), r.cache.v.clone()
+    for bad in ("seq", "pos", "negative", "page"):
+        r.err.zero_()
+        r.seq.fill_(-1), r.pos.copy_(pos)
+        r.seq[2] = seq[2]
+        pages = r.pages.clone()
+        if bad == "seq":
+            r.seq[2] = 2
+        elif bad == "pos":
+            r.pos[2] = r.pages.shape[1] * 16
+        elif bad == "negative":
+            r.pos[2] = -5
+        else:
+            pages[int(seq[2]), int(pos[2]) // 16] = r.cache.n_pages
+        K().attn_qkv_write(r.qkv, r.cache, r.seq, r.pos, pages, r.q_out, r.err)
+        ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+        assert int(r.err[0]) == 1 and int(r.err[1]) == 2
+        with pytest.raises(K().Error, match="token or sequence 2"):
+            K().check_attn_error(r.err, "write")
+        r.err.zero_()
+        K().kv_read(r.cache, r.seq, r.pos, pages, ko, vo, r.err)
+        torch.cuda.synchronize()
+        assert int(r.err[0]) == 1
+        assert torch.isnan(r.q_out[2]).all() and torch.isnan(ko[2]).all() and torch.isnan(vo[2]).all()
+        assert (ko[[0, 1, 3, 4, 5]] == 0).all()
+        assert torch.equal(r.cache.k.view(torch.uint8), old[0].view(torch.uint8)) and torch.equal(r.cache.v.view(torch.uint8), old[1].view(torch.uint8))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_written_groups_of_one_value_and_of_none(cuda, bits):
+    """A constant group comes back as its BF16 rounding, one with a NaN or an infinity as NaN, its neighbours as ever."""
+    r = Rows(cuda, 3, 1, 1, 1, 128, bits, 32, seed=6, norm=False)
+    x = r.qkv.view(3, 3, 128)
+    x[0, 1:, 32:64] = 1.0 / 3
+    x[1, 1:, 40] = float("nan")
+    x[2, 1:, 127] = -float("inf")
+    K().attn_qkv_write(r.qkv, r.cache, r.seq, r.pos, r.pages, r.q_out, r.err)
+    k, v = r.read()
+    for y in (k, v):
+        assert (y[0, 0, 32:64] == x[0, 1, 32].float()).all()
+        assert torch.isnan(y[1, 0, 32:64]).all() and torch.isfinite(y[1, 0, :32]).all() and torch.isfinite(y[1, 0, 64:]).all()
+        assert torch.isnan(y[2, 0, 96:]).all() and torch.isfinite(y[2, 0, :96]).all()
+
+
+def test_write_strided_rows_and_bf16_read(cuda):
+    r = Rows(cuda, 20, 2, 4, 2, 64, 8, 64, seed=2)
+    wide = torch.randn((20, 8 * 64 + 16), device=cuda).to(torch.bfloat16)
+    q_wide = torch.full((20, 4 * 64 + 24), 3.0, dtype=torch.bfloat16, device=cuda)
+    inv = r.inv_freq(64)
+    K().attn_qkv_write(wide[:, :512], r.cache, r.seq, r.pos, r.pages, q_wide[:, :256], r.err, inv_freq=inv)
+    k, v = r.read(torch.bfloat16)
+    k32, v32 = r.read()
+    assert torch.equal(k, k32.to(torch.bfloat16)) and torch.equal(v, v32.to(torch.bfloat16))
+    assert (q_wide[:, 256:] == 3.0).all()
+    q, size = plain.norm_rotate(plain.f64(wide[:, :256]).reshape(20, 4, 64), None, 0, r.pos.cpu().numpy(), inv, False)
+    assert (np.abs(plain.f64(q_wide[:, :256]).reshape(q.shape) - q) <= plain.BF16 * np.abs(q) + 2.0 ** -20 * size).all()
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_steps_of_write_and_attend_together(cuda, bits, G):
+    """A prompt of three conversations written, then decode steps of one token and of drafts: each step writes its keys and attends over them."""
+    D, n_q, n_kv, page, B = 128, 8, 2, 16, 3
+    cache = K().KvCache.empty(40, n_kv, page, D, bits, G, cuda)
+    pages = torch.randperm(39, device=cuda).to(torch.int32).view(3, 13)
+    lens, err = [0] * B, torch.zeros(4, dtype=torch.int32, device=cuda)
+    inv = (1e4 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).float().to(cuda)
+    ws = torch.zeros(K().attn_decode_workspace_bytes(cache, n_q, 64), dtype=torch.uint8, device=cuda)
+    for step, new in enumerate([(60, 17, 1), (1, 1, 1), (3, 1, 4), (1, 0, 8)]):
+        T = sum(new)
+        seq = torch.tensor([b for b in range(B) for _ in range(new[b])], dtype=torch.int32, device=cuda)
+        pos = torch.tensor([lens[b] + i for b in range(B) for i in range(new[b])], dtype=torch.int32, device=cuda)
+        lens = [n + m for n, m in zip(lens, new)]
+        qkv = torch.randn((T, (n_q + 2 * n_kv) * D), device=cuda).to(torch.bfloat16)
+        q, out = torch.empty((T, n_q * D), dtype=torch.bfloat16, device=cuda), torch.empty((T, n_q * D), dtype=torch.bfloat16, device=cuda)
+        starts = torch.tensor(np.concatenate(([0], np.cumsum(new))), dtype=torch.int32, device=cuda)
+        kv_len = torch.tensor(lens, dtype=torch.int32, device=cuda)
+        K().attn_qkv_write(qkv, cache, seq, pos, pages, q, err, inv_freq=inv, q_norm=torch.ones(D, device=cuda), k_norm=torch.ones(D, device=cuda))
+        K().attn_decode(q, cache, pages, starts, kv_len, max(new), out, ws, err)
+        torch.cuda.synchronize()
+        want, _, tol, _ = plain.attend(q, cache, pages, starts, kv_len, D ** -0.5)
+        assert (np.abs(plain.f64(out).reshape(want.shape) - want) <= tol).all(), step
+        assert int(err[0]) == 0
