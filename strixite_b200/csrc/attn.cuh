@@ -21,8 +21,6 @@ int kv_view(const char *fn, const SxbKvCache *c, KvView *out);
 
 inline bool is_pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
 
-// Page ids of a table entry that is none.
-constexpr int kBadPage = -1;
 
 __device__ inline int64_t kv_row(const KvView &c, int page, int head, int at) {
     return page * c.page_stride + head * c.head_stride + at * c.row_stride;

@@ -25,22 +25,28 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMinRun = 2;     // units a CTA takes at least
-constexpr int kMaxIds = 16;    // pages that a tile of 128 keys touches at most
+constexpr int kMaxIds = 32;    // a warp finds a tile's pages: at most 16 of 128 keys
+constexpr int kMostPerSm = 4;
+constexpr int kSlack = 8;      // powers of two that a weight may be above 1
+constexpr int64_t kNoPage = INT64_MIN;
 constexpr int64_t kMaxRows = 1ll << 24;
 
-template <int D_, int BITS_, int G_, int WR_> struct Shape {
-    static constexpr int D = D_, BITS = BITS_, G = G_, WR = WR_;
-    static constexpr int kWarps = WR == 1 ? 4 : 8, kThreads = 32 * kWarps, WK = kWarps / WR, R = 16 * WR;
+// R query rows: NT tiles of eight a warp, WR warps side by side; the other warps share a tile's keys, KI runs of sixteen each.
+template <int D_, int BITS_, int G_, int R_> struct Shape {
+    static constexpr int D = D_, BITS = BITS_, G = G_, R = R_;
+    static constexpr int kMostNT = D == 256 ? 2 : 4, NT = R / 8 < kMostNT ? R / 8 : kMostNT, WR = R / 8 / NT;
+    static constexpr bool kQuant = BITS != 16;
+    static constexpr int kWarps = WR > 1 || (kQuant && NT == 1 && D <= 128) ? 8 : 4, kThreads = 32 * kWarps, WK = kWarps / WR;
     static constexpr int RB = D * BITS / 8, CR = RB / 16;  // bytes and 16-byte chunks of a cache row
-    static constexpr int NG = BITS == 16 ? 0 : D / G;
-    static constexpr int TK = D == 64 || (BITS == 4 && D == 128) ? 128 : 64;
-    static constexpr int KI = TK / (16 * WK);  // runs of sixteen keys of a warp's share of a tile
+    static constexpr int NG = kQuant ? D / G : 0;
+    static constexpr int TK = D == 64 || (BITS == 4 && D == 128) || (kQuant && kWarps == 8 && D == 128) ? 128 : 64;
+    static constexpr int KI = TK / (16 * WK);
     static constexpr int kRows = TK * RB, kScales = TK * NG * 4, kStage = 2 * (kRows + kScales);
     static constexpr int kQ = R * D * 2;
     static constexpr int kMostJoint = WK * R * 32 * 4;
     static constexpr bool kOwnJoint = kStage < kMostJoint;  // 32 columns of every warp's rows do not fit a stage
-    static constexpr int kMisc = 1024 + WK * R * 8 + R * (NG + 1) * 4 + (kOwnJoint ? kMostJoint : 0);
-    static constexpr int kPerSm = WR == 1 && D <= 128 ? 2 : 1;
+    static constexpr int kMisc = 1280 + WK * R * 8 + R * (NG + 2) * 4 + (kOwnJoint ? kMostJoint : 0);
+    static constexpr int kPerSm = D <= 128 && (kWarps == 4 || NT == 1) ? 2 : 1;
     static constexpr int kBudget = 226 * 1024 / kPerSm;
     static constexpr int kFit = (kBudget - kMisc) / (kStage + kQ), kStages = kFit > 5 ? 5 : kFit;
     static constexpr int kSmem = kStages * (kStage + kQ) + kMisc;
@@ -50,7 +56,11 @@ template <int D_, int BITS_, int G_, int WR_> struct Shape {
         return dc;
     }
     static constexpr int DC = fit_columns();  // columns that the warps join at a time
-    static_assert(kStages >= 2 && KI >= 1 && kThreads % CR == 0, "");
+    // Codes stay 1024 (8 bits) or 64 (4 bits) too large as F16 operands, and what that adds is taken out of the sums
+    static constexpr float kOffset = BITS == 8 ? 1024.f : 64.f;
+    static constexpr bool kOffsetV = kQuant && NG * NT <= 8;  // for V it takes four accumulators a group and row tile
+    static constexpr bool kHoldQ = NT * D <= 256;             // q's fragments in registers
+    static_assert(kStages >= 2 && KI >= 1 && kThreads % CR == 0 && WK * WR == kWarps, "");
 };
 
 struct Args {
@@ -130,14 +140,19 @@ __device__ inline uint32_t pack_f16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// 1024 + code in both halves, less 1024: exact.
-__device__ inline uint32_t less_1024(uint32_t v) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&v), __half2half2(__ushort_as_half(0x6400)));
+// Two bytes of a word (named by the selector's nibbles 0 and 2) as F16 numbers 1024 + code; two nibbles (bits 4 to 7 of each half) as 64 + code.
+__device__ inline uint32_t bytes_f16(uint32_t w, uint32_t selector) { return __byte_perm(w, 0x64646464u, selector); }
+__device__ inline uint32_t nibbles_f16(uint32_t w) { return (w & 0x00f000f0u) | 0x54005400u; }
+// The same less the offset: exact.
+template <int BITS> __device__ inline uint32_t less_offset(uint32_t v) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&v), __half2half2(__ushort_as_half(BITS == 8 ? 0x6400 : 0x5400)));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-// Codes two bytes (named by the selector's nibbles 0 and 2) or two nibbles (at bits 0 and 16) of a word as F16.
-__device__ inline uint32_t bytes_f16(uint32_t w, uint32_t selector) { return less_1024(__byte_perm(w, 0x64646464u, selector)); }
-__device__ inline uint32_t nibbles_f16(uint32_t w) { return less_1024((w & 0x000f000fu) | 0x64006400u); }
+__device__ inline uint32_t transposed(uint32_t v) {  // of an 8 x 8 tile of 16-bit numbers, a lane's two neighbours in a row
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
 
 // Where chunk c of row r stands in a tile of rows of CR chunks: eight neighbouring rows' chunks of one number lie in eight different sixteenths of the
 // banks' 128 bytes.
@@ -154,19 +169,19 @@ template <class S> __device__ inline int k_chunk_at(int r, int c) {
 
 template <class S>
 __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(const __grid_constant__ Args a) {
-    constexpr int D = S::D, BITS = S::BITS, NG = S::NG, TK = S::TK, KI = S::KI, R = S::R, WK = S::WK, CR = S::CR, kStages = S::kStages;
-    constexpr bool kQuant = BITS != 16;
-    constexpr int kThreads = S::kThreads, kWarps = S::kWarps;
+    constexpr int D = S::D, BITS = S::BITS, NG = S::NG, TK = S::TK, KI = S::KI, R = S::R, WK = S::WK, CR = S::CR, NT = S::NT, kStages = S::kStages;
+    constexpr bool kQuant = S::kQuant;
+    constexpr int kThreads = S::kThreads, kWarps = S::kWarps, kGroups = kQuant ? NG : 1;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *const q_ring = smem + kStages * S::kStage;
     uint8_t *const own_joint = q_ring + kStages * S::kQ, *const misc = own_joint + (S::kOwnJoint ? S::kMostJoint : 0);
     auto *const row_max = reinterpret_cast<float *>(misc);  // [WK][R]
     float *const row_sum = row_max + WK * R;                // [WK][R]
     float *const q_factor = row_sum + WK * R;               // [R]
-    float *const q_sums = q_factor + R;                     // [R][NG]
-    auto *const segments = reinterpret_cast<Segment *>(q_sums + R * NG);  // [kStages]
-    auto *const ids = reinterpret_cast<int *>(segments + kStages);        // [2][kMaxIds]
-    auto *const scan = reinterpret_cast<int64_t *>((reinterpret_cast<uintptr_t>(ids + 2 * kMaxIds) + 7) & ~(uintptr_t)7);  // [kWarps + 4]
+    float *const q_sums = q_factor + R;                     // [NG][R]
+    auto *const places = reinterpret_cast<int64_t *>(q_sums + R * (NG + (NG & 1)));  // [2][kMaxIds]: row numbers of the tile's pages' first tokens
+    auto *const scan = places + 2 * kMaxIds;                                         // [kWarps + 2]
+    auto *const segments = reinterpret_cast<Segment *>(scan + kWarps + 2);           // [kStages]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int wr = warp % S::WR, wk = warp / S::WR;
 
@@ -235,15 +250,25 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     const int units = (int)(u1 - u0);
     const int page_mask = (1 << a.c.page_shift) - 1;
 
-    // page id number tid of the tile under the cursor
-    auto find_id = [&]() -> int {
+    // row number of the first token of the page number tid of the tile under the cursor; kNoPage where the sequence has none there or a bad one
+    auto find_page = [&]() -> int64_t {
         const int first = (l_s.tile0 + l_at) * TK, col = (first >> a.c.page_shift) + tid;
         const int end = min(l_s.len, first + TK);
-        if (((int64_t)col << a.c.page_shift) >= end || (((int64_t)col + 1) << a.c.page_shift) <= l_s.lo) return kBadPage;
+        if (((int64_t)col << a.c.page_shift) >= end || (((int64_t)col + 1) << a.c.page_shift) <= l_s.lo) return kNoPage;
         const int id = a.pages[l_b * a.pages_ld + col];
-        if ((unsigned)id < (unsigned)a.c.n_pages) return id;
+        if ((unsigned)id < (unsigned)a.c.n_pages) return id * a.c.page_stride + l_head * a.c.head_stride;
         raise_error(a.err, (uint32_t)l_b, (uint32_t)id);
-        return kBadPage;
+        return kNoPage;
+    };
+    // Lanes 0 .. kMaxIds - 1 of the first warp find them for the cursor's tile, and whether the tile is whole: every row there.
+    auto put_pages = [&](int which, int64_t place) {
+        if (tid < kMaxIds) {
+            places[which * kMaxIds + tid] = place;
+            const int first = (l_s.tile0 + l_at) * TK;
+            const int pages = max(1, TK >> a.c.page_shift);
+            const bool fine = __all_sync(0xffffffffu, tid >= pages || place != kNoPage) && first >= l_s.lo && first + TK <= l_s.len;
+            if (tid == 0) scan[which] = fine;
+        }
     };
     auto advance = [&]() {
         l_new = false;
@@ -258,38 +283,78 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             l_s = sequence<S>(a, l_b);
         } while (l_s.n == 0);
     };
-    auto load = [&](int stage, const int *id_of) {
+    constexpr int kPass = kThreads / CR, kPasses = TK / kPass;  // rows that the CTA's threads fetch at a time
+    static_assert(TK % kPass == 0, "");
+    const int l_chunk = tid % CR, l_row = tid / CR;
+    auto load = [&](int stage, int which) {
         uint8_t *const st = smem + stage * S::kStage;
-        const int first = (l_s.tile0 + l_at) * TK, col0 = first >> a.c.page_shift;
-        {
-            const int c = tid % CR;
-            const int64_t head_rows = l_head * a.c.head_stride;
-#pragma unroll 4
-            for (int r = tid / CR; r < TK; r += kThreads / CR) {
-                const int j = first + r, id = id_of[(j >> a.c.page_shift) - col0];
-                const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && id >= 0;
-                const int64_t off = there ? (id * a.c.page_stride + head_rows + (j & page_mask) * a.c.row_stride) * S::RB + c * 16 : 0;
-                uint8_t *const to = st + k_chunk_at<S>(r, c) * 16;
+        const int64_t *const place = places + which * kMaxIds;
+        const int first = (l_s.tile0 + l_at) * TK;
+        constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = kQuant ? NG * 4 / kBytes : 1;
+        if (scan[which] != 0) {
+            const bool one_page = TK <= page_mask + 1;
+            const int base = first & page_mask;
+            const int64_t row_bytes = a.c.row_stride * S::RB;
+            if (one_page) {
+                const int64_t off = (place[0] + (base + l_row) * a.c.row_stride) * S::RB + l_chunk * 16;
+                const uint8_t *k = a.c.k + off, *v = a.c.v + off;
+#pragma unroll
+                for (int i = 0; i < kPasses; ++i) {
+                    copy_async<16>(smem_of(st + k_chunk_at<S>(l_row + i * kPass, l_chunk) * 16), k, 16);
+                    copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(l_row + i * kPass, l_chunk) * 16), v, 16);
+                    k += kPass * row_bytes, v += kPass * row_bytes;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPasses; ++i) {
+                    const int r = l_row + i * kPass;
+                    const int64_t off = (place[r >> a.c.page_shift] + (r & page_mask) * a.c.row_stride) * S::RB + l_chunk * 16;
+                    copy_async<16>(smem_of(st + k_chunk_at<S>(r, l_chunk) * 16), a.c.k + off, 16);
+                    copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(r, l_chunk) * 16), a.c.v + off, 16);
+                }
+            }
+            if constexpr (kQuant) {
+                uint8_t *const sc = st + 2 * S::kRows;
+#pragma unroll
+                for (int i0 = 0; i0 < TK * kPieces; i0 += kThreads) {
+                    const int i = i0 + tid, r = i / kPieces;
+                    if (TK * kPieces % kThreads == 0 || i < TK * kPieces) {
+                        const int64_t off = (place[one_page ? 0 : r >> a.c.page_shift] + ((base + r) & page_mask) * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes;
+                        copy_async<kBytes>(smem_of(sc + i * kBytes), reinterpret_cast<const uint8_t *>(a.c.k_sm) + off, kBytes);
+                        copy_async<kBytes>(smem_of(sc + S::kScales + i * kBytes), reinterpret_cast<const uint8_t *>(a.c.v_sm) + off, kBytes);
+                    }
+                }
+            }
+        } else {  // a sequence's first or last tile, or one with a bad page: rows out of range are zeros, keys of a bad page NaN
+            const int col0 = first >> a.c.page_shift;
+#pragma unroll 1
+            for (int r = l_row; r < TK; r += kPass) {
+                const int j = first + r;
+                const int64_t page = place[(j >> a.c.page_shift) - col0];
+                const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && page != kNoPage;
+                const int64_t off = there ? (page + (j & page_mask) * a.c.row_stride) * S::RB + l_chunk * 16 : 0;
+                uint8_t *const to = st + k_chunk_at<S>(r, l_chunk) * 16;
                 if (!kQuant && wanted && !there) *reinterpret_cast<uint4 *>(to) = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
                 else copy_async<16>(smem_of(to), a.c.k + off, there ? 16 : 0);
-                copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(r, c) * 16), a.c.v + off, there ? 16 : 0);
+                copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(r, l_chunk) * 16), a.c.v + off, there ? 16 : 0);
             }
-        }
-        if constexpr (kQuant) {
-            constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = NG * 4 / kBytes;
-            uint8_t *const sc = st + 2 * S::kRows;
-            for (int i = tid; i < TK * kPieces; i += kThreads) {
-                const int r = i / kPieces, j = first + r, id = id_of[(j >> a.c.page_shift) - col0];
-                const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && id >= 0;
-                const int64_t off = there ? (id * a.c.page_stride + l_head * a.c.head_stride + (j & page_mask) * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes : 0;
-                uint8_t *const to = sc + i * kBytes;
-                if (wanted && !there) {
+            if constexpr (kQuant) {
+                uint8_t *const sc = st + 2 * S::kRows;
+#pragma unroll 1
+                for (int i = tid; i < TK * kPieces; i += kThreads) {
+                    const int r = i / kPieces, j = first + r;
+                    const int64_t page = place[(j >> a.c.page_shift) - col0];
+                    const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && page != kNoPage;
+                    const int64_t off = there ? (page + (j & page_mask) * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes : 0;
+                    uint8_t *const to = sc + i * kBytes;
+                    if (wanted && !there) {
 #pragma unroll
-                    for (int w = 0; w < kBytes / 4; ++w) reinterpret_cast<uint32_t *>(to)[w] = 0x7fc07fc0u;
-                } else {
-                    copy_async<kBytes>(smem_of(to), reinterpret_cast<const uint8_t *>(a.c.k_sm) + off, there ? kBytes : 0);
+                        for (int w = 0; w < kBytes / 4; ++w) reinterpret_cast<uint32_t *>(to)[w] = 0x7fc07fc0u;
+                    } else {
+                        copy_async<kBytes>(smem_of(to), reinterpret_cast<const uint8_t *>(a.c.k_sm) + off, there ? kBytes : 0);
+                    }
+                    copy_async<kBytes>(smem_of(to + S::kScales), reinterpret_cast<const uint8_t *>(a.c.v_sm) + off, there ? kBytes : 0);
                 }
-                copy_async<kBytes>(smem_of(to + S::kScales), reinterpret_cast<const uint8_t *>(a.c.v_sm) + off, there ? kBytes : 0);
             }
         }
         if (l_new) {
@@ -306,14 +371,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         }
     };
 
-    if (tid < kMaxIds) ids[tid] = find_id();
+    __syncthreads();  // scan is read
+    put_pages(0, tid < kMaxIds ? find_page() : kNoPage);
     __syncthreads();
     for (int s = 0; s < kStages - 1; ++s) {
         if (s < units) {
-            load(s, ids + (s & 1) * kMaxIds);
+            load(s, s & 1);
             if (s + 1 < units) {
                 advance();
-                if (tid < kMaxIds) ids[((s + 1) & 1) * kMaxIds + tid] = find_id();
+                put_pages((s + 1) & 1, tid < kMaxIds ? find_page() : kNoPage);
             }
             __syncthreads();
         }
@@ -321,27 +387,29 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     }
 
     // ---- sums ----
+    // Keys are the rows of the score product (A), queries its columns (B): an accumulator holds keys g and g + 8 of queries 2 t and 2 t + 1.  Of the
+    // second product V's columns are the rows, its accumulators hold the same two queries, and the weights get from the first one's layout to the
+    // second operand's by a transposition in registers.
     const int g = lane >> 2, t4 = lane & 3;
-    constexpr int kQRegs = D <= 128 ? D / 16 : 1;
-    uint32_t qf[kQRegs][4];
-    float o[D / 8][4];
-    float o_min[2][kQuant ? NG : 1];
-    float m[2], l[2], fac[2];
-    int hi[2], lo[2], v_exp = 20;
+    uint32_t qf[S::kHoldQ ? NT : 1][S::kHoldQ ? D / 16 : 1][2];
+    float o[D / 16][NT][4], w_sum[S::kOffsetV ? NG : 1][NT][4], o_min[kGroups][NT][2];
+    float m[NT][2], l[NT][2], fac[NT][2];
+    int hi[NT][2], lo[NT][2], v_exp = 20;
     Segment sg{};
     int at = 0, segment = 0;
     bool fresh = true;
+    const int a_row = lane & 15, a_half = lane >> 4;  // of a fragment of sixteen rows, two chunks
 
     for (int i = 0; i < units; ++i) {
         wait_async<kStages - 2>();
         __syncthreads();
-        int next_id = kBadPage;
         const int ahead = i + kStages - 1;
+        int64_t next_place = kNoPage;
         if (ahead < units) {
-            load(ahead % kStages, ids + (ahead & 1) * kMaxIds);
+            load(ahead % kStages, ahead & 1);
             if (ahead + 1 < units) {
                 advance();
-                if (tid < kMaxIds) next_id = find_id();
+                if (tid < kMaxIds) next_place = find_page();
             }
         }
         commit_async();
@@ -351,21 +419,26 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         if (fresh) {
             fresh = false;
             sg = segments[segment % kStages];
-            at = sg.at;
-            m[0] = m[1] = -CUDART_INF_F, l[0] = l[1] = 0.f, v_exp = 20;
+            at = sg.at, v_exp = 20;
 #pragma unroll
-            for (int d = 0; d < D / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+            for (int nt = 0; nt < NT; ++nt) {
+                m[nt][0] = m[nt][1] = -CUDART_INF_F, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-            for (int e = 0; e < (kQuant ? NG : 1); ++e) o_min[0][e] = o_min[1][e] = 0.f;
+                for (int d = 0; d < D / 16; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int tok = (sg.rows0 + wr * 16 + g + 8 * e) / a.group;
-                hi[e] = tok < sg.n ? sg.p0 + tok : -1;
-                lo[e] = a.window > 0 ? max(-1, hi[e] - a.window) : -1;
+                for (int e = 0; e < kGroups; ++e) o_min[e][nt][0] = o_min[e][nt][1] = 0.f;
+#pragma unroll
+                for (int e = 0; e < (S::kOffsetV ? NG : 1); ++e) w_sum[e][nt][0] = w_sum[e][nt][1] = w_sum[e][nt][2] = w_sum[e][nt][3] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int tok = (sg.rows0 + (wr * NT + nt) * 8 + 2 * t4 + e) / a.group;
+                    hi[nt][e] = tok < sg.n ? sg.p0 + tok : -1;
+                    lo[nt][e] = a.window > 0 ? max(-1, hi[nt][e] - a.window) : -1;
+                }
             }
             if constexpr (kQuant) {
                 // q to F16 times a power of two, elements in the order that the codes come in, and each group's sum of what they then are
-                constexpr int kPer = kThreads / R, kBlocks = D / 32;  // threads of a row; runs of 32 elements
+                constexpr int kPer = kThreads / R < 32 ? kThreads / R : 32, kBlocks = D / 32;  // threads of a row; runs of 32 elements
                 constexpr int kOwn = (kBlocks + kPer - 1) / kPer;
                 const int r = tid / kPer, part = tid % kPer;
                 float x[kOwn][32], most = 0.f;
@@ -413,150 +486,205 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     static_assert(kRuns <= kPer, "");
 #pragma unroll
                     for (int off = 1; off < kRuns; off <<= 1) sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], off);
-                    if (blk < kBlocks && blk % kRuns == 0) q_sums[r * NG + blk / kRuns] = sums[b];
+                    if (blk < kBlocks && blk % kRuns == 0) q_sums[blk / kRuns * R + r] = sums[b];
                 }
                 __syncthreads();
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e) fac[e] = a.scale * (kQuant ? q_factor[wr * 16 + g + 8 * e] : 1.f);
-            if constexpr (D <= 128) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    load_matrices(qf[ks], smem_of(qs + chunk_at<D / 8>(wr * 16 + (lane & 15), ks * 2 + (lane >> 4)) * 16));
+                for (int e = 0; e < 2; ++e) fac[nt][e] = a.scale * (a.softcap > 0.f ? 1.f : kLog2e) * (kQuant ? q_factor[(wr * NT + nt) * 8 + 2 * t4 + e] : 1.f);
+            if constexpr (S::kHoldQ) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ks += 2) {
+                        uint32_t r[4];
+                        load_matrices(r, smem_of(qs + chunk_at<D / 8>((wr * NT + nt) * 8 + (lane & 7), ks * 2 + (lane >> 3)) * 16));
+                        qf[nt][ks][0] = r[0], qf[nt][ks][1] = r[1], qf[nt][ks + 1][0] = r[2], qf[nt][ks + 1][1] = r[3];
+                    }
             }
         }
-        auto q_at = [&](int ks, uint32_t (&r)[4]) {
-            if constexpr (D <= 128) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = qf[ks][e];
-            } else {
-                load_matrices(r, smem_of(qs + chunk_at<D / 8>(wr * 16 + (lane & 15), ks * 2 + (lane >> 4)) * 16));
-            }
+        // q's fragments of two steps of sixteen elements
+        auto q_at = [&](int nt, int ks, uint32_t (&r)[4]) {
+            if constexpr (S::kHoldQ) r[0] = qf[nt][ks][0], r[1] = qf[nt][ks][1], r[2] = qf[nt][ks + 1][0], r[3] = qf[nt][ks + 1][1];
+            else load_matrices(r, smem_of(qs + chunk_at<D / 8>((wr * NT + nt) * 8 + (lane & 7), ks * 2 + (lane >> 3)) * 16));
         };
 
         // scores
         const int first = (sg.tile0 + at) * TK;
-        float s[KI][2][4];
+        float s[KI][NT][4];
         const auto *const k_sm = reinterpret_cast<const uint32_t *>(st + 2 * S::kRows), *const v_sm = k_sm + TK * NG;
 #pragma unroll
         for (int ki = 0; ki < KI; ++ki) {
             const int key0 = (wk * KI + ki) * 16;
 #pragma unroll
-            for (int tl = 0; tl < 2; ++tl) s[ki][tl][0] = s[ki][tl][1] = s[ki][tl][2] = s[ki][tl][3] = 0.f;
+            for (int nt = 0; nt < NT; ++nt) s[ki][nt][0] = s[ki][nt][1] = s[ki][nt][2] = s[ki][nt][3] = 0.f;
             if constexpr (!kQuant) {
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    uint32_t b[4], q[4];
-                    load_matrices(b, smem_of(st + k_chunk_at<S>(key0 + (lane & 7) + ((lane >> 4) & 1) * 8, ks * 2 + ((lane >> 3) & 1)) * 16));
-                    q_at(ks, q);
-                    mma_bf16(s[ki][0], q[0], q[1], q[2], q[3], b[0], b[1]);
-                    mma_bf16(s[ki][1], q[0], q[1], q[2], q[3], b[2], b[3]);
+                for (int ks = 0; ks < D / 16; ks += 2) {
+                    uint32_t k0[4], k1[4];
+                    load_matrices(k0, smem_of(st + k_chunk_at<S>(key0 + a_row, ks * 2 + a_half) * 16));
+                    load_matrices(k1, smem_of(st + k_chunk_at<S>(key0 + a_row, ks * 2 + 2 + a_half) * 16));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        uint32_t q[4];
+                        q_at(nt, ks, q);
+                        mma_bf16(s[ki][nt], k0[0], k0[1], k0[2], k0[3], q[0], q[1]);
+                        mma_bf16(s[ki][nt], k1[0], k1[1], k1[2], k1[3], q[2], q[3]);
+                    }
                 }
             } else {
 #pragma unroll
                 for (int grp = 0; grp < NG; ++grp) {
-                    float part[2][4] = {};
+                    float part[NT][4] = {};
 #pragma unroll
                     for (int run = 0; run < S::G / 32; ++run) {
                         const int blk = grp * (S::G / 32) + run;
-                        uint32_t q0[4], q1[4];
-                        q_at(blk * 2, q0), q_at(blk * 2 + 1, q1);
+                        uint32_t k0[4], k1[4];
+                        if constexpr (BITS == 8) {
+                            const uint2 w0 = *reinterpret_cast<const uint2 *>(st + k_chunk_at<S>(key0 + g, blk * 2 + (t4 >> 1)) * 16 + (t4 & 1) * 8);
+                            const uint2 w1 = *reinterpret_cast<const uint2 *>(st + k_chunk_at<S>(key0 + g + 8, blk * 2 + (t4 >> 1)) * 16 + (t4 & 1) * 8);
+                            k0[0] = bytes_f16(w0.x, 0x4140), k0[1] = bytes_f16(w1.x, 0x4140), k0[2] = bytes_f16(w0.x, 0x4342), k0[3] = bytes_f16(w1.x, 0x4342);
+                            k1[0] = bytes_f16(w0.y, 0x4140), k1[1] = bytes_f16(w1.y, 0x4140), k1[2] = bytes_f16(w0.y, 0x4342), k1[3] = bytes_f16(w1.y, 0x4342);
+                        } else {
+                            const uint32_t w0 = *reinterpret_cast<const uint32_t *>(st + k_chunk_at<S>(key0 + g, blk) * 16 + t4 * 4);
+                            const uint32_t w1 = *reinterpret_cast<const uint32_t *>(st + k_chunk_at<S>(key0 + g + 8, blk) * 16 + t4 * 4);
+                            k0[0] = nibbles_f16(w0 << 4), k0[1] = nibbles_f16(w1 << 4), k0[2] = nibbles_f16(w0), k0[3] = nibbles_f16(w1);
+                            k1[0] = nibbles_f16(w0 >> 4), k1[1] = nibbles_f16(w1 >> 4), k1[2] = nibbles_f16(w0 >> 8), k1[3] = nibbles_f16(w1 >> 8);
+                        }
 #pragma unroll
-                        for (int tl = 0; tl < 2; ++tl) {
-                            const int key = key0 + tl * 8 + g;
-                            if constexpr (BITS == 8) {
-                                const uint2 w = *reinterpret_cast<const uint2 *>(st + k_chunk_at<S>(key, blk * 2 + (t4 >> 1)) * 16 + (t4 & 1) * 8);
-                                mma_f16(part[tl], q0, bytes_f16(w.x, 0x4140), bytes_f16(w.x, 0x4342));
-                                mma_f16(part[tl], q1, bytes_f16(w.y, 0x4140), bytes_f16(w.y, 0x4342));
-                            } else {
-                                const uint32_t w = *reinterpret_cast<const uint32_t *>(st + k_chunk_at<S>(key, blk) * 16 + t4 * 4);
-                                mma_f16(part[tl], q0, nibbles_f16(w), nibbles_f16(w >> 4));
-                                mma_f16(part[tl], q1, nibbles_f16(w >> 8), nibbles_f16(w >> 12));
-                            }
+                        for (int nt = 0; nt < NT; ++nt) {
+                            uint32_t q[4];
+                            q_at(nt, blk * 2, q);
+                            mma_f16(part[nt], k0, q[0], q[1]);
+                            mma_f16(part[nt], k1, q[2], q[3]);
                         }
                     }
-                    const float qs0 = q_sums[(wr * 16 + g) * NG + grp], qs1 = q_sums[(wr * 16 + g + 8) * NG + grp];
+                    float sc[2], mn[2];
 #pragma unroll
-                    for (int tl = 0; tl < 2; ++tl)
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t w = k_sm[(key0 + g + 8 * e) * NG + grp];
+                        sc[e] = __uint_as_float(w << 16);
+                        mn[e] = fmaf(-S::kOffset, sc[e], __uint_as_float(w & 0xffff0000u));
+                    }
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t w = k_sm[(key0 + tl * 8 + 2 * t4 + e) * NG + grp];
-                            const float sc = __uint_as_float(w << 16), mn = __uint_as_float(w & 0xffff0000u);
-                            s[ki][tl][e] = fmaf(sc, part[tl][e], fmaf(mn, qs0, s[ki][tl][e]));
-                            s[ki][tl][2 + e] = fmaf(sc, part[tl][2 + e], fmaf(mn, qs1, s[ki][tl][2 + e]));
-                        }
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float2 qsum = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(sc[e >> 1], part[nt][e], fmaf(mn[e >> 1], e & 1 ? qsum.y : qsum.x, s[ki][nt][e]));
+                    }
                 }
             }
         }
         const int p_last = sg.p0 + sg.n - 1;
         const bool whole = first >= (a.window > 0 ? p_last - a.window + 1 : 0) && first + TK - 1 <= sg.p0;
-        auto seen = [&](int ki, int tl, int e) {  // e: as in an accumulator
-            const int j = first + (wk * KI + ki) * 16 + tl * 8 + 2 * t4 + (e & 1);
-            return j <= hi[e >> 1] && j > lo[e >> 1];
+        auto seen = [&](int ki, int nt, int e) {  // e: as in an accumulator
+            const int j = first + (wk * KI + ki) * 16 + g + 8 * (e >> 1);
+            return j <= hi[nt][e & 1] && j > lo[nt][e & 1];
         };
-        float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
         for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
-            for (int tl = 0; tl < 2; ++tl)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = s[ki][tl][e] * fac[e >> 1];
-                    if (a.softcap > 0.f) v = a.softcap * tanhf(v / a.softcap);
-                    v *= kLog2e;
-                    if (!whole && !seen(ki, tl, e)) v = -CUDART_INF_F;
-                    s[ki][tl][e] = v;
-                    top[e >> 1] = fmaxf(top[e >> 1], v);
-                }
-        float alpha[2];
+                for (int e = 0; e < 4; ++e) s[ki][nt][e] *= fac[nt][e & 1];
+        if (a.softcap > 0.f) {
+            const float by = 1.f / a.softcap, to = a.softcap * kLog2e;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-            const float now = fmaxf(m[e], top[e]), base = now == -CUDART_INF_F ? 0.f : now;
-            alpha[e] = exp2_fast(m[e] - base);
-            m[e] = now, top[e] = base;
+            for (int ki = 0; ki < KI; ++ki)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = to * tanhf(s[ki][nt][e] * by);
         }
-        float sum[2] = {0.f, 0.f};
+        if (!whole) {
 #pragma unroll
-        for (int ki = 0; ki < KI; ++ki)
+            for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
-            for (int tl = 0; tl < 2; ++tl)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[ki][tl][e] = exp2_fast(s[ki][tl][e] - top[e >> 1]);
-                    sum[e >> 1] += s[ki][tl][e];
-                }
-        l[0] = fmaf(l[0], alpha[0], sum[0]), l[1] = fmaf(l[1], alpha[1], sum[1]);
-
-        // the largest scale of this warp's values, for the power of two that keeps weight times scale inside F16
-        bool rescale = alpha[0] != 1.f || alpha[1] != 1.f;
-        float o_scale[2] = {alpha[0], alpha[1]};
+                    for (int e = 0; e < 4; ++e)
+                        if (!seen(ki, nt, e)) s[ki][nt][e] = -CUDART_INF_F;
+        }
+        // The maximum that the weights are relative to is moved when a score passes it by 2^kSlack only: most tiles then need no exchange between lanes and
+        // no sum is touched.  The scale that the weights of quantized values are relative to, likewise.
+        bool move = false;
+        float top[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float v = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
+#pragma unroll
+                for (int ki = 1; ki < KI; ++ki) v = fmaxf(v, fmaxf(s[ki][nt][e], s[ki][nt][2 + e]));
+                top[nt][e] = v;
+                move = move || v > m[nt][e] + kSlack;
+            }
+        float v_top = 0.f;
         if constexpr (kQuant) {
-            int e_top = 0;
 #pragma unroll
-            for (int ki = 0; ki < KI; ++ki) {
-                const int key = (wk * KI + ki) * 16 + (lane & 15);
+            for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
-                for (int grp = 0; grp < NG; ++grp) {
-                    const int ex = (int)(v_sm[key * NG + grp] >> 7 & 0xffu);
-                    if (ex != 255) e_top = max(e_top, ex);
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int grp = 0; grp < NG; ++grp) v_top = fmaxf(v_top, __uint_as_float(v_sm[((wk * KI + ki) * 16 + g + 8 * e) * NG + grp] << 16 & 0x7fffffffu));
+            move = move || (__float_as_uint(v_top) >> 23) > (uint32_t)v_exp;
+        }
+        if (__any_sync(0xffffffffu, move)) {
+            float f[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v = top[nt][e];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+                    const float now = fmaxf(m[nt][e], v);
+                    f[nt][e] = exp2_fast(m[nt][e] - (now == -CUDART_INF_F ? 0.f : now));
+                    m[nt][e] = now, l[nt][e] *= f[nt][e];
+#pragma unroll
+                    for (int grp = 0; grp < kGroups; ++grp) o_min[grp][nt][e] *= f[nt][e];
                 }
+            if constexpr (kQuant) {
+                int ex = 0;
+#pragma unroll
+                for (int ki = 0; ki < KI; ++ki)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int grp = 0; grp < NG; ++grp) {
+                            const int x = (int)(v_sm[((wk * KI + ki) * 16 + g + 8 * e) * NG + grp] >> 7 & 0xffu);
+                            if (x != 255) ex = max(ex, x);  // a scale that is none says nothing of the others
+                        }
+                ex = max(v_exp, __reduce_max_sync(0xffffffffu, ex));
+                const float down = exp2_fast((float)(v_exp - ex));
+                v_exp = ex;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) f[nt][0] *= down, f[nt][1] *= down;
             }
-            e_top = __reduce_max_sync(0xffffffffu, e_top);
-            if (e_top > v_exp) {
-                const float f = exp2_fast((float)(v_exp - e_top));
-                o_scale[0] *= f, o_scale[1] *= f;
-                v_exp = e_top, rescale = true;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][nt][e] *= f[nt][e & 1];
+#pragma unroll
+                for (int grp = 0; grp < (S::kOffsetV ? NG : 1); ++grp)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w_sum[grp][nt][e] *= f[nt][e & 1];
             }
         }
-        if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-            for (int d = 0; d < D / 8; ++d) o[d][0] *= o_scale[0], o[d][1] *= o_scale[0], o[d][2] *= o_scale[1], o[d][3] *= o_scale[1];
-            if constexpr (kQuant) {
+        for (int nt = 0; nt < NT; ++nt) {
+            const float base[2] = {m[nt][0] == -CUDART_INF_F ? 0.f : m[nt][0], m[nt][1] == -CUDART_INF_F ? 0.f : m[nt][1]};
 #pragma unroll
-                for (int grp = 0; grp < NG; ++grp) o_min[0][grp] *= alpha[0], o_min[1][grp] *= alpha[1];
-            }
+            for (int ki = 0; ki < KI; ++ki)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[ki][nt][e] = exp2_fast(s[ki][nt][e] - base[e & 1]);
+                    l[nt][e & 1] += s[ki][nt][e];
+                }
         }
 
         // weights times values
@@ -577,91 +705,116 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     clean = __all_sync(0xffffffffu, clean);
                 }
                 if (clean) {
-                    const uint32_t p0 = pack_bf16(s[ki][0][0], s[ki][0][1]), p1 = pack_bf16(s[ki][0][2], s[ki][0][3]);
-                    const uint32_t p2 = pack_bf16(s[ki][1][0], s[ki][1][1]), p3 = pack_bf16(s[ki][1][2], s[ki][1][3]);
+                    uint32_t p[NT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        p[nt][0] = transposed(pack_bf16(s[ki][nt][0], s[ki][nt][1]));
+                        p[nt][1] = transposed(pack_bf16(s[ki][nt][2], s[ki][nt][3]));
+                    }
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d) {
-                        uint32_t b[4];
-                        load_matrices_trans(b, smem_of(vt + chunk_at<CR>(key0 + (lane & 15), d * 2 + (lane >> 4)) * 16));
-                        mma_bf16(o[2 * d], p0, p1, p2, p3, b[0], b[1]);
-                        mma_bf16(o[2 * d + 1], p0, p1, p2, p3, b[2], b[3]);
+                        uint32_t v[4];  // columns 0 - 7 and 8 - 15 of keys 0 - 7, then of keys 8 - 15
+                        load_matrices_trans(v, smem_of(vt + chunk_at<CR>(key0 + (lane & 7) + 8 * (lane >> 4), d * 2 + ((lane >> 3) & 1)) * 16));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_bf16(o[d][nt], v[0], v[1], v[2], v[3], p[nt][0], p[nt][1]);
                     }
                 } else {
 #pragma unroll 1
                     for (int k = 0; k < 16; ++k) {
-                        const int from = (lane & ~3) | (k % 8 / 2), j = first + key0 + k;
-                        float w[2];
+                        const int from = (k % 8) * 4 + t4, j = first + key0 + k;
+                        float w[NT][2];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float even = __shfl_sync(0xffffffffu, k < 8 ? s[ki][0][2 * e] : s[ki][1][2 * e], from);
-                            const float odd = __shfl_sync(0xffffffffu, k < 8 ? s[ki][0][2 * e + 1] : s[ki][1][2 * e + 1], from);
-                            w[e] = k & 1 ? odd : even;
-                        }
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int d = 0; d < D / 8; ++d) {
-                            const uint32_t v = *reinterpret_cast<const uint32_t *>(vt + chunk_at<CR>(key0 + k, d) * 16 + t4 * 4);
-                            const float v0 = __uint_as_float(v << 16), v1 = __uint_as_float(v & 0xffff0000u);
+                            for (int e = 0; e < 2; ++e) {
+                                const float low = __shfl_sync(0xffffffffu, s[ki][nt][e], from), high = __shfl_sync(0xffffffffu, s[ki][nt][2 + e], from);
+                                w[nt][e] = k < 8 ? low : high;
+                            }
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if (j <= hi[e] && j > lo[e]) o[d][2 * e] = fmaf(w[e], v0, o[d][2 * e]), o[d][2 * e + 1] = fmaf(w[e], v1, o[d][2 * e + 1]);
+                        for (int d = 0; d < D / 16; ++d) {
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const float v = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(vt + chunk_at<CR>(key0 + k, 2 * d + half) * 16 + g * 2));
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e)
+                                        if (j <= hi[nt][e] && j > lo[nt][e]) o[d][nt][2 * half + e] = fmaf(w[nt][e], v, o[d][nt][2 * half + e]);
+                            }
                         }
                     }
                 }
             }
         } else {
-            const float v_up = __uint_as_float((uint32_t)(141 - v_exp + 127) << 23);  // 2^(14 - (v_exp - 127))
+            const float v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);  // 2^(14 - kSlack - (v_exp - 127))
 #pragma unroll
             for (int ki = 0; ki < KI; ++ki) {
                 const int key0 = (wk * KI + ki) * 16;
 #pragma unroll
                 for (int grp = 0; grp < NG; ++grp) {
-                    float w[2][4];
+                    float sc[2], mn[2];
 #pragma unroll
-                    for (int tl = 0; tl < 2; ++tl)
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t x = v_sm[(key0 + g + 8 * e) * NG + grp];
+                        sc[e] = __uint_as_float(x << 16) * v_up, mn[e] = __uint_as_float(x & 0xffff0000u);
+                    }
+                    uint32_t p[NT][2];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t x = v_sm[(key0 + tl * 8 + 2 * t4 + e) * NG + grp];
-                            const float sc = __uint_as_float(x << 16) * v_up, mn = __uint_as_float(x & 0xffff0000u);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float w[4];
+                        if (whole) {
 #pragma unroll
-                            for (int rr = 0; rr < 2; ++rr) {
-                                const float p = s[ki][tl][2 * rr + e];
-                                if (whole || seen(ki, tl, 2 * rr + e)) {  // a scale or min that is none must not reach a row that does not see it
-                                    w[tl][2 * rr + e] = p * sc;
-                                    o_min[rr][grp] = fmaf(p, mn, o_min[rr][grp]);
-                                } else {
-                                    w[tl][2 * rr + e] = 0.f;
+                            for (int e = 0; e < 4; ++e) {
+                                w[e] = s[ki][nt][e] * sc[e >> 1];
+                                o_min[grp][nt][e & 1] = fmaf(s[ki][nt][e], mn[e >> 1], o_min[grp][nt][e & 1]);
+                            }
+                        } else {  // a scale or min that is none must not reach a row that does not see it
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                w[e] = 0.f;
+                                if (seen(ki, nt, e)) {
+                                    w[e] = s[ki][nt][e] * sc[e >> 1];
+                                    o_min[grp][nt][e & 1] = fmaf(s[ki][nt][e], mn[e >> 1], o_min[grp][nt][e & 1]);
                                 }
                             }
                         }
-                    const uint32_t pa[4] = {pack_f16(w[0][0], w[0][1]), pack_f16(w[0][2], w[0][3]), pack_f16(w[1][0], w[1][1]), pack_f16(w[1][2], w[1][3])};
-                    if constexpr (BITS == 8) {
-#pragma unroll
-                        for (int run = 0; run < S::G / 32; ++run) {  // two chunks of sixteen columns
-                            const int c = grp * (S::G / 16) + run * 2;
-                            uint32_t b[4];
-                            load_matrices_trans(b, smem_of(vt + chunk_at<CR>(key0 + (lane & 15), c + (lane >> 4)) * 16));
-                            mma_f16(o[2 * c], pa, bytes_f16(b[0], 0x4240), bytes_f16(b[1], 0x4240));
-                            mma_f16(o[2 * c + 1], pa, bytes_f16(b[0], 0x4341), bytes_f16(b[1], 0x4341));
-                            mma_f16(o[2 * c + 2], pa, bytes_f16(b[2], 0x4240), bytes_f16(b[3], 0x4240));
-                            mma_f16(o[2 * c + 3], pa, bytes_f16(b[2], 0x4341), bytes_f16(b[3], 0x4341));
+                        p[nt][0] = transposed(pack_f16(w[0], w[1])), p[nt][1] = transposed(pack_f16(w[2], w[3]));
+                        if constexpr (S::kOffsetV) {
+                            constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+                            mma_f16(w_sum[grp][nt], kOnes, p[nt][0], p[nt][1]);
                         }
-                    } else {
+                    }
+                    auto code = [](uint32_t v) { return S::kOffsetV ? v : less_offset<BITS>(v); };
 #pragma unroll
-                        for (int run = 0; run < S::G / 32; ++run) {  // a chunk of 32 columns; the matrices of a second one belong to another run or group
+                    for (int run = 0; run < S::G / 32; ++run) {
+                        if constexpr (BITS == 8) {  // two chunks of sixteen columns, the even ones rows 0 - 7 of a fragment, the odd ones rows 8 - 15
+                            const int c = grp * (S::G / 16) + run * 2;
+                            uint32_t v[4];
+                            load_matrices_trans(v, smem_of(vt + chunk_at<CR>(key0 + a_row, c + a_half) * 16));
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const uint32_t va[4] = {code(bytes_f16(v[2 * x], 0x4240)), code(bytes_f16(v[2 * x], 0x4341)), code(bytes_f16(v[2 * x + 1], 0x4240)),
+                                                        code(bytes_f16(v[2 * x + 1], 0x4341))};
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) mma_f16(o[c + x][nt], va, p[nt][0], p[nt][1]);
+                            }
+                        } else {  // a chunk of 32 columns: 4 n and 4 n + 1 in the first fragment, 4 n + 2 and 4 n + 3 in the second
                             const int c = grp * (S::G / 32) + run;
-                            uint32_t b0, b1;
+                            uint32_t v0, v1;
                             asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
-                                         : "=r"(b0), "=r"(b1)
-                                         : "r"(smem_of(vt + chunk_at<CR>(key0 + (lane & 15), c) * 16))
+                                         : "=r"(v0), "=r"(v1)
+                                         : "r"(smem_of(vt + chunk_at<CR>(key0 + a_row, c) * 16))
                                          : "memory");
+                            const uint32_t va[4] = {code(nibbles_f16(v0 << 4)), code(nibbles_f16(v0)), code(nibbles_f16(v1 << 4)), code(nibbles_f16(v1))};
+                            const uint32_t vb[4] = {code(nibbles_f16(v0 >> 4)), code(nibbles_f16(v0 >> 8)), code(nibbles_f16(v1 >> 4)), code(nibbles_f16(v1 >> 8))};
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) mma_f16(o[4 * c + e], pa, nibbles_f16(b0 >> (4 * e)), nibbles_f16(b1 >> (4 * e)));
+                            for (int nt = 0; nt < NT; ++nt) mma_f16(o[2 * c][nt], va, p[nt][0], p[nt][1]), mma_f16(o[2 * c + 1][nt], vb, p[nt][0], p[nt][1]);
                         }
                     }
                 }
             }
         }
-        if (tid < kMaxIds) ids[((ahead + 1) & 1) * kMaxIds + tid] = next_id;
+        if (ahead + 1 < units) put_pages((ahead + 1) & 1, next_place);
 
         if (++at < sg.tiles && i + 1 < units) continue;
 
@@ -669,24 +822,34 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         const int64_t seg0 = u0 + (i + 1) - at, seg1 = seg0 + sg.tiles;  // the segment's units in the list
         const bool split = seg0 < u0 || seg1 > u1;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-            if (t4 == 0) row_max[wk * R + wr * 16 + g + 8 * e] = m[e], row_sum[wk * R + wr * 16 + g + 8 * e] = l[e];
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+                const int r = wk * R + (wr * NT + nt) * 8 + 2 * t4 + e;
+                if (g == 0) row_max[r] = m[nt][e], row_sum[r] = l[nt][e];
+            }
         if constexpr (kQuant) {
-            const float down = __uint_as_float((uint32_t)(v_exp - 141 + 127) << 23);
+            const float down = __uint_as_float((uint32_t)(v_exp + kSlack - 141 + 127) << 23);
 #pragma unroll
-            for (int grp = 0; grp < NG; ++grp)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    o_min[e][grp] += __shfl_xor_sync(0xffffffffu, o_min[e][grp], 1);
-                    o_min[e][grp] += __shfl_xor_sync(0xffffffffu, o_min[e][grp], 2);
-                }
+                for (int grp = 0; grp < NG; ++grp)
 #pragma unroll
-            for (int d = 0; d < D / 8; ++d)
+                    for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[d][e] = fmaf(o[d][e], down, o_min[e >> 1][d * 8 / S::G]);
+                        for (int off = 4; off < 32; off <<= 1) o_min[grp][nt][e] += __shfl_xor_sync(0xffffffffu, o_min[grp][nt][e], off);
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        constexpr float off = S::kOffset;
+                        const float v = S::kOffsetV ? fmaf(-off, w_sum[S::kOffsetV ? d * 16 / S::G : 0][nt][e], o[d][nt][e]) : o[d][nt][e];
+                        o[d][nt][e] = fmaf(v, down, o_min[d * 16 / S::G][nt][e & 1]);
+                    }
         }
         __syncthreads();
         auto factor = [&](int k, int r, float top_of) { return row_max[k * R + r] == -CUDART_INF_F ? 1.f : exp2_fast(row_max[k * R + r] - top_of); };
@@ -696,46 +859,45 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             for (int k = 1; k < WK; ++k) v = fmaxf(v, row_max[k * R + r]);
             return v;
         };
-        float mine_f[2];
+        float mine_f[NT][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) mine_f[e] = factor(wk, wr * 16 + g + 8 * e, top_of(wr * 16 + g + 8 * e));
-        constexpr int DC = S::DC, kTurn = (DC / 8 - 1) & 7;
-        auto *const joint = reinterpret_cast<float *>(S::kOwnJoint ? own_joint : st);  // [WK][R][DC], pairs of columns turned by the row
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = (wr * NT + nt) * 8 + 2 * t4 + e;
+                mine_f[nt][e] = factor(wk, r, top_of(r));
+            }
+        constexpr int DC = S::DC;
+        auto *const joint = reinterpret_cast<float *>(S::kOwnJoint ? own_joint : st);  // [WK][R][DC], runs of eight columns turned by the row
         float *const part = a.partial + (2 * (int64_t)blockIdx.x + (seg0 < u0 ? 0 : 1)) * R * (D + 2);
         const int rows = min(R, sg.n * a.group - sg.rows0);
 #pragma unroll
         for (int col0 = 0; col0 < D; col0 += DC) {
             if (col0 > 0) __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = wr * 16 + g + 8 * e;
-                float *const to = joint + (wk * R + r) * DC;
-                auto put = [&](int col, float x, float y) {
-                    *reinterpret_cast<float2 *>(to + 2 * (((col - col0) / 2) ^ ((r & kTurn) << 2))) = make_float2(x * mine_f[e], y * mine_f[e]);
-                };
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int d = col0 / 8; d < (col0 + DC) / 8; ++d) {
-                    if constexpr (BITS == 16) {
-                        put(8 * d + 2 * t4, o[d][2 * e], o[d][2 * e + 1]);
-                    } else if constexpr (BITS == 8) {  // accumulators 2 c, 2 c + 1: the even and the odd columns of sixteen
-                        if (d % 2 == 0) {
-                            put(8 * d + 4 * t4, o[d][2 * e], o[d + 1][2 * e]);
-                            put(8 * d + 4 * t4 + 2, o[d][2 * e + 1], o[d + 1][2 * e + 1]);
-                        }
-                    } else {  // accumulator 4 c + x: columns 4 n + x of 32
-                        if (d % 4 == 0) {
-                            put(8 * d + 8 * t4, o[d][2 * e], o[d + 1][2 * e]);
-                            put(8 * d + 8 * t4 + 2, o[d + 2][2 * e], o[d + 3][2 * e]);
-                            put(8 * d + 8 * t4 + 4, o[d][2 * e + 1], o[d + 1][2 * e + 1]);
-                            put(8 * d + 8 * t4 + 6, o[d + 2][2 * e + 1], o[d + 3][2 * e + 1]);
+                for (int e = 0; e < 2; ++e) {
+                    const int r = (wr * NT + nt) * 8 + 2 * t4 + e;
+                    float *const to = joint + (wk * R + r) * DC;
+                    const float f = mine_f[nt][e];
+#pragma unroll
+                    for (int d = col0 / 16; d < (col0 + DC) / 16; ++d) {
+                        if constexpr (BITS == 16) {
+                            to[(16 * d - col0 + g) ^ (t4 << 3)] = o[d][nt][e] * f;
+                            to[(16 * d - col0 + g + 8) ^ (t4 << 3)] = o[d][nt][2 + e] * f;
+                        } else if constexpr (BITS == 8) {
+                            *reinterpret_cast<float2 *>(to + ((16 * d - col0 + 2 * g) ^ (t4 << 3))) = make_float2(o[d][nt][e] * f, o[d][nt][2 + e] * f);
+                        } else if (d % 2 == 0) {
+                            *reinterpret_cast<float4 *>(to + ((16 * d - col0 + 4 * g) ^ (t4 << 3))) =
+                                make_float4(o[d][nt][e] * f, o[d][nt][2 + e] * f, o[d + 1][nt][e] * f, o[d + 1][nt][2 + e] * f);
                         }
                     }
                 }
-            }
             __syncthreads();
             for (int x = tid; x < rows * (DC / 4); x += kThreads) {
                 const int r = x / (DC / 4), c4 = x % (DC / 4);
-                const float *const from = joint + r * DC + 2 * ((2 * c4) ^ ((r & kTurn) << 2));
+                const float *const from = joint + r * DC + ((4 * c4) ^ ((r >> 1 & 3) << 3));
                 float4 v = *reinterpret_cast<const float4 *>(from);
                 const float top_r = top_of(r);
                 float sum_r = row_sum[r] * factor(0, r, top_r);
@@ -763,7 +925,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             // the CTAs that share the segment are those whose runs hold its units; the first one's number is the counter's
             auto cta_of = [&](int64_t u) { return ((u + 1) * ctas + total - 1) / total - 1; };
             const int64_t c0 = cta_of(seg0), c1 = cta_of(seg1 - 1);
-            auto *const last = reinterpret_cast<int *>(scan);
+            auto *const last = reinterpret_cast<int *>(scan + kWarps);
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -805,43 +967,49 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     }
 }
 
-// The form for the rows that a key head's queries make: more query heads a key head or more drafts, more rows a tile.
-inline int row_warps(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+// The rows of a tile for those that a key head's queries make: more query heads a key head or more drafts, more rows.
+inline int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+// The counters' place is every form's: calls of different ones share a workspace.
+inline size_t counter_bytes() { return ((size_t)sm_count() * kMostPerSm * 4 + 255) / 256 * 256; }
 
 template <class S> struct Launch {
+    static_assert(S::kPerSm <= kMostPerSm, "");
+
     static int64_t ctas() { return (int64_t)sm_count() * S::kPerSm; }
-    static size_t bytes() { return (size_t)((ctas() * 4 + 255) / 256 * 256 + ctas() * 2 * S::R * (S::D + 2) * 4); }
+    static size_t bytes() { return counter_bytes() + (size_t)(ctas() * 2 * S::R * (S::D + 2) * 4); }
     static cudaError_t run(Args a, void *ws, int64_t most_units, cudaStream_t st) {
         const int64_t n = std::max<int64_t>(1, std::min(ctas(), (most_units + kMinRun - 1) / kMinRun));
         a.count = static_cast<uint32_t *>(ws);
-        a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + (ctas() * 4 + 255) / 256 * 256);
+        a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + counter_bytes());
         const cudaError_t rc = cudaFuncSetAttribute(attn_decode_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
         if (rc != cudaSuccess) return rc;
         return launch_behind(attn_decode_kernel<S>, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a);
     }
 };
 
-// f(Shape) for the sizes of a call; -1 where there is none.
-template <int D, int BITS, int G, class F> auto with_rows(int wr, F f) {
-    if (wr == 1) return f(Shape<D, BITS, G, 1>{});
-    if (wr == 2) return f(Shape<D, BITS, G, 2>{});
-    return f(Shape<D, BITS, G, 4>{});
+// f(Shape) for the sizes of a call.
+template <int D, int BITS, int G, class F> auto with_rows(int rows, F f) {
+    if (rows == 8) return f(Shape<D, BITS, G, 8>{});
+    if (rows == 16) return f(Shape<D, BITS, G, 16>{});
+    if (rows == 32) return f(Shape<D, BITS, G, 32>{});
+    return f(Shape<D, BITS, G, 64>{});
 }
-template <int D, class F> auto with_cache(int bits, int64_t G, int wr, F f) {
-    if (bits == 16) return with_rows<D, 16, D>(wr, f);
+template <int D, class F> auto with_cache(int bits, int64_t G, int rows, F f) {
+    if (bits == 16) return with_rows<D, 16, D>(rows, f);
     if (bits == 8) {
-        if (G == 32) return with_rows<D, 8, 32>(wr, f);
-        if (G == 64) return with_rows<D, 8, 64>(wr, f);
-        return with_rows<D, 8, D < 128 ? D : 128>(wr, f);
+        if (G == 32) return with_rows<D, 8, 32>(rows, f);
+        if (G == 64) return with_rows<D, 8, 64>(rows, f);
+        return with_rows<D, 8, D < 128 ? D : 128>(rows, f);
     }
-    if (G == 32) return with_rows<D, 4, 32>(wr, f);
-    if (G == 64) return with_rows<D, 4, 64>(wr, f);
-    return with_rows<D, 4, D < 128 ? D : 128>(wr, f);
+    if (G == 32) return with_rows<D, 4, 32>(rows, f);
+    if (G == 64) return with_rows<D, 4, 64>(rows, f);
+    return with_rows<D, 4, D < 128 ? D : 128>(rows, f);
 }
-template <class F> auto with_shape(int64_t D, int bits, int64_t G, int wr, F f) {
-    if (D == 64) return with_cache<64>(bits, G, wr, f);
-    if (D == 128) return with_cache<128>(bits, G, wr, f);
-    return with_cache<256>(bits, G, wr, f);
+template <class F> auto with_shape(int64_t D, int bits, int64_t G, int rows, F f) {
+    if (D == 64) return with_cache<64>(bits, G, rows, f);
+    if (D == 128) return with_cache<128>(bits, G, rows, f);
+    return with_cache<256>(bits, G, rows, f);
 }
 
 }  // namespace
@@ -857,7 +1025,10 @@ extern "C" size_t sxb_attn_decode_workspace_bytes(int64_t n_q, int64_t n_kv, int
                    cat(fn, ": n_q = ", n_q, ", n_kv = ", n_kv, ", D = ", D, ", bits = ", bits, ", max_q = ", max_q, " unsupported"));
         return 0;
     }
-    return with_shape(D, bits, 32, row_warps(max_q * (n_q / n_kv)), [](auto s) { return Launch<decltype(s)>::bytes(); });
+    size_t most = 0;  // of a call with fewer rows too
+    for (int rows = 8; rows <= tile_rows(max_q * (n_q / n_kv)); rows *= 2)
+        most = std::max(most, with_shape(D, bits, 32, rows, [](auto s) { return Launch<decltype(s)>::bytes(); }));
+    return most;
 }
 
 extern "C" int sxb_attn_decode(const void *q, int64_t q_ld, int64_t T, int64_t n_q, const SxbKvCache *cache, const int32_t *pages, int64_t pages_ld,
@@ -883,14 +1054,14 @@ extern "C" int sxb_attn_decode(const void *q, int64_t q_ld, int64_t T, int64_t n
     SXB_CHECK(scale > -1e30f && scale < 1e30f, fn, ": scale must be finite");
     SXB_CHECK(softcap >= 0.f && softcap < 1e30f, fn, ": softcap must be finite and not negative (0: none)");
     SXB_CHECK(window >= 0 && window < (1ll << 31), fn, ": window = ", window, ", expected 0 (none) .. 2^31 - 1");
-    const int wr = row_warps(max_q * (n_q / n_kv));
+    const int rows = tile_rows(max_q * (n_q / n_kv));
     const size_t need = sxb_attn_decode_workspace_bytes(n_q, n_kv, D, cache->bits, max_q);
     SXB_CHECK(ws_bytes >= need, fn, ": workspace of ", ws_bytes, " bytes, needs ", need);
     a.q = static_cast<const uint16_t *>(q), a.q_ld = q_ld, a.pages = pages, a.pages_ld = pages_ld, a.capacity = n_cols * cache->page;
     a.q_start = q_start, a.kv_len = kv_len, a.B = (int)B, a.T = (int)T, a.n_q = (int)n_q, a.group = (int)(n_q / n_kv), a.window = (int)window;
     a.scale = scale, a.softcap = softcap, a.out = static_cast<uint16_t *>(out), a.out_ld = out_ld, a.lse = lse, a.err = err;
     auto st = static_cast<cudaStream_t>(stream);
-    const cudaError_t rc = with_shape(D, cache->bits, cache->G, wr, [&](auto s) {
+    const cudaError_t rc = with_shape(D, cache->bits, cache->G, rows, [&](auto s) {
         using S = decltype(s);
         // no list is longer than every sequence at its table's end (in a product that cannot overflow: the grid is a few hundred CTAs)
         const double most = (double)((a.capacity + S::TK - 1) / S::TK) * (double)B * n_kv * (double)((T * a.group + S::R - 1) / S::R + 1);

@@ -282,6 +282,19 @@ def test_attend_captured_and_replayed_with_other_lengths(cuda):
             b.check()
 
 
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_attend_calls_of_every_form_share_a_workspace(cuda, bits, G):
+    """A workspace made for many rows serves calls of few, in any order: each finds its counters at zero."""
+    ws = None
+    for turn, new in enumerate((8, 1, 4, 2, 1, 8, 2, 4)):
+        b = Batch(cuda, 128, bits, G, 1, 8, [5000, 900], [new, 1], page=64, seed=20 + turn)
+        if ws is None:
+            ws = b.ws
+        b.ws = ws
+        b.run()
+        b.check()
+
+
 def test_attend_on_another_stream(cuda):
     b = Batch(cuda, 128, 16, 0, 2, 4, [3000], [1], seed=16)
     side = torch.cuda.Stream()
