@@ -25,30 +25,33 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMinRun = 2;     // units a CTA takes at least
-constexpr int kMaxIds = 32;    // a warp finds a tile's pages: at most 16 of 128 keys
 constexpr int kMostPerSm = 4;
 constexpr int kSlack = 8;      // powers of two that a weight may be above 1
-constexpr int64_t kNoPage = INT64_MIN;
+constexpr float kLowest = -1e30f;  // below every score; a row that sees no key keeps it
 constexpr int64_t kMaxRows = 1ll << 24;
 
-// R query rows: NT tiles of eight a warp, WR warps side by side; the other warps share a tile's keys, KI runs of sixteen each.
+#ifndef SXB_KI
+#define SXB_KI(D, BITS, NT) ((D) == 64 || ((BITS) == 4 && (D) == 128) ? 2 : 1)
+#endif
+// R query rows: NT tiles of eight a warp, WR warps side by side.  The WK groups of such warps share a tile's keys, a run of KI times sixteen each, and
+// every group fetches its own run into its own ring: nothing but a segment's ends is the whole CTA's business.
 template <int D_, int BITS_, int G_, int R_> struct Shape {
     static constexpr int D = D_, BITS = BITS_, G = G_, R = R_;
-    static constexpr int kMostNT = D == 256 ? 2 : 4, NT = R / 8 < kMostNT ? R / 8 : kMostNT, WR = R / 8 / NT;
     static constexpr bool kQuant = BITS != 16;
-    static constexpr int kWarps = WR > 1 || (kQuant && NT == 1 && D <= 128) ? 8 : 4, kThreads = 32 * kWarps, WK = kWarps / WR;
+    static constexpr int kMostNT = D == 256 ? 2 : 4, NT = R / 8 < kMostNT ? R / 8 : kMostNT, WR = R / 8 / NT;
+    static constexpr int kWarps = WR > 1 ? 8 : 4, kThreads = 32 * kWarps, WK = kWarps / WR;
     static constexpr int RB = D * BITS / 8, CR = RB / 16;  // bytes and 16-byte chunks of a cache row
     static constexpr int NG = kQuant ? D / G : 0;
-    static constexpr int TK = D == 64 || (BITS == 4 && D == 128) || (kQuant && kWarps == 8 && D == 128) ? 128 : 64;
-    static constexpr int KI = TK / (16 * WK);
-    static constexpr int kRows = TK * RB, kScales = TK * NG * 4, kStage = 2 * (kRows + kScales);
+    static constexpr int KI = SXB_KI(D, BITS, NT), RUN = 16 * KI, TK = RUN * WK;
+    static constexpr int kRows = RUN * RB, kScales = RUN * NG * 4, kPart = 2 * (kRows + kScales), kStage = WK * kPart;
     static constexpr int kQ = R * D * 2;
     static constexpr int kMostJoint = WK * R * 32 * 4;
     static constexpr bool kOwnJoint = kStage < kMostJoint;  // 32 columns of every warp's rows do not fit a stage
-    static constexpr int kMisc = 1280 + WK * R * 8 + R * (NG + 2) * 4 + (kOwnJoint ? kMostJoint : 0);
-    static constexpr int kPerSm = D <= 128 && (kWarps == 4 || NT == 1) ? 2 : 1;
-    static constexpr int kBudget = 226 * 1024 / kPerSm;
-    static constexpr int kFit = (kBudget - kMisc) / (kStage + kQ), kStages = kFit > 5 ? 5 : kFit;
+    static constexpr int kMisc = 1024 + WK * R * 8 + R * (NG + 2) * 4 + (kOwnJoint ? kMostJoint : 0);
+    static constexpr int kByRegisters = WR > 1 ? 1 : D * NT <= 128 ? 3 : 2;
+    static constexpr int stages(int per_sm) { return (226 * 1024 / per_sm - kMisc) / (kStage + kQ); }
+    static constexpr int kPerSm = kByRegisters > 3 && stages(4) >= 3 ? 4 : kByRegisters > 2 && stages(3) >= 3 ? 3 : kByRegisters > 1 && stages(2) >= 3 ? 2 : 1;
+    static constexpr int kStages = stages(kPerSm) > 6 ? 6 : stages(kPerSm);
     static constexpr int kSmem = kStages * (kStage + kQ) + kMisc;
     static constexpr int fit_columns() {
         int dc = D;
@@ -58,9 +61,9 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     static constexpr int DC = fit_columns();  // columns that the warps join at a time
     // Codes stay 1024 (8 bits) or 64 (4 bits) too large as F16 operands, and what that adds is taken out of the sums
     static constexpr float kOffset = BITS == 8 ? 1024.f : 64.f;
-    static constexpr bool kOffsetV = kQuant && NG * NT <= 8;  // for V it takes four accumulators a group and row tile
+    static constexpr bool kOffsetV = kQuant && NG * NT <= 4;  // for V it takes four accumulators a group and row tile
     static constexpr bool kHoldQ = NT * D <= 256;             // q's fragments in registers
-    static_assert(kStages >= 2 && KI >= 1 && kThreads % CR == 0 && WK * WR == kWarps, "");
+    static_assert(kStages >= 2 && WK * WR == kWarps && KI * NT * 4 <= 32, "");
 };
 
 struct Args {
@@ -169,9 +172,10 @@ template <class S> __device__ inline int k_chunk_at(int r, int c) {
 
 template <class S>
 __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(const __grid_constant__ Args a) {
-    constexpr int D = S::D, BITS = S::BITS, NG = S::NG, TK = S::TK, KI = S::KI, R = S::R, WK = S::WK, CR = S::CR, NT = S::NT, kStages = S::kStages;
+    constexpr int D = S::D, BITS = S::BITS, NG = S::NG, TK = S::TK, KI = S::KI, RUN = S::RUN, R = S::R, WK = S::WK, WR = S::WR, CR = S::CR, NT = S::NT;
+    constexpr int kStages = S::kStages, kThreads = S::kThreads, kWarps = S::kWarps;
     constexpr bool kQuant = S::kQuant;
-    constexpr int kThreads = S::kThreads, kWarps = S::kWarps, kGroups = kQuant ? NG : 1;
+    constexpr int kGroups = kQuant ? NG : 1;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *const q_ring = smem + kStages * S::kStage;
     uint8_t *const own_joint = q_ring + kStages * S::kQ, *const misc = own_joint + (S::kOwnJoint ? S::kMostJoint : 0);
@@ -179,11 +183,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     float *const row_sum = row_max + WK * R;                // [WK][R]
     float *const q_factor = row_sum + WK * R;               // [R]
     float *const q_sums = q_factor + R;                     // [NG][R]
-    auto *const places = reinterpret_cast<int64_t *>(q_sums + R * (NG + (NG & 1)));  // [2][kMaxIds]: row numbers of the tile's pages' first tokens
-    auto *const scan = places + 2 * kMaxIds;                                         // [kWarps + 2]
-    auto *const segments = reinterpret_cast<Segment *>(scan + kWarps + 2);           // [kStages]
+    auto *const scan = reinterpret_cast<int64_t *>(q_sums + R * (NG + (NG & 1)));  // [kWarps + 2]
+    auto *const segments = reinterpret_cast<Segment *>(scan + kWarps + 2);         // [kStages]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int wr = warp % S::WR, wk = warp / S::WR;
+    const int wr = warp % WR, wk = warp / WR;
 
     behind_grid();
 
@@ -248,27 +251,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         l_row_tile = (int)(rest / l_s.tiles), l_at = (int)(rest % l_s.tiles);
     }
     const int units = (int)(u1 - u0);
-    const int page_mask = (1 << a.c.page_shift) - 1;
+    const int shift = a.c.page_shift, page_mask = (1 << shift) - 1;
+    const int run_pages = RUN > page_mask ? RUN >> shift : 1;  // pages of a run of keys: one, or two or four that end inside it
 
-    // row number of the first token of the page number tid of the tile under the cursor; kNoPage where the sequence has none there or a bad one
-    auto find_page = [&]() -> int64_t {
-        const int first = (l_s.tile0 + l_at) * TK, col = (first >> a.c.page_shift) + tid;
-        const int end = min(l_s.len, first + TK);
-        if (((int64_t)col << a.c.page_shift) >= end || (((int64_t)col + 1) << a.c.page_shift) <= l_s.lo) return kNoPage;
-        const int id = a.pages[l_b * a.pages_ld + col];
-        if ((unsigned)id < (unsigned)a.c.n_pages) return id * a.c.page_stride + l_head * a.c.head_stride;
-        raise_error(a.err, (uint32_t)l_b, (uint32_t)id);
-        return kNoPage;
-    };
-    // Lanes 0 .. kMaxIds - 1 of the first warp find them for the cursor's tile, and whether the tile is whole: every row there.
-    auto put_pages = [&](int which, int64_t place) {
-        if (tid < kMaxIds) {
-            places[which * kMaxIds + tid] = place;
-            const int first = (l_s.tile0 + l_at) * TK;
-            const int pages = max(1, TK >> a.c.page_shift);
-            const bool fine = __all_sync(0xffffffffu, tid >= pages || place != kNoPage) && first >= l_s.lo && first + TK <= l_s.len;
-            if (tid == 0) scan[which] = fine;
-        }
+    // The id of page number lane % run_pages of the run under the cursor; none where the sequence has no keys there or the table's entry is bad.
+    auto find_page = [&]() -> int {
+        const int run0 = (l_s.tile0 + l_at) * TK + wk * RUN, col = (run0 >> shift) + (lane & (run_pages - 1));
+        if (((int64_t)col << shift) >= l_s.len || (((int64_t)col + 1) << shift) <= l_s.lo) return -1;
+        return a.pages[l_b * a.pages_ld + col];
     };
     auto advance = [&]() {
         l_new = false;
@@ -283,70 +273,66 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             l_s = sequence<S>(a, l_b);
         } while (l_s.n == 0);
     };
-    constexpr int kPass = kThreads / CR, kPasses = TK / kPass;  // rows that the CTA's threads fetch at a time
-    static_assert(TK % kPass == 0, "");
-    const int l_chunk = tid % CR, l_row = tid / CR;
-    auto load = [&](int stage, int which) {
-        uint8_t *const st = smem + stage * S::kStage;
-        const int64_t *const place = places + which * kMaxIds;
-        const int first = (l_s.tile0 + l_at) * TK;
-        constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = kQuant ? NG * 4 / kBytes : 1;
-        if (scan[which] != 0) {
-            const bool one_page = TK <= page_mask + 1;
-            const int base = first & page_mask;
-            const int64_t row_bytes = a.c.row_stride * S::RB;
-            if (one_page) {
-                const int64_t off = (place[0] + (base + l_row) * a.c.row_stride) * S::RB + l_chunk * 16;
+    constexpr int kPass = 32 * WR / CR > RUN ? RUN : 32 * WR / CR, kPasses = RUN / kPass;  // rows that the group's threads fetch at a time
+    const int l_lane = wr * 32 + lane, l_chunk = l_lane % CR, l_row = l_lane / CR;
+    const bool l_on = l_row < kPass;
+    auto load = [&](int stage, int page) {
+        uint8_t *const st = smem + stage * S::kStage + wk * S::kPart;
+        const int run0 = (l_s.tile0 + l_at) * TK + wk * RUN;
+        constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = kQuant ? NG * 4 / kBytes : 1;  // of a row's scales
+        const bool fine = (unsigned)page < (unsigned)a.c.n_pages;
+        if (__all_sync(0xffffffffu, fine) && run0 >= l_s.lo && run0 + RUN <= l_s.len) {
+            if (run_pages == 1) {
+                const int64_t row0 = page * a.c.page_stride + l_head * a.c.head_stride + (run0 & page_mask) * a.c.row_stride;
+                const int64_t off = (row0 + l_row * a.c.row_stride) * S::RB + l_chunk * 16, step = kPass * S::RB * a.c.row_stride;
                 const uint8_t *k = a.c.k + off, *v = a.c.v + off;
 #pragma unroll
                 for (int i = 0; i < kPasses; ++i) {
-                    copy_async<16>(smem_of(st + k_chunk_at<S>(l_row + i * kPass, l_chunk) * 16), k, 16);
-                    copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(l_row + i * kPass, l_chunk) * 16), v, 16);
-                    k += kPass * row_bytes, v += kPass * row_bytes;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
-                    const int r = l_row + i * kPass;
-                    const int64_t off = (place[r >> a.c.page_shift] + (r & page_mask) * a.c.row_stride) * S::RB + l_chunk * 16;
-                    copy_async<16>(smem_of(st + k_chunk_at<S>(r, l_chunk) * 16), a.c.k + off, 16);
-                    copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(r, l_chunk) * 16), a.c.v + off, 16);
-                }
-            }
-            if constexpr (kQuant) {
-                uint8_t *const sc = st + 2 * S::kRows;
-#pragma unroll
-                for (int i0 = 0; i0 < TK * kPieces; i0 += kThreads) {
-                    const int i = i0 + tid, r = i / kPieces;
-                    if (TK * kPieces % kThreads == 0 || i < TK * kPieces) {
-                        const int64_t off = (place[one_page ? 0 : r >> a.c.page_shift] + ((base + r) & page_mask) * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes;
-                        copy_async<kBytes>(smem_of(sc + i * kBytes), reinterpret_cast<const uint8_t *>(a.c.k_sm) + off, kBytes);
-                        copy_async<kBytes>(smem_of(sc + S::kScales + i * kBytes), reinterpret_cast<const uint8_t *>(a.c.v_sm) + off, kBytes);
+                    if (kPass * CR == 32 * WR || l_on) {
+                        copy_async<16>(smem_of(st + k_chunk_at<S>(l_row + i * kPass, l_chunk) * 16), k, 16);
+                        copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(l_row + i * kPass, l_chunk) * 16), v, 16);
+                        k += step, v += step;
                     }
                 }
+                if constexpr (kQuant) {
+#pragma unroll
+                    for (int i0 = 0; i0 < RUN * kPieces; i0 += 32 * WR) {
+                        const int i = i0 + l_lane, r = i / kPieces;
+                        if (RUN * kPieces % (32 * WR) == 0 || i < RUN * kPieces) {
+                            const int64_t at = (row0 + r * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes;
+                            uint8_t *const to = st + 2 * S::kRows + i * kBytes;
+                            copy_async<kBytes>(smem_of(to), reinterpret_cast<const uint8_t *>(a.c.k_sm) + at, kBytes);
+                            copy_async<kBytes>(smem_of(to + S::kScales), reinterpret_cast<const uint8_t *>(a.c.v_sm) + at, kBytes);
+                        }
+                    }
+                }
+                return;
             }
-        } else {  // a sequence's first or last tile, or one with a bad page: rows out of range are zeros, keys of a bad page NaN
-            const int col0 = first >> a.c.page_shift;
+        }
+        // Several pages, or a sequence's first or last run, or a bad page: rows out of range are zeros, keys of a bad page NaN.
+        if (lane < run_pages && page != -1 && !fine) raise_error(a.err, (uint32_t)l_b, (uint32_t)page);
 #pragma unroll 1
-            for (int r = l_row; r < TK; r += kPass) {
-                const int j = first + r;
-                const int64_t page = place[(j >> a.c.page_shift) - col0];
-                const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && page != kNoPage;
-                const int64_t off = there ? (page + (j & page_mask) * a.c.row_stride) * S::RB + l_chunk * 16 : 0;
+        for (int i = 0; i < kPasses; ++i) {
+            const int r = l_row + i * kPass, j = run0 + r;
+            const int id = __shfl_sync(0xffffffffu, page, (r >> shift) & (run_pages - 1));
+            const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && (unsigned)id < (unsigned)a.c.n_pages;
+            const int64_t off = there ? (id * a.c.page_stride + l_head * a.c.head_stride + (j & page_mask) * a.c.row_stride) * S::RB + l_chunk * 16 : 0;
+            if (l_on) {
                 uint8_t *const to = st + k_chunk_at<S>(r, l_chunk) * 16;
                 if (!kQuant && wanted && !there) *reinterpret_cast<uint4 *>(to) = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
                 else copy_async<16>(smem_of(to), a.c.k + off, there ? 16 : 0);
                 copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(r, l_chunk) * 16), a.c.v + off, there ? 16 : 0);
             }
-            if constexpr (kQuant) {
-                uint8_t *const sc = st + 2 * S::kRows;
+        }
+        if constexpr (kQuant) {
 #pragma unroll 1
-                for (int i = tid; i < TK * kPieces; i += kThreads) {
-                    const int r = i / kPieces, j = first + r;
-                    const int64_t page = place[(j >> a.c.page_shift) - col0];
-                    const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && page != kNoPage;
-                    const int64_t off = there ? (page + (j & page_mask) * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes : 0;
-                    uint8_t *const to = sc + i * kBytes;
+            for (int i0 = 0; i0 < RUN * kPieces; i0 += 32 * WR) {
+                const int i = i0 + l_lane, r = i / kPieces, j = run0 + r;
+                const int id = __shfl_sync(0xffffffffu, page, (r >> shift) & (run_pages - 1));
+                const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && (unsigned)id < (unsigned)a.c.n_pages;
+                const int64_t off = there ? (id * a.c.page_stride + l_head * a.c.head_stride + (j & page_mask) * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes : 0;
+                if (i < RUN * kPieces) {
+                    uint8_t *const to = st + 2 * S::kRows + i * kBytes;
                     if (wanted && !there) {
 #pragma unroll
                         for (int w = 0; w < kBytes / 4; ++w) reinterpret_cast<uint32_t *>(to)[w] = 0x7fc07fc0u;
@@ -357,31 +343,31 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 }
             }
         }
-        if (l_new) {
-            const int slot = l_segment % kStages, rows0 = l_row_tile * R;
-            uint8_t *const qs = q_ring + slot * S::kQ;
-            for (int i = tid; i < R * (D / 8); i += kThreads) {
-                const int r = i / (D / 8), c = i % (D / 8), row = rows0 + r, tok = row / a.group;
-                const bool there = tok < l_s.n;
-                const int64_t off = there ? (l_s.q0 + tok) * a.q_ld + (int64_t)(l_head * a.group + row - tok * a.group) * D + c * 8 : 0;
-                copy_async<16>(smem_of(qs + chunk_at<D / 8>(r, c) * 16), a.q + off, there ? 16 : 0);
-            }
-            if (tid == 0)
-                segments[slot] = Segment{l_s.q0, l_s.n, l_s.len, l_s.p0, l_s.tile0, l_s.tiles, l_head, rows0, l_at, (int)l_s.bad};
+    };
+    // A segment's queries and what there is to know of it: the whole CTA's, into a ring of as many places as there are stages.
+    auto load_segment = [&]() {
+        const int slot = l_segment % kStages, rows0 = l_row_tile * R;
+        uint8_t *const qs = q_ring + slot * S::kQ;
+#pragma unroll 1
+        for (int i = tid; i < R * (D / 8); i += kThreads) {
+            const int r = i / (D / 8), c = i % (D / 8), row = rows0 + r, tok = row / a.group;
+            const bool there = tok < l_s.n;
+            const int64_t off = there ? (l_s.q0 + tok) * a.q_ld + (int64_t)(l_head * a.group + row - tok * a.group) * D + c * 8 : 0;
+            copy_async<16>(smem_of(qs + chunk_at<D / 8>(r, c) * 16), a.q + off, there ? 16 : 0);
         }
+        if (tid == 0) segments[slot] = Segment{l_s.q0, l_s.n, l_s.len, l_s.p0, l_s.tile0, l_s.tiles, l_head, rows0, l_at, (int)l_s.bad};
     };
 
-    __syncthreads();  // scan is read
-    put_pages(0, tid < kMaxIds ? find_page() : kNoPage);
-    __syncthreads();
+    int l_page = find_page();
+#pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) {
         if (s < units) {
-            load(s, s & 1);
+            if (l_new) load_segment();
+            load(s, l_page);
             if (s + 1 < units) {
                 advance();
-                put_pages((s + 1) & 1, tid < kMaxIds ? find_page() : kNoPage);
+                l_page = find_page();
             }
-            __syncthreads();
         }
         commit_async();
     }
@@ -391,50 +377,48 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     // second product V's columns are the rows, its accumulators hold the same two queries, and the weights get from the first one's layout to the
     // second operand's by a transposition in registers.
     const int g = lane >> 2, t4 = lane & 3;
+    const int a_row = lane & 15, a_half = lane >> 4;  // of a fragment of sixteen rows, two chunks
     uint32_t qf[S::kHoldQ ? NT : 1][S::kHoldQ ? D / 16 : 1][2];
     float o[D / 16][NT][4], w_sum[S::kOffsetV ? NG : 1][NT][4], o_min[kGroups][NT][2];
-    float m[NT][2], l[NT][2], fac[NT][2];
-    int hi[NT][2], lo[NT][2], v_exp = 20;
-    Segment sg{};
-    int at = 0, segment = 0;
+    float m[NT][2], l[NT][2];
+    int v_exp = 20, at = 0, tiles = 0, whole0 = 0, whole1 = 0, segment = 0, stage = 0;
     bool fresh = true;
-    const int a_row = lane & 15, a_half = lane >> 4;  // of a fragment of sixteen rows, two chunks
 
+#pragma unroll 1
     for (int i = 0; i < units; ++i) {
         wait_async<kStages - 2>();
-        __syncthreads();
-        const int ahead = i + kStages - 1;
-        int64_t next_place = kNoPage;
-        if (ahead < units) {
-            load(ahead % kStages, ahead & 1);
-            if (ahead + 1 < units) {
+        if constexpr (WR == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + wk), "n"(32 * WR) : "memory");
+        if (i + kStages - 1 < units) {
+            if (l_new) load_segment();
+            load(stage == 0 ? kStages - 1 : stage - 1, l_page);
+            if (i + kStages < units) {
                 advance();
-                if (tid < kMaxIds) next_place = find_page();
+                l_page = find_page();
             }
         }
         commit_async();
 
-        uint8_t *const st = smem + (i % kStages) * S::kStage;
+        uint8_t *const st = smem + stage * S::kStage + wk * S::kPart;
         uint8_t *const qs = q_ring + (segment % kStages) * S::kQ;
+        const Segment &sg = segments[segment % kStages];
         if (fresh) {
             fresh = false;
-            sg = segments[segment % kStages];
-            at = sg.at, v_exp = 20;
+            __syncthreads();
+            at = sg.at, tiles = sg.tiles, v_exp = 20;
+            {   // tiles that every row sees all of
+                const int p_last = sg.p0 + sg.n - 1, from = a.window > 0 ? max(0, p_last - a.window + 1) : 0;
+                whole0 = (from + TK - 1) / TK - sg.tile0, whole1 = (sg.p0 + 1 + TK) / TK - 1 - sg.tile0;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                m[nt][0] = m[nt][1] = -CUDART_INF_F, l[nt][0] = l[nt][1] = 0.f;
+                m[nt][0] = m[nt][1] = kLowest, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
 #pragma unroll
                 for (int e = 0; e < kGroups; ++e) o_min[e][nt][0] = o_min[e][nt][1] = 0.f;
 #pragma unroll
                 for (int e = 0; e < (S::kOffsetV ? NG : 1); ++e) w_sum[e][nt][0] = w_sum[e][nt][1] = w_sum[e][nt][2] = w_sum[e][nt][3] = 0.f;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int tok = (sg.rows0 + (wr * NT + nt) * 8 + 2 * t4 + e) / a.group;
-                    hi[nt][e] = tok < sg.n ? sg.p0 + tok : -1;
-                    lo[nt][e] = a.window > 0 ? max(-1, hi[nt][e] - a.window) : -1;
-                }
             }
             if constexpr (kQuant) {
                 // q to F16 times a power of two, elements in the order that the codes come in, and each group's sum of what they then are
@@ -461,7 +445,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 for (int off = 1; off < kPer; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
                 const int up = min(126, 14 - ((int)(__float_as_uint(most) >> 23) - 127));
                 const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-                if (part == 0) q_factor[r] = __uint_as_float((uint32_t)(127 - up) << 23);
+                if (part == 0) q_factor[r] = a.scale * (a.softcap > 0.f ? 1.f : kLog2e) * __uint_as_float((uint32_t)(127 - up) << 23);
                 float sums[kOwn];
 #pragma unroll
                 for (int b = 0; b < kOwn; ++b) {
@@ -489,11 +473,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     if (blk < kBlocks && blk % kRuns == 0) q_sums[blk / kRuns * R + r] = sums[b];
                 }
                 __syncthreads();
+            } else {
+                if (tid < R) q_factor[tid] = a.scale * (a.softcap > 0.f ? 1.f : kLog2e);
+                __syncthreads();
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) fac[nt][e] = a.scale * (a.softcap > 0.f ? 1.f : kLog2e) * (kQuant ? q_factor[(wr * NT + nt) * 8 + 2 * t4 + e] : 1.f);
             if constexpr (S::kHoldQ) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -512,12 +495,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         };
 
         // scores
-        const int first = (sg.tile0 + at) * TK;
         float s[KI][NT][4];
-        const auto *const k_sm = reinterpret_cast<const uint32_t *>(st + 2 * S::kRows), *const v_sm = k_sm + TK * NG;
+        const auto *const k_sm = reinterpret_cast<const uint32_t *>(st + 2 * S::kRows), *const v_sm = k_sm + RUN * NG;
 #pragma unroll
         for (int ki = 0; ki < KI; ++ki) {
-            const int key0 = (wk * KI + ki) * 16;
+            const int key0 = ki * 16;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[ki][nt][0] = s[ki][nt][1] = s[ki][nt][2] = s[ki][nt][3] = 0.f;
             if constexpr (!kQuant) {
@@ -570,25 +552,21 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        const float2 qsum = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
+                        const float2 q_sum = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(sc[e >> 1], part[nt][e], fmaf(mn[e >> 1], e & 1 ? qsum.y : qsum.x, s[ki][nt][e]));
+                        for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(sc[e >> 1], part[nt][e], fmaf(mn[e >> 1], e & 1 ? q_sum.y : q_sum.x, s[ki][nt][e]));
                     }
                 }
             }
         }
-        const int p_last = sg.p0 + sg.n - 1;
-        const bool whole = first >= (a.window > 0 ? p_last - a.window + 1 : 0) && first + TK - 1 <= sg.p0;
-        auto seen = [&](int ki, int nt, int e) {  // e: as in an accumulator
-            const int j = first + (wk * KI + ki) * 16 + g + 8 * (e >> 1);
-            return j <= hi[nt][e & 1] && j > lo[nt][e & 1];
-        };
 #pragma unroll
-        for (int ki = 0; ki < KI; ++ki)
+        for (int nt = 0; nt < NT; ++nt) {
+            const float2 f = *reinterpret_cast<const float2 *>(q_factor + (wr * NT + nt) * 8 + 2 * t4);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[ki][nt][e] *= fac[nt][e & 1];
+                for (int e = 0; e < 4; ++e) s[ki][nt][e] *= e & 1 ? f.y : f.x;
+        }
         if (a.softcap > 0.f) {
             const float by = 1.f / a.softcap, to = a.softcap * kLog2e;
 #pragma unroll
@@ -598,14 +576,27 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[ki][nt][e] = to * tanhf(s[ki][nt][e] * by);
         }
+        const bool whole = at >= whole0 && at < whole1;
+        uint32_t hidden = 0;  // bit (ki * NT + nt) * 4 + e: that query does not see that key
         if (!whole) {
+            const int j0 = (sg.tile0 + at) * TK + wk * RUN + g;
 #pragma unroll
-            for (int ki = 0; ki < KI; ++ki)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int e = 0; e < 2; ++e) {
+                    const int tok = (sg.rows0 + (wr * NT + nt) * 8 + 2 * t4 + e) / a.group;
+                    const int hi = tok < sg.n ? sg.p0 + tok : -1, lo = a.window > 0 ? max(-1, hi - a.window) : -1;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!seen(ki, nt, e)) s[ki][nt][e] = -CUDART_INF_F;
+                    for (int ki = 0; ki < KI; ++ki)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int j = j0 + ki * 16 + 8 * x;
+                            if (j > hi || j <= lo) {
+                                s[ki][nt][2 * x + e] = -CUDART_INF_F;
+                                hidden |= 1u << ((ki * NT + nt) * 4 + 2 * x + e);
+                            }
+                        }
+                }
         }
         // The maximum that the weights are relative to is moved when a score passes it by 2^kSlack only: most tiles then need no exchange between lanes and
         // no sum is touched.  The scale that the weights of quantized values are relative to, likewise.
@@ -621,14 +612,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 top[nt][e] = v;
                 move = move || v > m[nt][e] + kSlack;
             }
-        float v_top = 0.f;
         if constexpr (kQuant) {
+            float v_top = 0.f;
 #pragma unroll
             for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) v_top = fmaxf(v_top, __uint_as_float(v_sm[((wk * KI + ki) * 16 + g + 8 * e) * NG + grp] << 16 & 0x7fffffffu));
+                    for (int grp = 0; grp < NG; ++grp) v_top = fmaxf(v_top, fabsf(__uint_as_float(v_sm[(ki * 16 + g + 8 * e) * NG + grp] << 16)));
             move = move || (__float_as_uint(v_top) >> 23) > (uint32_t)v_exp;
         }
         if (__any_sync(0xffffffffu, move)) {
@@ -641,7 +632,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
                     const float now = fmaxf(m[nt][e], v);
-                    f[nt][e] = exp2_fast(m[nt][e] - (now == -CUDART_INF_F ? 0.f : now));
+                    f[nt][e] = exp2_fast(m[nt][e] - now);
                     m[nt][e] = now, l[nt][e] *= f[nt][e];
 #pragma unroll
                     for (int grp = 0; grp < kGroups; ++grp) o_min[grp][nt][e] *= f[nt][e];
@@ -654,7 +645,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
                         for (int grp = 0; grp < NG; ++grp) {
-                            const int x = (int)(v_sm[((wk * KI + ki) * 16 + g + 8 * e) * NG + grp] >> 7 & 0xffu);
+                            const int x = (int)(v_sm[(ki * 16 + g + 8 * e) * NG + grp] >> 7 & 0xffu);
                             if (x != 255) ex = max(ex, x);  // a scale that is none says nothing of the others
                         }
                 ex = max(v_exp, __reduce_max_sync(0xffffffffu, ex));
@@ -676,23 +667,21 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const float base[2] = {m[nt][0] == -CUDART_INF_F ? 0.f : m[nt][0], m[nt][1] == -CUDART_INF_F ? 0.f : m[nt][1]};
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[ki][nt][e] = exp2_fast(s[ki][nt][e] - base[e & 1]);
+                    s[ki][nt][e] = exp2_fast(s[ki][nt][e] - m[nt][e & 1]);
                     l[nt][e & 1] += s[ki][nt][e];
                 }
-        }
 
         // weights times values
         const uint8_t *const vt = st + S::kRows;
         if constexpr (!kQuant) {
 #pragma unroll
             for (int ki = 0; ki < KI; ++ki) {
-                const int key0 = (wk * KI + ki) * 16;
+                const int key0 = ki * 16;
                 // Keys that one row sees and another does not: an infinity or a NaN there must not reach the other through 0 * v.
                 bool clean = true;
                 if (!whole && sg.n > 1) {
@@ -721,7 +710,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 } else {
 #pragma unroll 1
                     for (int k = 0; k < 16; ++k) {
-                        const int from = (k % 8) * 4 + t4, j = first + key0 + k;
+                        const int from = (k % 8) * 4 + t4;
+                        const uint32_t out_of_sight = __shfl_sync(0xffffffffu, hidden, from) >> (ki * NT * 4 + (k < 8 ? 0 : 2));
                         float w[NT][2];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
@@ -739,7 +729,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                                     for (int e = 0; e < 2; ++e)
-                                        if (j <= hi[nt][e] && j > lo[nt][e]) o[d][nt][2 * half + e] = fmaf(w[nt][e], v, o[d][nt][2 * half + e]);
+                                        if ((out_of_sight >> (nt * 4 + e) & 1) == 0) o[d][nt][2 * half + e] = fmaf(w[nt][e], v, o[d][nt][2 * half + e]);
                             }
                         }
                     }
@@ -749,7 +739,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             const float v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);  // 2^(14 - kSlack - (v_exp - 127))
 #pragma unroll
             for (int ki = 0; ki < KI; ++ki) {
-                const int key0 = (wk * KI + ki) * 16;
+                const int key0 = ki * 16;
 #pragma unroll
                 for (int grp = 0; grp < NG; ++grp) {
                     float sc[2], mn[2];
@@ -762,7 +752,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float w[4];
-                        if (whole) {
+                        if (hidden == 0) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 w[e] = s[ki][nt][e] * sc[e >> 1];
@@ -772,7 +762,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 w[e] = 0.f;
-                                if (seen(ki, nt, e)) {
+                                if ((hidden >> ((ki * NT + nt) * 4 + e) & 1) == 0) {
                                     w[e] = s[ki][nt][e] * sc[e >> 1];
                                     o_min[grp][nt][e & 1] = fmaf(s[ki][nt][e], mn[e >> 1], o_min[grp][nt][e & 1]);
                                 }
@@ -814,12 +804,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 }
             }
         }
-        if (ahead + 1 < units) put_pages((ahead + 1) & 1, next_place);
-
-        if (++at < sg.tiles && i + 1 < units) continue;
+        uint8_t *const stage_base = smem + stage * S::kStage;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        if (++at < tiles && i + 1 < units) continue;
 
         // ---- the segment's end, or this CTA's share's: the warps' sums become one ----
-        const int64_t seg0 = u0 + (i + 1) - at, seg1 = seg0 + sg.tiles;  // the segment's units in the list
+        const int64_t seg0 = u0 + (i + 1) - at, seg1 = seg0 + tiles;  // the segment's units in the list
         const bool split = seg0 < u0 || seg1 > u1;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -852,7 +842,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     }
         }
         __syncthreads();
-        auto factor = [&](int k, int r, float top_of) { return row_max[k * R + r] == -CUDART_INF_F ? 1.f : exp2_fast(row_max[k * R + r] - top_of); };
+        auto factor = [&](int k, int r, float of) { return exp2_fast(row_max[k * R + r] - of); };
         auto top_of = [&](int r) {
             float v = row_max[r];
 #pragma unroll
@@ -868,7 +858,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 mine_f[nt][e] = factor(wk, r, top_of(r));
             }
         constexpr int DC = S::DC;
-        auto *const joint = reinterpret_cast<float *>(S::kOwnJoint ? own_joint : st);  // [WK][R][DC], runs of eight columns turned by the row
+        auto *const joint = reinterpret_cast<float *>(S::kOwnJoint ? own_joint : stage_base);  // [WK][R][DC], runs of eight columns turned by the row
         float *const part = a.partial + (2 * (int64_t)blockIdx.x + (seg0 < u0 ? 0 : 1)) * R * (D + 2);
         const int rows = min(R, sg.n * a.group - sg.rows0);
 #pragma unroll
@@ -949,7 +939,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll 4
                     for (int k = -1; k < more; ++k) {
                         const float *const p = k < 0 ? p0 : p1 + k * step;
-                        const float top_k = __ldcg(p + R * D + r), f = top_k == -CUDART_INF_F ? 1.f : exp2_fast(top_k - top_r);
+                        const float top_k = __ldcg(p + R * D + r), f = exp2_fast(top_k - top_r);
                         const float4 w = __ldcg(reinterpret_cast<const float4 *>(p + r * D + 4 * c4));
                         sum_r = fmaf(__ldcg(p + R * (D + 1) + r), f, sum_r);
                         v.x = fmaf(w.x, f, v.x), v.y = fmaf(w.y, f, v.y), v.z = fmaf(w.z, f, v.z), v.w = fmaf(w.w, f, v.w);
@@ -963,6 +953,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 }
             }
         }
+        __syncthreads();  // the joint's place is the next loads'
         fresh = true, ++segment;
     }
 }
