@@ -531,7 +531,7 @@ typedef struct SxbKvCache {
  * position pos[t] of sequence seq[t]: rounded once to BF16, or quantized from the FP32 values as sxb_quantize does (a group that
  * holds a NaN or an infinity reads back as NaN).  seq[t] < 0: a padding row, nothing of it is written.  A position or page out of
  * range: err = {1, token, pos}, the token's queries NaN, nothing written to the cache.  No (seq, pos) twice in one call.
- * Rows of qkv and q_out 16-byte aligned. */
+ * Rows of qkv and q_out and the norm weights 16-byte aligned. */
 int sxb_attn_qkv_write(const void *qkv, int64_t ld, int act, int64_t T, int64_t n_q, const float *q_norm, const float *k_norm,
                        float eps, const float *inv_freq, int64_t rot, int interleaved, const int32_t *seq, const int32_t *pos,
                        const int32_t *pages, int64_t pages_ld, int64_t n_cols, int64_t n_seq, const SxbKvCache *cache, void *q_out,

@@ -66,7 +66,7 @@ template <typename T, int N> __device__ inline void load_run(const T *p, float (
 template <int N> __device__ inline void store_bf16_run(uint16_t *p, const float (&v)[N]) {
     Words<2 * N> r;
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) r.w[i] = (uint32_t)f32_to_bf16_bits(v[2 * i]) | (uint32_t)f32_to_bf16_bits(v[2 * i + 1]) << 16;
+    for (int i = 0; i < N / 2; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r.w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
     store_words<2 * N>(p, r);
 }
 
@@ -147,6 +147,17 @@ __global__ void __launch_bounds__(kWriteThreads) qkv_write_kernel(const __grid_c
     __syncthreads();
     const int heads = a.n_q + 2 * a.n_kv, first = blockIdx.y * a.heads_per_cta, last = min(heads, first + a.heads_per_cta);
     if (place.state == 2 && threadIdx.x == 0 && first == 0) raise_error(a.err, (uint32_t)t, (uint32_t)pos);
+    // What a lane's elements are turned by is the same in every head: element i becomes x_i co_i + partner si_i, elements behind rot keep themselves.
+    float co[N], si[N];
+    const bool turned = lane * N < a.rot, low = lane * N < half;
+    const int partner = turned && !a.interleaved ? (low ? lane + half / N : lane - half / N) : lane;  // half is a multiple of 8 >= N
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = lane * N + i;
+        const float2 cs = turned ? turn[a.interleaved ? e / 2 : low ? e : e - half] : make_float2(1.f, 0.f);
+        co[i] = cs.x, si[i] = (a.interleaved ? i % 2 == 0 : low) ? -cs.y : cs.y;
+    }
+#pragma unroll 2
     for (int h = first + warp; h < last; h += kWriteWarps) {
         const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
         float v[N];
@@ -154,39 +165,22 @@ __global__ void __launch_bounds__(kWriteThreads) qkv_write_kernel(const __grid_c
         if (is_q || is_k) {
             const float *w = is_q ? a.q_norm : a.k_norm;
             if (w != nullptr) {
-                float sum = 0.f;
+                float sum = 0.f, by[N];
+                load_run<float, N>(w + lane * N, by);
 #pragma unroll
                 for (int i = 0; i < N; ++i) sum = fmaf(v[i], v[i], sum);
 #pragma unroll
                 for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                const float inv = 1.0f / sqrtf(sum * (1.0f / D) + a.eps);
+                const float inv = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[i] = v[i] * inv * w[lane * N + i];
+                for (int i = 0; i < N; ++i) v[i] = v[i] * inv * by[i];
             }
             if (a.rot != 0) {
-                const bool turned = lane * N < a.rot;
-                if (a.interleaved) {
-                    if (turned) {
+                float other[N];
 #pragma unroll
-                        for (int i = 0; i < N; i += 2) {
-                            const float2 cs = turn[(lane * N + i) / 2];
-                            const float x = v[i], y = v[i + 1];
-                            v[i] = x * cs.x - y * cs.y, v[i + 1] = y * cs.x + x * cs.y;
-                        }
-                    }
-                } else {
-                    const int off = half / N;  // lanes to the partner: half is a multiple of 8 >= N
-                    const bool low = lane < off;
-                    const int from = turned ? (low ? lane + off : lane - off) : lane;
+                for (int i = 0; i < N; ++i) other[i] = a.interleaved ? v[i ^ 1] : __shfl_sync(0xffffffffu, v[i], partner);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        const float other = __shfl_sync(0xffffffffu, v[i], from);
-                        if (turned) {
-                            const float2 cs = turn[low ? lane * N + i : lane * N + i - half];
-                            v[i] = low ? v[i] * cs.x - other * cs.y : v[i] * cs.x + other * cs.y;
-                        }
-                    }
-                }
+                for (int i = 0; i < N; ++i) v[i] = fmaf(v[i], co[i], other[i] * si[i]);
             }
         }
         if (is_q) {
@@ -202,35 +196,49 @@ __global__ void __launch_bounds__(kWriteThreads) qkv_write_kernel(const __grid_c
     }
 }
 
+constexpr int kReadThreads = 256, kReadTokens = 32;
+
 struct ReadArgs {
     const int32_t *seq, *pos, *pages;
-    int64_t pages_ld, items;
-    int n_seq, n_cols, G;
+    int64_t pages_ld;
+    int T, n_seq, n_cols, G, per_token, tokens;  // runs of eight elements a token has; tokens a CTA
     KvView c;
     void *k_out, *v_out;
     uint32_t *err;
 };
 
-// Eight elements a thread: neighbouring threads have neighbouring runs of a row.
+// The CTA's threads find the places of its tokens side by side, then read runs of eight elements: neighbouring threads neighbouring runs of a row, with
+// nothing between one load and the next.
 template <typename T, int D, int BITS>
-__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ ReadArgs a) {
+__global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_constant__ ReadArgs a) {
+    __shared__ int64_t rows[kReadTokens];  // row number of the token's first head; kSkip, kBad
+    constexpr int64_t kSkip = -1, kBad = -2;
     behind_grid();
     constexpr int kRuns = D / 8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.items; i += (int64_t)gridDim.x * 256) {
-        const int run = (int)(i % kRuns);
-        const int64_t row = i / kRuns, t = row / (2 * a.c.n_kv);
-        const int h = (int)(row - t * 2 * a.c.n_kv);
+    const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
+    const int tokens = (int)min((int64_t)a.tokens, a.T - t0);
+    if ((int)threadIdx.x < tokens) {
+        const int64_t t = t0 + threadIdx.x;
+        const int pos = a.pos[t];
+        const Place place = find_place(a.seq[t], pos, a.pages, a.pages_ld, a.n_seq, a.n_cols, a.c);
+        if (place.state == 2) raise_error(a.err, (uint32_t)t, (uint32_t)pos);
+        rows[threadIdx.x] = place.state == 0 ? kv_row(a.c, place.page, 0, place.at) : place.state == 1 ? kSkip : kBad;
+    }
+    __syncthreads();
+    const int items = tokens * a.per_token;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < items; i += kReadThreads) {
+        const int token = i / a.per_token, in = i - token * a.per_token, run = in % kRuns, h = in / kRuns;
+        const int64_t row0 = rows[token];
+        if (row0 == kSkip) continue;
         const bool is_k = h < a.c.n_kv;
         const int head = is_k ? h : h - a.c.n_kv;
-        const Place place = find_place(a.seq[t], a.pos[t], a.pages, a.pages_ld, a.n_seq, a.n_cols, a.c);
-        if (place.state == 1) continue;
         float v[8];
-        if (place.state == 2) {
-            if (h == 0 && run == 0) raise_error(a.err, (uint32_t)t, (uint32_t)a.pos[t]);
+        if (row0 == kBad) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = qnan_f32();
         } else {
-            const int64_t from = kv_row(a.c, place.page, head, place.at);
+            const int64_t from = row0 + head * a.c.head_stride;
             const uint8_t *p = (is_k ? a.c.k : a.c.v) + from * (D * BITS / 8) + run * BITS;
             if constexpr (BITS == 16) {
                 load_run(reinterpret_cast<const uint16_t *>(p), v);
@@ -239,10 +247,13 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ Re
                 const uint32_t sm = (is_k ? a.c.k_sm : a.c.v_sm)[from * (D / a.G) + run * 8 / a.G];
                 const float s = __uint_as_float(sm << 16), m = __uint_as_float(sm & 0xffff0000u);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = fmaf((float)((w.w[e * BITS / 32] >> (e * BITS % 32)) & ((1u << BITS) - 1)), s, m);
+                for (int e = 0; e < 8; ++e) {  // a code under the exponent of 2^23 is that number plus it
+                    const uint32_t c = BITS == 8 ? __byte_perm(w.w[e / 4], 0x4b000000u, 0x7540 + e % 4) : (w.w[0] >> (4 * e) & 15u) | 0x4b000000u;
+                    v[e] = fmaf(__uint_as_float(c) - 8388608.f, s, m);
+                }
             }
         }
-        T *to = static_cast<T *>(is_k ? a.k_out : a.v_out) + ((t * a.c.n_kv + head) * D + run * 8);
+        T *to = static_cast<T *>(is_k ? a.k_out : a.v_out) + (((t0 + token) * a.c.n_kv + head) * D + run * 8);
         if constexpr (sizeof(T) == 4) {
             reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
             reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -265,7 +276,7 @@ cudaError_t launch_write(const WriteArgs &a, int D, int bits, dim3 grid, cudaStr
 template <typename T>
 cudaError_t launch_read(const ReadArgs &a, int D, int bits, unsigned grid, cudaStream_t st) {
 #define SXB_R(DD, BB) \
-    if (D == DD && bits == BB) return launch_behind(kv_read_kernel<T, DD, BB>, grid, 256, 0, st, 1, a)
+    if (D == DD && bits == BB) return launch_behind(kv_read_kernel<T, DD, BB>, grid, kReadThreads, 0, st, 1, a)
     SXB_R(64, 16); SXB_R(64, 8); SXB_R(64, 4);
     SXB_R(128, 16); SXB_R(128, 8); SXB_R(128, 4);
     SXB_R(256, 16); SXB_R(256, 8); SXB_R(256, 4);
@@ -301,8 +312,8 @@ int kv_view(const char *fn, const SxbKvCache *c, KvView *out) {
     SXB_CHECK(c->n_kv >= 1 && c->n_kv <= 1024, fn, ": n_kv = ", c->n_kv, " heads, expected 1..1024");
     SXB_CHECK(is_pow2(c->page) && c->page >= 8 && c->page <= 4096, fn, ": pages of ", c->page, " tokens, expected a power of two of 8..4096");
     SXB_CHECK(c->page_stride >= 1 && c->head_stride >= 1 && c->row_stride >= 1 && c->page_stride < (1ll << 32) && c->head_stride < (1ll << 32) &&
-                  c->row_stride < (1ll << 32),
-              fn, ": strides of ", c->page_stride, " / ", c->head_stride, " / ", c->row_stride, " rows (page / head / token), expected 1..2^32 - 1");
+                  c->row_stride <= (1ll << 22),
+              fn, ": strides of ", c->page_stride, " / ", c->head_stride, " / ", c->row_stride, " rows (page / head / token), expected 1..2^32 - 1, of tokens up to 2^22");
     *out = KvView{static_cast<uint8_t *>(c->k), static_cast<uint8_t *>(c->v), c->k_sm, c->v_sm, c->page_stride, c->head_stride, c->row_stride,
                   (int)c->n_pages, __builtin_ctzll((unsigned long long)c->page), (int)c->n_kv};
     return SXB_OK;
@@ -330,6 +341,7 @@ extern "C" int sxb_attn_qkv_write(const void *qkv, int64_t ld, int act, int64_t 
     SXB_CHECK(apart(qkv, ((T - 1) * ld + heads * D) * es, q_out, ((T - 1) * q_ld + n_q * D) * 2), fn, ": q_out [", q_out, "] overlaps qkv [", qkv, "]");
     SXB_CHECK(inv_freq != nullptr || rot == 0, fn, ": rot = ", rot, " without inv_freq");
     SXB_CHECK(rot >= 0 && rot <= D && rot % 16 == 0, fn, ": rot = ", rot, ", expected a multiple of 16 of 0..", D);
+    SXB_CHECK(aligned16(q_norm) && aligned16(k_norm), fn, ": norm weights must be 16-byte aligned");
     SXB_CHECK((q_norm == nullptr && k_norm == nullptr) || (eps > 0.f && eps < 1e30f), fn, ": eps must be finite and positive");
     a.qkv = qkv, a.ld = ld, a.n_q = (int)n_q, a.n_kv = (int)cache->n_kv, a.rot = (int)rot, a.interleaved = interleaved != 0;
     a.q_norm = q_norm, a.k_norm = k_norm, a.inv_freq = inv_freq, a.eps = eps;
@@ -360,8 +372,9 @@ extern "C" int sxb_kv_read(const SxbKvCache *cache, const int32_t *seq, const in
     SXB_CHECK(apart(k_out, bytes, v_out, bytes), fn, ": v_out [", v_out, "] overlaps k_out [", k_out, "]");
     a.seq = seq, a.pos = pos, a.pages = pages, a.pages_ld = pages_ld, a.n_seq = (int)n_seq, a.n_cols = (int)n_cols;
     a.G = (int)(cache->bits == 16 ? D : cache->G), a.k_out = k_out, a.v_out = v_out, a.err = err;
-    a.items = T * 2 * cache->n_kv * (D / 8);
-    const unsigned grid = (unsigned)std::min<int64_t>((a.items + 255) / 256, (int64_t)sm_count() * 32);
+    a.T = (int)T, a.per_token = (int)(2 * cache->n_kv * (D / 8));
+    a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(kReadTokens, T / (8 * (int64_t)sm_count())));
+    const unsigned grid = (unsigned)((T + a.tokens - 1) / a.tokens);
     auto st = static_cast<cudaStream_t>(stream);
     if (out_act == SXB_ACT_F32) launch_read<float>(a, (int)D, cache->bits, grid, st);
     else launch_read<uint16_t>(a, (int)D, cache->bits, grid, st);

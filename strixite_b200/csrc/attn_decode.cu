@@ -16,7 +16,6 @@
 //   two that follows the largest scale seen so that F16's range is no limit (one rounding of 2^-11); the mins' share, sum p * min, is FP32.
 
 #include "attn.cuh"
-#include "skinny_mma.cuh"
 
 #include <math_constants.h>
 
@@ -62,6 +61,9 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     // Codes stay 1024 (8 bits) or 64 (4 bits) too large as F16 operands, and what that adds is taken out of the sums
     static constexpr float kOffset = BITS == 8 ? 1024.f : 64.f;
     static constexpr bool kOffsetV = kQuant && NG * NT <= 4;  // for V it takes four accumulators a group and row tile
+    // Few rows: the last CTA to bring its part joins them, a launch less.  Many: that CTA would read every part by itself (2 x 8 rows over 32 k keys:
+    // 19 parts of 33 KB, 30 us at the end of 80), a second kernel has the rows of all segments side by side.
+    static constexpr bool kJoinHere = R <= 16;
     static constexpr bool kHoldQ = NT * D <= 256;             // q's fragments in registers
     static_assert(kStages >= 2 && WK * WR == kWarps && KI * NT * 4 <= 32, "");
 };
@@ -78,6 +80,12 @@ struct Args {
     int64_t out_ld;
     float *lse, *partial;
     uint32_t *count, *err;
+    struct Join *joins;
+};
+
+// A split segment whose first part is the CTA's of the same number; parts = 0: that CTA began none.
+struct Join {
+    int q0, rows0, head, rows, parts, unused[3];
 };
 
 // What a sequence asks for.
@@ -109,28 +117,56 @@ struct Segment {
 };
 
 __device__ inline uint32_t smem_of(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-template <int BYTES> __device__ inline void copy_async(uint32_t to, const void *from, int n) {
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
-    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+// n bytes (0: zeros instead), to a place OFF bytes behind `to`.
+template <int BYTES, int OFF = 0> __device__ inline void copy_async(uint32_t to, const void *from, int n) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0 + %3], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n), "n"(OFF) : "memory");
+    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0 + %3], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(n), "n"(OFF) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0 + %3], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(n), "n"(OFF) : "memory");
+}
+template <int BYTES, int OFF = 0> __device__ inline void copy_async(uint32_t to, const void *from) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(to), "l"(from), "n"(OFF) : "memory");
+    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0 + %2], [%1], 8;" ::"r"(to), "l"(from), "n"(OFF) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0 + %2], [%1], 4;" ::"r"(to), "l"(from), "n"(OFF) : "memory");
 }
 __device__ inline void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ inline void wait_async() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Volatile: they stay behind the wait that they follow; nothing is written that the compiler knows of.
 __device__ inline void load_matrices(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 __device__ inline void load_matrices_trans(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
-__device__ inline void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ inline void load_matrices_trans(uint32_t (&r)[2], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at));
+}
+template <bool F16> __device__ inline void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// A row's words of scales.
+template <int N> __device__ inline void load_scales(uint32_t (&w)[N], const uint32_t *p) {
+    if constexpr (N == 1) w[0] = p[0];
+    else if constexpr (N == 2) *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(p);
+    else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) reinterpret_cast<uint4 *>(w)[i] = reinterpret_cast<const uint4 *>(p)[i];
+    }
 }
 __device__ inline float exp2_fast(float v) {  // 2 ulp; exp2(-inf) = 0
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ inline float reciprocal_fast(float v) {  // 1 ulp
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
 __device__ inline uint32_t pack_bf16(float lo, float hi) {
@@ -170,6 +206,68 @@ template <class S> __device__ inline int k_chunk_at(int r, int c) {
     else return chunk_at<S::CR>(r, c);
 }
 
+// BF16 NaN throughout.
+template <int BYTES> __device__ inline void store_nan(uint32_t to) {
+    for (int i = 0; i < BYTES; i += 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + i), "r"(0x7fc07fc0u) : "memory");
+}
+// Passes I .. N - 1 of PASS rows each of a run, K and V.  A place in pass i is the first one's with the turn of its rows, and a constant: a tile starts
+// at a multiple of 128 bytes, and where rows are shorter than that a pass is whole turns.
+template <class S, int PASS, int I, int N>
+__device__ inline void copy_rows(uint32_t k_to, uint32_t v_to, const uint8_t *k, const uint8_t *v, uint64_t step) {
+    static_assert((S::CR >= 8 || PASS % 8 == 0) && S::kPart % 128 == 0 && S::kRows % 128 == 0, "");
+    if constexpr (I < N) {
+        constexpr int kTurn = S::CR >= 8 ? I * PASS & 7 : 0, kTurnK = S::BITS == 8 ? 2 * (kTurn & 3) : kTurn;
+        copy_async<16, I * PASS * S::RB>(k_to ^ (kTurnK << 4), k);
+        copy_async<16, I * PASS * S::RB>(v_to ^ (kTurn << 4), v);
+        copy_rows<S, PASS, I + 1, N>(k_to, v_to, k + step, v + step, step);
+    }
+}
+
+// The parts of a split segment, [R][D] sums, [R] maxima, [R] sums of weights each: the first CTA's is its second one, the others' their first.
+template <int R, int D> struct Parts {
+    static constexpr int64_t kStep = 2 * (int64_t)R * (D + 2);
+    const float *first, *rest;
+    int n;
+    __device__ Parts(const float *partial, int c0, int parts) : first(partial + (2 * (int64_t)c0 + 1) * R * (D + 2)), rest(partial + 2 * (int64_t)c0 * R * (D + 2)), n(parts) {}
+    __device__ const float *of(int k) const { return k == 0 ? first : rest + k * kStep; }
+    __device__ float top(int k, int r) const { return __ldcg(of(k) + R * D + r); }
+};
+
+// Four columns of a row out of all parts, in the parts' order.
+template <int R, int D> __device__ inline void join_run(const Args &a, const Parts<R, D> &from, int q0, int rows0, int key_head, int r, int c4, float top) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < from.n; ++k) {
+        const float *const p = from.of(k);
+        const float4 w = __ldcg(reinterpret_cast<const float4 *>(p + r * D + 4 * c4));
+        const float f = exp2_fast(__ldcg(p + R * D + r) - top);
+        sum = fmaf(__ldcg(p + R * (D + 1) + r), f, sum);
+        v.x = fmaf(w.x, f, v.x), v.y = fmaf(w.y, f, v.y), v.z = fmaf(w.z, f, v.z), v.w = fmaf(w.w, f, v.w);
+    }
+    const int tok = (rows0 + r) / a.group, head = key_head * a.group + rows0 + r - tok * a.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint2 w;
+    w.x = pack_bf16(v.x * inv, v.y * inv), w.y = pack_bf16(v.z * inv, v.w * inv);
+    *reinterpret_cast<uint2 *>(a.out + (q0 + tok) * a.out_ld + (int64_t)head * D + 4 * c4) = w;
+    if (a.lse != nullptr && c4 == 0) a.lse[(int64_t)(q0 + tok) * a.n_q + head] = sum == 0.f ? -CUDART_INF_F : fmaf(top, kLn2, logf(sum));
+}
+
+constexpr int kJoinRows = 4;
+// Block (c, y): rows 4 y .. 4 y + 3 of the segment that began in CTA c, a thread four columns.
+template <class S>
+__global__ void __launch_bounds__(kJoinRows * S::D / 4) attn_join_kernel(const __grid_constant__ Args a) {
+    behind_grid();
+    const Join j = a.joins[blockIdx.x];
+    const int r = blockIdx.y * kJoinRows + threadIdx.x / (S::D / 4);
+    if (r >= j.rows || j.parts == 0) return;
+    const Parts<S::R, S::D> from(a.partial, (int)blockIdx.x, j.parts);
+    float top = kLowest;
+#pragma unroll 8
+    for (int k = 0; k < from.n; ++k) top = fmaxf(top, from.top(k, r));
+    join_run(a, from, j.q0, j.rows0, j.head, r, threadIdx.x % (S::D / 4), top);
+}
+
 template <class S>
 __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(const __grid_constant__ Args a) {
     constexpr int D = S::D, BITS = S::BITS, NG = S::NG, TK = S::TK, KI = S::KI, RUN = S::RUN, R = S::R, WK = S::WK, WR = S::WR, CR = S::CR, NT = S::NT;
@@ -197,6 +295,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         if (s.bad && blockIdx.x == 0) raise_error(a.err, (uint32_t)b, (uint32_t)a.kv_len[b]);
         total += (int64_t)s.tiles * s.row_tiles * a.c.n_kv;
     }
+    if (!S::kJoinHere && tid == 0) a.joins[blockIdx.x].parts = 0;
     const int64_t mine = total;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
@@ -254,11 +353,28 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     const int shift = a.c.page_shift, page_mask = (1 << shift) - 1;
     const int run_pages = RUN > page_mask ? RUN >> shift : 1;  // pages of a run of keys: one, or two or four that end inside it
 
-    // The id of page number lane % run_pages of the run under the cursor; none where the sequence has no keys there or the table's entry is bad.
+    constexpr int kPass = 32 * WR / CR > RUN ? RUN : 32 * WR / CR, kPasses = RUN / kPass;  // rows that the group's threads fetch at a time
+    constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = kQuant ? NG * 4 / kBytes : 1;  // of a row's scales
+    constexpr int kScalePass = 32 * WR / kPieces > RUN ? RUN : 32 * WR / kPieces, kScalePasses = RUN / kScalePass;
+    const int l_lane = wr * 32 + lane, l_chunk = l_lane % CR, l_row = l_lane / CR, s_row = l_lane / kPieces, s_piece = l_lane % kPieces;
+    const bool l_on = l_row < kPass, s_on = s_row < kScalePass;
+    const uint32_t stages0 = smem_of(smem) + wk * S::kPart;
+    const uint32_t row_bytes = (uint32_t)a.c.row_stride * S::RB, row_words = (uint32_t)a.c.row_stride * (NG * 4);
+    const uint64_t page_bytes = (uint64_t)a.c.page_stride * S::RB, page_words = (uint64_t)a.c.page_stride * (NG * 4);
+    const int64_t k_to_v = a.c.v - a.c.k, ks_to_vs = kQuant ? reinterpret_cast<const uint8_t *>(a.c.v_sm) - reinterpret_cast<const uint8_t *>(a.c.k_sm) : 0;
+    // this lane's place in the head's first row, of the codes and of the scales; the sequence's row of the table
+    const uint8_t *l_codes, *l_scales = nullptr;
+    const int32_t *l_table;
+    auto at_head = [&]() {
+        const int64_t rows = l_head * a.c.head_stride;
+        l_codes = a.c.k + (rows + l_row * a.c.row_stride) * S::RB + l_chunk * 16;
+        if constexpr (kQuant) l_scales = reinterpret_cast<const uint8_t *>(a.c.k_sm) + (rows + s_row * a.c.row_stride) * (NG * 4) + s_piece * kBytes;
+    };
+    // The id of page number lane % run_pages of the run under the cursor; none where the sequence has no keys there.
     auto find_page = [&]() -> int {
-        const int run0 = (l_s.tile0 + l_at) * TK + wk * RUN, col = (run0 >> shift) + (lane & (run_pages - 1));
-        if (((int64_t)col << shift) >= l_s.len || (((int64_t)col + 1) << shift) <= l_s.lo) return -1;
-        return a.pages[l_b * a.pages_ld + col];
+        const int run0 = (l_s.tile0 + l_at) * TK + wk * RUN, first = (run0 & ~page_mask) + ((lane & (run_pages - 1)) << shift);
+        if (first >= l_s.len || (first | page_mask) < l_s.lo) return -1;
+        return l_table[first >> shift];
     };
     auto advance = [&]() {
         l_new = false;
@@ -266,48 +382,39 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         l_at = 0, l_new = true, ++l_segment;
         if (++l_row_tile < l_s.row_tiles) return;
         l_row_tile = 0;
-        if (++l_head < a.c.n_kv) return;
-        l_head = 0;
-        do {
-            if (++l_b >= a.B) return;
-            l_s = sequence<S>(a, l_b);
-        } while (l_s.n == 0);
+        if (++l_head == a.c.n_kv) {
+            l_head = 0;
+            do {
+                if (++l_b >= a.B) return;
+                l_s = sequence<S>(a, l_b);
+            } while (l_s.n == 0);
+            l_table = a.pages + l_b * a.pages_ld;
+        }
+        at_head();
     };
-    constexpr int kPass = 32 * WR / CR > RUN ? RUN : 32 * WR / CR, kPasses = RUN / kPass;  // rows that the group's threads fetch at a time
-    const int l_lane = wr * 32 + lane, l_chunk = l_lane % CR, l_row = l_lane / CR;
-    const bool l_on = l_row < kPass;
     auto load = [&](int stage, int page) {
-        uint8_t *const st = smem + stage * S::kStage + wk * S::kPart;
+        const uint32_t st = stages0 + stage * S::kStage;
         const int run0 = (l_s.tile0 + l_at) * TK + wk * RUN;
-        constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = kQuant ? NG * 4 / kBytes : 1;  // of a row's scales
         const bool fine = (unsigned)page < (unsigned)a.c.n_pages;
-        if (__all_sync(0xffffffffu, fine) && run0 >= l_s.lo && run0 + RUN <= l_s.len) {
-            if (run_pages == 1) {
-                const int64_t row0 = page * a.c.page_stride + l_head * a.c.head_stride + (run0 & page_mask) * a.c.row_stride;
-                const int64_t off = (row0 + l_row * a.c.row_stride) * S::RB + l_chunk * 16, step = kPass * S::RB * a.c.row_stride;
-                const uint8_t *k = a.c.k + off, *v = a.c.v + off;
+        if (run_pages == 1 && __all_sync(0xffffffffu, fine) && run0 >= l_s.lo && run0 + RUN <= l_s.len) {
+            const uint32_t in_page = run0 & page_mask;
+            const uint8_t *k = l_codes + (uint64_t)(uint32_t)page * page_bytes + (uint64_t)in_page * row_bytes, *v = k + k_to_v;
+            const uint64_t step = (uint64_t)kPass * row_bytes;
+            if (kPass * CR == 32 * WR || l_on)
+                copy_rows<S, kPass, 0, kPasses>(st + k_chunk_at<S>(l_row, l_chunk) * 16, st + S::kRows + chunk_at<CR>(l_row, l_chunk) * 16, k, v, step);
+            if constexpr (kQuant) {
+                const uint8_t *ks = l_scales + (uint64_t)(uint32_t)page * page_words + (uint64_t)in_page * row_words;
+                const uint32_t to = st + 2 * S::kRows + l_lane * kBytes;
 #pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
-                    if (kPass * CR == 32 * WR || l_on) {
-                        copy_async<16>(smem_of(st + k_chunk_at<S>(l_row + i * kPass, l_chunk) * 16), k, 16);
-                        copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(l_row + i * kPass, l_chunk) * 16), v, 16);
-                        k += step, v += step;
+                for (int i = 0; i < kScalePasses; ++i) {
+                    if (kScalePass * kPieces == 32 * WR || s_on) {
+                        copy_async<kBytes>(to + i * kScalePass * NG * 4, ks);
+                        copy_async<kBytes>(to + S::kScales + i * kScalePass * NG * 4, ks + ks_to_vs);
                     }
+                    ks += (uint64_t)kScalePass * row_words;
                 }
-                if constexpr (kQuant) {
-#pragma unroll
-                    for (int i0 = 0; i0 < RUN * kPieces; i0 += 32 * WR) {
-                        const int i = i0 + l_lane, r = i / kPieces;
-                        if (RUN * kPieces % (32 * WR) == 0 || i < RUN * kPieces) {
-                            const int64_t at = (row0 + r * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes;
-                            uint8_t *const to = st + 2 * S::kRows + i * kBytes;
-                            copy_async<kBytes>(smem_of(to), reinterpret_cast<const uint8_t *>(a.c.k_sm) + at, kBytes);
-                            copy_async<kBytes>(smem_of(to + S::kScales), reinterpret_cast<const uint8_t *>(a.c.v_sm) + at, kBytes);
-                        }
-                    }
-                }
-                return;
             }
+            return;
         }
         // Several pages, or a sequence's first or last run, or a bad page: rows out of range are zeros, keys of a bad page NaN.
         if (lane < run_pages && page != -1 && !fine) raise_error(a.err, (uint32_t)l_b, (uint32_t)page);
@@ -318,28 +425,24 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && (unsigned)id < (unsigned)a.c.n_pages;
             const int64_t off = there ? (id * a.c.page_stride + l_head * a.c.head_stride + (j & page_mask) * a.c.row_stride) * S::RB + l_chunk * 16 : 0;
             if (l_on) {
-                uint8_t *const to = st + k_chunk_at<S>(r, l_chunk) * 16;
-                if (!kQuant && wanted && !there) *reinterpret_cast<uint4 *>(to) = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
-                else copy_async<16>(smem_of(to), a.c.k + off, there ? 16 : 0);
-                copy_async<16>(smem_of(st + S::kRows + chunk_at<CR>(r, l_chunk) * 16), a.c.v + off, there ? 16 : 0);
+                const uint32_t to = st + k_chunk_at<S>(r, l_chunk) * 16;
+                if (!kQuant && wanted && !there) store_nan<16>(to);
+                else copy_async<16>(to, a.c.k + off, there ? 16 : 0);
+                copy_async<16>(st + S::kRows + chunk_at<CR>(r, l_chunk) * 16, a.c.v + off, there ? 16 : 0);
             }
         }
         if constexpr (kQuant) {
 #pragma unroll 1
-            for (int i0 = 0; i0 < RUN * kPieces; i0 += 32 * WR) {
-                const int i = i0 + l_lane, r = i / kPieces, j = run0 + r;
+            for (int i = 0; i < kScalePasses; ++i) {
+                const int r = s_row + i * kScalePass, j = run0 + r;
                 const int id = __shfl_sync(0xffffffffu, page, (r >> shift) & (run_pages - 1));
                 const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && (unsigned)id < (unsigned)a.c.n_pages;
-                const int64_t off = there ? (id * a.c.page_stride + l_head * a.c.head_stride + (j & page_mask) * a.c.row_stride) * (NG * 4) + (i % kPieces) * kBytes : 0;
-                if (i < RUN * kPieces) {
-                    uint8_t *const to = st + 2 * S::kRows + i * kBytes;
-                    if (wanted && !there) {
-#pragma unroll
-                        for (int w = 0; w < kBytes / 4; ++w) reinterpret_cast<uint32_t *>(to)[w] = 0x7fc07fc0u;
-                    } else {
-                        copy_async<kBytes>(smem_of(to), reinterpret_cast<const uint8_t *>(a.c.k_sm) + off, there ? kBytes : 0);
-                    }
-                    copy_async<kBytes>(smem_of(to + S::kScales), reinterpret_cast<const uint8_t *>(a.c.v_sm) + off, there ? kBytes : 0);
+                const int64_t off = there ? (id * a.c.page_stride + l_head * a.c.head_stride + (j & page_mask) * a.c.row_stride) * (NG * 4) + s_piece * kBytes : 0;
+                if (s_on) {
+                    const uint32_t to = st + 2 * S::kRows + l_lane * kBytes + i * kScalePass * NG * 4;
+                    if (wanted && !there) store_nan<kBytes>(to);
+                    else copy_async<kBytes>(to, reinterpret_cast<const uint8_t *>(a.c.k_sm) + off, there ? kBytes : 0);
+                    copy_async<kBytes>(to + S::kScales, reinterpret_cast<const uint8_t *>(a.c.v_sm) + off, there ? kBytes : 0);
                 }
             }
         }
@@ -358,6 +461,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         if (tid == 0) segments[slot] = Segment{l_s.q0, l_s.n, l_s.len, l_s.p0, l_s.tile0, l_s.tiles, l_head, rows0, l_at, (int)l_s.bad};
     };
 
+    l_table = a.pages + l_b * a.pages_ld;
+    at_head();
     int l_page = find_page();
 #pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) {
@@ -512,11 +617,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     for (int nt = 0; nt < NT; ++nt) {
                         uint32_t q[4];
                         q_at(nt, ks, q);
-                        mma_bf16(s[ki][nt], k0[0], k0[1], k0[2], k0[3], q[0], q[1]);
-                        mma_bf16(s[ki][nt], k1[0], k1[1], k1[2], k1[3], q[2], q[3]);
+                        mma<false>(s[ki][nt], k0, q[0], q[1]);
+                        mma<false>(s[ki][nt], k1, q[2], q[3]);
                     }
                 }
             } else {
+                uint32_t k_words[2][NG];
+                load_scales(k_words[0], k_sm + (key0 + g) * NG), load_scales(k_words[1], k_sm + (key0 + g + 8) * NG);
 #pragma unroll
                 for (int grp = 0; grp < NG; ++grp) {
                     float part[NT][4] = {};
@@ -539,14 +646,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                         for (int nt = 0; nt < NT; ++nt) {
                             uint32_t q[4];
                             q_at(nt, blk * 2, q);
-                            mma_f16(part[nt], k0, q[0], q[1]);
-                            mma_f16(part[nt], k1, q[2], q[3]);
+                            mma<true>(part[nt], k0, q[0], q[1]);
+                            mma<true>(part[nt], k1, q[2], q[3]);
                         }
                     }
                     float sc[2], mn[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint32_t w = k_sm[(key0 + g + 8 * e) * NG + grp];
+                        const uint32_t w = k_words[e][grp];
                         sc[e] = __uint_as_float(w << 16);
                         mn[e] = fmaf(-S::kOffset, sc[e], __uint_as_float(w & 0xffff0000u));
                     }
@@ -568,13 +675,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 for (int e = 0; e < 4; ++e) s[ki][nt][e] *= e & 1 ? f.y : f.x;
         }
         if (a.softcap > 0.f) {
-            const float by = 1.f / a.softcap, to = a.softcap * kLog2e;
+            // tanh x = 1 - 2 / (exp(2 x) + 1): 2^-22 of the cap, as good as a score near it is in FP32
+            const float by = 2.f * kLog2e / a.softcap, to = a.softcap * kLog2e;
 #pragma unroll
             for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = to * tanhf(s[ki][nt][e] * by);
+                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(-2.f * to, reciprocal_fast(exp2_fast(s[ki][nt][e] * by) + 1.f), to);
         }
         const bool whole = at >= whole0 && at < whole1;
         uint32_t hidden = 0;  // bit (ki * NT + nt) * 4 + e: that query does not see that key
@@ -612,15 +720,28 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 top[nt][e] = v;
                 move = move || v > m[nt][e] + kSlack;
             }
+        uint32_t v_words[KI][2][kGroups];
+        bool odd = false;  // a scale or a min among them is none, and there are rows that must not hear of it
         if constexpr (kQuant) {
             float v_top = 0.f;
 #pragma unroll
             for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2; ++e) {
+                    load_scales(v_words[ki][e], v_sm + (ki * 16 + g + 8 * e) * NG);
 #pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) v_top = fmaxf(v_top, fabsf(__uint_as_float(v_sm[(ki * 16 + g + 8 * e) * NG + grp] << 16)));
+                    for (int grp = 0; grp < NG; ++grp) v_top = fmaxf(v_top, fabsf(__uint_as_float(v_words[ki][e][grp] << 16)));
+                }
             move = move || (__float_as_uint(v_top) >> 23) > (uint32_t)v_exp;
+            if (!whole) {
+#pragma unroll
+                for (int ki = 0; ki < KI; ++ki)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int grp = 0; grp < NG; ++grp) odd = odd || (v_words[ki][e][grp] & 0x7f80u) == 0x7f80u || (v_words[ki][e][grp] & 0x7f800000u) == 0x7f800000u;
+                odd = __any_sync(0xffffffffu, odd);
+            }
         }
         if (__any_sync(0xffffffffu, move)) {
             float f[NT][2];
@@ -645,7 +766,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
                         for (int grp = 0; grp < NG; ++grp) {
-                            const int x = (int)(v_sm[(ki * 16 + g + 8 * e) * NG + grp] >> 7 & 0xffu);
+                            const int x = (int)(v_words[ki][e][grp] >> 7 & 0xffu);
                             if (x != 255) ex = max(ex, x);  // a scale that is none says nothing of the others
                         }
                 ex = max(v_exp, __reduce_max_sync(0xffffffffu, ex));
@@ -705,7 +826,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                         uint32_t v[4];  // columns 0 - 7 and 8 - 15 of keys 0 - 7, then of keys 8 - 15
                         load_matrices_trans(v, smem_of(vt + chunk_at<CR>(key0 + (lane & 7) + 8 * (lane >> 4), d * 2 + ((lane >> 3) & 1)) * 16));
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_bf16(o[d][nt], v[0], v[1], v[2], v[3], p[nt][0], p[nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma<false>(o[d][nt], v, p[nt][0], p[nt][1]);
                     }
                 } else {
 #pragma unroll 1
@@ -745,14 +866,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     float sc[2], mn[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint32_t x = v_sm[(key0 + g + 8 * e) * NG + grp];
+                        const uint32_t x = v_words[ki][e][grp];
                         sc[e] = __uint_as_float(x << 16) * v_up, mn[e] = __uint_as_float(x & 0xffff0000u);
                     }
                     uint32_t p[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float w[4];
-                        if (hidden == 0) {
+                        if (!odd) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 w[e] = s[ki][nt][e] * sc[e >> 1];
@@ -771,7 +892,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                         p[nt][0] = transposed(pack_f16(w[0], w[1])), p[nt][1] = transposed(pack_f16(w[2], w[3]));
                         if constexpr (S::kOffsetV) {
                             constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-                            mma_f16(w_sum[grp][nt], kOnes, p[nt][0], p[nt][1]);
+                            mma<true>(w_sum[grp][nt], kOnes, p[nt][0], p[nt][1]);
                         }
                     }
                     auto code = [](uint32_t v) { return S::kOffsetV ? v : less_offset<BITS>(v); };
@@ -786,19 +907,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                                 const uint32_t va[4] = {code(bytes_f16(v[2 * x], 0x4240)), code(bytes_f16(v[2 * x], 0x4341)), code(bytes_f16(v[2 * x + 1], 0x4240)),
                                                         code(bytes_f16(v[2 * x + 1], 0x4341))};
 #pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) mma_f16(o[c + x][nt], va, p[nt][0], p[nt][1]);
+                                for (int nt = 0; nt < NT; ++nt) mma<true>(o[c + x][nt], va, p[nt][0], p[nt][1]);
                             }
                         } else {  // a chunk of 32 columns: 4 n and 4 n + 1 in the first fragment, 4 n + 2 and 4 n + 3 in the second
                             const int c = grp * (S::G / 32) + run;
-                            uint32_t v0, v1;
-                            asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
-                                         : "=r"(v0), "=r"(v1)
-                                         : "r"(smem_of(vt + chunk_at<CR>(key0 + a_row, c) * 16))
-                                         : "memory");
-                            const uint32_t va[4] = {code(nibbles_f16(v0 << 4)), code(nibbles_f16(v0)), code(nibbles_f16(v1 << 4)), code(nibbles_f16(v1))};
-                            const uint32_t vb[4] = {code(nibbles_f16(v0 >> 4)), code(nibbles_f16(v0 >> 8)), code(nibbles_f16(v1 >> 4)), code(nibbles_f16(v1 >> 8))};
+                            uint32_t v[2];
+                            load_matrices_trans(v, smem_of(vt + chunk_at<CR>(key0 + a_row, c) * 16));
+                            const uint32_t va[4] = {code(nibbles_f16(v[0] << 4)), code(nibbles_f16(v[0])), code(nibbles_f16(v[1] << 4)), code(nibbles_f16(v[1]))};
+                            const uint32_t vb[4] = {code(nibbles_f16(v[0] >> 4)), code(nibbles_f16(v[0] >> 8)), code(nibbles_f16(v[1] >> 4)), code(nibbles_f16(v[1] >> 8))};
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_f16(o[2 * c][nt], va, p[nt][0], p[nt][1]), mma_f16(o[2 * c + 1][nt], vb, p[nt][0], p[nt][1]);
+                            for (int nt = 0; nt < NT; ++nt) mma<true>(o[2 * c][nt], va, p[nt][0], p[nt][1]), mma<true>(o[2 * c + 1][nt], vb, p[nt][0], p[nt][1]);
                         }
                     }
                 }
@@ -915,41 +1033,37 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             // the CTAs that share the segment are those whose runs hold its units; the first one's number is the counter's
             auto cta_of = [&](int64_t u) { return ((u + 1) * ctas + total - 1) / total - 1; };
             const int64_t c0 = cta_of(seg0), c1 = cta_of(seg1 - 1);
-            auto *const last = reinterpret_cast<int *>(scan + kWarps);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t before = atomicAdd(a.count + c0, 1u);
-                *last = before == (uint32_t)(c1 - c0);
-                if (*last) a.count[c0] = 0;
-            }
-            __syncthreads();
-            if (*last) {
+            if constexpr (!S::kJoinHere) {
+                if (tid == 0 && seg0 >= u0) a.joins[blockIdx.x] = Join{sg.q0, sg.rows0, sg.head, rows, (int)(c1 - c0) + 1, {}};
+            } else {
+                auto *const last = reinterpret_cast<int *>(scan + kWarps);
                 __threadfence();
-                for (int x = tid; x < rows * (D / 4); x += kThreads) {
-                    const int r = x / (D / 4), c4 = x % (D / 4);
-                    const int64_t step = 2 * (int64_t)R * (D + 2);
-                    const float *const p0 = a.partial + (2 * c0 + 1) * R * (D + 2), *const p1 = a.partial + 2 * (c0 + 1) * R * (D + 2);
-                    const int more = (int)(c1 - c0);
-                    float top_r = __ldcg(p0 + R * D + r);
+                __syncthreads();
+                if (tid == 0) {
+                    const uint32_t before = atomicAdd(a.count + c0, 1u);
+                    *last = before == (uint32_t)(c1 - c0);
+                    if (*last) a.count[c0] = 0;
+                }
+                __syncthreads();
+                if (*last) {
+                    __threadfence();
+                    const Parts<R, D> from(a.partial, (int)c0, (int)(c1 - c0) + 1);
+                    {   // every row's maximum: a column of threads a row, then theirs
+                        constexpr int kCols = kThreads / R;
+                        const int r = tid % R;
+                        float v = kLowest;
 #pragma unroll 4
-                    for (int k = 0; k < more; ++k) top_r = fmaxf(top_r, __ldcg(p1 + k * step + R * D + r));
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    float sum_r = 0.f;
-#pragma unroll 4
-                    for (int k = -1; k < more; ++k) {
-                        const float *const p = k < 0 ? p0 : p1 + k * step;
-                        const float top_k = __ldcg(p + R * D + r), f = exp2_fast(top_k - top_r);
-                        const float4 w = __ldcg(reinterpret_cast<const float4 *>(p + r * D + 4 * c4));
-                        sum_r = fmaf(__ldcg(p + R * (D + 1) + r), f, sum_r);
-                        v.x = fmaf(w.x, f, v.x), v.y = fmaf(w.y, f, v.y), v.z = fmaf(w.z, f, v.z), v.w = fmaf(w.w, f, v.w);
+                        for (int k = tid / R; k < from.n; k += kCols) v = fmaxf(v, from.top(k, r));
+                        joint[tid] = v;
+                        __syncthreads();
+                        if (tid < R) {
+#pragma unroll
+                            for (int k = 1; k < kCols; ++k) v = fmaxf(v, joint[k * R + tid]);
+                            row_max[tid] = v;
+                        }
+                        __syncthreads();
                     }
-                    const int tok = (sg.rows0 + r) / a.group, head = sg.head * a.group + sg.rows0 + r - tok * a.group;
-                    const float inv = sum_r == 0.f ? 0.f : 1.f / sum_r;
-                    uint2 w;
-                    w.x = pack_bf16(v.x * inv, v.y * inv), w.y = pack_bf16(v.z * inv, v.w * inv);
-                    *reinterpret_cast<uint2 *>(a.out + (sg.q0 + tok) * a.out_ld + (int64_t)head * D + 4 * c4) = w;
-                    if (a.lse != nullptr && c4 == 0) a.lse[(int64_t)(sg.q0 + tok) * a.n_q + head] = sum_r == 0.f ? -CUDART_INF_F : fmaf(top_r, kLn2, logf(sum_r));
+                    for (int x = tid; x < rows * (D / 4); x += kThreads) join_run(a, from, sg.q0, sg.rows0, sg.head, x / (D / 4), x % (D / 4), row_max[x / (D / 4)]);
                 }
             }
         }
@@ -962,7 +1076,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 inline int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 // The counters' place is every form's: calls of different ones share a workspace.
-inline size_t counter_bytes() { return ((size_t)sm_count() * kMostPerSm * 4 + 255) / 256 * 256; }
+inline size_t counter_bytes() { return ((size_t)sm_count() * kMostPerSm * (sizeof(uint32_t) + sizeof(Join)) + 255) / 256 * 256; }
 
 template <class S> struct Launch {
     static_assert(S::kPerSm <= kMostPerSm, "");
@@ -972,10 +1086,13 @@ template <class S> struct Launch {
     static cudaError_t run(Args a, void *ws, int64_t most_units, cudaStream_t st) {
         const int64_t n = std::max<int64_t>(1, std::min(ctas(), (most_units + kMinRun - 1) / kMinRun));
         a.count = static_cast<uint32_t *>(ws);
+        a.joins = reinterpret_cast<Join *>(a.count + (size_t)sm_count() * kMostPerSm);
         a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + counter_bytes());
         const cudaError_t rc = cudaFuncSetAttribute(attn_decode_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
         if (rc != cudaSuccess) return rc;
-        return launch_behind(attn_decode_kernel<S>, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a);
+        const cudaError_t rc2 = launch_behind(attn_decode_kernel<S>, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a);
+        if (S::kJoinHere || rc2 != cudaSuccess) return rc2;
+        return launch_behind(attn_join_kernel<S>, dim3((unsigned)n, S::R / kJoinRows), dim3(kJoinRows * S::D / 4), 0, st, 1, a);
     }
 };
 
