@@ -514,7 +514,8 @@ int sxb_strixw_expert_views(const SxbStrixw *f, const char *name, int64_t E, Sxb
  * group's scale and min stand side by side in one 32-bit word, the scale in its lower half.
  * Row number of (page, head, token in page) = page * page_stride + head * head_stride + token * row_stride: a row's codes start at
  * number * D * bits / 8 bytes, its words of scales at number * D / G.  [n_pages, n_kv, page, D] has the strides n_kv * page, page, 1.
- * D = 64, 128 or 256; G = 32, 64 or 128, at most D; page = a power of two of 8..4096; all four arrays 16-byte aligned.
+ * D = 64, 128 or 256; G = 32, 64 or 128, at most D; page = a power of two of 8..4096; all four arrays 16-byte aligned, the
+ * codes of each at most 2^36 bytes.
  * Token p of a sequence lies in page pages[seq * pages_ld + p / page].  A page may stand in several tables (a shared prefix). */
 typedef struct SxbKvCache {
     void *k, *v;
@@ -532,20 +533,38 @@ typedef struct SxbKvCache {
  * holds a NaN or an infinity reads back as NaN).  seq[t] < 0: a padding row, nothing of it is written.  A position or page out of
  * range: err = {1, token, pos}, the token's queries NaN, nothing written to the cache.  No (seq, pos) twice in one call.
  * Rows of qkv and q_out and the norm weights 16-byte aligned. */
-int sxb_attn_qkv_write(const void *qkv, int64_t ld, int act, int64_t T, int64_t n_q, const float *q_norm, const float *k_norm,
-                       float eps, const float *inv_freq, int64_t rot, int interleaved, const int32_t *seq, const int32_t *pos,
-                       const int32_t *pages, int64_t pages_ld, int64_t n_cols, int64_t n_seq, const SxbKvCache *cache, void *q_out,
-                       int64_t q_ld, uint32_t *err, sxb_stream_t stream);
+typedef struct SxbAttnQkvWriteArgs {
+    const void *qkv;
+    int64_t ld, T, n_q;
+    const float *q_norm, *k_norm, *inv_freq;
+    int64_t rot;
+    const int32_t *seq, *pos, *pages; /* [T], [T], [n_seq, pages_ld] of which n_cols columns are entries */
+    int64_t pages_ld, n_cols, n_seq;
+    const SxbKvCache *cache;
+    void *q_out;
+    int64_t q_ld;
+    uint32_t *err;
+    float eps;
+    int act, interleaved;
+} SxbAttnQkvWriteArgs;
+int sxb_attn_qkv_write(const SxbAttnQkvWriteArgs *args, sxb_stream_t stream);
 /* Rows of the cache back: k_out, v_out [T, n_kv, D], BF16 or FP32 (out_act) = code * scale + min in FP32, rounded once.
  * seq, pos and err as above: seq[t] < 0 leaves the rows as they are, a bad place gives NaN. */
-int sxb_kv_read(const SxbKvCache *cache, const int32_t *seq, const int32_t *pos, const int32_t *pages, int64_t pages_ld,
-                int64_t n_cols, int64_t n_seq, int64_t T, void *k_out, void *v_out, int out_act, uint32_t *err, sxb_stream_t stream);
+typedef struct SxbKvReadArgs {
+    const SxbKvCache *cache;
+    const int32_t *seq, *pos, *pages;
+    int64_t pages_ld, n_cols, n_seq, T;
+    void *k_out, *v_out;
+    uint32_t *err;
+    int out_act;
+} SxbKvReadArgs;
+int sxb_kv_read(const SxbKvReadArgs *args, sxb_stream_t stream);
 /* Attention of the new tokens of B sequences over their pages.  q [T, q_ld] BF16 (n_q heads of D, as sxb_attn_qkv_write leaves them);
  * sequence b has the rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]) and kv_len[b] keys, the new tokens' own included: its row
  * i of n stands at position p = kv_len[b] - n + i and sees the keys j <= p, with window > 0 only j > p - window.  Query head h
  * reads key head h / (n_q / n_kv).  Scores scale * q . k, with softcap > 0 softcap * tanh(score / softcap).
  * out [T, out_ld] BF16 = softmax(scores) . V, lse [T, n_q] FP32 (or NULL) = log of the sum of exp(score); a row that sees no key
- * (or none with a score above -inf): 0 and -inf.  Rows outside every sequence are left as they are.  Scores, statistics and
+ * (or none with a score above -1e30): 0 and -inf.  Rows outside every sequence are left as they are.  Scores, statistics and
  * sums are FP32; weights are rounded to BF16 (BF16 cache) or, times a group's scale, to F16 for the product with V.
  * max_q: a sequence's largest count of new tokens, which picks the kernel (a sequence with more is handled, in several passes over
  * its keys).  Made for a token and its drafts; long chunks of queries are right but no match for a prefill kernel.
@@ -554,10 +573,24 @@ int sxb_kv_read(const SxbKvCache *cache, const int32_t *seq, const int32_t *pos,
  * Data errors (err = {1, sequence, value}): a page id out of range makes the keys on that page NaN; kv_len outside
  * 0 .. n_cols * page makes the sequence's rows NaN; a q_start that falls or leaves 0..T skips the sequence. */
 size_t sxb_attn_decode_workspace_bytes(int64_t n_q, int64_t n_kv, int64_t D, int bits, int64_t max_q);
-int sxb_attn_decode(const void *q, int64_t q_ld, int64_t T, int64_t n_q, const SxbKvCache *cache, const int32_t *pages,
-                    int64_t pages_ld, int64_t n_cols, const int32_t *q_start, const int32_t *kv_len, int64_t B, int64_t max_q,
-                    float scale, float softcap, int64_t window, void *out, int64_t out_ld, float *lse, void *ws, size_t ws_bytes,
-                    uint32_t *err, sxb_stream_t stream);
+typedef struct SxbAttnDecodeArgs {
+    const void *q;
+    int64_t q_ld, T, n_q;
+    const SxbKvCache *cache;
+    const int32_t *pages; /* [B, pages_ld] of which n_cols columns are entries */
+    int64_t pages_ld, n_cols;
+    const int32_t *q_start, *kv_len;
+    int64_t B, max_q;
+    void *out;
+    int64_t out_ld;
+    float *lse;
+    void *ws;
+    size_t ws_bytes;
+    uint32_t *err;
+    int64_t window;
+    float scale, softcap;
+} SxbAttnDecodeArgs;
+int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t stream);
 /* The error words of the three (a blocking 12-byte copy, as sxb_check_router_error) / already on the host. */
 int sxb_check_attn_error(const uint32_t *err, const char *what);
 int sxb_report_attn_error(const uint32_t e[3], const char *what);

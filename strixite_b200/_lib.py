@@ -55,7 +55,6 @@ class SxbMoeLayerArgs(C.Structure):
 
 QV = C.POINTER(SxbQView)
 SA = C.POINTER(SxbMoeSharedAdd)
-KV = C.POINTER(SxbKvCache)
 
 # name -> (restype, argtypes); mirrors include/strix_b200.h declaration by declaration.
 SIGNATURES = {
@@ -131,11 +130,11 @@ SIGNATURES = {
     "sxb_hc_mix_up_wmma_q8": (C.c_int, [vp, QV, vp, vp, vp, i64, i64, i64, vp, vp, sz, C.c_int, vp]),
     "sxb_moe_route_small": (C.c_int, [vp, i64, i64, i64, i64, i64, i64, vp, vp, vp, sz, vp, vp, vp]),
 }
-SIGNATURES.update({
-    "sxb_attn_qkv_write": (C.c_int, [vp, i64, C.c_int, i64, i64, vp, vp, C.c_float, vp, i64, C.c_int, vp, vp, vp, i64, i64, i64, KV, vp, i64, vp, vp]),
-    "sxb_kv_read": (C.c_int, [KV, vp, vp, vp, i64, i64, i64, i64, vp, vp, C.c_int, vp, vp]),
+SIGNATURES.update({  # argument blocks: bytes laid out as the header's structs (kernels.py), or a ctypes pointer
+    "sxb_attn_qkv_write": (C.c_int, [vp, vp]),
+    "sxb_kv_read": (C.c_int, [vp, vp]),
     "sxb_attn_decode_workspace_bytes": (sz, [i64, i64, i64, C.c_int, i64]),
-    "sxb_attn_decode": (C.c_int, [vp, i64, i64, i64, KV, vp, i64, i64, vp, vp, i64, i64, C.c_float, C.c_float, i64, vp, i64, vp, vp, sz, vp, vp]),
+    "sxb_attn_decode": (C.c_int, [vp, vp]),
     "sxb_check_attn_error": (C.c_int, [vp, cp]),
     "sxb_report_attn_error": (C.c_int, [C.POINTER(u32), cp]),
 })

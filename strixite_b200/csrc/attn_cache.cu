@@ -3,9 +3,10 @@
 //
 //   x' = x / sqrt(mean(x^2) + eps) * w,   (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = pos * inv_freq[i]
 //
-// One pass: a warp has a head of a token in registers (D / 32 neighbouring elements a lane), the norm's sum, the rotation's partner and a group's
-// extremes go by shuffles.  All FP32, but for the angle: pos * inv_freq loses 2^-24 of a number of turns that grows with the position (a hundred thousand
-// tokens: 6e-3 of a radian), so product and reduction are FP64, once a token and angle, into shared memory for all of its heads.
+// One pass: a lane has eight neighbouring elements of a head, D / 8 lanes a head, a warp one to four heads; the norm's sum, the rotation's partner and a
+// group's extremes go by shuffles.  All FP32, but for the angle: pos * inv_freq loses 2^-24 of a number of turns that grows with the position (a hundred
+// thousand tokens: 6e-3 of a radian), so product and reduction are FP64, once a token and angle, into shared memory for all of its heads.  Norm weight
+// and rotation are one pair of factors an element, the same for all heads: x'_i = inv * (x_i (w_i cos) + x_partner (w_partner +- sin)).
 // The same formulas as sxb_quantize's make the codes (formats/q4.cpp:44-88), from the FP32 values: nothing is rounded on the way.
 
 #include "attn.cuh"
@@ -24,7 +25,7 @@ struct WriteArgs {
     float eps;
     const int32_t *seq, *pos, *pages;
     int64_t pages_ld;
-    int n_seq, n_cols, G, heads_per_cta;
+    int n_seq, n_cols, G, items_per_cta;
     KvView c;
     uint16_t *q_out;
     int64_t q_ld;
@@ -70,20 +71,19 @@ template <int N> __device__ inline void store_bf16_run(uint16_t *p, const float 
     store_words<2 * N>(p, r);
 }
 
-// A head's elements into a cache row.  BITS 16: rounded to BF16.  Otherwise a group's lanes find its extremes; a group that holds a NaN or an infinity
-// has no code that stands for it and reads back as NaN throughout.
+// A lane's eight elements of a cache row, number `part` of the row's eights.  BITS 16: rounded to BF16.  Otherwise a group's lanes find its extremes; a
+// group that holds a NaN or an infinity has no code that stands for it and reads back as NaN throughout.  All lanes of the warp come here together.
 template <int D, int BITS>
-__device__ inline void store_row(uint8_t *rows, uint32_t *sm, int64_t row, const float (&v)[D / 32], int lane, int G) {
-    constexpr int N = D / 32;
+__device__ inline void store_run(uint8_t *rows, uint32_t *sm, int64_t row, const float (&v)[8], int part, int G, bool on) {
     if constexpr (BITS == 16) {
-        store_bf16_run(reinterpret_cast<uint16_t *>(rows) + row * D + lane * N, v);
+        if (on) store_bf16_run(reinterpret_cast<uint16_t *>(rows) + row * D + part * 8, v);
     } else {
         constexpr float kLevels = BITS == 4 ? 15.f : 255.f;
-        const int lanes = G / N;  // of a group: a power of two, 4 to 32 (G = 128 at D = 64 is refused)
+        const int lanes = G / 8;  // of a group: 4, 8 or 16
         float lo = v[0], hi = v[0];
         bool bad = !isfinite(v[0]);
 #pragma unroll
-        for (int i = 1; i < N; ++i) lo = fminf(lo, v[i]), hi = fmaxf(hi, v[i]), bad = bad || !isfinite(v[i]);
+        for (int i = 1; i < 8; ++i) lo = fminf(lo, v[i]), hi = fmaxf(hi, v[i]), bad = bad || !isfinite(v[i]);
         for (int off = 1; off < lanes; off <<= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
@@ -91,19 +91,17 @@ __device__ inline void store_row(uint8_t *rows, uint32_t *sm, int64_t row, const
         }
         const uint32_t s_bits = bad ? 0x7fc0u : f32_to_bf16_bits(__fdiv_rn(__fsub_rn(hi, lo), kLevels)), m_bits = bad ? 0x7fc0u : f32_to_bf16_bits(lo);
         const float s = bf16_bits_to_f32((uint16_t)s_bits), m = bf16_bits_to_f32((uint16_t)m_bits);
-        if (lane % lanes == 0) sm[row * (D / G) + lane / lanes] = s_bits | m_bits << 16;
-        uint32_t packed[(N * BITS + 31) / 32] = {};
+        Words<BITS> packed = {};
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < 8; ++i) {
             uint32_t code = 0;
             if (s > 0.f) code = (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v[i], m), s)), 0.f), kLevels);
-            packed[i * BITS / 32] |= code << (i * BITS % 32);
+            packed.w[i * BITS / 32] |= code << (i * BITS % 32);
         }
-        constexpr int kLaneBytes = N * BITS / 8;  // 1 to 8
-        uint8_t *dst = rows + row * (D * BITS / 8) + lane * kLaneBytes;
-        if constexpr (kLaneBytes >= 4) store_words<kLaneBytes>(dst, *reinterpret_cast<const Words<kLaneBytes> *>(packed));
-        else if constexpr (kLaneBytes == 2) *reinterpret_cast<uint16_t *>(dst) = (uint16_t)packed[0];
-        else *dst = (uint8_t)packed[0];
+        if (on) {
+            if (part % lanes == 0) sm[row * (D / G) + part / lanes] = s_bits | m_bits << 16;
+            store_words<BITS>(rows + row * (D * BITS / 8) + part * BITS, packed);
+        }
     }
 }
 
@@ -125,16 +123,37 @@ __device__ inline Place find_place(int seq, int pos, const int32_t *pages, int64
     return p;
 }
 
+// An item is the heads that a warp takes at once: the queries' items, then the keys', then the values'.
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(kWriteThreads) qkv_write_kernel(const __grid_constant__ WriteArgs a) {
     __shared__ float2 turn[D / 2];  // cos, sin of the token's angles
+    constexpr int kLanes = D / 8, kHeads = 32 / kLanes, kBatch = 4;
     behind_grid();
-    constexpr int N = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane % kLanes, sub = lane / kLanes;
     const int64_t t = blockIdx.x;
+    const int q_items = (a.n_q + kHeads - 1) / kHeads, kv_items = (a.n_kv + kHeads - 1) / kHeads;
+    const int first = blockIdx.y * a.items_per_cta, last = min(q_items + 2 * kv_items, first + a.items_per_cta);
+    const T *const row = static_cast<const T *>(a.qkv) + t * a.ld + part * 8;
+    // kind 0, 1, 2: queries, keys, values; this lane's head of that kind, none at an item's ragged end
+    auto which = [&](int item, int &kind, int &head) {
+        kind = item < q_items ? 0 : item < q_items + kv_items ? 1 : 2;
+        head = (item - (kind == 0 ? 0 : kind == 1 ? q_items : q_items + kv_items)) * kHeads + sub;
+        return item < last && head < (kind == 0 ? a.n_q : a.n_kv);
+    };
+    Words<8 * (int)sizeof(T)> raw[kBatch];
+    auto fetch = [&](int base) {  // a batch's loads side by side
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            int kind, head;
+            if (which(base + b * kWriteWarps + warp, kind, head)) raw[b] = load_words<8 * (int)sizeof(T)>(row + (int64_t)((kind == 0 ? 0 : kind == 1 ? a.n_q : a.n_q + a.n_kv) + head) * D);
+            else raw[b] = {};
+        }
+    };
+    fetch(first);
     const int seq = a.seq[t], pos = a.pos[t];
     const Place place = find_place(seq, pos, a.pages, a.pages_ld, a.n_seq, a.n_cols, a.c);
     if (place.state == 1) return;
+    if (place.state == 2 && threadIdx.x == 0 && first == 0) raise_error(a.err, (uint32_t)t, (uint32_t)pos);
     const int half = a.rot / 2;
     if ((int)threadIdx.x < half) {
         // the angle less whole turns: what is left of 2^31 * inv_freq in FP64 is good to 2^-22 of a radian, of 2^20 * 1 to 2^-33
@@ -145,53 +164,75 @@ __global__ void __launch_bounds__(kWriteThreads) qkv_write_kernel(const __grid_c
         turn[threadIdx.x] = make_float2(c, s);
     }
     __syncthreads();
-    const int heads = a.n_q + 2 * a.n_kv, first = blockIdx.y * a.heads_per_cta, last = min(heads, first + a.heads_per_cta);
-    if (place.state == 2 && threadIdx.x == 0 && first == 0) raise_error(a.err, (uint32_t)t, (uint32_t)pos);
-    // What a lane's elements are turned by is the same in every head: element i becomes x_i co_i + partner si_i, elements behind rot keep themselves.
-    float co[N], si[N];
-    const bool turned = lane * N < a.rot, low = lane * N < half;
-    const int partner = turned && !a.interleaved ? (low ? lane + half / N : lane - half / N) : lane;  // half is a multiple of 8 >= N
+    const bool turned = part * 8 < a.rot, low = part * 8 < half;
+    const int partner = turned && !a.interleaved ? (low ? part + half / 8 : part - half / 8) : part;  // half is a multiple of 8
+    float by[8], cross[8];
+    int have = -1;
+    for (int base = first; base < last; base += kBatch * kWriteWarps) {
+        if (base != first) fetch(base);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int e = lane * N + i;
-        const float2 cs = turned ? turn[a.interleaved ? e / 2 : low ? e : e - half] : make_float2(1.f, 0.f);
-        co[i] = cs.x, si[i] = (a.interleaved ? i % 2 == 0 : low) ? -cs.y : cs.y;
-    }
-#pragma unroll 2
-    for (int h = first + warp; h < last; h += kWriteWarps) {
-        const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
-        float v[N];
-        load_run<T, N>(static_cast<const T *>(a.qkv) + t * a.ld + (int64_t)h * D + lane * N, v);
-        if (is_q || is_k) {
-            const float *w = is_q ? a.q_norm : a.k_norm;
-            if (w != nullptr) {
-                float sum = 0.f, by[N];
-                load_run<float, N>(w + lane * N, by);
+        for (int b = 0; b < kBatch; ++b) {
+            const int item = base + b * kWriteWarps + warp;
+            if (item >= last) break;
+            int kind, head;
+            const bool on = which(item, kind, head);
+            float v[8];
 #pragma unroll
-                for (int i = 0; i < N; ++i) sum = fmaf(v[i], v[i], sum);
-#pragma unroll
-                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                const float inv = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
-#pragma unroll
-                for (int i = 0; i < N; ++i) v[i] = v[i] * inv * by[i];
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[b].w[i]);
+                else v[i] = __uint_as_float(i & 1 ? raw[b].w[i / 2] & 0xffff0000u : raw[b].w[i / 2] << 16);
             }
-            if (a.rot != 0) {
-                float other[N];
+            if (kind != 2) {
+                const float *const w = kind == 0 ? a.q_norm : a.k_norm;
+                if (kind != have) {
+                    have = kind;
 #pragma unroll
-                for (int i = 0; i < N; ++i) other[i] = a.interleaved ? v[i ^ 1] : __shfl_sync(0xffffffffu, v[i], partner);
+                    for (int i = 0; i < 8; ++i) by[i] = 1.f, cross[i] = 0.f;
+                    if (w != nullptr) load_run<float, 8>(w + part * 8, by);
+                    if (turned) {
+                        float by_other[8];
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[i] = fmaf(v[i], co[i], other[i] * si[i]);
+                        for (int i = 0; i < 8; ++i) by_other[i] = a.interleaved ? by[i ^ 1] : 1.f;
+                        if (w != nullptr && !a.interleaved) load_run<float, 8>(w + partner * 8, by_other);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) cross[i] = by_other[i];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int e = part * 8 + i;
+                            const float2 cs = turn[a.interleaved ? e / 2 : low ? e : e - half];
+                            by[i] *= cs.x, cross[i] *= (a.interleaved ? i % 2 == 0 : low) ? -cs.y : cs.y;
+                        }
+                    }
+                }
+                float inv = 1.f;
+                if (w != nullptr) {
+                    float sum = v[0] * v[0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
+#pragma unroll
+                    for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                    inv = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
+                }
+                if (a.rot != 0) {
+                    float other[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) other[i] = a.interleaved ? v[i ^ 1] : __shfl_sync(0xffffffffu, v[i], partner, kLanes);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = inv * fmaf(v[i], by[i], other[i] * cross[i]);
+                } else if (w != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = inv * (v[i] * by[i]);
+                }
             }
-        }
-        if (is_q) {
-            if (place.state == 2) {
+            if (kind == 0) {
+                if (place.state == 2) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[i] = qnan_f32();
+                    for (int i = 0; i < 8; ++i) v[i] = qnan_f32();
+                }
+                if (on) store_bf16_run(a.q_out + t * a.q_ld + (int64_t)head * D + part * 8, v);
+            } else if (place.state == 0) {
+                store_run<D, BITS>(kind == 1 ? a.c.k : a.c.v, kind == 1 ? a.c.k_sm : a.c.v_sm, kv_row(a.c, place.page, on ? head : 0, place.at), v, part, a.G, on);
             }
-            store_bf16_run(a.q_out + t * a.q_ld + (int64_t)h * D + lane * N, v);
-        } else if (place.state == 0) {
-            const int kv = is_k ? h - a.n_q : h - a.n_q - a.n_kv;
-            store_row<D, BITS>(is_k ? a.c.k : a.c.v, is_k ? a.c.k_sm : a.c.v_sm, kv_row(a.c, place.page, kv, place.at), v, lane, a.G);
         }
     }
 }
@@ -201,7 +242,7 @@ constexpr int kReadThreads = 256, kReadTokens = 32;
 struct ReadArgs {
     const int32_t *seq, *pos, *pages;
     int64_t pages_ld;
-    int T, n_seq, n_cols, G, per_token, tokens;  // runs of eight elements a token has; tokens a CTA
+    int T, n_seq, n_cols, G, tokens;  // tokens a CTA
     KvView c;
     void *k_out, *v_out;
     uint32_t *err;
@@ -225,10 +266,13 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_cons
         rows[threadIdx.x] = place.state == 0 ? kv_row(a.c, place.page, 0, place.at) : place.state == 1 ? kSkip : kBad;
     }
     __syncthreads();
-    const int items = tokens * a.per_token;
+    const int run = threadIdx.x % kRuns, heads = 2 * a.c.n_kv;
+    int token = 0, h = threadIdx.x / kRuns;
+    const uint32_t in_row = run * BITS, group = run * 8 / a.G, groups = D / a.G;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < items; i += kReadThreads) {
-        const int token = i / a.per_token, in = i - token * a.per_token, run = in % kRuns, h = in / kRuns;
+    for (;; h += kReadThreads / kRuns) {
+        while (h >= heads) h -= heads, ++token;
+        if (token >= tokens) break;
         const int64_t row0 = rows[token];
         if (row0 == kSkip) continue;
         const bool is_k = h < a.c.n_kv;
@@ -239,12 +283,12 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_cons
             for (int e = 0; e < 8; ++e) v[e] = qnan_f32();
         } else {
             const int64_t from = row0 + head * a.c.head_stride;
-            const uint8_t *p = (is_k ? a.c.k : a.c.v) + from * (D * BITS / 8) + run * BITS;
+            const uint8_t *p = (is_k ? a.c.k : a.c.v) + from * (D * BITS / 8) + in_row;
             if constexpr (BITS == 16) {
                 load_run(reinterpret_cast<const uint16_t *>(p), v);
             } else {
                 const auto w = load_words<BITS>(p);
-                const uint32_t sm = (is_k ? a.c.k_sm : a.c.v_sm)[from * (D / a.G) + run * 8 / a.G];
+                const uint32_t sm = (is_k ? a.c.k_sm : a.c.v_sm)[from * groups + group];
                 const float s = __uint_as_float(sm << 16), m = __uint_as_float(sm & 0xffff0000u);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {  // a code under the exponent of 2^23 is that number plus it
@@ -314,6 +358,8 @@ int kv_view(const char *fn, const SxbKvCache *c, KvView *out) {
     SXB_CHECK(c->page_stride >= 1 && c->head_stride >= 1 && c->row_stride >= 1 && c->page_stride < (1ll << 32) && c->head_stride < (1ll << 32) &&
                   c->row_stride <= (1ll << 22),
               fn, ": strides of ", c->page_stride, " / ", c->head_stride, " / ", c->row_stride, " rows (page / head / token), expected 1..2^32 - 1, of tokens up to 2^22");
+    const int64_t last = (c->n_pages - 1) * c->page_stride + (c->n_kv - 1) * c->head_stride + (c->page - 1) * c->row_stride;
+    SXB_CHECK((c->n_pages - 1) <= (1ll << 36) / c->page_stride && last < (1ll << 36) / (c->D * c->bits / 8), fn, ": keys of more than 2^36 bytes");
     *out = KvView{static_cast<uint8_t *>(c->k), static_cast<uint8_t *>(c->v), c->k_sm, c->v_sm, c->page_stride, c->head_stride, c->row_stride,
                   (int)c->n_pages, __builtin_ctzll((unsigned long long)c->page), (int)c->n_kv};
     return SXB_OK;
@@ -323,14 +369,17 @@ int kv_view(const char *fn, const SxbKvCache *c, KvView *out) {
 
 using namespace sxb;
 
-extern "C" int sxb_attn_qkv_write(const void *qkv, int64_t ld, int act, int64_t T, int64_t n_q, const float *q_norm, const float *k_norm, float eps,
-                                  const float *inv_freq, int64_t rot, int interleaved, const int32_t *seq, const int32_t *pos, const int32_t *pages,
-                                  int64_t pages_ld, int64_t n_cols, int64_t n_seq, const SxbKvCache *cache, void *q_out, int64_t q_ld, uint32_t *err,
-                                  sxb_stream_t stream) {
+extern "C" int sxb_attn_qkv_write(const SxbAttnQkvWriteArgs *args, sxb_stream_t stream) {
     const char *fn = "attn_qkv_write";
+    SXB_CHECK(args != nullptr, fn, ": null argument block");
+    const void *const qkv = args->qkv;
+    void *const q_out = args->q_out;
+    const SxbKvCache *const cache = args->cache;
+    const int64_t ld = args->ld, T = args->T, n_q = args->n_q, rot = args->rot, q_ld = args->q_ld;
+    const int act = args->act;
     WriteArgs a{};
     if (int rc = kv_view(fn, cache, &a.c)) return rc;
-    if (int rc = check_places(fn, seq, pos, pages, pages_ld, n_cols, n_seq, T, cache, err)) return rc;
+    if (int rc = check_places(fn, args->seq, args->pos, args->pages, args->pages_ld, args->n_cols, args->n_seq, T, cache, args->err)) return rc;
     SXB_CHECK(qkv != nullptr && q_out != nullptr, fn, ": null pointer (qkv=", qkv, ", q_out=", q_out, ")");
     SXB_CHECK(act_ok(act), fn, ": unsupported activation dtype ", act);
     SXB_CHECK(n_q >= 1 && n_q <= 1024, fn, ": n_q = ", n_q, " heads, expected 1..1024");
@@ -339,19 +388,20 @@ extern "C" int sxb_attn_qkv_write(const void *qkv, int64_t ld, int act, int64_t 
               heads * D, " and ", n_q * D, " elements");
     SXB_CHECK(aligned16(qkv) && aligned16(q_out) && ld * es % 16 == 0 && q_ld % 8 == 0, fn, ": rows of qkv and q_out must be 16-byte aligned");
     SXB_CHECK(apart(qkv, ((T - 1) * ld + heads * D) * es, q_out, ((T - 1) * q_ld + n_q * D) * 2), fn, ": q_out [", q_out, "] overlaps qkv [", qkv, "]");
-    SXB_CHECK(inv_freq != nullptr || rot == 0, fn, ": rot = ", rot, " without inv_freq");
+    SXB_CHECK(args->inv_freq != nullptr || rot == 0, fn, ": rot = ", rot, " without inv_freq");
     SXB_CHECK(rot >= 0 && rot <= D && rot % 16 == 0, fn, ": rot = ", rot, ", expected a multiple of 16 of 0..", D);
-    SXB_CHECK(aligned16(q_norm) && aligned16(k_norm), fn, ": norm weights must be 16-byte aligned");
-    SXB_CHECK((q_norm == nullptr && k_norm == nullptr) || (eps > 0.f && eps < 1e30f), fn, ": eps must be finite and positive");
-    a.qkv = qkv, a.ld = ld, a.n_q = (int)n_q, a.n_kv = (int)cache->n_kv, a.rot = (int)rot, a.interleaved = interleaved != 0;
-    a.q_norm = q_norm, a.k_norm = k_norm, a.inv_freq = inv_freq, a.eps = eps;
-    a.seq = seq, a.pos = pos, a.pages = pages, a.pages_ld = pages_ld, a.n_seq = (int)n_seq, a.n_cols = (int)n_cols;
-    a.G = (int)(cache->bits == 16 ? D : cache->G), a.q_out = static_cast<uint16_t *>(q_out), a.q_ld = q_ld, a.err = err;
-    // few tokens: a head a warp, so that the SMs share them; many: a CTA has all heads of its token and its angles are computed once
-    const int64_t whole = (heads + kWriteWarps - 1) / kWriteWarps;
+    SXB_CHECK(aligned16(args->q_norm) && aligned16(args->k_norm), fn, ": norm weights must be 16-byte aligned");
+    SXB_CHECK((args->q_norm == nullptr && args->k_norm == nullptr) || (args->eps > 0.f && args->eps < 1e30f), fn, ": eps must be finite and positive");
+    a.qkv = qkv, a.ld = ld, a.n_q = (int)n_q, a.n_kv = (int)cache->n_kv, a.rot = (int)rot, a.interleaved = args->interleaved != 0;
+    a.q_norm = args->q_norm, a.k_norm = args->k_norm, a.inv_freq = args->inv_freq, a.eps = args->eps;
+    a.seq = args->seq, a.pos = args->pos, a.pages = args->pages, a.pages_ld = args->pages_ld, a.n_seq = (int)args->n_seq, a.n_cols = (int)args->n_cols;
+    a.G = (int)(cache->bits == 16 ? D : cache->G), a.q_out = static_cast<uint16_t *>(q_out), a.q_ld = q_ld, a.err = args->err;
+    // few tokens: an item a warp, so that the SMs share them; many: a CTA has all heads of its token and its angles are computed once
+    const int64_t per = 256 / D, items = (n_q + per - 1) / per + 2 * ((cache->n_kv + per - 1) / per);
+    const int64_t whole = (items + kWriteWarps - 1) / kWriteWarps;
     const int64_t parts = std::min(whole, std::max<int64_t>(1, 4 * (int64_t)sm_count() / T));
-    a.heads_per_cta = (int)((whole + parts - 1) / parts) * kWriteWarps;
-    const dim3 grid((unsigned)T, (unsigned)((heads + a.heads_per_cta - 1) / a.heads_per_cta));
+    a.items_per_cta = (int)((whole + parts - 1) / parts) * kWriteWarps;
+    const dim3 grid((unsigned)T, (unsigned)((items + a.items_per_cta - 1) / a.items_per_cta));
     auto st = static_cast<cudaStream_t>(stream);
     if (act == SXB_ACT_F32) launch_write<float>(a, (int)D, cache->bits, grid, st);
     else launch_write<uint16_t>(a, (int)D, cache->bits, grid, st);
@@ -359,20 +409,24 @@ extern "C" int sxb_attn_qkv_write(const void *qkv, int64_t ld, int act, int64_t 
     return SXB_OK;
 }
 
-extern "C" int sxb_kv_read(const SxbKvCache *cache, const int32_t *seq, const int32_t *pos, const int32_t *pages, int64_t pages_ld, int64_t n_cols,
-                           int64_t n_seq, int64_t T, void *k_out, void *v_out, int out_act, uint32_t *err, sxb_stream_t stream) {
+extern "C" int sxb_kv_read(const SxbKvReadArgs *args, sxb_stream_t stream) {
     const char *fn = "kv_read";
+    SXB_CHECK(args != nullptr, fn, ": null argument block");
+    const SxbKvCache *const cache = args->cache;
+    void *const k_out = args->k_out, *const v_out = args->v_out;
+    const int64_t T = args->T;
+    const int out_act = args->out_act;
     ReadArgs a{};
     if (int rc = kv_view(fn, cache, &a.c)) return rc;
-    if (int rc = check_places(fn, seq, pos, pages, pages_ld, n_cols, n_seq, T, cache, err)) return rc;
+    if (int rc = check_places(fn, args->seq, args->pos, args->pages, args->pages_ld, args->n_cols, args->n_seq, T, cache, args->err)) return rc;
     SXB_CHECK(k_out != nullptr && v_out != nullptr, fn, ": null pointer (k_out=", k_out, ", v_out=", v_out, ")");
     SXB_CHECK(act_ok(out_act), fn, ": unsupported output dtype ", out_act);
     SXB_CHECK(aligned16(k_out) && aligned16(v_out), fn, ": k_out and v_out must be 16-byte aligned");
     const int64_t D = cache->D, bytes = T * cache->n_kv * D * act_bytes(out_act);
     SXB_CHECK(apart(k_out, bytes, v_out, bytes), fn, ": v_out [", v_out, "] overlaps k_out [", k_out, "]");
-    a.seq = seq, a.pos = pos, a.pages = pages, a.pages_ld = pages_ld, a.n_seq = (int)n_seq, a.n_cols = (int)n_cols;
-    a.G = (int)(cache->bits == 16 ? D : cache->G), a.k_out = k_out, a.v_out = v_out, a.err = err;
-    a.T = (int)T, a.per_token = (int)(2 * cache->n_kv * (D / 8));
+    a.seq = args->seq, a.pos = args->pos, a.pages = args->pages, a.pages_ld = args->pages_ld, a.n_seq = (int)args->n_seq, a.n_cols = (int)args->n_cols;
+    a.G = (int)(cache->bits == 16 ? D : cache->G), a.k_out = k_out, a.v_out = v_out, a.err = args->err;
+    a.T = (int)T;
     a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(kReadTokens, T / (8 * (int64_t)sm_count())));
     const unsigned grid = (unsigned)((T + a.tokens - 1) / a.tokens);
     auto st = static_cast<cudaStream_t>(stream);

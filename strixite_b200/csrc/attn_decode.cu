@@ -19,6 +19,9 @@
 
 #include <math_constants.h>
 
+#include <atomic>
+#include <type_traits>
+
 namespace sxb {
 namespace {
 
@@ -29,9 +32,12 @@ constexpr int kSlack = 8;      // powers of two that a weight may be above 1
 constexpr float kLowest = -1e30f;  // below every score; a row that sees no key keeps it
 constexpr int64_t kMaxRows = 1ll << 24;
 
-#ifndef SXB_KI
-#define SXB_KI(D, BITS, NT) ((D) == 64 || ((BITS) == 4 && (D) == 128) ? 2 : 1)
-#endif
+// Runs of sixteen keys that a warp takes at a time: two or four give it independent work and share what a step costs besides.
+constexpr int key_runs(int D, int bits, int nt) {
+    const int by_size = 4096 * 8 / (16 * D * bits);  // 4 KB of keys
+    const int most = nt * D <= 128 ? 4 : nt * D <= 256 ? 2 : 1;  // registers
+    return by_size < 1 ? 1 : by_size < most ? by_size : most;
+}
 // R query rows: NT tiles of eight a warp, WR warps side by side.  The WK groups of such warps share a tile's keys, a run of KI times sixteen each, and
 // every group fetches its own run into its own ring: nothing but a segment's ends is the whole CTA's business.
 template <int D_, int BITS_, int G_, int R_> struct Shape {
@@ -41,13 +47,13 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     static constexpr int kWarps = WR > 1 ? 8 : 4, kThreads = 32 * kWarps, WK = kWarps / WR;
     static constexpr int RB = D * BITS / 8, CR = RB / 16;  // bytes and 16-byte chunks of a cache row
     static constexpr int NG = kQuant ? D / G : 0;
-    static constexpr int KI = SXB_KI(D, BITS, NT), RUN = 16 * KI, TK = RUN * WK;
+    static constexpr int KI = key_runs(D, BITS, NT), RUN = 16 * KI, TK = RUN * WK;
     static constexpr int kRows = RUN * RB, kScales = RUN * NG * 4, kPart = 2 * (kRows + kScales), kStage = WK * kPart;
     static constexpr int kQ = R * D * 2;
     static constexpr int kMostJoint = WK * R * 32 * 4;
     static constexpr bool kOwnJoint = kStage < kMostJoint;  // 32 columns of every warp's rows do not fit a stage
     static constexpr int kMisc = 1024 + WK * R * 8 + R * (NG + 2) * 4 + (kOwnJoint ? kMostJoint : 0);
-    static constexpr int kByRegisters = WR > 1 ? 1 : D * NT <= 128 ? 3 : 2;
+    static constexpr int kByRegisters = WR > 1 ? 1 : 2;
     static constexpr int stages(int per_sm) { return (226 * 1024 / per_sm - kMisc) / (kStage + kQ); }
     static constexpr int kPerSm = kByRegisters > 3 && stages(4) >= 3 ? 4 : kByRegisters > 2 && stages(3) >= 3 ? 3 : kByRegisters > 1 && stages(2) >= 3 ? 2 : 1;
     static constexpr int kStages = stages(kPerSm) > 6 ? 6 : stages(kPerSm);
@@ -64,6 +70,7 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     // Few rows: the last CTA to bring its part joins them, a launch less.  Many: that CTA would read every part by itself (2 x 8 rows over 32 k keys:
     // 19 parts of 33 KB, 30 us at the end of 80), a second kernel has the rows of all segments side by side.
     static constexpr bool kJoinHere = R <= 16;
+    static constexpr bool kHoldSums = kQuant && NG * NT <= 4;
     static constexpr bool kHoldQ = NT * D <= 256;             // q's fragments in registers
     static_assert(kStages >= 2 && WK * WR == kWarps && KI * NT * 4 <= 32, "");
 };
@@ -113,7 +120,7 @@ template <class S> __device__ inline Sequence sequence(const Args &a, int b) {
 
 // A segment of the list that this CTA has units of.
 struct Segment {
-    int q0, n, len, p0, tile0, tiles, head, rows0, at, bad;  // rows0: first row of the tile, at: the CTA's first unit's place in the segment
+    int q0, n, len, p0, lo, tile0, tiles, head, rows0, at, bad;  // rows0: first row of the tile, at: the CTA's first unit's place in the segment
 };
 
 __device__ inline uint32_t smem_of(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -123,22 +130,40 @@ template <int BYTES, int OFF = 0> __device__ inline void copy_async(uint32_t to,
     else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0 + %3], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(n), "n"(OFF) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0 + %3], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(n), "n"(OFF) : "memory");
 }
-template <int BYTES, int OFF = 0> __device__ inline void copy_async(uint32_t to, const void *from) {
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(to), "l"(from), "n"(OFF) : "memory");
-    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0 + %2], [%1], 8;" ::"r"(to), "l"(from), "n"(OFF) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0 + %2], [%1], 4;" ::"r"(to), "l"(from), "n"(OFF) : "memory");
+template <int BYTES, int OFF = 0, int FROM = 0> __device__ inline void copy_async(uint32_t to, const void *from) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(OFF), "n"(FROM) : "memory");
+    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], 8;" ::"r"(to), "l"(from), "n"(OFF), "n"(FROM) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], 4;" ::"r"(to), "l"(from), "n"(OFF), "n"(FROM) : "memory");
 }
 __device__ inline void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ inline void wait_async() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // Volatile: they stay behind the wait that they follow; nothing is written that the compiler knows of.
-__device__ inline void load_matrices(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+template <int OFF = 0> __device__ inline void load_matrices(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at), "n"(OFF));
 }
-__device__ inline void load_matrices_trans(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+template <int OFF> __device__ inline void load_matrices_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at), "n"(OFF));
 }
-__device__ inline void load_matrices_trans(uint32_t (&r)[2], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at));
+template <int OFF> __device__ inline void load_matrices_trans(uint32_t (&r)[2], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2 + %3];" : "=r"(r[0]), "=r"(r[1]) : "r"(at), "n"(OFF));
+}
+template <int OFF> __device__ inline void load_shared(uint32_t (&w)[1], uint32_t at) { asm volatile("ld.shared.b32 %0, [%1 + %2];" : "=r"(w[0]) : "r"(at), "n"(OFF)); }
+template <int OFF> __device__ inline void load_shared(uint32_t (&w)[2], uint32_t at) {
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2 + %3];" : "=r"(w[0]), "=r"(w[1]) : "r"(at), "n"(OFF));
+}
+template <int OFF> __device__ inline void load_shared(uint32_t (&w)[4], uint32_t at) {
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at), "n"(OFF));
+}
+template <int OFF> __device__ inline void load_shared(uint32_t (&w)[8], uint32_t at) {
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at), "n"(OFF));
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "r"(at), "n"(OFF + 16));
+}
+// f(integral_constant) for 0 .. N - 1: loops whose counters are immediates.
+template <int N, int I = 0, class F> __device__ inline void each(F f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        each<N, I + 1>(f);
+    }
 }
 template <bool F16> __device__ inline void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (F16)
@@ -149,15 +174,6 @@ template <bool F16> __device__ inline void mma(float (&d)[4], const uint32_t (&a
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// A row's words of scales.
-template <int N> __device__ inline void load_scales(uint32_t (&w)[N], const uint32_t *p) {
-    if constexpr (N == 1) w[0] = p[0];
-    else if constexpr (N == 2) *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(p);
-    else {
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i) reinterpret_cast<uint4 *>(w)[i] = reinterpret_cast<const uint4 *>(p)[i];
-    }
 }
 __device__ inline float exp2_fast(float v) {  // 2 ulp; exp2(-inf) = 0
     float r;
@@ -210,16 +226,66 @@ template <class S> __device__ inline int k_chunk_at(int r, int c) {
 template <int BYTES> __device__ inline void store_nan(uint32_t to) {
     for (int i = 0; i < BYTES; i += 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + i), "r"(0x7fc07fc0u) : "memory");
 }
-// Passes I .. N - 1 of PASS rows each of a run, K and V.  A place in pass i is the first one's with the turn of its rows, and a constant: a tile starts
-// at a multiple of 128 bytes, and where rows are shorter than that a pass is whole turns.
-template <class S, int PASS, int I, int N>
-__device__ inline void copy_rows(uint32_t k_to, uint32_t v_to, const uint8_t *k, const uint8_t *v, uint64_t step) {
+// Sixteen rows, PASS of them at a time, K and V.  A place in a later pass is the first one's with the turn of its rows, and a constant: a tile starts
+// at a multiple of 128 bytes, and where rows are shorter than that a pass is whole turns.  Rows that follow each other in memory (NEXT) have constant
+// distances there too.  Of an EDGE only the rows from .. to - 1 are there, the others become zeros.
+template <class S, int PASS, int OFF, bool NEXT, bool EDGE>
+__device__ inline void copy_rows(uint32_t k_to, uint32_t v_to, const uint8_t *k, const uint8_t *v, uint64_t step, int row, int from, int to) {
     static_assert((S::CR >= 8 || PASS % 8 == 0) && S::kPart % 128 == 0 && S::kRows % 128 == 0, "");
-    if constexpr (I < N) {
-        constexpr int kTurn = S::CR >= 8 ? I * PASS & 7 : 0, kTurnK = S::BITS == 8 ? 2 * (kTurn & 3) : kTurn;
-        copy_async<16, I * PASS * S::RB>(k_to ^ (kTurnK << 4), k);
-        copy_async<16, I * PASS * S::RB>(v_to ^ (kTurn << 4), v);
-        copy_rows<S, PASS, I + 1, N>(k_to, v_to, k + step, v + step, step);
+    each<16 / PASS>([&](auto i) {
+        constexpr int I = decltype(i)::value, kOff = I * PASS * S::RB, kTurn = S::CR >= 8 ? I * PASS & 7 : 0, kTurnK = S::BITS == 8 ? 2 * (kTurn & 3) : kTurn;
+        if constexpr (EDGE) {
+            const int n = row + I * PASS >= from && row + I * PASS < to ? 16 : 0;
+            copy_async<16, OFF + kOff>(k_to ^ (kTurnK << 4), k, n);
+            copy_async<16, OFF + kOff>(v_to ^ (kTurn << 4), v, n);
+        } else {
+            copy_async<16, OFF + kOff, NEXT ? kOff : 0>(k_to ^ (kTurnK << 4), k);
+            copy_async<16, OFF + kOff, NEXT ? kOff : 0>(v_to ^ (kTurn << 4), v);
+        }
+        if (!NEXT) k += step, v += step;
+    });
+}
+
+// A run of keys with a bad page, or of pages of eight tokens: each row looks its page up.  Rows out of range become zeros, the keys of a bad page NaN.
+// Out of line: the loop keeps its registers.
+template <class S>
+__device__ __noinline__ void load_ragged(const Args &a, const int32_t *table, uint32_t st, int run0, int lo, int len, int head, int b, int group_lane) {
+    constexpr int CR = S::CR, NG = S::NG, RUN = S::RUN;
+    constexpr int kPass = 32 * S::WR / CR > RUN ? RUN : 32 * S::WR / CR;
+    const int page_mask = (1 << a.c.page_shift) - 1, chunk = group_lane % CR, row = group_lane / CR;
+    auto place = [&](int r, bool &wanted) -> int64_t {  // of row r, -1: none
+        const int j = run0 + r;
+        wanted = j >= lo && j < len;
+        if (!wanted) return -1;
+        const int id = table[j >> a.c.page_shift];
+        if ((unsigned)id < (unsigned)a.c.n_pages) return kv_row(a.c, id, head, j & page_mask);
+        raise_error(a.err, (uint32_t)b, (uint32_t)id);
+        return -1;
+    };
+    if (row < kPass) {
+#pragma unroll 1
+        for (int i = 0; i < RUN / kPass; ++i) {
+            const int r = row + i * kPass;
+            bool wanted;
+            const int64_t from = place(r, wanted), off = from < 0 ? 0 : from * S::RB + chunk * 16;
+            const uint32_t to = st + k_chunk_at<S>(r, chunk) * 16;
+            if (!S::kQuant && wanted && from < 0) store_nan<16>(to);
+            else copy_async<16>(to, a.c.k + off, from < 0 ? 0 : 16);
+            copy_async<16>(st + S::kRows + chunk_at<CR>(r, chunk) * 16, a.c.v + off, from < 0 ? 0 : 16);
+        }
+    }
+    if constexpr (S::kQuant) {
+        constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = NG * 4 / kBytes;  // of a row's scales
+#pragma unroll 1
+        for (int i = group_lane; i < RUN * kPieces; i += 32 * S::WR) {
+            const int r = i / kPieces, piece = i % kPieces;
+            bool wanted;
+            const int64_t from = place(r, wanted), off = from < 0 ? 0 : from * (NG * 4) + piece * kBytes;
+            const uint32_t to = st + 2 * S::kRows + i * kBytes;
+            if (wanted && from < 0) store_nan<kBytes>(to);
+            else copy_async<kBytes>(to, reinterpret_cast<const uint8_t *>(a.c.k_sm) + off, from < 0 ? 0 : kBytes);
+            copy_async<kBytes>(to + S::kScales, reinterpret_cast<const uint8_t *>(a.c.v_sm) + off, from < 0 ? 0 : kBytes);
+        }
     }
 }
 
@@ -351,101 +417,90 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     }
     const int units = (int)(u1 - u0);
     const int shift = a.c.page_shift, page_mask = (1 << shift) - 1;
-    const int run_pages = RUN > page_mask ? RUN >> shift : 1;  // pages of a run of keys: one, or two or four that end inside it
-
-    constexpr int kPass = 32 * WR / CR > RUN ? RUN : 32 * WR / CR, kPasses = RUN / kPass;  // rows that the group's threads fetch at a time
+    constexpr int kPass = 32 * WR / CR > 16 ? 16 : 32 * WR / CR;  // rows that the group's threads fetch at a time
     constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = kQuant ? NG * 4 / kBytes : 1;  // of a row's scales
-    constexpr int kScalePass = 32 * WR / kPieces > RUN ? RUN : 32 * WR / kPieces, kScalePasses = RUN / kScalePass;
+    constexpr int kScalePass = 32 * WR / kPieces > 16 ? 16 : 32 * WR / kPieces, kScalePasses = 16 / kScalePass;
     const int l_lane = wr * 32 + lane, l_chunk = l_lane % CR, l_row = l_lane / CR, s_row = l_lane / kPieces, s_piece = l_lane % kPieces;
-    const bool l_on = l_row < kPass, s_on = s_row < kScalePass;
-    const uint32_t stages0 = smem_of(smem) + wk * S::kPart;
-    const uint32_t row_bytes = (uint32_t)a.c.row_stride * S::RB, row_words = (uint32_t)a.c.row_stride * (NG * 4);
-    const uint64_t page_bytes = (uint64_t)a.c.page_stride * S::RB, page_words = (uint64_t)a.c.page_stride * (NG * 4);
-    const int64_t k_to_v = a.c.v - a.c.k, ks_to_vs = kQuant ? reinterpret_cast<const uint8_t *>(a.c.v_sm) - reinterpret_cast<const uint8_t *>(a.c.k_sm) : 0;
-    // this lane's place in the head's first row, of the codes and of the scales; the sequence's row of the table
-    const uint8_t *l_codes, *l_scales = nullptr;
+    const uint32_t smem0 = smem_of(smem);
+    const uint32_t k_to0 = smem0 + wk * S::kPart + k_chunk_at<S>(l_row, l_chunk) * 16, v_to0 = smem0 + wk * S::kPart + S::kRows + chunk_at<CR>(l_row, l_chunk) * 16;
+    const uint32_t s_to0 = smem0 + wk * S::kPart + 2 * S::kRows + l_lane * kBytes;
+    // distances in pieces of sixteen bytes (codes) and kBytes (scales): a cache has fewer than 2^32 of either
+    const uint32_t page_chunks = (uint32_t)a.c.page_stride * CR, row_chunks = (uint32_t)a.c.row_stride * CR;
+    const uint32_t page_pieces = (uint32_t)a.c.page_stride * kPieces, row_pieces = (uint32_t)a.c.row_stride * kPieces;
+    uint32_t l_codes, l_scales;  // this lane's place in the head's first row
+    int l_run0;                  // first key of the group's run
     const int32_t *l_table;
     auto at_head = [&]() {
-        const int64_t rows = l_head * a.c.head_stride;
-        l_codes = a.c.k + (rows + l_row * a.c.row_stride) * S::RB + l_chunk * 16;
-        if constexpr (kQuant) l_scales = reinterpret_cast<const uint8_t *>(a.c.k_sm) + (rows + s_row * a.c.row_stride) * (NG * 4) + s_piece * kBytes;
+        const uint32_t rows = (uint32_t)l_head * (uint32_t)a.c.head_stride;
+        l_codes = (rows + l_row * (uint32_t)a.c.row_stride) * CR + l_chunk;
+        l_scales = (rows + s_row * (uint32_t)a.c.row_stride) * kPieces + s_piece;
+        l_run0 = (l_s.tile0 + l_at) * TK + wk * RUN;
     };
-    // The id of page number lane % run_pages of the run under the cursor; none where the sequence has no keys there.
-    auto find_page = [&]() -> int {
-        const int run0 = (l_s.tile0 + l_at) * TK + wk * RUN, first = (run0 & ~page_mask) + ((lane & (run_pages - 1)) << shift);
-        if (first >= l_s.len || (first | page_mask) < l_s.lo) return -1;
-        return l_table[first >> shift];
+    int l_page[KI];  // of the run's sixteens of keys: a page has sixteen or more, or load_ragged looks its ids up
+    auto find_pages = [&]() {
+#pragma unroll
+        for (int ki = 0; ki < KI; ++ki) {
+            const int first = l_run0 + 16 * ki;
+            l_page[ki] = first < l_s.len && first + 15 >= l_s.lo ? l_table[first >> shift] : 0;
+        }
     };
     auto advance = [&]() {
-        l_new = false;
+        l_new = false, l_run0 += TK;
         if (++l_at < l_s.tiles) return;
         l_at = 0, l_new = true, ++l_segment;
-        if (++l_row_tile < l_s.row_tiles) return;
-        l_row_tile = 0;
-        if (++l_head == a.c.n_kv) {
-            l_head = 0;
-            do {
-                if (++l_b >= a.B) return;
-                l_s = sequence<S>(a, l_b);
-            } while (l_s.n == 0);
-            l_table = a.pages + l_b * a.pages_ld;
+        if (++l_row_tile == l_s.row_tiles) {
+            l_row_tile = 0;
+            if (++l_head == a.c.n_kv) {
+                l_head = 0;
+                do {
+                    if (++l_b >= a.B) return;
+                    l_s = sequence<S>(a, l_b);
+                } while (l_s.n == 0);
+                l_table = a.pages + l_b * a.pages_ld;
+            }
         }
         at_head();
     };
-    auto load = [&](int stage, int page) {
-        const uint32_t st = stages0 + stage * S::kStage;
-        const int run0 = (l_s.tile0 + l_at) * TK + wk * RUN;
-        const bool fine = (unsigned)page < (unsigned)a.c.n_pages;
-        if (run_pages == 1 && __all_sync(0xffffffffu, fine) && run0 >= l_s.lo && run0 + RUN <= l_s.len) {
-            const uint32_t in_page = run0 & page_mask;
-            const uint8_t *k = l_codes + (uint64_t)(uint32_t)page * page_bytes + (uint64_t)in_page * row_bytes, *v = k + k_to_v;
-            const uint64_t step = (uint64_t)kPass * row_bytes;
-            if (kPass * CR == 32 * WR || l_on)
-                copy_rows<S, kPass, 0, kPasses>(st + k_chunk_at<S>(l_row, l_chunk) * 16, st + S::kRows + chunk_at<CR>(l_row, l_chunk) * 16, k, v, step);
-            if constexpr (kQuant) {
-                const uint8_t *ks = l_scales + (uint64_t)(uint32_t)page * page_words + (uint64_t)in_page * row_words;
-                const uint32_t to = st + 2 * S::kRows + l_lane * kBytes;
+    auto load = [&](int stage) {
+        const uint32_t by = stage * S::kStage;
+        if (l_run0 >= l_s.len || l_run0 + RUN <= l_s.lo) return;  // nobody sees a key of it, and the sums leave it out
+        bool fine = page_mask >= 15;
 #pragma unroll
-                for (int i = 0; i < kScalePasses; ++i) {
-                    if (kScalePass * kPieces == 32 * WR || s_on) {
-                        copy_async<kBytes>(to + i * kScalePass * NG * 4, ks);
-                        copy_async<kBytes>(to + S::kScales + i * kScalePass * NG * 4, ks + ks_to_vs);
-                    }
-                    ks += (uint64_t)kScalePass * row_words;
-                }
-            }
+        for (int ki = 0; ki < KI; ++ki) fine = fine && (unsigned)l_page[ki] < (unsigned)a.c.n_pages;
+        if (!fine) {
+            load_ragged<S>(a, l_table, smem0 + wk * S::kPart + by, l_run0, l_s.lo, l_s.len, l_head, l_b, l_lane);
             return;
         }
-        // Several pages, or a sequence's first or last run, or a bad page: rows out of range are zeros, keys of a bad page NaN.
-        if (lane < run_pages && page != -1 && !fine) raise_error(a.err, (uint32_t)l_b, (uint32_t)page);
-#pragma unroll 1
-        for (int i = 0; i < kPasses; ++i) {
-            const int r = l_row + i * kPass, j = run0 + r;
-            const int id = __shfl_sync(0xffffffffu, page, (r >> shift) & (run_pages - 1));
-            const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && (unsigned)id < (unsigned)a.c.n_pages;
-            const int64_t off = there ? (id * a.c.page_stride + l_head * a.c.head_stride + (j & page_mask) * a.c.row_stride) * S::RB + l_chunk * 16 : 0;
-            if (l_on) {
-                const uint32_t to = st + k_chunk_at<S>(r, l_chunk) * 16;
-                if (!kQuant && wanted && !there) store_nan<16>(to);
-                else copy_async<16>(to, a.c.k + off, there ? 16 : 0);
-                copy_async<16>(st + S::kRows + chunk_at<CR>(r, l_chunk) * 16, a.c.v + off, there ? 16 : 0);
+        const bool edge = l_run0 < l_s.lo || l_run0 + RUN > l_s.len;
+        const uint64_t step = (uint64_t)row_chunks * (kPass * 16);
+        each<KI>([&](auto kic) {
+            constexpr int ki = decltype(kic)::value, kOff = ki * 16 * S::RB;
+            const uint32_t in_page = (l_run0 + 16 * ki) & page_mask;
+            const uint32_t chunk = (uint32_t)l_page[ki] * page_chunks + in_page * row_chunks + l_codes;
+            const uint8_t *const k = a.c.k + (uint64_t)chunk * 16, *const v = a.c.v + (uint64_t)chunk * 16;
+            if (kPass * CR == 32 * WR || l_row < kPass) {
+                if (edge) copy_rows<S, kPass, kOff, false, true>(k_to0 + by, v_to0 + by, k, v, step, l_row, l_s.lo - l_run0 - 16 * ki, l_s.len - l_run0 - 16 * ki);
+                else if (a.c.row_stride == 1) copy_rows<S, kPass, kOff, true, false>(k_to0 + by, v_to0 + by, k, v, 0, 0, 0, 0);
+                else copy_rows<S, kPass, kOff, false, false>(k_to0 + by, v_to0 + by, k, v, step, 0, 0, 0);
             }
-        }
-        if constexpr (kQuant) {
-#pragma unroll 1
-            for (int i = 0; i < kScalePasses; ++i) {
-                const int r = s_row + i * kScalePass, j = run0 + r;
-                const int id = __shfl_sync(0xffffffffu, page, (r >> shift) & (run_pages - 1));
-                const bool wanted = j >= l_s.lo && j < l_s.len, there = wanted && (unsigned)id < (unsigned)a.c.n_pages;
-                const int64_t off = there ? (id * a.c.page_stride + l_head * a.c.head_stride + (j & page_mask) * a.c.row_stride) * (NG * 4) + s_piece * kBytes : 0;
-                if (s_on) {
-                    const uint32_t to = st + 2 * S::kRows + l_lane * kBytes + i * kScalePass * NG * 4;
-                    if (wanted && !there) store_nan<kBytes>(to);
-                    else copy_async<kBytes>(to, reinterpret_cast<const uint8_t *>(a.c.k_sm) + off, there ? kBytes : 0);
-                    copy_async<kBytes>(to + S::kScales, reinterpret_cast<const uint8_t *>(a.c.v_sm) + off, there ? kBytes : 0);
-                }
+            if constexpr (kQuant) {
+                const uint32_t piece = (uint32_t)l_page[ki] * page_pieces + in_page * row_pieces + l_scales;
+                const uint8_t *ks = reinterpret_cast<const uint8_t *>(a.c.k_sm) + (uint64_t)piece * kBytes, *vs = reinterpret_cast<const uint8_t *>(a.c.v_sm) + (uint64_t)piece * kBytes;
+                each<kScalePasses>([&](auto i) {
+                    constexpr int kTo = (ki * 16 + decltype(i)::value * kScalePass) * NG * 4;
+                    if (kScalePass * kPieces == 32 * WR || s_row < kScalePass) {
+                        const int r = l_run0 + 16 * ki + decltype(i)::value * kScalePass + s_row;
+                        if (edge) {
+                            const int n = r >= l_s.lo && r < l_s.len ? kBytes : 0;
+                            copy_async<kBytes, kTo>(s_to0 + by, ks, n), copy_async<kBytes, kTo + S::kScales>(s_to0 + by, vs, n);
+                        } else {
+                            copy_async<kBytes, kTo>(s_to0 + by, ks), copy_async<kBytes, kTo + S::kScales>(s_to0 + by, vs);
+                        }
+                    }
+                    ks += (uint64_t)row_pieces * (kScalePass * kBytes), vs += (uint64_t)row_pieces * (kScalePass * kBytes);
+                });
             }
-        }
+        });
     };
     // A segment's queries and what there is to know of it: the whole CTA's, into a ring of as many places as there are stages.
     auto load_segment = [&]() {
@@ -458,20 +513,20 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             const int64_t off = there ? (l_s.q0 + tok) * a.q_ld + (int64_t)(l_head * a.group + row - tok * a.group) * D + c * 8 : 0;
             copy_async<16>(smem_of(qs + chunk_at<D / 8>(r, c) * 16), a.q + off, there ? 16 : 0);
         }
-        if (tid == 0) segments[slot] = Segment{l_s.q0, l_s.n, l_s.len, l_s.p0, l_s.tile0, l_s.tiles, l_head, rows0, l_at, (int)l_s.bad};
+        if (tid == 0) segments[slot] = Segment{l_s.q0, l_s.n, l_s.len, l_s.p0, l_s.lo, l_s.tile0, l_s.tiles, l_head, rows0, l_at, (int)l_s.bad};
     };
 
     l_table = a.pages + l_b * a.pages_ld;
     at_head();
-    int l_page = find_page();
+    find_pages();
 #pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) {
         if (s < units) {
             if (l_new) load_segment();
-            load(s, l_page);
+            load(s);
             if (s + 1 < units) {
                 advance();
-                l_page = find_page();
+                find_pages();
             }
         }
         commit_async();
@@ -482,10 +537,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     // second product V's columns are the rows, its accumulators hold the same two queries, and the weights get from the first one's layout to the
     // second operand's by a transposition in registers.
     const int g = lane >> 2, t4 = lane & 3;
+    // Places in a run's tiles: a lane's first, of which the others differ by the exclusive or with a chunk's number and by a constant.
     const int a_row = lane & 15, a_half = lane >> 4;  // of a fragment of sixteen rows, two chunks
+    const uint32_t k_at0 = BITS == 16 ? k_chunk_at<S>(a_row, a_half) * 16 : BITS == 8 ? k_chunk_at<S>(g, t4 >> 1) * 16 + (t4 & 1) * 8 : k_chunk_at<S>(g, 0) * 16 + t4 * 4;
+    const uint32_t v_at0 = S::kRows + (BITS == 16 ? chunk_at<CR>((lane & 7) + 8 * (lane >> 4), (lane >> 3) & 1) : chunk_at<CR>(a_row, BITS == 8 ? a_half : 0)) * 16;
+    const uint32_t q_at0 = chunk_at<D / 8>(wr * NT * 8 + (lane & 7), lane >> 3) * 16;
     uint32_t qf[S::kHoldQ ? NT : 1][S::kHoldQ ? D / 16 : 1][2];
     float o[D / 16][NT][4], w_sum[S::kOffsetV ? NG : 1][NT][4], o_min[kGroups][NT][2];
     float m[NT][2], l[NT][2];
+    float qsum[S::kHoldSums ? NG : 1][NT][2];
     int v_exp = 20, at = 0, tiles = 0, whole0 = 0, whole1 = 0, segment = 0, stage = 0;
     bool fresh = true;
 
@@ -496,15 +556,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         else asm volatile("bar.sync %0, %1;" ::"r"(1 + wk), "n"(32 * WR) : "memory");
         if (i + kStages - 1 < units) {
             if (l_new) load_segment();
-            load(stage == 0 ? kStages - 1 : stage - 1, l_page);
+            load(stage == 0 ? kStages - 1 : stage - 1);
             if (i + kStages < units) {
                 advance();
-                l_page = find_page();
+                find_pages();
             }
         }
         commit_async();
 
-        uint8_t *const st = smem + stage * S::kStage + wk * S::kPart;
+        const uint32_t st = smem0 + stage * S::kStage + wk * S::kPart;
         uint8_t *const qs = q_ring + (segment % kStages) * S::kQ;
         const Segment &sg = segments[segment % kStages];
         if (fresh) {
@@ -583,89 +643,98 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 __syncthreads();
             }
             if constexpr (S::kHoldQ) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int ks = 0; ks < D / 16; ks += 2) {
+                each<NT>([&](auto nt) {
+                    each<D / 32>([&](auto k2) {
+                        constexpr int t = decltype(nt)::value, ks = 2 * decltype(k2)::value;
                         uint32_t r[4];
-                        load_matrices(r, smem_of(qs + chunk_at<D / 8>((wr * NT + nt) * 8 + (lane & 7), ks * 2 + (lane >> 3)) * 16));
-                        qf[nt][ks][0] = r[0], qf[nt][ks][1] = r[1], qf[nt][ks + 1][0] = r[2], qf[nt][ks + 1][1] = r[3];
+                        load_matrices<t * 8 * D * 2>(r, (smem_of(qs) + q_at0) ^ (ks * 32));
+                        qf[t][ks][0] = r[0], qf[t][ks][1] = r[1], qf[t][ks + 1][0] = r[2], qf[t][ks + 1][1] = r[3];
+                    });
+                });
+            }
+            if constexpr (kQuant && S::kHoldSums) {
+#pragma unroll
+                for (int grp = 0; grp < NG; ++grp)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float2 v = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
+                        qsum[grp][nt][0] = v.x, qsum[grp][nt][1] = v.y;
                     }
             }
         }
-        // q's fragments of two steps of sixteen elements
-        auto q_at = [&](int nt, int ks, uint32_t (&r)[4]) {
-            if constexpr (S::kHoldQ) r[0] = qf[nt][ks][0], r[1] = qf[nt][ks][1], r[2] = qf[nt][ks + 1][0], r[3] = qf[nt][ks + 1][1];
-            else load_matrices(r, smem_of(qs + chunk_at<D / 8>((wr * NT + nt) * 8 + (lane & 7), ks * 2 + (lane >> 3)) * 16));
+        const bool whole = at >= whole0 && at < whole1;
+        const int run0 = (sg.tile0 + at) * TK + wk * RUN;
+        if (whole || (run0 < sg.len && run0 + RUN > sg.lo)) {
+        // q's fragments of two steps of sixteen elements, from step 2 K2
+        auto q_at = [&](auto nt, auto k2, uint32_t (&r)[4]) {
+            constexpr int t = decltype(nt)::value, ks = 2 * decltype(k2)::value;
+            if constexpr (S::kHoldQ) r[0] = qf[t][ks][0], r[1] = qf[t][ks][1], r[2] = qf[t][ks + 1][0], r[3] = qf[t][ks + 1][1];
+            else load_matrices<t * 8 * D * 2>(r, (smem_of(qs) + q_at0) ^ (ks * 32));
         };
 
         // scores
         float s[KI][NT][4];
-        const auto *const k_sm = reinterpret_cast<const uint32_t *>(st + 2 * S::kRows), *const v_sm = k_sm + RUN * NG;
-#pragma unroll
-        for (int ki = 0; ki < KI; ++ki) {
-            const int key0 = ki * 16;
+        const uint32_t k_at = st + k_at0, s_at = st + 2 * S::kRows + g * (NG * 4);
+        each<KI>([&](auto kic) {
+            constexpr int ki = decltype(kic)::value, kRun = ki * 16 * S::RB;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[ki][nt][0] = s[ki][nt][1] = s[ki][nt][2] = s[ki][nt][3] = 0.f;
             if constexpr (!kQuant) {
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ks += 2) {
+                each<D / 32>([&](auto k2) {
+                    constexpr int ks = 2 * decltype(k2)::value;
                     uint32_t k0[4], k1[4];
-                    load_matrices(k0, smem_of(st + k_chunk_at<S>(key0 + a_row, ks * 2 + a_half) * 16));
-                    load_matrices(k1, smem_of(st + k_chunk_at<S>(key0 + a_row, ks * 2 + 2 + a_half) * 16));
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
+                    load_matrices<kRun>(k0, k_at ^ (ks * 32)), load_matrices<kRun>(k1, k_at ^ (ks * 32 + 32));
+                    each<NT>([&](auto nt) {
                         uint32_t q[4];
-                        q_at(nt, ks, q);
-                        mma<false>(s[ki][nt], k0, q[0], q[1]);
-                        mma<false>(s[ki][nt], k1, q[2], q[3]);
-                    }
-                }
+                        q_at(nt, k2, q);
+                        mma<false>(s[ki][decltype(nt)::value], k0, q[0], q[1]);
+                        mma<false>(s[ki][decltype(nt)::value], k1, q[2], q[3]);
+                    });
+                });
             } else {
-                uint32_t k_words[2][NG];
-                load_scales(k_words[0], k_sm + (key0 + g) * NG), load_scales(k_words[1], k_sm + (key0 + g + 8) * NG);
-#pragma unroll
-                for (int grp = 0; grp < NG; ++grp) {
+                uint32_t words[2][NG];
+                load_shared<ki * 16 * NG * 4>(words[0], s_at), load_shared<(ki * 16 + 8) * NG * 4>(words[1], s_at);
+                each<NG>([&](auto grpc) {
+                    constexpr int grp = decltype(grpc)::value;
                     float part[NT][4] = {};
-#pragma unroll
-                    for (int run = 0; run < S::G / 32; ++run) {
-                        const int blk = grp * (S::G / 32) + run;
+                    each<S::G / 32>([&](auto run) {
+                        constexpr int blk = grp * (S::G / 32) + decltype(run)::value;
                         uint32_t k0[4], k1[4];
                         if constexpr (BITS == 8) {
-                            const uint2 w0 = *reinterpret_cast<const uint2 *>(st + k_chunk_at<S>(key0 + g, blk * 2 + (t4 >> 1)) * 16 + (t4 & 1) * 8);
-                            const uint2 w1 = *reinterpret_cast<const uint2 *>(st + k_chunk_at<S>(key0 + g + 8, blk * 2 + (t4 >> 1)) * 16 + (t4 & 1) * 8);
-                            k0[0] = bytes_f16(w0.x, 0x4140), k0[1] = bytes_f16(w1.x, 0x4140), k0[2] = bytes_f16(w0.x, 0x4342), k0[3] = bytes_f16(w1.x, 0x4342);
-                            k1[0] = bytes_f16(w0.y, 0x4140), k1[1] = bytes_f16(w1.y, 0x4140), k1[2] = bytes_f16(w0.y, 0x4342), k1[3] = bytes_f16(w1.y, 0x4342);
+                            uint32_t w0[2], w1[2];
+                            load_shared<kRun>(w0, k_at ^ (blk * 32)), load_shared<kRun + 8 * S::RB>(w1, k_at ^ (blk * 32));
+                            k0[0] = bytes_f16(w0[0], 0x4140), k0[1] = bytes_f16(w1[0], 0x4140), k0[2] = bytes_f16(w0[0], 0x4342), k0[3] = bytes_f16(w1[0], 0x4342);
+                            k1[0] = bytes_f16(w0[1], 0x4140), k1[1] = bytes_f16(w1[1], 0x4140), k1[2] = bytes_f16(w0[1], 0x4342), k1[3] = bytes_f16(w1[1], 0x4342);
                         } else {
-                            const uint32_t w0 = *reinterpret_cast<const uint32_t *>(st + k_chunk_at<S>(key0 + g, blk) * 16 + t4 * 4);
-                            const uint32_t w1 = *reinterpret_cast<const uint32_t *>(st + k_chunk_at<S>(key0 + g + 8, blk) * 16 + t4 * 4);
-                            k0[0] = nibbles_f16(w0 << 4), k0[1] = nibbles_f16(w1 << 4), k0[2] = nibbles_f16(w0), k0[3] = nibbles_f16(w1);
-                            k1[0] = nibbles_f16(w0 >> 4), k1[1] = nibbles_f16(w1 >> 4), k1[2] = nibbles_f16(w0 >> 8), k1[3] = nibbles_f16(w1 >> 8);
+                            uint32_t w0[1], w1[1];
+                            load_shared<kRun>(w0, k_at ^ (blk * 16)), load_shared<kRun + 8 * S::RB>(w1, k_at ^ (blk * 16));
+                            k0[0] = nibbles_f16(w0[0] << 4), k0[1] = nibbles_f16(w1[0] << 4), k0[2] = nibbles_f16(w0[0]), k0[3] = nibbles_f16(w1[0]);
+                            k1[0] = nibbles_f16(w0[0] >> 4), k1[1] = nibbles_f16(w1[0] >> 4), k1[2] = nibbles_f16(w0[0] >> 8), k1[3] = nibbles_f16(w1[0] >> 8);
                         }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
+                        each<NT>([&](auto nt) {
                             uint32_t q[4];
-                            q_at(nt, blk * 2, q);
-                            mma<true>(part[nt], k0, q[0], q[1]);
-                            mma<true>(part[nt], k1, q[2], q[3]);
-                        }
-                    }
+                            q_at(nt, std::integral_constant<int, blk>{}, q);
+                            mma<true>(part[decltype(nt)::value], k0, q[0], q[1]);
+                            mma<true>(part[decltype(nt)::value], k1, q[2], q[3]);
+                        });
+                    });
                     float sc[2], mn[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint32_t w = k_words[e][grp];
-                        sc[e] = __uint_as_float(w << 16);
-                        mn[e] = fmaf(-S::kOffset, sc[e], __uint_as_float(w & 0xffff0000u));
+                        sc[e] = __uint_as_float(words[e][grp] << 16);
+                        mn[e] = fmaf(-S::kOffset, sc[e], __uint_as_float(words[e][grp] & 0xffff0000u));
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        const float2 q_sum = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
+                        float2 q_sum;
+                        if constexpr (S::kHoldSums) q_sum = make_float2(qsum[grp][nt][0], qsum[grp][nt][1]);
+                        else q_sum = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(sc[e >> 1], part[nt][e], fmaf(mn[e >> 1], e & 1 ? q_sum.y : q_sum.x, s[ki][nt][e]));
                     }
-                }
+                });
             }
-        }
+        });
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const float2 f = *reinterpret_cast<const float2 *>(q_factor + (wr * NT + nt) * 8 + 2 * t4);
@@ -684,10 +753,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(-2.f * to, reciprocal_fast(exp2_fast(s[ki][nt][e] * by) + 1.f), to);
         }
-        const bool whole = at >= whole0 && at < whole1;
         uint32_t hidden = 0;  // bit (ki * NT + nt) * 4 + e: that query does not see that key
         if (!whole) {
-            const int j0 = (sg.tile0 + at) * TK + wk * RUN + g;
+            const int j0 = run0 + g;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -724,11 +792,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         bool odd = false;  // a scale or a min among them is none, and there are rows that must not hear of it
         if constexpr (kQuant) {
             float v_top = 0.f;
+            each<KI>([&](auto ki) {
+                constexpr int kOff = S::kScales + decltype(ki)::value * 16 * NG * 4;
+                load_shared<kOff>(v_words[decltype(ki)::value][0], s_at), load_shared<kOff + 8 * NG * 4>(v_words[decltype(ki)::value][1], s_at);
+            });
 #pragma unroll
             for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    load_scales(v_words[ki][e], v_sm + (ki * 16 + g + 8 * e) * NG);
 #pragma unroll
                     for (int grp = 0; grp < NG; ++grp) v_top = fmaxf(v_top, fabsf(__uint_as_float(v_words[ki][e][grp] << 16)));
                 }
@@ -798,37 +869,40 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 }
 
         // weights times values
-        const uint8_t *const vt = st + S::kRows;
+        const uint32_t v_at = st + v_at0;
         if constexpr (!kQuant) {
+            // Keys that one row sees and another does not: an infinity or a NaN there must not reach the other through 0 * v.
+            bool clean = true;
+            if (!whole && sg.n > 1) {
+                const uint8_t *const vt = smem + stage * S::kStage + wk * S::kPart + S::kRows;
+                for (int c = lane; c < RUN * CR; c += 32) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(vt + c * 16);
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int ki = 0; ki < KI; ++ki) {
-                const int key0 = ki * 16;
-                // Keys that one row sees and another does not: an infinity or a NaN there must not reach the other through 0 * v.
-                bool clean = true;
-                if (!whole && sg.n > 1) {
-                    for (int c = lane; c < 16 * CR; c += 32) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(vt + (key0 * CR + c) * 16);
-                        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) clean = clean && (ws[e] & 0x7f80u) != 0x7f80u && (ws[e] & 0x7f800000u) != 0x7f800000u;
-                    }
-                    clean = __all_sync(0xffffffffu, clean);
+                    for (int e = 0; e < 4; ++e) clean = clean && (ws[e] & 0x7f80u) != 0x7f80u && (ws[e] & 0x7f800000u) != 0x7f800000u;
                 }
-                if (clean) {
+                clean = __all_sync(0xffffffffu, clean);
+            }
+            if (clean) {
+                each<KI>([&](auto kic) {
+                    constexpr int ki = decltype(kic)::value, kRun = ki * 16 * S::RB;
                     uint32_t p[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         p[nt][0] = transposed(pack_bf16(s[ki][nt][0], s[ki][nt][1]));
                         p[nt][1] = transposed(pack_bf16(s[ki][nt][2], s[ki][nt][3]));
                     }
+                    each<D / 16>([&](auto d) {  // columns 0 - 7 and 8 - 15 of keys 0 - 7, then of keys 8 - 15
+                        uint32_t v[4];
+                        load_matrices_trans<kRun>(v, v_at ^ (decltype(d)::value * 32));
 #pragma unroll
-                    for (int d = 0; d < D / 16; ++d) {
-                        uint32_t v[4];  // columns 0 - 7 and 8 - 15 of keys 0 - 7, then of keys 8 - 15
-                        load_matrices_trans(v, smem_of(vt + chunk_at<CR>(key0 + (lane & 7) + 8 * (lane >> 4), d * 2 + ((lane >> 3) & 1)) * 16));
+                        for (int nt = 0; nt < NT; ++nt) mma<false>(o[decltype(d)::value][nt], v, p[nt][0], p[nt][1]);
+                    });
+                });
+            } else {
+                const uint8_t *const vt = smem + stage * S::kStage + wk * S::kPart + S::kRows;
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma<false>(o[d][nt], v, p[nt][0], p[nt][1]);
-                    }
-                } else {
+                for (int ki = 0; ki < KI; ++ki)
 #pragma unroll 1
                     for (int k = 0; k < 16; ++k) {
                         const int from = (k % 8) * 4 + t4;
@@ -845,7 +919,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                         for (int d = 0; d < D / 16; ++d) {
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
-                                const float v = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(vt + chunk_at<CR>(key0 + k, 2 * d + half) * 16 + g * 2));
+                                const float v = bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(vt + chunk_at<CR>(ki * 16 + k, 2 * d + half) * 16 + g * 2));
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -854,21 +928,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                             }
                         }
                     }
-                }
             }
         } else {
             const float v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);  // 2^(14 - kSlack - (v_exp - 127))
-#pragma unroll
-            for (int ki = 0; ki < KI; ++ki) {
-                const int key0 = ki * 16;
-#pragma unroll
-                for (int grp = 0; grp < NG; ++grp) {
+            each<KI>([&](auto kic) {
+                constexpr int ki = decltype(kic)::value, kRun = ki * 16 * S::RB;
+                each<NG>([&](auto grpc) {
+                    constexpr int grp = decltype(grpc)::value;
                     float sc[2], mn[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t x = v_words[ki][e][grp];
-                        sc[e] = __uint_as_float(x << 16) * v_up, mn[e] = __uint_as_float(x & 0xffff0000u);
-                    }
+                    for (int e = 0; e < 2; ++e) sc[e] = __uint_as_float(v_words[ki][e][grp] << 16) * v_up, mn[e] = __uint_as_float(v_words[ki][e][grp] & 0xffff0000u);
                     uint32_t p[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -891,17 +960,17 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                         }
                         p[nt][0] = transposed(pack_f16(w[0], w[1])), p[nt][1] = transposed(pack_f16(w[2], w[3]));
                         if constexpr (S::kOffsetV) {
-                            constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-                            mma<true>(w_sum[grp][nt], kOnes, p[nt][0], p[nt][1]);
+                            const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+                            mma<true>(w_sum[grp][nt], ones, p[nt][0], p[nt][1]);
                         }
                     }
                     auto code = [](uint32_t v) { return S::kOffsetV ? v : less_offset<BITS>(v); };
-#pragma unroll
-                    for (int run = 0; run < S::G / 32; ++run) {
+                    each<S::G / 32>([&](auto runc) {
+                        constexpr int run = decltype(runc)::value;
                         if constexpr (BITS == 8) {  // two chunks of sixteen columns, the even ones rows 0 - 7 of a fragment, the odd ones rows 8 - 15
-                            const int c = grp * (S::G / 16) + run * 2;
+                            constexpr int c = grp * (S::G / 16) + run * 2;
                             uint32_t v[4];
-                            load_matrices_trans(v, smem_of(vt + chunk_at<CR>(key0 + a_row, c + a_half) * 16));
+                            load_matrices_trans<kRun>(v, v_at ^ (c * 16));
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
                                 const uint32_t va[4] = {code(bytes_f16(v[2 * x], 0x4240)), code(bytes_f16(v[2 * x], 0x4341)), code(bytes_f16(v[2 * x + 1], 0x4240)),
@@ -910,17 +979,18 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                                 for (int nt = 0; nt < NT; ++nt) mma<true>(o[c + x][nt], va, p[nt][0], p[nt][1]);
                             }
                         } else {  // a chunk of 32 columns: 4 n and 4 n + 1 in the first fragment, 4 n + 2 and 4 n + 3 in the second
-                            const int c = grp * (S::G / 32) + run;
+                            constexpr int c = grp * (S::G / 32) + run;
                             uint32_t v[2];
-                            load_matrices_trans(v, smem_of(vt + chunk_at<CR>(key0 + a_row, c) * 16));
+                            load_matrices_trans<kRun>(v, v_at ^ (c * 16));
                             const uint32_t va[4] = {code(nibbles_f16(v[0] << 4)), code(nibbles_f16(v[0])), code(nibbles_f16(v[1] << 4)), code(nibbles_f16(v[1]))};
                             const uint32_t vb[4] = {code(nibbles_f16(v[0] >> 4)), code(nibbles_f16(v[0] >> 8)), code(nibbles_f16(v[1] >> 4)), code(nibbles_f16(v[1] >> 8))};
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) mma<true>(o[2 * c][nt], va, p[nt][0], p[nt][1]), mma<true>(o[2 * c + 1][nt], vb, p[nt][0], p[nt][1]);
                         }
-                    }
-                }
-            }
+                    });
+                });
+            });
+        }
         }
         uint8_t *const stage_base = smem + stage * S::kStage;
         stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -1088,8 +1158,14 @@ template <class S> struct Launch {
         a.count = static_cast<uint32_t *>(ws);
         a.joins = reinterpret_cast<Join *>(a.count + (size_t)sm_count() * kMostPerSm);
         a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + counter_bytes());
-        const cudaError_t rc = cudaFuncSetAttribute(attn_decode_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-        if (rc != cudaSuccess) return rc;
+        static std::atomic<uint64_t> told{0};  // devices that know of the kernel's shared memory, a bit each
+        int dev = 0;
+        if (const cudaError_t rc = cudaGetDevice(&dev); rc != cudaSuccess) return rc;
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if ((told.load(std::memory_order_acquire) & bit) == 0) {
+            if (const cudaError_t rc = cudaFuncSetAttribute(attn_decode_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); rc != cudaSuccess) return rc;
+            told.fetch_or(bit, std::memory_order_release);
+        }
         const cudaError_t rc2 = launch_behind(attn_decode_kernel<S>, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a);
         if (S::kJoinHere || rc2 != cudaSuccess) return rc2;
         return launch_behind(attn_join_kernel<S>, dim3((unsigned)n, S::R / kJoinRows), dim3(kJoinRows * S::D / 4), 0, st, 1, a);
@@ -1139,10 +1215,17 @@ extern "C" size_t sxb_attn_decode_workspace_bytes(int64_t n_q, int64_t n_kv, int
     return most;
 }
 
-extern "C" int sxb_attn_decode(const void *q, int64_t q_ld, int64_t T, int64_t n_q, const SxbKvCache *cache, const int32_t *pages, int64_t pages_ld,
-                               int64_t n_cols, const int32_t *q_start, const int32_t *kv_len, int64_t B, int64_t max_q, float scale, float softcap,
-                               int64_t window, void *out, int64_t out_ld, float *lse, void *ws, size_t ws_bytes, uint32_t *err, sxb_stream_t stream) {
+extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t stream) {
     const char *fn = "attn_decode";
+    SXB_CHECK(args != nullptr, fn, ": null argument block");
+    const SxbKvCache *const cache = args->cache;
+    const void *const q = args->q;
+    void *const out = args->out, *const ws = args->ws;
+    const int32_t *const pages = args->pages, *const q_start = args->q_start, *const kv_len = args->kv_len;
+    const int64_t q_ld = args->q_ld, out_ld = args->out_ld, T = args->T, n_q = args->n_q, pages_ld = args->pages_ld, n_cols = args->n_cols, B = args->B;
+    const int64_t max_q = args->max_q, window = args->window;
+    const float scale = args->scale, softcap = args->softcap;
+    uint32_t *const err = args->err;
     Args a{};
     if (int rc = kv_view(fn, cache, &a.c)) return rc;
     SXB_CHECK(q != nullptr && out != nullptr && pages != nullptr && q_start != nullptr && kv_len != nullptr && ws != nullptr && err != nullptr, fn,
@@ -1164,10 +1247,10 @@ extern "C" int sxb_attn_decode(const void *q, int64_t q_ld, int64_t T, int64_t n
     SXB_CHECK(window >= 0 && window < (1ll << 31), fn, ": window = ", window, ", expected 0 (none) .. 2^31 - 1");
     const int rows = tile_rows(max_q * (n_q / n_kv));
     const size_t need = sxb_attn_decode_workspace_bytes(n_q, n_kv, D, cache->bits, max_q);
-    SXB_CHECK(ws_bytes >= need, fn, ": workspace of ", ws_bytes, " bytes, needs ", need);
+    SXB_CHECK(args->ws_bytes >= need, fn, ": workspace of ", args->ws_bytes, " bytes, needs ", need);
     a.q = static_cast<const uint16_t *>(q), a.q_ld = q_ld, a.pages = pages, a.pages_ld = pages_ld, a.capacity = n_cols * cache->page;
     a.q_start = q_start, a.kv_len = kv_len, a.B = (int)B, a.T = (int)T, a.n_q = (int)n_q, a.group = (int)(n_q / n_kv), a.window = (int)window;
-    a.scale = scale, a.softcap = softcap, a.out = static_cast<uint16_t *>(out), a.out_ld = out_ld, a.lse = lse, a.err = err;
+    a.scale = scale, a.softcap = softcap, a.out = static_cast<uint16_t *>(out), a.out_ld = out_ld, a.lse = args->lse, a.err = err;
     auto st = static_cast<cudaStream_t>(stream);
     const cudaError_t rc = with_shape(D, cache->bits, cache->G, rows, [&](auto s) {
         using S = decltype(s);

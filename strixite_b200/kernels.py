@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import enum
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
@@ -454,6 +455,7 @@ def _on(dev, what: str, **tensors):
 
 _I32, _F32, _ROWS = (torch.int32,), (torch.float32,), (torch.bfloat16, torch.float32)
 _BF16 = (torch.bfloat16,)
+_WORDS = (torch.int32, torch.uint32)
 
 
 class KvCache:
@@ -495,7 +497,7 @@ class KvCache:
         self.k, self.v, self.k_sm, self.v_sm = k, v, k_sm, v_sm
         self._c = _lib.SxbKvCache(k.data_ptr(), v.data_ptr(), _ptr(k_sm), _ptr(v_sm), self.n_pages, self.n_kv, self.page, self.D, self.G,
                                   *[int(r) for r in rows], bits)
-        self._by_ref = C.byref(self._c)
+        self.index, self._at = k.get_device(), C.addressof(self._c)
 
     @classmethod
     def empty(cls, n_pages: int, n_kv: int, page: int, D: int, bits: int, G: int = 64, device="cuda") -> "KvCache":
@@ -512,47 +514,75 @@ class KvCache:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_sm, self.v_sm) if t is not None)
 
 
-def _places(what: str, cache: KvCache, seq, pos, pages, err, T: int):
-    _on(cache.device, what, seq=(seq, _I32), pos=(pos, _I32), pages=(pages, _I32), err=(err, (torch.int32, torch.uint32)))
-    if pages.dim() != 2 or seq.shape != (T,) or pos.shape != (T,):
-        raise Error(1, f"{what}: pages {tuple(pages.shape)}, seq {tuple(seq.shape)}, pos {tuple(pos.shape)}, expected [n_seq, n_cols] and [{T}] twice")
+# The argument blocks of include/strix_b200.h, field for field (native alignment): packed and passed as one pointer, a call of twenty arguments costs
+# ctypes more than the smallest kernel takes.
+_WRITE_ARGS = struct.Struct("@PqqqPPPqPPPqqqPPqPfii")
+_READ_ARGS = struct.Struct("@PPPPqqqqPPPi")
+_DECODE_ARGS = struct.Struct("@PqqqPPqqPPqqPqPPNPqff")
 
 
-def _here(cache: KvCache, what: str):
-    if cache.device.index != torch.cuda.current_device():
+def _rows(t: torch.Tensor) -> int:
+    """Elements from one row of a matrix to the next."""
+    return t.shape[1] if t.is_contiguous() else t.stride(0)
+
+
+def _refuse(cache, what, **tensors):
+    """A call's tensors are not what the kernels take them for: says which one."""
+    if cache.index != torch.cuda.current_device():
         raise Error(1, f"{what}: the cache lives on {cache.device}, the current device is {torch.cuda.current_device()}")
+    _on(cache.device, what, **tensors)
+    raise Error(1, f"{what}: a vector is not contiguous, or the shapes do not fit: " + ", ".join(f"{n} {tuple(t.shape)}" for n, (t, _) in tensors.items() if t is not None))
+
+
+def _places_ok(cache, seq, pos, pages, err, T):
+    dev = cache.index
+    return (seq.dtype is torch.int32 and pos.dtype is torch.int32 and pages.dtype is torch.int32 and err.dtype in _WORDS and seq.get_device() == dev
+            and pos.get_device() == dev and pages.get_device() == dev and err.get_device() == dev and seq.is_contiguous() and pos.is_contiguous()
+            and err.is_contiguous() and pages.dim() == 2 and (pages.is_contiguous() or pages.stride(1) == 1) and seq.numel() == T and pos.numel() == T
+            and err.numel() >= 3)
 
 
 def attn_qkv_write(qkv, cache: KvCache, seq, pos, pages, q_out, err, q_norm=None, k_norm=None, eps=1e-6, inv_freq=None, interleaved=False, stream=None):
     """sxb_attn_qkv_write: qkv [T, (n_q + 2 n_kv) D] BF16 or FP32 -> queries normed and rotated into q_out [T, n_q D] BF16, keys and values into the
     cache at position pos [T] of sequence seq [T] (int32; seq < 0: a padding row), pages [n_seq, n_cols] int32.  q_norm, k_norm [D] FP32 or None;
     inv_freq [rot / 2] FP32 or None.  err: 3 or more zeroed int32."""
-    what = "attn_qkv_write"
-    T, D = qkv.shape[0], cache.D
-    _here(cache, what)
-    _places(what, cache, seq, pos, pages, err, T)
-    _on(cache.device, what, qkv=(qkv, _ROWS), q_out=(q_out, _BF16), q_norm=(q_norm, _F32), k_norm=(k_norm, _F32), inv_freq=(inv_freq, _F32))
-    n_q, rest = divmod(qkv.shape[1] - 2 * cache.n_kv * D, D)
-    if rest or n_q < 1 or tuple(q_out.shape) != (T, n_q * D) or any(w is not None and w.shape != (D,) for w in (q_norm, k_norm)):
-        raise Error(1, f"{what}: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)} or a norm weight does not fit {cache.n_kv} key heads of {D}")
-    _check(_lib.load().sxb_attn_qkv_write(_ptr(qkv), qkv.stride(0) if T > 1 else qkv.shape[1], 0 if qkv.dtype == torch.float32 else 1, T, n_q, _ptr(q_norm), _ptr(k_norm),
-                                          eps, _ptr(inv_freq), 0 if inv_freq is None else 2 * inv_freq.numel(), int(bool(interleaved)), _ptr(seq),
-                                          _ptr(pos), _ptr(pages), pages.stride(0) if pages.shape[0] > 1 else pages.shape[1], pages.shape[1], pages.shape[0], cache._by_ref, _ptr(q_out),
-                                          q_out.stride(0) if T > 1 else q_out.shape[1], _ptr(err), _stream(stream)))
+    T, width = qkv.shape
+    D, dev, dt = cache.D, cache.index, qkv.dtype
+    n_q = width // D - 2 * cache.n_kv
+    rot = qn = kn = fr = 0
+    ok = (dev == torch._C._cuda_getDevice() and dt in _ROWS and q_out.dtype is torch.bfloat16 and qkv.get_device() == dev and q_out.get_device() == dev
+          and width % D == 0 and n_q >= 1 and q_out.shape == (T, n_q * D) and (qkv.is_contiguous() or qkv.stride(1) == 1)
+          and (q_out.is_contiguous() or q_out.stride(1) == 1) and _places_ok(cache, seq, pos, pages, err, T))
+    if q_norm is not None:
+        ok = ok and q_norm.dtype is torch.float32 and q_norm.get_device() == dev and q_norm.is_contiguous() and q_norm.numel() == D
+        qn = q_norm.data_ptr()
+    if k_norm is not None:
+        ok = ok and k_norm.dtype is torch.float32 and k_norm.get_device() == dev and k_norm.is_contiguous() and k_norm.numel() == D
+        kn = k_norm.data_ptr()
+    if inv_freq is not None:
+        ok = ok and inv_freq.dtype is torch.float32 and inv_freq.get_device() == dev and inv_freq.is_contiguous()
+        rot, fr = 2 * inv_freq.numel(), inv_freq.data_ptr()
+    if not ok:
+        _refuse(cache, "attn_qkv_write", qkv=(qkv, _ROWS), q_out=(q_out, _BF16), q_norm=(q_norm, _F32), k_norm=(k_norm, _F32), inv_freq=(inv_freq, _F32),
+                seq=(seq, _I32), pos=(pos, _I32), pages=(pages, _I32), err=(err, _WORDS))
+    n_seq, n_cols = pages.shape
+    _check(_lib.load().sxb_attn_qkv_write(_WRITE_ARGS.pack(
+        qkv.data_ptr(), _rows(qkv), T, n_q, qn, kn, fr, rot, seq.data_ptr(), pos.data_ptr(), pages.data_ptr(), _rows(pages), n_cols, n_seq, cache._at,
+        q_out.data_ptr(), _rows(q_out), err.data_ptr(), eps, dt is torch.bfloat16, bool(interleaved)), _stream(stream)))
 
 
 def kv_read(cache: KvCache, seq, pos, pages, k_out, v_out, err, stream=None):
     """sxb_kv_read: positions pos [T] of sequences seq [T] of the cache -> k_out, v_out [T, n_kv, D], BF16 or FP32."""
-    what = "kv_read"
-    T = seq.shape[0]
-    _here(cache, what)
-    _places(what, cache, seq, pos, pages, err, T)
-    _on(cache.device, what, k_out=(k_out, _ROWS), v_out=(v_out, (k_out.dtype,)))
-    for t in (k_out, v_out):
-        if tuple(t.shape) != (T, cache.n_kv, cache.D) or not t.is_contiguous():
-            raise Error(1, f"{what}: outputs {tuple(k_out.shape)} and {tuple(v_out.shape)}, expected contiguous {(T, cache.n_kv, cache.D)}")
-    _check(_lib.load().sxb_kv_read(cache._by_ref, _ptr(seq), _ptr(pos), _ptr(pages), pages.stride(0) if pages.shape[0] > 1 else pages.shape[1], pages.shape[1], pages.shape[0], T, _ptr(k_out),
-                                   _ptr(v_out), 0 if k_out.dtype == torch.float32 else 1, _ptr(err), _stream(stream)))
+    T, dev, dt = seq.shape[0], cache.index, k_out.dtype
+    shape = (T, cache.n_kv, cache.D)
+    if not (dev == torch._C._cuda_getDevice() and dt in _ROWS and v_out.dtype is dt and k_out.get_device() == dev and v_out.get_device() == dev
+            and k_out.shape == shape and v_out.shape == shape and k_out.is_contiguous() and v_out.is_contiguous()
+            and _places_ok(cache, seq, pos, pages, err, T)):
+        _refuse(cache, "kv_read", k_out=(k_out, _ROWS), v_out=(v_out, (dt,)), seq=(seq, _I32), pos=(pos, _I32), pages=(pages, _I32), err=(err, _WORDS))
+    n_seq, n_cols = pages.shape
+    _check(_lib.load().sxb_kv_read(_READ_ARGS.pack(
+        cache._at, seq.data_ptr(), pos.data_ptr(), pages.data_ptr(), _rows(pages), n_cols, n_seq, T, k_out.data_ptr(), v_out.data_ptr(), err.data_ptr(),
+        dt is torch.bfloat16), _stream(stream)))
 
 
 def attn_decode_workspace_bytes(cache: KvCache, n_q: int, max_q: int) -> int:
@@ -567,19 +597,25 @@ def attn_decode(q, cache: KvCache, pages, q_start, kv_len, max_q, out, ws, err, 
     """sxb_attn_decode: q [T, n_q D] BF16, rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]) the new tokens of sequence b, kv_len [B] int32 its
     keys, their own included -> out [T, n_q D] BF16, lse [T, n_q] FP32.  scale: None = D ** -0.5; softcap, window: 0 = none.  max_q: a
     sequence's largest count of new tokens."""
-    what = "attn_decode"
-    T, B, D = q.shape[0], kv_len.shape[0], cache.D
-    _here(cache, what)
-    _on(cache.device, what, q=(q, _BF16), out=(out, _BF16), pages=(pages, _I32), q_start=(q_start, _I32), kv_len=(kv_len, _I32), lse=(lse, _F32),
-        err=(err, (torch.int32, torch.uint32)), ws=(ws, (ws.dtype,)))
-    n_q, rest = divmod(q.shape[1], D)
-    if rest or out.shape != q.shape or pages.dim() != 2 or pages.shape[0] < B or q_start.shape != (B + 1,) or \
-            (lse is not None and (tuple(lse.shape) != (T, n_q) or not lse.is_contiguous())):
-        raise Error(1, f"{what}: q {tuple(q.shape)}, out {tuple(out.shape)}, pages {tuple(pages.shape)}, q_start {tuple(q_start.shape)}, kv_len "
-                       f"{tuple(kv_len.shape)} or lse do not fit heads of {D}")
-    _check(_lib.load().sxb_attn_decode(_ptr(q), q.stride(0) if T > 1 else q.shape[1], T, n_q, cache._by_ref, _ptr(pages), pages.stride(0) if pages.shape[0] > 1 else pages.shape[1], pages.shape[1], _ptr(q_start), _ptr(kv_len), B,
-                                       max_q, D ** -0.5 if scale is None else scale, softcap, window, _ptr(out), out.stride(0) if T > 1 else out.shape[1], _ptr(lse), _ptr(ws),
-                                       ws.numel() * ws.element_size(), _ptr(err), _stream(stream)))
+    T, width = q.shape
+    D, dev, B = cache.D, cache.index, kv_len.shape[0]
+    n_q = width // D
+    if not (dev == torch._C._cuda_getDevice() and q.dtype is torch.bfloat16 and out.dtype is torch.bfloat16 and pages.dtype is torch.int32
+            and q_start.dtype is torch.int32 and kv_len.dtype is torch.int32 and err.dtype in _WORDS and q.get_device() == dev and out.get_device() == dev
+            and pages.get_device() == dev and q_start.get_device() == dev and kv_len.get_device() == dev and ws.get_device() == dev
+            and err.get_device() == dev and width % D == 0 and out.shape == (T, width) and pages.dim() == 2 and pages.shape[0] >= B
+            and q_start.numel() == B + 1 and (q.is_contiguous() or q.stride(1) == 1) and (out.is_contiguous() or out.stride(1) == 1)
+            and (pages.is_contiguous() or pages.stride(1) == 1) and q_start.is_contiguous() and kv_len.is_contiguous() and ws.is_contiguous()
+            and err.is_contiguous() and err.numel() >= 3
+            and (lse is None or (lse.dtype is torch.float32 and lse.get_device() == dev and lse.shape == (T, n_q) and lse.is_contiguous()))):
+        _refuse(cache, "attn_decode", q=(q, _BF16), out=(out, _BF16), pages=(pages, _I32), q_start=(q_start, _I32), kv_len=(kv_len, _I32), lse=(lse, _F32),
+                ws=(ws, (ws.dtype,)), err=(err, _WORDS))
+    if max_q * (n_q // cache.n_kv) > 16:
+        _count()  # the parts of split sequences are joined by a second kernel
+    _check(_lib.load().sxb_attn_decode(_DECODE_ARGS.pack(
+        q.data_ptr(), _rows(q), T, n_q, cache._at, pages.data_ptr(), _rows(pages), pages.shape[1], q_start.data_ptr(), kv_len.data_ptr(), B, max_q,
+        out.data_ptr(), _rows(out), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(), err.data_ptr(), window,
+        D ** -0.5 if scale is None else scale, softcap), _stream(stream)))
 
 
 def check_attn_error(err, what: str):
