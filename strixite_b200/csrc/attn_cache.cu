@@ -10,12 +10,15 @@
 // The same formulas as sxb_quantize's make the codes (formats/q4.cpp:44-88), from the FP32 values: nothing is rounded on the way.
 
 #include "attn.cuh"
+#include "skinny_mma.cuh"
+
+#include <type_traits>
 
 namespace sxb {
 namespace {
 
-constexpr int kWriteWarps = 8, kWriteThreads = 32 * kWriteWarps;
-constexpr int64_t kMaxTokens = 1ll << 24;
+constexpr int kWriteWarps = 4, kWriteThreads = 32 * kWriteWarps;
+constexpr int64_t kMaxTokens = 1ll << 20;
 
 struct WriteArgs {
     const void *qkv;
@@ -25,7 +28,8 @@ struct WriteArgs {
     float eps;
     const int32_t *seq, *pos, *pages;
     int64_t pages_ld;
-    int n_seq, n_cols, G, items_per_cta;
+    int n_seq, n_cols, G, items_per_warp, warps_per_token;
+    int64_t T;
     KvView c;
     uint16_t *q_out;
     int64_t q_ld;
@@ -123,118 +127,126 @@ __device__ inline Place find_place(int seq, int pos, const int32_t *pages, int64
     return p;
 }
 
-// An item is the heads that a warp takes at once: the queries' items, then the keys', then the values'.
+// An item is the heads that a warp takes at once: the queries' items, then the keys', then the values'.  A warp has a run of one token's items, all of
+// them where there are many tokens, and the token's angles to itself.
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(kWriteThreads) qkv_write_kernel(const __grid_constant__ WriteArgs a) {
-    __shared__ float2 turn[D / 2];  // cos, sin of the token's angles
-    constexpr int kLanes = D / 8, kHeads = 32 / kLanes, kBatch = 4;
+    constexpr int kLanes = D / 8, kHeads = 32 / kLanes, kBatch = 4, kCols = D / 16;
+    __shared__ float2 turns[kWriteWarps][D / 2];  // cos, sin of angle i at [i % 8][i / 8]: lanes have eights
     behind_grid();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane % kLanes, sub = lane / kLanes;
-    const int64_t t = blockIdx.x;
-    const int q_items = (a.n_q + kHeads - 1) / kHeads, kv_items = (a.n_kv + kHeads - 1) / kHeads;
-    const int first = blockIdx.y * a.items_per_cta, last = min(q_items + 2 * kv_items, first + a.items_per_cta);
-    const T *const row = static_cast<const T *>(a.qkv) + t * a.ld + part * 8;
-    // kind 0, 1, 2: queries, keys, values; this lane's head of that kind, none at an item's ragged end
-    auto which = [&](int item, int &kind, int &head) {
-        kind = item < q_items ? 0 : item < q_items + kv_items ? 1 : 2;
-        head = (item - (kind == 0 ? 0 : kind == 1 ? q_items : q_items + kv_items)) * kHeads + sub;
-        return item < last && head < (kind == 0 ? a.n_q : a.n_kv);
-    };
-    Words<8 * (int)sizeof(T)> raw[kBatch];
-    auto fetch = [&](int base) {  // a batch's loads side by side
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            int kind, head;
-            if (which(base + b * kWriteWarps + warp, kind, head)) raw[b] = load_words<8 * (int)sizeof(T)>(row + (int64_t)((kind == 0 ? 0 : kind == 1 ? a.n_q : a.n_q + a.n_kv) + head) * D);
-            else raw[b] = {};
-        }
-    };
-    fetch(first);
+    const int64_t unit = (int64_t)blockIdx.x * kWriteWarps + warp, t = unit / a.warps_per_token;
+    if (t >= a.T) return;
+    const int first = (int)(unit - t * a.warps_per_token) * a.items_per_warp, last = first + a.items_per_warp;
     const int seq = a.seq[t], pos = a.pos[t];
     const Place place = find_place(seq, pos, a.pages, a.pages_ld, a.n_seq, a.n_cols, a.c);
     if (place.state == 1) return;
-    if (place.state == 2 && threadIdx.x == 0 && first == 0) raise_error(a.err, (uint32_t)t, (uint32_t)pos);
-    const int half = a.rot / 2;
-    if ((int)threadIdx.x < half) {
-        // the angle less whole turns: what is left of 2^31 * inv_freq in FP64 is good to 2^-22 of a radian, of 2^20 * 1 to 2^-33
-        const double angle = (double)pos * (double)a.inv_freq[threadIdx.x];
-        const double turns = rint(angle * 0.15915494309189533577);
-        float s, c;
-        sincosf((float)fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, angle)), &s, &c);
-        turn[threadIdx.x] = make_float2(c, s);
-    }
-    __syncthreads();
-    const bool turned = part * 8 < a.rot, low = part * 8 < half;
-    const int partner = turned && !a.interleaved ? (low ? part + half / 8 : part - half / 8) : part;  // half is a multiple of 8
-    float by[8], cross[8];
-    int have = -1;
-    for (int base = first; base < last; base += kBatch * kWriteWarps) {
-        if (base != first) fetch(base);
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const int item = base + b * kWriteWarps + warp;
-            if (item >= last) break;
-            int kind, head;
-            const bool on = which(item, kind, head);
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[b].w[i]);
-                else v[i] = __uint_as_float(i & 1 ? raw[b].w[i / 2] & 0xffff0000u : raw[b].w[i / 2] << 16);
-            }
-            if (kind != 2) {
-                const float *const w = kind == 0 ? a.q_norm : a.k_norm;
-                if (kind != have) {
-                    have = kind;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) by[i] = 1.f, cross[i] = 0.f;
-                    if (w != nullptr) load_run<float, 8>(w + part * 8, by);
-                    if (turned) {
-                        float by_other[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) by_other[i] = a.interleaved ? by[i ^ 1] : 1.f;
-                        if (w != nullptr && !a.interleaved) load_run<float, 8>(w + partner * 8, by_other);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) cross[i] = by_other[i];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int e = part * 8 + i;
-                            const float2 cs = turn[a.interleaved ? e / 2 : low ? e : e - half];
-                            by[i] *= cs.x, cross[i] *= (a.interleaved ? i % 2 == 0 : low) ? -cs.y : cs.y;
-                        }
-                    }
-                }
-                float inv = 1.f;
-                if (w != nullptr) {
-                    float sum = v[0] * v[0];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
-#pragma unroll
-                    for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-                    inv = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
-                }
-                if (a.rot != 0) {
-                    float other[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) other[i] = a.interleaved ? v[i ^ 1] : __shfl_sync(0xffffffffu, v[i], partner, kLanes);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = inv * fmaf(v[i], by[i], other[i] * cross[i]);
-                } else if (w != nullptr) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = inv * (v[i] * by[i]);
-                }
-            }
-            if (kind == 0) {
-                if (place.state == 2) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = qnan_f32();
-                }
-                if (on) store_bf16_run(a.q_out + t * a.q_ld + (int64_t)head * D + part * 8, v);
-            } else if (place.state == 0) {
-                store_run<D, BITS>(kind == 1 ? a.c.k : a.c.v, kind == 1 ? a.c.k_sm : a.c.v_sm, kv_row(a.c, place.page, on ? head : 0, place.at), v, part, a.G, on);
-            }
+    if (place.state == 2 && lane == 0 && first == 0) raise_error(a.err, (uint32_t)t, (uint32_t)pos);
+    const int half = a.rot / 2, kv_items = (a.n_kv + kHeads - 1) / kHeads, q_items = (a.n_q + kHeads - 1) / kHeads;
+    float2 *const turn = turns[warp];
+    if (first < q_items + kv_items) {
+        for (int i = lane; i < half; i += 32) {
+            // the angle less whole turns: what is left of 2^31 * inv_freq in FP64 is good to 2^-22 of a radian, of 2^20 * 1 to 2^-33
+            const double angle = (double)pos * (double)a.inv_freq[i];
+            const double whole = rint(angle * 0.15915494309189533577);
+            float s, c;
+            sincosf((float)fma(-whole, 2.4492935982947064e-16, fma(-whole, 6.283185307179586, angle)), &s, &c);
+            turn[(i & 7) * kCols + (i >> 3)] = make_float2(c, s);
         }
     }
+    __syncwarp();
+    const bool turned = part * 8 < a.rot, low = part * 8 < half;
+    const int partner = turned && !a.interleaved ? (low ? part + half / 8 : part - half / 8) : part;  // half is a multiple of 8
+    // kind 0, 1, 2: queries, keys, values; `before` items and `heads_before` heads of other kinds come first
+    auto take = [&](auto kindc, int before, int n_items, int heads_before, int n_heads) {
+        constexpr int kind = decltype(kindc)::value;
+        const int from = max(first - before, 0), to = min(last - before, n_items);
+        if (from >= to) return;
+        const float *const w = kind == 0 ? a.q_norm : a.k_norm;
+        uint64_t by[4], cross[4];  // factors of an element and of its partner, as pairs
+        if constexpr (kind != 2) {
+            float x[8], y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 1.f, y[i] = 1.f;
+            if (w != nullptr) load_run<float, 8>(w + part * 8, x), load_run<float, 8>(w + partner * 8, y);
+            float2 cs[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = a.interleaved ? part * 4 + i / 2 : low ? part * 8 + i : part * 8 + i - half;
+                cs[i] = turned ? turn[(e & 7) * kCols + (e >> 3)] : make_float2(1.f, 0.f);
+                if (a.interleaved ? i % 2 == 0 : low) cs[i].y = -cs[i].y;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                by[i] = pair(x[2 * i] * cs[2 * i].x, x[2 * i + 1] * cs[2 * i + 1].x);
+                cross[i] = a.interleaved ? pair(x[2 * i + 1] * cs[2 * i].y, x[2 * i] * cs[2 * i + 1].y) : pair(y[2 * i] * cs[2 * i].y, y[2 * i + 1] * cs[2 * i + 1].y);
+            }
+        }
+        const T *src = static_cast<const T *>(a.qkv) + t * a.ld + (int64_t)(heads_before + from * kHeads + sub) * D + part * 8;
+        for (int item = from; item < to; item += kBatch) {
+            Words<8 * (int)sizeof(T)> raw[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                if (item + b < to && (item + b) * kHeads + sub < n_heads) raw[b] = load_words<8 * (int)sizeof(T)>(src + b * 32 * 8);
+                else raw[b] = {};
+            src += kBatch * 32 * 8;
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                if (item + b >= to) break;
+                const int head = (item + b) * kHeads + sub;
+                const bool on = head < n_heads;
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(raw[b].w[i]);
+                    else v[i] = __uint_as_float(i & 1 ? raw[b].w[i / 2] & 0xffff0000u : raw[b].w[i / 2] << 16);
+                }
+                if constexpr (kind != 2) {
+                    uint64_t p[4], r[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
+                    float inv = 1.f;
+                    if (w != nullptr) {
+                        uint64_t sq = mul_pair(p[0], p[0]);
+#pragma unroll
+                        for (int i = 1; i < 4; ++i) sq = fma_pair(p[i], p[i], sq);
+                        float sum, odd;
+                        unpair(sq, sum, odd);
+                        sum += odd;
+#pragma unroll
+                        for (int off = kLanes / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                        inv = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
+                    }
+                    if (a.rot != 0) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint64_t other = a.interleaved ? pair(v[2 * i + 1], v[2 * i])
+                                                                 : pair(__shfl_sync(0xffffffffu, v[2 * i], partner, kLanes), __shfl_sync(0xffffffffu, v[2 * i + 1], partner, kLanes));
+                            r[i] = fma_pair(p[i], by[i], mul_pair(other, cross[i]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) r[i] = mul_pair(p[i], by[i]);
+                    }
+                    const uint64_t inv2 = pair(inv, inv);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) unpair(mul_pair(r[i], inv2), v[2 * i], v[2 * i + 1]);
+                }
+                if constexpr (kind == 0) {
+                    if (place.state == 2) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = qnan_f32();
+                    }
+                    if (on) store_bf16_run(a.q_out + t * a.q_ld + (int64_t)head * D + part * 8, v);
+                } else if (place.state == 0) {
+                    store_run<D, BITS>(kind == 1 ? a.c.k : a.c.v, kind == 1 ? a.c.k_sm : a.c.v_sm, kv_row(a.c, place.page, on ? head : 0, place.at), v, part, a.G, on);
+                }
+            }
+        }
+    };
+    take(std::integral_constant<int, 0>{}, 0, q_items, 0, a.n_q);
+    take(std::integral_constant<int, 1>{}, q_items, kv_items, a.n_q, a.n_kv);
+    take(std::integral_constant<int, 2>{}, q_items + kv_items, kv_items, a.n_q + a.n_kv, a.n_kv);
 }
 
 constexpr int kReadThreads = 256, kReadTokens = 32;
@@ -248,14 +260,14 @@ struct ReadArgs {
     uint32_t *err;
 };
 
-// The CTA's threads find the places of its tokens side by side, then read runs of eight elements: neighbouring threads neighbouring runs of a row, with
-// nothing between one load and the next.
+// The CTA's threads find the places of its tokens side by side, then read runs of sixteen elements (BF16: eight): neighbouring threads neighbouring runs of
+// a row, four rows' loads in flight a thread.
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_constant__ ReadArgs a) {
     __shared__ int64_t rows[kReadTokens];  // row number of the token's first head; kSkip, kBad
     constexpr int64_t kSkip = -1, kBad = -2;
+    constexpr int N = BITS == 16 ? 8 : 16, kBytes = N * BITS / 8, kRuns = D / N, kStep = kReadThreads / kRuns, kBatch = 4;
     behind_grid();
-    constexpr int kRuns = D / 8;
     const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
     const int tokens = (int)min((int64_t)a.tokens, a.T - t0);
     if ((int)threadIdx.x < tokens) {
@@ -266,43 +278,52 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const __grid_cons
         rows[threadIdx.x] = place.state == 0 ? kv_row(a.c, place.page, 0, place.at) : place.state == 1 ? kSkip : kBad;
     }
     __syncthreads();
-    const int run = threadIdx.x % kRuns, heads = 2 * a.c.n_kv;
+    const int run = threadIdx.x % kRuns, heads = 2 * a.c.n_kv, group = run * N / a.G, groups = D / a.G;
     int token = 0, h = threadIdx.x / kRuns;
-    const uint32_t in_row = run * BITS, group = run * 8 / a.G, groups = D / a.G;
-#pragma unroll 4
-    for (;; h += kReadThreads / kRuns) {
-        while (h >= heads) h -= heads, ++token;
-        if (token >= tokens) break;
-        const int64_t row0 = rows[token];
-        if (row0 == kSkip) continue;
-        const bool is_k = h < a.c.n_kv;
-        const int head = is_k ? h : h - a.c.n_kv;
-        float v[8];
-        if (row0 == kBad) {
+    while (h >= heads) h -= heads, ++token;
+    while (token < tokens) {
+        Words<kBytes> raw[kBatch];
+        uint32_t sm[kBatch];
+        int64_t row0[kBatch];
+        T *to[kBatch];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = qnan_f32();
-        } else {
-            const int64_t from = row0 + head * a.c.head_stride;
-            const uint8_t *p = (is_k ? a.c.k : a.c.v) + from * (D * BITS / 8) + in_row;
-            if constexpr (BITS == 16) {
-                load_run(reinterpret_cast<const uint16_t *>(p), v);
+        for (int b = 0; b < kBatch; ++b) {
+            row0[b] = token < tokens ? rows[token] : kSkip;
+            const bool is_k = h < a.c.n_kv;
+            const int head = is_k ? h : h - a.c.n_kv;
+            to[b] = static_cast<T *>(is_k ? a.k_out : a.v_out) + (((t0 + token) * a.c.n_kv + head) * D + run * N);
+            if (row0[b] >= 0) {
+                const int64_t from = row0[b] + head * a.c.head_stride;
+                raw[b] = load_words<kBytes>((is_k ? a.c.k : a.c.v) + from * (D * BITS / 8) + run * kBytes);
+                if constexpr (BITS != 16) sm[b] = (is_k ? a.c.k_sm : a.c.v_sm)[from * groups + group];
+            }
+            h += kStep;
+            while (h >= heads) h -= heads, ++token;
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (row0[b] == kSkip) continue;
+            float v[N];
+            if (row0[b] == kBad) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = qnan_f32();
+            } else if constexpr (BITS == 16) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = __uint_as_float(e & 1 ? raw[b].w[e / 2] & 0xffff0000u : raw[b].w[e / 2] << 16);
             } else {
-                const auto w = load_words<BITS>(p);
-                const uint32_t sm = (is_k ? a.c.k_sm : a.c.v_sm)[from * groups + group];
-                const float s = __uint_as_float(sm << 16), m = __uint_as_float(sm & 0xffff0000u);
+                const float s = __uint_as_float(sm[b] << 16), m = __uint_as_float(sm[b] & 0xffff0000u);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {  // a code under the exponent of 2^23 is that number plus it
-                    const uint32_t c = BITS == 8 ? __byte_perm(w.w[e / 4], 0x4b000000u, 0x7540 + e % 4) : (w.w[0] >> (4 * e) & 15u) | 0x4b000000u;
+                for (int e = 0; e < N; ++e) {  // a code under the exponent of 2^23 is that number plus it
+                    const uint32_t c = BITS == 8 ? __byte_perm(raw[b].w[e / 4], 0x4b000000u, 0x7540 + e % 4) : (raw[b].w[e / 8] >> (4 * (e % 8)) & 15u) | 0x4b000000u;
                     v[e] = fmaf(__uint_as_float(c) - 8388608.f, s, m);
                 }
             }
-        }
-        T *to = static_cast<T *>(is_k ? a.k_out : a.v_out) + (((t0 + token) * a.c.n_kv + head) * D + run * 8);
-        if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4 *>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            store_bf16_run(to, v);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int e = 0; e < N; e += 4) *reinterpret_cast<float4 *>(to[b] + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            } else {
+                store_bf16_run(to[b], v);
+            }
         }
     }
 }
@@ -332,7 +353,7 @@ int check_places(const char *fn, const int32_t *seq, const int32_t *pos, const i
                  const SxbKvCache *c, const uint32_t *err) {
     SXB_CHECK(seq != nullptr && pos != nullptr && pages != nullptr && err != nullptr, fn, ": null pointer (seq=", (const void *)seq, ", pos=",
               (const void *)pos, ", pages=", (const void *)pages, ", err=", (const void *)err, ")");
-    SXB_CHECK(T >= 1 && T <= kMaxTokens, fn, ": T = ", T, " tokens, expected 1..2^24");
+    SXB_CHECK(T >= 1 && T <= kMaxTokens, fn, ": T = ", T, " tokens, expected 1..2^20");
     SXB_CHECK(n_seq >= 1 && n_seq <= (1 << 20), fn, ": n_seq = ", n_seq, ", expected 1..2^20");
     SXB_CHECK(n_cols >= 1 && pages_ld >= n_cols, fn, ": page table of ", n_cols, " columns with a stride of ", pages_ld);
     SXB_CHECK(n_cols <= ((1ll << 31) - 1024) / c->page, fn, ": ", n_cols, " pages of ", c->page, " tokens a sequence, positions end below 2^31 - 1024");
@@ -396,12 +417,11 @@ extern "C" int sxb_attn_qkv_write(const SxbAttnQkvWriteArgs *args, sxb_stream_t 
     a.q_norm = args->q_norm, a.k_norm = args->k_norm, a.inv_freq = args->inv_freq, a.eps = args->eps;
     a.seq = args->seq, a.pos = args->pos, a.pages = args->pages, a.pages_ld = args->pages_ld, a.n_seq = (int)args->n_seq, a.n_cols = (int)args->n_cols;
     a.G = (int)(cache->bits == 16 ? D : cache->G), a.q_out = static_cast<uint16_t *>(q_out), a.q_ld = q_ld, a.err = args->err;
-    // few tokens: an item a warp, so that the SMs share them; many: a CTA has all heads of its token and its angles are computed once
+    // few tokens: an item a warp, so that the SMs share them; many: a warp has all of its token's and computes the angles once
     const int64_t per = 256 / D, items = (n_q + per - 1) / per + 2 * ((cache->n_kv + per - 1) / per);
-    const int64_t whole = (items + kWriteWarps - 1) / kWriteWarps;
-    const int64_t parts = std::min(whole, std::max<int64_t>(1, 4 * (int64_t)sm_count() / T));
-    a.items_per_cta = (int)((whole + parts - 1) / parts) * kWriteWarps;
-    const dim3 grid((unsigned)T, (unsigned)((items + a.items_per_cta - 1) / a.items_per_cta));
+    a.items_per_warp = (int)std::max<int64_t>(1, std::min(items, items * T / (24 * (int64_t)sm_count())));
+    a.warps_per_token = (int)((items + a.items_per_warp - 1) / a.items_per_warp), a.T = T;
+    const dim3 grid((unsigned)((T * a.warps_per_token + kWriteWarps - 1) / kWriteWarps));
     auto st = static_cast<cudaStream_t>(stream);
     if (act == SXB_ACT_F32) launch_write<float>(a, (int)D, cache->bits, grid, st);
     else launch_write<uint16_t>(a, (int)D, cache->bits, grid, st);

@@ -73,7 +73,7 @@ def test_null_cache_and_tables(lib, entry):
     (dict(qkv=0), "null pointer"), (dict(q_out=0), "null pointer"), (dict(seq=0), "null pointer"), (dict(act=2), "activation dtype 2"), (dict(n_q=0), "n_q = 0"),
     (dict(ld=1023), "row strides"), (dict(ld=1028), "16-byte aligned"), (dict(q_ld=516), "16-byte aligned"), (dict(q_out=(10 << 20) + 8), "16-byte aligned"),
     (dict(q_out=(5 << 20) + 512), "overlaps"), (dict(inv=0), "without inv_freq"), (dict(rot=24), "rot = 24"), (dict(rot=144), "rot = 144"), (dict(rot=-16), "rot = -16"),
-    (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(n_seq=0), "n_seq = 0"), (dict(T=(1 << 24) + 1), "T = "),
+    (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(n_seq=0), "n_seq = 0"), (dict(T=(1 << 20) + 1), "T = "),
 ])
 def test_write_refusals(lib, kw, message):
     rc, said = write(lib, **kw)
