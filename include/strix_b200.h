@@ -562,7 +562,7 @@ int sxb_kv_read(const SxbKvReadArgs *args, sxb_stream_t stream);
 /* Attention of the new tokens of B sequences over their pages.  q [T, q_ld] BF16 (n_q heads of D, as sxb_attn_qkv_write leaves them);
  * sequence b has the rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]) and kv_len[b] keys, the new tokens' own included: its row
  * i of n stands at position p = kv_len[b] - n + i and sees the keys j <= p, with window > 0 only j > p - window.  Query head h
- * reads key head h / (n_q / n_kv).  Scores scale * q . k, with softcap > 0 softcap * tanh(score / softcap).
+ * reads key head h / (n_q / n_kv).  Scores scale * q . k (scale > 0), with softcap > 0 softcap * tanh(score / softcap).
  * out [T, out_ld] BF16 = softmax(scores) . V, lse [T, n_q] FP32 (or NULL) = log of the sum of exp(score); a row that sees no key
  * (or none with a score above -1e30): 0 and -inf.  Rows outside every sequence are left as they are.  Scores, statistics and
  * sums are FP32; weights are rounded to BF16 (BF16 cache) or, times a group's scale, to F16 for the product with V.

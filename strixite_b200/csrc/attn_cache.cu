@@ -95,11 +95,18 @@ __device__ inline void store_run(uint8_t *rows, uint32_t *sm, int64_t row, const
         }
         const uint32_t s_bits = bad ? 0x7fc0u : f32_to_bf16_bits(__fdiv_rn(__fsub_rn(hi, lo), kLevels)), m_bits = bad ? 0x7fc0u : f32_to_bf16_bits(lo);
         const float s = bf16_bits_to_f32((uint16_t)s_bits), m = bf16_bits_to_f32((uint16_t)m_bits);
+        const float per = 1.f / s;
         Words<BITS> packed = {};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             uint32_t code = 0;
-            if (s > 0.f) code = (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v[i], m), s)), 0.f), kLevels);
+            if (s > 0.f) {
+                // (v - m) / s is within 2^-13 of the product with 1 / s below 256: where that is no nearer to a half, both round to the same code
+                const float d = __fsub_rn(v[i], m), x = d * per;
+                float r = rintf(x);
+                if (!(fabsf(x - r) < 0.5f - 1.f / 4096)) r = rintf(__fdiv_rn(d, s));
+                code = (uint32_t)fminf(fmaxf(r, 0.f), kLevels);
+            }
             packed.w[i * BITS / 32] |= code << (i * BITS % 32);
         }
         if (on) {

@@ -26,7 +26,6 @@ namespace sxb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kMinRun = 2;     // units a CTA takes at least
 constexpr int kMostPerSm = 4;
 constexpr int kSlack = 8;      // powers of two that a weight may be above 1
 constexpr float kLowest = -1e30f;  // below every score; a row that sees no key keeps it
@@ -52,7 +51,7 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     static constexpr int kQ = R * D * 2;
     static constexpr int kMostJoint = WK * R * 32 * 4;
     static constexpr bool kOwnJoint = kStage < kMostJoint;  // 32 columns of every warp's rows do not fit a stage
-    static constexpr int kMisc = 1024 + WK * R * 8 + R * (NG + 2) * 4 + (kOwnJoint ? kMostJoint : 0);
+    static constexpr int kMisc = 1024 + WK * R * 8 + R * (NG + 3) * 4 + (kOwnJoint ? kMostJoint : 0);
     static constexpr int kByRegisters = WR > 1 ? 1 : 2;
     static constexpr int stages(int per_sm) { return (226 * 1024 / per_sm - kMisc) / (kStage + kQ); }
     static constexpr int kPerSm = kByRegisters > 3 && stages(4) >= 3 ? 4 : kByRegisters > 2 && stages(3) >= 3 ? 3 : kByRegisters > 1 && stages(2) >= 3 ? 2 : 1;
@@ -69,7 +68,7 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     static constexpr bool kOffsetV = kQuant && NG * NT <= 4;  // for V it takes four accumulators a group and row tile
     // Few rows: the last CTA to bring its part joins them, a launch less.  Many: that CTA would read every part by itself (2 x 8 rows over 32 k keys:
     // 19 parts of 33 KB, 30 us at the end of 80), a second kernel has the rows of all segments side by side.
-    static constexpr bool kJoinHere = R <= 16;
+    static constexpr bool kJoinHere = R * D <= 8 * kThreads;  // a thread has two runs of four columns at most
     static constexpr bool kHoldSums = kQuant && NG * NT <= 4;
     static constexpr bool kHoldQ = NT * D <= 256;             // q's fragments in registers
     static_assert(kStages >= 2 && WK * WR == kWarps && KI * NT * 4 <= 32, "");
@@ -296,20 +295,32 @@ template <int R, int D> struct Parts {
     int n;
     __device__ Parts(const float *partial, int c0, int parts) : first(partial + (2 * (int64_t)c0 + 1) * R * (D + 2)), rest(partial + 2 * (int64_t)c0 * R * (D + 2)), n(parts) {}
     __device__ const float *of(int k) const { return k == 0 ? first : rest + k * kStep; }
-    __device__ float top(int k, int r) const { return __ldcg(of(k) + R * D + r); }
 };
 
-// Four columns of a row out of all parts, in the parts' order.
-template <int R, int D> __device__ inline void join_run(const Args &a, const Parts<R, D> &from, int q0, int rows0, int key_head, int r, int c4, float top) {
+// Four columns of a row out of all parts, in the parts' order, BATCH parts' loads at a time.
+template <int BATCH, int R, int D> __device__ inline void join_run(const Args &a, const Parts<R, D> &from, int q0, int rows0, int key_head, int r, int c4) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < from.n; ++k) {
-        const float *const p = from.of(k);
-        const float4 w = __ldcg(reinterpret_cast<const float4 *>(p + r * D + 4 * c4));
-        const float f = exp2_fast(__ldcg(p + R * D + r) - top);
-        sum = fmaf(__ldcg(p + R * (D + 1) + r), f, sum);
-        v.x = fmaf(w.x, f, v.x), v.y = fmaf(w.y, f, v.y), v.z = fmaf(w.z, f, v.z), v.w = fmaf(w.w, f, v.w);
+    float sum = 0.f, top = kLowest;
+    for (int k0 = 0; k0 < from.n; k0 += BATCH) {
+        float4 w[BATCH];
+        float m[BATCH], l[BATCH], now = top;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            m[k] = kLowest, l[k] = 0.f, w[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k0 + k < from.n) {
+                const float *const p = from.of(k0 + k);
+                w[k] = __ldcg(reinterpret_cast<const float4 *>(p + r * D + 4 * c4)), m[k] = __ldcg(p + R * D + r), l[k] = __ldcg(p + R * (D + 1) + r);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) now = fmaxf(now, m[k]);
+        const float before = exp2_fast(top - now);
+        v.x *= before, v.y *= before, v.z *= before, v.w *= before, sum *= before, top = now;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const float f = exp2_fast(m[k] - top);
+            sum = fmaf(l[k], f, sum), v.x = fmaf(w[k].x, f, v.x), v.y = fmaf(w[k].y, f, v.y), v.z = fmaf(w[k].z, f, v.z), v.w = fmaf(w[k].w, f, v.w);
+        }
     }
     const int tok = (rows0 + r) / a.group, head = key_head * a.group + rows0 + r - tok * a.group;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -319,19 +330,15 @@ template <int R, int D> __device__ inline void join_run(const Args &a, const Par
     if (a.lse != nullptr && c4 == 0) a.lse[(int64_t)(q0 + tok) * a.n_q + head] = sum == 0.f ? -CUDART_INF_F : fmaf(top, kLn2, logf(sum));
 }
 
-constexpr int kJoinRows = 4;
-// Block (c, y): rows 4 y .. 4 y + 3 of the segment that began in CTA c, a thread four columns.
+constexpr int kJoinRows = 8;
+// Block (c, y): rows 8 y .. 8 y + 7 of the segment that began in CTA c, a thread four columns.
 template <class S>
 __global__ void __launch_bounds__(kJoinRows * S::D / 4) attn_join_kernel(const __grid_constant__ Args a) {
     behind_grid();
     const Join j = a.joins[blockIdx.x];
     const int r = blockIdx.y * kJoinRows + threadIdx.x / (S::D / 4);
-    if (r >= j.rows || j.parts == 0) return;
-    const Parts<S::R, S::D> from(a.partial, (int)blockIdx.x, j.parts);
-    float top = kLowest;
-#pragma unroll 8
-    for (int k = 0; k < from.n; ++k) top = fmaxf(top, from.top(k, r));
-    join_run(a, from, j.q0, j.rows0, j.head, r, threadIdx.x % (S::D / 4), top);
+    if (j.parts == 0 || r >= j.rows) return;
+    join_run<8>(a, Parts<S::R, S::D>(a.partial, (int)blockIdx.x, j.parts), j.q0, j.rows0, j.head, r, threadIdx.x % (S::D / 4));
 }
 
 template <class S>
@@ -345,7 +352,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     uint8_t *const own_joint = q_ring + kStages * S::kQ, *const misc = own_joint + (S::kOwnJoint ? S::kMostJoint : 0);
     auto *const row_max = reinterpret_cast<float *>(misc);  // [WK][R]
     float *const row_sum = row_max + WK * R;                // [WK][R]
-    float *const q_factor = row_sum + WK * R;               // [R]
+    float *const row_top = row_sum + WK * R;                // [R]
+    float *const q_factor = row_top + R;                    // [R]
     float *const q_sums = q_factor + R;                     // [NG][R]
     auto *const scan = reinterpret_cast<int64_t *>(q_sums + R * (NG + (NG & 1)));  // [kWarps + 2]
     auto *const segments = reinterpret_cast<Segment *>(scan + kWarps + 2);         // [kStages]
@@ -370,7 +378,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) total += scan[w];
-    const int64_t ctas = min((int64_t)gridDim.x, (total + kMinRun - 1) / kMinRun);
+    const int64_t ctas = min((int64_t)gridDim.x, total);
     if ((int64_t)blockIdx.x >= ctas) return;
     const int64_t u0 = blockIdx.x * total / ctas, u1 = (blockIdx.x + 1) * total / ctas;
     for (int64_t base = 0, before = 0; base < a.B; base += kThreads) {
@@ -610,7 +618,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 for (int off = 1; off < kPer; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
                 const int up = min(126, 14 - ((int)(__float_as_uint(most) >> 23) - 127));
                 const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-                if (part == 0) q_factor[r] = a.scale * (a.softcap > 0.f ? 1.f : kLog2e) * __uint_as_float((uint32_t)(127 - up) << 23);
+                if (part == 0) q_factor[r] = fmaxf(a.scale * kLog2e * __uint_as_float((uint32_t)(127 - up) << 23), 1.2e-38f);  // not 0: it stands beside -inf
                 float sums[kOwn];
 #pragma unroll
                 for (int b = 0; b < kOwn; ++b) {
@@ -637,9 +645,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     for (int off = 1; off < kRuns; off <<= 1) sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], off);
                     if (blk < kBlocks && blk % kRuns == 0) q_sums[blk / kRuns * R + r] = sums[b];
                 }
-                __syncthreads();
-            } else {
-                if (tid < R) q_factor[tid] = a.scale * (a.softcap > 0.f ? 1.f : kLog2e);
                 __syncthreads();
             }
             if constexpr (S::kHoldQ) {
@@ -735,23 +740,27 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 });
             }
         });
+        // a score in powers of two is s * fac
+        float fac[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const float2 f = *reinterpret_cast<const float2 *>(q_factor + (wr * NT + nt) * 8 + 2 * t4);
-#pragma unroll
-            for (int ki = 0; ki < KI; ++ki)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[ki][nt][e] *= e & 1 ? f.y : f.x;
+            fac[nt][0] = fac[nt][1] = a.scale * kLog2e;
+            if constexpr (kQuant) {
+                const float2 f = *reinterpret_cast<const float2 *>(q_factor + (wr * NT + nt) * 8 + 2 * t4);
+                fac[nt][0] = f.x, fac[nt][1] = f.y;
+            }
         }
         if (a.softcap > 0.f) {
             // tanh x = 1 - 2 / (exp(2 x) + 1): 2^-22 of the cap, as good as a score near it is in FP32
-            const float by = 2.f * kLog2e / a.softcap, to = a.softcap * kLog2e;
+            const float by = 2.f / a.softcap, to = a.softcap * kLog2e;
 #pragma unroll
-            for (int ki = 0; ki < KI; ++ki)
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(-2.f * to, reciprocal_fast(exp2_fast(s[ki][nt][e] * by) + 1.f), to);
+                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(-2.f * to, reciprocal_fast(exp2_fast(s[ki][nt][e] * (fac[nt][e & 1] * by)) + 1.f), to);
+                fac[nt][0] = fac[nt][1] = 1.f;
+            }
         }
         uint32_t hidden = 0;  // bit (ki * NT + nt) * 4 + e: that query does not see that key
         if (!whole) {
@@ -776,8 +785,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         }
         // The maximum that the weights are relative to is moved when a score passes it by 2^kSlack only: most tiles then need no exchange between lanes and
         // no sum is touched.  The scale that the weights of quantized values are relative to, likewise.
-        bool move = false;
-        float top[NT][2];
+        float past = 0.f, top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -786,8 +794,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                 for (int ki = 1; ki < KI; ++ki) v = fmaxf(v, fmaxf(s[ki][nt][e], s[ki][nt][2 + e]));
                 top[nt][e] = v;
-                move = move || v > m[nt][e] + kSlack;
+                past = fmaxf(past, fmaf(v, fac[nt][e], -m[nt][e]));
             }
+        bool move = past > kSlack;
         uint32_t v_words[KI][2][kGroups];
         bool odd = false;  // a scale or a min among them is none, and there are rows that must not hear of it
         if constexpr (kQuant) {
@@ -823,7 +832,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     float v = top[nt][e];
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
-                    const float now = fmaxf(m[nt][e], v);
+                    const float now = fmaxf(m[nt][e], v * fac[nt][e]);
                     f[nt][e] = exp2_fast(m[nt][e] - now);
                     m[nt][e] = now, l[nt][e] *= f[nt][e];
 #pragma unroll
@@ -864,7 +873,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[ki][nt][e] = exp2_fast(s[ki][nt][e] - m[nt][e & 1]);
+                    s[ki][nt][e] = exp2_fast(fmaf(s[ki][nt][e], fac[nt][e & 1], -m[nt][e & 1]));
                     l[nt][e & 1] += s[ki][nt][e];
                 }
 
@@ -1030,21 +1039,25 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     }
         }
         __syncthreads();
-        auto factor = [&](int k, int r, float of) { return exp2_fast(row_max[k * R + r] - of); };
-        auto top_of = [&](int r) {
-            float v = row_max[r];
+        // what each group's sums of a row count for, the row's maximum and its sum of weights
+        if (tid < R) {
+            float top = row_max[tid], sum = 0.f;
 #pragma unroll
-            for (int k = 1; k < WK; ++k) v = fmaxf(v, row_max[k * R + r]);
-            return v;
-        };
+            for (int k = 1; k < WK; ++k) top = fmaxf(top, row_max[k * R + tid]);
+#pragma unroll
+            for (int k = 0; k < WK; ++k) {
+                const float f = exp2_fast(row_max[k * R + tid] - top);
+                row_max[k * R + tid] = f, sum = fmaf(row_sum[k * R + tid], f, sum);
+            }
+            row_top[tid] = top, row_sum[tid] = sum;
+        }
+        __syncthreads();
         float mine_f[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = (wr * NT + nt) * 8 + 2 * t4 + e;
-                mine_f[nt][e] = factor(wk, r, top_of(r));
-            }
+        for (int nt = 0; nt < NT; ++nt) {
+            const float2 f = *reinterpret_cast<const float2 *>(row_max + wk * R + (wr * NT + nt) * 8 + 2 * t4);
+            mine_f[nt][0] = f.x, mine_f[nt][1] = f.y;
+        }
         constexpr int DC = S::DC;
         auto *const joint = reinterpret_cast<float *>(S::kOwnJoint ? own_joint : stage_base);  // [WK][R][DC], runs of eight columns turned by the row
         float *const part = a.partial + (2 * (int64_t)blockIdx.x + (seg0 < u0 ? 0 : 1)) * R * (D + 2);
@@ -1077,13 +1090,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 const int r = x / (DC / 4), c4 = x % (DC / 4);
                 const float *const from = joint + r * DC + ((4 * c4) ^ ((r >> 1 & 3) << 3));
                 float4 v = *reinterpret_cast<const float4 *>(from);
-                const float top_r = top_of(r);
-                float sum_r = row_sum[r] * factor(0, r, top_r);
+                const float top_r = row_top[r], sum_r = row_sum[r];
 #pragma unroll
                 for (int k = 1; k < WK; ++k) {
                     const float4 w = *reinterpret_cast<const float4 *>(from + k * R * DC);
                     v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-                    sum_r = fmaf(row_sum[k * R + r], factor(k, r, top_r), sum_r);
                 }
                 if (split) {
                     *reinterpret_cast<float4 *>(part + r * D + col0 + 4 * c4) = v;
@@ -1118,22 +1129,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 if (*last) {
                     __threadfence();
                     const Parts<R, D> from(a.partial, (int)c0, (int)(c1 - c0) + 1);
-                    {   // every row's maximum: a column of threads a row, then theirs
-                        constexpr int kCols = kThreads / R;
-                        const int r = tid % R;
-                        float v = kLowest;
-#pragma unroll 4
-                        for (int k = tid / R; k < from.n; k += kCols) v = fmaxf(v, from.top(k, r));
-                        joint[tid] = v;
-                        __syncthreads();
-                        if (tid < R) {
-#pragma unroll
-                            for (int k = 1; k < kCols; ++k) v = fmaxf(v, joint[k * R + tid]);
-                            row_max[tid] = v;
-                        }
-                        __syncthreads();
-                    }
-                    for (int x = tid; x < rows * (D / 4); x += kThreads) join_run(a, from, sg.q0, sg.rows0, sg.head, x / (D / 4), x % (D / 4), row_max[x / (D / 4)]);
+                    for (int x = tid; x < rows * (D / 4); x += kThreads) join_run<8>(a, from, sg.q0, sg.rows0, sg.head, x / (D / 4), x % (D / 4));
                 }
             }
         }
@@ -1154,7 +1150,7 @@ template <class S> struct Launch {
     static int64_t ctas() { return (int64_t)sm_count() * S::kPerSm; }
     static size_t bytes() { return counter_bytes() + (size_t)(ctas() * 2 * S::R * (S::D + 2) * 4); }
     static cudaError_t run(Args a, void *ws, int64_t most_units, cudaStream_t st) {
-        const int64_t n = std::max<int64_t>(1, std::min(ctas(), (most_units + kMinRun - 1) / kMinRun));
+        const int64_t n = std::max<int64_t>(1, std::min(ctas(), most_units));
         a.count = static_cast<uint32_t *>(ws);
         a.joins = reinterpret_cast<Join *>(a.count + (size_t)sm_count() * kMostPerSm);
         a.partial = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + counter_bytes());
@@ -1242,8 +1238,8 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
               q_ld, " and ", out_ld, ", expected multiples of 8, at least n_q * D = ", n_q * D);
     SXB_CHECK(aligned16(q) && aligned16(out) && aligned16(ws), fn, ": q, out and ws must be 16-byte aligned");
     SXB_CHECK(apart(q, ((T - 1) * q_ld + n_q * D) * 2, out, ((T - 1) * out_ld + n_q * D) * 2), fn, ": out [", out, "] overlaps q [", q, "]");
-    SXB_CHECK(scale > -1e30f && scale < 1e30f, fn, ": scale must be finite");
-    SXB_CHECK(softcap >= 0.f && softcap < 1e30f, fn, ": softcap must be finite and not negative (0: none)");
+    SXB_CHECK(scale > 0.f && scale < 1e30f, fn, ": scale must be finite and positive");
+    SXB_CHECK(softcap == 0.f || (softcap >= 1e-6f && softcap < 1e30f), fn, ": softcap = ", softcap, ", expected 0 (none) or 1e-6 .. 1e30");
     SXB_CHECK(window >= 0 && window < (1ll << 31), fn, ": window = ", window, ", expected 0 (none) .. 2^31 - 1");
     const int rows = tile_rows(max_q * (n_q / n_kv));
     const size_t need = sxb_attn_decode_workspace_bytes(n_q, n_kv, D, cache->bits, max_q);
