@@ -31,12 +31,9 @@ constexpr int kSlack = 8;      // powers of two that a weight may be above 1
 constexpr float kLowest = -1e30f;  // below every score; a row that sees no key keeps it
 constexpr int64_t kMaxRows = 1ll << 24;
 
-// Runs of sixteen keys that a warp takes at a time: two or four give it independent work and share what a step costs besides.
-constexpr int key_runs(int D, int bits, int nt) {
-    const int by_size = 4096 * 8 / (16 * D * bits);  // 4 KB of keys
-    const int most = nt * D <= 128 ? 4 : nt * D <= 256 ? 2 : 1;  // registers
-    return by_size < 1 ? 1 : by_size < most ? by_size : most;
-}
+// Runs of sixteen keys that a warp takes at a time.  Two give it independent work and share what a step costs besides; the code of four does not fit the
+// instruction cache (32 sequences of 9509 keys, 4 bits: one run 173 us, two 152, four 302).
+constexpr int key_runs(int D, int bits, int nt) { return nt * D <= 256 && D * bits <= 1024 ? 2 : 1; }
 // R query rows: NT tiles of eight a warp, WR warps side by side.  The WK groups of such warps share a tile's keys, a run of KI times sixteen each, and
 // every group fetches its own run into its own ring: nothing but a segment's ends is the whole CTA's business.
 template <int D_, int BITS_, int G_, int R_> struct Shape {
@@ -1205,9 +1202,9 @@ extern "C" size_t sxb_attn_decode_workspace_bytes(int64_t n_q, int64_t n_kv, int
                    cat(fn, ": n_q = ", n_q, ", n_kv = ", n_kv, ", D = ", D, ", bits = ", bits, ", max_q = ", max_q, " unsupported"));
         return 0;
     }
-    size_t most = 0;  // of a call with fewer rows too
+    size_t most = 0;  // of a call with fewer rows too, and of any group size: how many CTAs an SM holds depends on both
     for (int rows = 8; rows <= tile_rows(max_q * (n_q / n_kv)); rows *= 2)
-        most = std::max(most, with_shape(D, bits, 32, rows, [](auto s) { return Launch<decltype(s)>::bytes(); }));
+        for (int G = 32; G <= D && G <= 128; G *= 2) most = std::max(most, with_shape(D, bits, G, rows, [](auto s) { return Launch<decltype(s)>::bytes(); }));
     return most;
 }
 
@@ -1250,6 +1247,7 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
     auto st = static_cast<cudaStream_t>(stream);
     const cudaError_t rc = with_shape(D, cache->bits, cache->G, rows, [&](auto s) {
         using S = decltype(s);
+        if (Launch<S>::bytes() > args->ws_bytes) return cudaErrorInvalidValue;  // nothing is written behind the workspace, whatever the sizes above say
         // no list is longer than every sequence at its table's end (in a product that cannot overflow: the grid is a few hundred CTAs)
         const double most = (double)((a.capacity + S::TK - 1) / S::TK) * (double)B * n_kv * (double)((T * a.group + S::R - 1) / S::R + 1);
         return Launch<S>::run(a, ws, (int64_t)std::min(most, 1e12), st);

@@ -45,6 +45,9 @@ def tables(lens, page, n_pages, seed, device):
     return torch.from_numpy(t).to(device)
 
 
+GUARD = 24 << 20  # more than a workspace: nothing may be written behind it
+
+
 class Batch:
     """A batch of sequences over a filled cache: new[b] new tokens of lens[b] keys."""
 
@@ -63,7 +66,10 @@ class Batch:
         self.out = torch.full_like(self.q, float("nan"))
         self.lse = torch.full((self.T, self.n_q), float("nan"), device=device)
         self.err = torch.zeros(4, dtype=torch.int32, device=device)
-        self.ws = torch.zeros(K().attn_decode_workspace_bytes(self.cache, self.n_q, self.max_q), dtype=torch.uint8, device=device)
+        n = K().attn_decode_workspace_bytes(self.cache, self.n_q, self.max_q)
+        self.ws_and_more = torch.zeros(n + GUARD, dtype=torch.uint8, device=device)
+        self.ws, self.guard = self.ws_and_more[:n], self.ws_and_more[n:]
+        self.guard.fill_(0xA5)
 
     def run(self, **kw):
         kw.setdefault("lse", self.lse)
@@ -71,6 +77,7 @@ class Batch:
 
     def check(self, scale=None, softcap=0.0, window=0):
         torch.cuda.synchronize()
+        assert (self.guard == 0xA5).all(), "written behind the workspace"
         assert int(self.err[0]) == 0
         D = self.cache.D
         want, lse, tol, lse_tol = plain.attend(self.q, self.cache, self.pages, self.q_start, self.kv_len, D ** -0.5 if scale is None else scale, softcap, window)
@@ -280,6 +287,16 @@ def test_attend_captured_and_replayed_with_other_lengths(cuda):
             b.out.fill_(float("nan"))
             graph.replay()
             b.check()
+
+
+@pytest.mark.parametrize("D,bits,G", FORMS)
+def test_attend_keeps_to_its_workspace(cuda, D, bits, G):
+    """Every form with all of its CTAs at work on segments that are split, in a workspace of the size asked for and not a byte more."""
+    for rows in (8, 16, 32, 64):
+        b = Batch(cuda, D, bits, G, 8, rows, [6000], [1], page=64, seed=rows)
+        b.run()
+        torch.cuda.synchronize()
+        assert (b.guard == 0xA5).all() and torch.isfinite(b.out).all() and int(b.err[0]) == 0
 
 
 @pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
