@@ -25,14 +25,16 @@
 namespace sxb {
 namespace {
 
+#define SXB_RARE(c) __builtin_expect(!!(c), 0)  // out of the loop's way: what the loop runs through has to stay in the instruction cache
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMostPerSm = 4;
 constexpr int kSlack = 8;      // powers of two that a weight may be above 1
 constexpr float kLowest = -1e30f;  // below every score; a row that sees no key keeps it
 constexpr int64_t kMaxRows = 1ll << 24;
 
-// Runs of sixteen keys that a warp takes at a time.  Two give it independent work and share what a step costs besides; the code of four does not fit the
-// instruction cache (32 sequences of 9509 keys, 4 bits: one run 173 us, two 152, four 302).
+// Runs of sixteen keys that a warp takes at a time: two give it independent work and share what a step costs besides, where registers allow.  (Two in a
+// loop, one after the other, are slower: 32 sequences of 9509 keys, 8 bits, 115 us side by side, 132 to 152 in turn.)
 constexpr int key_runs(int D, int bits, int nt) { return nt * D <= 256 && D * bits <= 1024 ? 2 : 1; }
 // R query rows: NT tiles of eight a warp, WR warps side by side.  The WK groups of such warps share a tile's keys, a run of KI times sixteen each, and
 // every group fetches its own run into its own ring: nothing but a segment's ends is the whole CTA's business.
@@ -48,10 +50,12 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     static constexpr int kQ = R * D * 2;
     static constexpr int kMostJoint = WK * R * 32 * 4;
     static constexpr bool kOwnJoint = kStage < kMostJoint;  // 32 columns of every warp's rows do not fit a stage
-    static constexpr int kMisc = 1024 + WK * R * 8 + R * (NG + 3) * 4 + (kOwnJoint ? kMostJoint : 0);
-    static constexpr int kByRegisters = WR > 1 ? 1 : 2;
+    static constexpr int kMisc = 1024 + kWarps * 64 + WK * R * 8 + R * (2 * NG + 2) * 4 + (kOwnJoint ? kMostJoint : 0);
+    // CTAs an SM: as many as registers allow (three of four warps with 168 registers a thread, two with 255), if their rings then still have 64 KB on the way
+    static constexpr int kByRegisters = WR > 1 ? 1 : kQuant && NT * D <= 128 ? 3 : 2;
     static constexpr int stages(int per_sm) { return (226 * 1024 / per_sm - kMisc) / (kStage + kQ); }
-    static constexpr int kPerSm = kByRegisters > 3 && stages(4) >= 3 ? 4 : kByRegisters > 2 && stages(3) >= 3 ? 3 : kByRegisters > 1 && stages(2) >= 3 ? 2 : 1;
+    static constexpr bool fits(int per_sm) { return kByRegisters >= per_sm && stages(per_sm) >= 2 && per_sm * (stages(per_sm) - 1) * kStage >= 64 * 1024; }
+    static constexpr int kPerSm = fits(3) ? 3 : fits(2) ? 2 : 1;
     static constexpr int kStages = stages(kPerSm) > 6 ? 6 : stages(kPerSm);
     static constexpr int kSmem = kStages * (kStage + kQ) + kMisc;
     static constexpr int fit_columns() {
@@ -60,14 +64,13 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
         return dc;
     }
     static constexpr int DC = fit_columns();  // columns that the warps join at a time
-    // Codes stay 1024 (8 bits) or 64 (4 bits) too large as F16 operands, and what that adds is taken out of the sums
-    static constexpr float kOffset = BITS == 8 ? 1024.f : 64.f;
-    static constexpr bool kOffsetV = kQuant && NG * NT <= 4;  // for V it takes four accumulators a group and row tile
+    // Codes stay too large by so much as F16 operands, and what that adds is taken out of the sums: K's by 1024 (8 bits) or 64, V's too, but for every
+    // second 4-bit code, which 1024 saves a shift - what that costs a score (an offset of a hundred times the codes) would be seen, of an output it is not.
+    static constexpr float kOffsetK = BITS == 8 ? 1024.f : 64.f, kOffset = 1024.f, kOffsetOdd = kOffsetK;
     // Few rows: the last CTA to bring its part joins them, a launch less.  Many: that CTA would read every part by itself (2 x 8 rows over 32 k keys:
     // 19 parts of 33 KB, 30 us at the end of 80), a second kernel has the rows of all segments side by side.
     static constexpr bool kJoinHere = R * D <= 8 * kThreads;  // a thread has two runs of four columns at most
-    static constexpr bool kHoldSums = kQuant && NG * NT <= 4;
-    static constexpr bool kHoldQ = NT * D <= 256;             // q's fragments in registers
+    static constexpr bool kHoldQ = !kQuant && NT * D <= 256;  // q's fragments in registers
     static_assert(kStages >= 2 && WK * WR == kWarps && KI * NT * 4 <= 32, "");
 };
 
@@ -84,6 +87,8 @@ struct Args {
     float *lse, *partial;
     uint32_t *count, *err;
     struct Join *joins;
+    // distances in pieces of sixteen bytes (codes) and of a row's scales: a cache has fewer than 2^32 of either
+    uint32_t page_chunks, head_chunks, row_chunks, page_pieces, head_pieces, row_pieces;
 };
 
 // A split segment whose first part is the CTA's of the same number; parts = 0: that CTA began none.
@@ -117,6 +122,12 @@ template <class S> __device__ inline Sequence sequence(const Args &a, int b) {
 // A segment of the list that this CTA has units of.
 struct Segment {
     int q0, n, len, p0, lo, tile0, tiles, head, rows0, at, bad;  // rows0: first row of the tile, at: the CTA's first unit's place in the segment
+};
+
+// Where a warp's loads are: in shared memory, what is looked at in the loop apart.
+struct Cursor {
+    Sequence s;
+    int b, head, row_tile, segment;
 };
 
 __device__ inline uint32_t smem_of(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -191,14 +202,11 @@ __device__ inline uint32_t pack_f16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Two bytes of a word (named by the selector's nibbles 0 and 2) as F16 numbers 1024 + code; two nibbles (bits 4 to 7 of each half) as 64 + code.
+// Two bytes of a word (named by the selector's nibbles 0 and 2) as F16 numbers 1024 + code; the lowest nibble of each half as 1024 + code, the next one as
+// 64 + code.
 __device__ inline uint32_t bytes_f16(uint32_t w, uint32_t selector) { return __byte_perm(w, 0x64646464u, selector); }
-__device__ inline uint32_t nibbles_f16(uint32_t w) { return (w & 0x00f000f0u) | 0x54005400u; }
-// The same less the offset: exact.
-template <int BITS> __device__ inline uint32_t less_offset(uint32_t v) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&v), __half2half2(__ushort_as_half(BITS == 8 ? 0x6400 : 0x5400)));
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
+__device__ inline uint32_t low_nibbles_f16(uint32_t w) { return (w & 0x000f000fu) | 0x64006400u; }
+__device__ inline uint32_t next_nibbles_f16(uint32_t w) { return (w & 0x00f000f0u) | 0x54005400u; }
 __device__ inline uint32_t transposed(uint32_t v) {  // of an 8 x 8 tile of 16-bit numbers, a lane's two neighbours in a row
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -217,6 +225,15 @@ template <class S> __device__ inline int k_chunk_at(int r, int c) {
     else if constexpr (S::BITS == 8) return r * S::CR + (c ^ (2 * ((r >> 1) & 1)));
     else return chunk_at<S::CR>(r, c);
 }
+
+// The words of a lane's two keys of run KI, V's.
+template <class S, int KI, int N> __device__ inline void value_words(uint32_t (&w)[2][N], uint32_t scales) {
+    constexpr int kOff = S::kScales + KI * 16 * N * 4;
+    load_shared<kOff>(w[0], scales), load_shared<kOff + 8 * N * 4>(w[1], scales);
+}
+
+// Whether a group's scale or min is an infinity or a NaN.
+__device__ inline bool none_of(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
 // BF16 NaN throughout.
 template <int BYTES> __device__ inline void store_nan(uint32_t to) {
@@ -351,9 +368,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     float *const row_sum = row_max + WK * R;                // [WK][R]
     float *const row_top = row_sum + WK * R;                // [R]
     float *const q_factor = row_top + R;                    // [R]
-    float *const q_sums = q_factor + R;                     // [NG][R]
-    auto *const scan = reinterpret_cast<int64_t *>(q_sums + R * (NG + (NG & 1)));  // [kWarps + 2]
-    auto *const segments = reinterpret_cast<Segment *>(scan + kWarps + 2);         // [kStages]
+    float *const q_sums = q_factor + R;                     // [NG][R]: a group's sum of q, then what the codes' offsets add to its dot, less
+    float *const q_extra = q_sums + NG * R;                 // [NG][R]
+    auto *const scan = reinterpret_cast<int64_t *>(q_extra + R * NG);  // [kWarps + 2]
+    auto *const list = scan + kWarps + 2;                                           // [4]: this CTA's first and last unit, all units, CTAs
+    auto *const segments = reinterpret_cast<Segment *>(list + 4);                  // [kStages]
+    Cursor &cur = reinterpret_cast<Cursor *>(segments + kStages)[threadIdx.x >> 5];  // [kWarps]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int wr = warp % WR, wk = warp / WR;
 
@@ -410,18 +430,18 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     __syncthreads();
 
     // ---- the cursor of the loads: kStages - 1 units ahead of the sums ----
-    int l_b = (int)scan[kWarps], l_head, l_row_tile, l_at, l_segment = 0;
-    Sequence l_s = sequence<S>(a, l_b);
-    bool l_new = true;
+    const int64_t in = scan[kWarps + 1];
     {
-        const int64_t in = scan[kWarps + 1];
-        const int64_t per_head = (int64_t)l_s.tiles * l_s.row_tiles;
-        l_head = (int)(in / per_head);
-        const int64_t rest = in - l_head * per_head;
-        l_row_tile = (int)(rest / l_s.tiles), l_at = (int)(rest % l_s.tiles);
+        Cursor c;
+        c.b = (int)scan[kWarps], c.s = sequence<S>(a, c.b), c.segment = 0;
+        const int64_t per_head = (int64_t)c.s.tiles * c.s.row_tiles;
+        c.head = (int)(in / per_head), c.row_tile = (int)((in - c.head * per_head) / c.s.tiles);
+        if (lane == 0) cur = c;
+        if (tid == 0) list[0] = u0, list[1] = u1, list[2] = total, list[3] = ctas;
     }
+    __syncthreads();
     const int units = (int)(u1 - u0);
-    const int shift = a.c.page_shift, page_mask = (1 << shift) - 1;
+    const int page_mask = (1 << a.c.page_shift) - 1;
     constexpr int kPass = 32 * WR / CR > 16 ? 16 : 32 * WR / CR;  // rows that the group's threads fetch at a time
     constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = kQuant ? NG * 4 / kBytes : 1;  // of a row's scales
     constexpr int kScalePass = 32 * WR / kPieces > 16 ? 16 : 32 * WR / kPieces, kScalePasses = 16 / kScalePass;
@@ -429,105 +449,103 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     const uint32_t smem0 = smem_of(smem);
     const uint32_t k_to0 = smem0 + wk * S::kPart + k_chunk_at<S>(l_row, l_chunk) * 16, v_to0 = smem0 + wk * S::kPart + S::kRows + chunk_at<CR>(l_row, l_chunk) * 16;
     const uint32_t s_to0 = smem0 + wk * S::kPart + 2 * S::kRows + l_lane * kBytes;
-    // distances in pieces of sixteen bytes (codes) and kBytes (scales): a cache has fewer than 2^32 of either
-    const uint32_t page_chunks = (uint32_t)a.c.page_stride * CR, row_chunks = (uint32_t)a.c.row_stride * CR;
-    const uint32_t page_pieces = (uint32_t)a.c.page_stride * kPieces, row_pieces = (uint32_t)a.c.row_stride * kPieces;
-    uint32_t l_codes, l_scales;  // this lane's place in the head's first row
-    int l_run0;                  // first key of the group's run
+    uint32_t l_codes, l_scales;             // this lane's place in the head's first row
+    int l_run0, l_lo, l_len, l_tiles;       // first key of the group's run; the sequence's keys; tiles of the segment from here on
     const int32_t *l_table;
-    auto at_head = [&]() {
-        const uint32_t rows = (uint32_t)l_head * (uint32_t)a.c.head_stride;
-        l_codes = (rows + l_row * (uint32_t)a.c.row_stride) * CR + l_chunk;
-        l_scales = (rows + s_row * (uint32_t)a.c.row_stride) * kPieces + s_piece;
-        l_run0 = (l_s.tile0 + l_at) * TK + wk * RUN;
+    bool l_new;                             // the run begins a segment
+    auto at_segment = [&](int at) {         // the cursor stands at tile `at` of its segment
+        l_codes = cur.head * a.head_chunks + l_row * a.row_chunks + l_chunk;
+        l_scales = cur.head * a.head_pieces + s_row * a.row_pieces + s_piece;
+        l_run0 = (cur.s.tile0 + at) * TK + wk * RUN, l_lo = cur.s.lo, l_len = cur.s.len, l_tiles = cur.s.tiles - at;
+        l_table = a.pages + cur.b * a.pages_ld;
+        l_new = true;
     };
     int l_page[KI];  // of the run's sixteens of keys: a page has sixteen or more, or load_ragged looks its ids up
     auto find_pages = [&]() {
 #pragma unroll
         for (int ki = 0; ki < KI; ++ki) {
             const int first = l_run0 + 16 * ki;
-            l_page[ki] = first < l_s.len && first + 15 >= l_s.lo ? l_table[first >> shift] : 0;
+            l_page[ki] = first < l_len && first + 15 >= l_lo ? l_table[first >> a.c.page_shift] : 0;
         }
     };
     auto advance = [&]() {
         l_new = false, l_run0 += TK;
-        if (++l_at < l_s.tiles) return;
-        l_at = 0, l_new = true, ++l_segment;
-        if (++l_row_tile == l_s.row_tiles) {
-            l_row_tile = 0;
-            if (++l_head == a.c.n_kv) {
-                l_head = 0;
+        if (__builtin_expect(--l_tiles > 0, 1)) return;
+        Cursor c = cur;
+        ++c.segment;
+        if (++c.row_tile == c.s.row_tiles) {
+            c.row_tile = 0;
+            if (++c.head == a.c.n_kv) {
+                c.head = 0;
                 do {
-                    if (++l_b >= a.B) return;
-                    l_s = sequence<S>(a, l_b);
-                } while (l_s.n == 0);
-                l_table = a.pages + l_b * a.pages_ld;
+                    if (++c.b >= a.B) return;
+                    c.s = sequence<S>(a, c.b);
+                } while (c.s.n == 0);
             }
         }
-        at_head();
+        __syncwarp();
+        if (lane == 0) cur = c;
+        __syncwarp();
+        at_segment(0);
     };
     auto load = [&](int stage) {
         const uint32_t by = stage * S::kStage;
-        if (l_run0 >= l_s.len || l_run0 + RUN <= l_s.lo) return;  // nobody sees a key of it, and the sums leave it out
+        if (l_run0 >= l_len || l_run0 + RUN <= l_lo) return;  // nobody sees a key of it, and the sums leave it out
         bool fine = page_mask >= 15;
 #pragma unroll
         for (int ki = 0; ki < KI; ++ki) fine = fine && (unsigned)l_page[ki] < (unsigned)a.c.n_pages;
-        if (!fine) {
-            load_ragged<S>(a, l_table, smem0 + wk * S::kPart + by, l_run0, l_s.lo, l_s.len, l_head, l_b, l_lane);
+        if (SXB_RARE(!fine)) {
+            load_ragged<S>(a, l_table, smem0 + wk * S::kPart + by, l_run0, l_lo, l_len, cur.head, cur.b, l_lane);
             return;
         }
-        const bool edge = l_run0 < l_s.lo || l_run0 + RUN > l_s.len;
-        const uint64_t step = (uint64_t)row_chunks * (kPass * 16);
+        const bool edge = l_run0 < l_lo || l_run0 + RUN > l_len;
+        const uint64_t step = (uint64_t)a.row_chunks * (kPass * 16);
         each<KI>([&](auto kic) {
             constexpr int ki = decltype(kic)::value, kOff = ki * 16 * S::RB;
             const uint32_t in_page = (l_run0 + 16 * ki) & page_mask;
-            const uint32_t chunk = (uint32_t)l_page[ki] * page_chunks + in_page * row_chunks + l_codes;
+            const uint32_t chunk = (uint32_t)l_page[ki] * a.page_chunks + in_page * a.row_chunks + l_codes;
             const uint8_t *const k = a.c.k + (uint64_t)chunk * 16, *const v = a.c.v + (uint64_t)chunk * 16;
             if (kPass * CR == 32 * WR || l_row < kPass) {
-                if (edge) copy_rows<S, kPass, kOff, false, true>(k_to0 + by, v_to0 + by, k, v, step, l_row, l_s.lo - l_run0 - 16 * ki, l_s.len - l_run0 - 16 * ki);
-                else if (a.c.row_stride == 1) copy_rows<S, kPass, kOff, true, false>(k_to0 + by, v_to0 + by, k, v, 0, 0, 0, 0);
-                else copy_rows<S, kPass, kOff, false, false>(k_to0 + by, v_to0 + by, k, v, step, 0, 0, 0);
+                if (SXB_RARE(edge)) copy_rows<S, kPass, kOff, false, true>(k_to0 + by, v_to0 + by, k, v, step, l_row, l_lo - l_run0 - 16 * ki, l_len - l_run0 - 16 * ki);
+                else if (SXB_RARE(a.c.row_stride != 1)) copy_rows<S, kPass, kOff, false, false>(k_to0 + by, v_to0 + by, k, v, step, 0, 0, 0);
+                else copy_rows<S, kPass, kOff, true, false>(k_to0 + by, v_to0 + by, k, v, 0, 0, 0, 0);
             }
             if constexpr (kQuant) {
-                const uint32_t piece = (uint32_t)l_page[ki] * page_pieces + in_page * row_pieces + l_scales;
+                const uint32_t piece = (uint32_t)l_page[ki] * a.page_pieces + in_page * a.row_pieces + l_scales;
                 const uint8_t *ks = reinterpret_cast<const uint8_t *>(a.c.k_sm) + (uint64_t)piece * kBytes, *vs = reinterpret_cast<const uint8_t *>(a.c.v_sm) + (uint64_t)piece * kBytes;
                 each<kScalePasses>([&](auto i) {
                     constexpr int kTo = (ki * 16 + decltype(i)::value * kScalePass) * NG * 4;
                     if (kScalePass * kPieces == 32 * WR || s_row < kScalePass) {
-                        const int r = l_run0 + 16 * ki + decltype(i)::value * kScalePass + s_row;
-                        if (edge) {
-                            const int n = r >= l_s.lo && r < l_s.len ? kBytes : 0;
-                            copy_async<kBytes, kTo>(s_to0 + by, ks, n), copy_async<kBytes, kTo + S::kScales>(s_to0 + by, vs, n);
-                        } else {
-                            copy_async<kBytes, kTo>(s_to0 + by, ks), copy_async<kBytes, kTo + S::kScales>(s_to0 + by, vs);
-                        }
+                        const int r = l_run0 + 16 * ki + decltype(i)::value * kScalePass + s_row, n = !edge || (r >= l_lo && r < l_len) ? kBytes : 0;
+                        copy_async<kBytes, kTo>(s_to0 + by, ks, n), copy_async<kBytes, kTo + S::kScales>(s_to0 + by, vs, n);
                     }
-                    ks += (uint64_t)row_pieces * (kScalePass * kBytes), vs += (uint64_t)row_pieces * (kScalePass * kBytes);
+                    ks += (uint64_t)a.row_pieces * (kScalePass * kBytes), vs += (uint64_t)a.row_pieces * (kScalePass * kBytes);
                 });
             }
         });
     };
     // A segment's queries and what there is to know of it: the whole CTA's, into a ring of as many places as there are stages.
-    auto load_segment = [&]() {
-        const int slot = l_segment % kStages, rows0 = l_row_tile * R;
+    auto load_segment = [&](int at) {
+        const Sequence q = cur.s;
+        const int slot = cur.segment % kStages, rows0 = cur.row_tile * R, head = cur.head;
         uint8_t *const qs = q_ring + slot * S::kQ;
 #pragma unroll 1
         for (int i = tid; i < R * (D / 8); i += kThreads) {
             const int r = i / (D / 8), c = i % (D / 8), row = rows0 + r, tok = row / a.group;
-            const bool there = tok < l_s.n;
-            const int64_t off = there ? (l_s.q0 + tok) * a.q_ld + (int64_t)(l_head * a.group + row - tok * a.group) * D + c * 8 : 0;
+            const bool there = tok < q.n;
+            const int64_t off = there ? (q.q0 + tok) * a.q_ld + (int64_t)(head * a.group + row - tok * a.group) * D + c * 8 : 0;
             copy_async<16>(smem_of(qs + chunk_at<D / 8>(r, c) * 16), a.q + off, there ? 16 : 0);
         }
-        if (tid == 0) segments[slot] = Segment{l_s.q0, l_s.n, l_s.len, l_s.p0, l_s.lo, l_s.tile0, l_s.tiles, l_head, rows0, l_at, (int)l_s.bad};
+        if (tid == 0) segments[slot] = Segment{q.q0, q.n, q.len, q.p0, q.lo, q.tile0, q.tiles, head, rows0, at, (int)q.bad};
     };
 
-    l_table = a.pages + l_b * a.pages_ld;
-    at_head();
+    const int first_at = (int)(in % cur.s.tiles);
+    at_segment(first_at);
     find_pages();
 #pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) {
         if (s < units) {
-            if (l_new) load_segment();
+            if (l_new) load_segment(s == 0 ? first_at : 0);
             load(s);
             if (s + 1 < units) {
                 advance();
@@ -548,9 +566,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     const uint32_t v_at0 = S::kRows + (BITS == 16 ? chunk_at<CR>((lane & 7) + 8 * (lane >> 4), (lane >> 3) & 1) : chunk_at<CR>(a_row, BITS == 8 ? a_half : 0)) * 16;
     const uint32_t q_at0 = chunk_at<D / 8>(wr * NT * 8 + (lane & 7), lane >> 3) * 16;
     uint32_t qf[S::kHoldQ ? NT : 1][S::kHoldQ ? D / 16 : 1][2];
-    float o[D / 16][NT][4], w_sum[S::kOffsetV ? NG : 1][NT][4], o_min[kGroups][NT][2];
+    float o[D / 16][NT][4], w_sum[NT][4], o_min[kGroups][NT][2];
     float m[NT][2], l[NT][2];
-    float qsum[S::kHoldSums ? NG : 1][NT][2];
     int v_exp = 20, at = 0, tiles = 0, whole0 = 0, whole1 = 0, segment = 0, stage = 0;
     bool fresh = true;
 
@@ -560,7 +577,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         if constexpr (WR == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(1 + wk), "n"(32 * WR) : "memory");
         if (i + kStages - 1 < units) {
-            if (l_new) load_segment();
+            if (SXB_RARE(l_new)) load_segment(0);
             load(stage == 0 ? kStages - 1 : stage - 1);
             if (i + kStages < units) {
                 advance();
@@ -572,7 +589,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         const uint32_t st = smem0 + stage * S::kStage + wk * S::kPart;
         uint8_t *const qs = q_ring + (segment % kStages) * S::kQ;
         const Segment &sg = segments[segment % kStages];
-        if (fresh) {
+        if (SXB_RARE(fresh)) {
             fresh = false;
             __syncthreads();
             at = sg.at, tiles = sg.tiles, v_exp = 20;
@@ -587,8 +604,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 for (int d = 0; d < D / 16; ++d) o[d][nt][0] = o[d][nt][1] = o[d][nt][2] = o[d][nt][3] = 0.f;
 #pragma unroll
                 for (int e = 0; e < kGroups; ++e) o_min[e][nt][0] = o_min[e][nt][1] = 0.f;
-#pragma unroll
-                for (int e = 0; e < (S::kOffsetV ? NG : 1); ++e) w_sum[e][nt][0] = w_sum[e][nt][1] = w_sum[e][nt][2] = w_sum[e][nt][3] = 0.f;
+                w_sum[nt][0] = w_sum[nt][1] = w_sum[nt][2] = w_sum[nt][3] = 0.f;
             }
             if constexpr (kQuant) {
                 // q to F16 times a power of two, elements in the order that the codes come in, and each group's sum of what they then are
@@ -630,7 +646,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                             w[pos / 2] = pack_f16(x[b][d0] * f, x[b][d1] * f);
                             const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&w[pos / 2]));
                             sums[b] += back.x + back.y;
-                        }
+                                                    }
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
                             *reinterpret_cast<uint4 *>(qs + chunk_at<D / 8>(r, blk * 4 + c) * 16) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
@@ -640,7 +656,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     static_assert(kRuns <= kPer, "");
 #pragma unroll
                     for (int off = 1; off < kRuns; off <<= 1) sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], off);
-                    if (blk < kBlocks && blk % kRuns == 0) q_sums[blk / kRuns * R + r] = sums[b];
+                    if (blk < kBlocks && blk % kRuns == 0) q_sums[blk / kRuns * R + r] = sums[b], q_extra[blk / kRuns * R + r] = -S::kOffsetK * sums[b];
                 }
                 __syncthreads();
             }
@@ -653,15 +669,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                         qf[t][ks][0] = r[0], qf[t][ks][1] = r[1], qf[t][ks + 1][0] = r[2], qf[t][ks + 1][1] = r[3];
                     });
                 });
-            }
-            if constexpr (kQuant && S::kHoldSums) {
-#pragma unroll
-                for (int grp = 0; grp < NG; ++grp)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const float2 v = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
-                        qsum[grp][nt][0] = v.x, qsum[grp][nt][1] = v.y;
-                    }
             }
         }
         const bool whole = at >= whole0 && at < whole1;
@@ -698,7 +705,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 load_shared<ki * 16 * NG * 4>(words[0], s_at), load_shared<(ki * 16 + 8) * NG * 4>(words[1], s_at);
                 each<NG>([&](auto grpc) {
                     constexpr int grp = decltype(grpc)::value;
-                    float part[NT][4] = {};
+                    float part[NT][4];
+                    float2 q_sum[NT];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        q_sum[nt] = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
+                        const float2 extra = *reinterpret_cast<const float2 *>(q_extra + grp * R + (wr * NT + nt) * 8 + 2 * t4);
+                        part[nt][0] = part[nt][2] = extra.x, part[nt][1] = part[nt][3] = extra.y;
+                    }
                     each<S::G / 32>([&](auto run) {
                         constexpr int blk = grp * (S::G / 32) + decltype(run)::value;
                         uint32_t k0[4], k1[4];
@@ -710,8 +724,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                         } else {
                             uint32_t w0[1], w1[1];
                             load_shared<kRun>(w0, k_at ^ (blk * 16)), load_shared<kRun + 8 * S::RB>(w1, k_at ^ (blk * 16));
-                            k0[0] = nibbles_f16(w0[0] << 4), k0[1] = nibbles_f16(w1[0] << 4), k0[2] = nibbles_f16(w0[0]), k0[3] = nibbles_f16(w1[0]);
-                            k1[0] = nibbles_f16(w0[0] >> 4), k1[1] = nibbles_f16(w1[0] >> 4), k1[2] = nibbles_f16(w0[0] >> 8), k1[3] = nibbles_f16(w1[0] >> 8);
+                            k0[0] = next_nibbles_f16(w0[0] << 4), k0[1] = next_nibbles_f16(w1[0] << 4), k0[2] = next_nibbles_f16(w0[0]), k0[3] = next_nibbles_f16(w1[0]);
+                            k1[0] = next_nibbles_f16(w0[0] >> 4), k1[1] = next_nibbles_f16(w1[0] >> 4), k1[2] = next_nibbles_f16(w0[0] >> 8), k1[3] = next_nibbles_f16(w1[0] >> 8);
                         }
                         each<NT>([&](auto nt) {
                             uint32_t q[4];
@@ -724,16 +738,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         sc[e] = __uint_as_float(words[e][grp] << 16);
-                        mn[e] = fmaf(-S::kOffset, sc[e], __uint_as_float(words[e][grp] & 0xffff0000u));
+                        mn[e] = __uint_as_float(words[e][grp] & 0xffff0000u);
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float2 q_sum;
-                        if constexpr (S::kHoldSums) q_sum = make_float2(qsum[grp][nt][0], qsum[grp][nt][1]);
-                        else q_sum = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
+                    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(sc[e >> 1], part[nt][e], fmaf(mn[e >> 1], e & 1 ? q_sum.y : q_sum.x, s[ki][nt][e]));
-                    }
+                        for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(sc[e >> 1], part[nt][e], fmaf(mn[e >> 1], e & 1 ? q_sum[nt].y : q_sum[nt].x, s[ki][nt][e]));
                 });
             }
         });
@@ -747,7 +757,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 fac[nt][0] = f.x, fac[nt][1] = f.y;
             }
         }
-        if (a.softcap > 0.f) {
+        if (SXB_RARE(a.softcap > 0.f)) {
             // tanh x = 1 - 2 / (exp(2 x) + 1): 2^-22 of the cap, as good as a score near it is in FP32
             const float by = 2.f / a.softcap, to = a.softcap * kLog2e;
 #pragma unroll
@@ -760,7 +770,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             }
         }
         uint32_t hidden = 0;  // bit (ki * NT + nt) * 4 + e: that query does not see that key
-        if (!whole) {
+        if (SXB_RARE(!whole)) {
             const int j0 = run0 + g;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -794,33 +804,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 past = fmaxf(past, fmaf(v, fac[nt][e], -m[nt][e]));
             }
         bool move = past > kSlack;
-        uint32_t v_words[KI][2][kGroups];
-        bool odd = false;  // a scale or a min among them is none, and there are rows that must not hear of it
-        if constexpr (kQuant) {
-            float v_top = 0.f;
-            each<KI>([&](auto ki) {
-                constexpr int kOff = S::kScales + decltype(ki)::value * 16 * NG * 4;
-                load_shared<kOff>(v_words[decltype(ki)::value][0], s_at), load_shared<kOff + 8 * NG * 4>(v_words[decltype(ki)::value][1], s_at);
-            });
-#pragma unroll
-            for (int ki = 0; ki < KI; ++ki)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) v_top = fmaxf(v_top, fabsf(__uint_as_float(v_words[ki][e][grp] << 16)));
-                }
-            move = move || (__float_as_uint(v_top) >> 23) > (uint32_t)v_exp;
-            if (!whole) {
-#pragma unroll
-                for (int ki = 0; ki < KI; ++ki)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int grp = 0; grp < NG; ++grp) odd = odd || (v_words[ki][e][grp] & 0x7f80u) == 0x7f80u || (v_words[ki][e][grp] & 0x7f800000u) == 0x7f800000u;
-                odd = __any_sync(0xffffffffu, odd);
-            }
-        }
-        if (__any_sync(0xffffffffu, move)) {
+        if (SXB_RARE(__any_sync(0xffffffffu, move))) {
             float f[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -835,33 +819,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                     for (int grp = 0; grp < kGroups; ++grp) o_min[grp][nt][e] *= f[nt][e];
                 }
-            if constexpr (kQuant) {
-                int ex = 0;
-#pragma unroll
-                for (int ki = 0; ki < KI; ++ki)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int grp = 0; grp < NG; ++grp) {
-                            const int x = (int)(v_words[ki][e][grp] >> 7 & 0xffu);
-                            if (x != 255) ex = max(ex, x);  // a scale that is none says nothing of the others
-                        }
-                ex = max(v_exp, __reduce_max_sync(0xffffffffu, ex));
-                const float down = exp2_fast((float)(v_exp - ex));
-                v_exp = ex;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) f[nt][0] *= down, f[nt][1] *= down;
-            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[d][nt][e] *= f[nt][e & 1];
-#pragma unroll
-                for (int grp = 0; grp < (S::kOffsetV ? NG : 1); ++grp)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w_sum[grp][nt][e] *= f[nt][e & 1];
+                w_sum[nt][0] *= f[nt][0], w_sum[nt][1] *= f[nt][1];
             }
         }
 #pragma unroll
@@ -879,7 +843,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         if constexpr (!kQuant) {
             // Keys that one row sees and another does not: an infinity or a NaN there must not reach the other through 0 * v.
             bool clean = true;
-            if (!whole && sg.n > 1) {
+            if (SXB_RARE(!whole && sg.n > 1)) {
                 const uint8_t *const vt = smem + stage * S::kStage + wk * S::kPart + S::kRows;
                 for (int c = lane; c < RUN * CR; c += 32) {
                     const uint4 w = *reinterpret_cast<const uint4 *>(vt + c * 16);
@@ -889,7 +853,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 }
                 clean = __all_sync(0xffffffffu, clean);
             }
-            if (clean) {
+            if (__builtin_expect(clean, 1)) {
                 each<KI>([&](auto kic) {
                     constexpr int ki = decltype(kic)::value, kRun = ki * 16 * S::RB;
                     uint32_t p[NT][2];
@@ -936,41 +900,81 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     }
             }
         } else {
-            const float v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);  // 2^(14 - kSlack - (v_exp - 127))
+            float v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);  // 2^(14 - kSlack - (v_exp - 127))
             each<KI>([&](auto kic) {
                 constexpr int ki = decltype(kic)::value, kRun = ki * 16 * S::RB;
+                uint32_t words[2][kGroups];
+                value_words<S, ki>(words, s_at);
+                bool odd = false;  // a scale or a min among them is none, and there are rows that must not hear of it
+                if (SXB_RARE(!whole)) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int grp = 0; grp < NG; ++grp) odd = odd || none_of(words[e][grp]);
+                }
+                if (SXB_RARE(odd)) {  // what is none stays with the rows that see it: their columns of the group end as NaN
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int grp = 0; grp < NG; ++grp)
+                            if (none_of(words[e][grp])) {
+                                words[e][grp] = 0;
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                    for (int x = 0; x < 2; ++x)
+                                        if ((hidden >> ((ki * NT + nt) * 4 + 2 * e + x) & 1) == 0) o_min[grp][nt][x] = CUDART_NAN_F;
+                            }
+                }
+                // scales times the power of two that keeps their products with weights inside F16; the largest so far sets it
+                float scales[2][kGroups], most = 0.f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int grp = 0; grp < NG; ++grp) scales[e][grp] = __uint_as_float(words[e][grp] << 16) * v_up, most = fmaxf(most, fabsf(scales[e][grp]));
+                if (SXB_RARE(__any_sync(0xffffffffu, most >= (float)(1 << (15 - kSlack))))) {
+                    int ex = 0;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int grp = 0; grp < NG; ++grp) {
+                            const int x = (int)(words[e][grp] >> 7 & 0xffu);
+                            if (x != 255) ex = max(ex, x);  // a scale that is none says nothing of the others
+                        }
+                    ex = max(v_exp, __reduce_max_sync(0xffffffffu, ex));
+                    const float down = exp2_fast((float)(v_exp - ex));
+                    v_exp = ex, v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int grp = 0; grp < NG; ++grp) scales[e][grp] = __uint_as_float(words[e][grp] << 16) * v_up;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[d][nt][e] *= down;
+                        w_sum[nt][0] *= down, w_sum[nt][1] *= down;
+                    }
+                }
                 each<NG>([&](auto grpc) {
                     constexpr int grp = decltype(grpc)::value;
-                    float sc[2], mn[2];
+                    float mn[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) sc[e] = __uint_as_float(v_words[ki][e][grp] << 16) * v_up, mn[e] = __uint_as_float(v_words[ki][e][grp] & 0xffff0000u);
+                    for (int e = 0; e < 2; ++e) mn[e] = __uint_as_float(words[e][grp] & 0xffff0000u);
                     uint32_t p[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float w[4];
-                        if (!odd) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                w[e] = s[ki][nt][e] * sc[e >> 1];
-                                o_min[grp][nt][e & 1] = fmaf(s[ki][nt][e], mn[e >> 1], o_min[grp][nt][e & 1]);
-                            }
-                        } else {  // a scale or min that is none must not reach a row that does not see it
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                w[e] = 0.f;
-                                if ((hidden >> ((ki * NT + nt) * 4 + e) & 1) == 0) {
-                                    w[e] = s[ki][nt][e] * sc[e >> 1];
-                                    o_min[grp][nt][e & 1] = fmaf(s[ki][nt][e], mn[e >> 1], o_min[grp][nt][e & 1]);
-                                }
-                            }
+                        for (int e = 0; e < 4; ++e) {
+                            w[e] = s[ki][nt][e] * scales[e >> 1][grp];
+                            o_min[grp][nt][e & 1] = fmaf(s[ki][nt][e], mn[e >> 1], o_min[grp][nt][e & 1]);
                         }
                         p[nt][0] = transposed(pack_f16(w[0], w[1])), p[nt][1] = transposed(pack_f16(w[2], w[3]));
-                        if constexpr (S::kOffsetV) {
-                            const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-                            mma<true>(w_sum[grp][nt], ones, p[nt][0], p[nt][1]);
-                        }
+                        const uint32_t one = g == grp ? 0x3c003c00u : 0u, ones[4] = {one, 0, one, 0};  // row grp of the sums
+                        mma<true>(w_sum[nt], ones, p[nt][0], p[nt][1]);
                     }
-                    auto code = [](uint32_t v) { return S::kOffsetV ? v : less_offset<BITS>(v); };
                     each<S::G / 32>([&](auto runc) {
                         constexpr int run = decltype(runc)::value;
                         if constexpr (BITS == 8) {  // two chunks of sixteen columns, the even ones rows 0 - 7 of a fragment, the odd ones rows 8 - 15
@@ -979,8 +983,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                             load_matrices_trans<kRun>(v, v_at ^ (c * 16));
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
-                                const uint32_t va[4] = {code(bytes_f16(v[2 * x], 0x4240)), code(bytes_f16(v[2 * x], 0x4341)), code(bytes_f16(v[2 * x + 1], 0x4240)),
-                                                        code(bytes_f16(v[2 * x + 1], 0x4341))};
+                                const uint32_t va[4] = {bytes_f16(v[2 * x], 0x4240), bytes_f16(v[2 * x], 0x4341), bytes_f16(v[2 * x + 1], 0x4240), bytes_f16(v[2 * x + 1], 0x4341)};
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) mma<true>(o[c + x][nt], va, p[nt][0], p[nt][1]);
                             }
@@ -988,8 +991,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                             constexpr int c = grp * (S::G / 32) + run;
                             uint32_t v[2];
                             load_matrices_trans<kRun>(v, v_at ^ (c * 16));
-                            const uint32_t va[4] = {code(nibbles_f16(v[0] << 4)), code(nibbles_f16(v[0])), code(nibbles_f16(v[1] << 4)), code(nibbles_f16(v[1]))};
-                            const uint32_t vb[4] = {code(nibbles_f16(v[0] >> 4)), code(nibbles_f16(v[0] >> 8)), code(nibbles_f16(v[1] >> 4)), code(nibbles_f16(v[1] >> 8))};
+                            const uint32_t va[4] = {low_nibbles_f16(v[0]), next_nibbles_f16(v[0]), low_nibbles_f16(v[1]), next_nibbles_f16(v[1])};
+                            const uint32_t u0 = v[0] >> 8, u1 = v[1] >> 8;
+                            const uint32_t vb[4] = {low_nibbles_f16(u0), next_nibbles_f16(u0), low_nibbles_f16(u1), next_nibbles_f16(u1)};
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) mma<true>(o[2 * c][nt], va, p[nt][0], p[nt][1]), mma<true>(o[2 * c + 1][nt], vb, p[nt][0], p[nt][1]);
                         }
@@ -1000,9 +1004,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         }
         uint8_t *const stage_base = smem + stage * S::kStage;
         stage = stage + 1 == kStages ? 0 : stage + 1;
-        if (++at < tiles && i + 1 < units) continue;
+        if (__builtin_expect(++at < tiles && i + 1 < units, 1)) continue;
 
         // ---- the segment's end, or this CTA's share's: the warps' sums become one ----
+        const int64_t u0 = list[0], u1 = list[1], total = list[2], ctas = list[3];
         const int64_t seg0 = u0 + (i + 1) - at, seg1 = seg0 + tiles;  // the segment's units in the list
         const bool split = seg0 < u0 || seg1 > u1;
 #pragma unroll
@@ -1025,15 +1030,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1) o_min[grp][nt][e] += __shfl_xor_sync(0xffffffffu, o_min[grp][nt][e], off);
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int grp = 0; grp < NG; ++grp) {
+                    const float sum[2] = {__shfl_sync(0xffffffffu, w_sum[nt][0], grp * 4 + t4), __shfl_sync(0xffffffffu, w_sum[nt][1], grp * 4 + t4)};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        constexpr float off = S::kOffset;
-                        const float v = S::kOffsetV ? fmaf(-off, w_sum[S::kOffsetV ? d * 16 / S::G : 0][nt][e], o[d][nt][e]) : o[d][nt][e];
-                        o[d][nt][e] = fmaf(v, down, o_min[d * 16 / S::G][nt][e & 1]);
-                    }
+                    for (int d = grp * S::G / 16; d < (grp + 1) * S::G / 16; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[d][nt][e] = fmaf(fmaf(e < 2 ? -S::kOffset : -S::kOffsetOdd, sum[e & 1], o[d][nt][e]), down, o_min[grp][nt][e & 1]);
+                }
         }
         __syncthreads();
         // what each group's sums of a row count for, the row's maximum and its sum of weights
@@ -1244,6 +1249,9 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
     a.q = static_cast<const uint16_t *>(q), a.q_ld = q_ld, a.pages = pages, a.pages_ld = pages_ld, a.capacity = n_cols * cache->page;
     a.q_start = q_start, a.kv_len = kv_len, a.B = (int)B, a.T = (int)T, a.n_q = (int)n_q, a.group = (int)(n_q / n_kv), a.window = (int)window;
     a.scale = scale, a.softcap = softcap, a.out = static_cast<uint16_t *>(out), a.out_ld = out_ld, a.lse = args->lse, a.err = err;
+    const uint32_t chunks = (uint32_t)(D * cache->bits / 8 / 16), words = cache->bits == 16 ? 0 : (uint32_t)(D / cache->G), pieces = words > 4 ? words / 4 : words ? 1 : 0;
+    a.page_chunks = (uint32_t)cache->page_stride * chunks, a.head_chunks = (uint32_t)cache->head_stride * chunks, a.row_chunks = (uint32_t)cache->row_stride * chunks;
+    a.page_pieces = (uint32_t)cache->page_stride * pieces, a.head_pieces = (uint32_t)cache->head_stride * pieces, a.row_pieces = (uint32_t)cache->row_stride * pieces;
     auto st = static_cast<cudaStream_t>(stream);
     const cudaError_t rc = with_shape(D, cache->bits, cache->G, rows, [&](auto s) {
         using S = decltype(s);
