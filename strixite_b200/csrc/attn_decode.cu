@@ -36,13 +36,12 @@ constexpr int64_t kMaxRows = 1ll << 24;
 // Runs of sixteen keys that a warp takes at a time: two give it independent work and share what a step costs besides, where registers allow.  (Two in a
 // loop, one after the other, are slower: 32 sequences of 9509 keys, 8 bits, 115 us side by side, 132 to 152 in turn.)
 constexpr int key_runs(int D, int bits, int nt) { return nt * D <= 256 && D * bits <= 1024 ? 2 : 1; }
-// R query rows: NT tiles of eight a warp, WR warps side by side.  The WK groups of such warps share a tile's keys, a run of KI times sixteen each, and
-// every group fetches its own run into its own ring: nothing but a segment's ends is the whole CTA's business.
+// R query rows, NT tiles of eight, all of them every warp's.  The four warps share a tile's keys, a run of KI times sixteen each, and every warp fetches its
+// own run into its own ring: nothing but a segment's ends is the whole CTA's business.
 template <int D_, int BITS_, int G_, int R_> struct Shape {
     static constexpr int D = D_, BITS = BITS_, G = G_, R = R_;
     static constexpr bool kQuant = BITS != 16;
-    static constexpr int kMostNT = D == 256 ? 2 : 4, NT = R / 8 < kMostNT ? R / 8 : kMostNT, WR = R / 8 / NT;
-    static constexpr int kWarps = WR > 1 ? 8 : 4, kThreads = 32 * kWarps, WK = kWarps / WR;
+    static constexpr int NT = R / 8, kWarps = 4, kThreads = 32 * kWarps, WK = kWarps;
     static constexpr int RB = D * BITS / 8, CR = RB / 16;  // bytes and 16-byte chunks of a cache row
     static constexpr int NG = kQuant ? D / G : 0;
     static constexpr int KI = key_runs(D, BITS, NT), RUN = 16 * KI, TK = RUN * WK;
@@ -52,7 +51,7 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     static constexpr bool kOwnJoint = kStage < kMostJoint;  // 32 columns of every warp's rows do not fit a stage
     static constexpr int kMisc = 1024 + kWarps * 64 + WK * R * 8 + R * (2 * NG + 2) * 4 + (kOwnJoint ? kMostJoint : 0);
     // CTAs an SM: as many as registers allow (three of four warps with 168 registers a thread, two with 255), if their rings then still have 64 KB on the way
-    static constexpr int kByRegisters = WR > 1 ? 1 : kQuant && NT * D <= 128 ? 3 : 2;
+    static constexpr int kByRegisters = kQuant && NT * D <= 128 ? 3 : 2;
     static constexpr int stages(int per_sm) { return (226 * 1024 / per_sm - kMisc) / (kStage + kQ); }
     static constexpr bool fits(int per_sm) { return kByRegisters >= per_sm && stages(per_sm) >= 2 && per_sm * (stages(per_sm) - 1) * kStage >= 64 * 1024; }
     static constexpr int kPerSm = fits(3) ? 3 : fits(2) ? 2 : 1;
@@ -71,7 +70,7 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     // 19 parts of 33 KB, 30 us at the end of 80), a second kernel has the rows of all segments side by side.
     static constexpr bool kJoinHere = R * D <= 8 * kThreads;  // a thread has two runs of four columns at most
     static constexpr bool kHoldQ = !kQuant && NT * D <= 256;  // q's fragments in registers
-    static_assert(kStages >= 2 && WK * WR == kWarps && KI * NT * 4 <= 32, "");
+    static_assert(kStages >= 2 && KI * NT * 4 <= 32, "");
 };
 
 struct Args {
@@ -262,10 +261,10 @@ __device__ inline void copy_rows(uint32_t k_to, uint32_t v_to, const uint8_t *k,
 // A run of keys with a bad page, or of pages of eight tokens: each row looks its page up.  Rows out of range become zeros, the keys of a bad page NaN.
 // Out of line: the loop keeps its registers.
 template <class S>
-__device__ __noinline__ void load_ragged(const Args &a, const int32_t *table, uint32_t st, int run0, int lo, int len, int head, int b, int group_lane) {
+__device__ __noinline__ void load_ragged(const Args &a, const int32_t *table, uint32_t st, int run0, int lo, int len, int head, int b, int lane) {
     constexpr int CR = S::CR, NG = S::NG, RUN = S::RUN;
-    constexpr int kPass = 32 * S::WR / CR > RUN ? RUN : 32 * S::WR / CR;
-    const int page_mask = (1 << a.c.page_shift) - 1, chunk = group_lane % CR, row = group_lane / CR;
+    constexpr int kPass = 32 / CR > RUN ? RUN : 32 / CR;
+    const int page_mask = (1 << a.c.page_shift) - 1, chunk = lane % CR, row = lane / CR;
     auto place = [&](int r, bool &wanted) -> int64_t {  // of row r, -1: none
         const int j = run0 + r;
         wanted = j >= lo && j < len;
@@ -290,7 +289,7 @@ __device__ __noinline__ void load_ragged(const Args &a, const int32_t *table, ui
     if constexpr (S::kQuant) {
         constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = NG * 4 / kBytes;  // of a row's scales
 #pragma unroll 1
-        for (int i = group_lane; i < RUN * kPieces; i += 32 * S::WR) {
+        for (int i = lane; i < RUN * kPieces; i += 32) {
             const int r = i / kPieces, piece = i % kPieces;
             bool wanted;
             const int64_t from = place(r, wanted), off = from < 0 ? 0 : from * (NG * 4) + piece * kBytes;
@@ -357,7 +356,7 @@ __global__ void __launch_bounds__(kJoinRows * S::D / 4) attn_join_kernel(const _
 
 template <class S>
 __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(const __grid_constant__ Args a) {
-    constexpr int D = S::D, BITS = S::BITS, NG = S::NG, TK = S::TK, KI = S::KI, RUN = S::RUN, R = S::R, WK = S::WK, WR = S::WR, CR = S::CR, NT = S::NT;
+    constexpr int D = S::D, BITS = S::BITS, NG = S::NG, TK = S::TK, KI = S::KI, RUN = S::RUN, R = S::R, WK = S::WK, CR = S::CR, NT = S::NT;
     constexpr int kStages = S::kStages, kThreads = S::kThreads, kWarps = S::kWarps;
     constexpr bool kQuant = S::kQuant;
     constexpr int kGroups = kQuant ? NG : 1;
@@ -375,7 +374,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     auto *const segments = reinterpret_cast<Segment *>(list + 4);                  // [kStages]
     Cursor &cur = reinterpret_cast<Cursor *>(segments + kStages)[threadIdx.x >> 5];  // [kWarps]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int wr = warp % WR, wk = warp / WR;
 
     behind_grid();
 
@@ -442,21 +440,21 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     __syncthreads();
     const int units = (int)(u1 - u0);
     const int page_mask = (1 << a.c.page_shift) - 1;
-    constexpr int kPass = 32 * WR / CR > 16 ? 16 : 32 * WR / CR;  // rows that the group's threads fetch at a time
+    constexpr int kPass = 32 / CR > 16 ? 16 : 32 / CR;  // rows that the warp fetches at a time
     constexpr int kBytes = NG * 4 > 16 ? 16 : NG * 4, kPieces = kQuant ? NG * 4 / kBytes : 1;  // of a row's scales
-    constexpr int kScalePass = 32 * WR / kPieces > 16 ? 16 : 32 * WR / kPieces, kScalePasses = 16 / kScalePass;
-    const int l_lane = wr * 32 + lane, l_chunk = l_lane % CR, l_row = l_lane / CR, s_row = l_lane / kPieces, s_piece = l_lane % kPieces;
+    constexpr int kScalePass = 32 / kPieces > 16 ? 16 : 32 / kPieces, kScalePasses = 16 / kScalePass;
+    const int l_chunk = lane % CR, l_row = lane / CR, s_row = lane / kPieces, s_piece = lane % kPieces;
     const uint32_t smem0 = smem_of(smem);
-    const uint32_t k_to0 = smem0 + wk * S::kPart + k_chunk_at<S>(l_row, l_chunk) * 16, v_to0 = smem0 + wk * S::kPart + S::kRows + chunk_at<CR>(l_row, l_chunk) * 16;
-    const uint32_t s_to0 = smem0 + wk * S::kPart + 2 * S::kRows + l_lane * kBytes;
+    const uint32_t k_to0 = smem0 + warp * S::kPart + k_chunk_at<S>(l_row, l_chunk) * 16, v_to0 = smem0 + warp * S::kPart + S::kRows + chunk_at<CR>(l_row, l_chunk) * 16;
+    const uint32_t s_to0 = smem0 + warp * S::kPart + 2 * S::kRows + lane * kBytes;
     uint32_t l_codes, l_scales;             // this lane's place in the head's first row
-    int l_run0, l_lo, l_len, l_tiles;       // first key of the group's run; the sequence's keys; tiles of the segment from here on
+    int l_run0, l_lo, l_len, l_tiles;       // first key of the warp's run; the sequence's keys; tiles of the segment from here on
     const int32_t *l_table;
     bool l_new;                             // the run begins a segment
     auto at_segment = [&](int at) {         // the cursor stands at tile `at` of its segment
         l_codes = cur.head * a.head_chunks + l_row * a.row_chunks + l_chunk;
         l_scales = cur.head * a.head_pieces + s_row * a.row_pieces + s_piece;
-        l_run0 = (cur.s.tile0 + at) * TK + wk * RUN, l_lo = cur.s.lo, l_len = cur.s.len, l_tiles = cur.s.tiles - at;
+        l_run0 = (cur.s.tile0 + at) * TK + warp * RUN, l_lo = cur.s.lo, l_len = cur.s.len, l_tiles = cur.s.tiles - at;
         l_table = a.pages + cur.b * a.pages_ld;
         l_new = true;
     };
@@ -495,7 +493,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
         for (int ki = 0; ki < KI; ++ki) fine = fine && (unsigned)l_page[ki] < (unsigned)a.c.n_pages;
         if (SXB_RARE(!fine)) {
-            load_ragged<S>(a, l_table, smem0 + wk * S::kPart + by, l_run0, l_lo, l_len, cur.head, cur.b, l_lane);
+            load_ragged<S>(a, l_table, smem0 + warp * S::kPart + by, l_run0, l_lo, l_len, cur.head, cur.b, lane);
             return;
         }
         const bool edge = l_run0 < l_lo || l_run0 + RUN > l_len;
@@ -505,7 +503,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             const uint32_t in_page = (l_run0 + 16 * ki) & page_mask;
             const uint32_t chunk = (uint32_t)l_page[ki] * a.page_chunks + in_page * a.row_chunks + l_codes;
             const uint8_t *const k = a.c.k + (uint64_t)chunk * 16, *const v = a.c.v + (uint64_t)chunk * 16;
-            if (kPass * CR == 32 * WR || l_row < kPass) {
+            if (kPass * CR == 32 || l_row < kPass) {
                 if (SXB_RARE(edge)) copy_rows<S, kPass, kOff, false, true>(k_to0 + by, v_to0 + by, k, v, step, l_row, l_lo - l_run0 - 16 * ki, l_len - l_run0 - 16 * ki);
                 else if (SXB_RARE(a.c.row_stride != 1)) copy_rows<S, kPass, kOff, false, false>(k_to0 + by, v_to0 + by, k, v, step, 0, 0, 0);
                 else copy_rows<S, kPass, kOff, true, false>(k_to0 + by, v_to0 + by, k, v, 0, 0, 0, 0);
@@ -515,7 +513,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 const uint8_t *ks = reinterpret_cast<const uint8_t *>(a.c.k_sm) + (uint64_t)piece * kBytes, *vs = reinterpret_cast<const uint8_t *>(a.c.v_sm) + (uint64_t)piece * kBytes;
                 each<kScalePasses>([&](auto i) {
                     constexpr int kTo = (ki * 16 + decltype(i)::value * kScalePass) * NG * 4;
-                    if (kScalePass * kPieces == 32 * WR || s_row < kScalePass) {
+                    if (kScalePass * kPieces == 32 || s_row < kScalePass) {
                         const int r = l_run0 + 16 * ki + decltype(i)::value * kScalePass + s_row, n = !edge || (r >= l_lo && r < l_len) ? kBytes : 0;
                         copy_async<kBytes, kTo>(s_to0 + by, ks, n), copy_async<kBytes, kTo + S::kScales>(s_to0 + by, vs, n);
                     }
@@ -564,7 +562,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     const int a_row = lane & 15, a_half = lane >> 4;  // of a fragment of sixteen rows, two chunks
     const uint32_t k_at0 = BITS == 16 ? k_chunk_at<S>(a_row, a_half) * 16 : BITS == 8 ? k_chunk_at<S>(g, t4 >> 1) * 16 + (t4 & 1) * 8 : k_chunk_at<S>(g, 0) * 16 + t4 * 4;
     const uint32_t v_at0 = S::kRows + (BITS == 16 ? chunk_at<CR>((lane & 7) + 8 * (lane >> 4), (lane >> 3) & 1) : chunk_at<CR>(a_row, BITS == 8 ? a_half : 0)) * 16;
-    const uint32_t q_at0 = chunk_at<D / 8>(wr * NT * 8 + (lane & 7), lane >> 3) * 16;
+    const uint32_t q_at0 = chunk_at<D / 8>((lane & 7), lane >> 3) * 16;
     uint32_t qf[S::kHoldQ ? NT : 1][S::kHoldQ ? D / 16 : 1][2];
     float o[D / 16][NT][4], w_sum[NT][4], o_min[kGroups][NT][2];
     float m[NT][2], l[NT][2];
@@ -574,8 +572,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll 1
     for (int i = 0; i < units; ++i) {
         wait_async<kStages - 2>();
-        if constexpr (WR == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(1 + wk), "n"(32 * WR) : "memory");
+        __syncwarp();
         if (i + kStages - 1 < units) {
             if (SXB_RARE(l_new)) load_segment(0);
             load(stage == 0 ? kStages - 1 : stage - 1);
@@ -586,7 +583,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         }
         commit_async();
 
-        const uint32_t st = smem0 + stage * S::kStage + wk * S::kPart;
+        const uint32_t st = smem0 + stage * S::kStage + warp * S::kPart;
         uint8_t *const qs = q_ring + (segment % kStages) * S::kQ;
         const Segment &sg = segments[segment % kStages];
         if (SXB_RARE(fresh)) {
@@ -672,7 +669,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             }
         }
         const bool whole = at >= whole0 && at < whole1;
-        const int run0 = (sg.tile0 + at) * TK + wk * RUN;
+        const int run0 = (sg.tile0 + at) * TK + warp * RUN;
         if (whole || (run0 < sg.len && run0 + RUN > sg.lo)) {
         // q's fragments of two steps of sixteen elements, from step 2 K2
         auto q_at = [&](auto nt, auto k2, uint32_t (&r)[4]) {
@@ -709,8 +706,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     float2 q_sum[NT];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        q_sum[nt] = *reinterpret_cast<const float2 *>(q_sums + grp * R + (wr * NT + nt) * 8 + 2 * t4);
-                        const float2 extra = *reinterpret_cast<const float2 *>(q_extra + grp * R + (wr * NT + nt) * 8 + 2 * t4);
+                        q_sum[nt] = *reinterpret_cast<const float2 *>(q_sums + grp * R + nt * 8 + 2 * t4);
+                        const float2 extra = *reinterpret_cast<const float2 *>(q_extra + grp * R + nt * 8 + 2 * t4);
                         part[nt][0] = part[nt][2] = extra.x, part[nt][1] = part[nt][3] = extra.y;
                     }
                     each<S::G / 32>([&](auto run) {
@@ -753,7 +750,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         for (int nt = 0; nt < NT; ++nt) {
             fac[nt][0] = fac[nt][1] = a.scale * kLog2e;
             if constexpr (kQuant) {
-                const float2 f = *reinterpret_cast<const float2 *>(q_factor + (wr * NT + nt) * 8 + 2 * t4);
+                const float2 f = *reinterpret_cast<const float2 *>(q_factor + nt * 8 + 2 * t4);
                 fac[nt][0] = f.x, fac[nt][1] = f.y;
             }
         }
@@ -776,7 +773,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int tok = (sg.rows0 + (wr * NT + nt) * 8 + 2 * t4 + e) / a.group;
+                    const int tok = (sg.rows0 + nt * 8 + 2 * t4 + e) / a.group;
                     const int hi = tok < sg.n ? sg.p0 + tok : -1, lo = a.window > 0 ? max(-1, hi - a.window) : -1;
 #pragma unroll
                     for (int ki = 0; ki < KI; ++ki)
@@ -844,7 +841,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             // Keys that one row sees and another does not: an infinity or a NaN there must not reach the other through 0 * v.
             bool clean = true;
             if (SXB_RARE(!whole && sg.n > 1)) {
-                const uint8_t *const vt = smem + stage * S::kStage + wk * S::kPart + S::kRows;
+                const uint8_t *const vt = smem + stage * S::kStage + warp * S::kPart + S::kRows;
                 for (int c = lane; c < RUN * CR; c += 32) {
                     const uint4 w = *reinterpret_cast<const uint4 *>(vt + c * 16);
                     const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
@@ -870,7 +867,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     });
                 });
             } else {
-                const uint8_t *const vt = smem + stage * S::kStage + wk * S::kPart + S::kRows;
+                const uint8_t *const vt = smem + stage * S::kStage + warp * S::kPart + S::kRows;
 #pragma unroll
                 for (int ki = 0; ki < KI; ++ki)
 #pragma unroll 1
@@ -1016,7 +1013,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
-                const int r = wk * R + (wr * NT + nt) * 8 + 2 * t4 + e;
+                const int r = warp * R + nt * 8 + 2 * t4 + e;
                 if (g == 0) row_max[r] = m[nt][e], row_sum[r] = l[nt][e];
             }
         if constexpr (kQuant) {
@@ -1057,7 +1054,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         float mine_f[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const float2 f = *reinterpret_cast<const float2 *>(row_max + wk * R + (wr * NT + nt) * 8 + 2 * t4);
+            const float2 f = *reinterpret_cast<const float2 *>(row_max + warp * R + nt * 8 + 2 * t4);
             mine_f[nt][0] = f.x, mine_f[nt][1] = f.y;
         }
         constexpr int DC = S::DC;
@@ -1071,8 +1068,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int r = (wr * NT + nt) * 8 + 2 * t4 + e;
-                    float *const to = joint + (wk * R + r) * DC;
+                    const int r = nt * 8 + 2 * t4 + e;
+                    float *const to = joint + (warp * R + r) * DC;
                     const float f = mine_f[nt][e];
 #pragma unroll
                     for (int d = col0 / 16; d < (col0 + DC) / 16; ++d) {
@@ -1140,8 +1137,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     }
 }
 
-// The rows of a tile for those that a key head's queries make: more query heads a key head or more drafts, more rows.
-inline int tile_rows(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// The rows of a tile for those that a key head's queries make: more query heads a key head or more drafts, more rows, until registers end; what is
+// above takes several tiles, and reads the keys for each.  Quantized keys' conversions are most of the work, and sixteen rows leave registers for two runs
+// side by side: eight conversations of one to eight rows of eight heads, 39 us with sixteen, 48 with 32; BF16, four rows of eight heads, 200 with sixteen,
+// 109 with 32.  (64 rows by pairs of warps: 54, and 184 where two tiles of 32 take 200 us.)
+constexpr int most_rows(int D, int bits) { return bits == 16 && D <= 128 ? 32 : 16; }
+inline int tile_rows(int D, int bits, int64_t rows) { return rows <= 8 ? 8 : rows <= 16 || most_rows(D, bits) == 16 ? 16 : 32; }
 
 // The counters' place is every form's: calls of different ones share a workspace.
 inline size_t counter_bytes() { return ((size_t)sm_count() * kMostPerSm * (sizeof(uint32_t) + sizeof(Join)) + 255) / 256 * 256; }
@@ -1173,9 +1174,9 @@ template <class S> struct Launch {
 // f(Shape) for the sizes of a call.
 template <int D, int BITS, int G, class F> auto with_rows(int rows, F f) {
     if (rows == 8) return f(Shape<D, BITS, G, 8>{});
-    if (rows == 16) return f(Shape<D, BITS, G, 16>{});
-    if (rows == 32) return f(Shape<D, BITS, G, 32>{});
-    return f(Shape<D, BITS, G, 64>{});
+    if constexpr (most_rows(D, BITS) == 32)
+        if (rows == 32) return f(Shape<D, BITS, G, 32>{});
+    return f(Shape<D, BITS, G, 16>{});
 }
 template <int D, class F> auto with_cache(int bits, int64_t G, int rows, F f) {
     if (bits == 16) return with_rows<D, 16, D>(rows, f);
@@ -1208,7 +1209,7 @@ extern "C" size_t sxb_attn_decode_workspace_bytes(int64_t n_q, int64_t n_kv, int
         return 0;
     }
     size_t most = 0;  // of a call with fewer rows too, and of any group size: how many CTAs an SM holds depends on both
-    for (int rows = 8; rows <= tile_rows(max_q * (n_q / n_kv)); rows *= 2)
+    for (int rows = 8; rows <= tile_rows((int)D, bits, max_q * (n_q / n_kv)); rows *= 2)
         for (int G = 32; G <= D && G <= 128; G *= 2) most = std::max(most, with_shape(D, bits, G, rows, [](auto s) { return Launch<decltype(s)>::bytes(); }));
     return most;
 }
@@ -1243,7 +1244,7 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
     SXB_CHECK(scale > 0.f && scale < 1e30f, fn, ": scale must be finite and positive");
     SXB_CHECK(softcap == 0.f || (softcap >= 1e-6f && softcap < 1e30f), fn, ": softcap = ", softcap, ", expected 0 (none) or 1e-6 .. 1e30");
     SXB_CHECK(window >= 0 && window < (1ll << 31), fn, ": window = ", window, ", expected 0 (none) .. 2^31 - 1");
-    const int rows = tile_rows(max_q * (n_q / n_kv));
+    const int rows = tile_rows((int)D, cache->bits, max_q * (n_q / n_kv));
     const size_t need = sxb_attn_decode_workspace_bytes(n_q, n_kv, D, cache->bits, max_q);
     SXB_CHECK(args->ws_bytes >= need, fn, ": workspace of ", args->ws_bytes, " bytes, needs ", need);
     a.q = static_cast<const uint16_t *>(q), a.q_ld = q_ld, a.pages = pages, a.pages_ld = pages_ld, a.capacity = n_cols * cache->page;

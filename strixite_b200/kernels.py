@@ -610,7 +610,9 @@ def attn_decode(q, cache: KvCache, pages, q_start, kv_len, max_q, out, ws, err, 
             and (lse is None or (lse.dtype is torch.float32 and lse.get_device() == dev and lse.shape == (T, n_q) and lse.is_contiguous()))):
         _refuse(cache, "attn_decode", q=(q, _BF16), out=(out, _BF16), pages=(pages, _I32), q_start=(q_start, _I32), kv_len=(kv_len, _I32), lse=(lse, _F32),
                 ws=(ws, (ws.dtype,)), err=(err, _WORDS))
-    if max_q * (n_q // cache.n_kv) > 16:
+    rows = max_q * (n_q // cache.n_kv)
+    tile = 8 if rows <= 8 else 16 if rows <= 16 or cache.bits != 16 or D == 256 else 32
+    if tile * D > 1024:
         _count()  # the parts of split sequences are joined by a second kernel
     _check(_lib.load().sxb_attn_decode(_DECODE_ARGS.pack(
         q.data_ptr(), _rows(q), T, n_q, cache._at, pages.data_ptr(), _rows(pages), pages.shape[1], q_start.data_ptr(), kv_len.data_ptr(), B, max_q,
