@@ -82,7 +82,7 @@ __device__ inline void store_run(uint8_t *rows, uint32_t *sm, int64_t row, const
     if constexpr (BITS == 16) {
         if (on) store_bf16_run(reinterpret_cast<uint16_t *>(rows) + row * D + part * 8, v);
     } else {
-        constexpr float kLevels = BITS == 4 ? 15.f : 255.f;
+        constexpr float kLevels = BITS == 4 ? 15.f : 255.f, kWhole = 12582912.f;
         const int lanes = G / 8;  // of a group: 4, 8 or 16
         float lo = v[0], hi = v[0];
         bool bad = !isfinite(v[0]);
@@ -102,10 +102,11 @@ __device__ inline void store_run(uint8_t *rows, uint32_t *sm, int64_t row, const
             uint32_t code = 0;
             if (s > 0.f) {
                 // (v - m) / s is within 2^-13 of the product with 1 / s below 256: where that is no nearer to a half, both round to the same code
+                // (rounded by way of 1.5 * 2^23, where neighbours are one apart and the number's low bits are the code)
                 const float d = __fsub_rn(v[i], m), x = d * per;
-                float r = rintf(x);
+                float r = (x + kWhole) - kWhole;
                 if (!(fabsf(x - r) < 0.5f - 1.f / 4096)) r = rintf(__fdiv_rn(d, s));
-                code = (uint32_t)fminf(fmaxf(r, 0.f), kLevels);
+                code = __float_as_uint(fminf(fmaxf(r, 0.f), kLevels) + kWhole) & 0xffu;
             }
             packed.w[i * BITS / 32] |= code << (i * BITS % 32);
         }

@@ -84,7 +84,7 @@ def test_write_refusals(lib, kw, message):
     (dict(q=0), "null pointer"), (dict(ws=0), "null pointer"), (dict(q_start=0), "null pointer"), (dict(n_q=3), "n_q = 3"), (dict(n_q=1), "n_q = 1"), (dict(B=0), "B = 0"),
     (dict(max_q=0), "max_q = 0"), (dict(q_ld=511), "row strides"), (dict(out_ld=516), "row strides"), (dict(q=(5 << 20) + 2), "16-byte aligned"),
     (dict(ws=(12 << 20) + 4), "16-byte aligned"), (dict(out=(5 << 20) + 64), "overlaps"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=0.0), "scale"), (dict(scale=-0.1), "scale"),
-    (dict(cap=-1.0), "softcap"), (dict(window=-1), "window = -1"), (dict(window=1 << 31), "window"), (dict(ws_bytes=16), "workspace of 16 bytes, needs"),
+    (dict(cap=-1.0), "softcap"), (dict(cap=1e-9), "softcap"), (dict(cap=float("nan")), "softcap"), (dict(window=-1), "window = -1"), (dict(window=1 << 31), "window"), (dict(ws_bytes=16), "workspace of 16 bytes, needs"),
 ])
 def test_attend_refusals(lib, kw, message):
     if "ws_bytes" in kw:

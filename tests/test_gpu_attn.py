@@ -538,3 +538,91 @@ def test_steps_of_write_and_attend_together(cuda, bits, G):
         want, _, tol, _ = plain.attend(q, cache, pages, starts, kv_len, D ** -0.5)
         assert (np.abs(plain.f64(out).reshape(want.shape) - want) <= tol).all(), step
         assert int(err[0]) == 0
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_layer_is_its_parts(cuda, bits, G):
+    """Two layers over buffers of their own stack: a prompt by the tensor-core projections, then steps of one token and of drafts.  Every step's output is
+    what the launchers give one by one, bit for bit, and the attention in it is the definition's."""
+    from strixite_b200.attention import AttnBatch, AttnBuffers, AttnLayer, AttnWeights
+    D, n_q, n_kv, page, d = 64, 4, 2, 16, 256
+    g = torch.Generator(device=cuda)
+    g.manual_seed(bits)
+    def weight(n, k):
+        return K().quantize(torch.randn((n, k), generator=g, device=cuda) * 0.05, 64, 8)
+    inv = (1e4 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).float().to(cuda)
+    caches = [K().KvCache.empty(20, n_kv, page, D, bits, G, cuda) for _ in range(2)]
+    buf = AttnBuffers(100, 80, n_q, caches[0])
+    layers = [AttnLayer(AttnWeights(weight((n_q + 2 * n_kv) * D, d), weight(d, n_q * D), 1 + 0.1 * torch.randn(D, generator=g, device=cuda),
+                                    1 + 0.1 * torch.randn(D, generator=g, device=cuda), inv), n_q, c, buf) for c in caches]
+    pages = torch.randperm(20, generator=g, device=cuda)[:18].to(torch.int32).view(2, 9)
+    kept = [0, 0]
+    for new in ((80, 3), (1, 1), (1, 4), (0, 1)):
+        x = torch.randn((sum(new), d), generator=g, device=cuda).to(torch.bfloat16)
+        batch = AttnBatch.of(kept, new, pages)
+        kept = [k + n for k, n in zip(kept, new)]
+        for layer in layers:
+            T, w = sum(new), layer.w
+            y = torch.empty((T, d), dtype=torch.bfloat16, device=cuda)
+            layer.forward(x, batch, y)
+            layer.check_errors()
+            o, q = buf.o[:T].clone(), buf.q[:T].clone()
+            want, _, tol, _ = plain.attend(q, layer.cache, pages, batch.q_start, batch.kv_len, D ** -0.5)
+            assert (np.abs(plain.f64(o).reshape(want.shape) - want) <= tol).all()
+            linear = K().linear_qw_wmma if T >= 64 else K().linear_qw
+            qkv, q2, o2, y2 = torch.empty_like(buf.qkv[:T]), torch.empty_like(q), torch.empty_like(o), torch.empty_like(y)
+            linear(x, w.qkv, qkv, T, K().Act.BF16, K().Act.F32)
+            K().attn_qkv_write(qkv, layer.cache, batch.seq, batch.pos, pages, q2, buf.err, q_norm=w.q_norm, k_norm=w.k_norm, inv_freq=inv)
+            K().attn_decode(q2, layer.cache, pages, batch.q_start, batch.kv_len, batch.max_q, o2, buf.ws, buf.err)
+            linear(o2, w.out, y2, T, K().Act.BF16, K().Act.BF16)
+            assert torch.equal(q, q2) and torch.equal(o, o2) and torch.equal(y, y2)
+            x = (x.float() + y.float()).to(torch.bfloat16)
+    with pytest.raises(K().Error, match="the buffers hold 100"):
+        layers[0].forward(torch.zeros((101, d), dtype=torch.bfloat16, device=cuda), batch, y)
+    with pytest.raises(K().Error, match="do not fit 3 query"):
+        AttnLayer(layers[0].w, 3, caches[0], buf)
+
+
+def test_python_refusals_on_the_device(cuda):
+    """Another type, another device, a vector that is not contiguous, shapes that do not fit: refused by name before anything is enqueued."""
+    b = Batch(cuda, 64, 16, 0, 2, 2, [40, 20], [2, 1], seed=1)
+    def attend(**kw):
+        a = dict(q=b.q, cache=b.cache, pages=b.pages, q_start=b.q_start, kv_len=b.kv_len, max_q=2, out=b.out, ws=b.ws, err=b.err, lse=b.lse)
+        a.update(kw)
+        K().attn_decode(**a)
+    for kw, said in ((dict(q=b.q.float()), "q is torch.float32"), (dict(kv_len=b.kv_len.long()), "kv_len is torch.int64"), (dict(pages=b.pages.cpu()), "pages is torch.int32 on cpu"),
+                     (dict(q_start=b.q_start[:2]), "shapes do not fit"), (dict(out=b.out[:, :64]), "shapes do not fit"), (dict(lse=b.lse[:2]), "shapes do not fit"),
+                     (dict(q=b.q.t().contiguous().t()), "last dimension contiguous"), (dict(err=b.err[:2]), "shapes do not fit"), (dict(ws=b.ws[:64]), "workspace of 64 bytes"),
+                     (dict(q_start=torch.zeros(6, dtype=torch.int32, device=cuda)[::2]), "q_start is"), (dict(softcap=1e-9), "softcap"), (dict(max_q=0), "max_q = 0")):
+        with pytest.raises(K().Error, match=said):
+            attend(**kw)
+    r = Rows(cuda, 4, 2, 2, 1, 64, 8, 32)
+    with pytest.raises(K().Error, match="shapes do not fit"):
+        K().attn_qkv_write(r.qkv, r.cache, r.seq[:3], r.pos, r.pages, r.q_out, r.err)
+    with pytest.raises(K().Error, match="q_out is torch.float32"):
+        K().attn_qkv_write(r.qkv, r.cache, r.seq, r.pos, r.pages, r.q_out.float(), r.err)
+    with pytest.raises(K().Error, match="rot = 24"):
+        K().attn_qkv_write(r.qkv, r.cache, r.seq, r.pos, r.pages, r.q_out, r.err, inv_freq=torch.ones(12, device=cuda))
+    with pytest.raises(K().Error, match="v_out is torch.float32"):
+        K().kv_read(r.cache, r.seq, r.pos, r.pages, torch.empty((4, 1, 64), dtype=torch.bfloat16, device=cuda), torch.empty((4, 1, 64), device=cuda), r.err)
+    with pytest.raises(K().Error, match="k_sm is"):
+        K().KvCache(r.cache.k, r.cache.v, 8, 32, r.cache.k_sm[..., :1, :], r.cache.v_sm)
+    with pytest.raises(K().Error, match="not whole rows|not those of k"):
+        K().KvCache(torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16, device=cuda), torch.zeros((2, 16, 2, 64), dtype=torch.bfloat16, device=cuda).transpose(1, 2), 16)
+
+
+def test_attend_queries_that_are_none_stay_in_their_rows(cuda):
+    """A NaN or an infinity in one query: its row is NaN, the others as ever (all heads of a key head share a tile)."""
+    for bits, G in ((16, 0), (8, 64), (4, 32)):
+        for bad in (float("nan"), float("inf")):
+            b = Batch(cuda, 128, bits, G, 2, 4, [300], [2], seed=17)
+            b.q[0, 128 + 7] = bad  # head 1 of the first token
+            b.run()
+            torch.cuda.synchronize()
+            got = plain.f64(b.out).reshape(2, 8, 128)
+            assert np.isnan(got[0, 1]).all()
+            b.q[0, 128 + 7] = 0.0
+            want, _, tol, _ = plain.attend(b.q, b.cache, b.pages, b.q_start, b.kv_len, 128 ** -0.5)
+            ok = np.ones((2, 8), bool)
+            ok[0, 1] = False
+            assert (np.abs(got[ok] - want[ok]) <= tol[ok]).all()
