@@ -6,14 +6,20 @@
 // of R query rows) - and every CTA takes an equal run of it, across the ends of heads and sequences: a batch of uneven lengths, or one long sequence
 // alone, keeps all SMs equally busy, whatever the host knows of the lengths, and a captured graph follows them.  A segment (all units of one row tile)
 // that lies in one CTA is written by it; the parts of one that several CTAs share go to the workspace, FP32 with their maxima and sums, at most two a
-// CTA, and the last CTA to arrive joins them in the list's order, so that no result depends on who came last.
+// CTA, and the last CTA to arrive (or, for many rows, a second kernel) joins them in the list's order, so that no result depends on who came last.
 //
 // The query heads of a key head and the new tokens of a sequence are the rows of one MMA tile: the cache is read once for all of them.  Products on
-// mma.sync, whose operands come from shared memory, tiles there by cp.async from wherever the pages lie.
+// mma.sync: the rows are eight to 32, a warp's keys sixteen, and what bounds is memory (BF16) or the conversion of codes, not the tensor cores; operands
+// come from shared memory, tiles there by cp.async from wherever the pages lie, each warp's by itself.
 //   BF16 cache: exact products; weights rounded to BF16 (one rounding of 2^-9 a key, against the sum's many keys).
 //   8 and 4 bits: the codes are F16 numbers exactly, q is F16 times a power of two a row (a BF16 number less than 2^28 below the row's largest is exact),
 //   scale and min go on in FP32: s = scale_k * (q . code) + min_k * sum(q) a group.  For V a key's weight takes its group's scale, times a power of
 //   two that follows the largest scale seen so that F16's range is no limit (one rounding of 2^-11); the mins' share, sum p * min, is FP32.
+//
+// Measured (B200; us, and the time of the bytes alone at the measured copy rate): one sequence of 200001 keys, 8 key heads of 128, BF16, 132 (125); 64
+// sequences of 100 to 16000 keys, 8 bits, 185 (172); 32 of 9509, 4 bits with groups of 32, 139 (59): there the bound is the integer pipe, half busy with
+// codes and scales, behind it two to three warps a scheduler.  Several rows: 32 sequences x 4 rows of 8 heads x 9509 keys BF16 109 (95), 8 bits 154 (51).
+// 300 keys of one sequence: 7, nothing but latencies - lengths, page table, keys, join.
 
 #include "attn.cuh"
 
@@ -110,7 +116,7 @@ template <class S> __device__ inline Sequence sequence(const Args &a, int b) {
     s.bad = s.len < 0 || s.len > a.capacity;
     if (s.bad) s.len = 0;
     s.p0 = s.len - s.n;
-    s.lo = a.window > 0 ? max(0, s.p0 - a.window + 1) : 0;
+    s.lo = a.window > 0 ? (int)max((int64_t)0, (int64_t)s.p0 - a.window + 1) : 0;
     s.tile0 = s.lo / S::TK;
     s.tiles = max(1, (s.len + S::TK - 1) / S::TK - s.tile0);
     s.row_tiles = (int)(((int64_t)s.n * a.group + S::R - 1) / S::R);
@@ -643,7 +649,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                             w[pos / 2] = pack_f16(x[b][d0] * f, x[b][d1] * f);
                             const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&w[pos / 2]));
                             sums[b] += back.x + back.y;
-                                                    }
+                        }
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
                             *reinterpret_cast<uint4 *>(qs + chunk_at<D / 8>(r, blk * 4 + c) * 16) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
@@ -774,7 +780,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int tok = (sg.rows0 + nt * 8 + 2 * t4 + e) / a.group;
-                    const int hi = tok < sg.n ? sg.p0 + tok : -1, lo = a.window > 0 ? max(-1, hi - a.window) : -1;
+                    const int hi = tok < sg.n ? sg.p0 + tok : -1, lo = a.window > 0 ? (int)max((int64_t)-1, (int64_t)hi - a.window) : -1;
 #pragma unroll
                     for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
@@ -1248,7 +1254,7 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
     const size_t need = sxb_attn_decode_workspace_bytes(n_q, n_kv, D, cache->bits, max_q);
     SXB_CHECK(args->ws_bytes >= need, fn, ": workspace of ", args->ws_bytes, " bytes, needs ", need);
     a.q = static_cast<const uint16_t *>(q), a.q_ld = q_ld, a.pages = pages, a.pages_ld = pages_ld, a.capacity = n_cols * cache->page;
-    a.q_start = q_start, a.kv_len = kv_len, a.B = (int)B, a.T = (int)T, a.n_q = (int)n_q, a.group = (int)(n_q / n_kv), a.window = (int)window;
+    a.q_start = q_start, a.kv_len = kv_len, a.B = (int)B, a.T = (int)T, a.n_q = (int)n_q, a.group = (int)(n_q / n_kv), a.window = window >= a.capacity ? 0 : (int)window;
     a.scale = scale, a.softcap = softcap, a.out = static_cast<uint16_t *>(out), a.out_ld = out_ld, a.lse = args->lse, a.err = err;
     const uint32_t chunks = (uint32_t)(D * cache->bits / 8 / 16), words = cache->bits == 16 ? 0 : (uint32_t)(D / cache->G), pieces = words > 4 ? words / 4 : words ? 1 : 0;
     a.page_chunks = (uint32_t)cache->page_stride * chunks, a.head_chunks = (uint32_t)cache->head_stride * chunks, a.row_chunks = (uint32_t)cache->row_stride * chunks;

@@ -115,7 +115,7 @@ def test_attend_pages(cuda, bits, G, page):
     b.check()
 
 
-@pytest.mark.parametrize("window", [1, 5, 64, 100, 5000])
+@pytest.mark.parametrize("window", [1, 5, 64, 100, 5000, (1 << 31) - 1])
 @pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
 def test_attend_window_and_cap(cuda, bits, G, window):
     b = Batch(cuda, 128, bits, G, 2, 4, [1000, 64, 3, 130, 2], [3, 2, 3, 1, 4], seed=window)
