@@ -567,7 +567,8 @@ int sxb_kv_read(const SxbKvReadArgs *args, sxb_stream_t stream);
  * (or none with a score above -1e30): 0 and -inf.  Rows outside every sequence are left as they are.  Scores, statistics and
  * sums are FP32; weights are rounded to BF16 (BF16 cache) or, times a group's scale, to F16 for the product with V.
  * max_q: a sequence's largest count of new tokens, which picks the kernel (a sequence with more is handled, in several passes over
- * its keys).  Made for a token and its drafts; long chunks of queries are right but no match for a prefill kernel.
+ * its keys).  Chunks of prompt tokens: over a BF16 cache with heads of 128 more than 32 rows a key head run on tcgen05, 128 at a time (a device-side
+ * wait that ran out there is reported by sxb_check_dense_status); other caches' are right, 16 or 32 rows at a time, and slow.
  * ws: sxb_attn_decode_workspace_bytes, device, 16-byte aligned, zeroed once before its first use; every call leaves what it needs
  * of it zeroed.  Calls that share a workspace must be ordered (one stream, or events); the sizes depend on the device.
  * Data errors (err = {1, sequence, value}): a page id out of range makes the keys on that page NaN; kv_len outside

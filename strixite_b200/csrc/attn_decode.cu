@@ -22,6 +22,8 @@
 // 300 keys of one sequence: 7, nothing but latencies - lengths, page table, keys, join.
 
 #include "attn.cuh"
+#include "skinny_mma.cuh"
+#include "tc_ptx.cuh"
 
 #include <math_constants.h>
 
@@ -31,7 +33,7 @@
 namespace sxb {
 namespace {
 
-#define SXB_RARE(c) __builtin_expect(!!(c), 0)  // out of the loop's way: what the loop runs through has to stay in the instruction cache
+#define SXB_RARE(c) __builtin_expect(!!(c), 0)  // out of the loop's way
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMostPerSm = 4;
@@ -92,6 +94,8 @@ struct Args {
     float *lse, *partial;
     uint32_t *count, *err;
     struct Join *joins;
+    uint32_t *status;                  // of the tcgen05 form: a wait that ran out
+    unsigned long long wait_limit_ns;
     // distances in pieces of sixteen bytes (codes) and of a row's scales: a cache has fewer than 2^32 of either
     uint32_t page_chunks, head_chunks, row_chunks, page_pieces, head_pieces, row_pieces;
 };
@@ -187,7 +191,7 @@ template <bool F16> __device__ inline void mma(float (&d)[4], const uint32_t (&a
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ inline float exp2_fast(float v) {  // 2 ulp; exp2(-inf) = 0
+__device__ inline float exp2_flushed(float v) {  // 2 ulp; exp2(-inf) = 0
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
@@ -333,11 +337,11 @@ template <int BATCH, int R, int D> __device__ inline void join_run(const Args &a
         }
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) now = fmaxf(now, m[k]);
-        const float before = exp2_fast(top - now);
+        const float before = exp2_flushed(top - now);
         v.x *= before, v.y *= before, v.z *= before, v.w *= before, sum *= before, top = now;
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
-            const float f = exp2_fast(m[k] - top);
+            const float f = exp2_flushed(m[k] - top);
             sum = fmaf(l[k], f, sum), v.x = fmaf(w[k].x, f, v.x), v.y = fmaf(w[k].y, f, v.y), v.z = fmaf(w[k].z, f, v.z), v.w = fmaf(w[k].w, f, v.w);
         }
     }
@@ -350,14 +354,96 @@ template <int BATCH, int R, int D> __device__ inline void join_run(const Args &a
 }
 
 constexpr int kJoinRows = 8;
-// Block (c, y): rows 8 y .. 8 y + 7 of the segment that began in CTA c, a thread four columns.
+// Block (c, y): rows 8 y .. 8 y + 7 of the segment that began in CTA c, and as many again while there are more than were told of; a thread four columns.
 template <class S>
 __global__ void __launch_bounds__(kJoinRows * S::D / 4) attn_join_kernel(const __grid_constant__ Args a) {
     behind_grid();
     const Join j = a.joins[blockIdx.x];
-    const int r = blockIdx.y * kJoinRows + threadIdx.x / (S::D / 4);
-    if (j.parts == 0 || r >= j.rows) return;
-    join_run<8>(a, Parts<S::R, S::D>(a.partial, (int)blockIdx.x, j.parts), j.q0, j.rows0, j.head, r, threadIdx.x % (S::D / 4));
+    if (j.parts == 0) return;
+    for (int r = blockIdx.y * kJoinRows + threadIdx.x / (S::D / 4); r < j.rows; r += gridDim.y * kJoinRows)
+        join_run<8>(a, Parts<S::R, S::D>(a.partial, (int)blockIdx.x, j.parts), j.q0, j.rows0, j.head, r, threadIdx.x % (S::D / 4));
+}
+
+// The cursor of a warp at its next segment; false: there is none.
+template <class S> __device__ inline bool next_segment(const Args &a, Cursor &cur, int lane) {
+    Cursor c = cur;
+    ++c.segment;
+    if (++c.row_tile == c.s.row_tiles) {
+        c.row_tile = 0;
+        if (++c.head == a.c.n_kv) {
+            c.head = 0;
+            do {
+                if (++c.b >= a.B) return false;
+                c.s = sequence<S>(a, c.b);
+            } while (c.s.n == 0);
+        }
+    }
+    __syncwarp();
+    if (lane == 0) cur = c;
+    __syncwarp();
+    return true;
+}
+
+// This CTA's run of the list: its first and last unit, all units, the CTAs that have one; the sequence of the first and the unit's number in it.  False: none.
+struct Share {
+    int64_t u0, u1, total, ctas;
+    int b;
+    int64_t in;
+};
+// By the whole CTA; scan: [kWarps + 2].
+template <class S> __device__ inline bool find_share(const Args &a, int64_t *scan, Share &out) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int64_t total = 0;
+    for (int b = tid; b < a.B; b += S::kThreads) {
+        const Sequence s = sequence<S>(a, b);
+        if (s.bad && blockIdx.x == 0) raise_error(a.err, (uint32_t)b, (uint32_t)a.kv_len[b]);
+        total += (int64_t)s.tiles * s.row_tiles * a.c.n_kv;
+    }
+    if (!S::kJoinHere && tid == 0) a.joins[blockIdx.x].parts = 0;
+    const int64_t mine = total;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    if (lane == 0) scan[warp] = total;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < S::kWarps; ++w) total += scan[w];
+    const int64_t ctas = min((int64_t)gridDim.x, total);
+    if ((int64_t)blockIdx.x >= ctas) return false;
+    const int64_t u0 = blockIdx.x * total / ctas, u1 = (blockIdx.x + 1) * total / ctas;
+    out = Share{u0, u1, total, ctas, 0, 0};
+    for (int64_t base = 0, before = 0; base < a.B; base += S::kThreads) {
+        int64_t own = mine;
+        if (a.B > S::kThreads) {
+            own = 0;
+            if (base + tid < a.B) {
+                const Sequence s = sequence<S>(a, (int)base + tid);
+                own = (int64_t)s.tiles * s.row_tiles * a.c.n_kv;
+            }
+        }
+        int64_t upto = own;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, upto, off);
+            if (lane >= off) upto += v;
+        }
+        __syncthreads();
+        if (lane == 31) scan[warp] = upto;
+        __syncthreads();
+        int64_t ahead = before, all = before;
+#pragma unroll
+        for (int w = 0; w < S::kWarps; ++w) {
+            if (w < warp) ahead += scan[w];
+            all += scan[w];
+        }
+        upto += ahead;
+        if (upto - own <= u0 && u0 < upto) scan[S::kWarps] = base + tid, scan[S::kWarps + 1] = u0 - (upto - own);
+        before = all;
+        if (before > u0) break;
+    }
+    __syncthreads();
+    out.b = (int)scan[S::kWarps], out.in = scan[S::kWarps + 1];
+    return true;
 }
 
 template <class S>
@@ -383,61 +469,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 
     behind_grid();
 
-    // ---- this CTA's run of the list ----
-    int64_t total = 0;
-    for (int b = tid; b < a.B; b += kThreads) {
-        const Sequence s = sequence<S>(a, b);
-        if (s.bad && blockIdx.x == 0) raise_error(a.err, (uint32_t)b, (uint32_t)a.kv_len[b]);
-        total += (int64_t)s.tiles * s.row_tiles * a.c.n_kv;
-    }
-    if (!S::kJoinHere && tid == 0) a.joins[blockIdx.x].parts = 0;
-    const int64_t mine = total;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-    if (lane == 0) scan[warp] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) total += scan[w];
-    const int64_t ctas = min((int64_t)gridDim.x, total);
-    if ((int64_t)blockIdx.x >= ctas) return;
-    const int64_t u0 = blockIdx.x * total / ctas, u1 = (blockIdx.x + 1) * total / ctas;
-    for (int64_t base = 0, before = 0; base < a.B; base += kThreads) {
-        int64_t own = mine;
-        if (a.B > kThreads) {
-            own = 0;
-            if (base + tid < a.B) {
-                const Sequence s = sequence<S>(a, (int)base + tid);
-                own = (int64_t)s.tiles * s.row_tiles * a.c.n_kv;
-            }
-        }
-        int64_t upto = own;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, upto, off);
-            if (lane >= off) upto += v;
-        }
-        __syncthreads();
-        if (lane == 31) scan[warp] = upto;
-        __syncthreads();
-        int64_t ahead = before, all = before;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) ahead += scan[w];
-            all += scan[w];
-        }
-        upto += ahead;
-        if (upto - own <= u0 && u0 < upto) scan[kWarps] = base + tid, scan[kWarps + 1] = u0 - (upto - own);
-        before = all;
-        if (before > u0) break;
-    }
-    __syncthreads();
+    Share share;
+    if (!find_share<S>(a, scan, share)) return;
+    const int64_t u0 = share.u0, u1 = share.u1, total = share.total, ctas = share.ctas, in = share.in;
 
     // ---- the cursor of the loads: kStages - 1 units ahead of the sums ----
-    const int64_t in = scan[kWarps + 1];
     {
         Cursor c;
-        c.b = (int)scan[kWarps], c.s = sequence<S>(a, c.b), c.segment = 0;
+        c.b = share.b, c.s = sequence<S>(a, c.b), c.segment = 0;
         const int64_t per_head = (int64_t)c.s.tiles * c.s.row_tiles;
         c.head = (int)(in / per_head), c.row_tile = (int)((in - c.head * per_head) / c.s.tiles);
         if (lane == 0) cur = c;
@@ -475,22 +514,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     auto advance = [&]() {
         l_new = false, l_run0 += TK;
         if (__builtin_expect(--l_tiles > 0, 1)) return;
-        Cursor c = cur;
-        ++c.segment;
-        if (++c.row_tile == c.s.row_tiles) {
-            c.row_tile = 0;
-            if (++c.head == a.c.n_kv) {
-                c.head = 0;
-                do {
-                    if (++c.b >= a.B) return;
-                    c.s = sequence<S>(a, c.b);
-                } while (c.s.n == 0);
-            }
-        }
-        __syncwarp();
-        if (lane == 0) cur = c;
-        __syncwarp();
-        at_segment(0);
+        if (next_segment<S>(a, cur, lane)) at_segment(0);
     };
     auto load = [&](int stage) {
         const uint32_t by = stage * S::kStage;
@@ -768,7 +792,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                 for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(-2.f * to, reciprocal_fast(exp2_fast(s[ki][nt][e] * (fac[nt][e & 1] * by)) + 1.f), to);
+                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(-2.f * to, reciprocal_fast(exp2_flushed(s[ki][nt][e] * (fac[nt][e & 1] * by)) + 1.f), to);
                 fac[nt][0] = fac[nt][1] = 1.f;
             }
         }
@@ -817,7 +841,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
                     const float now = fmaxf(m[nt][e], v * fac[nt][e]);
-                    f[nt][e] = exp2_fast(m[nt][e] - now);
+                    f[nt][e] = exp2_flushed(m[nt][e] - now);
                     m[nt][e] = now, l[nt][e] *= f[nt][e];
 #pragma unroll
                     for (int grp = 0; grp < kGroups; ++grp) o_min[grp][nt][e] *= f[nt][e];
@@ -837,7 +861,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[ki][nt][e] = exp2_fast(fmaf(s[ki][nt][e], fac[nt][e & 1], -m[nt][e & 1]));
+                    s[ki][nt][e] = exp2_flushed(fmaf(s[ki][nt][e], fac[nt][e & 1], -m[nt][e & 1]));
                     l[nt][e & 1] += s[ki][nt][e];
                 }
 
@@ -945,7 +969,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                             if (x != 255) ex = max(ex, x);  // a scale that is none says nothing of the others
                         }
                     ex = max(v_exp, __reduce_max_sync(0xffffffffu, ex));
-                    const float down = exp2_fast((float)(v_exp - ex));
+                    const float down = exp2_flushed((float)(v_exp - ex));
                     v_exp = ex, v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
@@ -1051,7 +1075,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             for (int k = 1; k < WK; ++k) top = fmaxf(top, row_max[k * R + tid]);
 #pragma unroll
             for (int k = 0; k < WK; ++k) {
-                const float f = exp2_fast(row_max[k * R + tid] - top);
+                const float f = exp2_flushed(row_max[k * R + tid] - top);
                 row_max[k * R + tid] = f, sum = fmaf(row_sum[k * R + tid], f, sum);
             }
             row_top[tid] = top, row_sum[tid] = sum;
@@ -1143,22 +1167,37 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     }
 }
 
+#include "attn_decode_tc.cuh"
+
 // The rows of a tile for those that a key head's queries make: more query heads a key head or more drafts, more rows, until registers end; what is
 // above takes several tiles, and reads the keys for each.  Quantized keys' conversions are most of the work, and sixteen rows leave registers for two runs
 // side by side: eight conversations of one to eight rows of eight heads, 39 us with sixteen, 48 with 32; BF16, four rows of eight heads, 200 with sixteen,
-// 109 with 32.  (64 rows by pairs of warps: 54, and 184 where two tiles of 32 take 200 us.)
+// 109 with 32.  (Tiles of 32 and 64 rows whose warps share out V's columns, the weights by way of shared memory, are slower everywhere: the first
+// of these 54 to 58.)
 constexpr int most_rows(int D, int bits) { return bits == 16 && D <= 128 ? 32 : 16; }
 inline int tile_rows(int D, int bits, int64_t rows) { return rows <= 8 ? 8 : rows <= 16 || most_rows(D, bits) == 16 ? 16 : 32; }
+// Tiles of 128 rows on tcgen05 (attn_decode_tc.cuh): more than 32 rows, and enough tiles a table has room for that its start - tensor memory, three stages to
+// fill before the first product - is no matter.  Rows, sequences x keys, us with tiles of 32 and with it: 64, 64 x 8000, 190 and 147; 2 x 33000, 52 and 47;
+// 16 x 1000, 25 and 27; 1 x 300, 11 and 16; 128, 64 x 8000, 463 and 185; 16 x 1000, 35 and 36; chunks of 512 tokens of eight heads on 4096 keys,
+// 170 and 62, of 2048 on 8192, 1341 and 293.
+constexpr bool has_tc(int D, int bits) { return D == TcShape::D && bits == TcShape::BITS; }
+inline bool takes_tc(int D, int bits, int64_t rows, int64_t B, int64_t n_kv, int64_t capacity) {
+    if (!has_tc(D, bits) || rows <= most_rows(D, bits)) return false;
+    return rows > TcShape::R || (double)B * (double)n_kv * (double)((capacity + TcShape::TK - 1) / TcShape::TK) >= 8.0 * sm_count();
+}
 
 // The counters' place is every form's: calls of different ones share a workspace.
 inline size_t counter_bytes() { return ((size_t)sm_count() * kMostPerSm * (sizeof(uint32_t) + sizeof(Join)) + 255) / 256 * 256; }
+
+template <class S> struct Kernel { static constexpr auto fn = attn_decode_kernel<S>; };
+template <> struct Kernel<TcShape> { static constexpr auto fn = attn_tc_kernel<TcShape>; };
 
 template <class S> struct Launch {
     static_assert(S::kPerSm <= kMostPerSm, "");
 
     static int64_t ctas() { return (int64_t)sm_count() * S::kPerSm; }
     static size_t bytes() { return counter_bytes() + (size_t)(ctas() * 2 * S::R * (S::D + 2) * 4); }
-    static cudaError_t run(Args a, void *ws, int64_t most_units, cudaStream_t st) {
+    static cudaError_t run(Args a, void *ws, int64_t most_units, int told_rows, cudaStream_t st) {
         const int64_t n = std::max<int64_t>(1, std::min(ctas(), most_units));
         a.count = static_cast<uint32_t *>(ws);
         a.joins = reinterpret_cast<Join *>(a.count + (size_t)sm_count() * kMostPerSm);
@@ -1168,18 +1207,22 @@ template <class S> struct Launch {
         if (const cudaError_t rc = cudaGetDevice(&dev); rc != cudaSuccess) return rc;
         const uint64_t bit = dev < 64 ? 1ull << dev : 0;
         if ((told.load(std::memory_order_acquire) & bit) == 0) {
-            if (const cudaError_t rc = cudaFuncSetAttribute(attn_decode_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); rc != cudaSuccess) return rc;
+            if (const cudaError_t rc = cudaFuncSetAttribute(Kernel<S>::fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); rc != cudaSuccess) return rc;
+            // (an SM's shared memory stays as the form wants it: it need not be empty for the next call's CTAs)
+            if (const cudaError_t rc = cudaFuncSetAttribute(attn_join_kernel<S>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); rc != cudaSuccess) return rc;
             told.fetch_or(bit, std::memory_order_release);
         }
-        const cudaError_t rc2 = launch_behind(attn_decode_kernel<S>, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a);
+        const cudaError_t rc2 = launch_behind(Kernel<S>::fn, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a);
         if (S::kJoinHere || rc2 != cudaSuccess) return rc2;
-        return launch_behind(attn_join_kernel<S>, dim3((unsigned)n, S::R / kJoinRows), dim3(kJoinRows * S::D / 4), 0, st, 1, a);
+        return launch_behind(attn_join_kernel<S>, dim3((unsigned)n, (unsigned)((told_rows + kJoinRows - 1) / kJoinRows)), dim3(kJoinRows * S::D / 4), 0, st, 1, a);
     }
 };
 
 // f(Shape) for the sizes of a call.
 template <int D, int BITS, int G, class F> auto with_rows(int rows, F f) {
     if (rows == 8) return f(Shape<D, BITS, G, 8>{});
+    if constexpr (has_tc(D, BITS))
+        if (rows == 128) return f(TcShape{});
     if constexpr (most_rows(D, BITS) == 32)
         if (rows == 32) return f(Shape<D, BITS, G, 32>{});
     return f(Shape<D, BITS, G, 16>{});
@@ -1215,8 +1258,10 @@ extern "C" size_t sxb_attn_decode_workspace_bytes(int64_t n_q, int64_t n_kv, int
         return 0;
     }
     size_t most = 0;  // of a call with fewer rows too, and of any group size: how many CTAs an SM holds depends on both
-    for (int rows = 8; rows <= tile_rows((int)D, bits, max_q * (n_q / n_kv)); rows *= 2)
+    const int64_t told = max_q * (n_q / n_kv);
+    for (int rows = 8; rows <= tile_rows((int)D, bits, told); rows *= 2)
         for (int G = 32; G <= D && G <= 128; G *= 2) most = std::max(most, with_shape(D, bits, G, rows, [](auto s) { return Launch<decltype(s)>::bytes(); }));
+    if (has_tc((int)D, bits) && told > most_rows((int)D, bits)) most = std::max(most, Launch<TcShape>::bytes());
     return most;
 }
 
@@ -1250,7 +1295,9 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
     SXB_CHECK(scale > 0.f && scale < 1e30f, fn, ": scale must be finite and positive");
     SXB_CHECK(softcap == 0.f || (softcap >= 1e-6f && softcap < 1e30f), fn, ": softcap = ", softcap, ", expected 0 (none) or 1e-6 .. 1e30");
     SXB_CHECK(window >= 0 && window < (1ll << 31), fn, ": window = ", window, ", expected 0 (none) .. 2^31 - 1");
-    const int rows = tile_rows((int)D, cache->bits, max_q * (n_q / n_kv));
+    const int64_t told = max_q * (n_q / n_kv);
+    const bool tc = takes_tc((int)D, cache->bits, told, B, n_kv, n_cols * cache->page);
+    const int rows = tc ? TcShape::R : tile_rows((int)D, cache->bits, told);
     const size_t need = sxb_attn_decode_workspace_bytes(n_q, n_kv, D, cache->bits, max_q);
     SXB_CHECK(args->ws_bytes >= need, fn, ": workspace of ", args->ws_bytes, " bytes, needs ", need);
     a.q = static_cast<const uint16_t *>(q), a.q_ld = q_ld, a.pages = pages, a.pages_ld = pages_ld, a.capacity = n_cols * cache->page;
@@ -1259,13 +1306,17 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
     const uint32_t chunks = (uint32_t)(D * cache->bits / 8 / 16), words = cache->bits == 16 ? 0 : (uint32_t)(D / cache->G), pieces = words > 4 ? words / 4 : words ? 1 : 0;
     a.page_chunks = (uint32_t)cache->page_stride * chunks, a.head_chunks = (uint32_t)cache->head_stride * chunks, a.row_chunks = (uint32_t)cache->row_stride * chunks;
     a.page_pieces = (uint32_t)cache->page_stride * pieces, a.head_pieces = (uint32_t)cache->head_stride * pieces, a.row_pieces = (uint32_t)cache->row_stride * pieces;
+    if (tc) {
+        if (int rc = library_status_words(fn, &a.status)) return rc;
+        a.wait_limit_ns = wait_limit_ns();
+    }
     auto st = static_cast<cudaStream_t>(stream);
     const cudaError_t rc = with_shape(D, cache->bits, cache->G, rows, [&](auto s) {
         using S = decltype(s);
         if (Launch<S>::bytes() > args->ws_bytes) return cudaErrorInvalidValue;  // nothing is written behind the workspace, whatever the sizes above say
         // no list is longer than every sequence at its table's end (in a product that cannot overflow: the grid is a few hundred CTAs)
         const double most = (double)((a.capacity + S::TK - 1) / S::TK) * (double)B * n_kv * (double)((T * a.group + S::R - 1) / S::R + 1);
-        return Launch<S>::run(a, ws, (int64_t)std::min(most, 1e12), st);
+        return Launch<S>::run(a, ws, (int64_t)std::min(most, 1e12), (int)std::min<int64_t>(S::R, told), st);
     });
     if (rc != cudaSuccess) return fail_cuda(SXB_FILE_, __LINE__, __func__, rc, cat(fn, " launch"));
     SXB_CHECK_LAUNCH(fn, " T=", T, " B=", B, " n_q=", n_q, " n_kv=", n_kv, " D=", D, " bits=", cache->bits);

@@ -1,0 +1,486 @@
+// The form of sxb_attn_decode for many rows (BF16 cache, heads of 128): products on tcgen05, accumulators in tensor memory.  Part of attn_decode.cu.
+//
+//   S [128 rows, 128 keys] = Q K^T,   P = exp2(S * scale - M),   O [128 rows, 128 columns] += P V
+//
+// K and V lie in shared memory as they lie in the cache, a line a key; the second product reads V across its lines and P from tensor memory, where P takes
+// S's place.  Eight warps make weights: a thread has a row and half of a tile's keys, with a maximum, a sum and sums of values of that half's own, which
+// are joined at a segment's end, so that no thread waits for another one's scores.  The maximum that a row goes by is raised, and its sums scaled, only by a
+// tile that passes it by more than 2^kSlack.  One warp issues the products, the next tile's scores ahead of this one's weights; three fetch.
+
+template <int STAGES> struct TcMisc {
+    float top[2][128], sum[2][128];
+    int64_t scan[12 + 2];
+    uint64_t full[STAGES], empty[STAGES], scores_done[2], weights[2], sums_done, queries;
+    Segment segments[STAGES + 1];       // of what is on its way, and of the tile whose sums go out
+    Cursor cur[3];
+    uint32_t tmem;
+    int abort, how[2];                  // what becomes of a tile's weights: kMma, kMade, kNone
+};
+constexpr int kMma = 0, kMade = 1, kNone = 2;  // the MMA takes them, the threads have, no row sees the tile
+struct TcShape {
+    static constexpr int D = 128, BITS = 16, R = 128;
+    static constexpr int kSums = 8, kLoads = 3;                  // warps that have the scores and sums, warps that fetch
+    static constexpr int kWarps = kSums + kLoads + 1, kThreads = 32 * kWarps, RUN = 16, TK = 128, kPerSm = 1;
+    static constexpr int RB = 2 * D, CR = RB / 16;
+    static constexpr int kPlane = TK * 128, kTile = 2 * kPlane, kStage = 2 * kTile;  // 64 columns of a tile's keys (lines of 128 bytes); keys or values; both
+    static constexpr int kQ = R * D * 2, kStages = 3;
+    static constexpr int H = TK / 2;                             // keys that a thread has in registers at a time
+    static constexpr int kColumns = 512;                         // of tensor memory: scores and weights of two tiles, two halves' sums
+    static constexpr int kSmem = kStages * kStage + kQ + (int)sizeof(TcMisc<kStages>);
+    static constexpr bool kJoinHere = false;
+    static_assert(kSmem <= 227 * 1024, "");
+};
+
+// Descriptor of an operand whose rows (or columns) stand side by side in 128-byte lines, a line a k: eights of lines 1024 bytes apart, the next 64 rows
+// `plane` bytes on.
+__device__ inline uint64_t smem_desc_across(uint32_t addr, uint32_t plane) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(plane >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16, BF16 operands, FP32 sums, 128 x 128: bit 16 for a B that lies across.
+__device__ constexpr uint32_t tc_instr(bool across) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24) | (across ? 1u << 16 : 0u);
+}
+__device__ inline void tc_mma_if(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                 "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+                 : "memory");
+}
+// The same with A in tensor memory.
+__device__ inline void tc_mma_ts_if(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+                 "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+                 : "memory");
+}
+__device__ inline uint32_t tc_ld1(uint32_t at) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(at) : "memory");
+    return r;
+}
+// 32 columns of this thread's lane of tensor memory.
+__device__ inline void tc_ld32(uint32_t at, float *v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// A run of keys with a bad page, of pages of eight tokens or at a sequence's ends: each row looks its page up, rows out of range become zeros, the keys of a bad
+// page NaN.
+template <class S>
+__device__ __noinline__ void load_ragged_tc(const Args &a, const int32_t *table, uint32_t to0, int run0, int lo, int len, int head, int b, int lane) {
+    const int page_mask = (1 << a.c.page_shift) - 1, chunk = lane & 15;
+#pragma unroll 1
+    for (int r = lane >> 4; r < S::RUN; r += 2) {
+        const int j = run0 + r;
+        const bool wanted = j >= lo && j < len;
+        int64_t from = -1;
+        if (wanted) {
+            const int id = table[j >> a.c.page_shift];
+            if ((unsigned)id < (unsigned)a.c.n_pages) from = kv_row(a.c, id, head, j & page_mask);
+            else raise_error(a.err, (uint32_t)b, (uint32_t)id);
+        }
+        const int64_t off = from < 0 ? 0 : from * S::RB + chunk * 16;
+        const uint32_t to = to0 + (chunk >> 3) * S::kPlane + swz(r, chunk & 7);
+        if (wanted && from < 0) store_nan<16>(to);
+        else copy_async<16>(to, a.c.k + off, from < 0 ? 0 : 16);
+        copy_async<16>(to + S::kTile, a.c.v + off, from < 0 ? 0 : 16);
+    }
+}
+
+// Barriers of the warps that have the sums.
+template <class S> __device__ inline void sums_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * S::kSums) : "memory"); }
+template <class S> __device__ inline bool sums_any(bool mine) {
+    int any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((int)mine), "n"(32 * S::kSums) : "memory");
+    return any != 0;
+}
+template <class S>
+__global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_constant__ Args a) {
+    constexpr int D = S::D, R = S::R, H = S::H, TK = S::TK, RUN = S::RUN, kStages = S::kStages, kSumThreads = 32 * S::kSums;
+    extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
+    uint8_t *const q_tile = tc_smem_raw + kStages * S::kStage;
+    auto &ms = *reinterpret_cast<TcMisc<kStages> *>(q_tile + S::kQ);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+
+    behind_grid();
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) mbar_init(&ms.full[s], S::kLoads), mbar_init(&ms.empty[s], 1);
+        for (int b = 0; b < 2; ++b) mbar_init(&ms.scores_done[b], 1), mbar_init(&ms.weights[b], S::kSums);
+        mbar_init(&ms.sums_done, 1), mbar_init(&ms.queries, S::kSums), ms.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    Share share;
+    if (!find_share<S>(a, ms.scan, share)) return;
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ms.tmem)), "r"(S::kColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // where the loads begin, and the first segment
+    Cursor start;
+    start.b = share.b, start.s = sequence<S>(a, start.b), start.segment = 0;
+    {
+        const int64_t per_head = (int64_t)start.s.tiles * start.s.row_tiles;
+        start.head = (int)(share.in / per_head), start.row_tile = (int)((share.in - start.head * per_head) / start.s.tiles);
+    }
+    auto segment_of = [&](const Cursor &c, int at) { return Segment{c.s.q0, c.s.n, c.s.len, c.s.p0, c.s.lo, c.s.tile0, c.s.tiles, c.head, c.row_tile * R, at, (int)c.s.bad}; };
+    if (tid == 32) ms.segments[0] = segment_of(start, (int)(share.in % start.s.tiles));
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ms.tmem, smem0 = smem_of(tc_smem_raw);
+    const int units = (int)(share.u1 - share.u0);
+    bool ok = true;
+
+    if (warp >= S::kSums + 1) {
+        // ---- loads: a warp fetches every third run of sixteen keys of a tile, two rows a pass ----
+        Cursor &cur = ms.cur[warp - S::kSums - 1];
+        if (lane == 0) cur = start;
+        __syncwarp();
+        const int page_mask = (1 << a.c.page_shift) - 1, l_chunk = lane & 15, l_row = lane >> 4, run = warp - S::kSums - 1;
+        const uint32_t run_at = smem0 + run * (RUN * 128), to0 = run_at + (l_chunk >> 3) * S::kPlane + swz(l_row, l_chunk & 7);
+        constexpr int kRuns = (TK / RUN + S::kLoads - 1) / S::kLoads, kNext = S::kLoads * RUN;  // a warp's, keys from one to the next
+        int at = (int)(share.in % cur.s.tiles);
+        bool begins = false, told = false;
+        auto landed = [&](int i) {  // this warp's share of tile i is here
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ms.full[i % kStages]);
+        };
+#pragma unroll 1
+        for (int i = 0; i < units; ++i) {
+            const int stage = i % kStages;
+            const int32_t *const table = a.pages + cur.b * a.pages_ld;
+            const uint32_t codes = cur.head * a.head_chunks + l_row * a.row_chunks + l_chunk;
+            const int lo = cur.s.lo, len = cur.s.len, run0 = (cur.s.tile0 + at) * TK + run * RUN;
+            int page[kRuns];
+#pragma unroll
+            for (int x = 0; x < kRuns; ++x) {
+                const int first = run0 + x * kNext;
+                page[x] = first < len && first + RUN > lo ? table[first >> a.c.page_shift] : 0;
+            }
+            if (i >= kStages) {
+                const uint32_t parity = (i / kStages - 1) & 1;
+                if (!__all_sync(0xffffffffu, mbar_test(&ms.empty[stage], parity))) {
+                    // the last tile is told of behind the next one's copies, unless those have to wait
+                    wait_async<0>();
+                    landed(i - 1);
+                    told = true;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&ms.empty[stage], parity, &ms.abort, a.wait_limit_ns));
+                    if (!ok) break;
+                }
+            }
+            if (begins && run == 0 && lane == 0) ms.segments[cur.segment % (kStages + 1)] = segment_of(cur, 0);
+#pragma unroll
+            for (int x = 0; x < kRuns; ++x) {
+                if (run + x * S::kLoads >= TK / RUN) break;
+                const uint32_t by = stage * S::kStage + x * (kNext * 128);
+                const int first = run0 + x * kNext;
+                // (a run that nobody sees, too: its weights are zeros, and so have its values to be)
+                if (SXB_RARE(first < lo || first + RUN > len || page_mask < 15 || (unsigned)page[x] >= (unsigned)a.c.n_pages)) {
+                    load_ragged_tc<S>(a, table, run_at + by, first, lo, len, cur.head, cur.b, lane);
+                    continue;
+                }
+                const uint32_t chunk = (uint32_t)page[x] * a.page_chunks + (uint32_t)(first & page_mask) * a.row_chunks + codes;
+                const uint8_t *k = a.c.k + (uint64_t)chunk * 16, *v = a.c.v + (uint64_t)chunk * 16;
+                const uint64_t step = (uint64_t)a.row_chunks * 32;
+                each<RUN / 2>([&](auto p) {
+                    constexpr int kTurn = 2 * decltype(p)::value & 7, kOff = decltype(p)::value * 256;
+                    const uint32_t to = (to0 + by) ^ (kTurn << 4);
+                    copy_async<16, kOff>(to, k), copy_async<16, kOff + S::kTile>(to, v);
+                    k += step, v += step;
+                });
+            }
+            commit_async();
+            if (i > 0 && !told) {
+                wait_async<1>();
+                landed(i - 1);
+            }
+            told = false;
+            begins = ++at == cur.s.tiles;
+            if (begins && i + 1 < units) at = 0, next_segment<S>(a, cur, lane);
+        }
+        wait_async<0>();
+        if (ok) landed(units - 1);
+        else ms.abort = 1;
+    } else if (warp == S::kSums) {
+        // ---- products ----
+        const uint32_t leader = elect_one() ? 1u : 0u;
+        const uint64_t q_desc = smem_desc(smem_of(q_tile)), k_desc = smem_desc(smem0), v_desc = smem_desc_across(smem0 + S::kTile, S::kPlane);
+        int left = 0, segment = 0;  // tiles of the segment behind tile i
+        auto wait = [&](uint64_t *bar, int n) {  // for its phase n
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, n & 1, &ms.abort, a.wait_limit_ns));
+            if (!ok) ms.abort = 1;
+            tc_fence_after();
+        };
+        auto scores = [&](int i) {
+            const int stage = i % kStages;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                tc_mma_if(leader, tmem + (i & 1) * TK, q_desc + ((k / 4) * S::kPlane + (k % 4) * 32) / 16, k_desc + (stage * S::kStage + (k / 4) * S::kPlane + (k % 4) * 32) / 16,
+                          tc_instr(false), k != 0);
+            tc_commit_if(leader, &ms.scores_done[i & 1]);
+        };
+        bool asked = false, more = false;  // the tile's scores are on their way; there are sums
+#pragma unroll 1
+        for (int i = 0; i < units && ok; ++i) {
+            if (left == 0) {
+                wait(&ms.full[i % kStages], i / kStages);
+                wait(&ms.queries, segment);
+                if (!ok) break;
+                const Segment &sg = ms.segments[segment++ % (kStages + 1)];
+                left = min(sg.tiles - sg.at, units - i), more = false;
+                scores(i);
+            } else if (!asked) {
+                wait(&ms.full[i % kStages], i / kStages);
+                if (!ok) break;
+                scores(i);
+            }
+            --left;
+            asked = left > 0 && __all_sync(0xffffffffu, mbar_test(&ms.full[(i + 1) % kStages], ((i + 1) / kStages) & 1));
+            if (asked) {
+                tc_fence_after();
+                scores(i + 1);
+            }
+            wait(&ms.weights[i & 1], i >> 1);
+            if (!ok) break;
+            const int stage = i % kStages;
+            const int how = ms.how[i & 1];
+            if (how == kMma) {
+#pragma unroll
+                for (int k = 0; k < TK / 16; ++k)
+                    tc_mma_ts_if(leader, tmem + 2 * TK + (k / 4) * D, tmem + (i & 1) * TK + (k / 4) * H + (k % 4) * 8, v_desc + (stage * S::kStage + k * 2048) / 16, tc_instr(true), more || k % 4 != 0);
+            }
+            more = more || how != kNone;
+            tc_commit_if(leader, &ms.empty[stage]);
+            tc_commit_if(leader, &ms.sums_done);
+        }
+    } else {
+        // ---- scores and sums ----
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes_at = tmem + ((uint32_t)(warp & 3) << 21), sums_at = lanes_at + 2 * TK + half * D;
+        auto wait = [&](uint64_t *bar, int n) {  // for its phase n
+            ok = ok && mbar_wait(bar, n & 1, &ms.abort, a.wait_limit_ns);
+            if (!ok) ms.abort = 1;
+            __syncwarp();
+            tc_fence_after();
+        };
+        // what this warp had of tensor and shared memory is read, or written
+        auto tell = [&](uint64_t *bar) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        const float fac = a.softcap > 0.f ? 1.f : a.scale * kLog2e;
+        int segment = 0;
+
+#pragma unroll 1
+        for (int first = 0, n; first < units; first += n, ++segment) {
+            const Segment &sg = ms.segments[segment % (kStages + 1)];
+            if (first > 0) {  // (the record comes with its first tile, the first one's has been there)
+                wait(&ms.full[first % kStages], first / kStages);
+                if (sums_any<S>(!ok)) break;
+            }
+            n = min(sg.tiles - sg.at, units - first);
+            const int rows = min(R, sg.n * a.group - sg.rows0), tok = (sg.rows0 + row) / a.group, head = sg.head * a.group + sg.rows0 + row - tok * a.group;
+            {   // the segment's queries: a thread half a row
+                uint4 w[8] = {};
+                if (row < rows) {
+                    const auto *const from = reinterpret_cast<const uint4 *>(a.q + (sg.q0 + tok) * a.q_ld + (int64_t)head * D + half * 64);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) w[c] = from[c];
+                }
+#pragma unroll
+                for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4 *>(q_tile + half * S::kPlane + swz(row, c)) = w[c];
+            }
+            fence_proxy_async();
+            tell(&ms.queries);
+            // what the row sees, and the tiles that all of them see all of
+            const int hi = row < rows ? sg.p0 + tok : -1, lo = a.window > 0 ? (int)max((int64_t)-1, (int64_t)hi - a.window) : -1;
+            const int hi0 = sg.p0 + sg.rows0 / a.group, hi1 = sg.p0 + min(sg.n - 1, (sg.rows0 + R - 1) / a.group), from = a.window > 0 ? max(0, hi1 - a.window + 1) : 0;
+            const int whole0 = (from + TK - 1) / TK, whole1 = (hi0 + 1 + TK) / TK - 1, lo0 = a.window > 0 ? (int)max((int64_t)-1, (int64_t)hi0 - a.window) : -1;
+            const bool idle = (warp & 3) * 32 >= rows;  // no row of the warp is one: what stands in its lanes nobody reads
+            float top = kLowest, l = 0.f;
+            bool more = false;
+
+#pragma unroll 1
+            for (int i = first; i < first + n; ++i) {
+                const int tile = sg.tile0 + sg.at + i - first, j0 = tile * TK + half * H;
+                const bool whole = tile >= whole0 && tile < whole1;
+                const uint32_t scores_at = lanes_at + (i & 1) * TK + half * H;
+                int how = kMma;
+                wait(&ms.scores_done[i & 1], i >> 1);
+                if (SXB_RARE(!whole) && (tile * TK > hi1 || tile * TK + TK - 1 <= lo0)) {
+                    how = kNone;
+                } else if (!idle) {
+                    uint4 w[H / 8];
+                    float sum;
+#pragma unroll 1
+                    for (int pass = 0; pass < 2; ++pass) {
+                        float most = -CUDART_INF_F;
+                        uint64_t sums = pair(0.f, 0.f);
+                        float s[H];
+#pragma unroll
+                        for (int c = 0; c < H; c += 32) tc_ld32(scores_at + c, s + c);
+                        if (SXB_RARE(a.softcap > 0.f)) {
+                            const float by = 2.f / a.softcap * (a.scale * kLog2e), to = a.softcap * kLog2e;
+#pragma unroll
+                            for (int c = 0; c < H; ++c) s[c] = fmaf(-2.f * to, reciprocal_fast(exp2_flushed(s[c] * by) + 1.f), to);
+                        }
+                        if (SXB_RARE(!whole)) {
+                            const int above = hi - j0, below = lo - j0;
+#pragma unroll
+                            for (int c = 0; c < H; ++c)
+                                if (c > above || c <= below) s[c] = -CUDART_INF_F;
+                        }
+                        const uint64_t fac2 = pair(fac, fac), top2 = pair(-top, -top);
+#pragma unroll
+                        for (int c = 0; c < H; c += 2) {
+                            most = fmaxf(most, fmaxf(s[c], s[c + 1]));
+                            float x0, x1;
+                            unpair(fma_pair(pair(s[c], s[c + 1]), fac2, top2), x0, x1);
+                            const float p0 = exp2_flushed(x0), p1 = exp2_flushed(x1);
+                            sums = add_pair(pair(p0, p1), sums);
+                            reinterpret_cast<uint32_t *>(w)[c / 2] = pack_bf16(p0, p1);
+                        }
+                        float odd;
+                        unpair(sums, sum, odd);
+                        sum += odd;
+                        most *= fac;
+                        if (pass == 1 || !SXB_RARE(__any_sync(0xffffffffu, most - top > (float)kSlack))) break;
+                        // the row's maximum from here on, and what there is of its sums
+                        const float now = fmaxf(top, most), f = exp2_flushed(top - now);
+                        top = now, l *= f;
+                        if (more) {
+                            wait(&ms.sums_done, i - 1);
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                float o[16];
+                                uint4 d[4];
+                                tc_ld16(sums_at + c, o);
+#pragma unroll
+                                for (int x = 0; x < 4; ++x)
+                                    d[x] = make_uint4(__float_as_uint(o[4 * x] * f), __float_as_uint(o[4 * x + 1] * f), __float_as_uint(o[4 * x + 2] * f), __float_as_uint(o[4 * x + 3] * f));
+                                tc_st16(sums_at + c, d);
+                            }
+                        }
+                    }
+                    l += sum;
+#pragma unroll
+                    for (int c = 0; c < H / 32; ++c) {
+                        const uint4 d[4] = {w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]};
+                        tc_st16(scores_at + 16 * c, d);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+                // Keys that one row sees and another does not: an infinity or a NaN there must not reach the other through 0 * v.
+                if (SXB_RARE(!whole && how == kMma && sg.n > 1)) {
+                    bool odd = false;
+                    wait(&ms.full[i % kStages], i / kStages);
+                    const uint8_t *const vt = tc_smem_raw + (i % kStages) * S::kStage + S::kTile;
+#pragma unroll 4
+                    for (int c = tid; c < S::kTile / 16; c += kSumThreads) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(vt + c * 16);
+                        const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) odd = odd || (vs[e] & 0x7f80u) == 0x7f80u || (vs[e] & 0x7f800000u) == 0x7f800000u;
+                    }
+                    __syncwarp();
+                    if (SXB_RARE(sums_any<S>(odd))) {
+                        how = kMade;
+                        if (!idle) {
+                            if (more) wait(&ms.sums_done, i - 1);
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                float o[16];
+                                if (more) {
+                                    tc_ld16(sums_at + c, o);
+                                } else {
+#pragma unroll
+                                    for (int x = 0; x < 16; ++x) o[x] = 0.f;
+                                }
+#pragma unroll 1
+                                for (int k = 0; k < H; ++k) {
+                                    const uint32_t p2 = tc_ld1(scores_at + k / 2);
+                                    const float p = __uint_as_float(k & 1 ? p2 & 0xffff0000u : p2 << 16);
+                                    if (j0 + k <= hi && j0 + k > lo) {
+#pragma unroll
+                                        for (int x = 0; x < 16; ++x)
+                                            o[x] = fmaf(p, bf16_bits_to_f32(*reinterpret_cast<const uint16_t *>(vt + (c >> 6) * S::kPlane + swz(half * H + k, ((c & 63) + x) >> 3) + (x & 7) * 2)), o[x]);
+                                    }
+                                    __syncwarp();
+                                }
+                                uint4 d[4];
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) d[x] = make_uint4(__float_as_uint(o[4 * x]), __float_as_uint(o[4 * x + 1]), __float_as_uint(o[4 * x + 2]), __float_as_uint(o[4 * x + 3]));
+                                tc_st16(sums_at + c, d);
+                            }
+                            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        }
+                    }
+                }
+                if (tid == 0) ms.how[i & 1] = how;
+                tell(&ms.weights[i & 1]);
+                more = more || how != kNone;
+            }
+
+            // ---- the segment's end, or this CTA's share's: the halves' sums, each by what its maximum is below the higher one ----
+            const int64_t seg0 = share.u0 + first - sg.at, seg1 = seg0 + sg.tiles;
+            const bool split = seg0 < share.u0 || seg1 > share.u1;
+            ms.top[half][row] = top, ms.sum[half][row] = l;
+            wait(&ms.sums_done, first + n - 1);
+            if (sums_any<S>(!ok)) break;
+            tc_fence_after();
+            const float top0 = ms.top[0][row], top1 = ms.top[1][row], both = fmaxf(top0, top1);
+            float f0 = exp2_flushed(top0 - both), f1 = exp2_flushed(top1 - both);
+            const float all = fmaf(ms.sum[0][row], f0, ms.sum[1][row] * f1), inv = split ? 1.f : sg.bad ? qnan_f32() : all == 0.f ? 0.f : 1.f / all;
+            f0 *= inv, f1 *= inv;
+            float *const part = a.partial + (2 * (int64_t)blockIdx.x + (seg0 < share.u0 ? 0 : 1)) * R * (D + 2);
+            if (half == 0 && row < rows) {
+                if (split) part[R * D + row] = both, part[R * (D + 1) + row] = all;
+                else if (a.lse != nullptr) a.lse[(int64_t)(sg.q0 + tok) * a.n_q + head] = sg.bad ? qnan_f32() : all == 0.f ? -CUDART_INF_F : fmaf(both, kLn2, logf(all));
+            }
+            if (split && tid == 0 && seg0 >= share.u0) {
+                auto cta_of = [&](int64_t u) { return ((u + 1) * share.ctas + share.total - 1) / share.total - 1; };
+                a.joins[blockIdx.x] = Join{sg.q0, sg.rows0, sg.head, rows, (int)(cta_of(seg1 - 1) - cta_of(seg0)) + 1, {}};
+            }
+            if (!idle) {
+#pragma unroll 1
+                for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 16) {
+                    float o0[16], o1[16];
+                    tc_ld16x2(lanes_at + 2 * TK + c, lanes_at + 2 * TK + D + c, o0, o1);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) o0[x] = more ? fmaf(o0[x], f0, o1[x] * f1) : 0.f * inv;
+                    if (row < rows) {
+                        if (split) {
+                            auto *const to = reinterpret_cast<float4 *>(part + row * D + c);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) to[x] = make_float4(o0[4 * x], o0[4 * x + 1], o0[4 * x + 2], o0[4 * x + 3]);
+                        } else {
+                            auto *const to = reinterpret_cast<uint4 *>(a.out + (sg.q0 + tok) * a.out_ld + (int64_t)head * D + c);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                to[x] = make_uint4(pack_bf16(o0[8 * x], o0[8 * x + 1]), pack_bf16(o0[8 * x + 2], o0[8 * x + 3]), pack_bf16(o0[8 * x + 4], o0[8 * x + 5]),
+                                                   pack_bf16(o0[8 * x + 6], o0[8 * x + 7]));
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            sums_sync<S>();
+        }
+        if (!ok && atomicExch(&ms.abort, 2) != 2 && atomicCAS(&a.status[0], 0u, 2u) == 0u) a.status[1] = (uint32_t)blockIdx.x, a.status[2] = 4;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
+    }
+}

@@ -626,3 +626,163 @@ def test_attend_queries_that_are_none_stay_in_their_rows(cuda):
             ok = np.ones((2, 8), bool)
             ok[0, 1] = False
             assert (np.abs(got[ok] - want[ok]) <= tol[ok]).all()
+
+
+# ---- tiles of 128 rows: a BF16 cache of heads of 128 and more than 128 rows a key head, or more than 32 and a table with room for many keys ----
+
+def with_room(b, keys=400_000):
+    """The batch's tables with columns for so many keys: what a table has room for picks the form."""
+    more = torch.full((len(b.lens), keys // b.cache.page), 0x7ffffff, dtype=torch.int32, device=b.pages.device)
+    b.pages = torch.cat((b.pages, more), 1)
+    return b
+
+
+@pytest.mark.parametrize("group,new", [(3, 11), (8, 8), (5, 13), (8, 16), (43, 3), (3, 50), (5, 77)], ids=["rows33", "rows64", "rows65", "rows128", "rows129", "rows150", "rows385"])
+def test_attend_many_rows_against_the_definition(cuda, group, new):
+    """Lengths around the tiles' ends, rows that see none, uneven counts of new tokens, in tiles of 128 rows and tokens that two of them share."""
+    lens = [1, new, 63, 127, 128, 129, 256, 0, 700, max(1, new - 2), 257]
+    news = [1, new, new, 1, max(1, new - 1), new, 1, 1, new, new, 2]
+    b = with_room(Batch(cuda, 128, 16, 0, 2, group, lens, news, seed=group + new))
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("page", [8, 16, 64, 1024])
+@pytest.mark.parametrize("window", [0, 1, 100, 1000])
+def test_attend_many_rows_pages_window_and_cap(cuda, page, window):
+    b = with_room(Batch(cuda, 128, 16, 0, 2, 7, [1300, 64, 3, 389], [21, 2, 7, 30], page=page, seed=page + window))
+    b.run(window=window, softcap=20.0, scale=0.3)
+    b.check(window=window, softcap=20.0, scale=0.3)
+
+
+def test_attend_many_rows_long_cache_is_split_and_joined(cuda):
+    b = Batch(cuda, 128, 16, 0, 1, 8, [20011, 17], [17, 3], page=64, seed=5)
+    b.run()
+    b.check()
+    first = b.out.clone(), b.lse.clone()
+    for _ in range(3):
+        b.out.fill_(7.0), b.lse.fill_(7.0)
+        b.run()
+        assert torch.equal(b.out, first[0]) and torch.equal(b.lse, first[1])
+
+
+def test_attend_many_rows_scores_that_rise(cuda):
+    """Keys whose scores rise tile by tile by more than the weights' slack, and fall again: sums are scaled on the way, and by hand what the last tile needs."""
+    b = Batch(cuda, 128, 16, 0, 1, 10, [1500], [14], seed=6)
+    for p in range(b.pages.shape[1] - 1):
+        b.cache.k[int(b.pages[0, p])] *= (1 + p / 8) if p < 60 else 0.1
+    b.run()
+    b.check()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_attend_many_rows_what_is_not_finite_reaches_only_rows_that_see_it(cuda, bad):
+    """As above: the newest key or value is none, 50 heads a key head; the sequences' first tile is their last, or not."""
+    for where in ("k", "v"):
+        b = Batch(cuda, 128, 16, 0, 1, 50, [70, 300], [3, 3], seed=11)
+        for s, n in enumerate(b.lens):
+            getattr(b.cache, where)[int(b.pages[s, (n - 1) // 16]), :, (n - 1) % 16, 5] = bad
+            for at in range(n % 16, 16):
+                getattr(b.cache, where)[int(b.pages[s, (n - 1) // 16]), :, at] = float("nan")
+        b.run()
+        torch.cuda.synchronize()
+        want, lse, tol, _ = plain.attend(b.q, b.cache, b.pages, b.q_start, b.kv_len, 128 ** -0.5)
+        got = plain.f64(b.out).reshape(want.shape)
+        rows = [0, 1, 3, 4]
+        assert np.isfinite(got[rows]).all() and (np.abs(got[rows] - want[rows]) <= tol[rows]).all()
+        if where == "v":
+            assert np.array_equal(np.isfinite(got[[2, 5]]), np.isfinite(want[[2, 5]])) and not np.isfinite(got[[2, 5], :, 5]).any()
+        elif bad != bad:
+            assert np.isnan(got[[2, 5]]).all()
+
+
+def test_attend_many_rows_one_query_that_is_none(cuda):
+    for bad in (float("nan"), float("inf")):
+        b = Batch(cuda, 128, 16, 0, 1, 70, [300], [2], seed=17)
+        b.q[0, 128 + 7] = bad
+        b.run()
+        torch.cuda.synchronize()
+        got = plain.f64(b.out).reshape(2, 70, 128)
+        assert np.isnan(got[0, 1]).all()
+        b.q[0, 128 + 7] = 0.0
+        want, _, tol, _ = plain.attend(b.q, b.cache, b.pages, b.q_start, b.kv_len, 128 ** -0.5)
+        ok = np.ones((2, 70), bool)
+        ok[0, 1] = False
+        assert (np.abs(got[ok] - want[ok]) <= tol[ok]).all()
+
+
+def test_attend_many_rows_bad_pages_lengths_and_rows(cuda):
+    b = Batch(cuda, 128, 16, 0, 1, 66, [100, 90, 80, 60, 50], [1, 2, 1, 1, 1], seed=14)
+    clean = b.pages.clone(), b.kv_len.clone(), b.q_start.clone()
+    want, lse, tol, _ = plain.attend(b.q, b.cache, b.pages, b.q_start, b.kv_len, 128 ** -0.5)
+    b.pages[0, 2] = b.cache.n_pages
+    b.pages[1, 5] = -3
+    b.kv_len[2] = b.pages.shape[1] * 16 + 1
+    b.kv_len[3] = -1
+    b.run()
+    torch.cuda.synchronize()
+    got = plain.f64(b.out).reshape(want.shape)
+    assert np.isnan(got[:5]).all() and torch.isnan(b.lse[:5]).all()
+    assert (np.abs(got[5] - want[5]) <= tol[5]).all() and int(b.err[0]) == 1
+    b.err.zero_()
+    b.pages, b.kv_len, b.q_start = clean[0], clean[1], clean[2].clone()
+    b.q_start[2] = b.T + 5
+    b.out.fill_(3.0)
+    b.run()
+    torch.cuda.synchronize()
+    got = plain.f64(b.out).reshape(want.shape)
+    assert (got[1:4] == 3.0).all() and int(b.err[0]) == 1
+    for t in (0, 4, 5):
+        assert (np.abs(got[t] - want[t]) <= tol[t]).all()
+    assert (b.guard == 0xA5).all()
+
+
+def test_attend_many_rows_strides_rows_and_captures(cuda):
+    """A token-major pool, a strided output, rows of no sequence, another stream, a graph replayed with other lengths and counts."""
+    b = Batch(cuda, 128, 16, 0, 2, 13, [500, 277, 40], [12, 11, 1], seed=9)
+    b.run()
+    b.check()
+    c = b.cache
+    both = torch.empty((c.n_pages, 2, c.page, 2, 128), dtype=torch.bfloat16, device=cuda)
+    both[:, 0].copy_(c.k.transpose(1, 2)), both[:, 1].copy_(c.v.transpose(1, 2))
+    other = K().KvCache(both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2), 16)
+    out = torch.full((b.T + 2, b.n_q * 128 + 8), 3.0, dtype=torch.bfloat16, device=cuda)
+    q = torch.cat((b.q[:1], b.q, b.q[:1]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    K().attn_decode(q, other, b.pages, b.q_start + 1, b.kv_len, b.max_q, out[:, :b.n_q * 128], b.ws, b.err, stream=side)
+    side.synchronize()
+    assert torch.equal(out[1:-1, :b.n_q * 128], b.out)
+    assert (out[0] == 3.0).all() and (out[-1] == 3.0).all() and (out[:, b.n_q * 128:] == 3.0).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.run()
+    for lens, starts in (([500, 277, 40], [0, 12, 23, 24]), ([12, 0, 33], [0, 1, 12, 24]), ([380, 129, 1], [0, 22, 24, 24])):
+        b.kv_len.copy_(torch.tensor(lens, dtype=torch.int32)), b.q_start.copy_(torch.tensor(starts, dtype=torch.int32))
+        b.out.fill_(float("nan")), b.lse.fill_(float("nan"))
+        graph.replay()
+        b.check()
+    K().check_dense_status("attention")
+
+
+def test_attend_many_rows_keeps_to_its_workspace_and_shares_it(cuda):
+    """All CTAs at work on split segments of full tiles in a workspace of the size asked for, which calls of fewer rows use in between."""
+    big = Batch(cuda, 128, 16, 0, 8, 64, [6000], [2], page=64, seed=3)
+    for turn, (group, new) in enumerate(((8, 1), (8, 4), (64, 2), (8, 2), (40, 5))):
+        b = Batch(cuda, 128, 16, 0, 8, group, [6000 if group > 8 else 900], [new], page=64, seed=30 + turn)
+        b.ws, b.guard = big.ws, big.guard
+        b.run()
+        if group == 8:
+            b.check()
+        torch.cuda.synchronize()
+        assert (big.guard == 0xA5).all() and torch.isfinite(b.out).all() and int(b.err[0]) == 0
+
+
+def test_attend_one_row_out_of_many_is_the_same_by_either_form(cuda):
+    """More rows than told of, in tiles of 128, whose join is laid out for those told of; and max_q beyond what there is."""
+    b = with_room(Batch(cuda, 128, 16, 0, 1, 8, [9000, 300], [40, 1], max_q=5, seed=4))
+    b.run()
+    b.check()
+    b = Batch(cuda, 128, 16, 0, 1, 8, [9000, 300], [1, 1], max_q=500, seed=4)
+    b.run()
+    b.check()
