@@ -96,6 +96,7 @@ struct Args {
     struct Join *joins;
     uint32_t *status;                  // of the tcgen05 form: a wait that ran out
     unsigned long long wait_limit_ns;
+    int box_rows;
     // distances in pieces of sixteen bytes (codes) and of a row's scales: a cache has fewer than 2^32 of either
     uint32_t page_chunks, head_chunks, row_chunks, page_pieces, head_pieces, row_pieces;
 };
@@ -1176,10 +1177,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
 // of these 54 to 58.)
 constexpr int most_rows(int D, int bits) { return bits == 16 && D <= 128 ? 32 : 16; }
 inline int tile_rows(int D, int bits, int64_t rows) { return rows <= 8 ? 8 : rows <= 16 || most_rows(D, bits) == 16 ? 16 : 32; }
-// Tiles of 128 rows on tcgen05 (attn_decode_tc.cuh): more than 32 rows, and enough tiles a table has room for that its start - tensor memory, three stages to
-// fill before the first product - is no matter.  Rows, sequences x keys, us with tiles of 32 and with it: 64, 64 x 8000, 190 and 147; 2 x 33000, 52 and 47;
-// 16 x 1000, 25 and 27; 1 x 300, 11 and 16; 128, 64 x 8000, 463 and 185; 16 x 1000, 35 and 36; chunks of 512 tokens of eight heads on 4096 keys,
-// 170 and 62, of 2048 on 8192, 1341 and 293.
+// Tiles of 128 rows on tcgen05 (attn_decode_tc.cuh): more than 32 rows, and enough tiles that a table has room for, so that its start - tensor memory, a stage
+// to fill before the first product - is no matter.  Rows, sequences x keys, us with tiles of 32 and with it: 64, 64 x up to 8000, 191 and 136; 2 x up to 33000, 52
+// and 44; 8 x up to 9000, 35 and 35; 16 x 1000, 25 and 27; 1 x 300, 11 and 14; 128, 64 x up to 8000, 460 and 176; 16 x 1000, 35 and 36.  Chunks of 512 tokens of eight
+// heads a key head on 4096 keys, 170 and 60, of 2048 on 8192, 1338 and 287.
 constexpr bool has_tc(int D, int bits) { return D == TcShape::D && bits == TcShape::BITS; }
 inline bool takes_tc(int D, int bits, int64_t rows, int64_t B, int64_t n_kv, int64_t capacity) {
     if (!has_tc(D, bits) || rows <= most_rows(D, bits)) return false;
@@ -1197,7 +1198,7 @@ template <class S> struct Launch {
 
     static int64_t ctas() { return (int64_t)sm_count() * S::kPerSm; }
     static size_t bytes() { return counter_bytes() + (size_t)(ctas() * 2 * S::R * (S::D + 2) * 4); }
-    static cudaError_t run(Args a, void *ws, int64_t most_units, int told_rows, cudaStream_t st) {
+    static cudaError_t run(Args a, void *ws, int64_t most_units, int told_rows, const CUtensorMap *maps, cudaStream_t st) {
         const int64_t n = std::max<int64_t>(1, std::min(ctas(), most_units));
         a.count = static_cast<uint32_t *>(ws);
         a.joins = reinterpret_cast<Join *>(a.count + (size_t)sm_count() * kMostPerSm);
@@ -1212,7 +1213,9 @@ template <class S> struct Launch {
             if (const cudaError_t rc = cudaFuncSetAttribute(attn_join_kernel<S>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared); rc != cudaSuccess) return rc;
             told.fetch_or(bit, std::memory_order_release);
         }
-        const cudaError_t rc2 = launch_behind(Kernel<S>::fn, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a);
+        cudaError_t rc2;
+        if constexpr (std::is_same_v<S, TcShape>) rc2 = launch_behind(Kernel<S>::fn, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a, maps[0], maps[1]);
+        else rc2 = launch_behind(Kernel<S>::fn, dim3((unsigned)n), dim3(S::kThreads), (size_t)S::kSmem, st, 1, a);
         if (S::kJoinHere || rc2 != cudaSuccess) return rc2;
         return launch_behind(attn_join_kernel<S>, dim3((unsigned)n, (unsigned)((told_rows + kJoinRows - 1) / kJoinRows)), dim3(kJoinRows * S::D / 4), 0, st, 1, a);
     }
@@ -1306,7 +1309,14 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
     const uint32_t chunks = (uint32_t)(D * cache->bits / 8 / 16), words = cache->bits == 16 ? 0 : (uint32_t)(D / cache->G), pieces = words > 4 ? words / 4 : words ? 1 : 0;
     a.page_chunks = (uint32_t)cache->page_stride * chunks, a.head_chunks = (uint32_t)cache->head_stride * chunks, a.row_chunks = (uint32_t)cache->row_stride * chunks;
     a.page_pieces = (uint32_t)cache->page_stride * pieces, a.head_pieces = (uint32_t)cache->head_stride * pieces, a.row_pieces = (uint32_t)cache->row_stride * pieces;
+    CUtensorMap maps[2];  // [page, head, token, column], boxes of 16 to 64 tokens of a page and 64 columns
     if (tc) {
+        const uint64_t dims[4] = {(uint64_t)D, (uint64_t)cache->page, (uint64_t)n_kv, (uint64_t)cache->n_pages}, row = (uint64_t)D * 2;
+        const uint64_t strides[3] = {(uint64_t)cache->row_stride * row, (uint64_t)cache->head_stride * row, (uint64_t)cache->page_stride * row};
+        a.box_rows = (int)std::min<int64_t>(64, std::max<int64_t>(16, cache->page));
+        const uint32_t box[4] = {64, (uint32_t)std::min<int64_t>(a.box_rows, cache->page), 1, 1};
+        for (int x = 0; x < 2; ++x)
+            if (int rc = tensor_map_4d(fn, x == 0 ? cache->k : cache->v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, &maps[x])) return rc;
         if (int rc = library_status_words(fn, &a.status)) return rc;
         a.wait_limit_ns = wait_limit_ns();
     }
@@ -1316,7 +1326,7 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
         if (Launch<S>::bytes() > args->ws_bytes) return cudaErrorInvalidValue;  // nothing is written behind the workspace, whatever the sizes above say
         // no list is longer than every sequence at its table's end (in a product that cannot overflow: the grid is a few hundred CTAs)
         const double most = (double)((a.capacity + S::TK - 1) / S::TK) * (double)B * n_kv * (double)((T * a.group + S::R - 1) / S::R + 1);
-        return Launch<S>::run(a, ws, (int64_t)std::min(most, 1e12), (int)std::min<int64_t>(S::R, told), st);
+        return Launch<S>::run(a, ws, (int64_t)std::min(most, 1e12), (int)std::min<int64_t>(S::R, told), maps, st);
     });
     if (rc != cudaSuccess) return fail_cuda(SXB_FILE_, __LINE__, __func__, rc, cat(fn, " launch"));
     SXB_CHECK_LAUNCH(fn, " T=", T, " B=", B, " n_q=", n_q, " n_kv=", n_kv, " D=", D, " bits=", cache->bits);

@@ -5,12 +5,17 @@
 // K and V lie in shared memory as they lie in the cache, a line a key; the second product reads V across its lines and P from tensor memory, where P takes
 // S's place.  Eight warps make weights: a thread has a row and half of a tile's keys, with a maximum, a sum and sums of values of that half's own, which
 // are joined at a segment's end, so that no thread waits for another one's scores.  The maximum that a row goes by is raised, and its sums scaled, only by a
-// tile that passes it by more than 2^kSlack.  One warp issues the products, the next tile's scores ahead of this one's weights; three fetch.
+// tile that passes it by more than 2^kSlack.  One warp issues the products, the next tile's scores ahead of this one's weights; three fetch, a stage each.
+//
+// Measured (B200): 2048 tokens of eight heads a key head on 8192 keys, four key heads, 287 us, 840 TFLOP/s of what the mask leaves; a tile of 128 x 128 takes about
+// 2000 cycles, of which the products are 1230 and the exponentials 1024.  64 rows over 64 sequences of 100 to 8000 keys 136 us (bytes alone 81): there a tile
+// is half empty, and a sequence's start and end, 5000 cycles, count.  Two warps' scores of one row with one maximum (a barrier of the two a tile) took 497 us
+// in the first case, the copies by cp.async (three warps, a third of each tile's rows) 294, boxes of sixteen rows whatever the pages 343.
 
 template <int STAGES> struct TcMisc {
     float top[2][128], sum[2][128];
     int64_t scan[12 + 2];
-    uint64_t full[STAGES], empty[STAGES], scores_done[2], weights[2], sums_done, queries;
+    uint64_t full[STAGES], values[STAGES], empty[STAGES], scores_done[2], weights[2], sums_done, queries;
     Segment segments[STAGES + 1];       // of what is on its way, and of the tile whose sums go out
     Cursor cur[3];
     uint32_t tmem;
@@ -19,11 +24,11 @@ template <int STAGES> struct TcMisc {
 constexpr int kMma = 0, kMade = 1, kNone = 2;  // the MMA takes them, the threads have, no row sees the tile
 struct TcShape {
     static constexpr int D = 128, BITS = 16, R = 128;
-    static constexpr int kSums = 8, kLoads = 3;                  // warps that have the scores and sums, warps that fetch
+    static constexpr int kSums = 8, kLoads = 3, kStages = kLoads;                  // warps that have the scores and sums, warps that fetch
     static constexpr int kWarps = kSums + kLoads + 1, kThreads = 32 * kWarps, RUN = 16, TK = 128, kPerSm = 1;
     static constexpr int RB = 2 * D, CR = RB / 16;
     static constexpr int kPlane = TK * 128, kTile = 2 * kPlane, kStage = 2 * kTile;  // 64 columns of a tile's keys (lines of 128 bytes); keys or values; both
-    static constexpr int kQ = R * D * 2, kStages = 3;
+    static constexpr int kQ = R * D * 2;
     static constexpr int H = TK / 2;                             // keys that a thread has in registers at a time
     static constexpr int kColumns = 512;                         // of tensor memory: scores and weights of two tiles, two halves' sums
     static constexpr int kSmem = kStages * kStage + kQ + (int)sizeof(TcMisc<kStages>);
@@ -70,26 +75,34 @@ __device__ inline void tc_ld32(uint32_t at, float *v) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-// A run of keys with a bad page, of pages of eight tokens or at a sequence's ends: each row looks its page up, rows out of range become zeros, the keys of a bad
-// page NaN.
+__device__ inline void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// A run of keys of pages of eight tokens or with a bad page: each row looks its page up, rows out of range become zeros, the keys of a bad page NaN.
 template <class S>
-__device__ __noinline__ void load_ragged_tc(const Args &a, const int32_t *table, uint32_t to0, int run0, int lo, int len, int head, int b, int lane) {
-    const int page_mask = (1 << a.c.page_shift) - 1, chunk = lane & 15;
-#pragma unroll 1
-    for (int r = lane >> 4; r < S::RUN; r += 2) {
-        const int j = run0 + r;
-        const bool wanted = j >= lo && j < len;
-        int64_t from = -1;
-        if (wanted) {
-            const int id = table[j >> a.c.page_shift];
-            if ((unsigned)id < (unsigned)a.c.n_pages) from = kv_row(a.c, id, head, j & page_mask);
-            else raise_error(a.err, (uint32_t)b, (uint32_t)id);
+__device__ __noinline__ void load_rows(const Args &a, const int32_t *table, uint32_t to0, int run0, int lo, int len, int head, int b, int lane) {
+    const int page_mask = (1 << a.c.page_shift) - 1, chunk = lane & 15, j0 = run0 + (lane & 15);
+    // lane r has the page of row r
+    int mine = -1;
+    const bool there = j0 >= lo && j0 < len;
+    if (there) {
+        mine = table[j0 >> a.c.page_shift];
+        if ((unsigned)mine >= (unsigned)a.c.n_pages) {
+            raise_error(a.err, (uint32_t)b, (uint32_t)mine);
+            mine = -2;
         }
-        const int64_t off = from < 0 ? 0 : from * S::RB + chunk * 16;
+    }
+#pragma unroll 1
+    for (int r0 = 0; r0 < S::RUN; r0 += 2) {
+        const int r = r0 + (lane >> 4), id = __shfl_sync(0xffffffffu, mine, r);
+        const int64_t off = id < 0 ? 0 : kv_row(a.c, id, head, (run0 + r) & page_mask) * S::RB + chunk * 16;
         const uint32_t to = to0 + (chunk >> 3) * S::kPlane + swz(r, chunk & 7);
-        if (wanted && from < 0) store_nan<16>(to);
-        else copy_async<16>(to, a.c.k + off, from < 0 ? 0 : 16);
-        copy_async<16>(to + S::kTile, a.c.v + off, from < 0 ? 0 : 16);
+        if (id == -2) store_nan<16>(to);
+        else copy_async<16>(to, a.c.k + off, id < 0 ? 0 : 16);
+        copy_async<16>(to + S::kTile, a.c.v + off, id < 0 ? 0 : 16);
     }
 }
 
@@ -101,7 +114,7 @@ template <class S> __device__ inline bool sums_any(bool mine) {
     return any != 0;
 }
 template <class S>
-__global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     constexpr int D = S::D, R = S::R, H = S::H, TK = S::TK, RUN = S::RUN, kStages = S::kStages, kSumThreads = 32 * S::kSums;
     extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
     uint8_t *const q_tile = tc_smem_raw + kStages * S::kStage;
@@ -110,7 +123,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
 
     behind_grid();
     if (tid == 0) {
-        for (int s = 0; s < kStages; ++s) mbar_init(&ms.full[s], S::kLoads), mbar_init(&ms.empty[s], 1);
+        for (int s = 0; s < kStages; ++s) mbar_init(&ms.full[s], 2), mbar_init(&ms.values[s], 2), mbar_init(&ms.empty[s], 1);
         for (int b = 0; b < 2; ++b) mbar_init(&ms.scores_done[b], 1), mbar_init(&ms.weights[b], S::kSums);
         mbar_init(&ms.sums_done, 1), mbar_init(&ms.queries, S::kSums), ms.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -138,76 +151,58 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
     bool ok = true;
 
     if (warp >= S::kSums + 1) {
-        // ---- loads: a warp fetches every third run of sixteen keys of a tile, two rows a pass ----
-        Cursor &cur = ms.cur[warp - S::kSums - 1];
+        // ---- loads: a warp has a stage, and so every third tile ----
+        const int stage = warp - S::kSums - 1;
+        Cursor &cur = ms.cur[stage];
         if (lane == 0) cur = start;
         __syncwarp();
-        const int page_mask = (1 << a.c.page_shift) - 1, l_chunk = lane & 15, l_row = lane >> 4, run = warp - S::kSums - 1;
-        const uint32_t run_at = smem0 + run * (RUN * 128), to0 = run_at + (l_chunk >> 3) * S::kPlane + swz(l_row, l_chunk & 7);
-        constexpr int kRuns = (TK / RUN + S::kLoads - 1) / S::kLoads, kNext = S::kLoads * RUN;  // a warp's, keys from one to the next
-        int at = (int)(share.in % cur.s.tiles);
-        bool begins = false, told = false;
-        auto landed = [&](int i) {  // this warp's share of tile i is here
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ms.full[i % kStages]);
-        };
+        const int page_mask = (1 << a.c.page_shift) - 1;
+        const uint32_t tile_to = smem0 + stage * S::kStage;
+        const int boxes = TK / a.box_rows;
+        int at = (int)(share.in % cur.s.tiles), skip = stage, last = -1;
 #pragma unroll 1
-        for (int i = 0; i < units; ++i) {
-            const int stage = i % kStages;
+        for (int i = stage; i < units; i += kStages, skip = kStages) {
+            for (at += skip; at >= cur.s.tiles;) at -= cur.s.tiles, next_segment<S>(a, cur, lane);
             const int32_t *const table = a.pages + cur.b * a.pages_ld;
-            const uint32_t codes = cur.head * a.head_chunks + l_row * a.row_chunks + l_chunk;
-            const int lo = cur.s.lo, len = cur.s.len, run0 = (cur.s.tile0 + at) * TK + run * RUN;
-            int page[kRuns];
+            const int lo = cur.s.lo, len = cur.s.len, head = cur.head, run0 = (cur.s.tile0 + at) * TK;
+            // Lane x has box x, sixteen to 64 keys of a page.  It comes whole where a row may see a key of it, what lies behind the sequence's end in the page too; one
+            // that nobody sees does not come: the scores of both are put out of sight and their values' places filled with zeros before the product.
+            const int first = run0 + lane * a.box_rows, to = tile_to + lane * (a.box_rows * 128);
+            const bool seen = lane < boxes && first < len && first + a.box_rows > lo;
+            int page = -1;
+            if (seen && page_mask >= 15) page = table[first >> a.c.page_shift];
+            const bool fine = (unsigned)page < (unsigned)a.c.n_pages;
+            const uint32_t ragged = __ballot_sync(0xffffffffu, seen && !fine), bytes = __popc(__ballot_sync(0xffffffffu, fine)) * (a.box_rows * S::RB);
+            if (i >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&ms.empty[stage], (i / kStages - 1) & 1, &ms.abort, a.wait_limit_ns));
+            if (!ok) break;
+            last = i;
+            if (at == 0 && i > 0 && lane == 0) ms.segments[cur.segment % (kStages + 1)] = segment_of(cur, 0);
+            if (lane == 0) mbar_expect_tx(&ms.full[stage], bytes), mbar_expect_tx(&ms.values[stage], bytes);
+            __syncwarp();
+            if (fine) {
+                const int row = first & page_mask;
 #pragma unroll
-            for (int x = 0; x < kRuns; ++x) {
-                const int first = run0 + x * kNext;
-                page[x] = first < len && first + RUN > lo ? table[first >> a.c.page_shift] : 0;
-            }
-            if (i >= kStages) {
-                const uint32_t parity = (i / kStages - 1) & 1;
-                if (!__all_sync(0xffffffffu, mbar_test(&ms.empty[stage], parity))) {
-                    // the last tile is told of behind the next one's copies, unless those have to wait
-                    wait_async<0>();
-                    landed(i - 1);
-                    told = true;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&ms.empty[stage], parity, &ms.abort, a.wait_limit_ns));
-                    if (!ok) break;
-                }
-            }
-            if (begins && run == 0 && lane == 0) ms.segments[cur.segment % (kStages + 1)] = segment_of(cur, 0);
+                for (int x = 0; x < 2; ++x) tma_load_4d(to + x * S::kPlane, &k_map, 64 * x, row, head, page, &ms.full[stage]);
 #pragma unroll
-            for (int x = 0; x < kRuns; ++x) {
-                if (run + x * S::kLoads >= TK / RUN) break;
-                const uint32_t by = stage * S::kStage + x * (kNext * 128);
-                const int first = run0 + x * kNext;
-                // (a run that nobody sees, too: its weights are zeros, and so have its values to be)
-                if (SXB_RARE(first < lo || first + RUN > len || page_mask < 15 || (unsigned)page[x] >= (unsigned)a.c.n_pages)) {
-                    load_ragged_tc<S>(a, table, run_at + by, first, lo, len, cur.head, cur.b, lane);
-                    continue;
-                }
-                const uint32_t chunk = (uint32_t)page[x] * a.page_chunks + (uint32_t)(first & page_mask) * a.row_chunks + codes;
-                const uint8_t *k = a.c.k + (uint64_t)chunk * 16, *v = a.c.v + (uint64_t)chunk * 16;
-                const uint64_t step = (uint64_t)a.row_chunks * 32;
-                each<RUN / 2>([&](auto p) {
-                    constexpr int kTurn = 2 * decltype(p)::value & 7, kOff = decltype(p)::value * 256;
-                    const uint32_t to = (to0 + by) ^ (kTurn << 4);
-                    copy_async<16, kOff>(to, k), copy_async<16, kOff + S::kTile>(to, v);
-                    k += step, v += step;
-                });
+                for (int x = 0; x < 2; ++x) tma_load_4d(to + S::kTile + x * S::kPlane, &v_map, 64 * x, row, head, page, &ms.values[stage]);
             }
-            commit_async();
-            if (i > 0 && !told) {
-                wait_async<1>();
-                landed(i - 1);
+            __syncwarp();
+            if (SXB_RARE(ragged != 0)) {
+#pragma unroll 1
+                for (int x = 0; x < TK / RUN; ++x)
+                    if ((ragged >> (x * RUN / a.box_rows) & 1) != 0) load_rows<S>(a, table, tile_to + x * (RUN * 128), run0 + x * RUN, lo, len, head, cur.b, lane);
+                commit_async();
+                wait_async<0>();
+                fence_proxy_async();
+                __syncwarp();
             }
-            told = false;
-            begins = ++at == cur.s.tiles;
-            if (begins && i + 1 < units) at = 0, next_segment<S>(a, cur, lane);
+            if (lane == 0) mbar_arrive(&ms.full[stage]), mbar_arrive(&ms.values[stage]);
         }
-        wait_async<0>();
-        if (ok) landed(units - 1);
-        else ms.abort = 1;
+        if (!ok) {
+            // the copies that are still on their way, before the shared memory is another CTA's
+            ms.abort = 1;
+            if (last >= 0) mbar_wait(&ms.full[stage], (last / kStages) & 1, nullptr, 1000000ull), mbar_wait(&ms.values[stage], (last / kStages) & 1, nullptr, 1000000ull);
+        }
     } else if (warp == S::kSums) {
         // ---- products ----
         const uint32_t leader = elect_one() ? 1u : 0u;
@@ -248,9 +243,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
                 scores(i + 1);
             }
             wait(&ms.weights[i & 1], i >> 1);
+            wait(&ms.values[i % kStages], i / kStages);
             if (!ok) break;
-            const int stage = i % kStages;
-            const int how = ms.how[i & 1];
+            const int stage = i % kStages, how = ms.how[i & 1];
             if (how == kMma) {
 #pragma unroll
                 for (int k = 0; k < TK / 16; ++k)
@@ -378,18 +373,26 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
-                // Keys that one row sees and another does not: an infinity or a NaN there must not reach the other through 0 * v.
-                if (SXB_RARE(!whole && how == kMma && sg.n > 1)) {
+                // Values of keys that no row sees become zeros, whatever they are: 0 * v has to be 0.  Of keys that one row sees and another does not, an infinity or a
+                // NaN must not reach the other: the threads add such a tile's up, each for its row.
+                if (SXB_RARE(!whole && how == kMma)) {
                     bool odd = false;
-                    wait(&ms.full[i % kStages], i / kStages);
-                    const uint8_t *const vt = tc_smem_raw + (i % kStages) * S::kStage + S::kTile;
-#pragma unroll 4
+                    wait(&ms.values[i % kStages], i / kStages);
+                    uint8_t *const vt = tc_smem_raw + (i % kStages) * S::kStage + S::kTile;
+#pragma unroll 1
                     for (int c = tid; c < S::kTile / 16; c += kSumThreads) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(vt + c * 16);
-                        const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
+                        auto *const at = reinterpret_cast<uint4 *>(vt + c * 16);
+                        const int j = tile * TK + (c >> 3) % TK;
+                        if (j > hi1 || j <= lo0) {
+                            *at = make_uint4(0, 0, 0, 0);
+                        } else if (sg.n > 1) {
+                            const uint4 v = *at;
+                            const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) odd = odd || (vs[e] & 0x7f80u) == 0x7f80u || (vs[e] & 0x7f800000u) == 0x7f800000u;
+                            for (int e = 0; e < 4; ++e) odd = odd || (vs[e] & 0x7f80u) == 0x7f80u || (vs[e] & 0x7f800000u) == 0x7f800000u;
+                        }
                     }
+                    fence_proxy_async();
                     __syncwarp();
                     if (SXB_RARE(sums_any<S>(odd))) {
                         how = kMade;

@@ -813,7 +813,7 @@ static int encode_map(const char *fn, CUtensorMap *map, CUtensorMapDataType dtyp
         return reinterpret_cast<TensorMapEncode>(p);
     }();
     SXB_CHECK(encode != nullptr, fn, ": the driver offers no cuTensorMapEncodeTiled");
-    const cuuint32_t elem[3] = {1u, 1u, 1u};
+    const cuuint32_t elem[4] = {1u, 1u, 1u, 1u};
     const CUresult rc = encode(map, dtype, (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     SXB_CHECK(rc == CUDA_SUCCESS || rank == 2, fn, ": tensor map over ", dims[2], " x ", dims[1], " rows of ", strides[0], " bytes refused (CUresult ", (int)rc, ")");
@@ -834,6 +834,13 @@ int tensor_map_3d_bytes(const char *fn, const void *base, uint64_t inner, uint64
     const cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)mid, (cuuint64_t)outer}, strides[2] = {(cuuint64_t)mid_stride, (cuuint64_t)outer_stride};
     const cuuint32_t box[3] = {box_inner, box_mid, box_outer};
     return encode_map(fn, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, 3, dims, strides, box, swizzle);
+}
+
+int tensor_map_4d(const char *fn, const void *base, CUtensorMapDataType dtype, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4],
+                  CUtensorMapSwizzle swizzle, CUtensorMap *map) {
+    const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, s[3] = {strides[0], strides[1], strides[2]};
+    const cuuint32_t b[4] = {box[0], box[1], box[2], box[3]};
+    return encode_map(fn, map, dtype, base, 4, d, s, b, swizzle);
 }
 
 template <int BITS>

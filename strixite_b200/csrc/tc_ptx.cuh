@@ -18,6 +18,9 @@ int tensor_map_2d(const char *fn, const void *base, CUtensorMapDataType dtype, i
 // ... a 3-D one over bytes: [outer][mid][inner], `mid_stride` and `outer_stride` bytes apart.
 int tensor_map_3d_bytes(const char *fn, const void *base, uint64_t inner, uint64_t mid, uint64_t outer, uint64_t mid_stride, uint64_t outer_stride,
                         uint32_t box_inner, uint32_t box_mid, uint32_t box_outer, CUtensorMapSwizzle swizzle, CUtensorMap *map);
+// ... a 4-D one, innermost dimension first, strides (of all but that one) in bytes.
+int tensor_map_4d(const char *fn, const void *base, CUtensorMapDataType dtype, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4],
+                  CUtensorMapSwizzle swizzle, CUtensorMap *map);
 int library_status_words(const char *fn, uint32_t **out);
 unsigned long long wait_limit_ns();
 // ... of the streaming expert kernel's, which wait for a whole unit of another warp as a matter of course: never below the default, whatever a

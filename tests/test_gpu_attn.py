@@ -786,3 +786,16 @@ def test_attend_one_row_out_of_many_is_the_same_by_either_form(cuda):
     b = Batch(cuda, 128, 16, 0, 1, 8, [9000, 300], [1, 1], max_q=500, seed=4)
     b.run()
     b.check()
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_attend_many_rows_nothing_unseen_counts(cuda, new):
+    """NaN in every row that no query sees: behind the sequences' ends and before their windows, in the same pages as what is seen."""
+    lens, window = [70, 129, 400], 40
+    b = Batch(cuda, 128, 16, 0, 1, 160, lens, [new] * 3, seed=19)
+    for s, n in enumerate(lens):
+        for j in list(range(0, n - new + 1 - window)) + list(range(n, -(-n // 16) * 16)):
+            for t in (b.cache.k, b.cache.v):
+                t[int(b.pages[s, j // 16]), :, j % 16] = float("nan")
+    b.run(window=window)
+    b.check(window=window)
