@@ -532,7 +532,7 @@ typedef struct SxbKvCache {
  * position pos[t] of sequence seq[t]: rounded once to BF16, or quantized from the FP32 values as sxb_quantize does (a group that
  * holds a NaN or an infinity reads back as NaN).  seq[t] < 0: a padding row, nothing of it is written.  A position or page out of
  * range: err = {1, token, pos}, the token's queries NaN, nothing written to the cache.  No (seq, pos) twice in one call.
- * Rows of qkv and q_out and the norm weights 16-byte aligned. */
+ * Rows of qkv and q_out and the norm weights 16-byte aligned; 1 to 2^20 tokens a call (sxb_kv_read too). */
 typedef struct SxbAttnQkvWriteArgs {
     const void *qkv;
     int64_t ld, T, n_q;
