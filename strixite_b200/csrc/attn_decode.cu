@@ -245,6 +245,54 @@ template <class S, int KI, int N> __device__ inline void value_words(uint32_t (&
 // Whether a group's scale or min is an infinity or a NaN.
 __device__ inline bool none_of(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
+// Sixteen keys' values of codes added up by the threads in FP32, each row's for itself: weights p of the score accumulators' layout, hidden: those that do not
+// count, o in the layout of the second product (less the codes' offsets).  What a group's scale or min is reaches its own columns and the rows that see the key.
+template <class S, int KI>
+__device__ inline void add_values(const uint8_t *values, const uint32_t (&words)[2][S::NG], const float (&p)[S::NT][4], uint32_t hidden, float v_up, int lane,
+                                  float (&o)[S::D / 16][S::NT][4], float (&o_min)[S::NG][S::NT][2]) {
+    constexpr int NT = S::NT, NG = S::NG, G = S::G;
+    const int g = lane >> 2, t4 = lane & 3;
+    const auto *const scales = reinterpret_cast<const uint32_t *>(values + S::kRows + S::kScales) + KI * 16 * NG;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if ((hidden >> (nt * 4 + e) & 1) == 0) {
+#pragma unroll
+                for (int grp = 0; grp < NG; ++grp) o_min[grp][nt][e & 1] = fmaf(p[nt][e], __uint_as_float(words[e >> 1][grp] & 0xffff0000u), o_min[grp][nt][e & 1]);
+            }
+#pragma unroll 1
+    for (int k = 0; k < 16; ++k) {
+        const int from = (k % 8) * 4 + t4;
+        const uint32_t out_of_sight = __shfl_sync(0xffffffffu, hidden, from) >> (k < 8 ? 0 : 2);
+        float w[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float low = __shfl_sync(0xffffffffu, p[nt][e], from), high = __shfl_sync(0xffffffffu, p[nt][2 + e], from);
+                w[nt][e] = k < 8 ? low : high;
+            }
+#pragma unroll
+        for (int c = 0; c < S::CR; ++c) {  // a chunk of sixteen bytes: this lane has two of them, two columns or four
+            constexpr int kCols = 128 / S::BITS;
+            const uint32_t code = *reinterpret_cast<const uint16_t *>(values + chunk_at<S::CR>(KI * 16 + k, c) * 16 + 2 * g);
+            const float scale = __uint_as_float(scales[k * NG + c * kCols / G] << 16) * v_up;
+#pragma unroll
+            for (int x = 0; x < 16 / S::BITS; ++x) {
+                const float v = scale * (float)(code >> (x * S::BITS) & ((1u << S::BITS) - 1));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float &to = o[c * kCols / 16 + x / 2][nt][2 * (x & 1) + e];
+                        if ((out_of_sight >> (nt * 4 + e) & 1) == 0) to = fmaf(w[nt][e], v, to);
+                    }
+            }
+        }
+    }
+}
+
 // BF16 NaN throughout.
 template <int BYTES> __device__ inline void store_nan(uint32_t to) {
     for (int i = 0; i < BYTES; i += 4) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + i), "r"(0x7fc07fc0u) : "memory");
@@ -933,34 +981,22 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 constexpr int ki = decltype(kic)::value, kRun = ki * 16 * S::RB;
                 uint32_t words[2][kGroups];
                 value_words<S, ki>(words, s_at);
+                // A power of two keeps the products of scales and weights inside F16; the largest scale so far sets it.  As bit patterns an infinity, a NaN and a negative
+                // scale are above every other.
+                uint32_t most = 0;
                 bool odd = false;  // a scale or a min among them is none, and there are rows that must not hear of it
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int grp = 0; grp < NG; ++grp) most = max(most, words[e][grp] << 16);
                 if (SXB_RARE(!whole)) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
                         for (int grp = 0; grp < NG; ++grp) odd = odd || none_of(words[e][grp]);
                 }
-                if (SXB_RARE(odd)) {  // what is none stays with the rows that see it: their columns of the group end as NaN
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int grp = 0; grp < NG; ++grp)
-                            if (none_of(words[e][grp])) {
-                                words[e][grp] = 0;
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                    for (int x = 0; x < 2; ++x)
-                                        if ((hidden >> ((ki * NT + nt) * 4 + 2 * e + x) & 1) == 0) o_min[grp][nt][x] = CUDART_NAN_F;
-                            }
-                }
-                // scales times the power of two that keeps their products with weights inside F16; the largest so far sets it
-                float scales[2][kGroups], most = 0.f;
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) scales[e][grp] = __uint_as_float(words[e][grp] << 16) * v_up, most = fmaxf(most, fabsf(scales[e][grp]));
-                if (SXB_RARE(__any_sync(0xffffffffu, most >= (float)(1 << (15 - kSlack))))) {
+                if (SXB_RARE(__any_sync(0xffffffffu, odd || most >= (uint32_t)(v_exp + 1) << 23))) {
+                    odd = odd || most >= 0x7f800000u;
                     int ex = 0;
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
@@ -973,10 +1009,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     const float down = exp2_flushed((float)(v_exp - ex));
                     v_exp = ex, v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int grp = 0; grp < NG; ++grp) scales[e][grp] = __uint_as_float(words[e][grp] << 16) * v_up;
-#pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                         for (int d = 0; d < D / 16; ++d)
@@ -984,7 +1016,17 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                             for (int e = 0; e < 4; ++e) o[d][nt][e] *= down;
                         w_sum[nt][0] *= down, w_sum[nt][1] *= down;
                     }
+                    // The matrix product would carry what is none to other columns (0 * NaN in the sums of weights) and other rows.
+                    if (__any_sync(0xffffffffu, odd)) {
+                        add_values<S, ki>(smem + stage * S::kStage + warp * S::kPart + S::kRows, words, s[ki], hidden >> (ki * NT * 4), v_up, lane, o, o_min);
+                        return;
+                    }
                 }
+                float scales[2][kGroups];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int grp = 0; grp < NG; ++grp) scales[e][grp] = __uint_as_float(words[e][grp] << 16) * v_up;
                 each<NG>([&](auto grpc) {
                     constexpr int grp = decltype(grpc)::value;
                     float mn[2];
