@@ -38,6 +38,10 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kMostPerSm = 4;
 constexpr int kSlack = 8;      // powers of two that a weight may be above 1
+// Powers of two that a value group's scale may be below the largest one so far.  The largest scale times a weight of 1 is 2^6 as an F16 number, one below by kSpread
+// 2^-2: weights down to 2^-12 then keep F16's eleven bits, and what the smaller ones lose, 2^-25 a key at most, is 2^-23 of that group's own scale.
+// Sixteen keys with a scale further down are added up in FP32 by the threads (twice to three times their time).
+constexpr int kSpread = 8;
 constexpr float kLowest = -1e30f;  // below every score; a row that sees no key keeps it
 constexpr int64_t kMaxRows = 1ll << 24;
 
@@ -982,20 +986,20 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 uint32_t words[2][kGroups];
                 value_words<S, ki>(words, s_at);
                 // A power of two keeps the products of scales and weights inside F16; the largest scale so far sets it.  As bit patterns an infinity, a NaN and a negative
-                // scale are above every other.
-                uint32_t most = 0;
+                // scale are above every other, and so is, less one, a zero.
+                uint32_t most = 0, least = 0xffffffffu;
                 bool odd = false;  // a scale or a min among them is none, and there are rows that must not hear of it
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) most = max(most, words[e][grp] << 16);
+                    for (int grp = 0; grp < NG; ++grp) most = max(most, words[e][grp] << 16), least = min(least, (words[e][grp] << 16) - 1);
                 if (SXB_RARE(!whole)) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
                         for (int grp = 0; grp < NG; ++grp) odd = odd || none_of(words[e][grp]);
                 }
-                if (SXB_RARE(__any_sync(0xffffffffu, odd || most >= (uint32_t)(v_exp + 1) << 23))) {
+                if (SXB_RARE(__any_sync(0xffffffffu, odd || most >= (uint32_t)(v_exp + 1) << 23 || least < (uint32_t)(v_exp - kSpread) << 23))) {
                     odd = odd || most >= 0x7f800000u;
                     int ex = 0;
 #pragma unroll
@@ -1016,7 +1020,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                             for (int e = 0; e < 4; ++e) o[d][nt][e] *= down;
                         w_sum[nt][0] *= down, w_sum[nt][1] *= down;
                     }
-                    // The matrix product would carry what is none to other columns (0 * NaN in the sums of weights) and other rows.
+                    odd = odd || least < (uint32_t)(v_exp - kSpread) << 23;
+                    // The matrix product would carry what is none to other columns (0 * NaN in the sums of weights) and other rows, and lose small values' weights.
                     if (__any_sync(0xffffffffu, odd)) {
                         add_values<S, ki>(smem + stage * S::kStage + warp * S::kPart + S::kRows, words, s[ki], hidden >> (ki * NT * 4), v_up, lane, o, o_min);
                         return;

@@ -49,3 +49,36 @@ def test_a_value_group_that_is_none_is_so_alone(cuda, D, bits, G, word, bad):
             b.cache.v_sm[int(b.pages[s, j // 16]), :, j % 16, 1, word] = bad
         got, want = run_and_compare(b)
         assert np.isfinite(want[:, :, :G]).all() and not np.isfinite(want[3:6, :, G:2 * G]).all()
+
+
+@pytest.mark.parametrize("D,bits,G", QUANT)
+@pytest.mark.parametrize("power", [-6, -9, -12, -20, -40, 9, 20, 40])
+def test_value_groups_of_very_different_sizes(cuda, D, bits, G, power):
+    """A head's last group is 2^power times as large as the others, and every seventh key's first group: each column is as exact as by itself."""
+    for group, new in ((1, 1), (4, 3)):
+        b = Batch(cuda, D, bits, G, 2, group, [900, 41], [new, new], seed=D + bits + power)
+        b.cache.v_sm[..., -1, :] *= 2.0 ** power
+        b.cache.v_sm[:, :, 3::7, 0, :] *= 2.0 ** power
+        run_and_compare(b)
+
+
+def against(cache, page, head, at, q, score, scale):
+    """Makes the key at (page, head, at) one whose score with the query row q is `score`, by the library's quantizer."""
+    x = q.float() * (score / (scale * float((q.float() ** 2).sum())))
+    w = K().quantize(x.view(1, -1).contiguous(), cache.G, cache.bits)
+    cache.k[page, head, at] = w.q.view(-1)
+    cache.k_sm[page, head, at] = torch.stack((w.scale, w.minv), -1).view(torch.bfloat16).view(cache.k_sm.shape[-2:])
+
+
+@pytest.mark.parametrize("D,bits,G", QUANT)
+@pytest.mark.parametrize("power", [14, 24, 40])
+def test_a_large_value_that_a_row_does_not_look_at(cuda, D, bits, G, power):
+    """One key's values are 2^power times the others', and its weight in the first query head is far below 2^-power (in the second it has its way): the first
+    head's output is the other keys'.  The key comes first, in the middle, last."""
+    for at in (0, 200, 511):
+        b = Batch(cuda, D, bits, G, 1, 2, [512], [1], seed=D + bits + power)
+        page, row = int(b.pages[0, at // 16]), at % 16
+        against(b.cache, page, 0, row, b.q[0, :D], -60.0, D ** -0.5)
+        b.cache.v_sm[page, 0, row] *= 2.0 ** power
+        got, want = run_and_compare(b)
+        assert np.abs(want[0, 0]).max() < 10.0
