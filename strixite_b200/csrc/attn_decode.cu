@@ -651,6 +651,22 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     float m[NT][2], l[NT][2];
     int v_exp = 20, at = 0, tiles = 0, whole0 = 0, whole1 = 0, segment = 0, stage = 0;
     bool fresh = true;
+    auto take_out = [&]() {  // what the codes' offsets have added to the sums of their products
+        if constexpr (kQuant) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int grp = 0; grp < NG; ++grp) {
+                    const float sum[2] = {__shfl_sync(0xffffffffu, w_sum[nt][0], grp * 4 + t4), __shfl_sync(0xffffffffu, w_sum[nt][1], grp * 4 + t4)};
+#pragma unroll
+                    for (int d = grp * S::G / 16; d < (grp + 1) * S::G / 16; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[d][nt][e] = fmaf(e < 2 ? -S::kOffset : -S::kOffsetOdd, sum[e & 1], o[d][nt][e]);
+                }
+                w_sum[nt][0] = w_sum[nt][1] = 0.f;
+            }
+        }
+    };
 
 #pragma unroll 1
     for (int i = 0; i < units; ++i) {
@@ -1077,6 +1093,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             });
         }
         }
+        // the accumulators' steps cut their last bit off, of sums that the offset makes 4 (8 bits) to 140 times as large: it goes before that adds up
+        if constexpr (kQuant) {
+            if (SXB_RARE((at & 15) == 15)) take_out();
+        }
         uint8_t *const stage_base = smem + stage * S::kStage;
         stage = stage + 1 == kStages ? 0 : stage + 1;
         if (__builtin_expect(++at < tiles && i + 1 < units, 1)) continue;
@@ -1104,16 +1124,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1) o_min[grp][nt][e] += __shfl_xor_sync(0xffffffffu, o_min[grp][nt][e], off);
+            take_out();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int grp = 0; grp < NG; ++grp) {
-                    const float sum[2] = {__shfl_sync(0xffffffffu, w_sum[nt][0], grp * 4 + t4), __shfl_sync(0xffffffffu, w_sum[nt][1], grp * 4 + t4)};
+                for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-                    for (int d = grp * S::G / 16; d < (grp + 1) * S::G / 16; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[d][nt][e] = fmaf(fmaf(e < 2 ? -S::kOffset : -S::kOffsetOdd, sum[e & 1], o[d][nt][e]), down, o_min[grp][nt][e & 1]);
-                }
+                    for (int e = 0; e < 4; ++e) o[d][nt][e] = fmaf(o[d][nt][e], down, o_min[d * 16 / S::G][nt][e & 1]);
         }
         __syncthreads();
         // what each group's sums of a row count for, the row's maximum and its sum of weights

@@ -82,3 +82,23 @@ def test_a_large_value_that_a_row_does_not_look_at(cuda, D, bits, G, power):
         b.cache.v_sm[page, 0, row] *= 2.0 ** power
         got, want = run_and_compare(b)
         assert np.abs(want[0, 0]).max() < 10.0
+
+
+@pytest.mark.parametrize("still", [False, True], ids=["scores", "alike"])
+@pytest.mark.parametrize("D,bits,G", [(128, 4, 32), (128, 8, 64), (128, 16, 0), (256, 4, 64), (64, 4, 32)])
+def test_many_thousand_keys_a_warp(cuda, D, bits, G, still):
+    """So many long sequences that a warp sums up thousands of keys by itself: what the codes are too large by, and what an accumulator rounds off in every step,
+    must not add up."""
+    B, n_kv, page = 64, 2, 256
+    keys = (3 << 30) // (B * n_kv * 2 * (D * bits // 8 + (0 if bits == 16 else 4 * D // G)))
+    b = Batch(cuda, D, bits, G, n_kv, 1, [keys] * B, [1] * B, page=page, seed=bits)
+    if still:
+        b.q.zero_()
+    b.out.fill_(UNTOUCHED), b.lse.fill_(UNTOUCHED)
+    b.run()
+    torch.cuda.synchronize()
+    for s in (7,):
+        want, lse, tol, lse_tol = plain.attend(b.q[s:s + 1], b.cache, b.pages[s:s + 1], b.q_start[:2], b.kv_len[s:s + 1], D ** -0.5)
+        got = plain.f64(b.out[s]).reshape(want.shape)
+        assert (np.abs(got - want) <= tol).all(), ((np.abs(got - want) / tol).max(), (np.abs(got - want) / (np.abs(want) + 1e-30)).max())
+        assert (np.abs(plain.f64(b.lse[s:s + 1]) - lse) <= lse_tol).all()
