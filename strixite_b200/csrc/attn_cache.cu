@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kWriteThreads) qkv_write_kernel(const __grid_c
                             const uint64_t other = a.interleaved ? pair(v[2 * i + 1], v[2 * i])
                                                                  : pair(__shfl_sync(0xffffffffu, v[2 * i], partner, kLanes), __shfl_sync(0xffffffffu, v[2 * i + 1], partner, kLanes));
                             r[i] = fma_pair(p[i], by[i], mul_pair(other, cross[i]));
+                            if (!turned) r[i] = mul_pair(p[i], by[i]);  // as it is: nothing of a neighbour, not even 0 times an infinity
                         }
                     } else {
 #pragma unroll

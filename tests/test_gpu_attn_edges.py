@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import attn_plain as plain
-from test_gpu_attn import Batch, K
+from test_gpu_attn import Batch, K, Rows
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,25 @@ def test_many_thousand_keys_a_warp(cuda, D, bits, G, still):
         got = plain.f64(b.out[s]).reshape(want.shape)
         assert (np.abs(got - want) <= tol).all(), ((np.abs(got - want) / tol).max(), (np.abs(got - want) / (np.abs(want) + 1e-30)).max())
         assert (np.abs(plain.f64(b.lse[s:s + 1]) - lse) <= lse_tol).all()
+
+
+# ---- the write -----------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("D,rot", [(64, 16), (128, 32), (128, 64), (256, 32)])
+def test_write_leaves_what_it_does_not_turn_alone(cuda, D, rot, f32, interleaved):
+    """Without a norm the elements behind the first rot go through as they are, infinities and NaN too, and none reaches its neighbour."""
+    r = Rows(cuda, 5, 2, 3, 2, D, 16, 0, f32=f32, seed=D + rot, norm=False)
+    x = r.qkv.view(5, 7, D)
+    x[0, :, rot], x[1, :, rot + 3], x[2, :, D - 1], x[3, :, rot + 8] = float("inf"), -float("inf"), float("nan"), float("inf")
+    K().attn_qkv_write(r.qkv, r.cache, r.seq, r.pos, r.pages, r.q_out, r.err, inv_freq=r.inv_freq(rot), interleaved=interleaved)
+    k, v = r.read()
+    torch.cuda.synchronize()
+    assert int(r.err[0]) == 0
+    bits = x.to(torch.bfloat16)
+    q = r.q_out.view(5, 3, D)
+    for got, put in ((q[..., rot:], bits[:, :3, rot:]), (k[..., rot:], bits[:, 3:5, rot:].float()), (v, bits[:, 5:].float())):
+        assert torch.equal(torch.isnan(got), torch.isnan(put))
+        assert torch.equal(got.nan_to_num(nan=0.0, posinf=1e9, neginf=-1e9), put.nan_to_num(nan=0.0, posinf=1e9, neginf=-1e9))
+    assert torch.isfinite(q[..., :rot]).all() and torch.isfinite(k[..., :rot]).all()
