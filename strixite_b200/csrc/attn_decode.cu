@@ -206,6 +206,15 @@ __device__ inline float reciprocal_fast(float v) {  // 1 ulp
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+// A score s * fac (in powers of two) under a cap: to * tanh(x), x = s * fac / to.  Below a quarter the odd series to its fourth term, x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315,
+// as a factor of the score itself (62 x^8 / 2835 is left off: 2^-21.5 at most); above it 1 - 2 / (exp(2 x) + 1), whose cancellation is 2^-19.9 of what it gives at a quarter, and
+// less further on: FP32's own error of a score, whatever the cap.  by = 2 ln 2 / to (as a power of two's exponent, 2 x is s * fac * by).
+__device__ inline float capped(float s, float fac, float by, float to) {
+    const float t = s * (fac * by), x2 = t * t * (0.25f * kLn2 * kLn2);
+    const float near = s * fac * fmaf(x2, fmaf(x2, fmaf(x2, -17.f / 315, 2.f / 15), -1.f / 3), 1.f);
+    const float far = fmaf(-2.f * to, reciprocal_fast(exp2_flushed(t) + 1.f), to);
+    return fabsf(t) < 0.5f * kLog2e ? near : far;
+}
 __device__ inline uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -854,14 +863,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
             }
         }
         if (SXB_RARE(a.softcap > 0.f)) {
-            // tanh x = 1 - 2 / (exp(2 x) + 1): 2^-22 of the cap, as good as a score near it is in FP32
             const float by = 2.f / a.softcap, to = a.softcap * kLog2e;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int ki = 0; ki < KI; ++ki)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = fmaf(-2.f * to, reciprocal_fast(exp2_flushed(s[ki][nt][e] * (fac[nt][e & 1] * by)) + 1.f), to);
+                    for (int e = 0; e < 4; ++e) s[ki][nt][e] = capped(s[ki][nt][e], fac[nt][e & 1], by, to);
                 fac[nt][0] = fac[nt][1] = 1.f;
             }
         }

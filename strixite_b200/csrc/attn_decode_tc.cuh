@@ -323,9 +323,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
 #pragma unroll
                         for (int c = 0; c < H; c += 32) tc_ld32(scores_at + c, s + c);
                         if (SXB_RARE(a.softcap > 0.f)) {
-                            const float by = 2.f / a.softcap * (a.scale * kLog2e), to = a.softcap * kLog2e;
+                            const float by = 2.f / a.softcap, to = a.softcap * kLog2e;
 #pragma unroll
-                            for (int c = 0; c < H; ++c) s[c] = fmaf(-2.f * to, reciprocal_fast(exp2_flushed(s[c] * by) + 1.f), to);
+                            for (int c = 0; c < H; ++c) s[c] = capped(s[c], a.scale * kLog2e, by, to);
                         }
                         if (SXB_RARE(!whole)) {
                             const int above = hi - j0, below = lo - j0;

@@ -104,6 +104,48 @@ def test_many_thousand_keys_a_warp(cuda, D, bits, G, still):
         assert (np.abs(plain.f64(b.lse[s:s + 1]) - lse) <= lse_tol).all()
 
 
+# ---- the cap -------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cap", [1e-6, 1e-3, 0.7, 5.0, 50.0, 1e3, 1e6, 1e9, 9e29])
+@pytest.mark.parametrize("D,bits,G,group,new", [(128, 16, 0, 4, 2), (128, 16, 0, 70, 2), (64, 8, 32, 4, 2), (256, 4, 64, 8, 2)], ids=["bf16", "rows140", "q8", "q4"])
+def test_caps_of_any_size(cuda, D, bits, G, group, new, cap):
+    """The capped score is as good as a score is in FP32, whatever the cap.
+
+    cap * tanh(s / cap) is within 2^-19 of itself: below a quarter of the cap by four terms of the odd series (the fifth is 2^-21.5) with a handful of roundings;
+    above by 1 - 2 r, r = 1 / (exp(2 s / cap) + 1), whose exponential is off by 2^-22, its sum by 2^-24, the reciprocal by 2^-23: at a quarter
+    0.755 * (0.62 + 0.25 + 0.5) * 2^-22 of a tanh of 0.245, 2^-19.9, and less above."""
+    b = Batch(cuda, D, bits, G, 1, group, [300, 40], [new, new], seed=9)
+    scale = 0.3
+    b.out.fill_(UNTOUCHED), b.lse.fill_(UNTOUCHED)
+    b.run(scale=scale, softcap=cap)
+    torch.cuda.synchronize()
+    assert int(b.err[0]) == 0 and (b.guard == 0xA5).all()
+    q, got, got_lse = plain.f64(b.q).reshape(b.T, group, D), plain.f64(b.out).reshape(b.T, group, D), plain.f64(b.lse)
+    kept, t = plain.BF16 if bits == 16 else plain.F16, 0
+    for s, (n, length) in enumerate(zip(b.new, b.lens)):
+        j = np.arange(length)
+        page = b.pages[s].cpu().numpy()[j // 16].astype(np.int64)
+        k, k_scaled, k_least = plain.values(b.cache, "k", page, 0, j % 16)
+        v, v_scaled, v_least = plain.values(b.cache, "v", page, 0, j % 16)
+        for i in range(n):
+            last = length - n + i + 1
+            x = q[t].T
+            raw = (k[:last] @ x) * scale
+            off = (D / 16 + 4) * 2.0 ** -22 * ((k_scaled + k_least)[:last] @ np.abs(x)) * scale
+            sc = cap * np.tanh(raw / cap)
+            off = np.minimum(off, 2 * cap) + 2.0 ** -19 * np.abs(sc)
+            top = sc.max(0)
+            w = np.exp(sc - top)
+            lse = top + np.log(w.sum(0))
+            w = w / w.sum(0)
+            want = w.T @ v[:last]
+            of_weights = (2 * off.max(0) + 2.0 ** -20)[:, None]
+            tol = plain.BF16 * np.abs(want) + (kept + of_weights) * (w.T @ v_scaled[:last]) + (of_weights + 2.0 ** -20) * (w.T @ v_least[:last]) + 1e-30
+            assert (np.abs(got[t] - want) <= tol).all(), (cap, (np.abs(got[t] - want) / tol).max())
+            assert (np.abs(got_lse[t] - lse) <= off.max(0) + 2.0 ** -20 + 2.0 ** -22 * np.abs(lse)).all(), cap
+            t += 1
+
+
 # ---- the write -----------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("interleaved", [False, True])
