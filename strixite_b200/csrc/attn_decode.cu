@@ -41,7 +41,8 @@ constexpr int kSlack = 8;      // powers of two that a weight may be above 1
 // Powers of two that a value group's scale may be below the largest one so far.  The largest scale times a weight of 1 is 2^6 as an F16 number, one below by kSpread
 // 2^-2: weights down to 2^-12 then keep F16's eleven bits, and what the smaller ones lose, 2^-25 a key at most, is 2^-23 of that group's own scale.
 // Sixteen keys with a scale further down are added up in FP32 by the threads (twice to three times their time).
-constexpr int kSpread = 8;
+constexpr uint32_t kSpread = 8;
+constexpr uint32_t kLowestScale = (20 - kSpread) << 23;  // as a bit pattern
 constexpr float kLowest = -1e30f;  // below every score; a row that sees no key keeps it
 constexpr int64_t kMaxRows = 1ll << 24;
 
@@ -255,6 +256,8 @@ template <class S, int KI, int N> __device__ inline void value_words(uint32_t (&
     load_shared<kOff>(w[0], scales), load_shared<kOff + 8 * N * 4>(w[1], scales);
 }
 
+// What the scales are multiplied by whose lowest power of two is v_low: 2^(14 - kSlack) over the largest.
+__device__ inline float scale_up(uint32_t v_low) { return __uint_as_float(((2 * 127u + 14 - kSlack - kSpread) << 23) - v_low); }
 // Whether a group's scale or min is an infinity or a NaN.
 __device__ inline bool none_of(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
@@ -658,7 +661,8 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
     uint32_t qf[S::kHoldQ ? NT : 1][S::kHoldQ ? D / 16 : 1][2];
     float o[D / 16][NT][4], w_sum[NT][4], o_min[kGroups][NT][2];
     float m[NT][2], l[NT][2];
-    int v_exp = 20, at = 0, tiles = 0, whole0 = 0, whole1 = 0, segment = 0, stage = 0;
+    uint32_t v_low = kLowestScale;
+    int at = 0, tiles = 0, whole0 = 0, whole1 = 0, segment = 0, stage = 0;
     bool fresh = true;
     auto take_out = [&]() {  // what the codes' offsets have added to the sums of their products
         if constexpr (kQuant) {
@@ -697,7 +701,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         if (SXB_RARE(fresh)) {
             fresh = false;
             __syncthreads();
-            at = sg.at, tiles = sg.tiles, v_exp = 20;
+            at = sg.at, tiles = sg.tiles, v_low = kLowestScale;
             {   // tiles that every row sees all of
                 const int p_last = sg.p0 + sg.n - 1, from = a.window > 0 ? max(0, p_last - a.window + 1) : 0;
                 whole0 = (from + TK - 1) / TK - sg.tile0, whole1 = (sg.p0 + 1 + TK) / TK - 1 - sg.tile0;
@@ -1004,47 +1008,50 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     }
             }
         } else {
-            float v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);  // 2^(14 - kSlack - (v_exp - 127))
+            float v_up = scale_up(v_low);
             each<KI>([&](auto kic) {
                 constexpr int ki = decltype(kic)::value, kRun = ki * 16 * S::RB;
                 uint32_t words[2][kGroups];
                 value_words<S, ki>(words, s_at);
-                // A power of two keeps the products of scales and weights inside F16; the largest scale so far sets it.  As bit patterns an infinity, a NaN and a negative
-                // scale are above every other, and so is, less one, a zero.
-                uint32_t most = 0, least = 0xffffffffu;
+                // A power of two keeps the products of scales and weights inside F16; the largest scale so far sets it.  As bit patterns, less that of the lowest that goes with it,
+                // what is larger, lower, an infinity, a NaN or negative is above what goes; a zero too, which changes nothing.
+                uint32_t over = 0;
                 bool odd = false;  // a scale or a min among them is none, and there are rows that must not hear of it
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int grp = 0; grp < NG; ++grp) most = max(most, words[e][grp] << 16), least = min(least, (words[e][grp] << 16) - 1);
+                    for (int grp = 0; grp < NG; ++grp) over = max(over, (words[e][grp] << 16) - v_low);
                 if (SXB_RARE(!whole)) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
                         for (int grp = 0; grp < NG; ++grp) odd = odd || none_of(words[e][grp]);
                 }
-                if (SXB_RARE(__any_sync(0xffffffffu, odd || most >= (uint32_t)(v_exp + 1) << 23 || least < (uint32_t)(v_exp - kSpread) << 23))) {
-                    odd = odd || most >= 0x7f800000u;
-                    int ex = 0;
+                if (SXB_RARE(__any_sync(0xffffffffu, odd || over >= (kSpread + 1) << 23))) {
+                    uint32_t most = 0, least = 0xffffffffu;  // of finite scales' sizes; of all but zeros
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
                         for (int grp = 0; grp < NG; ++grp) {
-                            const int x = (int)(words[e][grp] >> 7 & 0xffu);
-                            if (x != 255) ex = max(ex, x);  // a scale that is none says nothing of the others
+                            const uint32_t t = words[e][grp] << 16, size = t & 0x7f800000u;
+                            if (size != 0x7f800000u) most = max(most, size);  // a scale that is none says nothing of the others
+                            odd = odd || t > 0x7f7fffffu;
+                            least = min(least, t - 1);
                         }
-                    ex = max(v_exp, __reduce_max_sync(0xffffffffu, ex));
-                    const float down = exp2_flushed((float)(v_exp - ex));
-                    v_exp = ex, v_up = __uint_as_float((uint32_t)(141 - kSlack - v_exp + 127) << 23);
+                    most = __reduce_max_sync(0xffffffffu, most);
+                    if (most > v_low + (kSpread << 23)) {
+                        const float down = exp2_flushed((float)((int)(v_low + (kSpread << 23) - most) >> 23));
+                        v_low = most - (kSpread << 23), v_up = scale_up(v_low);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
+                        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                        for (int d = 0; d < D / 16; ++d)
+                            for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[d][nt][e] *= down;
-                        w_sum[nt][0] *= down, w_sum[nt][1] *= down;
+                                for (int e = 0; e < 4; ++e) o[d][nt][e] *= down;
+                            w_sum[nt][0] *= down, w_sum[nt][1] *= down;
+                        }
                     }
-                    odd = odd || least < (uint32_t)(v_exp - kSpread) << 23;
+                    odd = odd || least < v_low;
                     // The matrix product would carry what is none to other columns (0 * NaN in the sums of weights) and other rows, and lose small values' weights.
                     if (__any_sync(0xffffffffu, odd)) {
                         add_values<S, ki>(smem + stage * S::kStage + warp * S::kPart + S::kRows, words, s[ki], hidden >> (ki * NT * 4), v_up, lane, o, o_min);
@@ -1103,7 +1110,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
         }
         // the accumulators' steps cut their last bit off, of sums that the offset makes 4 (8 bits) to 140 times as large: it goes before that adds up
         if constexpr (kQuant) {
-            if (SXB_RARE((at & 15) == 15)) take_out();
+            if (SXB_RARE((at & 15) == 15 || at + 1 == tiles || i + 1 == units)) take_out();
         }
         uint8_t *const stage_base = smem + stage * S::kStage;
         stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -1123,7 +1130,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                 if (g == 0) row_max[r] = m[nt][e], row_sum[r] = l[nt][e];
             }
         if constexpr (kQuant) {
-            const float down = __uint_as_float((uint32_t)(v_exp + kSlack - 141 + 127) << 23);
+            const float down = __uint_as_float(2 * (127u << 23) - __float_as_uint(scale_up(v_low)));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1132,7 +1139,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kPerSm) attn_decode_kernel(con
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
                         for (int off = 4; off < 32; off <<= 1) o_min[grp][nt][e] += __shfl_xor_sync(0xffffffffu, o_min[grp][nt][e], off);
-            take_out();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
