@@ -22,6 +22,7 @@
 // 300 keys of one sequence: 7, nothing but latencies - lengths, page table, keys, join.
 
 #include "attn.cuh"
+#include "route_pack.cuh"
 #include "skinny_mma.cuh"
 #include "tc_ptx.cuh"
 
@@ -101,6 +102,7 @@ struct Args {
     struct Join *joins;
     uint32_t *status;                  // of the tcgen05 form: a wait that ran out
     unsigned long long wait_limit_ns;
+    int test_skip_slot;                // >= 0: CTA 0 of that form leaves that fill of keys and values out, so that a wait runs out (tests only)
     int box_rows;
     // distances in pieces of sixteen bytes (codes) and of a row's scales: a cache has fewer than 2^32 of either
     uint32_t page_chunks, head_chunks, row_chunks, page_pieces, head_pieces, row_pieces;
@@ -1396,7 +1398,7 @@ extern "C" int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t strea
         for (int x = 0; x < 2; ++x)
             if (int rc = tensor_map_4d(fn, x == 0 ? cache->k : cache->v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, &maps[x])) return rc;
         if (int rc = library_status_words(fn, &a.status)) return rc;
-        a.wait_limit_ns = wait_limit_ns();
+        a.wait_limit_ns = wait_limit_ns(), a.test_skip_slot = test_skip_slot();
     }
     auto st = static_cast<cudaStream_t>(stream);
     const cudaError_t rc = with_shape(D, cache->bits, cache->G, rows, [&](auto s) {

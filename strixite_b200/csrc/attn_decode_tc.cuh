@@ -15,7 +15,7 @@
 template <int STAGES> struct TcMisc {
     float top[2][128], sum[2][128];
     int64_t scan[12 + 2];
-    uint64_t full[STAGES], values[STAGES], empty[STAGES], scores_done[2], weights[2], sums_done, queries;
+    uint64_t full[STAGES], values[STAGES], empty[STAGES], scores_done[2], weights[2], sums_done, queries, drained;
     Segment segments[STAGES + 1];       // of what is on its way, and of the tile whose sums go out
     Cursor cur[3];
     uint32_t tmem;
@@ -113,6 +113,10 @@ template <class S> __device__ inline bool sums_any(bool mine) {
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"((int)mine), "n"(32 * S::kSums) : "memory");
     return any != 0;
 }
+// A wait ran out, or the news came that another warp's has: the first one is recorded, and every other wait ends.
+__device__ __noinline__ void give_up(const Args &a, int *abort, uint32_t role) {
+    if (atomicExch(abort, 1) == 0 && atomicCAS(&a.status[0], 0u, 2u) == 0u) a.status[1] = blockIdx.x, a.status[2] = role;
+}
 template <class S>
 __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     constexpr int D = S::D, R = S::R, H = S::H, TK = S::TK, RUN = S::RUN, kStages = S::kStages, kSumThreads = 32 * S::kSums;
@@ -125,7 +129,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) mbar_init(&ms.full[s], 2), mbar_init(&ms.values[s], 2), mbar_init(&ms.empty[s], 1);
         for (int b = 0; b < 2; ++b) mbar_init(&ms.scores_done[b], 1), mbar_init(&ms.weights[b], S::kSums);
-        mbar_init(&ms.sums_done, 1), mbar_init(&ms.queries, S::kSums), ms.abort = 0;
+        mbar_init(&ms.sums_done, 1), mbar_init(&ms.queries, S::kSums), mbar_init(&ms.drained, 1), ms.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     Share share;
@@ -149,6 +153,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
     const uint32_t tmem = ms.tmem, smem0 = smem_of(tc_smem_raw);
     const int units = (int)(share.u1 - share.u0);
     bool ok = true;
+    int last = -1;  // the fill that a copy warp has issued
 
     if (warp >= S::kSums + 1) {
         // ---- loads: a warp has a stage, and so every third tile ----
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
         const int page_mask = (1 << a.c.page_shift) - 1;
         const uint32_t tile_to = smem0 + stage * S::kStage;
         const int boxes = TK / a.box_rows;
-        int at = (int)(share.in % cur.s.tiles), skip = stage, last = -1;
+        int at = (int)(share.in % cur.s.tiles), skip = stage;
 #pragma unroll 1
         for (int i = stage; i < units; i += kStages, skip = kStages) {
             for (at += skip; at >= cur.s.tiles;) at -= cur.s.tiles, next_segment<S>(a, cur, lane);
@@ -174,7 +179,11 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
             const bool fine = (unsigned)page < (unsigned)a.c.n_pages;
             const uint32_t ragged = __ballot_sync(0xffffffffu, seen && !fine), bytes = __popc(__ballot_sync(0xffffffffu, fine)) * (a.box_rows * S::RB);
             if (i >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&ms.empty[stage], (i / kStages - 1) & 1, &ms.abort, a.wait_limit_ns));
-            if (!ok) break;
+            if (!ok) {
+                give_up(a, &ms.abort, kRoleAttnCopy);
+                break;
+            }
+            if (blockIdx.x == 0 && i == a.test_skip_slot) continue;  // the test hook's fill never comes
             last = i;
             if (at == 0 && i > 0 && lane == 0) ms.segments[cur.segment % (kStages + 1)] = segment_of(cur, 0);
             if (lane == 0) mbar_expect_tx(&ms.full[stage], bytes), mbar_expect_tx(&ms.values[stage], bytes);
@@ -198,11 +207,6 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
             }
             if (lane == 0) mbar_arrive(&ms.full[stage]), mbar_arrive(&ms.values[stage]);
         }
-        if (!ok) {
-            // the copies that are still on their way, before the shared memory is another CTA's
-            ms.abort = 1;
-            if (last >= 0) mbar_wait(&ms.full[stage], (last / kStages) & 1, nullptr, 1000000ull), mbar_wait(&ms.values[stage], (last / kStages) & 1, nullptr, 1000000ull);
-        }
     } else if (warp == S::kSums) {
         // ---- products ----
         const uint32_t leader = elect_one() ? 1u : 0u;
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
         int left = 0, segment = 0;  // tiles of the segment behind tile i
         auto wait = [&](uint64_t *bar, int n) {  // for its phase n
             ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, n & 1, &ms.abort, a.wait_limit_ns));
-            if (!ok) ms.abort = 1;
+            if (SXB_RARE(!ok)) give_up(a, &ms.abort, kRoleAttnMma);
             tc_fence_after();
         };
         auto scores = [&](int i) {
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
         const uint32_t lanes_at = tmem + ((uint32_t)(warp & 3) << 21), sums_at = lanes_at + 2 * TK + half * D;
         auto wait = [&](uint64_t *bar, int n) {  // for its phase n
             ok = ok && mbar_wait(bar, n & 1, &ms.abort, a.wait_limit_ns);
-            if (!ok) ms.abort = 1;
+            if (SXB_RARE(!ok)) give_up(a, &ms.abort, kRoleAttnSums);
             __syncwarp();
             tc_fence_after();
         };
@@ -430,6 +434,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
                 if (tid == 0) ms.how[i & 1] = how;
                 tell(&ms.weights[i & 1]);
                 more = more || how != kNone;
+                if (SXB_RARE((i & 63) == 63) && sums_any<S>(!ok)) break;  // no tile after tile of a segment that nobody finishes
             }
 
             // ---- the segment's end, or this CTA's share's: the halves' sums, each by what its maximum is below the higher one ----
@@ -478,10 +483,27 @@ __global__ void __launch_bounds__(S::kThreads, 1) attn_tc_kernel(const __grid_co
             tc_fence_before();
             sums_sync<S>();
         }
-        if (!ok && atomicExch(&ms.abort, 2) != 2 && atomicCAS(&a.status[0], 0u, 2u) == 0u) a.status[1] = (uint32_t)blockIdx.x, a.status[2] = 4;
+        // A CTA that has given up has parts that others' are joined with, of an earlier call: their sums of weights become NaN, and so do the rows.
+        if (*static_cast<volatile int *>(&ms.abort) != 0 && half == 0) {
+            float *const sums = a.partial + 2 * (int64_t)blockIdx.x * R * (D + 2) + R * (D + 1) + row;
+            if (segment == 0) sums[0] = qnan_f32();
+            sums[R * (D + 2)] = qnan_f32();
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (SXB_RARE(*static_cast<volatile int *>(&ms.abort) != 0)) {
+        // Nothing may still be on its way when shared and tensor memory go to another CTA: each copy warp waits for its last fill, the MMA warp for its products.
+        if (warp > S::kSums && last >= 0) {
+            const int stage = warp - S::kSums - 1;
+            mbar_wait(&ms.full[stage], (last / kStages) & 1, nullptr, 1000000ull), mbar_wait(&ms.values[stage], (last / kStages) & 1, nullptr, 1000000ull);
+        } else if (warp == S::kSums) {
+            tc_commit_if(elect_one() ? 1u : 0u, &ms.drained);
+            mbar_wait(&ms.drained, 0, nullptr, 1000000ull);
+        }
+        tc_fence_before();
+        __syncthreads();
+    }
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");

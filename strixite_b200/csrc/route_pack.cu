@@ -398,8 +398,8 @@ int route_small(const char *fn, const float *logits, int64_t ld, int64_t M, int6
 using namespace sxb;
 
 namespace sxb {
-// {2, work item, role}: the record of a device-side wait that ran out, of the tcgen05 kernels (grouped_tc.cu) or of the exact grouped forms
-// (kRoleStaged and kRoleLeft, the item being a tile of eight tokens).
+// {2, work item, role}: the record of a device-side wait that ran out, of the tcgen05 kernels (grouped_tc.cu), of the exact grouped forms
+// (kRoleStaged and kRoleLeft, the item being a tile of eight tokens) or of the attention of many rows (kRoleAttn..., the item being the CTA).
 int tc_status_error(const char *what, const uint32_t e[3]) {
     static const char *roles[] = {"an unknown role",
                                   "a weight producer waiting for a free operand stage",
@@ -414,9 +414,13 @@ int tc_status_error(const char *what, const uint32_t e[3]) {
                                   "a warp waiting for the tile's staged activations",
                                   "a staging warp waiting for the last warp to leave its buffer"};
     static_assert(sizeof(roles) / sizeof(roles[0]) == kRoleLeft + 1, "a text for each role");
-    const bool streaming = e[2] == kRoleStaged || e[2] == kRoleLeft;
-    last_error() = cat(what ? what : "", streaming ? ": the streaming expert kernel gave up a wait at tile " : ": a tcgen05 kernel gave up a wait at work item ",
-                       e[1], " (", roles[e[2] >= 1 && e[2] <= kRoleLeft ? e[2] : 0], "); its outputs are incomplete");
+    static const char *attn_roles[] = {"a copy warp waiting for a free place for keys and values",
+                                       "the MMA warp waiting for keys, values, queries or weights",
+                                       "a softmax warp waiting for scores, values or sums"};
+    const bool streaming = e[2] == kRoleStaged || e[2] == kRoleLeft, attn = e[2] >= kRoleAttnCopy && e[2] <= kRoleAttnSums;
+    last_error() = cat(what ? what : "", streaming ? ": the streaming expert kernel gave up a wait at tile " : attn ? ": the attention of many rows gave up a wait in CTA "
+                                                                                                             : ": a tcgen05 kernel gave up a wait at work item ",
+                       e[1], " (", attn ? attn_roles[e[2] - kRoleAttnCopy] : roles[e[2] >= 1 && e[2] <= kRoleLeft ? e[2] : 0], "); its outputs are incomplete");
     return SXB_ERR_DATA;
 }
 }  // namespace sxb

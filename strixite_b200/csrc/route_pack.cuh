@@ -35,6 +35,8 @@ int group_routes(const char *fn, const int32_t *ids, int64_t M, int64_t A, int64
 // Roles of the exact grouped forms in the status words (header words 5 .. 7), behind those of the tcgen05 kernels: a warp that waits for a tile's
 // staged activations, a staging warp that waits for the last warp to leave the buffer.
 constexpr int kRoleStaged = 10, kRoleLeft = 11;
+// ... and those of the attention of many rows (attn_decode_tc.cuh).
+constexpr int kRoleAttnCopy = 16, kRoleAttnMma = 17, kRoleAttnSums = 18;
 
 // The workspace of the grouping in which slot m * E + b belongs to bucket b, for all m < per_bucket: what sxb_moe_group_routes writes for
 // ids[m * E + b] = b, without the ids or the sort.  L = route_words(per_bucket * E, 1, E); by threads first, first + stride, ...

@@ -166,3 +166,41 @@ def test_write_leaves_what_it_does_not_turn_alone(cuda, D, rot, f32, interleaved
         assert torch.equal(torch.isnan(got), torch.isnan(put))
         assert torch.equal(got.nan_to_num(nan=0.0, posinf=1e9, neginf=-1e9), put.nan_to_num(nan=0.0, posinf=1e9, neginf=-1e9))
     assert torch.isfinite(q[..., :rot]).all() and torch.isfinite(k[..., :rot]).all()
+
+
+# ---- waits that run out ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("slot", [0, 1, 5, 9])
+@pytest.mark.parametrize("lens,new,page", [([60000], 17, 64), ([300] * 64, 17, 64), ([3000] * 6, 17, 8)], ids=["long", "many", "rows"])
+def test_many_rows_give_up_a_wait(cuda, lib, lens, new, page, slot):
+    """Tiles of 128 rows with CTA 0 told to leave one fill of keys and values out: the first, one behind a full turn of the places, one in a later segment.  The kernel
+    returns and frees what it holds, the status names the role, every output is the right one, NaN or untouched - nothing of the call before -, and the next
+    calls on the context, over the same workspace, have the bits of the first."""
+    b = Batch(cuda, 128, 16, 0, 8, 8, lens, [new] * len(lens), page=page, seed=2)
+    b.run()
+    torch.cuda.synchronize()
+    K().check_dense_status("warm-up")
+    want, q = (b.out.clone(), b.lse.clone()), b.q.clone()
+    b.q.copy_(torch.randn(b.q.shape, device=cuda))  # other parts in the workspace
+    b.run()
+    b.q.copy_(q)
+    b.out.fill_(UNTOUCHED), b.lse.fill_(UNTOUCHED)
+    try:
+        K().set_wait_limit(2_000_000)
+        assert lib.sxb_test_skip_ring_slot(slot) == 0
+        b.run()
+        torch.cuda.synchronize()
+    finally:
+        lib.sxb_test_skip_ring_slot(-1)
+        K().set_wait_limit(2_000_000_000)
+    with pytest.raises(K().Error, match=r"skipped fill: the attention of many rows gave up a wait in CTA 0 \((a copy warp|the MMA warp|a softmax warp) waiting for .*\); its outputs are incomplete"):
+        K().check_dense_status("skipped fill")
+    for got, right in zip((b.out, b.lse), want):
+        assert ((got == right) | torch.isnan(got) | (got == UNTOUCHED)).all() and not torch.equal(got, right)
+    for _ in range(3):
+        b.out.fill_(UNTOUCHED), b.lse.fill_(UNTOUCHED)
+        b.run()
+        torch.cuda.synchronize()
+        K().check_dense_status("after")
+        assert torch.equal(b.out, want[0]) and torch.equal(b.lse, want[1])
+    assert (b.guard == 0xA5).all() and int(b.err[0]) == 0
