@@ -77,6 +77,9 @@ class AttnLayer:
         D = cache.D
         if weights.qkv.N != (n_q + 2 * cache.n_kv) * D or weights.out.K != n_q * D:
             raise K.Error(1, f"AttnLayer: qkv of {weights.qkv.N} rows and out of {weights.out.K} columns do not fit {n_q} query and {cache.n_kv} key heads of {D}")
+        if buffers.qkv.shape[1] != weights.qkv.N or buffers.q.shape[1] != weights.out.K or buffers.qkv.device != cache.device:
+            raise K.Error(1, f"AttnLayer: buffers of {buffers.qkv.shape[1]} and {buffers.q.shape[1]} columns on {buffers.qkv.device}, the layer has {weights.qkv.N} and "
+                             f"{weights.out.K} on {cache.device}")
         self.w, self.n_q, self.cache, self.buf = weights, n_q, cache, buffers
         self.eps, self.scale, self.softcap, self.window = eps, scale, softcap, window
 
@@ -89,6 +92,10 @@ class AttnLayer:
         T, b, w = x.shape[0], self.buf, self.w
         if T > b.max_tokens or batch.max_q > b.max_q or x.dtype != torch.bfloat16:
             raise K.Error(1, f"AttnLayer: {T} rows of {x.dtype} with up to {batch.max_q} of a sequence, the buffers hold {b.max_tokens} of BF16 with {b.max_q}")
+        if (x.shape != (T, w.qkv.K) or y.shape != (T, w.out.N) or y.dtype not in (torch.bfloat16, torch.float32) or not (x.is_contiguous() and y.is_contiguous())
+                or x.device != self.cache.device or y.device != self.cache.device):
+            raise K.Error(1, f"AttnLayer: x {tuple(x.shape)} on {x.device} and y {tuple(y.shape)} of {y.dtype} on {y.device}, expected contiguous rows of {w.qkv.K} and of "
+                             f"{w.out.N}, y BF16 or FP32, on {self.cache.device}")
         qkv, q, o = b.qkv[:T], b.q[:T], b.o[:T]
         self._project(x, w.qkv, qkv, T)  # FP32: the norm, the rotation and the cache's codes are made of unrounded sums
         K.attn_qkv_write(qkv, self.cache, batch.seq, batch.pos, batch.pages, q, b.err, q_norm=w.q_norm, k_norm=w.k_norm, eps=self.eps, inv_freq=w.inv_freq,

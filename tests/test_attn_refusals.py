@@ -164,3 +164,31 @@ def test_report_attn_error(lib):
     K.report_attn_error([0, 0, 0], "step")
     with pytest.raises(K.Error, match=r"step: page, position, length or row range out of range at token or sequence 7 \(-1\)"):
         K.report_attn_error([1, 7, 0xFFFFFFFF], "step")
+
+
+def test_layer_refuses_rows_that_do_not_fit(lib, monkeypatch):
+    """What the projections would read or write beyond its end - x, y or buffers of another width, a view, another type - is refused before a launch."""
+    import types
+    import torch
+    from strixite_b200 import kernels as K
+    from strixite_b200.attention import AttnLayer, AttnWeights
+    for name in ("linear_qw", "linear_qw_wmma", "attn_qkv_write", "attn_decode"):
+        monkeypatch.setattr(K, name, lambda *a, **kw: pytest.fail("launched"))
+    cache = types.SimpleNamespace(D=64, n_kv=2, device=torch.device("cpu"))
+    def view(n, k):
+        return K.QDeviceView(None, None, None, n, k, 64, 8)
+    def buffers(n_qkv=512, n_q=256, rows=10):
+        return types.SimpleNamespace(max_tokens=rows, max_q=4, qkv=torch.zeros(rows, n_qkv), q=torch.zeros(rows, n_q), o=torch.zeros(rows, n_q))
+    weights = AttnWeights(view(512, 96), view(96, 256))
+    for bad in (buffers(n_qkv=384), buffers(n_q=128)):
+        with pytest.raises(K.Error, match="AttnLayer: buffers of"):
+            AttnLayer(weights, 4, cache, bad)
+    layer, batch = AttnLayer(weights, 4, cache, buffers()), types.SimpleNamespace(max_q=1)
+    bf = torch.bfloat16
+    x, y = torch.zeros(3, 96, dtype=bf), torch.zeros(3, 96, dtype=bf)
+    for bad_x, bad_y in ((torch.zeros(3, 64, dtype=bf), y), (torch.zeros(3, 96, 1, dtype=bf), y), (torch.zeros(3, 192, dtype=bf)[:, :96], y), (x, y[:2]), (x, y[:, :64]),
+                         (x, torch.zeros(96, 3, dtype=bf).t()), (x, y.double()), (x, y.to("meta"))):
+        with pytest.raises(K.Error, match="AttnLayer: x .* expected contiguous rows of 96 and of 96"):
+            layer.forward(bad_x, batch, bad_y)
+    with pytest.raises(K.Error, match="the buffers hold 10"):
+        layer.forward(torch.zeros(11, 96, dtype=bf), batch, torch.zeros(11, 96, dtype=bf))
