@@ -32,7 +32,7 @@ class AttnWeights:
 
 @dataclass
 class AttnBatch:
-    """A step's rows: row t is position pos[t] of sequence seq[t]; sequence b has the rows q_start[b] .. q_start[b + 1] - 1 and kv_len[b] keys, its new
+    """A step's rows: row t is position pos[t] of sequence seq[t] (seq[t] < 0: a padding row); sequence b has the rows q_start[b] .. q_start[b + 1] - 1 and kv_len[b] keys, its new
     tokens' included, on the pages of table row b.  All int32 on the device."""
 
     seq: torch.Tensor
@@ -65,6 +65,7 @@ class AttnBuffers:
         self.o = torch.empty((max_tokens, n_q * D), dtype=torch.bfloat16, device=dev)
         self.ws = torch.zeros(K.attn_decode_workspace_bytes(cache, n_q, max_q), dtype=torch.uint8, device=dev)
         self.err = torch.zeros(4, dtype=torch.int32, device=dev)
+        self.nothing, self.none = (torch.tensor(v, dtype=torch.bfloat16, device=dev) for v in (0.0, float("nan")))
 
 
 class AttnLayer:
@@ -88,7 +89,8 @@ class AttnLayer:
         (K.linear_qw_wmma if T >= self.wmma_min_tokens else K.linear_qw)(x, w, y, T, Act.BF16, out_act)
 
     def forward(self, x: torch.Tensor, batch: AttnBatch, y: torch.Tensor):
-        """x [T, d] BF16 -> y [T, d] (BF16 or FP32); the batch's keys and values are in the cache afterwards."""
+        """x [T, d] BF16 -> y [T, d] (BF16 or FP32); the batch's keys and values are in the cache afterwards.  A padding row (seq < 0, behind the last
+        sequence's rows) becomes zeros, a row that no accepted range of q_start holds NaN."""
         T, b, w = x.shape[0], self.buf, self.w
         if T > b.max_tokens or batch.max_q > b.max_q or x.dtype != torch.bfloat16:
             raise K.Error(1, f"AttnLayer: {T} rows of {x.dtype} with up to {batch.max_q} of a sequence, the buffers hold {b.max_tokens} of BF16 with {b.max_q}")
@@ -100,6 +102,8 @@ class AttnLayer:
         self._project(x, w.qkv, qkv, T)  # FP32: the norm, the rotation and the cache's codes are made of unrounded sums
         K.attn_qkv_write(qkv, self.cache, batch.seq, batch.pos, batch.pages, q, b.err, q_norm=w.q_norm, k_norm=w.k_norm, eps=self.eps, inv_freq=w.inv_freq,
                          interleaved=w.interleaved)
+        # the attention writes the rows of sequences; the buffer's others are an earlier layer's or step's
+        torch.where((batch.seq < 0).unsqueeze(1).expand_as(o), b.nothing, b.none, out=o)
         K.attn_decode(q, self.cache, batch.pages, batch.q_start, batch.kv_len, batch.max_q, o, b.ws, b.err, scale=self.scale, softcap=self.softcap,
                       window=self.window)
         self._project(o, w.out, y, T)

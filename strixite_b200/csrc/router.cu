@@ -203,7 +203,7 @@ int sxb_check_expert_error(const uint32_t *err, const char *what) {
 int sxb_report_attn_error(const uint32_t e[3], const char *what) {
     if (e[0] == 0) return SXB_OK;
     last_error() = cat(what, ": page, position, length or row range out of range at token or sequence ", e[1], " (", (int32_t)e[2],
-                       "); the affected outputs are NaN");
+                       "); the affected outputs are NaN, the rows of a refused range are left as they were");
     return SXB_ERR_DATA;
 }
 

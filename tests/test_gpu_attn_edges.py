@@ -204,3 +204,45 @@ def test_many_rows_give_up_a_wait(cuda, lib, lens, new, page, slot):
         K().check_dense_status("after")
         assert torch.equal(b.out, want[0]) and torch.equal(b.lse, want[1])
     assert (b.guard == 0xA5).all() and int(b.err[0]) == 0
+
+
+# ---- the sublayer ---------------------------------------------------------------------------------------------------------------------
+
+def small_layer(device, D, n_q, n_kv, d, bits, G, max_tokens, max_q, n_pages, page, seed):
+    from strixite_b200.attention import AttnBuffers, AttnLayer, AttnWeights
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    def weight(n, k):
+        return K().quantize(torch.randn((n, k), generator=g, device=device) * 0.05, 64, 8)
+    inv = (1e4 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)).float().to(device)
+    cache = K().KvCache.empty(n_pages, n_kv, page, D, bits, G, device)
+    norms = [1 + 0.1 * torch.randn(D, generator=g, device=device) for _ in range(2)]
+    layer = AttnLayer(AttnWeights(weight((n_q + 2 * n_kv) * D, d), weight(d, n_q * D), *norms, inv), n_q, cache, AttnBuffers(max_tokens, max_q, n_q, cache))
+    return layer, g
+
+
+def test_layer_shows_nothing_of_earlier_steps(cuda):
+    """Padding rows and rows of a refused range after a step that had other conversations in the same buffers: zeros and NaN, the rest as without them."""
+    from strixite_b200.attention import AttnBatch
+    d = 256
+    layer, g = small_layer(cuda, 64, 4, 2, d, 8, 32, 16, 16, 20, 16, 3)
+    pages = torch.arange(20, dtype=torch.int32, device=cuda).view(4, 5)
+    x = torch.randn((16, d), generator=g, device=cuda).to(torch.bfloat16)
+    y = torch.empty_like(x)
+    layer.forward(x, AttnBatch.of((0, 0, 0, 0), (9, 5, 1, 1), pages), y)
+    layer.check_errors()
+    x = torch.randn((8, d), generator=g, device=cuda).to(torch.bfloat16)
+    want, got = torch.empty((3, d), dtype=torch.bfloat16, device=cuda), torch.empty((8, d), dtype=torch.bfloat16, device=cuda)
+    plain_batch = AttnBatch.of((9, 5), (2, 1), pages[:2])
+    layer.forward(x[:3].contiguous(), plain_batch, want)
+    batch = AttnBatch.of((9, 5), (2, 1), pages[:2])
+    batch.seq = torch.cat((batch.seq, torch.full((5,), -1, dtype=torch.int32, device=cuda)))
+    batch.pos = torch.cat((batch.pos, torch.zeros(5, dtype=torch.int32, device=cuda)))
+    layer.forward(x, batch, got)
+    layer.check_errors()
+    assert torch.equal(got[:3], want) and (got[3:] == 0).all()
+    batch.q_start[2] = 99  # the second sequence's range is refused
+    layer.forward(x, batch, got)
+    assert torch.equal(got[:2], want[:2]) and torch.isnan(got[2]).all() and (got[3:] == 0).all()
+    with pytest.raises(K().Error, match="rows of a refused range"):
+        layer.check_errors()
