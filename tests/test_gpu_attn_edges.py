@@ -9,7 +9,7 @@ from test_gpu_attn import Batch, K, Rows
 
 pytestmark = pytest.mark.gpu
 
-UNTOUCHED = 12345.0
+UNTOUCHED = 2.0 ** 120  # a BF16 number that no case comes to
 
 
 def run_and_compare(b, scale=None, softcap=0.0, window=0, rows=None):
@@ -168,6 +168,82 @@ def test_write_leaves_what_it_does_not_turn_alone(cuda, D, rot, f32, interleaved
     assert torch.isfinite(q[..., :rot]).all() and torch.isfinite(k[..., :rot]).all()
 
 
+# ---- every row's log-sum -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("group,new", [(4, 1), (8, 2), (3, 7), (8, 8), (8, 17)], ids=["rows4", "rows16", "rows21", "rows64", "rows136"])
+@pytest.mark.parametrize("D,bits,G", [(64, 16, 0), (128, 16, 0), (256, 16, 0), (128, 8, 64), (256, 4, 32)])
+def test_every_log_sum_is_written(cuda, D, bits, G, group, new):
+    """Rows without a key, with one, in whole segments and in joined ones: an output and a log-sum each, none left as it was, none NaN."""
+    b = Batch(cuda, D, bits, G, 2, group, [1, new, 65, 0, 6000, max(1, new - 2)], [1, new, new, 1, new, new], page=16, seed=D + bits + group)
+    run_and_compare(b)
+
+
+def test_log_sums_beside_rows_of_no_sequence(cuda):
+    """Ranges that begin behind row 0 and leave rows out: their log-sums, and the others as they were."""
+    for group in (2, 40):
+        b = Batch(cuda, 128, 16, 0, 2, group, [40, 20, 333], [2, 1, 1], seed=8)
+        q = torch.randn((9, b.n_q * 128), device=cuda).to(torch.bfloat16)
+        out, lse = torch.full_like(q, UNTOUCHED), torch.full((9, b.n_q), UNTOUCHED, device=cuda)
+        starts = torch.tensor([1, 3, 3, 4], dtype=torch.int32, device=cuda)  # rows 1-2, none, row 3
+        K().attn_decode(q, b.cache, b.pages, starts, b.kv_len, 2, out, b.ws, b.err, lse=lse)
+        torch.cuda.synchronize()
+        want, want_lse, tol, lse_tol = plain.attend(q, b.cache, b.pages, starts, b.kv_len, 128 ** -0.5)
+        assert (np.abs(plain.f64(out).reshape(want.shape)[1:4] - want[1:4]) <= tol[1:4]).all() and (np.abs(plain.f64(lse)[1:4] - want_lse[1:4]) <= lse_tol[1:4]).all()
+        rest = [0, 4, 5, 6, 7, 8]
+        assert (lse[rest] == UNTOUCHED).all() and (out[rest] == UNTOUCHED).all()
+
+
+# ---- far pages, long chunks ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("page,token_major", [(64, False), (8, False), (64, True), (8, True)])
+def test_many_rows_beyond_32_bits(cuda, page, token_major):
+    """Tiles of 128 rows and of 32 on pages that lie more than 2^32 bytes behind a pool's start: by tensor copies, and row by row (pages of eight)."""
+    D, n_kv = 128, 8
+    n_pages = (9 << 30) // (n_kv * page * D * 2)
+    shape = (n_pages, page, n_kv, D) if token_major else (n_pages, n_kv, page, D)
+    k, v = (torch.empty(shape, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    if token_major:
+        k, v = k.transpose(1, 2), v.transpose(1, 2)
+    cache = K().KvCache(k, v, 16)
+    n, g = 150, torch.Generator(device=cuda)
+    g.manual_seed(page)
+    used = -(-n // page)
+    pages = torch.randperm(used, generator=g, device=cuda).add(n_pages - used).to(torch.int32).view(1, used)
+    for t in (k, v):
+        t[n_pages - used:] = torch.randn((used, n_kv, page, D), generator=g, device=cuda).to(torch.bfloat16)
+    err = torch.zeros(4, dtype=torch.int32, device=cuda)
+    lens = torch.tensor([n], dtype=torch.int32, device=cuda)
+    for new in (17, 3, 1):  # of eight heads a key head: 136, 24 and 8 rows
+        q = torch.randn((new, n_kv * 8 * D), generator=g, device=cuda).to(torch.bfloat16)
+        out, lse = torch.empty_like(q), torch.empty((new, n_kv * 8), device=cuda)
+        ws = torch.zeros(K().attn_decode_workspace_bytes(cache, n_kv * 8, new), dtype=torch.uint8, device=cuda)
+        starts = torch.tensor([0, new], dtype=torch.int32, device=cuda)
+        K().attn_decode(q, cache, pages, starts, lens, new, out, ws, err, lse=lse)
+        want, want_lse, tol, lse_tol = plain.attend(q, cache, pages, starts, lens, D ** -0.5)
+        assert (np.abs(plain.f64(out).reshape(want.shape) - want) <= tol).all() and (np.abs(plain.f64(lse) - want_lse) <= lse_tol).all()
+    assert int(err[0]) == 0
+    K().check_dense_status("far pages")
+
+
+@pytest.mark.parametrize("kept,window", [(0, 0), (6144, 0), (1000, 1024)])
+def test_a_chunk_of_2048_tokens(cuda, kept, window):
+    """A prompt's first chunk, one far into a context, one behind a window: rows at the tiles' ends and among them against the definition."""
+    new, group, D = 2048, 8, 128
+    b = Batch(cuda, D, 16, 0, 2, group, [kept + new], [new], page=64, seed=kept)
+    b.out.fill_(UNTOUCHED), b.lse.fill_(UNTOUCHED)
+    b.run(window=window)
+    torch.cuda.synchronize()
+    K().check_dense_status("chunk")
+    assert int(b.err[0]) == 0 and (b.guard == 0xA5).all() and not (b.out == UNTOUCHED).any() and not (b.lse == UNTOUCHED).any()
+    assert torch.isfinite(b.out).all() and torch.isfinite(b.lse).all()
+    # tiles are of sixteen tokens; the last sixteen rows a call: a sequence of its own that ends with the row
+    for t in (0, 1, 15, 16, 17, 127, 128, 1000, 1023, 1024, 2031, 2032, 2047):
+        lens = torch.tensor([kept + t + 1], dtype=torch.int32, device=cuda)
+        want, lse, tol, lse_tol = plain.attend(b.q[t:t + 1], b.cache, b.pages, torch.tensor([0, 1]), lens, D ** -0.5, 0.0, window)
+        assert (np.abs(plain.f64(b.out[t:t + 1]).reshape(want.shape) - want) <= tol).all(), t
+        assert (np.abs(plain.f64(b.lse[t:t + 1]) - lse) <= lse_tol).all(), t
+
+
 # ---- waits that run out ---------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("slot", [0, 1, 5, 9])
@@ -246,3 +322,89 @@ def test_layer_shows_nothing_of_earlier_steps(cuda):
     assert torch.equal(got[:2], want[:2]) and torch.isnan(got[2]).all() and (got[3:] == 0).all()
     with pytest.raises(K().Error, match="rows of a refused range"):
         layer.check_errors()
+
+
+def test_layer_of_chunks_on_tcgen05(cuda):
+    """Heads of 128 over a BF16 cache: a prompt in chunks of many rows a key head, then a step of one token; the attention is the definition's."""
+    from strixite_b200.attention import AttnBatch
+    d, n_q, n_kv, D = 256, 8, 2, 128
+    layer, g = small_layer(cuda, D, n_q, n_kv, d, 16, 0, 300, 200, 40, 16, 5)
+    pages = torch.randperm(40, generator=g, device=cuda).to(torch.int32).view(2, 20)
+    kept = [0, 0]
+    for new in ((200, 33), (90, 1), (1, 40), (1, 1)):
+        T = sum(new)
+        x = torch.randn((T, d), generator=g, device=cuda).to(torch.bfloat16)
+        batch = AttnBatch.of(kept, new, pages)
+        kept = [k + n for k, n in zip(kept, new)]
+        y = torch.empty((T, d), dtype=torch.float32, device=cuda)
+        layer.forward(x, batch, y)
+        layer.check_errors()
+        o, q = layer.buf.o[:T], layer.buf.q[:T]
+        want, _, tol, _ = plain.attend(q, layer.cache, pages, batch.q_start, batch.kv_len, D ** -0.5)
+        assert (np.abs(plain.f64(o).reshape(want.shape) - want) <= tol).all()
+        again = torch.empty_like(y)
+        (K().linear_qw_wmma if T >= 64 else K().linear_qw)(o.clone(), layer.w.out, again, T, K().Act.BF16, K().Act.F32)
+        assert torch.equal(y, again) and torch.isfinite(y).all()
+
+
+# ---- calls side by side, captured chains ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits,G,group", [(16, 0, 8), (16, 0, 40), (8, 64, 8), (4, 32, 16)])
+def test_two_calls_at_once(cuda, bits, G, group):
+    """Two streams with a workspace each: the bits of one call after the other."""
+    pair = [Batch(cuda, 128, bits, G, 2, group, [9000, 70, 3000], [1, 2, 1], page=32, seed=40 + i) for i in range(2)]
+    want = []
+    for b in pair:
+        b.run()
+        torch.cuda.synchronize()
+        want.append((b.out.clone(), b.lse.clone()))
+    streams = [torch.cuda.Stream() for _ in pair]
+    for _ in range(20):
+        for b in pair:
+            b.out.fill_(UNTOUCHED), b.lse.fill_(UNTOUCHED)
+        torch.cuda.synchronize()
+        for b, s in zip(pair, streams):
+            b.run(stream=s)
+        torch.cuda.synchronize()
+        for b, w in zip(pair, want):
+            assert torch.equal(b.out, w[0]) and torch.equal(b.lse, w[1]) and (b.guard == 0xA5).all() and int(b.err[0]) == 0
+
+
+@pytest.mark.parametrize("bits,G", [(16, 0), (8, 64), (4, 32)])
+def test_a_captured_step_replayed_with_other_batches(cuda, bits, G):
+    """The whole sublayer in a graph of eight rows and three sequences, replayed with other positions, lengths, ranges and padding: the bits of calls one by one."""
+    from strixite_b200.attention import AttnBatch
+    d, D = 256, 128
+    layer, g = small_layer(cuda, D, 8, 2, d, bits, G, 64, 16, 60, 16, 7)
+    def fresh():
+        layer.cache.k.zero_(), layer.cache.v.zero_()
+    pages = torch.randperm(60, generator=g, device=cuda).to(torch.int32).view(3, 20)
+    steps = [((0, 0, 0), (3, 4, 1)), ((3, 4, 1), (1, 1, 1)), ((4, 5, 2), (0, 2, 4)), ((4, 7, 6), (2, 0, 1)), ((200, 150, 300), (1, 6, 1))]
+    def batch_of(kept, new):
+        b = AttnBatch.of(kept, new, pages)
+        more = 8 - sum(new)
+        b.seq = torch.cat((b.seq, torch.full((more,), -1, dtype=torch.int32, device=cuda)))
+        b.pos = torch.cat((b.pos, torch.zeros(more, dtype=torch.int32, device=cuda)))
+        b.max_q = 8
+        return b
+    xs = [torch.randn((8, d), generator=g, device=cuda).to(torch.bfloat16) for _ in steps]
+    want = []
+    fresh()
+    for x, step in zip(xs, steps):
+        y = torch.empty_like(x)
+        layer.forward(x, batch_of(*step), y)
+        want.append(y.clone())
+    layer.check_errors()
+    held, x, y = batch_of(*steps[0]), xs[0].clone(), torch.empty_like(xs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.forward(x, held, y)
+    fresh()
+    for x_now, step, w in zip(xs, steps, want):
+        now = batch_of(*step)
+        for name in ("seq", "pos", "q_start", "kv_len"):
+            getattr(held, name).copy_(getattr(now, name))
+        x.copy_(x_now)
+        graph.replay()
+        assert torch.equal(y, w) and (y[sum(step[1]):] == 0).all()
+    layer.check_errors()
