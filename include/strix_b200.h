@@ -259,8 +259,8 @@ int sxb_route_layout(int64_t M, int64_t A, int64_t E, int64_t out[8]);
 int sxb_set_wait_limit(uint64_t nanoseconds);
 /* Test hook, no counterpart in the reference: slot >= 0 makes CTA 0 of the following launches leave that fill out - of the
  * weight-code ring in the tcgen05 expert kernels and dense projections, of the h stages in the up mix up to rank 512, of the
- * stages in the router-logits GEMM, of the places for keys and values in the attention of many rows - or, in the exact grouped forms, an arrival of its second (even slot) or third tile
- * (odd), so a bounded wait runs out and the kernel's give-up path runs; -1 (the default) = off. */
+ * stages in the router-logits GEMM, of the places for keys and values in the attention of many rows - or, in the exact grouped
+ * forms, an arrival of its second (even slot) or third tile (odd), so a bounded wait runs out and the kernel's give-up path runs; -1 (the default) = off. */
 int sxb_test_skip_ring_slot(int slot);
 
 /* ---- Dense quantized linear --------------------------------------------------------------------------------- */
@@ -565,9 +565,12 @@ int sxb_kv_read(const SxbKvReadArgs *args, sxb_stream_t stream);
  * reads key head h / (n_q / n_kv).  Scores scale * q . k (scale > 0), with softcap > 0 softcap * tanh(score / softcap).
  * out [T, out_ld] BF16 = softmax(scores) . V, lse [T, n_q] FP32 (or NULL) = log of the sum of exp(score); a row that sees no key
  * (or none with a score above -1e30): 0 and -inf.  Rows outside every sequence are left as they are.  Scores, statistics and
- * sums are FP32; weights are rounded to BF16 (BF16 cache) or, times a group's scale, to F16 for the product with V.
- * max_q: a sequence's largest count of new tokens, which picks the kernel (a sequence with more is handled, in several passes over
- * its keys).  Chunks of prompt tokens: over a BF16 cache with heads of 128 more than 32 rows a key head run on tcgen05, 128 at a time (a device-side
+ * sums are FP32; weights are rounded to BF16 (BF16 cache) or, times a group's scale, to F16 for the product with V (keys beside a group scale more than
+ * 2^8 below the largest one so far: not rounded, and three times as slow); with codes, elements of a query more than 2^28 below its largest lose bits.
+ * A key, value, scale or min that is not finite reaches the rows that see it, a value's only its own column, a value group's only its own columns.
+ * max_q: a sequence's largest count of new tokens, which picks the kernel together with B, the heads and n_cols (a sequence with more is handled, in
+ * several passes over its keys); kernels add in different orders, so the same rows may differ in last bits between calls whose sizes differ.
+ * Chunks of prompt tokens: over a BF16 cache with heads of 128 more than 32 rows a key head run on tcgen05, 128 at a time (a device-side
  * wait that ran out there is reported by sxb_check_dense_status); other caches' are right, 16 or 32 rows at a time, and slow.
  * ws: sxb_attn_decode_workspace_bytes, device, 16-byte aligned, zeroed once before its first use; every call leaves what it needs
  * of it zeroed.  Calls that share a workspace must be ordered (one stream, or events); the sizes depend on the device.

@@ -9,7 +9,7 @@
 // and rotation are one pair of factors an element, the same for all heads: x'_i = inv * (x_i (w_i cos) + x_partner (w_partner +- sin)).
 // The same formulas as sxb_quantize's make the codes (formats/q4.cpp:44-88), from the FP32 values: nothing is rounded on the way.
 //
-// Measured (B200; us, and the time of the bytes alone at the measured copy rate): 4096 tokens of 32 + 2 x 8 heads of 128 into a BF16 cache 22.6 (15.4), one
+// Measured (B200; us, and the time of the bytes alone at the measured copy rate): 4096 tokens of 32 + 2 x 8 heads of 128 into a BF16 cache 22.2 (15.4), one
 // token 3.2 (a launch and four round trips); 33000 rows of 2 x 8 heads of 128 at 8 bits read back as BF16 41 (32).  A warp a token in the first: with a warp
 // for half a token 26, a CTA a token 40 (angles and factors made again for every few heads).
 

@@ -11,14 +11,17 @@
 // The query heads of a key head and the new tokens of a sequence are the rows of one MMA tile: the cache is read once for all of them.  Products on
 // mma.sync: the rows are eight to 32, a warp's keys sixteen, and what bounds is memory (BF16) or the conversion of codes, not the tensor cores; operands
 // come from shared memory, tiles there by cp.async from wherever the pages lie, each warp's by itself.
-//   BF16 cache: exact products; weights rounded to BF16 (one rounding of 2^-9 a key, against the sum's many keys).
+//   BF16 cache: exact products; weights rounded to BF16, as the second product's operands have one type (one rounding of 2^-9 a key, to either side, against
+//   the sum's many keys; the sum of weights keeps them unrounded).
 //   8 and 4 bits: the codes are F16 numbers exactly, q is F16 times a power of two a row (a BF16 number less than 2^28 below the row's largest is exact),
 //   scale and min go on in FP32: s = scale_k * (q . code) + min_k * sum(q) a group.  For V a key's weight takes its group's scale, times a power of
-//   two that follows the largest scale seen so that F16's range is no limit (one rounding of 2^-11); the mins' share, sum p * min, is FP32.
+//   two that follows the largest scale seen so that F16's range is no limit (one rounding of 2^-11); the mins' share, sum p * min, is FP32.  Sixteen keys among
+//   whose scales one is far below the largest, or none, are added up by the threads in FP32 (add_values).
+// Exponentials are ex2.approx (2^-22 of a weight, below either rounding).
 //
-// Measured (B200; us, and the time of the bytes alone at the measured copy rate): one sequence of 200001 keys, 8 key heads of 128, BF16, 132 (125); 64
-// sequences of 100 to 16000 keys, 8 bits, 185 (172); 32 of 9509, 4 bits with groups of 32, 139 (59): there the bound is the integer pipe, half busy with
-// codes and scales, behind it two to three warps a scheduler.  Several rows: 32 sequences x 4 rows of 8 heads x 9509 keys BF16 109 (95), 8 bits 154 (51).
+// Measured (B200; us, and the time of the bytes alone at the measured copy rate): one sequence of 200001 keys, 8 key heads of 128, BF16, 129 (125); 64
+// sequences of 100 to 16000 keys, 8 bits, 190 (172); 32 of 9509, 4 bits with groups of 32, 144 (59): there the bound is the integer pipe, half busy with
+// codes and scales, behind it two to three warps a scheduler.  Several rows: 32 sequences x 4 rows of 8 heads x 9509 keys BF16 109 (95), 8 bits 160 (51).
 // 300 keys of one sequence: 7, nothing but latencies - lengths, page table, keys, join.
 
 #include "attn.cuh"
@@ -41,7 +44,7 @@ constexpr int kMostPerSm = 4;
 constexpr int kSlack = 8;      // powers of two that a weight may be above 1
 // Powers of two that a value group's scale may be below the largest one so far.  The largest scale times a weight of 1 is 2^6 as an F16 number, one below by kSpread
 // 2^-2: weights down to 2^-12 then keep F16's eleven bits, and what the smaller ones lose, 2^-25 a key at most, is 2^-23 of that group's own scale.
-// Sixteen keys with a scale further down are added up in FP32 by the threads (twice to three times their time).
+// Sixteen keys with a scale further down are added up in FP32 by the threads (three times their time: 32 sequences of 4009 keys, 8 bits, 35 us, 104 if all of them are).
 constexpr uint32_t kSpread = 8;
 constexpr uint32_t kLowestScale = (20 - kSpread) << 23;  // as a bit pattern
 constexpr float kLowest = -1e30f;  // below every score; a row that sees no key keeps it
@@ -78,7 +81,8 @@ template <int D_, int BITS_, int G_, int R_> struct Shape {
     }
     static constexpr int DC = fit_columns();  // columns that the warps join at a time
     // Codes stay too large by so much as F16 operands, and what that adds is taken out of the sums: K's by 1024 (8 bits) or 64, V's too, but for every
-    // second 4-bit code, which 1024 saves a shift - what that costs a score (an offset of a hundred times the codes) would be seen, of an output it is not.
+    // second 4-bit code, which 1024 saves a shift - what that costs a score (an offset of a hundred times the codes) would be seen, of an output it is not
+    // (where it leaves the sums every sixteen tiles: see take_out).
     static constexpr float kOffsetK = BITS == 8 ? 1024.f : 64.f, kOffset = 1024.f, kOffsetOdd = kOffsetK;
     // Few rows: the last CTA to bring its part joins them, a launch less.  Many: that CTA would read every part by itself (2 x 8 rows over 32 k keys:
     // 19 parts of 33 KB, 30 us at the end of 80), a second kernel has the rows of all segments side by side.
@@ -1260,7 +1264,8 @@ inline int tile_rows(int D, int bits, int64_t rows) { return rows <= 8 ? 8 : row
 // Tiles of 128 rows on tcgen05 (attn_decode_tc.cuh): more than 32 rows, and enough tiles that a table has room for, so that its start - tensor memory, a stage
 // to fill before the first product - is no matter.  Rows, sequences x keys, us with tiles of 32 and with it: 64, 64 x up to 8000, 191 and 136; 2 x up to 33000, 52
 // and 44; 8 x up to 9000, 35 and 35; 16 x 1000, 25 and 27; 1 x 300, 11 and 14; 128, 64 x up to 8000, 460 and 176; 16 x 1000, 35 and 36.  Chunks of 512 tokens of eight
-// heads a key head on 4096 keys, 170 and 60, of 2048 on 8192, 1338 and 287.
+// heads a key head on 4096 keys, 170 and 60, of 2048 on 8192, 1338 and 290.  The lengths are the device's to know; a host whose tables have room for far longer
+// sequences than there are pays those 3 us, and gets by passing fewer columns what shorter tables give (the bits too: the forms add in other orders).
 constexpr bool has_tc(int D, int bits) { return D == TcShape::D && bits == TcShape::BITS; }
 inline bool takes_tc(int D, int bits, int64_t rows, int64_t B, int64_t n_kv, int64_t capacity) {
     if (!has_tc(D, bits) || rows <= most_rows(D, bits)) return false;

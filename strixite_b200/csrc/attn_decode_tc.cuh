@@ -7,7 +7,7 @@
 // are joined at a segment's end, so that no thread waits for another one's scores.  The maximum that a row goes by is raised, and its sums scaled, only by a
 // tile that passes it by more than 2^kSlack.  One warp issues the products, the next tile's scores ahead of this one's weights; three fetch, a stage each.
 //
-// Measured (B200): 2048 tokens of eight heads a key head on 8192 keys, four key heads, 287 us, 840 TFLOP/s of what the mask leaves; a tile of 128 x 128 takes about
+// Measured (B200): 2048 tokens of eight heads a key head on 8192 keys, four key heads, 290 us, 830 TFLOP/s of what the mask leaves; a tile of 128 x 128 takes about
 // 2000 cycles, of which the products are 1230 and the exponentials 1024.  64 rows over 64 sequences of 100 to 8000 keys 136 us (bytes alone 81): there a tile
 // is half empty, and a sequence's start and end, 5000 cycles, count.  Two warps' scores of one row with one maximum (a barrier of the two a tile) took 497 us
 // in the first case, the copies by cp.async (three warps, a third of each tile's rows) 294, boxes of sixteen rows whatever the pages 343.
