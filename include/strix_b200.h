@@ -526,7 +526,7 @@ typedef struct SxbKvCache {
 } SxbKvCache;
 
 /* The step between the projections and the attention.  qkv [T, ld >= (n_q + 2 n_kv) D], BF16 or FP32 (act): per token the query
- * heads, the key heads, the value heads.  Queries and keys: x / sqrt(mean(x^2) + eps) * norm weight [D] (FP32; NULL: no norm), then
+ * heads, the key heads, the value heads.  Queries and keys: x / sqrt(mean(x^2) + eps) * norm weight [D] (FP32, the squares' sum too; NULL: no norm), then
  * the first rot elements turned by pos * inv_freq[i] (FP32 [rot / 2]; the product in FP64): pairs (i, i + rot / 2), or (2i, 2i + 1)
  * if interleaved; rot = 0: none, else a multiple of 16.  Queries to q_out [T, q_ld >= n_q D] BF16; keys and values of token t to
  * position pos[t] of sequence seq[t]: rounded once to BF16, or quantized from the FP32 values as sxb_quantize does (a group that
