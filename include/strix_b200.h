@@ -599,6 +599,84 @@ int sxb_attn_decode(const SxbAttnDecodeArgs *args, sxb_stream_t stream);
 int sxb_check_attn_error(const uint32_t *err, const char *what);
 int sxb_report_attn_error(const uint32_t e[3], const char *what);
 
+/* ---- Around the head: norm into 8-bit codes, products of 8-bit floating point, verification of drafts ----------- */
+
+/* No counterparts among the reference's launchers mirrored here.  Codes are e4m3 (4 exponent and 3 fraction bits, +-448, NaN = 0x7f), with an
+ * FP32 scale for every block of 128 along a row: element = code * scale.  An activation's scales [rows, ceil(K / 128)] are its own, a weight's
+ * [ceil(N / 128), ceil(K / 128)] belong to 128 rows; the last block of a row, or of rows, may be short. */
+typedef struct SxbF8View {
+    const uint8_t *q;   /* [N, K], rows contiguous */
+    const float *scale; /* [ceil(N / 128), ceil(K / 128)] */
+    int64_t N, K;
+} SxbF8View;
+
+/* Residual's addition and norm.  s = x + y, rounded to x's type; n = s / sqrt(mean(s^2) + eps) * weight (FP32 [d], the factor itself, NULL: 1; FP32
+ * throughout, the squares' sum too: a row whose squares sum to more than FP32 holds becomes zeros); normed = 0: n = s, no norm.  Outputs, each may be NULL, one
+ * at least given: total [T, d] = s in x's type (with y only; may be x or y itself), out [T, d] BF16 = n, codes and scales (both or none): per block of 128, scale = the larger of
+ * max|n| / 448 and 2^-64, code = n / scale to the nearest, ties to even.  A block that holds a NaN or an infinity has a NaN scale and reads back as NaN.
+ * y: NULL, BF16 or FP32 (y_act).  act: BF16 or FP32, of x and total.  d = 16 .. 32768, a multiple of 16; T = 1 .. 2^24.  Strides in elements; every row 16-byte
+ * aligned, scales 4-byte. */
+typedef struct SxbAddNormArgs {
+    const void *x, *y;
+    const float *weight;
+    void *total, *out;
+    uint8_t *codes;
+    float *scales;
+    int64_t T, d, x_ld, y_ld, total_ld, out_ld, codes_ld, scales_ld;
+    float eps;
+    int act, y_act, normed;
+} SxbAddNormArgs;
+int sxb_add_norm(const SxbAddNormArgs *args, sxb_stream_t stream);
+
+/* A weight w [N, K] (FP32 or BF16: act), rows contiguous, to codes [N, K] and scales of blocks of 128 x 128 by the formulas above.  Non-finite input sets err =
+ * {1, row, column} and makes its block's scale NaN.  K a multiple of 16, w and q 16-byte aligned. */
+int sxb_quantize_f8(const void *w, int act, int64_t N, int64_t K, uint8_t *q, float *scale, uint32_t *err, sxb_stream_t stream);
+
+/* y [M, N] = x W^T of codes: exact products of codes, summed in FP32 over a block of 128, times the two scales' product, added up over the blocks in FP32;
+ * one rounding to out_act (BF16 or FP32).  x [M, x_ld >= K] codes with x_scale [M, xs_ld >= ceil(K / 128)]; y [M, y_ld >= N].  M = 1 .. 2^20, N = 1 .. 2^24, K = 16 .. 2^20, a
+ * multiple of 16; x, w->q and their rows 16-byte aligned, y's rows on their type's.  Kernels for few and for many rows add in different orders: the same row may differ in
+ * last bits between calls of different M.  A device-side wait that ran out is reported by sxb_check_dense_status. */
+typedef struct SxbLinearF8Args {
+    const uint8_t *x;
+    const float *x_scale;
+    const SxbF8View *w;
+    void *y;
+    int64_t M, x_ld, xs_ld, y_ld;
+    int out_act;
+} SxbLinearF8Args;
+int sxb_linear_f8(const SxbLinearF8Args *args, sxb_stream_t stream);
+
+/* Verification of drafted tokens.  Sequence b has the rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]): the tokens ids [T] that were fed to the target there, the first one
+ * known, the others drafted, and the target's logits [T, ld >= V] (BF16 or FP32: act; masked tokens -inf).  With p_i = softmax(logits of row i / temperature[b]) and q_i the same of
+ * draft_logits [T, draft_ld >= V] (draft_act; row i is what row i + 1's token was drawn from, a sequence's last row is not read), or all of it on the drafted token if draft_logits is NULL:
+ * the token x of row i + 1 is kept if u[i] * q_i(x) < p_i(x).  At the first that is not, the sequence's next token is drawn from max(p_i - q_i, 0); if all are kept, from p of the last
+ * row: the lowest token up to which more than u_pick[b] of the sum has come.  A difference that sums to zero: p instead.  temperature (NULL: 1) of 0: the largest logit, the lowest token among equals;
+ * no random number is used.  Probabilities in FP32 (a draw finds no
+ * token below 2^-126 of the row's largest), sums of chunks in FP64; a random number within some 2^-22 of a border may fall on either side of it.
+ * Out: next_ids [T], for each row the token that comes behind it (kept drafts, then the drawn token), -1 in the rows behind; n_new [B] = tokens kept + 1; logp [T] (or NULL) = log of
+ * each such token's p (greedy: of softmax(logits)), 0 in the rows behind.  A sequence without rows has n_new = 0; rows outside every sequence are left as they are.
+ * ws: sxb_verify_drafts_workspace_bytes, device, 16-byte aligned, needs no clearing; calls that share it must be ordered.  T = 1 .. 2^20, V = 1 .. 2^20, B = 1 .. 2^20.
+ * Data errors, found in the rows that the decision reads (err = {1, row, code}): logits of a row that hold a NaN or +inf or nothing above -inf (code 1), a drafter's (2), a drafted token
+ * outside 0 .. V - 1 (3), a random number outside [0, 1) (4), a temperature other than 0 below 2^-126, or not finite (5): n_new = 0, the sequence's
+ * next_ids -1 and logp NaN.  A q_start that falls, leaves 0..T or starts below an earlier one (err = {1, sequence, 6}): n_new = 0, the rows are left as they are. */
+size_t sxb_verify_drafts_workspace_bytes(int64_t T, int64_t B, int64_t V);
+typedef struct SxbVerifyDraftsArgs {
+    const void *logits, *draft_logits;
+    int64_t ld, draft_ld, T, V, B;
+    const int32_t *ids, *q_start;
+    const float *u, *u_pick, *temperature;
+    int32_t *next_ids, *n_new;
+    float *logp;
+    void *ws;
+    size_t ws_bytes;
+    uint32_t *err;
+    int act, draft_act;
+} SxbVerifyDraftsArgs;
+int sxb_verify_drafts(const SxbVerifyDraftsArgs *args, sxb_stream_t stream);
+/* Its error words (a blocking 12-byte copy, as sxb_check_router_error) / already on the host. */
+int sxb_check_verify_error(const uint32_t *err, const char *what);
+int sxb_report_verify_error(const uint32_t e[3], const char *what);
+
 /* ---- Quantizers on the device ------------------------------------------------------------------------------- */
 
 /* formats/q4.hpp:32 quantize_q4 / formats/q8.hpp:32 quantize_q8, for weights already on the device: w [N, K] FP32 ->

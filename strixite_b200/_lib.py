@@ -33,6 +33,12 @@ class SxbKvCache(C.Structure):
                 ("page_stride", i64), ("head_stride", i64), ("row_stride", i64), ("bits", C.c_int)]
 
 
+class SxbF8View(C.Structure):
+    """A weight of 8-bit floating-point codes with a scale for each block of 128 x 128 (include/strix_b200.h), field for field."""
+
+    _fields_ = [("q", vp), ("scale", vp), ("N", i64), ("K", i64)]
+
+
 class SxbStrixwTensor(C.Structure):
     """formats/strixw.hpp:37-48 StrixwTensor, flattened (include/strix_b200.h)."""
 
@@ -137,6 +143,13 @@ SIGNATURES.update({  # argument blocks: bytes laid out as the header's structs (
     "sxb_attn_decode": (C.c_int, [vp, vp]),
     "sxb_check_attn_error": (C.c_int, [vp, cp]),
     "sxb_report_attn_error": (C.c_int, [C.POINTER(u32), cp]),
+    "sxb_add_norm": (C.c_int, [vp, vp]),
+    "sxb_quantize_f8": (C.c_int, [vp, C.c_int, i64, i64, vp, vp, vp, vp]),
+    "sxb_linear_f8": (C.c_int, [vp, vp]),
+    "sxb_verify_drafts_workspace_bytes": (sz, [i64, i64, i64]),
+    "sxb_verify_drafts": (C.c_int, [vp, vp]),
+    "sxb_check_verify_error": (C.c_int, [vp, cp]),
+    "sxb_report_verify_error": (C.c_int, [C.POINTER(u32), cp]),
 })
 for _b in ("q4", "q8"):
     SIGNATURES[f"sxb_linear_{_b}_experts_gather"] = (C.c_int, [vp, QV, i64, vp, i64, i64, vp, C.c_int, vp, vp])

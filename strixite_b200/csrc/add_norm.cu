@@ -1,0 +1,252 @@
+// The residual's addition and root-mean-square norm between two sublayers, with the outputs that the next product reads: s = x + y as stored, n = s /
+// sqrt(mean(s^2) + eps) * weight, n as BF16 or as e4m3 codes with a scale for every block of 128 (f8.cuh).  And the same codes, in blocks of 128 x 128, of a weight.
+//
+// One pass: a CTA has a row in registers between the sum of its squares and its codes, so x and y are read and s and the codes written once.
+
+#include "f8.cuh"
+
+namespace sxb {
+namespace {
+
+constexpr int kVec = 8;           // elements of a thread's piece of a row: sixteen neighbouring threads have a block
+constexpr int64_t kMaxD = 32768;
+
+struct NormArgs {
+    const void *x, *y;
+    const float *weight;
+    void *total;
+    uint16_t *out;
+    uint8_t *codes;
+    float *scales;
+    int64_t x_ld, y_ld, total_ld, out_ld, codes_ld, scales_ld;
+    int d, normed;
+    float eps;
+};
+
+__device__ inline void load8(const float *p, float (&v)[kVec]) {
+    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ inline void load8(const uint16_t *p, float (&v)[kVec]) {
+    const uint4 a = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ inline void store8(float *p, const float (&v)[kVec]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ inline void store8(uint16_t *p, const float (&v)[kVec]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f32_to_bf16_bits(v[2 * i]) | ((uint32_t)f32_to_bf16_bits(v[2 * i + 1]) << 16);
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Y: 0 = none, 1 = BF16, 2 = FP32.  NV: pieces of a row that a thread has, blockDim.x apart (a multiple of 32, so that blocks stay with sixteen lanes).
+template <typename TX, int Y, int NV>
+__global__ void __launch_bounds__(1024) add_norm_kernel(const NormArgs a) {
+    behind_grid();
+    __shared__ float parts[32];
+    const int64_t row = blockIdx.x;
+    const TX *const x = static_cast<const TX *>(a.x) + row * a.x_ld;
+    float s[NV][kVec];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
+        if (at < a.d) load8(x + at, s[j]);
+        else
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) s[j][i] = 0.f;
+    }
+    if constexpr (Y != 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
+            if (at >= a.d) continue;
+            float y[kVec];
+            if constexpr (Y == 1) load8(static_cast<const uint16_t *>(a.y) + row * a.y_ld + at, y);
+            else load8(static_cast<const float *>(a.y) + row * a.y_ld + at, y);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) s[j][i] = as_stored<TX>(s[j][i] + y[i]);
+            if (a.total != nullptr) store8(static_cast<TX *>(a.total) + row * a.total_ld + at, s[j]);
+        }
+    }
+    float r = 1.f;
+    if (a.normed) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) sum = fmaf(s[j][i], s[j][i], sum);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (blockDim.x > 32) {
+            if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = sum;
+            __syncthreads();
+            const int warps = (int)blockDim.x >> 5, lane = threadIdx.x & 31;
+            sum = lane < warps ? parts[lane] : 0.f;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        }
+        r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum, (float)a.d) + a.eps));
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
+        if (at < a.d) {
+            float w[kVec];
+            if (a.weight != nullptr) load8(a.weight + at, w);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                if (a.normed) s[j][i] *= r;
+                if (a.weight != nullptr) s[j][i] *= w[i];
+            }
+            if (a.out != nullptr) store8(a.out + row * a.out_ld + at, s[j]);
+        }
+        if (a.codes != nullptr) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) most = max(most, magnitude(s[j][i]));
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+            const float scale = f8_scale(most), inv = __fdiv_rn(1.f, scale);
+            if (at < a.d) {
+                uint2 c;
+                c.x = f8_quad(s[j][0] * inv, s[j][1] * inv, s[j][2] * inv, s[j][3] * inv);
+                c.y = f8_quad(s[j][4] * inv, s[j][5] * inv, s[j][6] * inv, s[j][7] * inv);
+                *reinterpret_cast<uint2 *>(a.codes + row * a.codes_ld + at) = c;
+                if (at % kF8Block == 0) a.scales[row * a.scales_ld + at / kF8Block] = scale;
+            }
+        }
+    }
+}
+
+template <typename TX, int Y>
+cudaError_t launch_norm(const NormArgs &a, int64_t T, cudaStream_t st) {
+    const int pieces = a.d / kVec;
+    // few rows: a piece a thread, the shortest way through a row
+    const int nv = pieces > 2048 ? 4 : pieces > 1024 ? 2 : 1;
+    const dim3 grid((unsigned)T), block((unsigned)(((pieces + nv - 1) / nv + 31) / 32 * 32));
+    if (nv == 4) return launch_behind(add_norm_kernel<TX, Y, 4>, grid, block, 0, st, 1, a);
+    if (nv == 2) return launch_behind(add_norm_kernel<TX, Y, 2>, grid, block, 0, st, 1, a);
+    return launch_behind(add_norm_kernel<TX, Y, 1>, grid, block, 0, st, 1, a);
+}
+
+// A CTA has a block of 128 x 128: a thread half a row of it, in registers between the largest magnitude and the codes.
+template <typename TW>
+__global__ void __launch_bounds__(256) quantize_f8_kernel(const TW *__restrict__ w, int64_t N, int64_t K, int64_t kb, uint8_t *__restrict__ q,
+                                                          float *__restrict__ scale, uint32_t *err) {
+    __shared__ uint32_t parts[8];
+    const int64_t rb = blockIdx.x / kb, cb = blockIdx.x % kb;
+    // sixteen neighbouring threads read a row's 128 columns, eight rows... a thread has the columns at 8 (t % 16) of the rows t / 16, t / 16 + 16, ...
+    const int64_t col = cb * kF8Block + (threadIdx.x & 15) * kVec, row0 = rb * kF8Block + (threadIdx.x >> 4);
+    float v[8][kVec];
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int64_t row = row0 + 16 * j;
+        if (row < N && col < K) load8(w + row * K + col, v[j]);
+        else
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) v[j][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            most = max(most, magnitude(v[j][i]));
+            if (magnitude(v[j][i]) >= 0x7f800000u) raise_error(err, (uint32_t)row, (uint32_t)(col + i));
+        }
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, parts[i]);
+    const float s = f8_scale(most), inv = __fdiv_rn(1.f, s);
+    if (threadIdx.x == 0) scale[blockIdx.x] = s;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int64_t row = row0 + 16 * j;
+        if (row >= N || col >= K) continue;
+        uint2 c;
+        c.x = f8_quad(v[j][0] * inv, v[j][1] * inv, v[j][2] * inv, v[j][3] * inv);
+        c.y = f8_quad(v[j][4] * inv, v[j][5] * inv, v[j][6] * inv, v[j][7] * inv);
+        *reinterpret_cast<uint2 *>(q + row * K + col) = c;
+    }
+}
+
+}  // namespace
+}  // namespace sxb
+
+using namespace sxb;
+
+extern "C" int sxb_add_norm(const SxbAddNormArgs *args, sxb_stream_t stream) {
+    const char *fn = "add_norm";
+    SXB_CHECK(args != nullptr, fn, ": null argument block");
+    const SxbAddNormArgs &g = *args;
+    const int64_t T = g.T, d = g.d;
+    SXB_CHECK(g.x != nullptr, fn, ": null pointer (x)");
+    SXB_CHECK(act_ok(g.act) && (g.y == nullptr || act_ok(g.y_act)), fn, ": unsupported dtypes ", g.act, " of x, ", g.y_act, " of y");
+    SXB_CHECK(T >= 1 && T <= (1 << 24), fn, ": T = ", T, " rows, expected 1..2^24");
+    SXB_CHECK(d >= 16 && d <= kMaxD && d % 16 == 0, fn, ": d = ", d, ", expected a multiple of 16 of 16..", kMaxD);
+    SXB_CHECK(g.total != nullptr || g.out != nullptr || g.codes != nullptr, fn, ": no output");
+    SXB_CHECK(g.total == nullptr || g.y != nullptr, fn, ": a total without y");
+    SXB_CHECK((g.codes == nullptr) == (g.scales == nullptr), fn, ": codes and scales come together (codes=", (const void *)g.codes, ", scales=", (const void *)g.scales, ")");
+    SXB_CHECK(g.normed || g.weight == nullptr, fn, ": a weight without the norm");
+    SXB_CHECK(!g.normed || (g.eps > 0.f && g.eps < 1e30f), fn, ": eps must be finite and positive");
+    SXB_CHECK(aligned16(g.weight), fn, ": the weight must be 16-byte aligned");
+    const int64_t es = act_bytes(g.act), ys = g.y != nullptr ? act_bytes(g.y_act) : 0, blocks = (d + kF8Block - 1) / kF8Block;
+    struct Rows {
+        const char *name;
+        const void *p;
+        int64_t ld, n, es;
+        int64_t bytes(int64_t T) const { return ((T - 1) * ld + n) * es; }
+    };
+    const Rows rows[6] = {{"x", g.x, g.x_ld, d, es},         {"y", g.y, g.y_ld, d, ys},         {"total", g.total, g.total_ld, d, es},
+                          {"out", g.out, g.out_ld, d, 2}, {"codes", g.codes, g.codes_ld, d, 1}, {"scales", g.scales, g.scales_ld, blocks, 4}};
+    for (const Rows &r : rows) {
+        if (r.p == nullptr) continue;
+        SXB_CHECK(r.ld >= r.n && r.ld <= (1ll << 32), fn, ": row stride ", r.ld, " of ", r.name, ", rows have ", r.n, " elements");
+        SXB_CHECK(r.n == blocks && r.es == 4 && r.p == (const void *)g.scales ? reinterpret_cast<uintptr_t>(r.p) % 4 == 0 : aligned16(r.p) && r.ld * r.es % 16 == 0, fn,
+                  ": rows of ", r.name, " must be 16-byte aligned (scales: 4)");
+    }
+    // an element of total is written by the thread that has read those of x and y: it may lie on either, row for row
+    for (int o = 2; o < 6; ++o)
+        for (int i = 0; i < o; ++i) {
+            const Rows &a = rows[o], &b = rows[i];
+            if (a.p == nullptr || b.p == nullptr || (o == 2 && i < 2 && a.p == b.p && a.ld == b.ld && a.es == b.es)) continue;
+            SXB_CHECK(apart(a.p, a.bytes(T), b.p, b.bytes(T)), fn, ": ", a.name, " [", a.p, "] overlaps ", b.name, " [", b.p, "]");
+        }
+    if (g.weight != nullptr)
+        for (int o = 2; o < 6; ++o)
+            SXB_CHECK(rows[o].p == nullptr || apart(rows[o].p, rows[o].bytes(T), g.weight, d * 4), fn, ": ", rows[o].name, " overlaps the weight");
+    NormArgs a{};
+    a.x = g.x, a.y = g.y, a.weight = g.weight, a.total = g.total, a.out = static_cast<uint16_t *>(g.out), a.codes = g.codes, a.scales = g.scales;
+    a.x_ld = g.x_ld, a.y_ld = g.y_ld, a.total_ld = g.total_ld, a.out_ld = g.out_ld, a.codes_ld = g.codes_ld, a.scales_ld = g.scales_ld;
+    a.d = (int)d, a.normed = g.normed != 0, a.eps = g.eps;
+    auto st = static_cast<cudaStream_t>(stream);
+    const int y = g.y == nullptr ? 0 : g.y_act == SXB_ACT_F32 ? 2 : 1;
+    cudaError_t e;
+    if (g.act == SXB_ACT_F32) e = y == 0 ? launch_norm<float, 0>(a, T, st) : y == 1 ? launch_norm<float, 1>(a, T, st) : launch_norm<float, 2>(a, T, st);
+    else e = y == 0 ? launch_norm<uint16_t, 0>(a, T, st) : y == 1 ? launch_norm<uint16_t, 1>(a, T, st) : launch_norm<uint16_t, 2>(a, T, st);
+    SXB_CUDA(e, fn, ": launching T=", T, " d=", d);
+    SXB_CHECK_LAUNCH(fn, " ", act_name(g.act), " T=", T, " d=", d);
+    return SXB_OK;
+}
+
+extern "C" int sxb_quantize_f8(const void *w, int act, int64_t N, int64_t K, uint8_t *q, float *scale, uint32_t *err, sxb_stream_t stream) {
+    const char *fn = "quantize_f8";
+    SXB_CHECK(w != nullptr && q != nullptr && scale != nullptr && err != nullptr, fn, ": null pointer (w=", w, ", q=", (const void *)q, ", scale=", (const void *)scale,
+              ", err=", (const void *)err, ")");
+    SXB_CHECK(act_ok(act), fn, ": unsupported dtype ", act, " of w");
+    SXB_CHECK(N >= 1 && N <= (1 << 24) && K >= 16 && K <= (1 << 20) && K % 16 == 0, fn, ": N = ", N, ", K = ", K, " (K a multiple of 16)");
+    SXB_CHECK(aligned16(w) && aligned16(q) && reinterpret_cast<uintptr_t>(scale) % 4 == 0, fn, ": w and q must be 16-byte aligned, scales 4-byte");
+    const int64_t kb = (K + kF8Block - 1) / kF8Block, blocks = (N + kF8Block - 1) / kF8Block * kb;
+    SXB_CHECK(blocks <= 0x7fffffff, fn, ": ", blocks, " blocks");
+    SXB_CHECK(apart(w, N * K * act_bytes(act), q, N * K), fn, ": q overlaps w");
+    auto st = static_cast<cudaStream_t>(stream);
+    if (act == SXB_ACT_F32) quantize_f8_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const float *>(w), N, K, kb, q, scale, err);
+    else quantize_f8_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const uint16_t *>(w), N, K, kb, q, scale, err);
+    SXB_CHECK_LAUNCH(fn, " N=", N, " K=", K);
+    return SXB_OK;
+}

@@ -1,0 +1,25 @@
+// Codes of 8-bit floating point (e4m3) with an FP32 scale for every block of 128 along a row: element = code * scale.  What the kernels that make
+// and read them share.
+#pragma once
+
+#include "common.cuh"
+
+namespace sxb {
+
+constexpr int kF8Block = 128;
+constexpr float kF8Top = 448.0f;        // the largest e4m3 number
+constexpr float kF8Least = 0x1p-64f;    // of a scale: its reciprocal, and its product with another scale, stay normal FP32 numbers
+
+// The scale of a block whose largest magnitude has the bits `most` (as integers, magnitudes compare as the numbers do, infinities and NaN above them all).
+__device__ inline float f8_scale(uint32_t most) { return most >= 0x7f800000u ? qnan_f32() : fmaxf(__fdiv_rn(__uint_as_float(most), kF8Top), kF8Least); }
+__device__ inline uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// Two values to two codes (the first in the lower byte): nearest, ties to even, beyond +-448 the last number, NaN stays NaN.
+__device__ inline uint32_t f8_pair(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ inline uint32_t f8_quad(float a, float b, float c, float d) { return f8_pair(a, b) | (f8_pair(c, d) << 16); }
+
+}  // namespace sxb

@@ -628,6 +628,137 @@ def report_attn_error(e, what: str):
     _check(_lib.load().sxb_report_attn_error((C.c_uint32 * 3)(*[int(v) for v in e]), what.encode()))
 
 
+# ---- around the head: norm into 8-bit codes, products of 8-bit floating point, verification of drafts ---------------------
+
+F8 = torch.float8_e4m3fn
+_F8_BLOCK = 128
+_NORM_ARGS = struct.Struct("@PPPPPPPqqqqqqqqfiii")
+_LINEAR_F8_ARGS = struct.Struct("@PPPPqqqqi")
+_VERIFY_ARGS = struct.Struct("@PPqqqqqPPPPPPPPPNPii")
+
+
+def _blocks(n: int) -> int:
+    return -(-n // _F8_BLOCK)
+
+
+def _refuse_all(dev, what, **tensors):
+    """A call's tensors are not what the kernels take them for: says which one."""
+    if dev != torch.cuda.current_device():
+        raise Error(1, f"{what}: the tensors live on device {dev}, the current device is {torch.cuda.current_device()}")
+    _on(torch.device("cuda", dev), what, **tensors)
+    raise Error(1, f"{what}: a vector is not contiguous, or the shapes do not fit: " + ", ".join(f"{n} {tuple(t.shape)}" for n, (t, _) in tensors.items() if t is not None))
+
+
+class F8View:
+    """A weight in 8-bit floating point (SxbF8View): codes q [N, K] float8_e4m3fn, contiguous, scale [ceil(N / 128), ceil(K / 128)] FP32."""
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor):
+        if q.dim() != 2 or q.dtype != F8 or not q.is_contiguous():
+            raise Error(1, f"F8View: q is {tuple(q.shape)} of {q.dtype}, expected contiguous [N, K] of {F8}")
+        self.N, self.K = q.shape
+        if scale.dtype != torch.float32 or tuple(scale.shape) != (_blocks(self.N), _blocks(self.K)) or not scale.is_contiguous() or scale.device != q.device:
+            raise Error(1, f"F8View: scale is {tuple(scale.shape)} of {scale.dtype} on {scale.device}, expected contiguous {(_blocks(self.N), _blocks(self.K))} FP32 on {q.device}")
+        if not q.is_cuda:
+            raise Error(1, "F8View: the weight must live on a CUDA device (no CPU path exists)")
+        self.q, self.scale, self.device, self.index = q, scale, q.device, q.get_device()
+        self._c = _lib.SxbF8View(q.data_ptr(), scale.data_ptr(), self.N, self.K)
+        self._at = C.addressof(self._c)
+
+    def bytes(self) -> int:
+        return self.q.numel() + 4 * self.scale.numel()
+
+
+def quantize_f8(w: torch.Tensor, err: Optional[torch.Tensor] = None, stream=None) -> F8View:
+    """sxb_quantize_f8 of a contiguous FP32 or BF16 [N, K] tensor: codes and a scale for each block of 128 x 128."""
+    if w.dtype not in _ROWS or w.dim() != 2 or not w.is_contiguous():
+        raise Error(1, "quantize_f8: w must be a contiguous FP32 or BF16 [N, K] tensor")
+    N, K = w.shape
+    q = torch.empty((N, K), dtype=torch.uint8, device=w.device).view(F8)
+    scale = torch.empty((_blocks(N), _blocks(K)), dtype=torch.float32, device=w.device)
+    own = err is None
+    if own:
+        err = torch.zeros(4, dtype=torch.int32, device=w.device)
+    _check(_lib.load().sxb_quantize_f8(_ptr(w), _w_act(w), N, K, _ptr(q), _ptr(scale), _ptr(err), _stream(stream)))
+    if own and int(err[0].item()) != 0:
+        raise Error(1, f"quantize_f8: non-finite weight at [{int(err[1])}, {int(err[2])}]")
+    return F8View(q, scale)
+
+
+def add_norm(x, y=None, weight=None, eps=1e-6, total=None, out=None, codes=None, scales=None, norm=True, stream=None):
+    """sxb_add_norm: s = x + y in x's type (x [T, d] BF16 or FP32, y BF16, FP32 or None) -> total (may be x or y), its norm times weight [d] FP32 (None: 1) -> out
+    BF16, codes float8_e4m3fn with scales [T, ceil(d / 128)] FP32; each of them or None.  norm=False: s itself in the place of its norm."""
+    T, d = x.shape
+    dev, dt = x.get_device(), x.dtype
+    ok = dev == torch._C._cuda_getDevice() and dt in _ROWS and (x.is_contiguous() or x.stride(1) == 1)
+    p = [0] * 5
+    ld = [0] * 5
+    for i, t, types, n in ((0, y, _ROWS, d), (1, total, (dt,), d), (2, out, _BF16, d), (3, codes, (F8,), d), (4, scales, _F32, _blocks(d))):
+        if t is not None:
+            ok = ok and t.dtype in types and t.get_device() == dev and t.shape == (T, n) and (t.is_contiguous() or t.stride(1) == 1 or n == 1)
+            p[i], ld[i] = t.data_ptr(), (_rows(t) if ok else n)
+    if weight is not None:
+        ok = ok and weight.dtype is torch.float32 and weight.get_device() == dev and weight.is_contiguous() and weight.numel() == d
+    if not ok:
+        _refuse_all(dev, "add_norm", x=(x, _ROWS), y=(y, _ROWS), weight=(weight, _F32), total=(total, (dt,)), out=(out, _BF16), codes=(codes, (F8,)), scales=(scales, _F32))
+    _check(_lib.load().sxb_add_norm(_NORM_ARGS.pack(
+        x.data_ptr(), p[0], 0 if weight is None else weight.data_ptr(), p[1], p[2], p[3], p[4], T, d, _rows(x), ld[0], ld[1], ld[2], ld[3], ld[4], eps,
+        dt is torch.bfloat16, y is not None and y.dtype is torch.bfloat16, bool(norm)), _stream(stream)))
+
+
+def linear_f8(x, x_scale, w: F8View, y, stream=None):
+    """sxb_linear_f8: y [M, N] BF16 or FP32 = x [M, K] float8_e4m3fn (scales x_scale [M, ceil(K / 128)] FP32) times w^T."""
+    M, K = x.shape
+    dev = w.index
+    if not (dev == torch._C._cuda_getDevice() and x.dtype is F8 and x_scale.dtype is torch.float32 and y.dtype in _ROWS and x.get_device() == dev and x_scale.get_device() == dev
+            and y.get_device() == dev and K == w.K and x_scale.shape == (M, _blocks(K)) and y.shape == (M, w.N) and (x.is_contiguous() or x.stride(1) == 1)
+            and (x_scale.is_contiguous() or x_scale.stride(1) == 1 or K <= _F8_BLOCK) and (y.is_contiguous() or y.stride(1) == 1 or w.N == 1)):
+        _refuse_all(dev, "linear_f8", x=(x, (F8,)), x_scale=(x_scale, _F32), w=(w.q, (F8,)), y=(y, _ROWS))
+    _check(_lib.load().sxb_linear_f8(_LINEAR_F8_ARGS.pack(
+        x.data_ptr(), x_scale.data_ptr(), w._at, y.data_ptr(), M, _rows(x), _rows(x_scale), _rows(y), y.dtype is torch.bfloat16), _stream(stream)))
+
+
+def verify_drafts_workspace_bytes(T: int, B: int, V: int) -> int:
+    """Bytes of workspace that verify_drafts needs for T rows of B sequences over V tokens."""
+    n = _lib.load().sxb_verify_drafts_workspace_bytes(T, B, V)
+    if n == 0:
+        _check(1)
+    return n
+
+
+def verify_drafts(logits, ids, q_start, u, u_pick, next_ids, n_new, ws, err, draft_logits=None, temperature=None, logp=None, stream=None):
+    """sxb_verify_drafts: rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]) are sequence b's: the tokens ids [T] int32 fed there, the drafted ones behind the first, the target's
+    logits [T, V] BF16 or FP32, the drafter's (or None: its tokens are all that is known of it), random numbers u [T] and u_pick [B] FP32, temperature [B] FP32 (None: 1; 0: greedy)
+    -> next_ids [T] int32 (-1 behind the last), n_new [B] int32, logp [T] FP32 or None.  err: 3 or more zeroed int32."""
+    T, V = logits.shape
+    dev, B = logits.get_device(), n_new.shape[0]
+    ok = dev == torch._C._cuda_getDevice() and logits.dtype in _ROWS and (logits.is_contiguous() or logits.stride(1) == 1 or V == 1)
+    for t, dt, n in ((ids, torch.int32, T), (q_start, torch.int32, B + 1), (u, torch.float32, T), (u_pick, torch.float32, B), (next_ids, torch.int32, T), (n_new, torch.int32, B),
+                     (temperature, torch.float32, B), (logp, torch.float32, T)):
+        ok = ok and (t is None or (t.dtype is dt and t.get_device() == dev and t.is_contiguous() and t.numel() == n))
+    ok = ok and ws.get_device() == dev and ws.is_contiguous() and err.get_device() == dev and err.dtype in _WORDS and err.is_contiguous() and err.numel() >= 3
+    dp = dld = 0
+    if draft_logits is not None:
+        d = draft_logits
+        ok = ok and d.dtype in _ROWS and d.get_device() == dev and d.shape == (T, V) and (d.is_contiguous() or d.stride(1) == 1 or V == 1)
+        dp, dld = d.data_ptr(), (_rows(d) if ok else V)
+    if not ok:
+        _refuse_all(dev, "verify_drafts", logits=(logits, _ROWS), draft_logits=(draft_logits, _ROWS), ids=(ids, _I32), q_start=(q_start, _I32), u=(u, _F32), u_pick=(u_pick, _F32),
+                    temperature=(temperature, _F32), next_ids=(next_ids, _I32), n_new=(n_new, _I32), logp=(logp, _F32), ws=(ws, (ws.dtype,)), err=(err, _WORDS))
+    _count()  # two launches
+    _check(_lib.load().sxb_verify_drafts(_VERIFY_ARGS.pack(
+        logits.data_ptr(), dp, _rows(logits), dld, T, V, B, ids.data_ptr(), q_start.data_ptr(), u.data_ptr(), u_pick.data_ptr(),
+        0 if temperature is None else temperature.data_ptr(), next_ids.data_ptr(), n_new.data_ptr(), 0 if logp is None else logp.data_ptr(), ws.data_ptr(),
+        ws.numel() * ws.element_size(), err.data_ptr(), logits.dtype is torch.bfloat16, draft_logits is not None and draft_logits.dtype is torch.bfloat16), _stream(stream)))
+
+
+def check_verify_error(err, what: str):
+    _check(_lib.load().sxb_check_verify_error(_ptr(err), what.encode()))
+
+
+def report_verify_error(e, what: str):
+    _check(_lib.load().sxb_report_verify_error((C.c_uint32 * 3)(*[int(v) for v in e]), what.encode()))
+
+
 # ---- the whole block as one call ------------------------------------------------------------------------------
 
 def _layer_args(x, logits, y, gate_up, down, E, A, ids, coef, ws, ws_bytes, h, partial, router_err, expert_err, xs, math, E_total,
