@@ -2,20 +2,10 @@
 //   y[m, n] = sum over blocks b of k:  (xs[m, b] ws[n / 128, b]) * sum over k in b:  x[m, k] w[n, k]
 // The inner sums are exact products of codes added up in FP32 by the tensor cores, from zero for every block; the threads scale them and add them up in FP32.
 
-#include "f8.cuh"
-
-#include <cuda_bf16.h>
+#include "linear_f8.cuh"
 
 namespace sxb {
 namespace {
-
-struct F8Args {
-    const uint8_t *x, *w;
-    const float *xs, *ws;
-    void *y;
-    int64_t x_ld, xs_ld, y_ld, K;
-    int M, N, kb;  // kb: blocks of 128 along k
-};
 
 // ---- few rows: the weights stream through the registers -------------------------------------------------------------------------
 
@@ -34,7 +24,7 @@ __device__ inline uint4 load16(const uint8_t *p, bool there) { return there ? __
 // k inside a block is permuted alike on both operands: lane (g = lane / 4, c = lane % 4) holds the sixteen codes at 16 c and at 64 + 16 c of its weight rows g and
 // g + 8 and of its token g, four MMAs' worth.
 template <int NT>
-__global__ void __launch_bounds__(32 * kWarps) f8_rows_kernel(const F8Args a, int out_f32) {
+__global__ void __launch_bounds__(32 * kWarps) f8_rows_kernel(const F8Args a) {
     behind_grid();
     __shared__ float parts[kWarps][kRows][NT * kTokens + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -79,7 +69,7 @@ __global__ void __launch_bounds__(32 * kWarps) f8_rows_kernel(const F8Args a, in
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += parts[w][row][m];
         const int64_t at = (int64_t)(m0 + m) * a.y_ld + n0 + row;
-        if (out_f32) static_cast<float *>(a.y)[at] = sum;
+        if (a.f32) static_cast<float *>(a.y)[at] = sum;
         else static_cast<uint16_t *>(a.y)[at] = f32_to_bf16_bits(sum);
     }
 }
@@ -112,18 +102,13 @@ extern "C" int sxb_linear_f8(const SxbLinearF8Args *args, sxb_stream_t stream) {
               fn, ": y [", g.y, ", +", yb, " B) overlaps x, the weight or their scales");
     F8Args a{};
     a.x = g.x, a.w = g.w->q, a.xs = g.x_scale, a.ws = g.w->scale, a.y = g.y, a.x_ld = g.x_ld, a.xs_ld = g.xs_ld, a.y_ld = g.y_ld, a.K = K;
-    a.M = (int)M, a.N = (int)N, a.kb = (int)kb;
+    a.M = (int)M, a.N = (int)N, a.kb = (int)kb, a.f32 = g.out_act == SXB_ACT_F32;
     auto st = static_cast<cudaStream_t>(stream);
-    const int f32 = g.out_act == SXB_ACT_F32;
-    const unsigned tiles = (unsigned)((N + kRows - 1) / kRows);
-    cudaError_t e = cudaSuccess;
-    for (int64_t m0 = 0; m0 < M && e == cudaSuccess; m0 += 32768 * 32) {  // a grid's second dimension
-        F8Args p = a;
-        p.M = (int)std::min<int64_t>(M - m0, 32768 * 32), p.x += m0 * a.x_ld, p.xs += m0 * a.xs_ld, p.y = static_cast<uint8_t *>(a.y) + m0 * a.y_ld * os;
-        if (M <= 8) e = launch_behind(f8_rows_kernel<1>, dim3(tiles, (unsigned)((p.M + 7) / 8)), dim3(32 * kWarps), 0, st, 1, p, f32);
-        else if (M <= 16) e = launch_behind(f8_rows_kernel<2>, dim3(tiles, (unsigned)((p.M + 15) / 16)), dim3(32 * kWarps), 0, st, 1, p, f32);
-        else e = launch_behind(f8_rows_kernel<4>, dim3(tiles, (unsigned)((p.M + 31) / 32)), dim3(32 * kWarps), 0, st, 1, p, f32);
-    }
+    if (M > 32) return linear_f8_tc(fn, a, st);
+    const dim3 grid((unsigned)((N + kRows - 1) / kRows)), block(32 * kWarps);
+    const cudaError_t e = M <= 8    ? launch_behind(f8_rows_kernel<1>, grid, block, 0, st, 1, a)
+                          : M <= 16 ? launch_behind(f8_rows_kernel<2>, grid, block, 0, st, 1, a)
+                                    : launch_behind(f8_rows_kernel<4>, grid, block, 0, st, 1, a);
     SXB_CUDA(e, fn, ": launching M=", M, " N=", N, " K=", K);
     SXB_CHECK_LAUNCH(fn, " M=", M, " N=", N, " K=", K);
     return SXB_OK;

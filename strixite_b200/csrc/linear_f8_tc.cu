@@ -1,0 +1,446 @@
+// The 8-bit floating-point product for many rows: y[m, n] = sum over blocks b of 128 k: xs[m, b] ws[n / 128, b] * (x w^T of the block), tcgen05.
+//
+// The tensor cores cannot apply FP32 scales, so a block's product is an accumulator of its own: four MMAs (32 k each) start it from zero, and eight warps read it back from
+// tensor memory, scale it and add it to sums that they hold in registers, while the MMAs of the next block fill the other of two accumulators.  A thread has one row of x (a
+// lane of tensor memory) and half the tile's columns, all of one block of weight rows, so its scale is one number a block: one read and half a packed multiply-add a column.
+//
+// Warp 8 brings x and w in stages of 128 k by tensor copies, warp 9 issues the MMAs.  Two forms:
+//   pairs    a cluster of two CTAs has a tile of 256 x 256 (MMAs of cta_group::2: each CTA holds 128 rows of x and half the weight rows, so a stage's bytes feed twice the work);
+//            pairs are persistent, the MMAs run on into the next tile while the sums of the last are stored.
+//   tiles    a CTA has a tile of 128 x 128; where tiles are few, a cluster of up to eight CTAs shares its k, and adds the parts up through distributed shared memory in rank order.
+
+#include "linear_f8.cuh"
+#include "tc_ptx.cuh"
+
+#include <cooperative_groups.h>
+
+namespace sxb {
+namespace {
+
+constexpr int kSumWarps = 8, kCopyWarp = kSumWarps, kMmaWarp = kSumWarps + 1;
+constexpr int kTileM = 128;                  // rows of x of a CTA: the lanes of tensor memory
+constexpr int kLine = kF8Block;              // bytes of a stage's row: a block of k
+constexpr int kMaxStages = 6;
+
+template <int CTAS, int BN>
+struct Shape {
+    static constexpr int kBRows = BN / CTAS;                                   // weight rows that a CTA holds
+    static constexpr int kStageBytes = (kTileM + kBRows) * kLine;
+    static constexpr int kStages = CTAS == 2 ? kMaxStages : 3;                 // tiles: two CTAs an SM
+    static constexpr int kTmemCols = 2 * BN;
+    // Pairs: a third warpgroup, most of whose registers go to the two that sum (40 and 232 a thread are what 384 threads were launched with, 168 each).
+    static constexpr int kThreads = CTAS == 2 ? 384 : 32 * (kSumWarps + 2);
+    static constexpr int kAtOnce = CTAS == 2 ? 32 : 16;                        // columns of an accumulator that a thread reads at once
+    static constexpr int kPitch = BN + 4;                                      // floats of a row of a part
+    static constexpr size_t kRing = (size_t)kStages * kStageBytes, kPart = CTAS == 1 ? (size_t)kTileM * kPitch * 4 : 0;
+    static constexpr size_t kSmem = (kRing > kPart ? kRing : kPart) + 1024;
+};
+
+struct TcArgs8 {
+    F8Args g;
+    int n_m, n_n, band;  // tiles along m and n; tiles along m of a band, in which all of n is gone through
+    int split;           // CTAs that share a tile's k (tiles)
+    int vec;             // bytes of y that may be stored at once
+    uint32_t *status;
+    unsigned long long wait_limit_ns;
+    int test_skip_slot;
+};
+
+// Instruction descriptor of kind::f8f6f4: D FP32 (bits [4,6) = 1), A and B e4m3 (formats 0), both K-major, N >> 3 at bits [17,23), M >> 4 at bits [24,29).
+__device__ inline uint32_t instr_desc_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+// D[tmem] = A[smem] * B[smem] over a stage, both 128-byte-swizzled: four MMAs of 32 k, issued by the lane with leader = 1 of a whole warp.
+template <int CTAS>
+__device__ inline void tc_block_e4m3(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc) {
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "{\n\t.reg .pred q, zero, one;\n\t.reg .b32 x1, x2, x3, y1, y2, y3;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t"
+            "setp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 zero, 0, 0;\n\tsetp.eq.b32 one, 0, 0;\n\t"
+            "add.u32 x1, %1, 2;\n\tadd.u32 x2, %1, 4;\n\tadd.u32 x3, %1, 6;\n\tadd.u32 y1, %2, 2;\n\tadd.u32 y2, %2, 4;\n\tadd.u32 y3, %2, 6;\n\t"
+            "mov.b64 a0, {%1, %3};\n\tmov.b64 a1, {x1, %3};\n\tmov.b64 a2, {x2, %3};\n\tmov.b64 a3, {x3, %3};\n\t"
+            "mov.b64 b0, {%2, %3};\n\tmov.b64 b1, {y1, %3};\n\tmov.b64 b2, {y2, %3};\n\tmov.b64 b3, {y3, %3};\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a0, b0, %4, zero;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %4, one;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %4, one;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %4, one;\n\t}" ::"r"(d),
+            "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(leader)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred q, zero, one;\n\t.reg .b32 x1, x2, x3, y1, y2, y3;\n\t.reg .b64 a0, a1, a2, a3, b0, b1, b2, b3;\n\t"
+            "setp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 zero, 0, 0;\n\tsetp.eq.b32 one, 0, 0;\n\t"
+            "add.u32 x1, %1, 2;\n\tadd.u32 x2, %1, 4;\n\tadd.u32 x3, %1, 6;\n\tadd.u32 y1, %2, 2;\n\tadd.u32 y2, %2, 4;\n\tadd.u32 y3, %2, 6;\n\t"
+            "mov.b64 a0, {%1, %3};\n\tmov.b64 a1, {x1, %3};\n\tmov.b64 a2, {x2, %3};\n\tmov.b64 a3, {x3, %3};\n\t"
+            "mov.b64 b0, {%2, %3};\n\tmov.b64 b1, {y1, %3};\n\tmov.b64 b2, {y2, %3};\n\tmov.b64 b3, {y3, %3};\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a0, b0, %4, zero;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a1, b1, %4, one;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a2, b2, %4, one;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a3, b3, %4, one;\n\t}" ::"r"(d),
+            "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(leader)
+            : "memory");
+}
+// What was issued before has completed: an arrival at the barrier, in both CTAs of a pair.
+template <int CTAS>
+__device__ inline void commit_to(uint32_t leader, uint64_t *bar) {
+    if constexpr (CTAS == 1) tc_commit_if(leader, bar);
+    else
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(smem_u32(bar)),
+            "r"(leader), "h"((uint16_t)3)
+            : "memory");
+}
+// A box of x or w into this CTA's shared memory, counted at the barrier `bar` (an address in the cluster's window: the first CTA's of a pair).
+template <int CTAS>
+__device__ inline void load_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    if constexpr (CTAS == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+}
+__device__ inline uint32_t in_first_cta(uint64_t *bar) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+    return r;
+}
+__device__ inline void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ inline void cluster_meet() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+
+// 16 or 32 consecutive columns of this thread's TMEM lane.
+__device__ inline void tc_ld(uint32_t taddr, float (&v)[16]) { tc_ld16(taddr, v); }
+__device__ inline void tc_ld(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ inline uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ inline uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ inline void store32(void *p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+// n values (a multiple of 32 bytes' worth) to y at `at`, `left` of which lie inside the row.
+template <int NV>
+__device__ inline void store_run(const TcArgs8 &a, int64_t at, int left, const float (&v)[NV]) {
+    if (a.g.f32) {
+        float *p = static_cast<float *>(a.g.y) + at;
+#pragma unroll
+        for (int i = 0; i < NV; i += 8) {
+            uint32_t w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(v[i + k]);
+            if (i + 8 <= left && a.vec >= 32) store32(p + i, w);
+            else if (i + 8 <= left && a.vec >= 16) {
+                reinterpret_cast<uint4 *>(p + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                reinterpret_cast<uint4 *>(p + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            } else
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (i + k < left) p[i + k] = v[i + k];
+        }
+    } else {
+        uint16_t *p = static_cast<uint16_t *>(a.g.y) + at;
+#pragma unroll
+        for (int i = 0; i < NV; i += 16) {
+            uint32_t w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = (uint32_t)f32_to_bf16_bits(v[i + 2 * k]) | ((uint32_t)f32_to_bf16_bits(v[i + 2 * k + 1]) << 16);
+            if (i + 16 <= left && a.vec >= 32) store32(p + i, w);
+            else if (i + 16 <= left && a.vec >= 16) {
+                reinterpret_cast<uint4 *>(p + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                reinterpret_cast<uint4 *>(p + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            } else
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (i + k < left) p[i + k] = f32_to_bf16_bits(v[i + k]);
+        }
+    }
+}
+
+// A place in a ring of n barriers and the parity of the phase it is in.
+struct Turn {
+    int at;
+    uint32_t phase;
+    __device__ inline void advance(int n) {
+        if (++at == n) at = 0, phase ^= 1u;
+    }
+};
+
+struct Tile {
+    int m, n;
+};
+__device__ inline Tile tile_of(const TcArgs8 &a, int64_t item) {
+    const int64_t per = (int64_t)a.band * a.n_n, b = item / per, rest = item % per;
+    const int in_band = min(a.band, a.n_m - (int)b * a.band);
+    return Tile{(int)b * a.band + (int)(rest % in_band), (int)(rest / in_band)};
+}
+
+template <int CTAS, int BN>
+__global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, CTAS == 2 ? 1 : 2)
+    f8_tc_kernel(const TcArgs8 a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+    using S = Shape<CTAS, BN>;
+    constexpr int kCols = BN / 2;  // of a summing thread
+    behind_grid();
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *const smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full_bar[S::kStages], empty_bar[S::kStages], acc_full[2], acc_empty[2], drain_bar;
+    __shared__ uint32_t tmem_base_smem;
+    __shared__ int abort_flag;
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int group = CTAS == 2 ? 2 : a.split, rank = (int)blockIdx.x % group;  // of the cluster
+    const int64_t n_items = (int64_t)a.n_m * a.n_n, first = blockIdx.x / group, step = gridDim.x / group;
+    const int kb0 = CTAS == 2 ? 0 : (int)((int64_t)a.g.kb * rank / group), kb1 = CTAS == 2 ? a.g.kb : (int)((int64_t)a.g.kb * (rank + 1) / group);
+    volatile int *const abort_v = &abort_flag;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
+        for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1), mbar_init(&acc_empty[b], kSumWarps * CTAS);
+        mbar_init(&drain_bar, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        if constexpr (CTAS == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(S::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(S::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CTAS == 2) cluster_meet();  // the other CTA's barriers are there
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_smem;
+
+    auto raise_abort = [&](int64_t item, int role) {
+        if (atomicExch(&abort_flag, 1) == 0 && atomicCAS(&a.status[0], 0u, 2u) == 0u) {
+            a.status[1] = (uint32_t)item;
+            a.status[2] = (uint32_t)role;
+        }
+    };
+
+    // What every warp does last.  (Called in both branches: the warps of a pair have different numbers of registers by then.)
+    auto leave = [&] {
+        if (*abort_v) {  // copies that a CTA issued before it gave up have landed within this time
+            const unsigned long long t0 = global_ns();
+            while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
+        }
+        tc_fence_before();
+        __syncthreads();
+        if (CTAS == 1 && a.split > 1) {
+            namespace cg = cooperative_groups;
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster_meet();
+            const Tile t = tile_of(a, first);
+            const int row0 = t.m * kTileM, col0 = t.n * BN;
+            // four neighbouring columns a thread, in turn the cluster's CTAs'
+            if (!*abort_v)
+                for (int i = rank * S::kThreads + (int)threadIdx.x; i < kTileM * BN / 4; i += group * S::kThreads) {
+                    const int r = i / (BN / 4), c = i % (BN / 4) * 4;
+                    if (row0 + r >= a.g.M || col0 + c >= a.g.N) continue;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int k = 0; k < group; ++k) {
+                        const float4 p = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(reinterpret_cast<float *>(smem), k) + r * S::kPitch + c);
+                        v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
+                    }
+                    const int64_t at = (int64_t)(row0 + r) * a.g.y_ld + col0 + c;
+                    const int left = a.g.N - col0 - c;
+                    if (a.g.f32) {
+                        float *p = static_cast<float *>(a.g.y) + at;
+                        if (left >= 4 && a.vec >= 16) *reinterpret_cast<float4 *>(p) = v;
+                        else {
+                            p[0] = v.x;
+                            if (left > 1) p[1] = v.y;
+                            if (left > 2) p[2] = v.z;
+                            if (left > 3) p[3] = v.w;
+                        }
+                    } else {
+                        uint16_t *p = static_cast<uint16_t *>(a.g.y) + at;
+                        const uint16_t w[4] = {f32_to_bf16_bits(v.x), f32_to_bf16_bits(v.y), f32_to_bf16_bits(v.z), f32_to_bf16_bits(v.w)};
+                        if (left >= 4 && a.vec >= 8) *reinterpret_cast<uint2 *>(p) = make_uint2((uint32_t)w[0] | ((uint32_t)w[1] << 16), (uint32_t)w[2] | ((uint32_t)w[3] << 16));
+                        else
+                            for (int k = 0; k < 4; ++k)
+                                if (k < left) p[k] = w[k];
+                    }
+                }
+            cluster_meet();  // nobody's part is read from here on
+        }
+        if constexpr (CTAS == 2) cluster_meet();
+        if (warp == kMmaWarp) {
+            tc_fence_after();
+            if constexpr (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+            else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+        }
+    };
+
+    if (warp >= kSumWarps) {
+        if constexpr (CTAS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == kCopyWarp) {
+            // ===================== copies: one thread, as far ahead as free stages allow =====================
+            if (lane == 0) {
+                Turn turn{0, 1u};  // the phase before the first leaves every stage free
+                int issued = 0;
+                for (int64_t item = first; item < n_items && !*abort_v; item += step) {
+                    const Tile t = tile_of(a, item);
+                    const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM, wrow = t.n * BN + (CTAS == 2 ? rank * S::kBRows : 0);
+                    for (int kb = kb0; kb < kb1; ++kb, ++issued, turn.advance(S::kStages)) {
+                        if (!mbar_wait(&empty_bar[turn.at], turn.phase, abort_v, a.wait_limit_ns)) {
+                            raise_abort(item, 5);
+                            break;
+                        }
+                        if (blockIdx.x == 0 && issued == a.test_skip_slot) continue;
+                        const uint32_t dst = smem_u32(smem) + (uint32_t)(turn.at * S::kStageBytes), bar = CTAS == 2 ? in_first_cta(&full_bar[turn.at]) : smem_u32(&full_bar[turn.at]);
+                        if (CTAS == 1 || rank == 0) mbar_expect_tx(&full_bar[turn.at], (uint32_t)(CTAS * S::kStageBytes));
+                        load_box<CTAS>(dst, &xmap, kb * kLine, row, bar);
+                        load_box<CTAS>(dst + kTileM * kLine, &wmap, kb * kLine, wrow, bar);
+                    }
+                }
+            }
+            __syncwarp();
+        } else if (warp == kMmaWarp) {
+            // ===================== MMA issue: the pair's first CTA for both =====================
+            if (CTAS == 1 || rank == 0) {
+                const uint32_t leader = elect_one() ? 1u : 0u, idesc = instr_desc_e4m3(kTileM * CTAS, BN);
+                const uint64_t desc0 = smem_desc(smem_u32(smem));
+                const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0;
+                Turn turn{0, 0u}, acc{0, 1u};
+                bool ok = true;
+                for (int64_t item = first; item < n_items && ok; item += step)
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc.at], acc.phase, abort_v, a.wait_limit_ns));
+                        if (!ok) {
+                            if (leader) raise_abort(item, 2);
+                            break;
+                        }
+                        ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[turn.at], turn.phase, abort_v, a.wait_limit_ns));
+                        if (!ok) {
+                            if (leader) raise_abort(item, 3);
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t lo = lo0 + (uint32_t)(turn.at * (S::kStageBytes / 16));
+                        tc_block_e4m3<CTAS>(leader, tmem_base + (uint32_t)(acc.at * BN), lo, lo + kTileM * kLine / 16, hi, idesc);
+                        commit_to<CTAS>(leader, &empty_bar[turn.at]);  // the stage is free once these MMAs have read it
+                        commit_to<CTAS>(leader, &acc_full[acc.at]);
+                        turn.advance(S::kStages), acc.advance(2);
+                    }
+                // every MMA has completed before shared and tensor memory are given up (not skipped while aborting)
+                commit_to<CTAS>(leader, &drain_bar);
+            }
+            mbar_wait(&drain_bar, 0u, nullptr, a.wait_limit_ns);
+            __syncwarp();
+        }
+        leave();
+    } else {
+        if constexpr (CTAS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        // ===================== sums and stores =====================
+        const int quad = warp & 3, half = warp >> 2;  // the TMEM lanes a warp may read: 32 (warp % 4) ..; its half of the columns
+        const uint32_t lanes = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * kCols);
+        const uint32_t empty_at[2] = {CTAS == 2 ? in_first_cta(&acc_empty[0]) : smem_u32(&acc_empty[0]), CTAS == 2 ? in_first_cta(&acc_empty[1]) : smem_u32(&acc_empty[1])};
+        Turn acc{0, 0u};
+        for (int64_t item = first; item < n_items && !*abort_v; item += step) {
+            const Tile t = tile_of(a, item);
+            const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM + quad * 32 + lane, col = t.n * BN + half * kCols;
+            const bool there = row < a.g.M;
+            const float *const xs = a.g.xs + (int64_t)row * a.g.xs_ld, *const ws = a.g.ws + (int64_t)(min(col, a.g.N - 1) / kF8Block) * a.g.kb;
+            uint64_t sum[kCols / 2];
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) sum[i] = 0;
+            float next = there && kb0 < kb1 ? xs[kb0] * ws[kb0] : 0.f;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const float s = next;
+                if (kb + 1 < kb1 && there) next = xs[kb + 1] * ws[kb + 1];
+                if (lane == 0 && !mbar_wait(&acc_full[acc.at], acc.phase, abort_v, a.wait_limit_ns)) raise_abort(item, 4);
+                __syncwarp();
+                if (*abort_v) break;
+                tc_fence_after();
+                const uint64_t s2 = pack2(s, s);
+#pragma unroll
+                for (int c = 0; c < kCols; c += S::kAtOnce) {
+                    float v[S::kAtOnce];
+                    tc_ld(lanes + (uint32_t)(acc.at * BN + c), v);
+                    if (c + S::kAtOnce == kCols) {  // the last columns are in registers: the accumulator may be overwritten
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive_at(empty_at[acc.at]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < S::kAtOnce / 2; ++i) sum[c / 2 + i] = fma2(pack2(v[2 * i], v[2 * i + 1]), s2, sum[c / 2 + i]);
+                }
+                acc.advance(2);
+            }
+            if (*abort_v) break;
+            if (CTAS == 1 && a.split > 1) {
+                // this CTA's part to shared memory: the ring is not needed any more (its one item's MMAs have completed)
+                float *const part = reinterpret_cast<float *>(smem) + (quad * 32 + lane) * S::kPitch + half * kCols;
+#pragma unroll
+                for (int i = 0; i < kCols / 2; i += 2) *reinterpret_cast<ulonglong2 *>(part + 2 * i) = make_ulonglong2(sum[i], sum[i + 1]);
+            } else if (there) {
+#pragma unroll
+                for (int c = 0; c < kCols; c += 32) {
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[2 * i] = __uint_as_float((uint32_t)sum[c / 2 + i]), v[2 * i + 1] = __uint_as_float((uint32_t)(sum[c / 2 + i] >> 32));
+                    store_run(a, (int64_t)row * a.g.y_ld + col + c, a.g.N - col - c, v);
+                }
+            }
+        }
+        leave();
+    }
+}
+
+template <int CTAS, int BN>
+int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
+    using S = Shape<CTAS, BN>;
+    CUtensorMap xmap, wmap;
+    if (int rc = tensor_map_2d(fn, a.g.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.M, (uint64_t)a.g.x_ld, kLine, kTileM, CU_TENSOR_MAP_SWIZZLE_128B, &xmap))
+        return rc;
+    if (int rc = tensor_map_2d(fn, a.g.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.N, (uint64_t)a.g.K, kLine, S::kBRows, CU_TENSOR_MAP_SWIZZLE_128B, &wmap))
+        return rc;
+    a.n_m = (a.g.M + kTileM * CTAS - 1) / (kTileM * CTAS), a.n_n = (a.g.N + BN - 1) / BN;
+    a.band = std::min(a.n_m, 16);
+    const int64_t items = (int64_t)a.n_m * a.n_n;
+    const int cluster = CTAS == 2 ? 2 : a.split;
+    SXB_CUDA(cudaFuncSetAttribute(f8_tc_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), fn, ": reserving shared memory");
+    const int64_t places = CTAS == 2 ? sm_count() / 2 : a.split > 1 ? items : 2 * (int64_t)sm_count();
+    const cudaError_t e = launch_behind(f8_tc_kernel<CTAS, BN>, dim3((unsigned)(std::min(items, places) * cluster)), dim3(S::kThreads), S::kSmem, st, cluster, a, xmap, wmap);
+    SXB_CUDA(e, fn, ": launching M=", a.g.M, " N=", a.g.N, " K=", a.g.K);
+    return SXB_OK;
+}
+
+}  // namespace
+
+int linear_f8_tc(const char *fn, const F8Args &g, cudaStream_t st) {
+    TcArgs8 a{};
+    a.g = g;
+    const int64_t es = g.f32 ? 4 : 2;
+    for (a.vec = 32; a.vec > 4 && (reinterpret_cast<uintptr_t>(g.y) % a.vec != 0 || g.y_ld * es % a.vec != 0); a.vec /= 2) {}
+    a.wait_limit_ns = wait_limit_ns(), a.test_skip_slot = test_skip_slot();
+    if (int rc = library_status_words(fn, &a.status)) return rc;
+    const int64_t sms = sm_count(), pairs = (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256), tiles = (int64_t)((g.M + 127) / 128) * ((g.N + 127) / 128);
+    if (g.M > 128 && pairs * 2 >= sms) return launch_tc8<2, 256>(fn, a, st);
+    a.split = (int)std::max<int64_t>(1, std::min<int64_t>({8, 2 * sms / tiles, g.kb / 2}));
+    return launch_tc8<1, 128>(fn, a, st);
+}
+
+}  // namespace sxb

@@ -174,7 +174,7 @@ def test_linear_strides(K, cuda, M, f32, wide):
     check_linear(K, cuda, M, 333, 656, f32, seed=M, wide=wide)
 
 
-@pytest.mark.parametrize("M,N,K_", [(3, 20000, 256), (64, 4096, 16384), (5, 64, 131072), (130, 64, 65536), (2000, 2000, 128), (777, 1000, 1040), (150, 2560, 4096), (4000, 520, 272),
+@pytest.mark.parametrize("M,N,K_", [(3, 20000, 256), (64, 4096, 16384), (5, 64, 131072), (130, 64, 65536), (2000, 2000, 128), (777, 1000, 1040), (150, 2560, 4096), (4000, 520, 272), (1100, 5000, 656), (2049, 4097, 400),
                                     (1024, 4096, 1024), (8200, 130, 144)])
 def test_linear_long(K, cuda, M, N, K_):
     check_linear(K, cuda, M, N, K_, True, seed=M)
@@ -220,6 +220,29 @@ def test_linear_repeats_bit_for_bit(K, cuda, M):
         y = torch.zeros_like(first)
         K.linear_f8(x, xs, v, y)
         assert torch.equal(y, first)
+
+
+@pytest.mark.parametrize("M,N,K_,slot", [(2048, 4096, 1024, 0), (2048, 4096, 1024, 7), (2048, 4096, 1024, 10), (100, 300, 2048, 0), (100, 300, 2048, 1), (300, 40000, 1024, 2), (300, 40000, 1024, 9)])
+def test_linear_gives_up_a_wait(K, cuda, lib, M, N, K_, slot):
+    """The product with CTA 0 told to leave a stage out, in a pair's first and second tile, in a tile that a cluster shares and in one of its own.  The kernel returns, the status names
+    the role, the next call has the bits of the call before."""
+    x, xs, w, ws = operands(K, cuda, M, N, K_, slot)
+    v, out = K.F8View(w, ws), [torch.full((M, N), float("nan"), device=cuda) for _ in range(3)]
+    K.linear_f8(x, xs, v, out[0])
+    K.check_dense_status("warm-up")
+    try:
+        K.set_wait_limit(2_000_000)
+        assert lib.sxb_test_skip_ring_slot(slot) == 0
+        K.linear_f8(x, xs, v, out[1])
+        torch.cuda.synchronize()
+    finally:
+        lib.sxb_test_skip_ring_slot(-1)
+        K.set_wait_limit(2_000_000_000)
+    with pytest.raises(K.Error, match=r"skipped fill: a tcgen05 kernel gave up a wait at work item \d+ \((an MMA warp|the epilogue|the activation copy)"):
+        K.check_dense_status("skipped fill")
+    K.linear_f8(x, xs, v, out[2])
+    K.check_dense_status("after")
+    assert torch.equal(out[2], out[0]) and not bool(torch.isnan(out[2]).any())
 
 
 # ---- verification ----------------------------------------------------------------------------------------------------------------------
