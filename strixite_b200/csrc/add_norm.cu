@@ -40,8 +40,19 @@ __device__ inline void store8(float *p, const float (&v)[kVec]) {
 __device__ inline void store8(uint16_t *p, const float (&v)[kVec]) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)f32_to_bf16_bits(v[2 * i]) | ((uint32_t)f32_to_bf16_bits(v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The values as they are stored in TX.
+template <typename TX>
+__device__ inline void as_kept(float (&v)[kVec]) {
+    if constexpr (sizeof(TX) == 2)
+#pragma unroll
+        for (int i = 0; i < kVec; i += 2) {
+            const uint32_t w = bf16_pair(v[i], v[i + 1]);
+            v[i] = __uint_as_float(w << 16), v[i + 1] = __uint_as_float(w & 0xffff0000u);
+        }
 }
 
 // Y: 0 = none, 1 = BF16, 2 = FP32.  NV: pieces of a row that a thread has, blockDim.x apart (a multiple of 32, so that blocks stay with sixteen lanes).
@@ -69,7 +80,8 @@ __global__ void __launch_bounds__(1024) add_norm_kernel(const NormArgs a) {
             if constexpr (Y == 1) load8(static_cast<const uint16_t *>(a.y) + row * a.y_ld + at, y);
             else load8(static_cast<const float *>(a.y) + row * a.y_ld + at, y);
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) s[j][i] = as_stored<TX>(s[j][i] + y[i]);
+            for (int i = 0; i < kVec; ++i) s[j][i] += y[i];
+            as_kept<TX>(s[j]);
             if (a.total != nullptr) store8(static_cast<TX *>(a.total) + row * a.total_ld + at, s[j]);
         }
     }

@@ -22,4 +22,11 @@ __device__ inline uint32_t f8_pair(float lo, float hi) {
 }
 __device__ inline uint32_t f8_quad(float a, float b, float c, float d) { return f8_pair(a, b) | (f8_pair(c, d) << 16); }
 
+// Two values rounded to BF16 (the first in the lower half).
+__device__ inline uint32_t bf16_pair(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 }  // namespace sxb

@@ -20,17 +20,17 @@ namespace {
 constexpr int kSumWarps = 8, kCopyWarp = kSumWarps, kMmaWarp = kSumWarps + 1;
 constexpr int kTileM = 128;                  // rows of x of a CTA: the lanes of tensor memory
 constexpr int kLine = kF8Block;              // bytes of a stage's row: a block of k
-constexpr int kMaxStages = 6;
+constexpr int kStages = 6;
+constexpr int kTmemCols = 512;
+// A third warpgroup beside the two that sum, to which most of its registers go: 40 and 232 a thread are the 168 that 384 threads were launched with.
+constexpr int kThreads = 384;
+constexpr int kAtOnce = 32;                  // columns of an accumulator that a thread asks for at once
 
 template <int CTAS, int BN>
 struct Shape {
     static constexpr int kBRows = BN / CTAS;                                   // weight rows that a CTA holds
     static constexpr int kStageBytes = (kTileM + kBRows) * kLine;
-    static constexpr int kStages = CTAS == 2 ? kMaxStages : 3;                 // tiles: two CTAs an SM
-    static constexpr int kTmemCols = 2 * BN;
-    // Pairs: a third warpgroup, most of whose registers go to the two that sum (40 and 232 a thread are what 384 threads were launched with, 168 each).
-    static constexpr int kThreads = CTAS == 2 ? 384 : 32 * (kSumWarps + 2);
-    static constexpr int kAtOnce = CTAS == 2 ? 32 : 16;                        // columns of an accumulator that a thread reads at once
+    static constexpr int kAccs = 512 / BN;                                     // accumulators: all of tensor memory
     static constexpr int kPitch = BN + 4;                                      // floats of a row of a part
     static constexpr size_t kRing = (size_t)kStages * kStageBytes, kPart = CTAS == 1 ? (size_t)kTileM * kPitch * 4 : 0;
     static constexpr size_t kSmem = (kRing > kPart ? kRing : kPart) + 1024;
@@ -41,6 +41,7 @@ struct TcArgs8 {
     int n_m, n_n, band;  // tiles along m and n; tiles along m of a band, in which all of n is gone through
     int split;           // CTAs that share a tile's k (tiles)
     int vec;             // bytes of y that may be stored at once
+    int xs4;             // four scales of a row of x may be loaded at once
     uint32_t *status;
     unsigned long long wait_limit_ns;
     int test_skip_slot;
@@ -107,20 +108,24 @@ __device__ inline uint32_t in_first_cta(uint64_t *bar) {
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
     return r;
 }
-__device__ inline void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ inline void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ inline void cluster_meet() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
 
-// 16 or 32 consecutive columns of this thread's TMEM lane.
-__device__ inline void tc_ld(uint32_t taddr, float (&v)[16]) { tc_ld16(taddr, v); }
-__device__ inline void tc_ld(uint32_t taddr, float (&v)[32]) {
+// 32 consecutive columns of this thread's TMEM lane: asked for, and there.  (The second names the registers, so that nothing reads them before it.)
+__device__ inline void tc_ask(uint32_t taddr, float (&v)[32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
           "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
           "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(taddr)
         : "memory");
+}
+__device__ inline void tc_there(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                   "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                   "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])::"memory");
 }
 __device__ inline uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -161,7 +166,7 @@ __device__ inline void store_run(const TcArgs8 &a, int64_t at, int left, const f
         for (int i = 0; i < NV; i += 16) {
             uint32_t w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = (uint32_t)f32_to_bf16_bits(v[i + 2 * k]) | ((uint32_t)f32_to_bf16_bits(v[i + 2 * k + 1]) << 16);
+            for (int k = 0; k < 8; ++k) w[k] = bf16_pair(v[i + 2 * k], v[i + 2 * k + 1]);
             if (i + 16 <= left && a.vec >= 32) store32(p + i, w);
             else if (i + 16 <= left && a.vec >= 16) {
                 reinterpret_cast<uint4 *>(p + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -193,14 +198,14 @@ __device__ inline Tile tile_of(const TcArgs8 &a, int64_t item) {
 }
 
 template <int CTAS, int BN>
-__global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, CTAS == 2 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, 1)
     f8_tc_kernel(const TcArgs8 a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
     using S = Shape<CTAS, BN>;
     constexpr int kCols = BN / 2;  // of a summing thread
     behind_grid();
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *const smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full_bar[S::kStages], empty_bar[S::kStages], acc_full[2], acc_empty[2], drain_bar;
+    __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[S::kAccs], acc_empty[S::kAccs], drain_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ int abort_flag;
 
@@ -211,18 +216,18 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, CTAS == 2 ? 1 : 2)
     volatile int *const abort_v = &abort_flag;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
-        for (int b = 0; b < 2; ++b) mbar_init(&acc_full[b], 1), mbar_init(&acc_empty[b], kSumWarps * CTAS);
+        for (int s = 0; s < kStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
+        for (int b = 0; b < S::kAccs; ++b) mbar_init(&acc_full[b], 1), mbar_init(&acc_empty[b], kSumWarps * CTAS);
         mbar_init(&drain_bar, 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
         if constexpr (CTAS == 1) {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(S::kTmemCols) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(kTmemCols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         } else {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(S::kTmemCols) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(kTmemCols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
@@ -255,7 +260,7 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, CTAS == 2 ? 1 : 2)
             const int row0 = t.m * kTileM, col0 = t.n * BN;
             // four neighbouring columns a thread, in turn the cluster's CTAs'
             if (!*abort_v)
-                for (int i = rank * S::kThreads + (int)threadIdx.x; i < kTileM * BN / 4; i += group * S::kThreads) {
+                for (int i = rank * kThreads + (int)threadIdx.x; i < kTileM * BN / 4; i += group * kThreads) {
                     const int r = i / (BN / 4), c = i % (BN / 4) * 4;
                     if (row0 + r >= a.g.M || col0 + c >= a.g.N) continue;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -288,13 +293,13 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, CTAS == 2 ? 1 : 2)
         if constexpr (CTAS == 2) cluster_meet();
         if (warp == kMmaWarp) {
             tc_fence_after();
-            if constexpr (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
-            else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmemCols) : "memory");
+            if constexpr (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+            else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
         }
     };
 
     if (warp >= kSumWarps) {
-        if constexpr (CTAS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == kCopyWarp) {
             // ===================== copies: one thread, as far ahead as free stages allow =====================
             if (lane == 0) {
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, CTAS == 2 ? 1 : 2)
                 for (int64_t item = first; item < n_items && !*abort_v; item += step) {
                     const Tile t = tile_of(a, item);
                     const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM, wrow = t.n * BN + (CTAS == 2 ? rank * S::kBRows : 0);
-                    for (int kb = kb0; kb < kb1; ++kb, ++issued, turn.advance(S::kStages)) {
+                    for (int kb = kb0; kb < kb1; ++kb, ++issued, turn.advance(kStages)) {
                         if (!mbar_wait(&empty_bar[turn.at], turn.phase, abort_v, a.wait_limit_ns)) {
                             raise_abort(item, 5);
                             break;
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, CTAS == 2 ? 1 : 2)
                         tc_block_e4m3<CTAS>(leader, tmem_base + (uint32_t)(acc.at * BN), lo, lo + kTileM * kLine / 16, hi, idesc);
                         commit_to<CTAS>(leader, &empty_bar[turn.at]);  // the stage is free once these MMAs have read it
                         commit_to<CTAS>(leader, &acc_full[acc.at]);
-                        turn.advance(S::kStages), acc.advance(2);
+                        turn.advance(kStages), acc.advance(S::kAccs);
                     }
                 // every MMA has completed before shared and tensor memory are given up (not skipped while aborting)
                 commit_to<CTAS>(leader, &drain_bar);
@@ -352,42 +357,74 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, CTAS == 2 ? 1 : 2)
         }
         leave();
     } else {
-        if constexpr (CTAS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         // ===================== sums and stores =====================
         const int quad = warp & 3, half = warp >> 2;  // the TMEM lanes a warp may read: 32 (warp % 4) ..; its half of the columns
         const uint32_t lanes = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * kCols);
-        const uint32_t empty_at[2] = {CTAS == 2 ? in_first_cta(&acc_empty[0]) : smem_u32(&acc_empty[0]), CTAS == 2 ? in_first_cta(&acc_empty[1]) : smem_u32(&acc_empty[1])};
+        const uint32_t empty_at = CTAS == 2 ? in_first_cta(&acc_empty[0]) : smem_u32(&acc_empty[0]);
         Turn acc{0, 0u};
-        for (int64_t item = first; item < n_items && !*abort_v; item += step) {
+        // A thread's scales, four blocks (a group) at a time, a group ahead of its use: next holds the factors of the group behind kb's.
+        struct Four {
+            float x[4], w[4];
+        };
+        auto group_of = [&](int64_t item, int group) {
+            const Tile t = tile_of(a, item);
+            const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM + quad * 32 + lane, col = t.n * BN + half * kCols, kb = 4 * group;
+            Four f{};
+            if (row >= a.g.M || col >= a.g.N || kb >= kb1) return f;
+            const float *const xs = a.g.xs + (int64_t)row * a.g.xs_ld + kb, *const ws = a.g.ws + (int64_t)(col / kF8Block) * a.g.kb + kb;
+            if (a.xs4 && kb + 4 <= a.g.kb) {
+                const float4 x = __ldg(reinterpret_cast<const float4 *>(xs));
+                f.x[0] = x.x, f.x[1] = x.y, f.x[2] = x.z, f.x[3] = x.w;
+            } else
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (kb + i < a.g.kb) f.x[i] = __ldg(xs + i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (kb + i < a.g.kb) f.w[i] = __ldg(ws + i);
+            return f;
+        };
+        float now[4] = {};
+        Four next = group_of(first, kb0 / 4);
+        for (int64_t item = first; item < n_items; item += step) {
             const Tile t = tile_of(a, item);
             const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM + quad * 32 + lane, col = t.n * BN + half * kCols;
             const bool there = row < a.g.M;
-            const float *const xs = a.g.xs + (int64_t)row * a.g.xs_ld, *const ws = a.g.ws + (int64_t)(min(col, a.g.N - 1) / kF8Block) * a.g.kb;
             uint64_t sum[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) sum[i] = 0;
-            float next = there && kb0 < kb1 ? xs[kb0] * ws[kb0] : 0.f;
             for (int kb = kb0; kb < kb1; ++kb) {
-                const float s = next;
-                if (kb + 1 < kb1 && there) next = xs[kb + 1] * ws[kb + 1];
-                if (lane == 0 && !mbar_wait(&acc_full[acc.at], acc.phase, abort_v, a.wait_limit_ns)) raise_abort(item, 4);
-                __syncwarp();
-                if (*abort_v) break;
+                if ((kb & 3) == 0 || kb == kb0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) now[i] = next.x[i] * next.w[i];
+                    next = (kb | 3) + 1 < kb1 ? group_of(item, kb / 4 + 1) : item + step < n_items ? group_of(item + step, kb0 / 4) : Four{};
+                }
+                const float s = kb & 2 ? (kb & 1 ? now[3] : now[2]) : (kb & 1 ? now[1] : now[0]);
+                if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc.at], acc.phase, abort_v, a.wait_limit_ns))) {
+                    if (lane == 0) raise_abort(item, 4);
+                    break;
+                }
                 tc_fence_after();
                 const uint64_t s2 = pack2(s, s);
+                constexpr int AT = kAtOnce;
+                float v[2][AT];
+                const uint32_t from = lanes + (uint32_t)(acc.at * BN);
+                tc_ask(from, v[0]);
 #pragma unroll
-                for (int c = 0; c < kCols; c += S::kAtOnce) {
-                    float v[S::kAtOnce];
-                    tc_ld(lanes + (uint32_t)(acc.at * BN + c), v);
-                    if (c + S::kAtOnce == kCols) {  // the last columns are in registers: the accumulator may be overwritten
+                for (int c = 0; c < kCols; c += AT) {
+                    float(&u)[AT] = v[c / AT & 1];
+                    tc_there(u);
+                    if (c + AT < kCols) tc_ask(from + (uint32_t)(c + AT), v[c / AT + 1 & 1]);  // on its way under these columns' sums
+                    else {  // the last columns are in registers: the accumulator may be overwritten
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) arrive_at(empty_at[acc.at]);
+                        if (lane == 0) arrive_at(empty_at + 8u * (uint32_t)acc.at);
                     }
 #pragma unroll
-                    for (int i = 0; i < S::kAtOnce / 2; ++i) sum[c / 2 + i] = fma2(pack2(v[2 * i], v[2 * i + 1]), s2, sum[c / 2 + i]);
+                    for (int i = 0; i < AT / 2; ++i) sum[c / 2 + i] = fma2(pack2(u[2 * i], u[2 * i + 1]), s2, sum[c / 2 + i]);
                 }
-                acc.advance(2);
+                acc.advance(S::kAccs);
             }
             if (*abort_v) break;
             if (CTAS == 1 && a.split > 1) {
@@ -422,8 +459,8 @@ int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
     const int64_t items = (int64_t)a.n_m * a.n_n;
     const int cluster = CTAS == 2 ? 2 : a.split;
     SXB_CUDA(cudaFuncSetAttribute(f8_tc_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), fn, ": reserving shared memory");
-    const int64_t places = CTAS == 2 ? sm_count() / 2 : a.split > 1 ? items : 2 * (int64_t)sm_count();
-    const cudaError_t e = launch_behind(f8_tc_kernel<CTAS, BN>, dim3((unsigned)(std::min(items, places) * cluster)), dim3(S::kThreads), S::kSmem, st, cluster, a, xmap, wmap);
+    const int64_t places = CTAS == 2 ? sm_count() / 2 : a.split > 1 ? items : (int64_t)sm_count();
+    const cudaError_t e = launch_behind(f8_tc_kernel<CTAS, BN>, dim3((unsigned)(std::min(items, places) * cluster)), dim3(kThreads), S::kSmem, st, cluster, a, xmap, wmap);
     SXB_CUDA(e, fn, ": launching M=", a.g.M, " N=", a.g.N, " K=", a.g.K);
     return SXB_OK;
 }
@@ -435,11 +472,12 @@ int linear_f8_tc(const char *fn, const F8Args &g, cudaStream_t st) {
     a.g = g;
     const int64_t es = g.f32 ? 4 : 2;
     for (a.vec = 32; a.vec > 4 && (reinterpret_cast<uintptr_t>(g.y) % a.vec != 0 || g.y_ld * es % a.vec != 0); a.vec /= 2) {}
+    a.xs4 = reinterpret_cast<uintptr_t>(g.xs) % 16 == 0 && g.xs_ld % 4 == 0;
     a.wait_limit_ns = wait_limit_ns(), a.test_skip_slot = test_skip_slot();
     if (int rc = library_status_words(fn, &a.status)) return rc;
     const int64_t sms = sm_count(), pairs = (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256), tiles = (int64_t)((g.M + 127) / 128) * ((g.N + 127) / 128);
     if (g.M > 128 && pairs * 2 >= sms) return launch_tc8<2, 256>(fn, a, st);
-    a.split = (int)std::max<int64_t>(1, std::min<int64_t>({8, 2 * sms / tiles, g.kb / 2}));
+    a.split = (int)std::max<int64_t>(1, std::min<int64_t>({8, sms / tiles, g.kb / 2}));
     return launch_tc8<1, 128>(fn, a, st);
 }
 
