@@ -20,7 +20,7 @@ namespace {
 constexpr int kSumWarps = 8, kCopyWarp = kSumWarps, kMmaWarp = kSumWarps + 1;
 constexpr int kTileM = 128;                  // rows of x of a CTA: the lanes of tensor memory
 constexpr int kLine = kF8Block;              // bytes of a stage's row: a block of k
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kTmemCols = 512;
 // A third warpgroup beside the two that sum, to which most of its registers go: 40 and 232 a thread are the 168 that 384 threads were launched with.
 constexpr int kThreads = 384;
@@ -33,7 +33,9 @@ struct Shape {
     static constexpr int kAccs = 512 / BN;                                     // accumulators: all of tensor memory
     static constexpr int kPitch = BN + 4;                                      // floats of a row of a part
     static constexpr size_t kRing = (size_t)kStages * kStageBytes, kPart = CTAS == 1 ? (size_t)kTileM * kPitch * 4 : 0;
-    static constexpr size_t kSmem = (kRing > kPart ? kRing : kPart) + 1024;
+    static constexpr size_t kOut = (size_t)kTileM * BN * 2;                    // a tile's rows of y in BF16, on their way out
+    static constexpr size_t kSmem = kRing + kOut + 1024;
+    static_assert(kPart <= kRing && kSmem <= 231 * 1024);
 };
 
 struct TcArgs8 {
@@ -41,6 +43,7 @@ struct TcArgs8 {
     int n_m, n_n, band;  // tiles along m and n; tiles along m of a band, in which all of n is gone through
     int split;           // CTAs that share a tile's k (tiles)
     int vec;             // bytes of y that may be stored at once
+    int tensor_out;      // y (BF16) takes tensor copies
     int xs4;             // four scales of a row of x may be loaded at once
     uint32_t *status;
     unsigned long long wait_limit_ns;
@@ -191,15 +194,15 @@ struct Turn {
 struct Tile {
     int m, n;
 };
-__device__ inline Tile tile_of(const TcArgs8 &a, int64_t item) {
-    const int64_t per = (int64_t)a.band * a.n_n, b = item / per, rest = item % per;
-    const int in_band = min(a.band, a.n_m - (int)b * a.band);
-    return Tile{(int)b * a.band + (int)(rest % in_band), (int)(rest / in_band)};
+__device__ inline Tile tile_of(const TcArgs8 &a, int item) {  // at most 2^13 x 2^17 tiles
+    const int per = a.band * a.n_n, b = item / per, rest = item - b * per;
+    const int in_band = min(a.band, a.n_m - b * a.band);
+    return Tile{b * a.band + rest % in_band, rest / in_band};
 }
 
 template <int CTAS, int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-    f8_tc_kernel(const TcArgs8 a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+    f8_tc_kernel(const TcArgs8 a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap ymap) {
     using S = Shape<CTAS, BN>;
     constexpr int kCols = BN / 2;  // of a summing thread
     behind_grid();
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int group = CTAS == 2 ? 2 : a.split, rank = (int)blockIdx.x % group;  // of the cluster
-    const int64_t n_items = (int64_t)a.n_m * a.n_n, first = blockIdx.x / group, step = gridDim.x / group;
+    const int n_items = a.n_m * a.n_n, first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
     const int kb0 = CTAS == 2 ? 0 : (int)((int64_t)a.g.kb * rank / group), kb1 = CTAS == 2 ? a.g.kb : (int)((int64_t)a.g.kb * (rank + 1) / group);
     volatile int *const abort_v = &abort_flag;
 
@@ -237,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_smem;
 
-    auto raise_abort = [&](int64_t item, int role) {
+    auto raise_abort = [&](int item, int role) {
         if (atomicExch(&abort_flag, 1) == 0 && atomicCAS(&a.status[0], 0u, 2u) == 0u) {
             a.status[1] = (uint32_t)item;
             a.status[2] = (uint32_t)role;
@@ -305,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) {
                 Turn turn{0, 1u};  // the phase before the first leaves every stage free
                 int issued = 0;
-                for (int64_t item = first; item < n_items && !*abort_v; item += step) {
+                for (int item = first; item < n_items && !*abort_v; item += step) {
                     const Tile t = tile_of(a, item);
                     const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM, wrow = t.n * BN + (CTAS == 2 ? rank * S::kBRows : 0);
                     for (int kb = kb0; kb < kb1; ++kb, ++issued, turn.advance(kStages)) {
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0;
                 Turn turn{0, 0u}, acc{0, 1u};
                 bool ok = true;
-                for (int64_t item = first; item < n_items && ok; item += step)
+                for (int item = first; item < n_items && ok; item += step)
                     for (int kb = kb0; kb < kb1; ++kb) {
                         ok = __all_sync(0xffffffffu, mbar_wait(&acc_empty[acc.at], acc.phase, abort_v, a.wait_limit_ns));
                         if (!ok) {
@@ -367,8 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         struct Four {
             float x[4], w[4];
         };
-        auto group_of = [&](int64_t item, int group) {
-            const Tile t = tile_of(a, item);
+        auto group_of = [&](const Tile &t, int group) {
             const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM + quad * 32 + lane, col = t.n * BN + half * kCols, kb = 4 * group;
             Four f{};
             if (row >= a.g.M || col >= a.g.N || kb >= kb1) return f;
@@ -386,9 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             return f;
         };
         float now[4] = {};
-        Four next = group_of(first, kb0 / 4);
-        for (int64_t item = first; item < n_items; item += step) {
-            const Tile t = tile_of(a, item);
+        Tile t = tile_of(a, first), then = t;
+        Four next = group_of(t, kb0 / 4);
+        for (int item = first; item < n_items; item += step, t = then) {
             const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM + quad * 32 + lane, col = t.n * BN + half * kCols;
             const bool there = row < a.g.M;
             uint64_t sum[kCols / 2];
@@ -398,7 +400,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if ((kb & 3) == 0 || kb == kb0) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) now[i] = next.x[i] * next.w[i];
-                    next = (kb | 3) + 1 < kb1 ? group_of(item, kb / 4 + 1) : item + step < n_items ? group_of(item + step, kb0 / 4) : Four{};
+                    if ((kb | 3) + 1 < kb1) next = group_of(t, kb / 4 + 1);
+                    else if (item + step < n_items) then = tile_of(a, item + step), next = group_of(then, kb0 / 4);
                 }
                 const float s = kb & 2 ? (kb & 1 ? now[3] : now[2]) : (kb & 1 ? now[1] : now[0]);
                 if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc.at], acc.phase, abort_v, a.wait_limit_ns))) {
@@ -432,6 +435,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float *const part = reinterpret_cast<float *>(smem) + (quad * 32 + lane) * S::kPitch + half * kCols;
 #pragma unroll
                 for (int i = 0; i < kCols / 2; i += 2) *reinterpret_cast<ulonglong2 *>(part + 2 * i) = make_ulonglong2(sum[i], sum[i + 1]);
+            } else if (a.tensor_out) {
+                // rows of 64 columns, 128 bytes, their 16-byte pieces swizzled: eight lanes' stores touch all banks; a warp's 32 rows are a box of their own
+                unsigned char *const out = smem + S::kRing + quad * 32 * 128;
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile's have been read
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < kCols; c += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = bf16_pair(__uint_as_float((uint32_t)sum[c / 2 + i]), __uint_as_float((uint32_t)(sum[c / 2 + i] >> 32)));
+                    const int at = half * kCols + c;
+                    *reinterpret_cast<uint4 *>(out + (at / 64) * (kTileM * 128) + swz(lane, at % 64 / 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0 && row < a.g.M) {
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 64)
+                        if (col + c < a.g.N)
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(&ymap)), "r"(col + c), "r"(row),
+                                         "r"(smem_u32(out + ((half * kCols + c) / 64) * (kTileM * 128)))
+                                         : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
             } else if (there) {
 #pragma unroll
                 for (int c = 0; c < kCols; c += 32) {
@@ -442,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // what was stored from shared memory has been written
         leave();
     }
 }
@@ -449,10 +477,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int CTAS, int BN>
 int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
     using S = Shape<CTAS, BN>;
-    CUtensorMap xmap, wmap;
+    CUtensorMap xmap, wmap, ymap;
     if (int rc = tensor_map_2d(fn, a.g.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.M, (uint64_t)a.g.x_ld, kLine, kTileM, CU_TENSOR_MAP_SWIZZLE_128B, &xmap))
         return rc;
     if (int rc = tensor_map_2d(fn, a.g.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.N, (uint64_t)a.g.K, kLine, S::kBRows, CU_TENSOR_MAP_SWIZZLE_128B, &wmap))
+        return rc;
+    a.tensor_out = !a.g.f32 && a.vec >= 16 && (CTAS == 2 || a.split == 1);
+    if (!a.tensor_out) ymap = xmap;  // not used
+    else if (int rc = tensor_map_2d(fn, a.g.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.g.N, (uint64_t)a.g.M, (uint64_t)a.g.y_ld * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, &ymap))
         return rc;
     a.n_m = (a.g.M + kTileM * CTAS - 1) / (kTileM * CTAS), a.n_n = (a.g.N + BN - 1) / BN;
     a.band = std::min(a.n_m, 16);
@@ -460,7 +492,7 @@ int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
     const int cluster = CTAS == 2 ? 2 : a.split;
     SXB_CUDA(cudaFuncSetAttribute(f8_tc_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), fn, ": reserving shared memory");
     const int64_t places = CTAS == 2 ? sm_count() / 2 : a.split > 1 ? items : (int64_t)sm_count();
-    const cudaError_t e = launch_behind(f8_tc_kernel<CTAS, BN>, dim3((unsigned)(std::min(items, places) * cluster)), dim3(kThreads), S::kSmem, st, cluster, a, xmap, wmap);
+    const cudaError_t e = launch_behind(f8_tc_kernel<CTAS, BN>, dim3((unsigned)(std::min(items, places) * cluster)), dim3(kThreads), S::kSmem, st, cluster, a, xmap, wmap, ymap);
     SXB_CUDA(e, fn, ": launching M=", a.g.M, " N=", a.g.N, " K=", a.g.K);
     return SXB_OK;
 }
