@@ -7,11 +7,15 @@
 namespace sxb {
 namespace {
 
-// ---- few rows: the weights stream through the registers -------------------------------------------------------------------------
+// ---- up to eight rows of x over a weight that is not large ------------------------------------------------------------------------
+//
+// A CTA has 16 weight rows, its warps a run of k each: every warp asks for AHEAD blocks of k at once, codes and scales of both operands, and the parts are added up in shared
+// memory in the warps' order.  What bounds it is the round trips: launch, operands, parts (6144 x 4096, one row of x: 7.8 us with the weights in HBM; the form on tcgen05 9.7, from
+// 2^26 codes on that one is ahead).
 
-constexpr int kRows = 16, kTokens = 8, kWarps = 8;  // weight rows and tokens of an MMA; warps of a CTA, which share out k
+constexpr int kRows = 16, kTokens = 8;  // weight rows and rows of x of an MMA
 
-// d += 16 weight rows x 8 tokens x 32 k of codes: exact products, FP32 sums.
+// d += 16 weight rows x 8 rows of x x 32 k of codes: exact products, FP32 sums.
 __device__ inline void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -20,58 +24,76 @@ __device__ inline void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_
 }
 
 __device__ inline uint4 load16(const uint8_t *p, bool there) { return there ? __ldg(reinterpret_cast<const uint4 *>(p)) : make_uint4(0u, 0u, 0u, 0u); }
+__device__ inline uint4 stream16(const uint8_t *p, bool there) {  // read once: not kept in L1
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (there) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 
 // k inside a block is permuted alike on both operands: lane (g = lane / 4, c = lane % 4) holds the sixteen codes at 16 c and at 64 + 16 c of its weight rows g and
-// g + 8 and of its token g, four MMAs' worth.
-template <int NT>
+// g + 8 and of its row g of x, four MMAs' worth.
+struct Block {
+    uint4 lo[2], hi[2], x[2];  // of weight rows g and g + 8, of x
+    float ws, xs[2];           // scales: the weight's, those of rows 2 c and 2 c + 1 of x
+};
+
+template <int kWarps, int AHEAD>
 __global__ void __launch_bounds__(32 * kWarps) f8_rows_kernel(const F8Args a) {
     behind_grid();
-    __shared__ float parts[kWarps][kRows][NT * kTokens + 1];
+    __shared__ float parts[kWarps][kTokens][kRows + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * NT * kTokens;
-    float acc[NT][4] = {};
-    for (int b = warp; b < a.kb; b += kWarps) {
-        uint4 lo[2], hi[2];
+    const int n0 = blockIdx.x * kRows, kb0 = (int)((int64_t)a.kb * warp / kWarps), kb1 = (int)((int64_t)a.kb * (warp + 1) / kWarps);
+    const bool lo = n0 + g < a.N, hi = n0 + g + 8 < a.N, there = g < a.M;
+    const uint8_t *const w = a.w + (int64_t)(n0 + g) * a.K + 16 * c, *const w8 = w + 8 * a.K, *const x = a.x + g * a.x_ld + 16 * c;
+    const float *const ws = a.ws + (int64_t)(n0 / kF8Block) * a.kb, *const xs = a.xs + 2 * c * a.xs_ld;
+    float acc[4] = {};
+    for (int b0 = kb0; b0 < kb1; b0 += AHEAD) {
+        Block k[AHEAD];
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            const int64_t k = (int64_t)b * kF8Block + v * 64 + c * 16;
-            lo[v] = load16(a.w + (int64_t)(n0 + g) * a.K + k, n0 + g < a.N && k < a.K);
-            hi[v] = load16(a.w + (int64_t)(n0 + g + 8) * a.K + k, n0 + g + 8 < a.N && k < a.K);
+        for (int i = 0; i < AHEAD; ++i) {
+            const int64_t at = (int64_t)(b0 + i) * kF8Block;
+            const bool v0 = b0 + i < kb1 && at + 16 * c < a.K, v1 = b0 + i < kb1 && at + 64 + 16 * c < a.K;
+            k[i].lo[0] = stream16(w + at, lo && v0), k[i].lo[1] = stream16(w + at + 64, lo && v1);
+            k[i].hi[0] = stream16(w8 + at, hi && v0), k[i].hi[1] = stream16(w8 + at + 64, hi && v1);
+            k[i].x[0] = load16(x + at, there && v0), k[i].x[1] = load16(x + at + 64, there && v1);
+            k[i].xs[0] = b0 + i < kb1 && 2 * c < a.M ? __ldg(xs + b0 + i) : 0.f;
+            k[i].xs[1] = b0 + i < kb1 && 2 * c + 1 < a.M ? __ldg(xs + a.xs_ld + b0 + i) : 0.f;
+            k[i].ws = b0 + i < kb1 ? __ldg(ws + b0 + i) : 0.f;
         }
-        const float ws = a.ws[(int64_t)(n0 / kF8Block) * a.kb + b];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float part[4] = {};
-            const int m = m0 + t * kTokens + g;
+        for (int i = 0; i < AHEAD; ++i) {
+            float d[4] = {};
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                const int64_t k = (int64_t)b * kF8Block + v * 64 + c * 16;
-                const uint4 x = load16(a.x + m * a.x_ld + k, m < a.M && k < a.K);
-                mma_e4m3(part, lo[v].x, hi[v].x, lo[v].y, hi[v].y, x.x, x.y);
-                mma_e4m3(part, lo[v].z, hi[v].z, lo[v].w, hi[v].w, x.z, x.w);
+                mma_e4m3(d, k[i].lo[v].x, k[i].hi[v].x, k[i].lo[v].y, k[i].hi[v].y, k[i].x[v].x, k[i].x[v].y);
+                mma_e4m3(d, k[i].lo[v].z, k[i].hi[v].z, k[i].lo[v].w, k[i].hi[v].w, k[i].x[v].z, k[i].x[v].w);
             }
-            const int m1 = m0 + t * kTokens + 2 * c;
-            const float s0 = m1 < a.M ? a.xs[m1 * a.xs_ld + b] * ws : 0.f, s1 = m1 + 1 < a.M ? a.xs[(m1 + 1) * a.xs_ld + b] * ws : 0.f;
-            acc[t][0] = fmaf(part[0], s0, acc[t][0]), acc[t][1] = fmaf(part[1], s1, acc[t][1]);
-            acc[t][2] = fmaf(part[2], s0, acc[t][2]), acc[t][3] = fmaf(part[3], s1, acc[t][3]);
+            const float s0 = k[i].xs[0] * k[i].ws, s1 = k[i].xs[1] * k[i].ws;
+            acc[0] = fmaf(d[0], s0, acc[0]), acc[1] = fmaf(d[1], s1, acc[1]), acc[2] = fmaf(d[2], s0, acc[2]), acc[3] = fmaf(d[3], s1, acc[3]);
         }
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int m = t * kTokens + 2 * c;
-        parts[warp][g][m] = acc[t][0], parts[warp][g][m + 1] = acc[t][1], parts[warp][g + 8][m] = acc[t][2], parts[warp][g + 8][m + 1] = acc[t][3];
-    }
+    parts[warp][2 * c][g] = acc[0], parts[warp][2 * c + 1][g] = acc[1], parts[warp][2 * c][g + 8] = acc[2], parts[warp][2 * c + 1][g + 8] = acc[3];
     __syncthreads();
-    for (int i = threadIdx.x; i < kRows * NT * kTokens; i += 32 * kWarps) {
-        const int row = i % kRows, m = i / kRows;
-        if (n0 + row >= a.N || m0 + m >= a.M) continue;
+    const int n = n0 + threadIdx.x % kRows, m = threadIdx.x / kRows;  // kWarps >= 4: a thread an output
+    if (m < kTokens && n < a.N && m < a.M) {
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum += parts[w][row][m];
-        const int64_t at = (int64_t)(m0 + m) * a.y_ld + n0 + row;
-        if (a.f32) static_cast<float *>(a.y)[at] = sum;
-        else static_cast<uint16_t *>(a.y)[at] = f32_to_bf16_bits(sum);
+        for (int i = 0; i < kWarps; ++i) sum += parts[i][m][threadIdx.x % kRows];
+        if (a.f32) static_cast<float *>(a.y)[m * a.y_ld + n] = sum;
+        else static_cast<uint16_t *>(a.y)[m * a.y_ld + n] = f32_to_bf16_bits(sum);
     }
+}
+
+// Warps of a CTA, and blocks that one asks for at once.  Many tiles hide a round trip behind one another: few warps a tile, few blocks (16384 x 4096, one row of x: 15.0 us, sixteen
+// warps by fours 26.2; 65536 x 512: 10.0, eight by fours 28.7).  Few tiles want all their k on its way at once (1024 x 8192: 5.2 us, four warps by twos 19.1; 4096 x 4096: eight by
+// fours 5.9, by ones 7.1), but no more registers than that takes (2048 x 2048: sixteen by ones 2.4, by fours 3.9; 6144 x 4096, whose 384 CTAs then are all there: eight by ones 7.8,
+// by fours 8.4).
+cudaError_t launch_rows(const F8Args &a, cudaStream_t st) {
+    const unsigned tiles = (unsigned)((a.N + kRows - 1) / kRows);
+    auto go = [&](auto kern, int warps) { return launch_behind(kern, dim3(tiles), dim3(32 * warps), 0, st, 1, a); };
+    if (tiles >= 512) return a.kb <= 4 ? go(f8_rows_kernel<4, 1>, 4) : go(f8_rows_kernel<4, 2>, 4);
+    if (tiles >= 320 || a.kb < 8) return go(f8_rows_kernel<8, 1>, 8);
+    return a.kb >= 64 ? go(f8_rows_kernel<16, 4>, 16) : a.kb >= 24 ? go(f8_rows_kernel<8, 4>, 8) : go(f8_rows_kernel<16, 1>, 16);
 }
 
 }  // namespace
@@ -104,11 +126,8 @@ extern "C" int sxb_linear_f8(const SxbLinearF8Args *args, sxb_stream_t stream) {
     a.x = g.x, a.w = g.w->q, a.xs = g.x_scale, a.ws = g.w->scale, a.y = g.y, a.x_ld = g.x_ld, a.xs_ld = g.xs_ld, a.y_ld = g.y_ld, a.K = K;
     a.M = (int)M, a.N = (int)N, a.kb = (int)kb, a.f32 = g.out_act == SXB_ACT_F32;
     auto st = static_cast<cudaStream_t>(stream);
-    if (M > 32) return linear_f8_tc(fn, a, st);
-    const dim3 grid((unsigned)((N + kRows - 1) / kRows)), block(32 * kWarps);
-    const cudaError_t e = M <= 8    ? launch_behind(f8_rows_kernel<1>, grid, block, 0, st, 1, a)
-                          : M <= 16 ? launch_behind(f8_rows_kernel<2>, grid, block, 0, st, 1, a)
-                                    : launch_behind(f8_rows_kernel<4>, grid, block, 0, st, 1, a);
+    if (M > kTokens || N * K > (1ll << 26)) return linear_f8_tc(fn, a, st);
+    const cudaError_t e = launch_rows(a, st);
     SXB_CUDA(e, fn, ": launching M=", M, " N=", N, " K=", K);
     SXB_CHECK_LAUNCH(fn, " M=", M, " N=", N, " K=", K);
     return SXB_OK;

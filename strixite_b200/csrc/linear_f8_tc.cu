@@ -12,8 +12,6 @@
 #include "linear_f8.cuh"
 #include "tc_ptx.cuh"
 
-#include <cooperative_groups.h>
-
 namespace sxb {
 namespace {
 
@@ -31,11 +29,9 @@ struct Shape {
     static constexpr int kBRows = BN / CTAS;                                   // weight rows that a CTA holds
     static constexpr int kStageBytes = (kTileM + kBRows) * kLine;
     static constexpr int kAccs = 512 / BN;                                     // accumulators: all of tensor memory
-    static constexpr int kPitch = BN + 4;                                      // floats of a row of a part
-    static constexpr size_t kRing = (size_t)kStages * kStageBytes, kPart = CTAS == 1 ? (size_t)kTileM * kPitch * 4 : 0;
-    static constexpr size_t kOut = (size_t)kTileM * BN * 2;                    // a tile's rows of y in BF16, on their way out
+    static constexpr size_t kRing = (size_t)kStages * kStageBytes, kOut = (size_t)kTileM * BN * 2;  // and a tile's rows of y in BF16, on their way out
     static constexpr size_t kSmem = kRing + kOut + 1024;
-    static_assert(kPart <= kRing && kSmem <= 231 * 1024);
+    static_assert(kSmem <= 226 * 1024 && (CTAS == 2 || (size_t)kTileM * BN * 4 <= kRing));
 };
 
 struct TcArgs8 {
@@ -106,11 +102,15 @@ __device__ inline void load_box(uint32_t dst, const CUtensorMap *map, int x, int
                      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
                      : "memory");
 }
-__device__ inline uint32_t in_first_cta(uint64_t *bar) {
+// The same place in the shared memory of the cluster's CTA `rank`.
+__device__ inline uint32_t in_cta(const void *p, int rank) {
     uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
     return r;
 }
+__device__ inline uint32_t in_first_cta(uint64_t *bar) { return in_cta(bar, 0); }
+// What a kernel does before it may touch memory of the grid ahead: its tensor maps are fetched.
+__device__ inline void fetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
 __device__ inline void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ inline void cluster_meet() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
 
@@ -129,6 +129,18 @@ __device__ inline void tc_there(float (&v)[32]) {
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
                    "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
                    "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])::"memory");
+}
+__device__ inline void tc_ask(uint32_t taddr, float (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+                   "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ inline void tc_there(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                   "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
 __device__ inline uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -205,7 +217,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     f8_tc_kernel(const TcArgs8 a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap ymap) {
     using S = Shape<CTAS, BN>;
     constexpr int kCols = BN / 2;  // of a summing thread
-    behind_grid();
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *const smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[S::kAccs], acc_empty[S::kAccs], drain_bar;
@@ -224,6 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&drain_bar, 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fetch_map(&xmap), fetch_map(&wmap);
     }
     if (warp == kMmaWarp) {
         if constexpr (CTAS == 1) {
@@ -237,6 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     if constexpr (CTAS == 2) cluster_meet();  // the other CTA's barriers are there
+    behind_grid();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_smem;
 
@@ -256,19 +269,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncthreads();
         if (CTAS == 1 && a.split > 1) {
-            namespace cg = cooperative_groups;
-            cg::cluster_group cluster = cg::this_cluster();
-            cluster_meet();
+            cluster_meet();  // every part is there
             const Tile t = tile_of(a, first);
             const int row0 = t.m * kTileM, col0 = t.n * BN;
-            // four neighbouring columns a thread, in turn the cluster's CTAs'
+            // four neighbouring columns a thread, in turn the cluster's CTAs', parts in rank order
             if (!*abort_v)
                 for (int i = rank * kThreads + (int)threadIdx.x; i < kTileM * BN / 4; i += group * kThreads) {
                     const int r = i / (BN / 4), c = i % (BN / 4) * 4;
                     if (row0 + r >= a.g.M || col0 + c >= a.g.N) continue;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     for (int k = 0; k < group; ++k) {
-                        const float4 p = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(reinterpret_cast<float *>(smem), k) + r * S::kPitch + c);
+                        float4 p;
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
+                                     : "r"(in_cta(smem, k) + 4u * (uint32_t)(r * BN + (c ^ (r & 7) * 4)))
+                                     : "memory");
                         v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
                     }
                     const int64_t at = (int64_t)(row0 + r) * a.g.y_ld + col0 + c;
@@ -284,11 +299,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     } else {
                         uint16_t *p = static_cast<uint16_t *>(a.g.y) + at;
-                        const uint16_t w[4] = {f32_to_bf16_bits(v.x), f32_to_bf16_bits(v.y), f32_to_bf16_bits(v.z), f32_to_bf16_bits(v.w)};
-                        if (left >= 4 && a.vec >= 8) *reinterpret_cast<uint2 *>(p) = make_uint2((uint32_t)w[0] | ((uint32_t)w[1] << 16), (uint32_t)w[2] | ((uint32_t)w[3] << 16));
-                        else
-                            for (int k = 0; k < 4; ++k)
-                                if (k < left) p[k] = w[k];
+                        const uint32_t lo = bf16_pair(v.x, v.y), hi = bf16_pair(v.z, v.w);
+                        if (left >= 4 && a.vec >= 8) *reinterpret_cast<uint2 *>(p) = make_uint2(lo, hi);
+                        else {
+                            p[0] = (uint16_t)lo;
+                            if (left > 1) p[1] = (uint16_t)(lo >> 16);
+                            if (left > 2) p[2] = (uint16_t)hi;
+                            if (left > 3) p[3] = (uint16_t)(hi >> 16);
+                        }
                     }
                 }
             cluster_meet();  // nobody's part is read from here on
@@ -431,10 +449,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (*abort_v) break;
             if (CTAS == 1 && a.split > 1) {
-                // this CTA's part to shared memory: the ring is not needed any more (its one item's MMAs have completed)
-                float *const part = reinterpret_cast<float *>(smem) + (quad * 32 + lane) * S::kPitch + half * kCols;
+                // this CTA's part to shared memory: the ring is not needed any more (its one item's MMAs have completed); sixteen bytes' place within eight of them by the row, so
+                // that eight lanes' stores touch all banks
+                const int r = quad * 32 + lane;
+                float *const to = reinterpret_cast<float *>(smem) + r * BN;
 #pragma unroll
-                for (int i = 0; i < kCols / 2; i += 2) *reinterpret_cast<ulonglong2 *>(part + 2 * i) = make_ulonglong2(sum[i], sum[i + 1]);
+                for (int i = 0; i < kCols / 2; i += 2) *reinterpret_cast<ulonglong2 *>(to + ((half * kCols + 2 * i) ^ (r & 7) * 4)) = make_ulonglong2(sum[i], sum[i + 1]);
             } else if (a.tensor_out) {
                 // rows of 64 columns, 128 bytes, their 16-byte pieces swizzled: eight lanes' stores touch all banks; a warp's 32 rows are a box of their own
                 unsigned char *const out = smem + S::kRing + quad * 32 * 128;
@@ -474,6 +494,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// CTAs that share a tile's k: a power of two that leaves every tile's their places on the machine at once (48 clusters of three did not find them: 6144 weight rows, one row of x
+// 14.7 us, in pairs 9.8), two blocks each at least, and no more than pay for the parts' way through the cluster, which costs as much as `parts` blocks.
+int shares(int64_t tiles, int64_t kb, int64_t parts) {
+    int best = 1;
+    for (int s = 2; s <= 8 && tiles * s <= (s == 8 ? 64 : sm_count()) && kb >= s * 2; s *= 2)
+        if ((kb + s - 1) / s + parts < (kb + best - 1) / best + (best > 1 ? parts : 0)) best = s;
+    return best;
+}
+
 template <int CTAS, int BN>
 int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
     using S = Shape<CTAS, BN>;
@@ -482,17 +511,244 @@ int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
         return rc;
     if (int rc = tensor_map_2d(fn, a.g.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.N, (uint64_t)a.g.K, kLine, S::kBRows, CU_TENSOR_MAP_SWIZZLE_128B, &wmap))
         return rc;
-    a.tensor_out = !a.g.f32 && a.vec >= 16 && (CTAS == 2 || a.split == 1);
-    if (!a.tensor_out) ymap = xmap;  // not used
-    else if (int rc = tensor_map_2d(fn, a.g.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.g.N, (uint64_t)a.g.M, (uint64_t)a.g.y_ld * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, &ymap))
-        return rc;
     a.n_m = (a.g.M + kTileM * CTAS - 1) / (kTileM * CTAS), a.n_n = (a.g.N + BN - 1) / BN;
     a.band = std::min(a.n_m, 16);
     const int64_t items = (int64_t)a.n_m * a.n_n;
     const int cluster = CTAS == 2 ? 2 : a.split;
-    SXB_CUDA(cudaFuncSetAttribute(f8_tc_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), fn, ": reserving shared memory");
     const int64_t places = CTAS == 2 ? sm_count() / 2 : a.split > 1 ? items : (int64_t)sm_count();
+    // BF16 rows leave through shared memory, under the next tile's MMAs; a CTA's only tile too (777 x 1000 x 512: 5.4 us, from the registers 6.4)
+    a.tensor_out = !a.g.f32 && a.vec >= 16 && (CTAS == 2 || a.split == 1);
+    if (!a.tensor_out) ymap = xmap;  // not used
+    else if (int rc = tensor_map_2d(fn, a.g.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.g.N, (uint64_t)a.g.M, (uint64_t)a.g.y_ld * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, &ymap))
+        return rc;
+    SXB_CUDA(cudaFuncSetAttribute(f8_tc_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), fn, ": reserving shared memory");
     const cudaError_t e = launch_behind(f8_tc_kernel<CTAS, BN>, dim3((unsigned)(std::min(items, places) * cluster)), dim3(kThreads), S::kSmem, st, cluster, a, xmap, wmap, ymap);
+    SXB_CUDA(e, fn, ": launching M=", a.g.M, " N=", a.g.N, " K=", a.g.K);
+    return SXB_OK;
+}
+
+// ---- a few rows of x: the weights on the MMAs' M side ------------------------------------------------------------------------------
+//
+// What bounds it is the weights' bytes, 16 KB a block of k and tile of 128 weight rows; the rows of x, 16 to 64, are the MMA's columns.  The accumulators of all stages fit tensor
+// memory, so one commit a stage, of two blocks, says that its codes have been read and that its sums are there.  A lane of tensor memory is a weight row: a thread has all columns of
+// one, the weight's scale is one number for the warp, and those of x go round by shuffles.
+
+template <int NB>
+struct FewShape {
+    static constexpr int kBlocks = 2;                                             // of k, of a stage
+    static constexpr int kBlockBytes = (kTileM + NB) * kLine, kStageBytes = kBlocks * kBlockBytes;
+    static constexpr int kStages = NB == 32 ? 5 : 6;
+    static constexpr int kCols = kStages * kBlocks * NB, kTmem = kCols > 256 ? 512 : 256;
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
+    static_assert(kCols <= 512 && kSmem <= 226 * 1024 && NB * kTileM * 4 <= kStages * kStageBytes);
+};
+constexpr int kFewSumWarps = 4, kFewThreads = 32 * (kFewSumWarps + 2);
+
+template <int NB>
+__global__ void __launch_bounds__(kFewThreads, 1)
+    f8_few_kernel(const TcArgs8 a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap) {
+    using S = FewShape<NB>;
+    constexpr int PER = S::kBlocks;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *const smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full_bar[S::kStages], done_bar[S::kStages], drained_bar[S::kStages];
+    __shared__ uint32_t tmem_base_smem;
+    __shared__ int abort_flag;
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int group = a.split, rank = (int)blockIdx.x % group;
+    const int n_items = a.n_n, first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
+    const int kb0 = (int)((int64_t)a.g.kb * rank / group), kb1 = (int)((int64_t)a.g.kb * (rank + 1) / group);
+    volatile int *const abort_v = &abort_flag;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&done_bar[s], 1), mbar_init(&drained_bar[s], kFewSumWarps);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fetch_map(&xmap), fetch_map(&wmap);
+    }
+    if (warp == kFewSumWarps + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(S::kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    behind_grid();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_smem;
+
+    auto raise_abort = [&](int item, int role) {
+        if (atomicExch(&abort_flag, 1) == 0 && atomicCAS(&a.status[0], 0u, 2u) == 0u) {
+            a.status[1] = (uint32_t)item;
+            a.status[2] = (uint32_t)role;
+        }
+    };
+
+    if (warp == kFewSumWarps) {
+        // ===================== copies =====================
+        if (lane == 0) {
+            Turn turn{0, 1u};
+            int issued = 0;
+            for (int item = first; item < n_items && !*abort_v; item += step)
+                for (int kb = kb0; kb < kb1; kb += PER, ++issued, turn.advance(S::kStages)) {
+                    if (!mbar_wait(&done_bar[turn.at], turn.phase, abort_v, a.wait_limit_ns)) {
+                        raise_abort(item, 5);
+                        break;
+                    }
+                    if (blockIdx.x == 0 && issued == a.test_skip_slot) continue;
+                    const int n = min(PER, kb1 - kb);
+                    mbar_expect_tx(&full_bar[turn.at], (uint32_t)(n * S::kBlockBytes));
+                    for (int i = 0; i < n; ++i) {
+                        const uint32_t dst = smem_u32(smem) + (uint32_t)(turn.at * S::kStageBytes + i * S::kBlockBytes);
+                        tma_load_2d(dst, &wmap, (kb + i) * kLine, item * kTileM, &full_bar[turn.at]);
+                        tma_load_2d(dst + kTileM * kLine, &xmap, (kb + i) * kLine, 0, &full_bar[turn.at]);
+                    }
+                }
+        }
+        __syncwarp();
+    } else if (warp == kFewSumWarps + 1) {
+        // ===================== MMA issue =====================
+        const uint32_t leader = elect_one() ? 1u : 0u, idesc = instr_desc_e4m3(kTileM, NB);
+        const uint64_t desc0 = smem_desc(smem_u32(smem));
+        const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0;
+        Turn turn{0, 0u};
+        bool ok = true;
+        for (int item = first; item < n_items && ok; item += step)
+            for (int kb = kb0; kb < kb1; kb += PER, turn.advance(S::kStages)) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&drained_bar[turn.at], turn.phase ^ 1u, abort_v, a.wait_limit_ns));
+                if (!ok) {
+                    if (leader) raise_abort(item, 2);
+                    break;
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[turn.at], turn.phase, abort_v, a.wait_limit_ns));
+                if (!ok) {
+                    if (leader) raise_abort(item, 3);
+                    break;
+                }
+                tc_fence_after();
+                for (int i = 0; i < min(PER, kb1 - kb); ++i) {
+                    const uint32_t lo = lo0 + (uint32_t)(turn.at * S::kStageBytes + i * S::kBlockBytes) / 16;
+                    tc_block_e4m3<1>(leader, tmem_base + (uint32_t)((turn.at * PER + i) * NB), lo, lo + kTileM * kLine / 16, hi, idesc);
+                }
+                commit_to<1>(leader, &done_bar[turn.at]);
+            }
+        __syncwarp();
+    } else {
+        // ===================== sums and stores =====================
+        const uint32_t lanes = tmem_base + ((uint32_t)(warp * 32) << 16);
+        Turn turn{0, 0u};
+        constexpr int NV = (NB + 31) / 32;  // scales of x that a lane holds
+        // of a stage's blocks: those of the lane's rows of x, and the weight's (a tile lies in one block of weight rows); asked for a stage ahead of their use
+        struct Scales {
+            float x[PER][NV], w[PER];
+        };
+        auto scales = [&](int item, int kb) {
+            Scales s;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                s.w[i] = kb + i < kb1 ? __ldg(a.g.ws + (int64_t)item * a.g.kb + kb + i) : 0.f;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const int m = j * 32 + lane;
+                    s.x[i][j] = m < a.g.M && m < NB && kb + i < kb1 ? __ldg(a.g.xs + m * a.g.xs_ld + kb + i) : 0.f;
+                }
+            }
+            return s;
+        };
+        Scales next = scales(first, kb0);
+        for (int item = first; item < n_items; item += step) {
+            float sum[NB];
+#pragma unroll
+            for (int i = 0; i < NB; ++i) sum[i] = 0.f;
+            for (int kb = kb0; kb < kb1; kb += PER, turn.advance(S::kStages)) {
+                float now[PER][NV];
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) now[i][j] = next.x[i][j] * next.w[i];
+                if (!__all_sync(0xffffffffu, mbar_wait(&done_bar[turn.at], turn.phase, abort_v, a.wait_limit_ns))) {
+                    if (lane == 0) raise_abort(item, 4);
+                    break;
+                }
+                if (kb + PER < kb1) next = scales(item, kb + PER);
+                else if (item + step < n_items) next = scales(item + step, kb0);
+                tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    if (kb + i >= kb1) break;
+                    constexpr int AT = NB < 32 ? 16 : 32;
+#pragma unroll
+                    for (int c = 0; c < NB; c += AT) {
+                        float v[AT];
+                        tc_ask(lanes + (uint32_t)((turn.at * PER + i) * NB + c), v);
+                        tc_there(v);
+                        if (c + AT == NB && (i + 1 == PER || kb + i + 1 == kb1)) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&drained_bar[turn.at]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < AT; ++k) sum[c + k] = fmaf(v[k], __shfl_sync(0xffffffffu, now[i][(c + k) / 32], (c + k) % 32), sum[c + k]);
+                    }
+                }
+            }
+            if (*abort_v) break;
+            const int row = warp * 32 + lane, n = item * kTileM + row;
+            if (a.split > 1) {
+#pragma unroll
+                for (int m = 0; m < NB; ++m) reinterpret_cast<float *>(smem)[m * kTileM + row] = sum[m];  // the ring is not needed any more: all its MMAs have completed
+            } else if (n < a.g.N) {
+#pragma unroll
+                for (int m = 0; m < NB; ++m)
+                    if (m < a.g.M) {
+                        if (a.g.f32) static_cast<float *>(a.g.y)[m * a.g.y_ld + n] = sum[m];
+                        else static_cast<uint16_t *>(a.g.y)[m * a.g.y_ld + n] = f32_to_bf16_bits(sum[m]);
+                    }
+            }
+        }
+    }
+
+    if (*abort_v) {  // copies that a CTA issued, and MMAs, before it gave up are over within this time
+        const unsigned long long t0 = global_ns();
+        while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (a.split > 1) {
+        cluster_meet();  // every part is there
+        if (!*abort_v)
+            for (int i = rank * kFewThreads + (int)threadIdx.x; i < min(NB, a.g.M) * kTileM; i += group * kFewThreads) {
+                const int m = i / kTileM, n = first * kTileM + i % kTileM;
+                if (n >= a.g.N) continue;
+                float v = 0.f;
+                for (int k = 0; k < group; ++k) {
+                    float p;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p) : "r"(in_cta(smem, k) + 4u * (uint32_t)i) : "memory");
+                    v += p;
+                }
+                if (a.g.f32) static_cast<float *>(a.g.y)[m * a.g.y_ld + n] = v;
+                else static_cast<uint16_t *>(a.g.y)[m * a.g.y_ld + n] = f32_to_bf16_bits(v);
+            }
+        cluster_meet();  // nobody's part is read from here on
+    }
+    if (warp == kFewSumWarps + 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::kTmem) : "memory");
+    }
+}
+
+template <int NB>
+int launch_few(const char *fn, TcArgs8 a, cudaStream_t st) {
+    using S = FewShape<NB>;
+    CUtensorMap xmap, wmap;
+    if (int rc = tensor_map_2d(fn, a.g.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.M, (uint64_t)a.g.x_ld, kLine, NB, CU_TENSOR_MAP_SWIZZLE_128B, &xmap)) return rc;
+    if (int rc = tensor_map_2d(fn, a.g.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.N, (uint64_t)a.g.K, kLine, kTileM, CU_TENSOR_MAP_SWIZZLE_128B, &wmap)) return rc;
+    const int64_t sms = sm_count();
+    a.n_n = (a.g.N + kTileM - 1) / kTileM;
+    a.split = shares(a.n_n, a.g.kb, 5);
+    SXB_CUDA(cudaFuncSetAttribute(f8_few_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), fn, ": reserving shared memory");
+    const int64_t places = a.split > 1 ? a.n_n : std::min<int64_t>(a.n_n, sms);
+    const cudaError_t e = launch_behind(f8_few_kernel<NB>, dim3((unsigned)(places * a.split)), dim3(kFewThreads), S::kSmem, st, a.split, a, xmap, wmap);
     SXB_CUDA(e, fn, ": launching M=", a.g.M, " N=", a.g.N, " K=", a.g.K);
     return SXB_OK;
 }
@@ -507,9 +763,11 @@ int linear_f8_tc(const char *fn, const F8Args &g, cudaStream_t st) {
     a.xs4 = reinterpret_cast<uintptr_t>(g.xs) % 16 == 0 && g.xs_ld % 4 == 0;
     a.wait_limit_ns = wait_limit_ns(), a.test_skip_slot = test_skip_slot();
     if (int rc = library_status_words(fn, &a.status)) return rc;
+    if (g.M <= 16) return launch_few<16>(fn, a, st);
+    if (g.M <= 32) return launch_few<32>(fn, a, st);
     const int64_t sms = sm_count(), pairs = (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256), tiles = (int64_t)((g.M + 127) / 128) * ((g.N + 127) / 128);
     if (g.M > 128 && pairs * 2 >= sms) return launch_tc8<2, 256>(fn, a, st);
-    a.split = (int)std::max<int64_t>(1, std::min<int64_t>({8, sms / tiles, g.kb / 2}));
+    a.split = shares(tiles, g.kb, 11);
     return launch_tc8<1, 128>(fn, a, st);
 }
 
