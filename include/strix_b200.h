@@ -655,7 +655,7 @@ int sxb_linear_f8(const SxbLinearF8Args *args, sxb_stream_t stream);
  * token below 2^-126 of the row's largest), sums of chunks in FP64; a random number within some 2^-22 of a border may fall on either side of it.
  * Out: next_ids [T], for each row the token that comes behind it (kept drafts, then the drawn token), -1 in the rows behind; n_new [B] = tokens kept + 1; logp [T] (or NULL) = log of
  * each such token's p (greedy: of softmax(logits)), 0 in the rows behind.  A sequence without rows has n_new = 0; rows outside every sequence are left as they are.
- * ws: sxb_verify_drafts_workspace_bytes, device, 16-byte aligned, needs no clearing; calls that share it must be ordered.  T = 1 .. 2^20, V = 1 .. 2^20, B = 1 .. 2^20.
+ * ws: sxb_verify_drafts_workspace_bytes, device, 16-byte aligned, needs no clearing; calls that share it must be ordered.  T = 1 .. 2^20, V = 1 .. 2^20, B = 1 .. 8192.
  * Data errors, found in the rows that the decision reads (err = {1, row, code}): logits of a row that hold a NaN or +inf or nothing above -inf (code 1), a drafter's (2), a drafted token
  * outside 0 .. V - 1 (3), a random number outside [0, 1) (4), a temperature other than 0 below 2^-126, or not finite (5): n_new = 0, the sequence's
  * next_ids -1 and logp NaN.  A q_start that falls, leaves 0..T or starts below an earlier one (err = {1, sequence, 6}): n_new = 0, the rows are left as they are. */

@@ -1,13 +1,13 @@
 // Verification of drafted tokens against the target's probabilities, from given random numbers (include/strix_b200.h has the rules).
 //
-// Two launches.  The first reads every row's logits once, in chunks: a chunk's largest logit, the first token that has it, and the sum of 2^(c x - c max),
-// c = log2(e) / temperature.  The second, a CTA a sequence (a cluster of eight where the drafter gives its distribution), joins a row's chunks, tests the
-// drafts, and draws the next token: from the chunks' sums it knows the chunk in which the random number falls and reads that one again; only a difference of
-// two distributions takes the whole row of both, once more, shared by the cluster.  Nothing is counted or left behind in the workspace: no atomics, and
-// results do not depend on who comes first.
+// Two launches.  The first reads every row's logits once, a warp a chunk of 4 KB: its largest logit (and, for greedy sequences, the first token that has it) and the sum of 2^(c (x -
+// max)), c = log2(e) / temperature.  What bounds it is memory; a logit takes four to five instructions, one of them the exponential.  The second, a CTA a sequence (a cluster of eight
+// where the drafter gives its distribution), joins a row's chunks, tests the drafts, and draws the next token: from the chunks' sums it knows the chunk in which the random number
+// falls and reads that one again; only a difference of two distributions takes the whole row of both, once more, shared by the cluster.  It is bound by its chain of loads, of which
+// those that do not wait for the first launch are made ahead of its end.  Nothing is counted or left behind in the workspace: no atomics, and results do not depend on who comes first.
 //
-// A border's error: a term takes c (x - max) in FP32 (2^-23 of the exponent, which is small where the term is large), one ex2 (2^-22), sums of sixteen
-// terms a thread and 256 threads in FP32; chunks are joined in FP64, where the exponents c max are exact, and no logit is too large for them.
+// A border's error: a term takes c (x - max) in FP32 (2^-23 of the exponent, which is small where the term is large), one ex2 (2^-22), sums of up to sixteen
+// terms and then seven more in FP32; chunks are joined in FP64, where the exponents are exact, and no logit is too large for them.
 
 #include "common.cuh"
 #include "tc_ptx.cuh"
@@ -18,8 +18,11 @@ namespace sxb {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kChunk = 4096;   // tokens of a chunk: sixteen a thread, all loads at once
-constexpr int kRanks = 8;      // CTAs that share a difference of two rows
+constexpr int kStatThreads = 128, kStatCtas = 4;       // of the first kernel; CTAs an SM
+constexpr int kPieces = kThreads, kPerLane = kPieces / 32;  // of sixteen bytes, of a chunk: eight a lane of a warp, or one a thread of a CTA
+constexpr int kRanks = 8;                              // CTAs that share a difference of two rows
+constexpr int64_t kMaxV = 1 << 20, kMaxB = 8192;
+constexpr int kMaxChunks = (int)(kMaxV / (4 * kPieces)) + 1, kMaxRun = (kMaxChunks + kRanks - 1) / kRanks;  // of a row; of a CTA's share of one
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994531;
 
@@ -27,8 +30,8 @@ enum { kBadLogits = 1, kBadDraft = 2, kBadId = 3, kBadRandom = 4, kBadTemperatur
 
 struct ChunkStat {  // of 2^(c x) over a chunk
     double sum;     // relative to 2^(c best)
-    float best;     // NaN: the chunk holds a NaN or +inf
-    int at;
+    float best;     // NaN: the chunk holds a NaN; +inf: an infinity
+    int at;         // greedy sequences: the first token that has it
 };
 
 struct VerifyArgs {
@@ -38,37 +41,48 @@ struct VerifyArgs {
     const float *u, *u_pick, *temperature;
     int32_t *next_ids, *n_new;
     float *logp;
-    ChunkStat *stats;  // [T (, T of the drafter)][n_chunks]
+    ChunkStat *stats;  // [T (, T of the drafter)][pitch]
     uint32_t *err;
-    int T, V, B, n_chunks;
+    int T, V, B, pitch;
 };
 
 // Tokens are read in pieces of sixteen aligned bytes.  A row may begin inside one: piece i holds the tokens i * VE - mis ..., those outside 0 .. V - 1 are none.
 template <typename T>
 struct Row {
-    static constexpr int VE = 16 / (int)sizeof(T);
+    static constexpr int VE = 16 / (int)sizeof(T), kChunk = kPieces * VE;
     const T *p;
     int mis, V;
     __device__ inline Row(const void *base, int64_t ld, int64_t row, int n) : p(static_cast<const T *>(base) + row * ld), V(n) {
         mis = (int)((reinterpret_cast<uintptr_t>(p) / sizeof(T)) % VE);
     }
     __device__ inline int pieces() const { return (V + mis + VE - 1) / VE; }
+    __device__ inline int chunks() const { return (V + mis + kChunk - 1) / kChunk; }
     __device__ inline int token(int piece) const { return piece * VE - mis; }
     __device__ inline float at(int t) const { return load_as_f32(p, t); }
-    // The tokens t0 .. t0 + VE - 1, -inf where there are none.
-    __device__ inline void load(int t0, float (&v)[VE]) const {
-        if (t0 >= 0 && t0 + VE <= V && (reinterpret_cast<uintptr_t>(p + t0) & 15) == 0) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p + t0));
-            if constexpr (sizeof(T) == 4) {
-                v[0] = __uint_as_float(w.x), v[1] = __uint_as_float(w.y), v[2] = __uint_as_float(w.z), v[3] = __uint_as_float(w.w);
-            } else {
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    // A piece as it lies in memory, -inf where there are no tokens.
+    __device__ inline uint4 raw(int piece) const {
+        const int t0 = token(piece);
+        return t0 >= 0 && t0 + VE <= V ? __ldg(reinterpret_cast<const uint4 *>(p + t0)) : edge(t0);
+    }
+    __device__ inline uint4 edge(int t0) const {
+        uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = t0 + i >= 0 && t0 + i < V ? __float_as_uint((float)p[t0 + i]) : 0xff800000u;
+            else {
+                const int t = t0 + 2 * i;
+                w[i] = (t >= 0 && t < V ? (uint32_t)p[t] : 0xff80u) | ((t + 1 >= 0 && t + 1 < V ? (uint32_t)p[t + 1] : 0xff80u) << 16);
             }
-        } else {
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    // The same as numbers.
+    __device__ static inline void values(const uint4 &w, float (&v)[VE]) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int i = 0; i < VE; ++i) v[i] = t0 + i >= 0 && t0 + i < V ? load_as_f32(p, t0 + i) : -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(u[i]);
+            else v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         }
     }
 };
@@ -88,120 +102,223 @@ __device__ inline int sequence_of(const int32_t *q_start, int B, int row) {
     return -1;
 }
 
-template <typename TX>
-__device__ inline void chunk_stats(const VerifyArgs &a, const void *base, int64_t ld, int64_t row, int chunk, ChunkStat *out) {
-    constexpr int VE = Row<TX>::VE, NP = kChunk / VE / kThreads;
-    __shared__ float most_s[kWarps], sum_s[kWarps];
-    __shared__ int at_s[kWarps];
-    const Row<TX> r(base, ld, row, a.V);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float v[NP][VE];
+__device__ inline float max_nan(float a, float b) {  // NaN if one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ inline uint32_t max_nan_pair(uint32_t a, uint32_t b) {  // of two BF16
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ inline float warp_max_nan(float v) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ inline uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ inline uint64_t add_two(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ inline uint64_t mul_two(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ inline float first_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ inline float second_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+// 2^(c (x - best)) of two, each with the rounding that one alone has.
+__device__ inline uint64_t weight_two(float x0, float x1, uint64_t minus_best, uint64_t c) {
+    const uint64_t e = mul_two(add_two(two(x0, x1), minus_best), c);
+    return two(exp2_fast(first_of(e)), exp2_fast(second_of(e)));
+}
+
+// A lane's part of a chunk: piece 32 j + lane is its j-th.  Where the row does not begin or end with a piece, the tokens before the first and behind the last whole one are a lane's each.
+struct Loaded {
+    uint4 w[kPerLane];
+    float head, tail;
+};
+template <typename T>
+__device__ inline void load_chunk(const Row<T> &r, int chunk, Loaded &l) {
+    constexpr int VE = Row<T>::VE;
+    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+    const int lane = threadIdx.x & 31, whole0 = r.mis != 0, whole1 = (r.V + r.mis) / VE, p0 = chunk * kPieces;  // the whole pieces are whole0 .. whole1 - 1
+    const uint4 *const p = reinterpret_cast<const uint4 *>(r.p - r.mis);
 #pragma unroll
-    for (int j = 0; j < NP; ++j) r.load(r.token(chunk * (kChunk / VE) + j * kThreads + (int)threadIdx.x), v[j]);
-    float c = kLog2e;
-    if (a.temperature != nullptr) {
-        const int b = sequence_of(a.q_start, a.B, (int)row);
-        if (b < 0) return;  // the same for every warp
-        c = exponent_scale(a.temperature[b]);
+    for (int j = 0; j < kPerLane; ++j) {
+        const int i = p0 + 32 * j + lane;
+        l.w[j] = i >= whole0 && i < whole1 ? __ldg(p + i) : make_uint4(kNone, kNone, kNone, kNone);
     }
-    float most = -INFINITY;
+    l.head = l.tail = -INFINITY;
+    if (p0 == 0 && whole0 && lane < min(VE - r.mis, r.V)) l.head = r.at(lane);
+    const int tail = r.pieces() - 1;  // not whole, and not the head
+    if (tail == whole1 && tail > 0 && tail >= p0 && tail < p0 + kPieces && lane < r.V - r.token(tail)) l.tail = r.at(r.token(tail) + lane);
+    else if (tail == whole1 && tail == 0 && !whole0 && p0 == 0 && lane < r.V) l.tail = r.at(lane);
+}
+
+// A chunk's statistics, by a warp.
+template <typename T>
+__device__ inline ChunkStat chunk_stat(const Row<T> &r, int chunk, const Loaded &l, float c, bool greedy) {
+    constexpr int VE = Row<T>::VE;
+    const int lane = threadIdx.x & 31;
+    const uint4(&w)[kPerLane] = l.w;
+    float most = max_nan(l.head, l.tail);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < kPerLane; ++j)
+            most = max_nan(most, max_nan(max_nan(__uint_as_float(w[j].x), __uint_as_float(w[j].y)), max_nan(__uint_as_float(w[j].z), __uint_as_float(w[j].w))));
+    } else {
+        uint32_t m = 0xff80ff80u;
+#pragma unroll
+        for (int j = 0; j < kPerLane; ++j) m = max_nan_pair(m, max_nan_pair(max_nan_pair(w[j].x, w[j].y), max_nan_pair(w[j].z, w[j].w)));
+        most = max_nan(most, max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u)));
+    }
+    most = warp_max_nan(most);
+    uint64_t sum[2] = {0, 0};
     int at = 0x7fffffff;
-    bool bad = false;
+    if (most > -INFINITY && most < INFINITY) {
+        const uint64_t minus = two(-most, -most), cc = two(c, c);
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int t0 = r.token(chunk * (kChunk / VE) + j * kThreads + (int)threadIdx.x);
+        for (int j = 0; j < kPerLane; ++j) {
+            float v[VE];
+            Row<T>::values(w[j], v);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            bad = bad || !(v[j][i] < INFINITY);
-            if (v[j][i] > most) most = v[j][i], at = t0 + i;
+            for (int i = 0; i < VE; i += 2) sum[i / 2 & 1] = add_two(sum[i / 2 & 1], weight_two(v[i], v[i + 1], minus, cc));
+        }
+        sum[0] = add_two(sum[0], weight_two(l.head, l.tail, minus, cc));
+        if (greedy) {
+            if (l.tail == most) at = r.token(r.pieces() - 1) + lane;
+#pragma unroll
+            for (int j = kPerLane - 1; j >= 0; --j) {
+                float v[VE];
+                Row<T>::values(w[j], v);
+                const int t0 = r.token(chunk * kPieces + j * 32 + lane);
+#pragma unroll
+                for (int i = VE - 1; i >= 0; --i)
+                    if (v[i] == most) at = t0 + i;
+            }
+            if (l.head == most) at = lane;
+            at = __reduce_min_sync(0xffffffffu, at);
         }
     }
+    const uint64_t both = add_two(sum[0], sum[1]);
+    float s = first_of(both) + second_of(both);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, most, off);
-        const int i = __shfl_xor_sync(0xffffffffu, at, off);
-        if (m > most || (m == most && i < at)) most = m, at = i;
-    }
-    if (__any_sync(0xffffffffu, bad)) most = qnan_f32();
-    if (lane == 0) most_s[warp] = most, at_s[warp] = at;
-    __syncthreads();
-    most = most_s[0], at = at_s[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) {
-        const float m = most_s[w];
-        if (m != m || m > most || (m == most && at_s[w] < at)) most = m, at = at_s[w];
-    }
-    float sum = 0.f;
-    if (most > -INFINITY) {
-#pragma unroll
-        for (int j = 0; j < NP; ++j)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) sum += exp2_fast((v[j][i] - most) * c);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (lane == 0) sum_s[warp] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double total = 0;
-        for (int w = 0; w < kWarps; ++w) total += (double)sum_s[w];
-        *out = ChunkStat{total, most, at};
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    return ChunkStat{(double)s, most, at};
+}
+
+// The warps' chunks: an equal run of all rows' each, the next chunk asked for ahead of the work on one.
+template <typename T>
+__device__ inline void stats_run(const VerifyArgs &a, const void *base, int64_t ld, ChunkStat *out, bool drafter) {
+    const int lane = threadIdx.x & 31, n = (a.V + Row<T>::VE - 1 + Row<T>::kChunk - 1) / Row<T>::kChunk;  // of a row that begins at a piece's last token
+    const int64_t units = (int64_t)a.T * n, warps = (int64_t)gridDim.x * (kStatThreads / 32), w = (int64_t)blockIdx.x * (kStatThreads / 32) + (threadIdx.x >> 5);
+    const int64_t lo = units * w / warps, hi = units * (w + 1) / warps;
+    if (lo >= hi) return;
+    int row = (int)(lo / n), chunk = (int)(lo % n);
+    Loaded now, next;
+    load_chunk(Row<T>(base, ld, row, a.V), chunk, now);
+    float c = kLog2e;
+    bool greedy = false, wanted = true;
+    int known = -1;
+    for (int64_t i = lo; i < hi; ++i) {
+        int row2 = row, chunk2 = chunk + 1;
+        if (chunk2 == n) ++row2, chunk2 = 0;
+        if (i + 1 < hi) load_chunk(Row<T>(base, ld, row2, a.V), chunk2, next);
+        if (row != known) {
+            known = row;
+            if (a.temperature != nullptr || drafter) {
+                const int b = sequence_of(a.q_start, a.B, row);
+                const float t = b >= 0 && a.temperature != nullptr ? a.temperature[b] : 1.f;
+                wanted = b >= 0 && !(drafter && (row + 1 == a.q_start[b + 1] || t == 0.f));  // a sequence's last row has no draft behind it, a greedy one's drafter is not asked
+                c = exponent_scale(t), greedy = t == 0.f;
+            }
+        }
+        if (wanted) {
+            const ChunkStat s = chunk_stat<T>(Row<T>(base, ld, row, a.V), chunk, now, c, greedy);
+            if (lane == 0) out[(int64_t)row * a.pitch + chunk] = s;
+        }
+        row = row2, chunk = chunk2, now = next;
     }
 }
 
 template <typename TX, typename TD>
-__global__ void __launch_bounds__(kThreads) verify_stats_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kStatThreads, kStatCtas) verify_stats_kernel(const VerifyArgs a) {
     behind_grid();
-    const int64_t row = blockIdx.x / a.n_chunks;
-    const int chunk = (int)(blockIdx.x % a.n_chunks);
-    ChunkStat *const out = a.stats + (blockIdx.y * (int64_t)a.T + row) * a.n_chunks + chunk;
-    if (blockIdx.y == 0) chunk_stats<TX>(a, a.logits, a.ld, row, chunk, out);
-    else chunk_stats<TD>(a, a.draft, a.draft_ld, row, chunk, out);
+    if (blockIdx.y == 0) stats_run<TX>(a, a.logits, a.ld, a.stats, false);
+    else stats_run<TD>(a, a.draft, a.draft_ld, a.stats + (int64_t)a.T * a.pitch, true);
 }
+
+// log2 of 2^(c (x - best)), exact but for FP64's rounding.
+__device__ inline double exponent(float x, float best, float c) { return ((double)x - (double)best) * (double)c; }
 
 // A chunk's sum in units of 2^(c best) of its row.  A chunk whose largest term is below 2^-126 there counts as none, so that whatever chunk is chosen has a
 // term that FP32 holds.
 __device__ inline double chunk_weight(const ChunkStat &s, float c, float best) {
-    const double off = ((double)s.best - (double)best) * (double)c;  // -inf: nothing in it
-    return off < -126.0 ? 0.0 : s.sum * exp2(off);
+    const double off = exponent(s.best, best, c);  // -inf: nothing in it
+    return off < -126.0 ? 0.0 : s.sum * (double)exp2_fast((float)off);
+}
+__device__ inline double warp_sum(double v) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+}
+// The sum over this and the lanes below.
+__device__ inline double warp_upto(double v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, v, off);
+        if (lane >= off) v += o;
+    }
+    return v;
 }
 
-// A row's chunks joined, the sum in units of 2^(c best).  By a whole warp.
+// A row's chunks joined, the sum in units of 2^(c best).  By a whole warp; a lane asks for several chunks at once.
 struct RowStat {
     double sum;
     float best;
     int at, code;
 };
 __device__ inline RowStat join_chunks(const ChunkStat *s, int n, float c, int bad_code) {
+    constexpr int kHeld = 5;  // of 160 chunks: 163,840 logits in FP32 and twice as many in BF16
     const int lane = threadIdx.x & 31;
+    ChunkStat held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = 32 * i + lane < n ? s[32 * i + lane] : ChunkStat{0.0, -INFINITY, 0x7fffffff};
     float best = -INFINITY;
     int at = 0x7fffffff;
-    bool bad = false;
-    for (int k = lane; k < n; k += 32) {
-        const float m = s[k].best;
-        bad = bad || m != m;
-        if (m > best) best = m, at = s[k].at;
-    }
+    auto larger = [&](const ChunkStat &k) {
+        if (k.best > best) at = k.at;  // the first of those that are as large
+        best = max_nan(best, k.best);
+    };
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, best, off);
-        const int i = __shfl_xor_sync(0xffffffffu, at, off);
-        if (m > best || (m == best && i < at)) best = m, at = i;
-    }
-    RowStat r{0.0, best, at, 0};
-    if (__any_sync(0xffffffffu, bad) || best == -INFINITY) {
+    for (int i = 0; i < kHeld; ++i) larger(held[i]);
+#pragma unroll 1
+    for (int k = 32 * kHeld + lane; k < n; k += 32) larger(s[k]);
+    const float most = warp_max_nan(best);
+    RowStat r{0.0, most, (int)__reduce_min_sync(0xffffffffu, best == most ? at : 0x7fffffff), 0};
+    if (!(most > -INFINITY && most < INFINITY)) {
         r.code = bad_code;
         return r;
     }
     double sum = 0;
-    for (int k = lane; k < n; k += 32) sum += chunk_weight(s[k], c, best);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    r.sum = sum;
+    for (int i = 0; i < kHeld; ++i) sum += chunk_weight(held[i], c, most);
+#pragma unroll 1
+    for (int k = 32 * kHeld + lane; k < n; k += 32) sum += chunk_weight(s[k], c, most);
+    r.sum = warp_sum(sum);
     return r;
 }
 
-// What is drawn from: weights of the tokens of a piece.
+// What is drawn from: weights of a piece's tokens.
 template <typename TX>
 struct OfTarget {  // 2^(c (x - best)), nothing for the token `without`
     Row<TX> r;
@@ -210,10 +327,9 @@ struct OfTarget {  // 2^(c (x - best)), nothing for the token `without`
     static constexpr int VE = Row<TX>::VE;
     __device__ inline int token(int piece) const { return r.token(piece); }
     __device__ inline void weights(int piece, float (&w)[VE]) const {
-        const int t0 = r.token(piece);
-        r.load(t0, w);
+        Row<TX>::values(r.raw(piece), w);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = t0 + i == without ? 0.f : exp2_fast((w[i] - best) * c);
+        for (int i = 0; i < VE; ++i) w[i] = r.token(piece) + i == without ? 0.f : exp2_fast((w[i] - best) * c);
     }
 };
 template <typename TX, typename TD>
@@ -224,140 +340,143 @@ struct OfDifference {  // max(p - q, 0)
     static constexpr int VE = Row<TX>::VE;
     __device__ inline int token(int piece) const { return r.token(piece); }
     __device__ inline void weights(int piece, float (&w)[VE]) const {
-        const int t0 = r.token(piece);
-        r.load(t0, w);
         float d[VE];
-        if constexpr (Row<TD>::VE == VE) q.load(t0, d);
-        else
+        const int t0 = r.token(piece);
+        if (sizeof(TX) == sizeof(TD) && r.mis == q.mis) {  // the rows' pieces hold the same tokens
+            const uint4 x = r.raw(piece), y = q.raw(piece);
+            Row<TX>::values(x, w), Row<TX>::values(y, d);
+        } else {
+            Row<TX>::values(r.raw(piece), w);
 #pragma unroll
             for (int i = 0; i < VE; ++i) d[i] = t0 + i >= 0 && t0 + i < q.V ? q.at(t0 + i) : -INFINITY;
+        }
 #pragma unroll
         for (int i = 0; i < VE; ++i) w[i] = fmaxf(exp2_fast((w[i] - best) * c) * inv - exp2_fast((d[i] - q_best) * c) * q_inv, 0.f);
     }
 };
+template <int N>
+__device__ inline float sum_of(const float (&w)[N]) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) s += w[k];
+    return s;
+}
 
-// The pieces lo .. hi - 1 summed, by a warp.
+// Drawing, by all threads of a CTA: these have parts that lie one behind the other.
+struct Draw {
+    double warp_s[kWarps];
+    int first, last;
+};
+// The sum over this and the threads before; the whole sum in *all.
+__device__ inline double block_upto(Draw &sh, double v, double *all) {
+    const int warp = threadIdx.x >> 5;
+    double upto = warp_upto(v), sum = 0;
+    __syncthreads();  // what was there before has been read
+    if ((threadIdx.x & 31) == 31) sh.warp_s[warp] = upto;
+    if (threadIdx.x == 0) sh.first = kThreads, sh.last = -1;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) upto += sum;
+        sum += sh.warp_s[w];
+    }
+    *all = sum;
+    return upto;
+}
+// After block_upto: the thread in whose part `target` falls, the last one that has any if rounding leaves none.
+__device__ inline int block_find(Draw &sh, double mine, double upto, double target) {
+    const uint32_t over = __ballot_sync(0xffffffffu, mine > 0 && upto > target), some = __ballot_sync(0xffffffffu, mine > 0);
+    if ((threadIdx.x & 31) == 0) {
+        if (over) atomicMin(&sh.first, (int)threadIdx.x + __ffs(over) - 1);
+        if (some) atomicMax(&sh.last, (int)threadIdx.x + 31 - __clz(some));
+    }
+    __syncthreads();
+    return sh.first < kThreads ? sh.first : sh.last;
+}
+// The first token of a piece up to which more than `target` has come, the last one with a weight if rounding leaves none.
 template <typename F>
-__device__ inline double sum_pieces(const F &f, int lo, int hi) {
-    const int lane = threadIdx.x & 31;
+__device__ inline int pick_in_piece(const F &f, int piece, double target) {
+    float w[F::VE];
+    f.weights(piece, w);
     double sum = 0;
-    for (int i = lo + lane; i < hi; i += 32) {
-        float w[F::VE];
-        f.weights(i, w);
-        float s = 0.f;
+    int token = -1;
+    bool found = false;
 #pragma unroll
-        for (int k = 0; k < F::VE; ++k) s += w[k];
-        sum += (double)s;
+    for (int k = 0; k < F::VE; ++k) {
+        sum += (double)w[k];
+        if (!found && w[k] > 0.f) token = f.token(piece) + k, found = sum > target;
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    return sum;
+    return token;
 }
-// The first token of these pieces up to which more than `target` has come; the last one with a weight if rounding leaves none.  By a warp, at least one weight is not zero.
-template <typename F>
-__device__ inline int pick_in_pieces(const F &f, int lo, int hi, double target) {
-    const int lane = threadIdx.x & 31;
-    double before = 0;
-    int last = -1;
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const int i = i0 + lane;
-        float w[F::VE];
-#pragma unroll
-        for (int k = 0; k < F::VE; ++k) w[k] = 0.f;
-        if (i < hi) f.weights(i, w);
-        double mine = 0, upto;
-        int my_last = -1;
-#pragma unroll
-        for (int k = 0; k < F::VE; ++k) {
-            mine += (double)w[k];
-            if (w[k] > 0.f) my_last = f.token(i) + k;
-        }
-        upto = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const double o = __shfl_up_sync(0xffffffffu, upto, off);
-            if (lane >= off) upto += o;
-        }
-        const uint32_t over = __ballot_sync(0xffffffffu, mine > 0 && before + upto > target);
-        if (over) {
-            const int src = __ffs(over) - 1;
-            int token = my_last;
-            double sum = before + (upto - mine);
-#pragma unroll
-            for (int k = F::VE - 1; k >= 0; --k) {  // from the end: the first that is over is the last one written
-                double s = sum;
-#pragma unroll
-                for (int m = 0; m <= k; ++m) s += (double)w[m];
-                if (w[k] > 0.f && s > target) token = f.token(i) + k;
-            }
-            return __shfl_sync(0xffffffffu, token, src);
-        }
-        const uint32_t some = __ballot_sync(0xffffffffu, my_last >= 0);
-        if (some) last = __shfl_sync(0xffffffffu, my_last, 31 - __clz(some));
-        before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    return last;
-}
-
-// log2 of 2^(c (x - best)), exact but for FP64's rounding.
-__device__ inline double exponent(float x, float best, float c) { return ((double)x - (double)best) * (double)c; }
 
 struct Decision {
     RowStat p, q;
-    double logp;
+    float x;                // the drafted token's logit
     int token, keep, code;  // the drafted token behind the row; keep: 1 kept, 0 not, -1 there is none
 };
+__device__ inline float log_probability(float x, const RowStat &p, float c) { return (float)(exponent(x, p.best, c) * kLn2) - logf((float)p.sum); }
 
 template <typename TX, typename TD, bool DRAFT>
-__global__ void __launch_bounds__(kThreads) verify_decide_kernel(const VerifyArgs a) {
-    behind_grid();
+__global__ void __launch_bounds__(kThreads, DRAFT ? 4 : 2) verify_decide_kernel(const VerifyArgs a) {
     __shared__ Decision dec[kWarps];
-    __shared__ double part_s[kWarps], all_s[kWarps * kRanks];
-    __shared__ int chosen_s[2];
-    __shared__ double from_s;
+    __shared__ Draw draw;
+    __shared__ double total_s, from_s;
+    __shared__ int chunk_s;
+    __shared__ float run_s[DRAFT ? kMaxRun * kWarps : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = DRAFT ? (int)(blockIdx.x % kRanks) : 0, b = DRAFT ? (int)(blockIdx.x / kRanks) : (int)blockIdx.x;
+    // The caller's arrays were complete before the launch ahead, the first of the two, began its work: they are read ahead of its end.
     const int first = a.q_start[b], end = a.q_start[b + 1];
+    const float t = a.temperature != nullptr ? a.temperature[b] : 1.f, u_pick = a.u_pick[b], c = exponent_scale(t);
     bool falls = false;
     for (int i = threadIdx.x; i < b; i += kThreads) falls = falls || a.q_start[i] > first;
-    if (__syncthreads_or(falls) || first < 0 || end < first || end > a.T) {
-        if (rank == 0 && threadIdx.x == 0) a.n_new[b] = 0, raise_error(a.err, (uint32_t)b, kBadRange);
+    falls = __syncthreads_or(falls);
+    if (falls || first < 0 || end < first || end > a.T || first == end) {
+        behind_grid();
+        if (rank == 0 && threadIdx.x == 0) {
+            a.n_new[b] = 0;
+            if (falls || first != end || first < 0 || end > a.T) raise_error(a.err, (uint32_t)b, kBadRange);
+        }
         return;
     }
-    if (first == end) {
-        if (rank == 0 && threadIdx.x == 0) a.n_new[b] = 0;
-        return;
-    }
-    const float t = a.temperature != nullptr ? a.temperature[b] : 1.f, c = exponent_scale(t);
     const bool greedy = t == 0.f;
     int code = t == 0.f || (t >= 0x1p-126f && t < INFINITY) ? 0 : kBadTemperature, bad_row = first, stop = first;
     Decision d{};
     // ---- rows in order, a warp a row, up to the first whose draft is not kept
-    for (int r0 = first; code == 0; r0 += kWarps) {
+#pragma unroll 1
+    for (int r0 = first;; r0 += kWarps) {
         const int row = r0 + warp;
+        Decision e{};
+        e.keep = -1;
+        float u = 0.f, qx = 0.f;
+        if (row + 1 < end) {
+            e.token = a.ids[row + 1];
+            u = a.u[row];
+            if (e.token < 0 || e.token >= a.V) e.code = kBadId;
+            else {
+                e.x = Row<TX>(a.logits, a.ld, row, a.V).at(e.token);
+                if constexpr (DRAFT) qx = Row<TD>(a.draft, a.draft_ld, row, a.V).at(e.token);
+            }
+        }
+        if (r0 == first) behind_grid();
+        if (code != 0) break;
         if (row < end) {
-            Decision e{};
-            const Row<TX> x(a.logits, a.ld, row, a.V);
-            e.p = join_chunks(a.stats + (int64_t)row * a.n_chunks, a.n_chunks, c, kBadLogits);
-            e.code = e.p.code;
-            e.keep = -1;
+            const int bad_id = e.code;
+            e.p = join_chunks(a.stats + (int64_t)row * a.pitch, Row<TX>(a.logits, a.ld, row, a.V).chunks(), c, kBadLogits);
+            e.code = e.p.code != 0 ? e.p.code : bad_id;
             if (row + 1 < end && e.code == 0) {
-                e.token = a.ids[row + 1];
-                if (e.token < 0 || e.token >= a.V) e.code = kBadId;
-                else if (greedy) e.keep = e.token == e.p.at;
+                if (greedy) e.keep = e.token == e.p.at;
                 else {
-                    const float u = a.u[row];
-                    double q = 1.0;
+                    // u q < p without the divisions: u 2^.. P < 2^.. Q
+                    double q = 1.0, q_sum = 1.0;
                     if (!(u >= 0.f && u < 1.f)) e.code = kBadRandom;
                     if constexpr (DRAFT) {
-                        e.q = join_chunks(a.stats + ((int64_t)a.T + row) * a.n_chunks, a.n_chunks, c, kBadDraft);
+                        e.q = join_chunks(a.stats + ((int64_t)a.T + row) * a.pitch, Row<TD>(a.draft, a.draft_ld, row, a.V).chunks(), c, kBadDraft);
                         if (e.code == 0) e.code = e.q.code;
-                        if (e.code == 0) q = exp2(exponent(Row<TD>(a.draft, a.draft_ld, row, a.V).at(e.token), e.q.best, c)) / e.q.sum;
+                        if (e.code == 0) q = (double)exp2_fast((float)exponent(qx, e.q.best, c)), q_sum = e.q.sum;
                     }
-                    const double p = exp2(exponent(x.at(e.token), e.p.best, c)) / e.p.sum;
-                    e.keep = (double)u * q < p;
+                    if (e.code == 0) e.keep = (double)u * q * e.p.sum < (double)exp2_fast((float)exponent(e.x, e.p.best, c)) * q_sum;
                 }
-                if (e.code == 0) e.logp = exponent(x.at(e.token), e.p.best, c) * kLn2 - log(e.p.sum);
             }
             if (lane == 0) dec[warp] = e;
         }
@@ -369,23 +488,19 @@ __global__ void __launch_bounds__(kThreads) verify_decide_kernel(const VerifyArg
             else if (dec[n].keep != 1) d = dec[n], done = true;
             else ++n;
         }
-        if (rank == 0 && (int)threadIdx.x < n) {
-            a.next_ids[r0 + threadIdx.x] = dec[threadIdx.x].token;
-            if (a.logp != nullptr) a.logp[r0 + threadIdx.x] = (float)dec[threadIdx.x].logp;
+        if (rank == 0 && warp < n && lane == 0) {
+            a.next_ids[row] = e.token;
+            if (a.logp != nullptr) a.logp[row] = log_probability(e.x, e.p, c);
         }
         stop = r0 + n;
         __syncthreads();
         if (done) break;
     }
-    float u = 0.f;
-    if (code == 0 && !greedy) {
-        u = a.u_pick[b];
-        if (!(u >= 0.f && u < 1.f)) code = kBadRandom, bad_row = stop;
-    }
+    if (code == 0 && !greedy && !(u_pick >= 0.f && u_pick < 1.f)) code = kBadRandom, bad_row = stop;
     if (code != 0) {
         if (rank == 0) {
             if (threadIdx.x == 0) a.n_new[b] = 0, raise_error(a.err, (uint32_t)bad_row, (uint32_t)code);
-            for (int i = first + (int)threadIdx.x; i < end; i += kThreads) {
+            for (int i = first + (int)threadIdx.x; i < end; i += kThreads) {  // those of the rows before too, written ahead of the last barrier
                 a.next_ids[i] = -1;
                 if (a.logp != nullptr) a.logp[i] = qnan_f32();
             }
@@ -400,116 +515,128 @@ __global__ void __launch_bounds__(kThreads) verify_decide_kernel(const VerifyArg
         }
     }
     const Row<TX> x(a.logits, a.ld, stop, a.V);
+    const int n = x.chunks();
     auto say = [&](int token) {  // one thread
         a.next_ids[stop] = token;
-        if (a.logp != nullptr) a.logp[stop] = (float)(exponent(x.at(token), d.p.best, c) * kLn2 - log(d.p.sum));
+        if (a.logp != nullptr) a.logp[stop] = log_probability(x.at(token), d.p, c);
     };
     if (greedy) {
         if (rank == 0 && threadIdx.x == 0) say(d.p.at);
         return;
     }
-    // ---- from the difference of two distributions: the cluster's warps have a run of the row each
+    double all;
+    // ---- from the difference of two distributions: the cluster's CTAs have a run of the row's chunks each, a warp an eighth of every chunk, a thread a piece of it
     if (DRAFT && d.keep == 0) {
         namespace cg = cooperative_groups;
         cg::cluster_group cluster = cg::this_cluster();
         const OfDifference<TX, TD> f{x, Row<TD>(a.draft, a.draft_ld, stop, a.V), c, d.p.best, (float)(1.0 / d.p.sum), d.q.best, (float)(1.0 / d.q.sum)};
-        const int pieces = x.pieces(), run = (pieces + kWarps * kRanks - 1) / (kWarps * kRanks), lo = (rank * kWarps + warp) * run, hi = min(pieces, lo + run);
-        const double mine = sum_pieces(f, lo, hi);
-        if (lane == 0) part_s[warp] = mine;
+        const int lo = n * rank / kRanks, parts = (n * (rank + 1) / kRanks - lo) * kWarps;
+#pragma unroll 4
+        for (int k = warp; k < parts; k += kWarps) {
+            float w[Row<TX>::VE];
+            f.weights((lo + k / kWarps) * kPieces + (int)threadIdx.x, w);
+            float s = sum_of(w);
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+            if (lane == 0) run_s[k] = s;
+        }
+        __syncthreads();
+        const int per = (parts + kThreads - 1) / kThreads, k0 = min(parts, (int)threadIdx.x * per), k1 = min(parts, k0 + per);
+        double mine = 0;
+        for (int k = k0; k < k1; ++k) mine += (double)run_s[k];
+        const double upto = block_upto(draw, mine, &all);
+        if (threadIdx.x == 0) total_s = all;
         cluster.sync();
-        if (threadIdx.x < kWarps * kRanks) all_s[threadIdx.x] = *cluster.map_shared_rank(&part_s[threadIdx.x % kWarps], threadIdx.x / kWarps);
-        cluster.sync();  // nobody's part is read from here on
-        double total = 0;
-        for (int i = 0; i < kWarps * kRanks; ++i) total += all_s[i];
+        double before = 0, total = 0, from = 0;
+        int owner = -1;
+        double sums[kRanks];
+        for (int k = 0; k < kRanks; ++k) sums[k] = *cluster.map_shared_rank(&total_s, k), total += sums[k];
+        cluster.sync();  // nobody's sum is read from here on
         if (total > 0) {
-            const double target = (double)u * total;
-            double before = 0, from = 0;
-            int at = -1;
-            for (int i = 0; i < kWarps * kRanks; ++i) {
-                if (all_s[i] > 0) at = i, from = before;
-                before += all_s[i];
-                if (at == i && before > target) break;
+            const double target = (double)u_pick * total;
+            bool found = false;
+            for (int k = 0; k < kRanks; ++k) {
+                if (!found && sums[k] > 0) owner = k, from = before, found = before + sums[k] > target;
+                before += sums[k];
             }
-            if (at == rank * kWarps + warp) {
-                const int token = pick_in_pieces(f, lo, hi, target - from);
-                if (lane == 0) say(token);
+            if (owner != rank) return;
+            if (block_find(draw, mine, upto, target - from) == (int)threadIdx.x) {
+                double sum = upto - mine, at_from = sum;
+                int at = k0;
+                found = false;
+                for (int k = k0; k < k1; ++k) {
+                    if (!found && run_s[k] > 0.f) at = k, at_from = sum, found = sum + (double)run_s[k] > target - from;
+                    sum += (double)run_s[k];
+                }
+                chunk_s = at, from_s = target - from - at_from;
             }
+            __syncthreads();
+            if (warp != 0) return;
+            const int piece = (lo + chunk_s / kWarps) * kPieces + chunk_s % kWarps * 32 + lane;
+            float w[Row<TX>::VE];
+            f.weights(piece, w);
+            const double part = (double)sum_of(w), sofar = warp_upto(part);
+            const uint32_t over = __ballot_sync(0xffffffffu, part > 0 && sofar > from_s), some = __ballot_sync(0xffffffffu, part > 0);
+            if (lane == (over ? __ffs(over) - 1 : 31 - __clz(some))) say(pick_in_piece(f, piece, from_s - (sofar - part)));
             return;
         }
     }
     if (rank != 0) return;
     // ---- from the target's distribution, without the refused token where the drafter gave no more than that
-    constexpr int VE = Row<TX>::VE, kPieces = kChunk / VE, kRun = kPieces / kWarps;
-    const ChunkStat *const s = a.stats + (int64_t)stop * a.n_chunks;
+    const ChunkStat *const s = a.stats + (int64_t)stop * a.pitch;
     OfTarget<TX> f{x, c, d.p.best, -1};
-    auto chunk_parts = [&](int chunk) {
-        const int lo = chunk * kPieces + warp * kRun;
-        const double mine = sum_pieces(f, lo, min(x.pieces(), lo + kRun));
-        __syncthreads();
-        if (lane == 0) part_s[warp] = mine;
-        __syncthreads();
-    };
     int refused = -1;
     double rest = 0;
     if (!DRAFT && d.keep == 0) {
-        f.without = d.token;
-        refused = (d.token + x.mis) / kChunk;
-        chunk_parts(refused);
-        for (int w = 0; w < kWarps; ++w) rest += part_s[w];
+        f.without = d.token, refused = (d.token + x.mis) / Row<TX>::kChunk;
+        float w[Row<TX>::VE];
+        f.weights(refused * kPieces + (int)threadIdx.x, w);
+        block_upto(draw, (double)sum_of(w), &rest);
     }
-    if (warp == 0) {
-        auto of = [&](int k) { return k >= a.n_chunks ? 0.0 : k == refused ? rest : chunk_weight(s[k], c, d.p.best); };
-        double total = 0;
-        for (int k0 = 0; k0 < a.n_chunks; k0 += 32) total += of(k0 + lane);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-        if (!(total > 0)) {  // nothing but the refused token: from all of it
-            refused = -1, total = d.p.sum;
-            if (lane == 0) chosen_s[1] = 1;
-        } else if (lane == 0) chosen_s[1] = 0;
-        const double target = (double)u * total;
-        double before = 0, from = 0;
-        int at = -1;
-        for (int k0 = 0; k0 < a.n_chunks; k0 += 32) {
-            const double mine = of(k0 + lane);
-            double upto = mine;
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const double o = __shfl_up_sync(0xffffffffu, upto, off);
-                if (lane >= off) upto += o;
-            }
-            const uint32_t over = __ballot_sync(0xffffffffu, mine > 0 && before + upto > target), some = __ballot_sync(0xffffffffu, mine > 0);
-            const int src = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : -1;
-            if (src >= 0) at = k0 + src, from = before + __shfl_sync(0xffffffffu, upto - mine, src);
-            if (over) break;
-            before += __shfl_sync(0xffffffffu, upto, 31);
+    // chunks: a thread's run of them, one behind the other
+    const int per = (n + kThreads - 1) / kThreads, k0 = min(n, (int)threadIdx.x * per), k1 = min(n, k0 + per);
+    double mine = 0, upto;
+#pragma unroll 1
+    for (int again = 0;; ++again) {
+        mine = 0;
+        for (int k = k0; k < k1; ++k) mine += k == refused ? rest : chunk_weight(s[k], c, d.p.best);
+        upto = block_upto(draw, mine, &all);
+        if (all > 0 || again) break;
+        refused = -1, f.without = -1;  // nothing but the refused token: from all of it
+    }
+    double target = (double)u_pick * all;
+    if (block_find(draw, mine, upto, target) == (int)threadIdx.x) {
+        double sum = upto - mine, from = sum;
+        int at = k0;
+        bool found = false;
+        for (int k = k0; k < k1; ++k) {
+            const double w = k == refused ? rest : chunk_weight(s[k], c, d.p.best);
+            if (!found && w > 0) at = k, from = sum, found = sum + w > target;
+            sum += w;
         }
-        if (lane == 0) chosen_s[0] = at, from_s = target - from;
+        chunk_s = at, from_s = target - from;
     }
     __syncthreads();
-    if (chosen_s[1]) f.without = -1;
-    const int chunk = chosen_s[0];
-    double target = from_s;
-    chunk_parts(chunk);
-    double from = 0, before = 0;
-    int at = -1;
-    for (int w = 0; w < kWarps; ++w) {
-        if (part_s[w] > 0) at = w, from = before;
-        before += part_s[w];
-        if (at == w && before > target) break;
-    }
-    if (warp == at) {
-        const int lo = chunk * kPieces + warp * kRun, token = pick_in_pieces(f, lo, min(x.pieces(), lo + kRun), target - from);
-        if (lane == 0) say(token);
-    }
+    // pieces of the chunk: one a thread
+    const int piece = chunk_s * kPieces + (int)threadIdx.x;
+    target = from_s;
+    float w[Row<TX>::VE];
+    f.weights(piece, w);
+    mine = (double)sum_of(w);
+    upto = block_upto(draw, mine, &all);
+    if (block_find(draw, mine, upto, target) == (int)threadIdx.x) say(pick_in_piece(f, piece, target - (upto - mine)));
 }
 
-int64_t chunks(int64_t V) { return (V + 7 + kChunk - 1) / kChunk; }  // a row may begin up to seven tokens inside a piece
+// Chunks of a row of FP32 that begins at a piece's last token: no row has more.
+int64_t most_chunks(int64_t V) { return (V + 3 + 4 * kPieces - 1) / (4 * kPieces); }
 
 template <typename TX, typename TD>
 cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t st) {
     const bool draft = a.draft != nullptr;
-    const cudaError_t e = launch_behind(verify_stats_kernel<TX, TD>, dim3((unsigned)((int64_t)a.T * a.n_chunks), draft ? 2 : 1), dim3(kThreads), 0, st, 1, a);
+    // a warp a chunk until the machine is full
+    const int64_t chunks = (int64_t)a.T * ((a.V + 4 * kPieces - 1) / (4 * kPieces)), per = kStatThreads / 32;
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((chunks + per - 1) / per, (int64_t)sm_count() * kStatCtas));
+    const cudaError_t e = launch_behind(verify_stats_kernel<TX, TD>, dim3(grid, draft ? 2 : 1), dim3(kStatThreads), 0, st, 1, a);
     if (e != cudaSuccess) return e;
     return draft ? launch_behind(verify_decide_kernel<TX, TD, true>, dim3((unsigned)(a.B * kRanks)), dim3(kThreads), 0, st, kRanks, a)
                  : launch_behind(verify_decide_kernel<TX, TD, false>, dim3((unsigned)a.B), dim3(kThreads), 0, st, 1, a);
@@ -523,11 +650,11 @@ using namespace sxb;
 extern "C" {
 
 size_t sxb_verify_drafts_workspace_bytes(int64_t T, int64_t B, int64_t V) {
-    if (!(T >= 1 && T <= (1 << 20) && B >= 1 && B <= (1 << 20) && V >= 1 && V <= (1 << 20))) {
-        fail_check(SXB_FILE_, __LINE__, __func__, "1 <= T, B, V <= 2^20", cat("verify_drafts_workspace_bytes: T = ", T, ", B = ", B, ", V = ", V));
+    if (!(T >= 1 && T <= (1 << 20) && B >= 1 && B <= kMaxB && V >= 1 && V <= kMaxV)) {
+        fail_check(SXB_FILE_, __LINE__, __func__, "1 <= T, V <= 2^20, 1 <= B <= 8192", cat("verify_drafts_workspace_bytes: T = ", T, ", B = ", B, ", V = ", V));
         return 0;
     }
-    return (size_t)(2 * T * chunks(V)) * sizeof(ChunkStat);
+    return (size_t)(2 * T * most_chunks(V)) * sizeof(ChunkStat);
 }
 
 int sxb_verify_drafts(const SxbVerifyDraftsArgs *args, sxb_stream_t stream) {
@@ -535,7 +662,8 @@ int sxb_verify_drafts(const SxbVerifyDraftsArgs *args, sxb_stream_t stream) {
     SXB_CHECK(args != nullptr, fn, ": null argument block");
     const SxbVerifyDraftsArgs &g = *args;
     const int64_t T = g.T, V = g.V, B = g.B;
-    SXB_CHECK(T >= 1 && T <= (1 << 20) && B >= 1 && B <= (1 << 20) && V >= 1 && V <= (1 << 20), fn, ": T = ", T, " rows, B = ", B, " sequences, V = ", V, " tokens, expected 1..2^20");
+    SXB_CHECK(T >= 1 && T <= (1 << 20) && B >= 1 && B <= kMaxB && V >= 1 && V <= kMaxV, fn, ": T = ", T, " rows, B = ", B, " sequences, V = ", V, " tokens, expected 1..2^20, ",
+              kMaxB, " sequences at most");
     SXB_CHECK(g.logits != nullptr && g.ids != nullptr && g.q_start != nullptr && g.u != nullptr && g.u_pick != nullptr && g.next_ids != nullptr && g.n_new != nullptr &&
                   g.ws != nullptr && g.err != nullptr,
               fn, ": null pointer (logits=", g.logits, ", ids=", (const void *)g.ids, ", q_start=", (const void *)g.q_start, ", u=", (const void *)g.u, ", u_pick=",
@@ -565,7 +693,7 @@ int sxb_verify_drafts(const SxbVerifyDraftsArgs *args, sxb_stream_t stream) {
     VerifyArgs a{};
     a.logits = g.logits, a.draft = g.draft_logits, a.ld = g.ld, a.draft_ld = g.draft_ld, a.ids = g.ids, a.q_start = g.q_start, a.u = g.u, a.u_pick = g.u_pick;
     a.temperature = g.temperature, a.next_ids = g.next_ids, a.n_new = g.n_new, a.logp = g.logp, a.stats = static_cast<ChunkStat *>(g.ws), a.err = g.err;
-    a.T = (int)T, a.V = (int)V, a.B = (int)B, a.n_chunks = (int)chunks(V);
+    a.T = (int)T, a.V = (int)V, a.B = (int)B, a.pitch = (int)most_chunks(V);
     auto st = static_cast<cudaStream_t>(stream);
     const bool x32 = g.act == SXB_ACT_F32, d32 = g.draft_logits != nullptr ? g.draft_act == SXB_ACT_F32 : x32;
     const cudaError_t e = x32 ? (d32 ? launch_verify<float, float>(a, st) : launch_verify<float, uint16_t>(a, st))
