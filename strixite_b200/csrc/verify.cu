@@ -1,8 +1,8 @@
 // Verification of drafted tokens against the target's probabilities, from given random numbers (include/strix_b200.h has the rules).
 //
 // Two launches.  The first reads every row's logits once, a warp a chunk of 4 KB: its largest logit (and, for greedy sequences, the first token that has it) and the sum of 2^(c (x -
-// max)), c = log2(e) / temperature.  What bounds it is memory; a logit takes four to five instructions, one of them the exponential.  The second, a CTA a sequence (a cluster of eight
-// where the drafter gives its distribution), joins a row's chunks, tests the drafts, and draws the next token: from the chunks' sums it knows the chunk in which the random number
+// max)), c = log2(e) / temperature.  What bounds it is memory; a logit takes four to five instructions, one of them the exponential.  The second, a CTA a sequence (a cluster of four or
+// eight where the drafter gives its distribution), joins a row's chunks, tests the drafts, and draws the next token: from the chunks' sums it knows the chunk in which the random number
 // falls and reads that one again; only a difference of two distributions takes the whole row of both, once more, shared by the cluster.  It is bound by its chain of loads, of which
 // those that do not wait for the first launch are made ahead of its end.  Nothing is counted or left behind in the workspace: no atomics, and results do not depend on who comes first.
 //
@@ -10,7 +10,6 @@
 // terms and then seven more in FP32; chunks are joined in FP64, where the exponents are exact, and no logit is too large for them.
 
 #include "common.cuh"
-#include "tc_ptx.cuh"
 
 #include <cooperative_groups.h>
 
@@ -20,9 +19,9 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kStatThreads = 128, kStatCtas = 4;       // of the first kernel; CTAs an SM
 constexpr int kPieces = kThreads, kPerLane = kPieces / 32;  // of sixteen bytes, of a chunk: eight a lane of a warp, or one a thread of a CTA
-constexpr int kRanks = 8;                              // CTAs that share a difference of two rows
+constexpr int kMinRanks = 4, kMaxRanks = 8;            // CTAs that share a difference of two rows
 constexpr int64_t kMaxV = 1 << 20, kMaxB = 8192;
-constexpr int kMaxChunks = (int)(kMaxV / (4 * kPieces)) + 1, kMaxRun = (kMaxChunks + kRanks - 1) / kRanks;  // of a row; of a CTA's share of one
+constexpr int kMaxChunks = (int)(kMaxV / (4 * kPieces)) + 1, kMaxRun = (kMaxChunks + kMinRanks - 1) / kMinRanks;  // of a row; of a CTA's share of one
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994531;
 
@@ -44,6 +43,7 @@ struct VerifyArgs {
     ChunkStat *stats;  // [T (, T of the drafter)][pitch]
     uint32_t *err;
     int T, V, B, pitch;
+    int ranks;  // CTAs of the second kernel that share a difference of two rows
 };
 
 // Tokens are read in pieces of sixteen aligned bytes.  A row may begin inside one: piece i holds the tokens i * VE - mis ..., those outside 0 .. V - 1 are none.
@@ -102,6 +102,12 @@ __device__ inline int sequence_of(const int32_t *q_start, int B, int row) {
     return -1;
 }
 
+// 2^v on the special-function unit, nothing below 2^-126: with the smaller numbers that a weight this far down is not drawn by, it takes four instructions more.
+__device__ inline float exp2_of(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ inline float max_nan(float a, float b) {  // NaN if one is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -137,7 +143,7 @@ __device__ inline float second_of(uint64_t v) { return __uint_as_float((uint32_t
 // 2^(c (x - best)) of two, each with the rounding that one alone has.
 __device__ inline uint64_t weight_two(float x0, float x1, uint64_t minus_best, uint64_t c) {
     const uint64_t e = mul_two(add_two(two(x0, x1), minus_best), c);
-    return two(exp2_fast(first_of(e)), exp2_fast(second_of(e)));
+    return two(exp2_of(first_of(e)), exp2_of(second_of(e)));
 }
 
 // A lane's part of a chunk: piece 32 j + lane is its j-th.  Where the row does not begin or end with a piece, the tokens before the first and behind the last whole one are a lane's each.
@@ -217,9 +223,9 @@ __device__ inline ChunkStat chunk_stat(const Row<T> &r, int chunk, const Loaded 
 
 // The warps' chunks: an equal run of all rows' each, the next chunk asked for ahead of the work on one.
 template <typename T>
-__device__ inline void stats_run(const VerifyArgs &a, const void *base, int64_t ld, ChunkStat *out, bool drafter) {
+__device__ inline void stats_run(const VerifyArgs &a, const void *base, int64_t ld, ChunkStat *out, bool drafter, int block, int blocks) {
     const int lane = threadIdx.x & 31, n = (a.V + Row<T>::VE - 1 + Row<T>::kChunk - 1) / Row<T>::kChunk;  // of a row that begins at a piece's last token
-    const int64_t units = (int64_t)a.T * n, warps = (int64_t)gridDim.x * (kStatThreads / 32), w = (int64_t)blockIdx.x * (kStatThreads / 32) + (threadIdx.x >> 5);
+    const int64_t units = (int64_t)a.T * n, warps = (int64_t)blocks * (kStatThreads / 32), w = (int64_t)block * (kStatThreads / 32) + (threadIdx.x >> 5);
     const int64_t lo = units * w / warps, hi = units * (w + 1) / warps;
     if (lo >= hi) return;
     int row = (int)(lo / n), chunk = (int)(lo % n);
@@ -252,18 +258,20 @@ __device__ inline void stats_run(const VerifyArgs &a, const void *base, int64_t 
 template <typename TX, typename TD>
 __global__ void __launch_bounds__(kStatThreads, kStatCtas) verify_stats_kernel(const VerifyArgs a) {
     behind_grid();
-    if (blockIdx.y == 0) stats_run<TX>(a, a.logits, a.ld, a.stats, false);
-    else stats_run<TD>(a, a.draft, a.draft_ld, a.stats + (int64_t)a.T * a.pitch, true);
+    // half the CTAs have the drafter's rows
+    if (a.draft == nullptr) stats_run<TX>(a, a.logits, a.ld, a.stats, false, (int)blockIdx.x, (int)gridDim.x);
+    else if ((blockIdx.x & 1) == 0) stats_run<TX>(a, a.logits, a.ld, a.stats, false, (int)blockIdx.x / 2, (int)gridDim.x / 2);
+    else stats_run<TD>(a, a.draft, a.draft_ld, a.stats + (int64_t)a.T * a.pitch, true, (int)blockIdx.x / 2, (int)gridDim.x / 2);
 }
 
 // log2 of 2^(c (x - best)), exact but for FP64's rounding.
 __device__ inline double exponent(float x, float best, float c) { return ((double)x - (double)best) * (double)c; }
 
-// A chunk's sum in units of 2^(c best) of its row.  A chunk whose largest term is below 2^-126 there counts as none, so that whatever chunk is chosen has a
-// term that FP32 holds.
+// A chunk's sum in units of 2^(c best) of its row.  A chunk whose largest term is below 2^-125 there counts as none, so that whatever chunk is chosen has a
+// term that FP32 holds (down to 2^-126: exp2_of).
 __device__ inline double chunk_weight(const ChunkStat &s, float c, float best) {
     const double off = exponent(s.best, best, c);  // -inf: nothing in it
-    return off < -126.0 ? 0.0 : s.sum * (double)exp2_fast((float)off);
+    return off < -125.0 ? 0.0 : s.sum * (double)exp2_of((float)off);
 }
 __device__ inline double warp_sum(double v) {
 #pragma unroll
@@ -287,12 +295,17 @@ struct RowStat {
     float best;
     int at, code;
 };
-__device__ inline RowStat join_chunks(const ChunkStat *s, int n, float c, int bad_code) {
-    constexpr int kHeld = 5;  // of 160 chunks: 163,840 logits in FP32 and twice as many in BF16
+constexpr int kHeld = 5;  // of 160 chunks: 163,840 logits in FP32 and twice as many in BF16
+struct Held {
+    ChunkStat k[kHeld];
+};
+__device__ inline void ask_stats(const ChunkStat *s, int n, Held &h) {
     const int lane = threadIdx.x & 31;
-    ChunkStat held[kHeld];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) held[i] = 32 * i + lane < n ? s[32 * i + lane] : ChunkStat{0.0, -INFINITY, 0x7fffffff};
+    for (int i = 0; i < kHeld; ++i) h.k[i] = 32 * i + lane < n ? s[32 * i + lane] : ChunkStat{0.0, -INFINITY, 0x7fffffff};
+}
+__device__ inline RowStat join_chunks(const ChunkStat *s, int n, const Held &h, float c, int bad_code) {
+    const int lane = threadIdx.x & 31;
     float best = -INFINITY;
     int at = 0x7fffffff;
     auto larger = [&](const ChunkStat &k) {
@@ -300,7 +313,7 @@ __device__ inline RowStat join_chunks(const ChunkStat *s, int n, float c, int ba
         best = max_nan(best, k.best);
     };
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) larger(held[i]);
+    for (int i = 0; i < kHeld; ++i) larger(h.k[i]);
 #pragma unroll 1
     for (int k = 32 * kHeld + lane; k < n; k += 32) larger(s[k]);
     const float most = warp_max_nan(best);
@@ -311,7 +324,7 @@ __device__ inline RowStat join_chunks(const ChunkStat *s, int n, float c, int ba
     }
     double sum = 0;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) sum += chunk_weight(held[i], c, most);
+    for (int i = 0; i < kHeld; ++i) sum += chunk_weight(h.k[i], c, most);
 #pragma unroll 1
     for (int k = 32 * kHeld + lane; k < n; k += 32) sum += chunk_weight(s[k], c, most);
     r.sum = warp_sum(sum);
@@ -329,7 +342,7 @@ struct OfTarget {  // 2^(c (x - best)), nothing for the token `without`
     __device__ inline void weights(int piece, float (&w)[VE]) const {
         Row<TX>::values(r.raw(piece), w);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = r.token(piece) + i == without ? 0.f : exp2_fast((w[i] - best) * c);
+        for (int i = 0; i < VE; ++i) w[i] = r.token(piece) + i == without ? 0.f : exp2_of((w[i] - best) * c);
     }
 };
 template <typename TX, typename TD>
@@ -339,19 +352,40 @@ struct OfDifference {  // max(p - q, 0)
     float c, best, inv, q_best, q_inv;
     static constexpr int VE = Row<TX>::VE;
     __device__ inline int token(int piece) const { return r.token(piece); }
+    __device__ inline bool together() const { return sizeof(TX) == sizeof(TD) && r.mis == q.mis; }  // the rows' pieces hold the same tokens
+    __device__ inline void differ(float (&w)[VE], const float (&d)[VE]) const {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[i] = fmaxf(exp2_of((w[i] - best) * c) * inv - exp2_of((d[i] - q_best) * c) * q_inv, 0.f);
+    }
     __device__ inline void weights(int piece, float (&w)[VE]) const {
         float d[VE];
         const int t0 = r.token(piece);
-        if (sizeof(TX) == sizeof(TD) && r.mis == q.mis) {  // the rows' pieces hold the same tokens
-            const uint4 x = r.raw(piece), y = q.raw(piece);
-            Row<TX>::values(x, w), Row<TX>::values(y, d);
-        } else {
-            Row<TX>::values(r.raw(piece), w);
+        Row<TX>::values(r.raw(piece), w);
 #pragma unroll
-            for (int i = 0; i < VE; ++i) d[i] = t0 + i >= 0 && t0 + i < q.V ? q.at(t0 + i) : -INFINITY;
+        for (int i = 0; i < VE; ++i) d[i] = t0 + i >= 0 && t0 + i < q.V ? q.at(t0 + i) : -INFINITY;
+        differ(w, d);
+    }
+    // The weights' sum of one piece each of `N` chunks, kPieces apart, of rows whose pieces hold the same tokens: all are asked for before one is looked at; pieces that are not whole
+    // count as nothing here.
+    template <int N>
+    __device__ inline void sums(int piece, int end, float (&s)[N]) const {
+        const int whole0 = r.mis != 0, whole1 = min(end, (r.V + r.mis) / VE);
+        const uint4 *const xp = reinterpret_cast<const uint4 *>(r.p - r.mis) + piece, *const yp = reinterpret_cast<const uint4 *>(q.p - q.mis) + piece;
+        uint4 x[N], y[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (piece + i * kPieces >= whole0 && piece + i * kPieces < whole1) x[i] = __ldg(xp + i * kPieces), y[i] = __ldg(yp + i * kPieces);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s[i] = 0.f;
+            if (piece + i * kPieces >= whole0 && piece + i * kPieces < whole1) {
+                float w[VE], d[VE];
+                Row<TX>::values(x[i], w), Row<TX>::values(y[i], d);
+                differ(w, d);
+#pragma unroll
+                for (int k = 0; k < VE; ++k) s[i] += w[k];
+            }
         }
-#pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = fmaxf(exp2_fast((w[i] - best) * c) * inv - exp2_fast((d[i] - q_best) * c) * q_inv, 0.f);
     }
 };
 template <int N>
@@ -417,14 +451,14 @@ struct Decision {
 __device__ inline float log_probability(float x, const RowStat &p, float c) { return (float)(exponent(x, p.best, c) * kLn2) - logf((float)p.sum); }
 
 template <typename TX, typename TD, bool DRAFT>
-__global__ void __launch_bounds__(kThreads, DRAFT ? 4 : 2) verify_decide_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) verify_decide_kernel(const VerifyArgs a) {
     __shared__ Decision dec[kWarps];
     __shared__ Draw draw;
     __shared__ double total_s, from_s;
     __shared__ int chunk_s;
     __shared__ float run_s[DRAFT ? kMaxRun * kWarps : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = DRAFT ? (int)(blockIdx.x % kRanks) : 0, b = DRAFT ? (int)(blockIdx.x / kRanks) : (int)blockIdx.x;
+    const int ranks = DRAFT ? a.ranks : 1, rank = (int)blockIdx.x % ranks, b = (int)blockIdx.x / ranks;
     // The caller's arrays were complete before the launch ahead, the first of the two, began its work: they are read ahead of its end.
     const int first = a.q_start[b], end = a.q_start[b + 1];
     const float t = a.temperature != nullptr ? a.temperature[b] : 1.f, u_pick = a.u_pick[b], c = exponent_scale(t);
@@ -461,8 +495,12 @@ __global__ void __launch_bounds__(kThreads, DRAFT ? 4 : 2) verify_decide_kernel(
         if (r0 == first) behind_grid();
         if (code != 0) break;
         if (row < end) {
-            const int bad_id = e.code;
-            e.p = join_chunks(a.stats + (int64_t)row * a.pitch, Row<TX>(a.logits, a.ld, row, a.V).chunks(), c, kBadLogits);
+            const int bad_id = e.code, np = Row<TX>(a.logits, a.ld, row, a.V).chunks(), nq = DRAFT && row + 1 < end ? Row<TD>(a.draft, a.draft_ld, row, a.V).chunks() : 0;
+            const ChunkStat *const ps = a.stats + (int64_t)row * a.pitch, *const qs = ps + (int64_t)a.T * a.pitch;
+            Held hp, hq;
+            ask_stats(ps, np, hp);
+            if constexpr (DRAFT) ask_stats(qs, nq, hq);
+            e.p = join_chunks(ps, np, hp, c, kBadLogits);
             e.code = e.p.code != 0 ? e.p.code : bad_id;
             if (row + 1 < end && e.code == 0) {
                 if (greedy) e.keep = e.token == e.p.at;
@@ -471,11 +509,11 @@ __global__ void __launch_bounds__(kThreads, DRAFT ? 4 : 2) verify_decide_kernel(
                     double q = 1.0, q_sum = 1.0;
                     if (!(u >= 0.f && u < 1.f)) e.code = kBadRandom;
                     if constexpr (DRAFT) {
-                        e.q = join_chunks(a.stats + ((int64_t)a.T + row) * a.pitch, Row<TD>(a.draft, a.draft_ld, row, a.V).chunks(), c, kBadDraft);
+                        e.q = join_chunks(qs, nq, hq, c, kBadDraft);
                         if (e.code == 0) e.code = e.q.code;
-                        if (e.code == 0) q = (double)exp2_fast((float)exponent(qx, e.q.best, c)), q_sum = e.q.sum;
+                        if (e.code == 0) q = (double)exp2_of((float)exponent(qx, e.q.best, c)), q_sum = e.q.sum;
                     }
-                    if (e.code == 0) e.keep = (double)u * q * e.p.sum < (double)exp2_fast((float)exponent(e.x, e.p.best, c)) * q_sum;
+                    if (e.code == 0) e.keep = (double)u * q * e.p.sum < (double)exp2_of((float)exponent(e.x, e.p.best, c)) * q_sum;
                 }
             }
             if (lane == 0) dec[warp] = e;
@@ -530,16 +568,45 @@ __global__ void __launch_bounds__(kThreads, DRAFT ? 4 : 2) verify_decide_kernel(
         namespace cg = cooperative_groups;
         cg::cluster_group cluster = cg::this_cluster();
         const OfDifference<TX, TD> f{x, Row<TD>(a.draft, a.draft_ld, stop, a.V), c, d.p.best, (float)(1.0 / d.p.sum), d.q.best, (float)(1.0 / d.q.sum)};
-        const int lo = n * rank / kRanks, parts = (n * (rank + 1) / kRanks - lo) * kWarps;
-#pragma unroll 4
-        for (int k = warp; k < parts; k += kWarps) {
-            float w[Row<TX>::VE];
-            f.weights((lo + k / kWarps) * kPieces + (int)threadIdx.x, w);
-            float s = sum_of(w);
+        const int lo = n * rank / ranks, hi = n * (rank + 1) / ranks, parts = (hi - lo) * kWarps;
+        auto lanes_sum = [](float s) {
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-            if (lane == 0) run_s[k] = s;
-        }
+            return s;
+        };
+        if (f.together()) {
+            constexpr int kBatch = 4;
+#pragma unroll 1
+            for (int k = lo; k < hi; k += kBatch) {
+                float sums[kBatch];
+                f.sums(k * kPieces + (int)threadIdx.x, hi * kPieces, sums);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const float sum = lanes_sum(sums[i]);
+                    if (lane == 0 && k + i < hi) run_s[(k + i - lo) * kWarps + warp] = sum;
+                }
+            }
+            __syncthreads();
+            // the row's first and last piece, where they are not whole
+            const int last = x.pieces() - 1;
+            for (int i = 0; i < 2; ++i) {
+                const int piece = i ? last : 0, chunk = piece / kPieces;
+                const bool part = i ? (x.V + x.mis) % Row<TX>::VE != 0 && (last > 0 || x.mis == 0) : x.mis != 0;
+                if (part && chunk >= lo && chunk < hi && (int)threadIdx.x == piece % kPieces) {
+                    float w[Row<TX>::VE];
+                    f.weights(piece, w);
+                    run_s[(chunk - lo) * kWarps + warp] += sum_of(w);
+                }
+                __syncwarp();
+            }
+        } else
+#pragma unroll 1
+            for (int k = warp; k < parts; k += kWarps) {
+                float w[Row<TX>::VE];
+                f.weights((lo + k / kWarps) * kPieces + (int)threadIdx.x, w);
+                const float sum = lanes_sum(sum_of(w));
+                if (lane == 0) run_s[k] = sum;
+            }
         __syncthreads();
         const int per = (parts + kThreads - 1) / kThreads, k0 = min(parts, (int)threadIdx.x * per), k1 = min(parts, k0 + per);
         double mine = 0;
@@ -549,13 +616,13 @@ __global__ void __launch_bounds__(kThreads, DRAFT ? 4 : 2) verify_decide_kernel(
         cluster.sync();
         double before = 0, total = 0, from = 0;
         int owner = -1;
-        double sums[kRanks];
-        for (int k = 0; k < kRanks; ++k) sums[k] = *cluster.map_shared_rank(&total_s, k), total += sums[k];
+        double sums[kMaxRanks];
+        for (int k = 0; k < ranks; ++k) sums[k] = *cluster.map_shared_rank(&total_s, k), total += sums[k];
         cluster.sync();  // nobody's sum is read from here on
         if (total > 0) {
             const double target = (double)u_pick * total;
             bool found = false;
-            for (int k = 0; k < kRanks; ++k) {
+            for (int k = 0; k < ranks; ++k) {
                 if (!found && sums[k] > 0) owner = k, from = before, found = before + sums[k] > target;
                 before += sums[k];
             }
@@ -634,11 +701,11 @@ template <typename TX, typename TD>
 cudaError_t launch_verify(const VerifyArgs &a, cudaStream_t st) {
     const bool draft = a.draft != nullptr;
     // a warp a chunk until the machine is full
-    const int64_t chunks = (int64_t)a.T * ((a.V + 4 * kPieces - 1) / (4 * kPieces)), per = kStatThreads / 32;
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((chunks + per - 1) / per, (int64_t)sm_count() * kStatCtas));
-    const cudaError_t e = launch_behind(verify_stats_kernel<TX, TD>, dim3(grid, draft ? 2 : 1), dim3(kStatThreads), 0, st, 1, a);
+    const int64_t chunks = (int64_t)a.T * ((a.V + 4 * kPieces - 1) / (4 * kPieces)), per = kStatThreads / 32, most = (int64_t)sm_count() * kStatCtas / 2 * 2;
+    const unsigned grid = (unsigned)std::min<int64_t>((chunks + per - 1) / per * (draft ? 2 : 1), most);
+    const cudaError_t e = launch_behind(verify_stats_kernel<TX, TD>, dim3(grid), dim3(kStatThreads), 0, st, 1, a);
     if (e != cudaSuccess) return e;
-    return draft ? launch_behind(verify_decide_kernel<TX, TD, true>, dim3((unsigned)(a.B * kRanks)), dim3(kThreads), 0, st, kRanks, a)
+    return draft ? launch_behind(verify_decide_kernel<TX, TD, true>, dim3((unsigned)(a.B * a.ranks)), dim3(kThreads), 0, st, a.ranks, a)
                  : launch_behind(verify_decide_kernel<TX, TD, false>, dim3((unsigned)a.B), dim3(kThreads), 0, st, 1, a);
 }
 
@@ -694,6 +761,7 @@ int sxb_verify_drafts(const SxbVerifyDraftsArgs *args, sxb_stream_t stream) {
     a.logits = g.logits, a.draft = g.draft_logits, a.ld = g.ld, a.draft_ld = g.draft_ld, a.ids = g.ids, a.q_start = g.q_start, a.u = g.u, a.u_pick = g.u_pick;
     a.temperature = g.temperature, a.next_ids = g.next_ids, a.n_new = g.n_new, a.logp = g.logp, a.stats = static_cast<ChunkStat *>(g.ws), a.err = g.err;
     a.T = (int)T, a.V = (int)V, a.B = (int)B, a.pitch = (int)most_chunks(V);
+    a.ranks = B * kMaxRanks <= 2 * (int64_t)sm_count() ? kMaxRanks : kMinRanks;  // eight while all find their places at once
     auto st = static_cast<cudaStream_t>(stream);
     const bool x32 = g.act == SXB_ACT_F32, d32 = g.draft_logits != nullptr ? g.draft_act == SXB_ACT_F32 : x32;
     const cudaError_t e = x32 ? (d32 ? launch_verify<float, float>(a, st) : launch_verify<float, uint16_t>(a, st))
