@@ -1,9 +1,13 @@
 // The residual's addition and root-mean-square norm between two sublayers, with the outputs that the next product reads: s = x + y as stored, n = s /
 // sqrt(mean(s^2) + eps) * weight, n as BF16 or as e4m3 codes with a scale for every block of 128 (f8.cuh).  And the same codes, in blocks of 128 x 128, of a weight.
 //
-// One pass: a CTA has a row in registers between the sum of its squares and its codes, so x and y are read and s and the codes written once.
+// One pass: a CTA has a row in registers between the sum of its squares and its codes, so x and y are read and s and the codes written once.  The arithmetic is by pairs: one after the other,
+// with divisions for what is a product here, the instructions were what bounded it (16384 x 4096: 87 us for 81).
 
 #include "f8.cuh"
+#include "skinny_mma.cuh"
+
+#include <type_traits>
 
 namespace sxb {
 namespace {
@@ -19,8 +23,9 @@ struct NormArgs {
     uint8_t *codes;
     float *scales;
     int64_t x_ld, y_ld, total_ld, out_ld, codes_ld, scales_ld;
+    int64_t T;
     int d, normed;
-    float eps;
+    float eps, inv_d;
 };
 
 __device__ inline void load8(const float *p, float (&v)[kVec]) {
@@ -44,6 +49,17 @@ __device__ inline void store8(uint16_t *p, const float (&v)[kVec]) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+__device__ inline float max_nan(float a, float b) {  // NaN if one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// 1 / v to the last place, for normal numbers whose reciprocals are.
+__device__ inline float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 // The values as they are stored in TX.
 template <typename TX>
 __device__ inline void as_kept(float (&v)[kVec]) {
@@ -55,95 +71,139 @@ __device__ inline void as_kept(float (&v)[kVec]) {
         }
 }
 
-// Y: 0 = none, 1 = BF16, 2 = FP32.  NV: pieces of a row that a thread has, blockDim.x apart (a multiple of 32, so that blocks stay with sixteen lanes).
-template <typename TX, int Y, int NV>
-__global__ void __launch_bounds__(1024) add_norm_kernel(const NormArgs a) {
-    behind_grid();
-    __shared__ float parts[32];
-    const int64_t row = blockIdx.x;
-    const TX *const x = static_cast<const TX *>(a.x) + row * a.x_ld;
-    float s[NV][kVec];
+// Eight elements as they lie in memory.
+template <typename T>
+struct Raw8 {
+    uint4 v[sizeof(T) / 2];
+    __device__ inline void load(const T *p) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
-        if (at < a.d) load8(x + at, s[j]);
-        else
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) s[j][i] = 0.f;
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4 *>(p)[i];
     }
-    if constexpr (Y != 0) {
+    __device__ inline void clear() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ inline float at(int i) const {
+        const uint32_t w[4] = {v[i / (16 / (int)sizeof(T))].x, v[i / (16 / (int)sizeof(T))].y, v[i / (16 / (int)sizeof(T))].z, v[i / (16 / (int)sizeof(T))].w};
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i % 4]);
+        else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+};
+
+// Y: 0 = none, 1 = BF16, 2 = FP32.  NV: pieces of a row that a thread has, blockDim.x apart (a multiple of 32, so that blocks stay with sixteen lanes).  LOOP: a CTA goes on to further rows, the
+// next one's x and y on their way; else it has blockDim.y rows, of a warp each if there are several.
+template <typename TX, int Y, int NV, bool LOOP>
+__global__ void __launch_bounds__(LOOP ? 512 : 1024) add_norm_kernel(const NormArgs a) {
+    using TY = std::conditional_t<Y == 2, float, uint16_t>;
+    behind_grid();
+    __shared__ float parts[2][32];
+    Raw8<TX> x[NV];
+    Raw8<TY> y[NV];
+    auto ask = [&](int64_t row) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
-            if (at >= a.d) continue;
-            float y[kVec];
-            if constexpr (Y == 1) load8(static_cast<const uint16_t *>(a.y) + row * a.y_ld + at, y);
-            else load8(static_cast<const float *>(a.y) + row * a.y_ld + at, y);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) s[j][i] += y[i];
-            as_kept<TX>(s[j]);
-            if (a.total != nullptr) store8(static_cast<TX *>(a.total) + row * a.total_ld + at, s[j]);
+            if (at < a.d) {
+                x[j].load(static_cast<const TX *>(a.x) + row * a.x_ld + at);
+                if constexpr (Y != 0) y[j].load(static_cast<const TY *>(a.y) + row * a.y_ld + at);
+            } else {
+                x[j].clear();
+                if constexpr (Y != 0) y[j].clear();
+            }
         }
-    }
-    float r = 1.f;
-    if (a.normed) {
-        float sum = 0.f;
+    };
+    const int64_t row0 = LOOP ? blockIdx.x : (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    if (!LOOP && row0 >= a.T) return;
+    ask(row0);
+    int turn = 0;
+    for (int64_t row = row0; row < a.T; row += gridDim.x, turn ^= 1) {
+        float s[NV][kVec];
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) sum = fmaf(s[j][i], s[j][i], sum);
+            for (int i = 0; i < kVec; ++i) s[j][i] = Y != 0 ? x[j].at(i) + y[j].at(i) : x[j].at(i);
+            if constexpr (Y != 0) {
+                as_kept<TX>(s[j]);
+                if (a.total != nullptr && at < a.d) store8(static_cast<TX *>(a.total) + row * a.total_ld + at, s[j]);
+            }
+        }
+        if (LOOP && row + gridDim.x < a.T) ask(row + gridDim.x);
+        float r = 1.f;
+        if (a.normed) {
+            uint64_t squares[2] = {0, 0};
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (blockDim.x > 32) {
-            if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = sum;
-            __syncthreads();
-            const int warps = (int)blockDim.x >> 5, lane = threadIdx.x & 31;
-            sum = lane < warps ? parts[lane] : 0.f;
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < kVec; i += 2) {
+                    const uint64_t v = pair(s[j][i], s[j][i + 1]);
+                    squares[i / 2 & 1] = fma_pair(v, v, squares[i / 2 & 1]);
+                }
+            float sum, other;
+            unpair(add_pair(squares[0], squares[1]), sum, other);
+            sum += other;
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        }
-        r = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum, (float)a.d) + a.eps));
-    }
+            if (blockDim.x > 32) {
+                if ((threadIdx.x & 31) == 0) parts[turn][threadIdx.x >> 5] = sum;
+                __syncthreads();
+                const int warps = (int)blockDim.x >> 5, lane = threadIdx.x & 31;
+                sum = lane < warps ? parts[turn][lane] : 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
-        if (at < a.d) {
-            float w[kVec];
-            if (a.weight != nullptr) load8(a.weight + at, w);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-                if (a.normed) s[j][i] *= r;
-                if (a.weight != nullptr) s[j][i] *= w[i];
+                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
             }
-            if (a.out != nullptr) store8(a.out + row * a.out_ld + at, s[j]);
+            r = rsqrtf(fmaf(sum, a.inv_d, a.eps));
         }
-        if (a.codes != nullptr) {
-            uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) most = max(most, magnitude(s[j][i]));
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-            const float scale = f8_scale(most), inv = __fdiv_rn(1.f, scale);
+        for (int j = 0; j < NV; ++j) {
+            const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
             if (at < a.d) {
-                uint2 c;
-                c.x = f8_quad(s[j][0] * inv, s[j][1] * inv, s[j][2] * inv, s[j][3] * inv);
-                c.y = f8_quad(s[j][4] * inv, s[j][5] * inv, s[j][6] * inv, s[j][7] * inv);
-                *reinterpret_cast<uint2 *>(a.codes + row * a.codes_ld + at) = c;
-                if (at % kF8Block == 0) a.scales[row * a.scales_ld + at / kF8Block] = scale;
+                float w[kVec];
+                if (a.weight != nullptr) load8(a.weight + at, w);
+#pragma unroll
+                for (int i = 0; i < kVec; i += 2) {
+                    uint64_t v = mul_pair(pair(s[j][i], s[j][i + 1]), pair(r, r));
+                    if (a.weight != nullptr) v = mul_pair(v, pair(w[i], w[i + 1]));
+                    unpair(v, s[j][i], s[j][i + 1]);
+                }
+                if (a.out != nullptr) store8(a.out + row * a.out_ld + at, s[j]);
+            }
+            if (a.codes != nullptr) {
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) most = max_nan(most, fabsf(s[j][i]));
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
+                const float scale = f8_scale(__float_as_uint(most) & 0x7fffffffu), inv = reciprocal(scale);
+                if (at < a.d) {
+                    const uint64_t by = pair(inv, inv);
+#pragma unroll
+                    for (int i = 0; i < kVec; i += 2) unpair(mul_pair(pair(s[j][i], s[j][i + 1]), by), s[j][i], s[j][i + 1]);
+                    const uint2 c = make_uint2(f8_quad(s[j][0], s[j][1], s[j][2], s[j][3]), f8_quad(s[j][4], s[j][5], s[j][6], s[j][7]));
+                    *reinterpret_cast<uint2 *>(a.codes + row * a.codes_ld + at) = c;
+                    if (at % kF8Block == 0) a.scales[row * a.scales_ld + at / kF8Block] = scale;
+                }
             }
         }
+        if (!LOOP) break;
     }
 }
 
+// A thread has one piece of a row, the shortest way through it; short rows are a warp's, eight of them a CTA's.  Many long rows keep the CTAs on the machine and two pieces a thread: what
+// bounds a CTA that comes and goes is its chain of loads, sums and stores (16384 x 4096, BF16 x and y: 80.9 us, so 77.4, the bytes at the copy's rate 71.8; 8192 x 8192 86.9, 79.3; x alone
+// 61.8, 52.1), unless y is FP32 (90.7, 93.3: the bytes take 92.4 at that rate).  16384 x 256: 17.9 with a CTA a row.
 template <typename TX, int Y>
-cudaError_t launch_norm(const NormArgs &a, int64_t T, cudaStream_t st) {
+cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
     const int pieces = a.d / kVec;
-    // few rows: a piece a thread, the shortest way through a row
-    const int nv = pieces > 2048 ? 4 : pieces > 1024 ? 2 : 1;
-    const dim3 grid((unsigned)T), block((unsigned)(((pieces + nv - 1) / nv + 31) / 32 * 32));
-    if (nv == 4) return launch_behind(add_norm_kernel<TX, Y, 4>, grid, block, 0, st, 1, a);
-    if (nv == 2) return launch_behind(add_norm_kernel<TX, Y, 2>, grid, block, 0, st, 1, a);
-    return launch_behind(add_norm_kernel<TX, Y, 1>, grid, block, 0, st, 1, a);
+    auto go = [&](auto kern, int nv, int rows, int64_t grid) {
+        return launch_behind(kern, dim3((unsigned)grid), dim3((unsigned)(((pieces + nv - 1) / nv + 31) / 32 * 32), rows), 0, st, 1, a);
+    };
+    if (pieces <= 32) return go(add_norm_kernel<TX, Y, 1, false>, 1, 8, (a.T + 7) / 8);
+    const int64_t places = (int64_t)sm_count() * 4;
+    if (Y != 2 && pieces >= 256 && pieces <= 1024 && a.T >= 4 * places) return go(add_norm_kernel<TX, Y, 2, true>, 2, 1, places);
+    if (pieces > 2048) return go(add_norm_kernel<TX, Y, 4, false>, 4, 1, a.T);
+    if (pieces > 1024) return go(add_norm_kernel<TX, Y, 2, false>, 2, 1, a.T);
+    return go(add_norm_kernel<TX, Y, 1, false>, 1, 1, a.T);
 }
 
 // A CTA has a block of 128 x 128: a thread half a row of it, in registers between the largest magnitude and the codes.
@@ -235,12 +295,12 @@ extern "C" int sxb_add_norm(const SxbAddNormArgs *args, sxb_stream_t stream) {
     NormArgs a{};
     a.x = g.x, a.y = g.y, a.weight = g.weight, a.total = g.total, a.out = static_cast<uint16_t *>(g.out), a.codes = g.codes, a.scales = g.scales;
     a.x_ld = g.x_ld, a.y_ld = g.y_ld, a.total_ld = g.total_ld, a.out_ld = g.out_ld, a.codes_ld = g.codes_ld, a.scales_ld = g.scales_ld;
-    a.d = (int)d, a.normed = g.normed != 0, a.eps = g.eps;
+    a.T = T, a.d = (int)d, a.normed = g.normed != 0, a.eps = g.eps, a.inv_d = 1.f / (float)d;
     auto st = static_cast<cudaStream_t>(stream);
     const int y = g.y == nullptr ? 0 : g.y_act == SXB_ACT_F32 ? 2 : 1;
     cudaError_t e;
-    if (g.act == SXB_ACT_F32) e = y == 0 ? launch_norm<float, 0>(a, T, st) : y == 1 ? launch_norm<float, 1>(a, T, st) : launch_norm<float, 2>(a, T, st);
-    else e = y == 0 ? launch_norm<uint16_t, 0>(a, T, st) : y == 1 ? launch_norm<uint16_t, 1>(a, T, st) : launch_norm<uint16_t, 2>(a, T, st);
+    if (g.act == SXB_ACT_F32) e = y == 0 ? launch_norm<float, 0>(a, st) : y == 1 ? launch_norm<float, 1>(a, st) : launch_norm<float, 2>(a, st);
+    else e = y == 0 ? launch_norm<uint16_t, 0>(a, st) : y == 1 ? launch_norm<uint16_t, 1>(a, st) : launch_norm<uint16_t, 2>(a, st);
     SXB_CUDA(e, fn, ": launching T=", T, " d=", d);
     SXB_CHECK_LAUNCH(fn, " ", act_name(g.act), " T=", T, " d=", d);
     return SXB_OK;

@@ -690,19 +690,33 @@ def add_norm(x, y=None, weight=None, eps=1e-6, total=None, out=None, codes=None,
     T, d = x.shape
     dev, dt = x.get_device(), x.dtype
     ok = dev == torch._C._cuda_getDevice() and dt in _ROWS and (x.is_contiguous() or x.stride(1) == 1)
-    p = [0] * 5
-    ld = [0] * 5
-    for i, t, types, n in ((0, y, _ROWS, d), (1, total, (dt,), d), (2, out, _BF16, d), (3, codes, (F8,), d), (4, scales, _F32, _blocks(d))):
-        if t is not None:
-            ok = ok and t.dtype in types and t.get_device() == dev and t.shape == (T, n) and (t.is_contiguous() or t.stride(1) == 1 or n == 1)
-            p[i], ld[i] = t.data_ptr(), (_rows(t) if ok else n)
+    yp = wp = tp = op = cp = sp = 0
+    y_ld = t_ld = o_ld = c_ld = s_ld = d
+    if y is not None:
+        ok = ok and y.dtype in _ROWS and y.get_device() == dev and y.shape == x.shape and (y.is_contiguous() or y.stride(1) == 1)
+        yp, y_ld = y.data_ptr(), y.stride(0)
     if weight is not None:
-        ok = ok and weight.dtype is torch.float32 and weight.get_device() == dev and weight.is_contiguous() and weight.numel() == d
+        ok = ok and weight.dtype is torch.float32 and weight.get_device() == dev and weight.is_contiguous() and weight.shape == (d,)
+        wp = weight.data_ptr()
+    if total is not None:
+        ok = ok and total.dtype is dt and total.get_device() == dev and total.shape == x.shape and (total.is_contiguous() or total.stride(1) == 1)
+        tp, t_ld = total.data_ptr(), total.stride(0)
+    if out is not None:
+        ok = ok and out.dtype is torch.bfloat16 and out.get_device() == dev and out.shape == x.shape and (out.is_contiguous() or out.stride(1) == 1)
+        op, o_ld = out.data_ptr(), out.stride(0)
+    if codes is not None:
+        ok = ok and codes.dtype is F8 and codes.get_device() == dev and codes.shape == x.shape and (codes.is_contiguous() or codes.stride(1) == 1)
+        cp, c_ld = codes.data_ptr(), codes.stride(0)
+    if scales is not None:
+        ok = ok and scales.dtype is torch.float32 and scales.get_device() == dev and scales.shape == (T, -(-d // _F8_BLOCK)) and (scales.is_contiguous() or scales.stride(1) == 1)
+        sp, s_ld = scales.data_ptr(), scales.stride(0)
     if not ok:
         _refuse_all(dev, "add_norm", x=(x, _ROWS), y=(y, _ROWS), weight=(weight, _F32), total=(total, (dt,)), out=(out, _BF16), codes=(codes, (F8,)), scales=(scales, _F32))
+    if T == 1:  # a single row's stride may be anything
+        y_ld, t_ld, o_ld, c_ld, s_ld = d, d, d, d, -(-d // _F8_BLOCK)
     _check(_lib.load().sxb_add_norm(_NORM_ARGS.pack(
-        x.data_ptr(), p[0], 0 if weight is None else weight.data_ptr(), p[1], p[2], p[3], p[4], T, d, _rows(x), ld[0], ld[1], ld[2], ld[3], ld[4], eps,
-        dt is torch.bfloat16, y is not None and y.dtype is torch.bfloat16, bool(norm)), _stream(stream)))
+        x.data_ptr(), yp, wp, tp, op, cp, sp, T, d, x.stride(0) if T > 1 else d, y_ld, t_ld, o_ld, c_ld, s_ld, eps, dt is torch.bfloat16, y is not None and y.dtype is torch.bfloat16,
+        bool(norm)), _stream(stream)))
 
 
 def linear_f8(x, x_scale, w: F8View, y, stream=None):
