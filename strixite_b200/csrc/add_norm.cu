@@ -60,6 +60,19 @@ __device__ inline float reciprocal(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+// A block's values v, `most` their largest magnitude, to what its codes are rounded from: 448 v / most to the last bit (a quotient, put right by its remainder), so that values that
+// stand between two codes round to the even one, as the definition says, whatever the row's factor r.  Where the scale is its least, v r / scale.
+__device__ inline void f8_codes(float (&v)[kVec], float most, float exact, float r, float scale) {
+    const bool least = !(exact >= kF8Least);  // zeros and NaN too
+    const float shrink = most >= 0x1p100f ? 0x1p-40f : 1.f, top = kF8Top * shrink, by = least ? 1.f : most * shrink;
+    const float inv = least ? __fdiv_rn(r, scale) : reciprocal(by);
+    const uint64_t tops = pair(least ? 1.f : top, least ? 1.f : top), invs = pair(inv, inv), minus = pair(least ? 0.f : -by, least ? 0.f : -by), again = pair(least ? 0.f : inv, least ? 0.f : inv);
+#pragma unroll
+    for (int i = 0; i < kVec; i += 2) {
+        const uint64_t t = mul_pair(pair(v[i], v[i + 1]), tops), q = mul_pair(t, invs);
+        unpair(fma_pair(fma_pair(q, minus, t), again, q), v[i], v[i + 1]);
+    }
+}
 // The values as they are stored in TX.
 template <typename TX>
 __device__ inline void as_kept(float (&v)[kVec]) {
@@ -157,16 +170,20 @@ __global__ void __launch_bounds__(LOOP ? 512 : 1024) add_norm_kernel(const NormA
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int at = (j * (int)blockDim.x + (int)threadIdx.x) * kVec;
+            // s times the weight; the row's factor r, which a block's codes do not depend on, comes to the scale (and out) alone
             if (at < a.d) {
-                float w[kVec];
-                if (a.weight != nullptr) load8(a.weight + at, w);
+                if (a.weight != nullptr) {
+                    float w[kVec];
+                    load8(a.weight + at, w);
 #pragma unroll
-                for (int i = 0; i < kVec; i += 2) {
-                    uint64_t v = mul_pair(pair(s[j][i], s[j][i + 1]), pair(r, r));
-                    if (a.weight != nullptr) v = mul_pair(v, pair(w[i], w[i + 1]));
-                    unpair(v, s[j][i], s[j][i + 1]);
+                    for (int i = 0; i < kVec; i += 2) unpair(mul_pair(pair(s[j][i], s[j][i + 1]), pair(w[i], w[i + 1])), s[j][i], s[j][i + 1]);
                 }
-                if (a.out != nullptr) store8(a.out + row * a.out_ld + at, s[j]);
+                if (a.out != nullptr) {
+                    float n[kVec];
+#pragma unroll
+                    for (int i = 0; i < kVec; i += 2) unpair(mul_pair(pair(s[j][i], s[j][i + 1]), pair(r, r)), n[i], n[i + 1]);
+                    store8(a.out + row * a.out_ld + at, n);
+                }
             }
             if (a.codes != nullptr) {
                 float most = 0.f;
@@ -174,11 +191,9 @@ __global__ void __launch_bounds__(LOOP ? 512 : 1024) add_norm_kernel(const NormA
                 for (int i = 0; i < kVec; ++i) most = max_nan(most, fabsf(s[j][i]));
 #pragma unroll
                 for (int off = 8; off > 0; off >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
-                const float scale = f8_scale(__float_as_uint(most) & 0x7fffffffu), inv = reciprocal(scale);
+                const float exact = __fdiv_rn(most * r, kF8Top), scale = f8_scale(most, exact);
                 if (at < a.d) {
-                    const uint64_t by = pair(inv, inv);
-#pragma unroll
-                    for (int i = 0; i < kVec; i += 2) unpair(mul_pair(pair(s[j][i], s[j][i + 1]), by), s[j][i], s[j][i + 1]);
+                    f8_codes(s[j], most, exact, r, scale);
                     const uint2 c = make_uint2(f8_quad(s[j][0], s[j][1], s[j][2], s[j][3]), f8_quad(s[j][4], s[j][5], s[j][6], s[j][7]));
                     *reinterpret_cast<uint2 *>(a.codes + row * a.codes_ld + at) = c;
                     if (at % kF8Block == 0) a.scales[row * a.scales_ld + at / kF8Block] = scale;
@@ -234,16 +249,14 @@ __global__ void __launch_bounds__(256) quantize_f8_kernel(const TW *__restrict__
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = max(most, parts[i]);
-    const float s = f8_scale(most), inv = __fdiv_rn(1.f, s);
+    const float largest = __uint_as_float(most), exact = __fdiv_rn(largest, kF8Top), s = f8_scale(largest, exact);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const int64_t row = row0 + 16 * j;
         if (row >= N || col >= K) continue;
-        uint2 c;
-        c.x = f8_quad(v[j][0] * inv, v[j][1] * inv, v[j][2] * inv, v[j][3] * inv);
-        c.y = f8_quad(v[j][4] * inv, v[j][5] * inv, v[j][6] * inv, v[j][7] * inv);
-        *reinterpret_cast<uint2 *>(q + row * K + col) = c;
+        f8_codes(v[j], largest, exact, 1.f, s);
+        *reinterpret_cast<uint2 *>(q + row * K + col) = make_uint2(f8_quad(v[j][0], v[j][1], v[j][2], v[j][3]), f8_quad(v[j][4], v[j][5], v[j][6], v[j][7]));
     }
 }
 
@@ -265,7 +278,7 @@ extern "C" int sxb_add_norm(const SxbAddNormArgs *args, sxb_stream_t stream) {
     SXB_CHECK(g.total == nullptr || g.y != nullptr, fn, ": a total without y");
     SXB_CHECK((g.codes == nullptr) == (g.scales == nullptr), fn, ": codes and scales come together (codes=", (const void *)g.codes, ", scales=", (const void *)g.scales, ")");
     SXB_CHECK(g.normed || g.weight == nullptr, fn, ": a weight without the norm");
-    SXB_CHECK(!g.normed || (g.eps > 0.f && g.eps < 1e30f), fn, ": eps must be finite and positive");
+    SXB_CHECK(!g.normed || (g.eps >= 0x1p-100f && g.eps < 1e30f), fn, ": eps must be finite and at least 2^-100");
     SXB_CHECK(aligned16(g.weight), fn, ": the weight must be 16-byte aligned");
     const int64_t es = act_bytes(g.act), ys = g.y != nullptr ? act_bytes(g.y_act) : 0, blocks = (d + kF8Block - 1) / kF8Block;
     struct Rows {

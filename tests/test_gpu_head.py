@@ -63,10 +63,24 @@ def test_norm(K, cuda, T, d, x32, y):
 
 
 @pytest.mark.parametrize("kw", [dict(weight=False), dict(norm=False, weight=False), dict(wide=48), dict(wide=48, x32=True, y=torch.float32), dict(in_place="x"), dict(in_place="y"),
-                                dict(in_place="x", x32=True, y=torch.float32), dict(size=1e-18), dict(size=1e15), dict(eps=1.0), dict(size=1e-30, norm=False, weight=False)])
+                                dict(in_place="x", x32=True, y=torch.float32), dict(size=1e33, norm=False, weight=False, x32=True, y=torch.float32), dict(size=1e-18), dict(size=1e15), dict(eps=1.0), dict(size=1e-30, norm=False, weight=False)])
 @pytest.mark.parametrize("T,d", [(3, 400), (33, 4096), (600, 2560)])
 def test_norm_forms(K, cuda, T, d, kw):
     run_norm(K, cuda, T, d, **kw)
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("most", [64, 56, 96, 127])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_codes_between_two_numbers_go_to_the_even_one(K, cuda, norm, most, dtype):
+    """Whole numbers, a block's largest one known: 448 x / most is a number that FP64 holds or is far from a tie, and the row's factor must not move it."""
+    x = torch.randint(-most, most + 1, (64, 512), generator=gen(most, cuda), device=cuda).to(dtype)
+    x[:, ::128] = most
+    codes, scales = codes_like(K, (64, 512), cuda), torch.zeros((64, 4), device=cuda)
+    K.add_norm(x, codes=codes, scales=scales, norm=norm)
+    v = P.f64(x) * 448 / most
+    step = 2.0 ** (np.floor(np.log2(np.maximum(np.abs(v), 2.0 ** -6))) - 3)
+    assert np.array_equal(P.f64(codes), np.round(v / step) * step)  # numpy rounds halves to even
 
 
 def test_norm_one_output_at_a_time(K, cuda):
