@@ -660,7 +660,7 @@ class F8View:
             raise Error(1, f"F8View: scale is {tuple(scale.shape)} of {scale.dtype} on {scale.device}, expected contiguous {(_blocks(self.N), _blocks(self.K))} FP32 on {q.device}")
         if not q.is_cuda:
             raise Error(1, "F8View: the weight must live on a CUDA device (no CPU path exists)")
-        self.q, self.scale, self.device, self.index = q, scale, q.device, q.get_device()
+        self.q, self.scale, self.device, self.index, self.blocks = q, scale, q.device, q.get_device(), _blocks(self.K)
         self._c = _lib.SxbF8View(q.data_ptr(), scale.data_ptr(), self.N, self.K)
         self._at = C.addressof(self._c)
 
@@ -722,13 +722,15 @@ def add_norm(x, y=None, weight=None, eps=1e-6, total=None, out=None, codes=None,
 def linear_f8(x, x_scale, w: F8View, y, stream=None):
     """sxb_linear_f8: y [M, N] BF16 or FP32 = x [M, K] float8_e4m3fn (scales x_scale [M, ceil(K / 128)] FP32) times w^T."""
     M, K = x.shape
-    dev = w.index
-    if not (dev == torch._C._cuda_getDevice() and x.dtype is F8 and x_scale.dtype is torch.float32 and y.dtype in _ROWS and x.get_device() == dev and x_scale.get_device() == dev
-            and y.get_device() == dev and K == w.K and x_scale.shape == (M, _blocks(K)) and y.shape == (M, w.N) and (x.is_contiguous() or x.stride(1) == 1)
-            and (x_scale.is_contiguous() or x_scale.stride(1) == 1 or K <= _F8_BLOCK) and (y.is_contiguous() or y.stride(1) == 1 or w.N == 1)):
+    dev, dt = w.index, y.dtype
+    if not (dev == torch._C._cuda_getDevice() and x.dtype is F8 and x_scale.dtype is torch.float32 and dt in _ROWS and x.get_device() == dev and x_scale.get_device() == dev
+            and y.get_device() == dev and K == w.K and x_scale.shape == (M, w.blocks) and y.shape == (M, w.N) and (x.is_contiguous() or x.stride(1) == 1)
+            and (x_scale.is_contiguous() or x_scale.stride(1) == 1 or w.blocks == 1) and (y.is_contiguous() or y.stride(1) == 1 or w.N == 1)):
         _refuse_all(dev, "linear_f8", x=(x, (F8,)), x_scale=(x_scale, _F32), w=(w.q, (F8,)), y=(y, _ROWS))
+    many = M > 1
     _check(_lib.load().sxb_linear_f8(_LINEAR_F8_ARGS.pack(
-        x.data_ptr(), x_scale.data_ptr(), w._at, y.data_ptr(), M, _rows(x), _rows(x_scale), _rows(y), y.dtype is torch.bfloat16), _stream(stream)))
+        x.data_ptr(), x_scale.data_ptr(), w._at, y.data_ptr(), M, x.stride(0) if many else K, x_scale.stride(0) if many else w.blocks, y.stride(0) if many else w.N,
+        dt is torch.bfloat16), _stream(stream)))
 
 
 def verify_drafts_workspace_bytes(T: int, B: int, V: int) -> int:
@@ -745,24 +747,33 @@ def verify_drafts(logits, ids, q_start, u, u_pick, next_ids, n_new, ws, err, dra
     -> next_ids [T] int32 (-1 behind the last), n_new [B] int32, logp [T] FP32 or None.  err: 3 or more zeroed int32."""
     T, V = logits.shape
     dev, B = logits.get_device(), n_new.shape[0]
-    ok = dev == torch._C._cuda_getDevice() and logits.dtype in _ROWS and (logits.is_contiguous() or logits.stride(1) == 1 or V == 1)
-    for t, dt, n in ((ids, torch.int32, T), (q_start, torch.int32, B + 1), (u, torch.float32, T), (u_pick, torch.float32, B), (next_ids, torch.int32, T), (n_new, torch.int32, B),
-                     (temperature, torch.float32, B), (logp, torch.float32, T)):
-        ok = ok and (t is None or (t.dtype is dt and t.get_device() == dev and t.is_contiguous() and t.numel() == n))
-    ok = ok and ws.get_device() == dev and ws.is_contiguous() and err.get_device() == dev and err.dtype in _WORDS and err.is_contiguous() and err.numel() >= 3
-    dp = dld = 0
+    rows, seqs = (T,), (B,)
+    ok = (dev == torch._C._cuda_getDevice() and logits.dtype in _ROWS and (logits.is_contiguous() or logits.stride(1) == 1 or V == 1) and ids.dtype is torch.int32 and ids.get_device() == dev
+          and ids.shape == rows and ids.is_contiguous() and q_start.dtype is torch.int32 and q_start.get_device() == dev and q_start.shape == (B + 1,) and q_start.is_contiguous()
+          and u.dtype is torch.float32 and u.get_device() == dev and u.shape == rows and u.is_contiguous() and u_pick.dtype is torch.float32 and u_pick.get_device() == dev
+          and u_pick.shape == seqs and u_pick.is_contiguous() and next_ids.dtype is torch.int32 and next_ids.get_device() == dev and next_ids.shape == rows and next_ids.is_contiguous()
+          and n_new.dtype is torch.int32 and n_new.get_device() == dev and n_new.dim() == 1 and n_new.is_contiguous() and ws.get_device() == dev and ws.is_contiguous()
+          and err.get_device() == dev and err.dtype in _WORDS and err.is_contiguous() and err.numel() >= 3)
+    dp = tp = lp = d_bf16 = 0
+    dld = V
     if draft_logits is not None:
         d = draft_logits
-        ok = ok and d.dtype in _ROWS and d.get_device() == dev and d.shape == (T, V) and (d.is_contiguous() or d.stride(1) == 1 or V == 1)
-        dp, dld = d.data_ptr(), (_rows(d) if ok else V)
+        ok = ok and d.dtype in _ROWS and d.get_device() == dev and d.shape == logits.shape and (d.is_contiguous() or d.stride(1) == 1 or V == 1)
+        dp, dld, d_bf16 = d.data_ptr(), d.stride(0), d.dtype is torch.bfloat16
+    if temperature is not None:
+        ok = ok and temperature.dtype is torch.float32 and temperature.get_device() == dev and temperature.shape == seqs and temperature.is_contiguous()
+        tp = temperature.data_ptr()
+    if logp is not None:
+        ok = ok and logp.dtype is torch.float32 and logp.get_device() == dev and logp.shape == rows and logp.is_contiguous()
+        lp = logp.data_ptr()
     if not ok:
         _refuse_all(dev, "verify_drafts", logits=(logits, _ROWS), draft_logits=(draft_logits, _ROWS), ids=(ids, _I32), q_start=(q_start, _I32), u=(u, _F32), u_pick=(u_pick, _F32),
                     temperature=(temperature, _F32), next_ids=(next_ids, _I32), n_new=(n_new, _I32), logp=(logp, _F32), ws=(ws, (ws.dtype,)), err=(err, _WORDS))
+    many = T > 1  # a single row's stride may be anything
     _count()  # two launches
     _check(_lib.load().sxb_verify_drafts(_VERIFY_ARGS.pack(
-        logits.data_ptr(), dp, _rows(logits), dld, T, V, B, ids.data_ptr(), q_start.data_ptr(), u.data_ptr(), u_pick.data_ptr(),
-        0 if temperature is None else temperature.data_ptr(), next_ids.data_ptr(), n_new.data_ptr(), 0 if logp is None else logp.data_ptr(), ws.data_ptr(),
-        ws.numel() * ws.element_size(), err.data_ptr(), logits.dtype is torch.bfloat16, draft_logits is not None and draft_logits.dtype is torch.bfloat16), _stream(stream)))
+        logits.data_ptr(), dp, logits.stride(0) if many else V, dld if many else V, T, V, B, ids.data_ptr(), q_start.data_ptr(), u.data_ptr(), u_pick.data_ptr(), tp,
+        next_ids.data_ptr(), n_new.data_ptr(), lp, ws.data_ptr(), ws.nbytes, err.data_ptr(), logits.dtype is torch.bfloat16, d_bf16), _stream(stream)))
 
 
 def check_verify_error(err, what: str):
