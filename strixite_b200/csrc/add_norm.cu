@@ -49,11 +49,6 @@ __device__ inline void store8(uint16_t *p, const float (&v)[kVec]) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ inline float max_nan(float a, float b) {  // NaN if one is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 // 1 / v to the last place, for normal numbers whose reciprocals are.
 __device__ inline float reciprocal(float v) {
     float r;

@@ -10,6 +10,7 @@
 //   tiles    a CTA has a tile of 128 x 128; where tiles are few, a cluster of up to eight CTAs shares its k, and adds the parts up through distributed shared memory in rank order.
 
 #include "linear_f8.cuh"
+#include "skinny_mma.cuh"
 #include "tc_ptx.cuh"
 
 namespace sxb {
@@ -142,21 +143,11 @@ __device__ inline void tc_there(float (&v)[16]) {
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
                    "+f"(v[13]), "+f"(v[14]), "+f"(v[15])::"memory");
 }
-__device__ inline uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ inline uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 __device__ inline void store32(void *p, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
-// n values (a multiple of 32 bytes' worth) to y at `at`, `left` of which lie inside the row.
+// Values to y at `at`, `left` of which lie inside the row.  (BF16 rows that sixteen bytes may be stored to at once leave by tensor copies.)
 template <int NV>
 __device__ inline void store_run(const TcArgs8 &a, int64_t at, int left, const float (&v)[NV]) {
     if (a.g.f32) {
@@ -178,19 +169,8 @@ __device__ inline void store_run(const TcArgs8 &a, int64_t at, int left, const f
     } else {
         uint16_t *p = static_cast<uint16_t *>(a.g.y) + at;
 #pragma unroll
-        for (int i = 0; i < NV; i += 16) {
-            uint32_t w[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = bf16_pair(v[i + 2 * k], v[i + 2 * k + 1]);
-            if (i + 16 <= left && a.vec >= 32) store32(p + i, w);
-            else if (i + 16 <= left && a.vec >= 16) {
-                reinterpret_cast<uint4 *>(p + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                reinterpret_cast<uint4 *>(p + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-            } else
-#pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    if (i + k < left) p[i + k] = f32_to_bf16_bits(v[i + k]);
-        }
+        for (int i = 0; i < NV; ++i)
+            if (i < left) p[i] = f32_to_bf16_bits(v[i]);
     }
 }
 
@@ -427,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 tc_fence_after();
-                const uint64_t s2 = pack2(s, s);
+                const uint64_t s2 = pair(s, s);
                 constexpr int AT = kAtOnce;
                 float v[2][AT];
                 const uint32_t from = lanes + (uint32_t)(acc.at * BN);
@@ -443,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (lane == 0) arrive_at(empty_at + 8u * (uint32_t)acc.at);
                     }
 #pragma unroll
-                    for (int i = 0; i < AT / 2; ++i) sum[c / 2 + i] = fma2(pack2(u[2 * i], u[2 * i + 1]), s2, sum[c / 2 + i]);
+                    for (int i = 0; i < AT / 2; ++i) sum[c / 2 + i] = fma_pair(pair(u[2 * i], u[2 * i + 1]), s2, sum[c / 2 + i]);
                 }
                 acc.advance(S::kAccs);
             }
@@ -529,7 +509,7 @@ int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
 
 // ---- a few rows of x: the weights on the MMAs' M side ------------------------------------------------------------------------------
 //
-// What bounds it is the weights' bytes, 16 KB a block of k and tile of 128 weight rows; the rows of x, 16 to 64, are the MMA's columns.  The accumulators of all stages fit tensor
+// What bounds it is the weights' bytes, 16 KB a block of k and tile of 128 weight rows; the rows of x, 16 or 32, are the MMA's columns.  The accumulators of all stages fit tensor
 // memory, so one commit a stage, of two blocks, says that its codes have been read and that its sums are there.  A lane of tensor memory is a weight row: a thread has all columns of
 // one, the weight's scale is one number for the warp, and those of x go round by shuffles.
 
@@ -637,21 +617,16 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         // ===================== sums and stores =====================
         const uint32_t lanes = tmem_base + ((uint32_t)(warp * 32) << 16);
         Turn turn{0, 0u};
-        constexpr int NV = (NB + 31) / 32;  // scales of x that a lane holds
-        // of a stage's blocks: those of the lane's rows of x, and the weight's (a tile lies in one block of weight rows); asked for a stage ahead of their use
+        // of a stage's blocks: that of the lane's row of x, and the weight's (a tile lies in one block of weight rows); asked for a stage ahead of their use
         struct Scales {
-            float x[PER][NV], w[PER];
+            float x[PER], w[PER];
         };
         auto scales = [&](int item, int kb) {
             Scales s;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 s.w[i] = kb + i < kb1 ? __ldg(a.g.ws + (int64_t)item * a.g.kb + kb + i) : 0.f;
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int m = j * 32 + lane;
-                    s.x[i][j] = m < a.g.M && m < NB && kb + i < kb1 ? __ldg(a.g.xs + m * a.g.xs_ld + kb + i) : 0.f;
-                }
+                s.x[i] = lane < a.g.M && kb + i < kb1 ? __ldg(a.g.xs + lane * a.g.xs_ld + kb + i) : 0.f;
             }
             return s;
         };
@@ -661,11 +636,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
             for (int i = 0; i < NB; ++i) sum[i] = 0.f;
             for (int kb = kb0; kb < kb1; kb += PER, turn.advance(S::kStages)) {
-                float now[PER][NV];
+                float now[PER];
 #pragma unroll
-                for (int i = 0; i < PER; ++i)
-#pragma unroll
-                    for (int j = 0; j < NV; ++j) now[i][j] = next.x[i][j] * next.w[i];
+                for (int i = 0; i < PER; ++i) now[i] = next.x[i] * next.w[i];
                 if (!__all_sync(0xffffffffu, mbar_wait(&done_bar[turn.at], turn.phase, abort_v, a.wait_limit_ns))) {
                     if (lane == 0) raise_abort(item, 4);
                     break;
@@ -676,20 +649,16 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
                     if (kb + i >= kb1) break;
-                    constexpr int AT = NB < 32 ? 16 : 32;
-#pragma unroll
-                    for (int c = 0; c < NB; c += AT) {
-                        float v[AT];
-                        tc_ask(lanes + (uint32_t)((turn.at * PER + i) * NB + c), v);
-                        tc_there(v);
-                        if (c + AT == NB && (i + 1 == PER || kb + i + 1 == kb1)) {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&drained_bar[turn.at]);
-                        }
-#pragma unroll
-                        for (int k = 0; k < AT; ++k) sum[c + k] = fmaf(v[k], __shfl_sync(0xffffffffu, now[i][(c + k) / 32], (c + k) % 32), sum[c + k]);
+                    float v[NB];
+                    tc_ask(lanes + (uint32_t)((turn.at * PER + i) * NB), v);
+                    tc_there(v);
+                    if (i + 1 == PER || kb + i + 1 == kb1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&drained_bar[turn.at]);
                     }
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) sum[k] = fmaf(v[k], __shfl_sync(0xffffffffu, now[i], k), sum[k]);
                 }
             }
             if (*abort_v) break;

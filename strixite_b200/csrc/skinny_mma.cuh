@@ -48,6 +48,12 @@ __device__ inline uint64_t add_pair(uint64_t a, uint64_t b) {
     return r;
 }
 
+__device__ inline float max_nan(float a, float b) {  // NaN if one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // Two FP32 values that fit BF16 as a pair (the first in the lower half).
 __device__ inline uint32_t pack_bf16_exact(float lo, float hi) { return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632); }
 // The upper sixteen bits of an FP32 value: a BF16, and what is left of the value is an FP32 with eight bits fewer.

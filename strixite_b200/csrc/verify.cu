@@ -9,7 +9,7 @@
 // A border's error: a term takes c (x - max) in FP32 (2^-23 of the exponent, which is small where the term is large), one ex2 (2^-22), sums of up to sixteen
 // terms and then seven more in FP32; chunks are joined in FP64, where the exponents are exact, and no logit is too large for them.
 
-#include "common.cuh"
+#include "skinny_mma.cuh"
 
 #include <cooperative_groups.h>
 
@@ -108,11 +108,6 @@ __device__ inline float exp2_of(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ inline float max_nan(float a, float b) {  // NaN if one is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 __device__ inline uint32_t max_nan_pair(uint32_t a, uint32_t b) {  // of two BF16
     uint32_t r;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -123,27 +118,11 @@ __device__ inline float warp_max_nan(float v) {
     asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ inline uint64_t two(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ inline uint64_t add_two(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ inline uint64_t mul_two(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ inline float first_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ inline float second_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 // 2^(c (x - best)) of two, each with the rounding that one alone has.
-__device__ inline uint64_t weight_two(float x0, float x1, uint64_t minus_best, uint64_t c) {
-    const uint64_t e = mul_two(add_two(two(x0, x1), minus_best), c);
-    return two(exp2_of(first_of(e)), exp2_of(second_of(e)));
+__device__ inline uint64_t weight_pair(float x0, float x1, uint64_t minus_best, uint64_t c) {
+    float e0, e1;
+    unpair(mul_pair(add_pair(pair(x0, x1), minus_best), c), e0, e1);
+    return pair(exp2_of(e0), exp2_of(e1));
 }
 
 // A lane's part of a chunk: piece 32 j + lane is its j-th.  Where the row does not begin or end with a piece, the tokens before the first and behind the last whole one are a lane's each.
@@ -190,15 +169,15 @@ __device__ inline ChunkStat chunk_stat(const Row<T> &r, int chunk, const Loaded 
     uint64_t sum[2] = {0, 0};
     int at = 0x7fffffff;
     if (most > -INFINITY && most < INFINITY) {
-        const uint64_t minus = two(-most, -most), cc = two(c, c);
+        const uint64_t minus = pair(-most, -most), cc = pair(c, c);
 #pragma unroll
         for (int j = 0; j < kPerLane; ++j) {
             float v[VE];
             Row<T>::values(w[j], v);
 #pragma unroll
-            for (int i = 0; i < VE; i += 2) sum[i / 2 & 1] = add_two(sum[i / 2 & 1], weight_two(v[i], v[i + 1], minus, cc));
+            for (int i = 0; i < VE; i += 2) sum[i / 2 & 1] = add_pair(sum[i / 2 & 1], weight_pair(v[i], v[i + 1], minus, cc));
         }
-        sum[0] = add_two(sum[0], weight_two(l.head, l.tail, minus, cc));
+        sum[0] = add_pair(sum[0], weight_pair(l.head, l.tail, minus, cc));
         if (greedy) {
             if (l.tail == most) at = r.token(r.pieces() - 1) + lane;
 #pragma unroll
@@ -214,8 +193,9 @@ __device__ inline ChunkStat chunk_stat(const Row<T> &r, int chunk, const Loaded 
             at = __reduce_min_sync(0xffffffffu, at);
         }
     }
-    const uint64_t both = add_two(sum[0], sum[1]);
-    float s = first_of(both) + second_of(both);
+    float s, odd;
+    unpair(add_pair(sum[0], sum[1]), s, odd);
+    s += odd;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
     return ChunkStat{(double)s, most, at};
