@@ -729,8 +729,8 @@ int sxb_verify_drafts(const SxbVerifyDraftsArgs *args, sxb_stream_t stream) {
         const void *p;
         int64_t n;
     } outs[4] = {{"next_ids", g.next_ids, 4 * T}, {"n_new", g.n_new, 4 * B}, {"logp", g.logp, g.logp != nullptr ? 4 * T : 0}, {"ws", g.ws, (int64_t)need}},
-      ins[6] = {{"logits", g.logits, lb}, {"draft_logits", g.draft_logits, db}, {"ids", g.ids, 4 * T}, {"q_start", g.q_start, 4 * (B + 1)}, {"u", g.u, 4 * T},
-                {"u_pick", g.u_pick, 4 * B}};
+      ins[8] = {{"logits", g.logits, lb}, {"draft_logits", g.draft_logits, db}, {"ids", g.ids, 4 * T}, {"q_start", g.q_start, 4 * (B + 1)}, {"u", g.u, 4 * T},
+                {"u_pick", g.u_pick, 4 * B}, {"temperature", g.temperature, 4 * B}, {"err", g.err, 12}};
     for (int o = 0; o < 4; ++o) {
         if (outs[o].p == nullptr) continue;
         for (const auto &i : ins) SXB_CHECK(i.p == nullptr || apart(outs[o].p, outs[o].n, i.p, i.n), fn, ": ", outs[o].name, " [", outs[o].p, "] overlaps ", i.name, " [", i.p, "]");

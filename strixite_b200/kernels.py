@@ -672,6 +672,10 @@ def quantize_f8(w: torch.Tensor, err: Optional[torch.Tensor] = None, stream=None
     """sxb_quantize_f8 of a contiguous FP32 or BF16 [N, K] tensor: codes and a scale for each block of 128 x 128."""
     if w.dtype not in _ROWS or w.dim() != 2 or not w.is_contiguous():
         raise Error(1, "quantize_f8: w must be a contiguous FP32 or BF16 [N, K] tensor")
+    if w.is_cuda and w.get_device() != torch.cuda.current_device():
+        raise Error(1, f"quantize_f8: w lives on device {w.get_device()}, the current device is {torch.cuda.current_device()}")
+    if err is not None and (err.device != w.device or err.dtype not in _WORDS or not err.is_contiguous() or err.numel() < 3):
+        raise Error(1, f"quantize_f8: err is {err.dtype} {tuple(err.shape)} on {err.device}, expected 3 or more contiguous int32 on {w.device}")
     N, K = w.shape
     q = torch.empty((N, K), dtype=torch.uint8, device=w.device).view(F8)
     scale = torch.empty((_blocks(N), _blocks(K)), dtype=torch.float32, device=w.device)

@@ -69,6 +69,13 @@ def test_norm_forms(K, cuda, T, d, kw):
     run_norm(K, cuda, T, d, **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(y=None), dict(wide=16), dict(in_place="x"), dict(in_place="y"), dict(x32=True), dict(x32=True, y=torch.float32), dict(norm=False, weight=False)])
+@pytest.mark.parametrize("T,d", [(2368, 2048), (2500, 2064), (3001, 8192), (20011, 256), (20011, 16)])
+def test_norm_of_many_rows(K, cuda, T, d, kw):
+    """CTAs that go on from row to row, and rows of a warp each, the last CTA's not all there."""
+    run_norm(K, cuda, T, d, seed=d, **kw)
+
+
 @pytest.mark.parametrize("norm", [True, False])
 @pytest.mark.parametrize("most", [64, 56, 96, 127])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -315,6 +322,14 @@ def test_verify(K, cuda, V, draft, f32):
 @pytest.mark.parametrize("wide", [1, 2, 3, 5, 8])
 def test_verify_rows_that_begin_anywhere(K, cuda, draft, f32, wide):
     check(K, cuda, batch(cuda, [3, 5, 2, 6], 5000, seed=wide, f32=f32, draft=draft, wide=wide))
+
+
+@pytest.mark.parametrize("draft", [None, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("V", [163841, 327681, 600001, 1 << 20])
+def test_verify_long_rows(K, cuda, V, draft, f32):
+    """More chunks than a warp holds, more than a CTA has threads, the largest."""
+    check(K, cuda, batch(cuda, [2, 1, 3], V, seed=V, f32=f32, draft=draft))
 
 
 @pytest.mark.parametrize("draft", [None, torch.float32])

@@ -72,7 +72,7 @@ def test_null_argument_blocks(lib):
 @pytest.mark.parametrize("kw,message", [
     (dict(x=0), "null pointer"), (dict(act=2), "unsupported dtypes"), (dict(y_act=3), "unsupported dtypes"), (dict(T=0), "T = 0"), (dict(T=(1 << 24) + 1), "T = "), (dict(d=0), "d = 0"),
     (dict(d=250), "d = 250"), (dict(d=32784), "d = 32784"), (dict(total=0, out=0, codes=0, scales=0), "no output"), (dict(y=0), "total without y"), (dict(codes=0), "come together"),
-    (dict(scales=0), "come together"), (dict(normed=0), "weight without the norm"), (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(weight=(3 << 24) + 4), "weight must be 16"),
+    (dict(scales=0), "come together"), (dict(normed=0), "weight without the norm"), (dict(eps=0.0), "eps"), (dict(eps=7e-31), "eps"), (dict(eps=float("nan")), "eps"), (dict(weight=(3 << 24) + 4), "weight must be 16"),
     (dict(x_ld=255), "row stride 255 of x"), (dict(y_ld=0), "of y"), (dict(total_ld=-1), "of total"), (dict(scales_ld=1), "of scales"), (dict(x_ld=260), "rows of x must be"),
     (dict(codes_ld=264), "rows of codes must be"), (dict(out=(5 << 24) + 8), "rows of out must be"), (dict(scales=(7 << 24) + 2), "rows of scales must be"),
     (dict(total=1 << 24, total_ld=512), "total [0x1000000] overlaps x"), (dict(total=(1 << 24) + 512), "overlaps x"), (dict(out=1 << 24), "out [0x1000000] overlaps x"),
@@ -102,7 +102,8 @@ def test_linear_refusals(lib, v, kw, message):
     (dict(err=0), "null pointer"), (dict(act=2), "unsupported dtypes"), (dict(draft=11 << 24, draft_act=2), "unsupported dtypes"), (dict(ld=999), "row strides"),
     (dict(draft=11 << 24, draft_ld=999), "row strides"), (dict(logits=(1 << 24) + 2), "aligned to their type"), (dict(draft=(11 << 24) + 1, draft_act=1), "aligned to their type"),
     (dict(ws_bytes=100), "workspace of 100 bytes"), (dict(ws=(9 << 24) + 8), "16-byte aligned"), (dict(next_ids=2 << 24), "next_ids [0x2000000] overlaps ids"), (dict(n_new=5 << 24), "overlaps u_pick"),
-    (dict(logp=6 << 24), "logp [0x6000000] overlaps next_ids"), (dict(ws=1 << 24), "overlaps logits"),
+    (dict(logp=6 << 24), "logp [0x6000000] overlaps next_ids"), (dict(ws=1 << 24), "overlaps logits"), (dict(temperature=7 << 24), "n_new [0x7000000] overlaps temperature"),
+    (dict(temperature=(8 << 24) + 16), "overlaps temperature"), (dict(err=6 << 24), "overlaps err"), (dict(B=8193), "B = 8193"),
 ])
 def test_verify_refusals(lib, kw, message):
     rc, said = verify(lib, **kw)
@@ -147,3 +148,18 @@ def test_python_refuses_before_the_library():
         K.F8View(codes, torch.zeros((1, 1)))
     with pytest.raises(K.Error, match="quantize_f8"):
         K.quantize_f8(torch.zeros((4, 16), dtype=torch.float16))
+    for err in (torch.zeros(2, dtype=torch.int32), torch.zeros(4), torch.zeros(8, dtype=torch.int32)[::2], torch.zeros(4, dtype=torch.int32, device="meta")):
+        with pytest.raises(K.Error, match="quantize_f8: err"):
+            K.quantize_f8(torch.zeros((4, 16)), err=err)
+
+
+def test_quantize_on_another_device_than_the_current(monkeypatch):
+    """Its launch would be the current device's: a stand-in for a weight on a second one."""
+    from strixite_b200 import kernels as K
+
+    class There:
+        dtype, shape, is_cuda, device = torch.float32, (4, 16), True, torch.device("cuda", 1)
+        dim, is_contiguous, get_device = (lambda self: 2), (lambda self: True), (lambda self: 1)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(K.Error, match="lives on device 1, the current device is 0"):
+        K.quantize_f8(There())
