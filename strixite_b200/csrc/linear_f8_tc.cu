@@ -39,6 +39,7 @@ struct TcArgs8 {
     F8Args g;
     int n_m, n_n, band;  // tiles along m and n; tiles along m of a band, in which all of n is gone through
     int split;           // CTAs that share a tile's k (tiles)
+    int rows;            // of x, of a tile of one CTA: up to kTileM, alike in all tiles
     int vec;             // bytes of y that may be stored at once
     int tensor_out;      // y (BF16) takes tensor copies
     int xs4;             // four scales of a row of x may be loaded at once
@@ -206,6 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int group = CTAS == 2 ? 2 : a.split, rank = (int)blockIdx.x % group;  // of the cluster
     const int n_items = a.n_m * a.n_n, first = (int)blockIdx.x / group, step = (int)gridDim.x / group;
+    const int rows = CTAS == 2 ? kTileM : a.rows;
+    auto row_of = [&](const Tile &t) { return CTAS == 2 ? (t.m * 2 + rank) * kTileM : t.m * rows; };  // of x, this CTA's first
     const int kb0 = CTAS == 2 ? 0 : (int)((int64_t)a.g.kb * rank / group), kb1 = CTAS == 2 ? a.g.kb : (int)((int64_t)a.g.kb * (rank + 1) / group);
     volatile int *const abort_v = &abort_flag;
 
@@ -251,10 +254,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (CTAS == 1 && a.split > 1) {
             cluster_meet();  // every part is there
             const Tile t = tile_of(a, first);
-            const int row0 = t.m * kTileM, col0 = t.n * BN;
+            const int row0 = row_of(t), col0 = t.n * BN;
             // four neighbouring columns a thread, in turn the cluster's CTAs', parts in rank order
             if (!*abort_v)
-                for (int i = rank * kThreads + (int)threadIdx.x; i < kTileM * BN / 4; i += group * kThreads) {
+                for (int i = rank * kThreads + (int)threadIdx.x; i < rows * BN / 4; i += group * kThreads) {
                     const int r = i / (BN / 4), c = i % (BN / 4) * 4;
                     if (row0 + r >= a.g.M || col0 + c >= a.g.N) continue;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int issued = 0;
                 for (int item = first; item < n_items && !*abort_v; item += step) {
                     const Tile t = tile_of(a, item);
-                    const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM, wrow = t.n * BN + (CTAS == 2 ? rank * S::kBRows : 0);
+                    const int row = row_of(t), wrow = t.n * BN + (CTAS == 2 ? rank * S::kBRows : 0);
                     for (int kb = kb0; kb < kb1; ++kb, ++issued, turn.advance(kStages)) {
                         if (!mbar_wait(&empty_bar[turn.at], turn.phase, abort_v, a.wait_limit_ns)) {
                             raise_abort(item, 5);
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         if (blockIdx.x == 0 && issued == a.test_skip_slot) continue;
                         const uint32_t dst = smem_u32(smem) + (uint32_t)(turn.at * S::kStageBytes), bar = CTAS == 2 ? in_first_cta(&full_bar[turn.at]) : smem_u32(&full_bar[turn.at]);
-                        if (CTAS == 1 || rank == 0) mbar_expect_tx(&full_bar[turn.at], (uint32_t)(CTAS * S::kStageBytes));
+                        if (CTAS == 1 || rank == 0) mbar_expect_tx(&full_bar[turn.at], (uint32_t)(CTAS * (rows + S::kBRows) * kLine));
                         load_box<CTAS>(dst, &xmap, kb * kLine, row, bar);
                         load_box<CTAS>(dst + kTileM * kLine, &wmap, kb * kLine, wrow, bar);
                     }
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float x[4], w[4];
         };
         auto group_of = [&](const Tile &t, int group) {
-            const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM + quad * 32 + lane, col = t.n * BN + half * kCols, kb = 4 * group;
+            const int row = row_of(t) + quad * 32 + lane, col = t.n * BN + half * kCols, kb = 4 * group;
             Four f{};
             if (row >= a.g.M || col >= a.g.N || kb >= kb1) return f;
             const float *const xs = a.g.xs + (int64_t)row * a.g.xs_ld + kb, *const ws = a.g.ws + (int64_t)(col / kF8Block) * a.g.kb + kb;
@@ -389,8 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         Tile t = tile_of(a, first), then = t;
         Four next = group_of(t, kb0 / 4);
         for (int item = first; item < n_items; item += step, t = then) {
-            const int row = (t.m * CTAS + (CTAS == 2 ? rank : 0)) * kTileM + quad * 32 + lane, col = t.n * BN + half * kCols;
-            const bool there = row < a.g.M;
+            const int row = row_of(t) + quad * 32 + lane, col = t.n * BN + half * kCols;
+            const bool there = quad * 32 + lane < rows && row < a.g.M;
             uint64_t sum[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) sum[i] = 0;
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0 && row < a.g.M) {
+                if (lane == 0 && there) {
 #pragma unroll
                     for (int c = 0; c < kCols; c += 64)
                         if (col + c < a.g.N)
@@ -486,18 +489,23 @@ int shares(int64_t tiles, int64_t kb, int64_t parts) {
 template <int CTAS, int BN>
 int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
     using S = Shape<CTAS, BN>;
+    a.n_m = (a.g.M + kTileM * CTAS - 1) / (kTileM * CTAS);
+    // BF16 rows leave through shared memory, under the next tile's MMAs; a CTA's only tile too (777 x 1000 x 512: 5.4 us, from the registers 6.4)
+    a.tensor_out = !a.g.f32 && a.vec >= 16 && (CTAS == 2 || a.split == 1);
+    // Tiles of a CTA share the rows alike: what the fullest one has to fetch, and in a cluster to add up, bounds the call (150 x 2560 x 4096: 11.7 us, with 128 and 22 rows 13.8; 300 x
+    // 4096 x 4096 14.8 for 17.4).  Tensor copies take 32 rows.
+    const int even = (a.g.M + a.n_m - 1) / a.n_m, by = a.tensor_out ? 32 : 8;
+    a.rows = CTAS == 2 ? kTileM : (even + by - 1) / by * by;
     CUtensorMap xmap, wmap, ymap;
-    if (int rc = tensor_map_2d(fn, a.g.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.M, (uint64_t)a.g.x_ld, kLine, kTileM, CU_TENSOR_MAP_SWIZZLE_128B, &xmap))
+    if (int rc = tensor_map_2d(fn, a.g.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.M, (uint64_t)a.g.x_ld, kLine, (uint32_t)a.rows, CU_TENSOR_MAP_SWIZZLE_128B, &xmap))
         return rc;
     if (int rc = tensor_map_2d(fn, a.g.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)a.g.K, (uint64_t)a.g.N, (uint64_t)a.g.K, kLine, S::kBRows, CU_TENSOR_MAP_SWIZZLE_128B, &wmap))
         return rc;
-    a.n_m = (a.g.M + kTileM * CTAS - 1) / (kTileM * CTAS), a.n_n = (a.g.N + BN - 1) / BN;
+    a.n_n = (a.g.N + BN - 1) / BN;
     a.band = std::min(a.n_m, 16);
     const int64_t items = (int64_t)a.n_m * a.n_n;
     const int cluster = CTAS == 2 ? 2 : a.split;
     const int64_t places = CTAS == 2 ? sm_count() / 2 : a.split > 1 ? items : (int64_t)sm_count();
-    // BF16 rows leave through shared memory, under the next tile's MMAs; a CTA's only tile too (777 x 1000 x 512: 5.4 us, from the registers 6.4)
-    a.tensor_out = !a.g.f32 && a.vec >= 16 && (CTAS == 2 || a.split == 1);
     if (!a.tensor_out) ymap = xmap;  // not used
     else if (int rc = tensor_map_2d(fn, a.g.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.g.N, (uint64_t)a.g.M, (uint64_t)a.g.y_ld * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, &ymap))
         return rc;
