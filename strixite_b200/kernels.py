@@ -691,25 +691,25 @@ def quantize_f8(w: torch.Tensor, err: Optional[torch.Tensor] = None, stream=None
 def add_norm(x, y=None, weight=None, eps=1e-6, total=None, out=None, codes=None, scales=None, norm=True, stream=None):
     """sxb_add_norm: s = x + y in x's type (x [T, d] BF16 or FP32, y BF16, FP32 or None) -> total (may be x or y), its norm times weight [d] FP32 (None: 1) -> out
     BF16, codes float8_e4m3fn with scales [T, ceil(d / 128)] FP32; each of them or None.  norm=False: s itself in the place of its norm."""
-    T, d = x.shape
-    dev, dt = x.get_device(), x.dtype
+    shape, dev, dt = x.shape, x.get_device(), x.dtype
+    T, d = shape
     ok = dev == torch._C._cuda_getDevice() and dt in _ROWS and (x.is_contiguous() or x.stride(1) == 1)
     yp = wp = tp = op = cp = sp = 0
     y_ld = t_ld = o_ld = c_ld = s_ld = d
     if y is not None:
-        ok = ok and y.dtype in _ROWS and y.get_device() == dev and y.shape == x.shape and (y.is_contiguous() or y.stride(1) == 1)
+        ok = ok and y.dtype in _ROWS and y.get_device() == dev and y.shape == shape and (y.is_contiguous() or y.stride(1) == 1)
         yp, y_ld = y.data_ptr(), y.stride(0)
     if weight is not None:
-        ok = ok and weight.dtype is torch.float32 and weight.get_device() == dev and weight.is_contiguous() and weight.shape == (d,)
+        ok = ok and weight.dtype is torch.float32 and weight.get_device() == dev and weight.is_contiguous() and weight.numel() == d
         wp = weight.data_ptr()
     if total is not None:
-        ok = ok and total.dtype is dt and total.get_device() == dev and total.shape == x.shape and (total.is_contiguous() or total.stride(1) == 1)
+        ok = ok and total.dtype is dt and total.get_device() == dev and total.shape == shape and (total.is_contiguous() or total.stride(1) == 1)
         tp, t_ld = total.data_ptr(), total.stride(0)
     if out is not None:
-        ok = ok and out.dtype is torch.bfloat16 and out.get_device() == dev and out.shape == x.shape and (out.is_contiguous() or out.stride(1) == 1)
+        ok = ok and out.dtype is torch.bfloat16 and out.get_device() == dev and out.shape == shape and (out.is_contiguous() or out.stride(1) == 1)
         op, o_ld = out.data_ptr(), out.stride(0)
     if codes is not None:
-        ok = ok and codes.dtype is F8 and codes.get_device() == dev and codes.shape == x.shape and (codes.is_contiguous() or codes.stride(1) == 1)
+        ok = ok and codes.dtype is F8 and codes.get_device() == dev and codes.shape == shape and (codes.is_contiguous() or codes.stride(1) == 1)
         cp, c_ld = codes.data_ptr(), codes.stride(0)
     if scales is not None:
         ok = ok and scales.dtype is torch.float32 and scales.get_device() == dev and scales.shape == (T, -(-d // _F8_BLOCK)) and (scales.is_contiguous() or scales.stride(1) == 1)
@@ -720,7 +720,7 @@ def add_norm(x, y=None, weight=None, eps=1e-6, total=None, out=None, codes=None,
         y_ld, t_ld, o_ld, c_ld, s_ld = d, d, d, d, -(-d // _F8_BLOCK)
     _check(_lib.load().sxb_add_norm(_NORM_ARGS.pack(
         x.data_ptr(), yp, wp, tp, op, cp, sp, T, d, x.stride(0) if T > 1 else d, y_ld, t_ld, o_ld, c_ld, s_ld, eps, dt is torch.bfloat16, y is not None and y.dtype is torch.bfloat16,
-        bool(norm)), _stream(stream)))
+        bool(norm)), torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)))
 
 
 def linear_f8(x, x_scale, w: F8View, y, stream=None):
@@ -734,7 +734,7 @@ def linear_f8(x, x_scale, w: F8View, y, stream=None):
     many = M > 1
     _check(_lib.load().sxb_linear_f8(_LINEAR_F8_ARGS.pack(
         x.data_ptr(), x_scale.data_ptr(), w._at, y.data_ptr(), M, x.stride(0) if many else K, x_scale.stride(0) if many else w.blocks, y.stride(0) if many else w.N,
-        dt is torch.bfloat16), _stream(stream)))
+        dt is torch.bfloat16), torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)))
 
 
 def verify_drafts_workspace_bytes(T: int, B: int, V: int) -> int:
@@ -749,26 +749,25 @@ def verify_drafts(logits, ids, q_start, u, u_pick, next_ids, n_new, ws, err, dra
     """sxb_verify_drafts: rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]) are sequence b's: the tokens ids [T] int32 fed there, the drafted ones behind the first, the target's
     logits [T, V] BF16 or FP32, the drafter's (or None: its tokens are all that is known of it), random numbers u [T] and u_pick [B] FP32, temperature [B] FP32 (None: 1; 0: greedy)
     -> next_ids [T] int32 (-1 behind the last), n_new [B] int32, logp [T] FP32 or None.  err: 3 or more zeroed int32."""
-    T, V = logits.shape
-    dev, B = logits.get_device(), n_new.shape[0]
-    rows, seqs = (T,), (B,)
+    shape, dev, B = logits.shape, logits.get_device(), n_new.numel()
+    T, V = shape
     ok = (dev == torch._C._cuda_getDevice() and logits.dtype in _ROWS and (logits.is_contiguous() or logits.stride(1) == 1 or V == 1) and ids.dtype is torch.int32 and ids.get_device() == dev
-          and ids.shape == rows and ids.is_contiguous() and q_start.dtype is torch.int32 and q_start.get_device() == dev and q_start.shape == (B + 1,) and q_start.is_contiguous()
-          and u.dtype is torch.float32 and u.get_device() == dev and u.shape == rows and u.is_contiguous() and u_pick.dtype is torch.float32 and u_pick.get_device() == dev
-          and u_pick.shape == seqs and u_pick.is_contiguous() and next_ids.dtype is torch.int32 and next_ids.get_device() == dev and next_ids.shape == rows and next_ids.is_contiguous()
-          and n_new.dtype is torch.int32 and n_new.get_device() == dev and n_new.dim() == 1 and n_new.is_contiguous() and ws.get_device() == dev and ws.is_contiguous()
+          and ids.numel() == T and ids.is_contiguous() and q_start.dtype is torch.int32 and q_start.get_device() == dev and q_start.numel() == B + 1 and q_start.is_contiguous()
+          and u.dtype is torch.float32 and u.get_device() == dev and u.numel() == T and u.is_contiguous() and u_pick.dtype is torch.float32 and u_pick.get_device() == dev
+          and u_pick.numel() == B and u_pick.is_contiguous() and next_ids.dtype is torch.int32 and next_ids.get_device() == dev and next_ids.numel() == T and next_ids.is_contiguous()
+          and n_new.dtype is torch.int32 and n_new.get_device() == dev and n_new.is_contiguous() and ws.get_device() == dev and ws.is_contiguous()
           and err.get_device() == dev and err.dtype in _WORDS and err.is_contiguous() and err.numel() >= 3)
     dp = tp = lp = d_bf16 = 0
     dld = V
     if draft_logits is not None:
         d = draft_logits
-        ok = ok and d.dtype in _ROWS and d.get_device() == dev and d.shape == logits.shape and (d.is_contiguous() or d.stride(1) == 1 or V == 1)
+        ok = ok and d.dtype in _ROWS and d.get_device() == dev and d.shape == shape and (d.is_contiguous() or d.stride(1) == 1 or V == 1)
         dp, dld, d_bf16 = d.data_ptr(), d.stride(0), d.dtype is torch.bfloat16
     if temperature is not None:
-        ok = ok and temperature.dtype is torch.float32 and temperature.get_device() == dev and temperature.shape == seqs and temperature.is_contiguous()
+        ok = ok and temperature.dtype is torch.float32 and temperature.get_device() == dev and temperature.numel() == B and temperature.is_contiguous()
         tp = temperature.data_ptr()
     if logp is not None:
-        ok = ok and logp.dtype is torch.float32 and logp.get_device() == dev and logp.shape == rows and logp.is_contiguous()
+        ok = ok and logp.dtype is torch.float32 and logp.get_device() == dev and logp.numel() == T and logp.is_contiguous()
         lp = logp.data_ptr()
     if not ok:
         _refuse_all(dev, "verify_drafts", logits=(logits, _ROWS), draft_logits=(draft_logits, _ROWS), ids=(ids, _I32), q_start=(q_start, _I32), u=(u, _F32), u_pick=(u_pick, _F32),
@@ -777,7 +776,8 @@ def verify_drafts(logits, ids, q_start, u, u_pick, next_ids, n_new, ws, err, dra
     _count()  # two launches
     _check(_lib.load().sxb_verify_drafts(_VERIFY_ARGS.pack(
         logits.data_ptr(), dp, logits.stride(0) if many else V, dld if many else V, T, V, B, ids.data_ptr(), q_start.data_ptr(), u.data_ptr(), u_pick.data_ptr(), tp,
-        next_ids.data_ptr(), n_new.data_ptr(), lp, ws.data_ptr(), ws.nbytes, err.data_ptr(), logits.dtype is torch.bfloat16, d_bf16), _stream(stream)))
+        next_ids.data_ptr(), n_new.data_ptr(), lp, ws.data_ptr(), ws.nbytes, err.data_ptr(), logits.dtype is torch.bfloat16, d_bf16),
+        torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)))
 
 
 def check_verify_error(err, what: str):
