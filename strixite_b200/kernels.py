@@ -649,6 +649,13 @@ def _refuse_all(dev, what, **tensors):
     raise Error(1, f"{what}: a vector is not contiguous, or the shapes do not fit: " + ", ".join(f"{n} {tuple(t.shape)}" for n, (t, _) in tensors.items() if t is not None))
 
 
+def _ld(t, what: str, name: str) -> int:
+    """The row stride of a tensor that is not contiguous.  (The wrappers below ask for no strides of those that are: each costs 0.17 us.)"""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1):
+        raise Error(1, f"{what}: {name} is {tuple(t.shape)} with strides {tuple(t.stride())}, expected two dimensions, the last one contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 class F8View:
     """A weight in 8-bit floating point (SxbF8View): codes q [N, K] float8_e4m3fn, contiguous, scale [ceil(N / 128), ceil(K / 128)] FP32."""
 
@@ -693,34 +700,44 @@ def add_norm(x, y=None, weight=None, eps=1e-6, total=None, out=None, codes=None,
     BF16, codes float8_e4m3fn with scales [T, ceil(d / 128)] FP32; each of them or None.  norm=False: s itself in the place of its norm."""
     shape, dev, dt = x.shape, x.get_device(), x.dtype
     T, d = shape
-    ok = dev == torch._C._cuda_getDevice() and dt in _ROWS and (x.is_contiguous() or x.stride(1) == 1)
-    yp = wp = tp = op = cp = sp = 0
+    ok = dev == torch._C._cuda_getDevice() and dt in _ROWS
+    x_ld = d if x.is_contiguous() else _ld(x, "add_norm", "x")
+    yp = wp = tp = op = cp = sp = y_bf16 = 0
     y_ld = t_ld = o_ld = c_ld = s_ld = d
     if y is not None:
-        ok = ok and y.dtype in _ROWS and y.get_device() == dev and y.shape == shape and (y.is_contiguous() or y.stride(1) == 1)
-        yp, y_ld = y.data_ptr(), y.stride(0)
+        ok = ok and y.dtype in _ROWS and y.get_device() == dev and y.shape == shape
+        yp, y_bf16 = y.data_ptr(), y.dtype is torch.bfloat16
+        if not y.is_contiguous():
+            y_ld = _ld(y, "add_norm", "y")
     if weight is not None:
         ok = ok and weight.dtype is torch.float32 and weight.get_device() == dev and weight.is_contiguous() and weight.numel() == d
         wp = weight.data_ptr()
     if total is not None:
-        ok = ok and total.dtype is dt and total.get_device() == dev and total.shape == shape and (total.is_contiguous() or total.stride(1) == 1)
-        tp, t_ld = total.data_ptr(), total.stride(0)
+        ok = ok and total.dtype is dt and total.get_device() == dev and total.shape == shape
+        tp = total.data_ptr()
+        if not total.is_contiguous():
+            t_ld = _ld(total, "add_norm", "total")
     if out is not None:
-        ok = ok and out.dtype is torch.bfloat16 and out.get_device() == dev and out.shape == shape and (out.is_contiguous() or out.stride(1) == 1)
-        op, o_ld = out.data_ptr(), out.stride(0)
+        ok = ok and out.dtype is torch.bfloat16 and out.get_device() == dev and out.shape == shape
+        op = out.data_ptr()
+        if not out.is_contiguous():
+            o_ld = _ld(out, "add_norm", "out")
     if codes is not None:
-        ok = ok and codes.dtype is F8 and codes.get_device() == dev and codes.shape == shape and (codes.is_contiguous() or codes.stride(1) == 1)
-        cp, c_ld = codes.data_ptr(), codes.stride(0)
+        ok = ok and codes.dtype is F8 and codes.get_device() == dev and codes.shape == shape
+        cp = codes.data_ptr()
+        if not codes.is_contiguous():
+            c_ld = _ld(codes, "add_norm", "codes")
     if scales is not None:
-        ok = ok and scales.dtype is torch.float32 and scales.get_device() == dev and scales.shape == (T, -(-d // _F8_BLOCK)) and (scales.is_contiguous() or scales.stride(1) == 1)
-        sp, s_ld = scales.data_ptr(), scales.stride(0)
+        s_ld = -(-d // _F8_BLOCK)
+        ok = ok and scales.dtype is torch.float32 and scales.get_device() == dev and scales.shape == (T, s_ld)
+        sp = scales.data_ptr()
+        if not scales.is_contiguous():
+            s_ld = _ld(scales, "add_norm", "scales")
     if not ok:
         _refuse_all(dev, "add_norm", x=(x, _ROWS), y=(y, _ROWS), weight=(weight, _F32), total=(total, (dt,)), out=(out, _BF16), codes=(codes, (F8,)), scales=(scales, _F32))
-    if T == 1:  # a single row's stride may be anything
-        y_ld, t_ld, o_ld, c_ld, s_ld = d, d, d, d, -(-d // _F8_BLOCK)
     _check(_lib.load().sxb_add_norm(_NORM_ARGS.pack(
-        x.data_ptr(), yp, wp, tp, op, cp, sp, T, d, x.stride(0) if T > 1 else d, y_ld, t_ld, o_ld, c_ld, s_ld, eps, dt is torch.bfloat16, y is not None and y.dtype is torch.bfloat16,
-        bool(norm)), torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)))
+        x.data_ptr(), yp, wp, tp, op, cp, sp, T, d, x_ld, y_ld, t_ld, o_ld, c_ld, s_ld, eps, dt is torch.bfloat16, y_bf16, bool(norm)),
+        torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)))
 
 
 def linear_f8(x, x_scale, w: F8View, y, stream=None):
@@ -728,12 +745,11 @@ def linear_f8(x, x_scale, w: F8View, y, stream=None):
     M, K = x.shape
     dev, dt = w.index, y.dtype
     if not (dev == torch._C._cuda_getDevice() and x.dtype is F8 and x_scale.dtype is torch.float32 and dt in _ROWS and x.get_device() == dev and x_scale.get_device() == dev
-            and y.get_device() == dev and K == w.K and x_scale.shape == (M, w.blocks) and y.shape == (M, w.N) and (x.is_contiguous() or x.stride(1) == 1)
-            and (x_scale.is_contiguous() or x_scale.stride(1) == 1 or w.blocks == 1) and (y.is_contiguous() or y.stride(1) == 1 or w.N == 1)):
+            and y.get_device() == dev and K == w.K and x_scale.shape == (M, w.blocks) and y.shape == (M, w.N)):
         _refuse_all(dev, "linear_f8", x=(x, (F8,)), x_scale=(x_scale, _F32), w=(w.q, (F8,)), y=(y, _ROWS))
-    many = M > 1
     _check(_lib.load().sxb_linear_f8(_LINEAR_F8_ARGS.pack(
-        x.data_ptr(), x_scale.data_ptr(), w._at, y.data_ptr(), M, x.stride(0) if many else K, x_scale.stride(0) if many else w.blocks, y.stride(0) if many else w.N,
+        x.data_ptr(), x_scale.data_ptr(), w._at, y.data_ptr(), M, K if x.is_contiguous() else _ld(x, "linear_f8", "x"),
+        w.blocks if x_scale.is_contiguous() else _ld(x_scale, "linear_f8", "x_scale"), w.N if y.is_contiguous() else _ld(y, "linear_f8", "y"),
         dt is torch.bfloat16), torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)))
 
 
@@ -751,18 +767,21 @@ def verify_drafts(logits, ids, q_start, u, u_pick, next_ids, n_new, ws, err, dra
     -> next_ids [T] int32 (-1 behind the last), n_new [B] int32, logp [T] FP32 or None.  err: 3 or more zeroed int32."""
     shape, dev, B = logits.shape, logits.get_device(), n_new.numel()
     T, V = shape
-    ok = (dev == torch._C._cuda_getDevice() and logits.dtype in _ROWS and (logits.is_contiguous() or logits.stride(1) == 1 or V == 1) and ids.dtype is torch.int32 and ids.get_device() == dev
+    ok = (dev == torch._C._cuda_getDevice() and logits.dtype in _ROWS and ids.dtype is torch.int32 and ids.get_device() == dev
           and ids.numel() == T and ids.is_contiguous() and q_start.dtype is torch.int32 and q_start.get_device() == dev and q_start.numel() == B + 1 and q_start.is_contiguous()
           and u.dtype is torch.float32 and u.get_device() == dev and u.numel() == T and u.is_contiguous() and u_pick.dtype is torch.float32 and u_pick.get_device() == dev
           and u_pick.numel() == B and u_pick.is_contiguous() and next_ids.dtype is torch.int32 and next_ids.get_device() == dev and next_ids.numel() == T and next_ids.is_contiguous()
           and n_new.dtype is torch.int32 and n_new.get_device() == dev and n_new.is_contiguous() and ws.get_device() == dev and ws.is_contiguous()
           and err.get_device() == dev and err.dtype in _WORDS and err.is_contiguous() and err.numel() >= 3)
     dp = tp = lp = d_bf16 = 0
+    ld = V if logits.is_contiguous() else _ld(logits, "verify_drafts", "logits")
     dld = V
     if draft_logits is not None:
         d = draft_logits
-        ok = ok and d.dtype in _ROWS and d.get_device() == dev and d.shape == shape and (d.is_contiguous() or d.stride(1) == 1 or V == 1)
-        dp, dld, d_bf16 = d.data_ptr(), d.stride(0), d.dtype is torch.bfloat16
+        ok = ok and d.dtype in _ROWS and d.get_device() == dev and d.shape == shape
+        dp, d_bf16 = d.data_ptr(), d.dtype is torch.bfloat16
+        if not d.is_contiguous():
+            dld = _ld(d, "verify_drafts", "draft_logits")
     if temperature is not None:
         ok = ok and temperature.dtype is torch.float32 and temperature.get_device() == dev and temperature.numel() == B and temperature.is_contiguous()
         tp = temperature.data_ptr()
@@ -772,10 +791,9 @@ def verify_drafts(logits, ids, q_start, u, u_pick, next_ids, n_new, ws, err, dra
     if not ok:
         _refuse_all(dev, "verify_drafts", logits=(logits, _ROWS), draft_logits=(draft_logits, _ROWS), ids=(ids, _I32), q_start=(q_start, _I32), u=(u, _F32), u_pick=(u_pick, _F32),
                     temperature=(temperature, _F32), next_ids=(next_ids, _I32), n_new=(n_new, _I32), logp=(logp, _F32), ws=(ws, (ws.dtype,)), err=(err, _WORDS))
-    many = T > 1  # a single row's stride may be anything
     _count()  # two launches
     _check(_lib.load().sxb_verify_drafts(_VERIFY_ARGS.pack(
-        logits.data_ptr(), dp, logits.stride(0) if many else V, dld if many else V, T, V, B, ids.data_ptr(), q_start.data_ptr(), u.data_ptr(), u_pick.data_ptr(), tp,
+        logits.data_ptr(), dp, ld, dld, T, V, B, ids.data_ptr(), q_start.data_ptr(), u.data_ptr(), u_pick.data_ptr(), tp,
         next_ids.data_ptr(), n_new.data_ptr(), lp, ws.data_ptr(), ws.nbytes, err.data_ptr(), logits.dtype is torch.bfloat16, d_bf16),
         torch._C._cuda_getCurrentRawStream(dev) if stream is None else _stream(stream)))
 
