@@ -201,37 +201,46 @@ __device__ inline ChunkStat chunk_stat(const Row<T> &r, int chunk, const Loaded 
     return ChunkStat{(double)s, most, at};
 }
 
-// The warps' chunks: an equal run of all rows' each, the next chunk asked for ahead of the work on one.
-template <typename T>
-__device__ inline void stats_run(const VerifyArgs &a, const void *base, int64_t ld, ChunkStat *out, bool drafter, int block, int blocks) {
+// The warps' chunks: an equal run of all rows' each, the next chunk asked for ahead of the work on one.  What a row's sequence says is looked up behind its first chunk's loads, but ahead of
+// the drafter's: a sequence's last row has no draft behind it, a greedy one's drafter is not asked, and those are not read.
+template <typename T, bool DRAFTER>
+__device__ inline void stats_run(const VerifyArgs &a, const void *base, int64_t ld, ChunkStat *out, int block, int blocks) {
     const int lane = threadIdx.x & 31, n = (a.V + Row<T>::VE - 1 + Row<T>::kChunk - 1) / Row<T>::kChunk;  // of a row that begins at a piece's last token
     const int64_t units = (int64_t)a.T * n, warps = (int64_t)blocks * (kStatThreads / 32), w = (int64_t)block * (kStatThreads / 32) + (threadIdx.x >> 5);
     const int64_t lo = units * w / warps, hi = units * (w + 1) / warps;
     if (lo >= hi) return;
     int row = (int)(lo / n), chunk = (int)(lo % n);
-    Loaded now, next;
-    load_chunk(Row<T>(base, ld, row, a.V), chunk, now);
     float c = kLog2e;
-    bool greedy = false, wanted = true;
-    int known = -1;
+    bool greedy = false, wanted = true, wanted2 = true;
+    auto look_up = [&](int of) {  // -> wanted
+        const int b = sequence_of(a.q_start, a.B, of);
+        const float t = b >= 0 && a.temperature != nullptr ? a.temperature[b] : 1.f;
+        c = exponent_scale(t), greedy = t == 0.f;
+        return b >= 0 && !(DRAFTER && (of + 1 == a.q_start[b + 1] || greedy));
+    };
+    Loaded now, next;
+    if (DRAFTER) wanted = look_up(row);
+    if (wanted) load_chunk(Row<T>(base, ld, row, a.V), chunk, now);
+    int known = DRAFTER ? row : -1;
     for (int64_t i = lo; i < hi; ++i) {
         int row2 = row, chunk2 = chunk + 1;
         if (chunk2 == n) ++row2, chunk2 = 0;
-        if (i + 1 < hi) load_chunk(Row<T>(base, ld, row2, a.V), chunk2, next);
-        if (row != known) {
+        const float c0 = c;
+        if (i + 1 < hi) {
+            if (DRAFTER && row2 != row) wanted2 = look_up(row2);
+            else wanted2 = wanted;
+            if (!DRAFTER || wanted2) load_chunk(Row<T>(base, ld, row2, a.V), chunk2, next);
+        }
+        if (!DRAFTER && row != known) {
             known = row;
-            if (a.temperature != nullptr || drafter) {
-                const int b = sequence_of(a.q_start, a.B, row);
-                const float t = b >= 0 && a.temperature != nullptr ? a.temperature[b] : 1.f;
-                wanted = b >= 0 && !(drafter && (row + 1 == a.q_start[b + 1] || t == 0.f));  // a sequence's last row has no draft behind it, a greedy one's drafter is not asked
-                c = exponent_scale(t), greedy = t == 0.f;
-            }
+            if (a.temperature != nullptr) wanted = look_up(row);
         }
         if (wanted) {
-            const ChunkStat s = chunk_stat<T>(Row<T>(base, ld, row, a.V), chunk, now, c, greedy);
+            const ChunkStat s = chunk_stat<T>(Row<T>(base, ld, row, a.V), chunk, now, DRAFTER ? c0 : c, !DRAFTER && greedy);
             if (lane == 0) out[(int64_t)row * a.pitch + chunk] = s;
         }
         row = row2, chunk = chunk2, now = next;
+        if (DRAFTER) wanted = wanted2;
     }
 }
 
@@ -239,9 +248,9 @@ template <typename TX, typename TD>
 __global__ void __launch_bounds__(kStatThreads, kStatCtas) verify_stats_kernel(const VerifyArgs a) {
     behind_grid();
     // half the CTAs have the drafter's rows
-    if (a.draft == nullptr) stats_run<TX>(a, a.logits, a.ld, a.stats, false, (int)blockIdx.x, (int)gridDim.x);
-    else if ((blockIdx.x & 1) == 0) stats_run<TX>(a, a.logits, a.ld, a.stats, false, (int)blockIdx.x / 2, (int)gridDim.x / 2);
-    else stats_run<TD>(a, a.draft, a.draft_ld, a.stats + (int64_t)a.T * a.pitch, true, (int)blockIdx.x / 2, (int)gridDim.x / 2);
+    if (a.draft == nullptr) stats_run<TX, false>(a, a.logits, a.ld, a.stats, (int)blockIdx.x, (int)gridDim.x);
+    else if ((blockIdx.x & 1) == 0) stats_run<TX, false>(a, a.logits, a.ld, a.stats, (int)blockIdx.x / 2, (int)gridDim.x / 2);
+    else stats_run<TD, true>(a, a.draft, a.draft_ld, a.stats + (int64_t)a.T * a.pitch, (int)blockIdx.x / 2, (int)gridDim.x / 2);
 }
 
 // log2 of 2^(c (x - best)), exact but for FP64's rounding.
