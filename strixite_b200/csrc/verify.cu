@@ -6,6 +6,9 @@
 // falls and reads that one again; only a difference of two distributions takes the whole row of both, once more, shared by the cluster.  It is bound by its chain of loads, of which
 // those that do not wait for the first launch are made ahead of its end.  Nothing is counted or left behind in the workspace: no atomics, and results do not depend on who comes first.
 //
+// 64 sequences of 1 to 8 rows of 131072 BF16 logits, the drafter's too (134 MB): 30 us (4.5 TB/s; half the issue slots and half the special-function unit's) and 15; 2 sequences of 8 rows of
+// FP32 8.3 together, one row 6.3.  A CTA a chunk, its parts joined by barriers, took 108 us for the 64 sequences where a warp a chunk takes 52 (before the differences were read by batches).
+//
 // A border's error: a term takes c (x - max) in FP32 (2^-23 of the exponent, which is small where the term is large), one ex2 (2^-22), sums of up to sixteen
 // terms and then seven more in FP32; chunks are joined in FP64, where the exponents are exact, and no logit is too large for them.
 
