@@ -339,6 +339,12 @@ def test_verify_many_sequences(K, cuda, draft):
     assert n.min() == 1 and n.max() == 5  # some of everything
 
 
+@pytest.mark.parametrize("draft", [None, torch.bfloat16])
+def test_verify_the_most_sequences(K, cuda, draft):
+    ids, n, _ = check(K, cuda, batch(cuda, [1 + (b % 7 == 3) for b in range(8192)], 130, seed=16, draft=draft, greedy=True))
+    assert n.min() == 1 and n.max() == 2
+
+
 @pytest.mark.parametrize("draft", [None, torch.float32])
 def test_verify_long_runs_of_drafts(K, cuda, draft):
     """More rows of one sequence than a CTA has warps, kept to the end and refused far inside."""
