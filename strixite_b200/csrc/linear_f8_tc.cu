@@ -35,7 +35,7 @@ struct Shape {
     static constexpr int kAccs = 512 / BN;                                     // accumulators: all of tensor memory
     static constexpr size_t kRing = (size_t)kStages * kStageBytes, kOut = (size_t)kTileM * BN * 2;  // and a tile's rows of y in BF16, on their way out
     static constexpr size_t kSmem = kRing + kOut + 1024;
-    static_assert(kSmem <= 226 * 1024 && (CTAS == 2 || (size_t)kTileM * BN * 4 <= kRing));
+    static_assert(kOut >= kSumWarps * 4096 && kSmem <= 226 * 1024 && (CTAS == 2 || (size_t)kTileM * BN * 4 <= kRing));
 };
 
 struct TcArgs8 {
@@ -151,30 +151,23 @@ __device__ inline void store32(void *p, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
-// Values to y at `at`, `left` of which lie inside the row.  (BF16 rows that sixteen bytes may be stored to at once leave by tensor copies.)
+// FP32 values to y at `at`, 16-byte aligned, `left` of which lie inside the row.
 template <int NV>
 __device__ inline void store_run(const TcArgs8 &a, int64_t at, int left, const float (&v)[NV]) {
-    if (a.g.f32) {
-        float *p = static_cast<float *>(a.g.y) + at;
+    float *p = static_cast<float *>(a.g.y) + at;
 #pragma unroll
-        for (int i = 0; i < NV; i += 8) {
-            uint32_t w[8];
+    for (int i = 0; i < NV; i += 8) {
+        uint32_t w[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(v[i + k]);
-            if (i + 8 <= left && a.vec >= 32) store32(p + i, w);
-            else if (i + 8 <= left && a.vec >= 16) {
-                reinterpret_cast<uint4 *>(p + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                reinterpret_cast<uint4 *>(p + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-            } else
+        for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(v[i + k]);
+        if (i + 8 <= left && a.vec >= 32) store32(p + i, w);
+        else if (i + 8 <= left) {
+            reinterpret_cast<uint4 *>(p + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4 *>(p + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (i + k < left) p[i + k] = v[i + k];
-        }
-    } else {
-        uint16_t *p = static_cast<uint16_t *>(a.g.y) + at;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (i < left) p[i] = f32_to_bf16_bits(v[i]);
+            for (int k = 0; k < 8; ++k)
+                if (i + k < left) p[i + k] = v[i + k];
     }
 }
 
@@ -465,13 +458,45 @@ __global__ void __launch_bounds__(kThreads, 1)
                                          : "memory");
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
-            } else if (there) {
+            } else if (a.g.f32 && a.vec >= 16) {
+                if (there)
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 32) {
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) unpair(sum[c / 2 + i], v[2 * i], v[2 * i + 1]);
+                        store_run(a, (int64_t)row * a.g.y_ld + col + c, a.g.N - col - c, v);
+                    }
+            } else {
+                // rows that sixteen bytes may not be stored to: 32 x 32 values change places in shared memory (the column's by the row, so that both ways touch all banks), and a row's
+                // leave side by side (1049 x 2852 x 1168: 15.7 us, each thread along its own row 49.6; 4139 x 1827 x 448 23 and 89)
+                float *const turned = reinterpret_cast<float *>(smem + S::kRing) + warp * 1024;
+                const int n = min(32, min(rows - quad * 32, a.g.M - (row - lane)));
 #pragma unroll
                 for (int c = 0; c < kCols; c += 32) {
-                    float v[32];
+                    __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[2 * i] = __uint_as_float((uint32_t)sum[c / 2 + i]), v[2 * i + 1] = __uint_as_float((uint32_t)(sum[c / 2 + i] >> 32));
-                    store_run(a, (int64_t)row * a.g.y_ld + col + c, a.g.N - col - c, v);
+                    for (int i = 0; i < 16; ++i) unpair(sum[c / 2 + i], turned[lane * 32 + (2 * i ^ lane)], turned[lane * 32 + (2 * i + 1 ^ lane)]);
+                    __syncwarp();
+                    if (!a.g.f32 && a.vec >= 4) {  // two columns a lane, two rows at once
+                        const int k = 2 * (lane & 15), left = a.g.N - col - c - k;
+                        uint16_t *const p = static_cast<uint16_t *>(a.g.y) + (int64_t)(row - lane) * a.g.y_ld + col + c + k;
+                        if (left > 0)
+#pragma unroll 8
+                            for (int r = lane >> 4; r < n; r += 2) {
+                                const uint32_t w = bf16_pair(turned[r * 32 + (k ^ r)], turned[r * 32 + (k + 1 ^ r)]);
+                                if (left > 1) *reinterpret_cast<uint32_t *>(p + r * a.g.y_ld) = w;
+                                else p[r * a.g.y_ld] = (uint16_t)w;
+                            }
+                    } else if (col + c + lane < a.g.N) {
+                        const int64_t at = (int64_t)(row - lane) * a.g.y_ld + col + c + lane;
+#pragma unroll 8
+                        for (int r = 0; r < n; ++r) {
+                            const float v = turned[r * 32 + (lane ^ r)];
+                            if (a.g.f32) static_cast<float *>(a.g.y)[at + r * a.g.y_ld] = v;
+                            else static_cast<uint16_t *>(a.g.y)[at + r * a.g.y_ld] = f32_to_bf16_bits(v);
+                        }
+                    }
                 }
             }
         }
@@ -740,7 +765,7 @@ int linear_f8_tc(const char *fn, const F8Args &g, cudaStream_t st) {
     TcArgs8 a{};
     a.g = g;
     const int64_t es = g.f32 ? 4 : 2;
-    for (a.vec = 32; a.vec > 4 && (reinterpret_cast<uintptr_t>(g.y) % a.vec != 0 || g.y_ld * es % a.vec != 0); a.vec /= 2) {}
+    for (a.vec = 32; a.vec > 2 && (reinterpret_cast<uintptr_t>(g.y) % a.vec != 0 || g.y_ld * es % a.vec != 0); a.vec /= 2) {}
     a.xs4 = reinterpret_cast<uintptr_t>(g.xs) % 16 == 0 && g.xs_ld % 4 == 0;
     a.wait_limit_ns = wait_limit_ns(), a.test_skip_slot = test_skip_slot();
     if (int rc = library_status_words(fn, &a.status)) return rc;
