@@ -189,7 +189,8 @@ __device__ inline Tile tile_of(const TcArgs8 &a, int item) {  // at most 2^13 x 
     return Tile{b * a.band + rest % in_band, rest / in_band};
 }
 
-template <int CTAS, int BN>
+// TENSOR: y leaves by tensor copies, and a pair's kernel knows no other way (with all of them in one the compiler holds the sums worse: 8192 x 8192 x 4096 271 us, so 241).
+template <int CTAS, int BN, bool TENSOR>
 __global__ void __launch_bounds__(kThreads, 1)
     f8_tc_kernel(const TcArgs8 a, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap ymap) {
     using S = Shape<CTAS, BN>;
@@ -434,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float *const to = reinterpret_cast<float *>(smem) + r * BN;
 #pragma unroll
                 for (int i = 0; i < kCols / 2; i += 2) *reinterpret_cast<ulonglong2 *>(to + ((half * kCols + 2 * i) ^ (r & 7) * 4)) = make_ulonglong2(sum[i], sum[i + 1]);
-            } else if (a.tensor_out) {
+            } else if (TENSOR || (CTAS == 1 && a.tensor_out)) {
                 // rows of 64 columns, 128 bytes, their 16-byte pieces swizzled: eight lanes' stores touch all banks; a warp's 32 rows are a box of their own
                 unsigned char *const out = smem + S::kRing + quad * 32 * 128;
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile's have been read
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                          : "memory");
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
-            } else if (a.g.f32 && a.vec >= 16) {
+            } else if (!TENSOR && a.g.f32 && a.vec >= 16) {
                 if (there)
 #pragma unroll
                     for (int c = 0; c < kCols; c += 32) {
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int i = 0; i < 16; ++i) unpair(sum[c / 2 + i], v[2 * i], v[2 * i + 1]);
                         store_run(a, (int64_t)row * a.g.y_ld + col + c, a.g.N - col - c, v);
                     }
-            } else {
+            } else if constexpr (!TENSOR) {
                 // rows that sixteen bytes may not be stored to: 32 x 32 values change places in shared memory (the column's by the row, so that both ways touch all banks), and a row's
                 // leave side by side (1049 x 2852 x 1168: 15.7 us, each thread along its own row 49.6; 4139 x 1827 x 448 23 and 89)
                 float *const turned = reinterpret_cast<float *>(smem + S::kRing) + warp * 1024;
@@ -537,8 +538,11 @@ int launch_tc8(const char *fn, TcArgs8 a, cudaStream_t st) {
     if (!a.tensor_out) ymap = xmap;  // not used
     else if (int rc = tensor_map_2d(fn, a.g.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (uint64_t)a.g.N, (uint64_t)a.g.M, (uint64_t)a.g.y_ld * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, &ymap))
         return rc;
-    SXB_CUDA(cudaFuncSetAttribute(f8_tc_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), fn, ": reserving shared memory");
-    const cudaError_t e = launch_behind(f8_tc_kernel<CTAS, BN>, dim3((unsigned)(std::min(items, places) * cluster)), dim3(kThreads), S::kSmem, st, cluster, a, xmap, wmap, ymap);
+    auto *kern = f8_tc_kernel<CTAS, BN, false>;
+    if constexpr (CTAS == 2)
+        if (a.tensor_out) kern = f8_tc_kernel<CTAS, BN, true>;
+    SXB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem), fn, ": reserving shared memory");
+    const cudaError_t e = launch_behind(kern, dim3((unsigned)(std::min(items, places) * cluster)), dim3(kThreads), S::kSmem, st, cluster, a, xmap, wmap, ymap);
     SXB_CUDA(e, fn, ": launching M=", a.g.M, " N=", a.g.N, " K=", a.g.K);
     return SXB_OK;
 }
