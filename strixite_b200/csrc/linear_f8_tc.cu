@@ -7,7 +7,7 @@
 // Warp 8 brings x and w in stages of 128 k by tensor copies, warp 9 issues the MMAs.  Two forms:
 //   pairs    a cluster of two CTAs has a tile of 256 x 256 (MMAs of cta_group::2: each CTA holds 128 rows of x and half the weight rows, so a stage's bytes feed twice the work);
 //            pairs are persistent, the MMAs run on into the next tile while the sums of the last are stored.
-//            A block takes 512 cycles, the MMAs' and the fill's of 32 KB; 8192 x 8192 x 4096: 234 us (2.35 PFLOP/s) in bursts, 276 at the power limit, copies and MMAs alone 176.
+//            A block takes 512 cycles, the MMAs' and the fill's of 32 KB; 8192 x 8192 x 4096: 230 us (2.39 PFLOP/s) in bursts, 276 at the power limit, copies and MMAs alone 176.
 //   tiles    a CTA has a tile of 128 x 128; where tiles are few, a cluster of up to eight CTAs shares its k, and adds the parts up through distributed shared memory in rank order.
 //            What bounds it is the fill from L2, some 48 bytes a clock and SM, and behind it the parts' way (150 x 2560 x 4096: 11.6 us, of them 4.2 to the first block).
 // Up to 32 rows of x take a form of their own, further down.
