@@ -201,6 +201,13 @@ def test_linear_long(K, cuda, M, N, K_):
     check_linear(K, cuda, M, N, K_, True, seed=M)
 
 
+@pytest.mark.parametrize("M,N,K_,wide", [(2049, 4097, 400, 0), (2100, 4098, 144, 0), (1500, 4100, 272, 2), (2303, 4099, 128, 4), (2049, 4104, 272, 0), (600, 1003, 128, 0), (600, 1002, 1040, 0)])
+@pytest.mark.parametrize("f32", [True, False])
+def test_linear_rows_of_any_alignment(K, cuda, M, N, K_, wide, f32):
+    """Pairs' tiles and single ones whose rows begin on 2, 4, 8 and 16 bytes."""
+    check_linear(K, cuda, M, N, K_, f32, seed=N, wide=wide)
+
+
 @pytest.mark.parametrize("M", [4, 40, 100, 300, 1500])
 def test_linear_what_is_not_finite_stays_in_its_row_and_column(K, cuda, M):
     N, K_ = 300, 400
