@@ -613,7 +613,7 @@ typedef struct SxbF8View {
 /* Residual's addition and norm.  s = x + y, rounded to x's type; n = s / sqrt(mean(s^2) + eps) * weight (FP32 [d], the factor itself, NULL: 1; FP32
  * throughout, the squares' sum too: a row whose squares sum to more than FP32 holds becomes zeros, an s * weight beyond it counts as an infinity); normed = 0: n = s, no norm.  Outputs, each may be NULL, one
  * at least given: total [T, d] = s in x's type (with y only; may be x or y itself), out [T, d] BF16 = n, codes and scales (both or none): per block of 128, scale = the larger of
- * max|n| / 448 and 2^-64, code = n / scale (448 n / max|n|) to the nearest, ties to even.  A block that holds a NaN or an infinity has a NaN scale and reads back as NaN.
+ * max|n| / 448 and 2^-64, code = n / scale (448 n / max|n|, to the nearest FP32) to the nearest, ties to even.  A block that holds a NaN or an infinity has a NaN scale and reads back as NaN.
  * y: NULL, BF16 or FP32 (y_act).  act: BF16 or FP32, of x and total.  d = 16 .. 32768, a multiple of 16; T = 1 .. 2^24; eps at least 2^-100.  Strides in elements; every row 16-byte
  * aligned, scales 4-byte. */
 typedef struct SxbAddNormArgs {

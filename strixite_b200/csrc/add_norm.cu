@@ -55,17 +55,18 @@ __device__ inline float reciprocal(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// A block's values v, `most` their largest magnitude, to what its codes are rounded from: 448 v / most to the last bit (a quotient, put right by its remainder), so that values that
-// stand between two codes round to the even one, as the definition says, whatever the row's factor r.  Where the scale is its least, v r / scale.
+// A block's values v, `most` their largest magnitude, to what its codes are rounded from: the nearest FP32 of 448 v / most (a quotient by Newton's method: v times an approximate reciprocal, put right
+// by its remainder, which one multiply-add gives; 448 comes in with the correction, so that nothing is rounded before it), whatever the row's factor r.  A value that stands between two codes stays
+// there and goes to the even one, as the definition says; one that is not a tie but within 2^-25 of it may round as the tie.  Where the scale is its least, v r / scale.
 __device__ inline void f8_codes(float (&v)[kVec], float most, float exact, float r, float scale) {
     const bool least = !(exact >= kF8Least);  // zeros and NaN too
-    const float shrink = most >= 0x1p100f ? 0x1p-40f : 1.f, top = kF8Top * shrink, by = least ? 1.f : most * shrink;
-    const float inv = least ? __fdiv_rn(r, scale) : reciprocal(by);
-    const uint64_t tops = pair(least ? 1.f : top, least ? 1.f : top), invs = pair(inv, inv), minus = pair(least ? 0.f : -by, least ? 0.f : -by), again = pair(least ? 0.f : inv, least ? 0.f : inv);
+    const float shrink = most >= 0x1p100f ? 0x1p-40f : 1.f, by = most * shrink;
+    const float inv = least ? __fdiv_rn(r, scale) : reciprocal(by), top = least ? 1.f : kF8Top * shrink, put = least ? 0.f : inv * top;
+    const uint64_t tops = pair(top, top), invs = pair(inv, inv), minus = pair(least ? 0.f : -by, least ? 0.f : -by), puts = pair(put, put);
 #pragma unroll
     for (int i = 0; i < kVec; i += 2) {
-        const uint64_t t = mul_pair(pair(v[i], v[i + 1]), tops), q = mul_pair(t, invs);
-        unpair(fma_pair(fma_pair(q, minus, t), again, q), v[i], v[i + 1]);
+        const uint64_t x = pair(v[i], v[i + 1]), q = mul_pair(x, invs);
+        unpair(fma_pair(q, tops, mul_pair(fma_pair(q, minus, x), puts)), v[i], v[i + 1]);
     }
 }
 // The values as they are stored in TX.
