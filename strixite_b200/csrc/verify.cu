@@ -10,7 +10,7 @@
 // FP32 8.3 together, one row 6.3.  A CTA a chunk, its parts joined by barriers, took 108 us for the 64 sequences where a warp a chunk takes 52 (before the differences were read by batches).
 //
 // A border's error: a term takes c (x - max) in FP32 (2^-23 of the exponent, which is small where the term is large), one ex2 (2^-22), sums of up to sixteen
-// terms and then seven more in FP32; chunks are joined in FP64, where the exponents are exact, and no logit is too large for them.
+// terms and then seven more in FP32; chunks are joined in FP64, where the exponents are exact.  No finite logit is too large for either.
 
 #include "skinny_mma.cuh"
 
@@ -121,10 +121,12 @@ __device__ inline float warp_max_nan(float v) {
     asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
-// 2^(c (x - best)) of two, each with the rounding that one alone has.
-__device__ inline uint64_t weight_pair(float x0, float x1, uint64_t minus_best, uint64_t c) {
+// 2^(c (x - best)), of one and of two.  The difference is taken of halves, its factor twice c (finite: temperatures are 2^-126 at least): two logits may lie further apart than FP32 reaches and
+// still both count, at temperatures as large as they are.  But for subnormal logits, whose last bit no exponent shows, halves round as the whole.
+__device__ inline float weight_of(float x, float half_best, float twice_c) { return exp2_of(__fmul_rn(fmaf(x, 0.5f, -half_best), twice_c)); }
+__device__ inline uint64_t weight_pair(float x0, float x1, uint64_t minus_half_best, uint64_t twice_c) {
     float e0, e1;
-    unpair(mul_pair(add_pair(pair(x0, x1), minus_best), c), e0, e1);
+    unpair(mul_pair(fma_pair(pair(x0, x1), pair(0.5f, 0.5f), minus_half_best), twice_c), e0, e1);
     return pair(exp2_of(e0), exp2_of(e1));
 }
 
@@ -172,7 +174,7 @@ __device__ inline ChunkStat chunk_stat(const Row<T> &r, int chunk, const Loaded 
     uint64_t sum[2] = {0, 0};
     int at = 0x7fffffff;
     if (most > -INFINITY && most < INFINITY) {
-        const uint64_t minus = pair(-most, -most), cc = pair(c, c);
+        const uint64_t minus = pair(-0.5f * most, -0.5f * most), cc = pair(2.f * c, 2.f * c);
 #pragma unroll
         for (int j = 0; j < kPerLane; ++j) {
             float v[VE];
@@ -334,7 +336,7 @@ struct OfTarget {  // 2^(c (x - best)), nothing for the token `without`
     __device__ inline void weights(int piece, float (&w)[VE]) const {
         Row<TX>::values(r.raw(piece), w);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = r.token(piece) + i == without ? 0.f : exp2_of((w[i] - best) * c);
+        for (int i = 0; i < VE; ++i) w[i] = r.token(piece) + i == without ? 0.f : weight_of(w[i], 0.5f * best, 2.f * c);
     }
 };
 template <typename TX, typename TD>
@@ -347,7 +349,7 @@ struct OfDifference {  // max(p - q, 0)
     __device__ inline bool together() const { return sizeof(TX) == sizeof(TD) && r.mis == q.mis; }  // the rows' pieces hold the same tokens
     __device__ inline void differ(float (&w)[VE], const float (&d)[VE]) const {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = fmaxf(exp2_of((w[i] - best) * c) * inv - exp2_of((d[i] - q_best) * c) * q_inv, 0.f);
+        for (int i = 0; i < VE; ++i) w[i] = fmaxf(weight_of(w[i], 0.5f * best, 2.f * c) * inv - weight_of(d[i], 0.5f * q_best, 2.f * c) * q_inv, 0.f);
     }
     __device__ inline void weights(int piece, float (&w)[VE]) const {
         float d[VE];
