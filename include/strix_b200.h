@@ -650,7 +650,7 @@ int sxb_linear_f8(const SxbLinearF8Args *args, sxb_stream_t stream);
  * known, the others drafted, and the target's logits [T, ld >= V] (BF16 or FP32: act; masked tokens -inf).  With p_i = softmax(logits of row i / temperature[b]) and q_i the same of
  * draft_logits [T, draft_ld >= V] (draft_act; row i is what row i + 1's token was drawn from, a sequence's last row is not read), or all of it on the drafted token if draft_logits is NULL:
  * the token x of row i + 1 is kept if u[i] * q_i(x) < p_i(x).  At the first that is not, the sequence's next token is drawn from max(p_i - q_i, 0); if all are kept, from p of the last
- * row: the lowest token up to which more than u_pick[b] of the sum has come.  A difference that sums to zero: p instead.  temperature (NULL: 1) of 0: the largest logit, the lowest token among equals;
+ * row: the lowest token up to which more than u_pick[b] of the sum has come.  A difference that sums to 2^-18 or less, which may be rounding alone: p instead.  temperature (NULL: 1) of 0: the largest logit, the lowest token among equals;
  * no random number is used.  Probabilities in FP32 (a draw finds no
  * token below 2^-125 of the row's largest), sums of chunks in FP64; a random number within some 2^-22 of a border may fall on either side of it.
  * Out: next_ids [T], for each row the token that comes behind it (kept drafts, then the drawn token), -1 in the rows behind; n_new [B] = tokens kept + 1; logp [T] (or NULL) = log of

@@ -27,6 +27,9 @@ constexpr int64_t kMaxV = 1 << 20, kMaxB = 8192;
 constexpr int kMaxChunks = (int)(kMaxV / (4 * kPieces)) + 1, kMaxRun = (kMaxChunks + kMinRanks - 1) / kMinRanks;  // of a row; of a CTA's share of one
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994531;
+// Of a sum of max(p - q, 0): that much may be rounding alone.  Probabilities are within 2^-19 of their size; where rows of the same numbers begin at different places in sixteen bytes or differ in
+// type their chunks are not the same tokens, and their sums not the same bits.  A draft is refused with that chance at most, so what is drawn keeps its distribution to 2^-18.
+constexpr double kNoDifference = 0x1p-18;
 
 enum { kBadLogits = 1, kBadDraft = 2, kBadId = 3, kBadRandom = 4, kBadTemperature = 5, kBadRange = 6 };
 
@@ -347,9 +350,11 @@ struct OfDifference {  // max(p - q, 0)
     static constexpr int VE = Row<TX>::VE;
     __device__ inline int token(int piece) const { return r.token(piece); }
     __device__ inline bool together() const { return sizeof(TX) == sizeof(TD) && r.mis == q.mis; }  // the rows' pieces hold the same tokens
+    // Products and difference are rounded each by itself: equal probabilities leave nothing (a fused multiply-add would leave the other product's rounding), and a run's sum has a weight behind
+    // it wherever it is computed again.
     __device__ inline void differ(float (&w)[VE], const float (&d)[VE]) const {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = fmaxf(weight_of(w[i], 0.5f * best, 2.f * c) * inv - weight_of(d[i], 0.5f * q_best, 2.f * c) * q_inv, 0.f);
+        for (int i = 0; i < VE; ++i) w[i] = fmaxf(__fsub_rn(__fmul_rn(weight_of(w[i], 0.5f * best, 2.f * c), inv), __fmul_rn(weight_of(d[i], 0.5f * q_best, 2.f * c), q_inv)), 0.f);
     }
     __device__ inline void weights(int piece, float (&w)[VE]) const {
         float d[VE];
@@ -613,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 2) verify_decide_kernel(const Verify
         double sums[kMaxRanks];
         for (int k = 0; k < ranks; ++k) sums[k] = *cluster.map_shared_rank(&total_s, k), total += sums[k];
         cluster.sync();  // nobody's sum is read from here on
-        if (total > 0) {
+        if (total > kNoDifference) {
             const double target = (double)u_pick * total;
             bool found = false;
             for (int k = 0; k < ranks; ++k) {

@@ -1,10 +1,11 @@
-"""Calls of the operators around the head at which their formulas are easily missed: FP32 values between two codes, logits at FP32's ends."""
+"""Calls of the operators around the head at which their formulas are easily missed: FP32 values between two codes, logits at FP32's ends, differences of two distributions that
+are zero or small."""
 import numpy as np
 import pytest
 import torch
 
 import head_plain as P
-from test_gpu_head import batch, check, gen
+from test_gpu_head import batch, check, gen, run_verify
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +85,82 @@ def test_verify_draws_from_chunks_of_far_tokens_alone(K, cuda, f32):
     s["logits"][:, 20002] = 3e38
     ids, n, _ = check(K, cuda, s)
     assert torch.all(n == 1) and torch.all(ids[[0, 1, 4, 5, 7]] == 0)
+
+
+def laid_out(dev, rows, dtype, lead):
+    """Rows [T, V] as they are in a wider buffer, each `lead` elements behind a multiple of sixteen bytes."""
+    T, V = rows.shape
+    wide = torch.zeros((T, (V + lead + 15) // 8 * 8), dtype=dtype, device=dev)
+    wide[:, lead:lead + V] = rows
+    return wide[:, lead:lead + V]
+
+
+LAYOUTS = [(torch.float32, 0, torch.float32, 0), (torch.float32, 1, torch.float32, 1), (torch.float32, 1, torch.float32, 0), (torch.float32, 2, torch.float32, 3), (torch.bfloat16, 0, torch.bfloat16, 0),
+           (torch.bfloat16, 5, torch.bfloat16, 5), (torch.bfloat16, 0, torch.bfloat16, 3), (torch.float32, 0, torch.bfloat16, 0), (torch.bfloat16, 1, torch.float32, 2)]
+
+
+def drawn(K, dev, p, q, drafted, u, picks, t, layout):
+    """Two rows a sequence, each the same p and q [V], the drafted token refused by u: the token drawn for each of picks."""
+    (xt, xl, qt, ql), B, V = layout, len(picks), p.shape[0]
+    s = dict(logits=laid_out(dev, p.expand(2 * B, V), xt, xl), draft=laid_out(dev, q.expand(2 * B, V), qt, ql), ids=torch.full((2 * B,), drafted, dtype=torch.int32, device=dev),
+             q_start=torch.arange(0, 2 * B + 1, 2, dtype=torch.int32, device=dev), u=torch.full((2 * B,), u, device=dev), u_pick=torch.tensor(picks, dtype=torch.float32, device=dev),
+             t=torch.full((B,), t, device=dev))
+    assert torch.equal(s["logits"][0].float(), p) and torch.equal(s["draft"][0].float(), q)
+    ids, n, lp, err = run_verify(K, dev, s)
+    assert err.tolist() == [0, 0, 0, 0] and torch.all(n == 1) and torch.all(ids[1::2] == -1)
+    return ids[::2].tolist(), lp[::2]
+
+
+def centres(p):
+    """The middles of the tokens' shares of [0, 1), of tokens that have some."""
+    p = p / p.sum()
+    return [(i, c - w / 2) for i, (w, c) in enumerate(zip(p, np.cumsum(p))) if w > 1e-3]
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("V", [9, 1000, 9001])
+def test_verify_equal_distributions_draw_from_the_target(K, cuda, layout, V):
+    """The drafter's row is the target's, the drafted token masked in both: the difference is zero, whatever type and place the rows have, and the token comes from p."""
+    g = gen(V, cuda)
+    p = 2 * torch.randn(V, generator=g, device=cuda)
+    p[torch.randperm(V, generator=g, device=cuda)[40:]] -= 30
+    p = p.to(torch.bfloat16).float()
+    m = V // 3
+    p[m] = -float("inf")
+    want = centres(P.softmax(P.f64(p), 0.75))
+    said, lp = drawn(K, cuda, p, p, m, 0.0, [c for _, c in want], 0.75, layout)
+    assert said == [i for i, _ in want]
+    logs = np.log(P.softmax(P.f64(p), 0.75)[said])
+    assert np.all(np.abs(P.f64(lp) - logs) <= P.P_OFF + 4 * P.U * np.abs(logs))
+
+
+@pytest.mark.parametrize("layout", [l for l in LAYOUTS if l[0] == l[2] and l[1] == l[3]])
+def test_verify_equal_probabilities_have_no_weight(K, cuda, layout):
+    """Weights that are powers of two, so that both sums are exact and alike: all tokens but two have the same chance twice, and the one that has more of it now is drawn for every number."""
+    V, a, b = 5000, 4321, 17
+    p = -torch.randint(0, 12, (V,), generator=gen(1, cuda), device=cuda).float()
+    p[a], p[b] = 0.0, -6.0
+    q = p.clone()
+    q[a], q[b] = -6.0, 0.0
+    said, _ = drawn(K, cuda, p, q, b, 1 - 2.0 ** -24, [0.0, 2.0 ** -24, 0.25, 1 - 2.0 ** -24], float(np.float32(1.4426950408889634)), layout)
+    assert said == [a] * 4
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("step", [2.0 ** -8, 2.0 ** -10])
+def test_verify_draws_from_a_small_difference(K, cuda, layout, step):
+    """Sixteen tokens of 1 / 16, of which the drafter takes `step` from four and gives it to four others: a quarter of the difference's sum 4 step each.  A draw is off by at most
+    2^-17 / (4 step), an eighth of which the middles are from their borders."""
+    V = 9001
+    at = np.sort(np.random.default_rng(5).choice(V, 16, replace=False))
+    pp, qq = np.full(16, 1 / 16), np.full(16, 1 / 16)
+    more, less = [2, 5, 11, 15], [0, 4, 8, 13]
+    qq[more] -= step
+    qq[less] += step
+    p, q = (torch.full((V,), -float("inf"), device=cuda) for _ in range(2))
+    for t, of, kind in ((p, pp, layout[0]), (q, qq, layout[2])):
+        t[torch.from_numpy(at).to(cuda)] = torch.from_numpy(np.log(of)).to(cuda).to(kind).float()
+    rest = np.maximum(P.softmax(P.f64(p), 1.0) - P.softmax(P.f64(q), 1.0), 0)
+    want = centres(rest)
+    said, _ = drawn(K, cuda, p, q, int(at[0]), 1 - 2.0 ** -24, [c for _, c in want], 1.0, layout)
+    assert said == [i for i, _ in want]
