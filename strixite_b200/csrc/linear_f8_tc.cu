@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 acc.advance(S::kAccs);
             }
-            if (*abort_v) break;
+            if (__any_sync(0xffffffffu, *abort_v)) break;  // as one: lanes that read it at different times would not meet again in the stores below
             if (CTAS == 1 && a.split > 1) {
                 // this CTA's part to shared memory: the ring is not needed any more (its one item's MMAs have completed); sixteen bytes' place within eight of them by the row, so
                 // that eight lanes' stores touch all banks
@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                     for (int k = 0; k < NB; ++k) sum[k] = fmaf(v[k], __shfl_sync(0xffffffffu, now[i], k), sum[k]);
                 }
             }
-            if (*abort_v) break;
+            if (__any_sync(0xffffffffu, *abort_v)) break;  // as one, see above
             const int row = warp * 32 + lane, n = item * kTileM + row;
             if (a.split > 1) {
 #pragma unroll

@@ -1,11 +1,11 @@
 """Calls of the operators around the head at which their formulas are easily missed: FP32 values between two codes, logits at FP32's ends, differences of two distributions that
-are zero or small."""
+are zero or small, waits that run out."""
 import numpy as np
 import pytest
 import torch
 
 import head_plain as P
-from test_gpu_head import batch, check, gen, run_verify
+from test_gpu_head import batch, check, gen, operands, run_verify
 
 pytestmark = pytest.mark.gpu
 
@@ -49,6 +49,36 @@ def test_codes_of_weights_between_two_numbers(K, cuda):
     want = np.round(t * 8) / 8
     want[5, 9] = 448
     assert np.array_equal(P.f64(K.quantize_f8(torch.from_numpy(w.astype(np.float32)).to(cuda)).q), want)
+
+
+# ---- product -------------------------------------------------------------------------------------------------------------------------
+
+def gives_up(K, dev, lib, M, N, K_, slot, f32):
+    """The product with CTA 0 told to leave stage `slot` out: the kernel returns, the status names the role, the next call has the bits of the call before."""
+    x, xs, w, ws = operands(K, dev, M, N, K_, slot)
+    v, out = K.F8View(w, ws), [torch.full((M, N), float("nan"), dtype=torch.float32 if f32 else torch.bfloat16, device=dev) for _ in range(3)]
+    K.linear_f8(x, xs, v, out[0])
+    K.check_dense_status("warm-up")
+    try:
+        K.set_wait_limit(2_000_000)
+        assert lib.sxb_test_skip_ring_slot(slot) == 0
+        K.linear_f8(x, xs, v, out[1])
+        torch.cuda.synchronize()
+    finally:
+        lib.sxb_test_skip_ring_slot(-1)
+        K.set_wait_limit(2_000_000_000)
+    with pytest.raises(K.Error, match=r"skipped fill: a tcgen05 kernel gave up a wait at work item \d+ \((an MMA warp|the epilogue|the activation copy)"):
+        K.check_dense_status("skipped fill")
+    K.linear_f8(x, xs, v, out[2])
+    K.check_dense_status("after")
+    assert torch.equal(out[2], out[0]) and not bool(torch.isnan(out[2]).any())
+
+
+@pytest.mark.parametrize("M,N,K_,slot", [(2049, 4099, 1024, 0), (2049, 4099, 1024, 10), (600, 1003, 1024, 3), (2048, 4096, 1024, 9), (600, 1000, 1024, 5)])
+@pytest.mark.parametrize("f32", [True, False])
+def test_linear_gives_up_a_wait_whatever_way_its_rows_leave(K, cuda, lib, M, N, K_, slot, f32):
+    """Rows that turn in shared memory, leave from registers or by tensor copies."""
+    gives_up(K, cuda, lib, M, N, K_, slot, f32)
 
 
 # ---- verification --------------------------------------------------------------------------------------------------------------------
