@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     constexpr int PER = S::kBlocks;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *const smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ uint64_t full_bar[S::kStages], done_bar[S::kStages], drained_bar[S::kStages];
+    __shared__ uint64_t full_bar[S::kStages], done_bar[S::kStages], drained_bar[S::kStages], drain_bar;
     __shared__ uint32_t tmem_base_smem;
     __shared__ int abort_flag;
 
@@ -584,6 +584,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&done_bar[s], 1), mbar_init(&drained_bar[s], kFewSumWarps);
+        mbar_init(&drain_bar, 1);
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fetch_map(&xmap), fetch_map(&wmap);
@@ -653,6 +654,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                 }
                 commit_to<1>(leader, &done_bar[turn.at]);
             }
+        // every MMA has completed before shared and tensor memory are given up (not skipped while aborting)
+        commit_to<1>(leader, &drain_bar);
+        mbar_wait(&drain_bar, 0u, nullptr, a.wait_limit_ns);
         __syncwarp();
     } else {
         // ===================== sums and stores =====================
@@ -718,7 +722,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         }
     }
 
-    if (*abort_v) {  // copies that a CTA issued, and MMAs, before it gave up are over within this time
+    if (*abort_v) {  // copies that a CTA issued before it gave up have landed within this time
         const unsigned long long t0 = global_ns();
         while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
     }

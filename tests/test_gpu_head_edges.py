@@ -81,6 +81,13 @@ def test_linear_gives_up_a_wait_whatever_way_its_rows_leave(K, cuda, lib, M, N, 
     gives_up(K, cuda, lib, M, N, K_, slot, f32)
 
 
+@pytest.mark.parametrize("M,N,K_,slot", [(16, 300, 2048, 0), (32, 300, 2048, 0), (16, 40000, 1024, 2), (32, 40000, 1024, 9), (4, 70000, 1024, 5), (9, 130, 144, 0)])
+@pytest.mark.parametrize("f32", [True, False])
+def test_linear_of_few_rows_gives_up_a_wait(K, cuda, lib, M, N, K_, slot, f32):
+    """Both widths, k shared by a cluster and not, the first tile of a CTA and a later one."""
+    gives_up(K, cuda, lib, M, N, K_, slot, f32)
+
+
 # ---- verification --------------------------------------------------------------------------------------------------------------------
 
 def far_apart(dev, V, f32, draft, seed):
