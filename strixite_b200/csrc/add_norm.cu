@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(LOOP ? 512 : 1024) add_norm_kernel(const NormA
                 for (int i = 0; i < kVec; ++i) most = max_nan(most, fabsf(s[j][i]));
 #pragma unroll
                 for (int off = 8; off > 0; off >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, off));
-                const float exact = __fdiv_rn(most * r, kF8Top), scale = f8_scale(most, exact);
+                const float exact = __fdiv_rn(most * r, kF8Top), scale = f8_scale(exact);
                 if (at < a.d) {
                     f8_codes(s[j], most, exact, r, scale);
                     const uint2 c = make_uint2(f8_quad(s[j][0], s[j][1], s[j][2], s[j][3]), f8_quad(s[j][4], s[j][5], s[j][6], s[j][7]));
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(256) quantize_f8_kernel(const TW *__restrict__
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) most = max(most, parts[i]);
-    const float largest = __uint_as_float(most), exact = __fdiv_rn(largest, kF8Top), s = f8_scale(largest, exact);
+    const float largest = __uint_as_float(most), exact = __fdiv_rn(largest, kF8Top), s = f8_scale(exact);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

@@ -10,8 +10,8 @@ constexpr int kF8Block = 128;
 constexpr float kF8Top = 448.0f;        // the largest e4m3 number
 constexpr float kF8Least = 0x1p-64f;    // of a scale: its reciprocal, and its product with another scale, stay normal FP32 numbers
 
-// The scale of a block whose largest magnitude is `most` (times a factor; NaN if one is), `exact` the 448th part of it.
-__device__ inline float f8_scale(float most, float exact) { return most < INFINITY && exact == exact ? fmaxf(exact, kF8Least) : qnan_f32(); }
+// The scale of a block, `exact` the 448th part of its largest magnitude: NaN if that is NaN or beyond FP32.
+__device__ inline float f8_scale(float exact) { return exact < INFINITY ? fmaxf(exact, kF8Least) : qnan_f32(); }
 __device__ inline uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // Two values to two codes (the first in the lower byte): nearest, ties to even, beyond +-448 the last number, NaN stays NaN.

@@ -51,6 +51,20 @@ def test_codes_of_weights_between_two_numbers(K, cuda):
     assert np.array_equal(P.f64(K.quantize_f8(torch.from_numpy(w.astype(np.float32)).to(cuda)).q), want)
 
 
+@pytest.mark.parametrize("T", [1, 3000])
+def test_norm_beyond_fp32_counts_as_an_infinity(K, cuda, T):
+    """s * weight still fits FP32, its product with the row's factor does not: the block is lost, the others are not."""
+    x = torch.full((T, 4096), 1e-3, device=cuda)
+    x[:, 130] = 1.0
+    codes, scales = torch.zeros(x.shape, dtype=torch.uint8, device=cuda).view(K.F8), torch.zeros((T, 32), device=cuda)
+    K.add_norm(x, weight=torch.full((4096,), 1e38, device=cuda), codes=codes, scales=scales)
+    v = codes.float() * scales.repeat_interleave(128, 1)
+    assert torch.all(scales[:, 1].isnan()) and torch.all(v[:, 128:256].isnan())
+    rest = torch.cat((scales[:, :1], scales[:, 2:]), 1)
+    n = 1e35 / np.sqrt((1 + 4095e-6) / 4096 + 1e-6)
+    assert np.all(np.abs(P.f64(rest) / (n / 448) - 1) <= P.NORM + 4 * P.U)
+
+
 # ---- product -------------------------------------------------------------------------------------------------------------------------
 
 def gives_up(K, dev, lib, M, N, K_, slot, f32):
