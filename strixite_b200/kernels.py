@@ -7,6 +7,7 @@ memory: BF16 activations may be passed as torch.bfloat16 or as raw uint16/int16 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import enum
 import struct
@@ -78,6 +79,15 @@ def _stream(stream) -> int:
             return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
         return torch.cuda.current_stream().cuda_stream
     return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _within(stream, device):
+    """The context in which what a call allocates, clears and reads itself is ordered with the kernels that it gives to `stream`."""
+    if stream is None or device.type != "cuda":
+        return contextlib.nullcontext()
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device) if stream else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)
 
 
 @dataclass
@@ -428,15 +438,16 @@ def quantize(w: torch.Tensor, G: int, bits: int, err: Optional[torch.Tensor] = N
     N, K = w.shape
     if bits not in (4, 8) or G not in (32, 64, 128) or K % G:
         raise Error(1, f"quantize: bits = {bits}, G = {G}, K = {K} unsupported")
-    q = torch.empty((N, K // 2 if bits == 4 else K), dtype=torch.uint8, device=w.device)
-    scale = torch.empty((N, K // G), dtype=torch.int16, device=w.device)
-    minv = torch.empty((N, K // G), dtype=torch.int16, device=w.device)
-    own = err is None
-    if own:
-        err = torch.zeros(4, dtype=torch.int32, device=w.device)
-    _check(_lib.load().sxb_quantize(_ptr(w), N, K, G, bits, _ptr(q), _ptr(scale), _ptr(minv), _ptr(err), _stream(stream)))
-    if own and int(err[0].item()) != 0:
-        raise Error(1, f"quantize: non-finite weight at [{int(err[1])}, {int(err[2])}]")
+    with _within(stream, w.device):
+        q = torch.empty((N, K // 2 if bits == 4 else K), dtype=torch.uint8, device=w.device)
+        scale = torch.empty((N, K // G), dtype=torch.int16, device=w.device)
+        minv = torch.empty((N, K // G), dtype=torch.int16, device=w.device)
+        own = err is None
+        if own:
+            err = torch.zeros(4, dtype=torch.int32, device=w.device)
+        _check(_lib.load().sxb_quantize(_ptr(w), N, K, G, bits, _ptr(q), _ptr(scale), _ptr(minv), _ptr(err), _stream(stream)))
+        if own and int(err[0].item()) != 0:
+            raise Error(1, f"quantize: non-finite weight at [{int(err[1])}, {int(err[2])}]")
     return QDeviceView(q, scale, minv, N, K, G, bits)
 
 
@@ -684,14 +695,15 @@ def quantize_f8(w: torch.Tensor, err: Optional[torch.Tensor] = None, stream=None
     if err is not None and (err.device != w.device or err.dtype not in _WORDS or not err.is_contiguous() or err.numel() < 3):
         raise Error(1, f"quantize_f8: err is {err.dtype} {tuple(err.shape)} on {err.device}, expected 3 or more contiguous int32 on {w.device}")
     N, K = w.shape
-    q = torch.empty((N, K), dtype=torch.uint8, device=w.device).view(F8)
-    scale = torch.empty((_blocks(N), _blocks(K)), dtype=torch.float32, device=w.device)
-    own = err is None
-    if own:
-        err = torch.zeros(4, dtype=torch.int32, device=w.device)
-    _check(_lib.load().sxb_quantize_f8(_ptr(w), _w_act(w), N, K, _ptr(q), _ptr(scale), _ptr(err), _stream(stream)))
-    if own and int(err[0].item()) != 0:
-        raise Error(1, f"quantize_f8: non-finite weight at [{int(err[1])}, {int(err[2])}]")
+    with _within(stream, w.device):
+        q = torch.empty((N, K), dtype=torch.uint8, device=w.device).view(F8)
+        scale = torch.empty((_blocks(N), _blocks(K)), dtype=torch.float32, device=w.device)
+        own = err is None
+        if own:
+            err = torch.zeros(4, dtype=torch.int32, device=w.device)
+        _check(_lib.load().sxb_quantize_f8(_ptr(w), _w_act(w), N, K, _ptr(q), _ptr(scale), _ptr(err), _stream(stream)))
+        if own and int(err[0].item()) != 0:
+            raise Error(1, f"quantize_f8: non-finite weight at [{int(err[1])}, {int(err[2])}]")
     return F8View(q, scale)
 
 

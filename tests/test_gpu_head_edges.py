@@ -1,5 +1,5 @@
 """Calls of the operators around the head at which their formulas are easily missed: FP32 values between two codes, logits at FP32's ends, differences of two distributions that
-are zero or small, waits that run out."""
+are zero or small, waits that run out, other streams."""
 import numpy as np
 import pytest
 import torch
@@ -215,3 +215,27 @@ def test_verify_draws_from_a_small_difference(K, cuda, layout, step):
     want = centres(rest)
     said, _ = drawn(K, cuda, p, q, int(at[0]), 1 - 2.0 ** -24, [c for _, c in want], 1.0, layout)
     assert said == [i for i, _ in want]
+
+
+# ---- streams -------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_quantize_on_another_stream(K, cuda, raw):
+    """The call's own error words are cleared, written and read on the stream that it was given, not on the current one, which is busy."""
+    w = torch.ones((200, 256), device=cuda)
+    w[150, 17] = float("inf")
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)
+    with pytest.raises(K.Error, match=r"non-finite weight at \[150, 17\]"):
+        K.quantize_f8(w, stream=st.cuda_stream if raw else st)
+    with pytest.raises(K.Error, match=r"non-finite weight at \[150, \d+\]"):
+        K.quantize(w, 64, 8, stream=st.cuda_stream if raw else st)
+    w[150, 17] = 1.0
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)
+    v = K.quantize_f8(w, stream=st.cuda_stream if raw else st)
+    st.synchronize()
+    with torch.cuda.stream(st):
+        assert torch.all(v.scale == 1 / 448) and torch.all(v.q.float() == 448)
+    torch.cuda.synchronize()
