@@ -324,7 +324,13 @@ extern "C" int sxb_quantize_f8(const void *w, int act, int64_t N, int64_t K, uin
     SXB_CHECK(aligned16(w) && aligned16(q) && reinterpret_cast<uintptr_t>(scale) % 4 == 0, fn, ": w and q must be 16-byte aligned, scales 4-byte");
     const int64_t kb = (K + kF8Block - 1) / kF8Block, blocks = (N + kF8Block - 1) / kF8Block * kb;
     SXB_CHECK(blocks <= 0x7fffffff, fn, ": ", blocks, " blocks");
-    SXB_CHECK(apart(w, N * K * act_bytes(act), q, N * K), fn, ": q overlaps w");
+    const struct {
+        const char *name;
+        const void *p;
+        int64_t n;
+    } of[4] = {{"w", w, N * K * act_bytes(act)}, {"err", err, 12}, {"q", q, N * K}, {"scale", scale, 4 * blocks}};
+    for (int o = 1; o < 4; ++o)
+        for (int i = 0; i < o; ++i) SXB_CHECK(apart(of[o].p, of[o].n, of[i].p, of[i].n), fn, ": ", of[o].name, " [", of[o].p, "] overlaps ", of[i].name, " [", of[i].p, "]");
     auto st = static_cast<cudaStream_t>(stream);
     if (act == SXB_ACT_F32) quantize_f8_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const float *>(w), N, K, kb, q, scale, err);
     else quantize_f8_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const uint16_t *>(w), N, K, kb, q, scale, err);
