@@ -667,6 +667,12 @@ def _ld(t, what: str, name: str) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _matrix(t, what: str, name: str):
+    if t.dim() != 2:
+        raise Error(1, f"{what}: {name} is {tuple(t.shape)}, expected two dimensions")
+    return t.shape
+
+
 class F8View:
     """A weight in 8-bit floating point (SxbF8View): codes q [N, K] float8_e4m3fn, contiguous, scale [ceil(N / 128), ceil(K / 128)] FP32."""
 
@@ -710,8 +716,8 @@ def quantize_f8(w: torch.Tensor, err: Optional[torch.Tensor] = None, stream=None
 def add_norm(x, y=None, weight=None, eps=1e-6, total=None, out=None, codes=None, scales=None, norm=True, stream=None):
     """sxb_add_norm: s = x + y in x's type (x [T, d] BF16 or FP32, y BF16, FP32 or None) -> total (may be x or y), its norm times weight [d] FP32 (None: 1) -> out
     BF16, codes float8_e4m3fn with scales [T, ceil(d / 128)] FP32; each of them or None.  norm=False: s itself in the place of its norm."""
-    shape, dev, dt = x.shape, x.get_device(), x.dtype
-    T, d = shape
+    T, d = shape = _matrix(x, "add_norm", "x")
+    dev, dt = x.get_device(), x.dtype
     ok = dev == torch._C._cuda_getDevice() and dt in _ROWS
     x_ld = d if x.is_contiguous() else _ld(x, "add_norm", "x")
     yp = wp = tp = op = cp = sp = y_bf16 = 0
@@ -754,7 +760,7 @@ def add_norm(x, y=None, weight=None, eps=1e-6, total=None, out=None, codes=None,
 
 def linear_f8(x, x_scale, w: F8View, y, stream=None):
     """sxb_linear_f8: y [M, N] BF16 or FP32 = x [M, K] float8_e4m3fn (scales x_scale [M, ceil(K / 128)] FP32) times w^T."""
-    M, K = x.shape
+    M, K = _matrix(x, "linear_f8", "x")
     dev, dt = w.index, y.dtype
     if not (dev == torch._C._cuda_getDevice() and x.dtype is F8 and x_scale.dtype is torch.float32 and dt in _ROWS and x.get_device() == dev and x_scale.get_device() == dev
             and y.get_device() == dev and K == w.K and x_scale.shape == (M, w.blocks) and y.shape == (M, w.N)):
@@ -777,8 +783,8 @@ def verify_drafts(logits, ids, q_start, u, u_pick, next_ids, n_new, ws, err, dra
     """sxb_verify_drafts: rows q_start[b] .. q_start[b + 1] - 1 (int32 [B + 1]) are sequence b's: the tokens ids [T] int32 fed there, the drafted ones behind the first, the target's
     logits [T, V] BF16 or FP32, the drafter's (or None: its tokens are all that is known of it), random numbers u [T] and u_pick [B] FP32, temperature [B] FP32 (None: 1; 0: greedy)
     -> next_ids [T] int32 (-1 behind the last), n_new [B] int32, logp [T] FP32 or None.  err: 3 or more zeroed int32."""
-    shape, dev, B = logits.shape, logits.get_device(), n_new.numel()
-    T, V = shape
+    T, V = shape = _matrix(logits, "verify_drafts", "logits")
+    dev, B = logits.get_device(), n_new.numel()
     ok = (dev == torch._C._cuda_getDevice() and logits.dtype in _ROWS and ids.dtype is torch.int32 and ids.get_device() == dev
           and ids.numel() == T and ids.is_contiguous() and q_start.dtype is torch.int32 and q_start.get_device() == dev and q_start.numel() == B + 1 and q_start.is_contiguous()
           and u.dtype is torch.float32 and u.get_device() == dev and u.numel() == T and u.is_contiguous() and u_pick.dtype is torch.float32 and u_pick.get_device() == dev
