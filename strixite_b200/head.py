@@ -37,7 +37,8 @@ class HeadBuffers:
         self.scales = empty(max_tokens, -(-d // 128), dtype=torch.float32)
         self.logits = empty(max_tokens, V, dtype=torch.float32)
         self.ws = empty(K.verify_drafts_workspace_bytes(max_tokens, max_seqs, V), dtype=torch.uint8)
-        self.next_ids, self.logp = empty(max_tokens, dtype=torch.int32), empty(max_tokens, dtype=torch.float32)
+        self.said = empty(2, max_tokens, dtype=torch.int32)
+        self.next_ids, self.logp = self.said[0], self.said[1].view(torch.float32)
         self.n_new = empty(max_seqs, dtype=torch.int32)
         self.err = torch.zeros(4, dtype=torch.int32, device=device)
         self.device = self.total.device
@@ -52,12 +53,14 @@ class VerifyHead:
     def forward(self, x: torch.Tensor, y: Optional[torch.Tensor], ids: torch.Tensor, q_start: torch.Tensor, u: torch.Tensor, u_pick: torch.Tensor,
                 draft_logits: Optional[torch.Tensor] = None, temperature: Optional[torch.Tensor] = None):
         """x [T, d] BF16 the residual stream, y [T, d] the last sublayer's output or None; rows q_start[b] .. q_start[b + 1] - 1 are sequence b's, ids [T] the tokens fed there.
-        -> next_ids [T], n_new [B], logp [T] of kernels.verify_drafts, views of the buffers; the logits stay in them too."""
+        -> next_ids [T], n_new [B], logp [T] of kernels.verify_drafts, views of the buffers; the logits stay in them too.  Rows of no sequence (padding), or of a refused range, have -1 and NaN."""
         T, b, B = x.shape[0], self.buf, u_pick.shape[0]
         if T > b.max_tokens or B > b.max_seqs or x.dtype != torch.bfloat16:
             raise K.Error(1, f"VerifyHead: {T} rows of {x.dtype} of {B} sequences, the buffers hold {b.max_tokens} of BF16 of {b.max_seqs}")
         codes, scales, logits = b.codes[:T], b.scales[:T], b.logits[:T]
         next_ids, n_new, logp = b.next_ids[:T], b.n_new[:B], b.logp[:T]
+        # the verification writes the rows of sequences; the others would be an earlier step's.  As FP32 these bits are a NaN.  (3 us of a step of 98, 4096 x 131072, one row.)
+        b.said.fill_(-1)
         K.add_norm(x, y, weight=self.w.norm, eps=self.eps, total=None if y is None else b.total[:T], codes=codes, scales=scales)
         K.linear_f8(codes, scales, self.w.out, logits)
         K.verify_drafts(logits, ids, q_start, u, u_pick, next_ids, n_new, b.ws, b.err, draft_logits=draft_logits, temperature=temperature, logp=logp)

@@ -1,11 +1,11 @@
 """Calls of the operators around the head at which their formulas are easily missed: FP32 values between two codes, logits at FP32's ends, differences of two distributions that
-are zero or small, waits that run out, other streams."""
+are zero or small, waits that run out, other streams, padded steps."""
 import numpy as np
 import pytest
 import torch
 
 import head_plain as P
-from test_gpu_head import batch, check, gen, operands, run_verify
+from test_gpu_head import batch, check, gen, head, operands, run_verify
 
 pytestmark = pytest.mark.gpu
 
@@ -239,3 +239,24 @@ def test_quantize_on_another_stream(K, cuda, raw):
     with torch.cuda.stream(st):
         assert torch.all(v.scale == 1 / 448) and torch.all(v.q.float() == 448)
     torch.cuda.synchronize()
+
+
+def test_head_rows_of_no_sequence(K, cuda):
+    """A padded step: rows of no sequence and of a refused range say so, instead of what an earlier step left there."""
+    h, buf = head(K, cuda)
+    g = gen(31, cuda)
+    x = torch.randn((12, 512), generator=g, device=cuda).to(torch.bfloat16)
+    ids = torch.randint(0, 3000, (12,), generator=g, device=cuda, dtype=torch.int32)
+    u, u_pick = torch.rand(12, generator=g, device=cuda), torch.rand(3, generator=g, device=cuda)
+    h.forward(x, None, ids, torch.tensor([0, 4, 8, 12], dtype=torch.int32, device=cuda), u, u_pick)
+    h.check_errors()
+    next_ids, n_new, logp = h.forward(x, None, ids, torch.tensor([1, 3, 3, 7], dtype=torch.int32, device=cuda), u, u_pick)
+    h.check_errors()
+    assert n_new.tolist()[1] == 0
+    for row in (0, 7, 8, 9, 10, 11):
+        assert int(next_ids[row]) == -1 and bool(logp[row].isnan())
+    P.check_verified(buf.logits[:12], ids, torch.tensor([1, 3, 3, 7]), u, u_pick, None, None, next_ids, n_new, logp)
+    next_ids, n_new, logp = h.forward(x, None, ids, torch.tensor([0, 4, 2, 12], dtype=torch.int32, device=cuda), u, u_pick)
+    assert n_new.tolist()[1:] == [0, 0] and torch.all(next_ids[4:] == -1) and torch.all(logp[4:].isnan())
+    with pytest.raises(K.Error, match="at sequence"):
+        h.check_errors()
