@@ -652,9 +652,10 @@ int sxb_linear_f8(const SxbLinearF8Args *args, sxb_stream_t stream);
  * the token x of row i + 1 is kept if u[i] * q_i(x) < p_i(x).  At the first that is not, the sequence's next token is drawn from max(p_i - q_i, 0); if all are kept, from p of the last
  * row: the lowest token up to which more than u_pick[b] of the sum has come.  A difference that sums to 2^-18 or less, which may be rounding alone: p instead.  temperature (NULL: 1) of 0: the largest logit, the lowest token among equals;
  * no random number is used.  Probabilities in FP32 (a draw finds no
- * token below 2^-125 of the row's largest), sums of chunks in FP64; a random number within some 2^-22 of a border may fall on either side of it.
+ * token below 2^-125 of the row's largest), good to some 2^-19 of their size, sums of chunks in FP64: a random number may fall on either side of a border that it is close to, u[i] when u q and p are within
+ * 2^-17 of the larger of q and p, u_pick[b] within 2^-17, or 2^-17 / R where the difference drawn from sums to R.
  * Out: next_ids [T], for each row the token that comes behind it (kept drafts, then the drawn token), -1 in the rows behind; n_new [B] = tokens kept + 1; logp [T] (or NULL) = log of
- * each such token's p (greedy: of softmax(logits)), 0 in the rows behind.  A sequence without rows has n_new = 0; rows outside every sequence are left as they are.
+ * each such token's p (greedy: of softmax(logits)), the difference of two FP32 numbers, 0 in the rows behind.  A sequence without rows has n_new = 0; rows outside every sequence are left as they are.
  * ws: sxb_verify_drafts_workspace_bytes, device, 16-byte aligned, needs no clearing; calls that share it must be ordered.  T = 1 .. 2^20, V = 1 .. 2^20, B = 1 .. 8192.
  * Data errors, found in the rows that the decision reads (err = {1, row, code}): logits of a row that hold a NaN or +inf or nothing above -inf (code 1), a drafter's (2), a drafted token
  * outside 0 .. V - 1 (3), a random number outside [0, 1) (4), a temperature other than 0 below 2^-126, or not finite (5): n_new = 0, the sequence's

@@ -8,7 +8,7 @@ namespace sxb {
 
 constexpr int kF8Block = 128;
 constexpr float kF8Top = 448.0f;        // the largest e4m3 number
-constexpr float kF8Least = 0x1p-64f;    // of a scale: its reciprocal, and its product with another scale, stay normal FP32 numbers
+constexpr float kF8Least = 0x1p-64f;    // of a scale: its reciprocal stays a normal FP32 number, and its product with another scale loses no more than 2^-22 (2^-128 and more: the least ones are subnormal)
 
 // The scale of a block, `exact` the 448th part of its largest magnitude: NaN if that is NaN or beyond FP32.
 __device__ inline float f8_scale(float exact) { return exact < INFINITY ? fmaxf(exact, kF8Least) : qnan_f32(); }

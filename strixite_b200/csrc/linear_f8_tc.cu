@@ -7,7 +7,9 @@
 // Warp 8 brings x and w in stages of 128 k by tensor copies, warp 9 issues the MMAs.  Two forms:
 //   pairs    a cluster of two CTAs has a tile of 256 x 256 (MMAs of cta_group::2: each CTA holds 128 rows of x and half the weight rows, so a stage's bytes feed twice the work);
 //            pairs are persistent, the MMAs run on into the next tile while the sums of the last are stored.
-//            A block takes 512 cycles, the MMAs' and the fill's of 32 KB; 8192 x 8192 x 4096: 230 us (2.39 PFLOP/s) in bursts, 276 at the power limit, copies and MMAs alone 176.
+//            8192 x 8192 x 4096: 230 to 240 us (2.29 to 2.40 PFLOP/s) in bursts, 276 at the power limit, copies and MMAs alone 176; FP32 rows, which leave from registers, 304.  A pair has 448 blocks of
+//            some 890 cycles there (1.64 GHz), of which the tensor pipe is busy for 560: the rest is taken to be the
+//            hand-over (two accumulators, given back when the last of their columns has been read), which has not been measured apart.
 //   tiles    a CTA has a tile of 128 x 128; where tiles are few, a cluster of up to eight CTAs shares its k, and adds the parts up through distributed shared memory in rank order.
 //            What bounds it is the fill from L2, some 48 bytes a clock and SM, and behind it the parts' way (150 x 2560 x 4096: 11.6 us, of them 4.2 to the first block).
 // Up to 32 rows of x take a form of their own, further down.
@@ -780,6 +782,9 @@ int linear_f8_tc(const char *fn, const F8Args &g, cudaStream_t st) {
     if (g.M <= 16) return launch_few<16>(fn, a, st);
     if (g.M <= 32) return launch_few<32>(fn, a, st);
     const int64_t sms = sm_count(), pairs = (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256), tiles = (int64_t)((g.M + 127) / 128) * ((g.N + 127) / 128);
+    // Pairs from as many tiles on as there are places for them, whatever K is: 2304 x 2304 x 4096 (81 tiles, two rounds) 33 us, tiles of one CTA 35; 2304 x 4096 x 4096 35 and 46; 3000 x 4096 x 4096
+    // 48 and 65; 600 x 8192 x 4096 33 and 34; 2048 x 4096 x 256 8.6 and 9.5; 4096 x 4096 x 512 17.7 and 17.9, but 2304 x 2304 x 448 10.5 and 9.7.  Below, few tiles share their k and pairs cannot;
+    // the largest of those would gain (2048 x 2304 x 4096, 72 tiles: 20 and 26 us).
     if (g.M > 128 && pairs * 2 >= sms) return launch_tc8<2, 256>(fn, a, st);
     a.split = shares(tiles, g.kb, 11);
     return launch_tc8<1, 128>(fn, a, st);

@@ -1,12 +1,13 @@
 // Verification of drafted tokens against the target's probabilities, from given random numbers (include/strix_b200.h has the rules).
 //
 // Two launches.  The first reads every row's logits once, a warp a chunk of 4 KB: its largest logit (and, for greedy sequences, the first token that has it) and the sum of 2^(c (x -
-// max)), c = log2(e) / temperature.  What bounds it is memory; a logit takes four to five instructions, one of them the exponential.  The second, a CTA a sequence (a cluster of four or
+// max)), c = log2(e) / temperature.  A logit takes eight instructions, one of them the exponential, and issue slots, the
+// special-function unit and memory all stand at 55 to 60 %.  The second, a CTA a sequence (a cluster of four or
 // eight where the drafter gives its distribution), joins a row's chunks, tests the drafts, and draws the next token: from the chunks' sums it knows the chunk in which the random number
 // falls and reads that one again; only a difference of two distributions takes the whole row of both, once more, shared by the cluster.  It is bound by its chain of loads, of which
 // those that do not wait for the first launch are made ahead of its end.  Nothing is counted or left behind in the workspace: no atomics, and results do not depend on who comes first.
 //
-// 64 sequences of 1 to 8 rows of 131072 BF16 logits, the drafter's too (134 MB): 30 us (4.5 TB/s; half the issue slots and half the special-function unit's) and 15; 2 sequences of 8 rows of
+// 64 sequences of 1 to 8 rows of 131072 BF16 logits, the drafter's too (134 MB): 46 us, some 30 of them the first's (4.5 TB/s); 304 such rows in FP32 73 us (304 in BF16 48); 2 sequences of 8 rows of
 // FP32 8.3 together, one row 6.3.  A CTA a chunk, its parts joined by barriers, took 108 us for the 64 sequences where a warp a chunk takes 52 (before the differences were read by batches).
 //
 // A border's error: a term takes c (x - max) in FP32 (2^-23 of the exponent, which is small where the term is large), one ex2 (2^-22), sums of up to sixteen
@@ -96,7 +97,8 @@ struct Row {
 // The scale of a sequence's exponents; greedy sequences' log-probabilities are those of temperature 1.
 __device__ inline float exponent_scale(float t) { return t == 0.f ? kLog2e : __fdiv_rn(kLog2e, t); }
 
-// The first sequence that has the row, -1 if none has.  By a whole warp.
+// The first sequence that has the row, -1 if none has.  By a whole warp, 32 starts a step: nothing beside a row's logits for hundreds of sequences (512 of two rows of 4096: 53 us in all with a drafter's
+// distribution), what bounds thousands over few tokens (8192 over 130: 260 us, with a drafter's distribution 721).
 __device__ inline int sequence_of(const int32_t *q_start, int B, int row) {
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < B; b0 += 32) {
