@@ -90,6 +90,13 @@ def _within(stream, device):
     return torch.cuda.stream(stream)
 
 
+def _handed(stream, *tensors):
+    """What was allocated within `stream` goes to the caller, whose current stream may still use it when it is let go."""
+    if stream is not None and tensors[0].is_cuda:
+        for t in tensors:
+            t.record_stream(torch.cuda.current_stream(t.device))
+
+
 @dataclass
 class QDeviceView:
     """A quantized matrix on the device: Q4DeviceView / Q8DeviceView (runtime/q4_device.hpp:14-19) plus its bit width."""
@@ -448,6 +455,7 @@ def quantize(w: torch.Tensor, G: int, bits: int, err: Optional[torch.Tensor] = N
         _check(_lib.load().sxb_quantize(_ptr(w), N, K, G, bits, _ptr(q), _ptr(scale), _ptr(minv), _ptr(err), _stream(stream)))
         if own and int(err[0].item()) != 0:
             raise Error(1, f"quantize: non-finite weight at [{int(err[1])}, {int(err[2])}]")
+    _handed(stream, q, scale, minv)
     return QDeviceView(q, scale, minv, N, K, G, bits)
 
 
@@ -710,6 +718,7 @@ def quantize_f8(w: torch.Tensor, err: Optional[torch.Tensor] = None, stream=None
         _check(_lib.load().sxb_quantize_f8(_ptr(w), _w_act(w), N, K, _ptr(q), _ptr(scale), _ptr(err), _stream(stream)))
         if own and int(err[0].item()) != 0:
             raise Error(1, f"quantize_f8: non-finite weight at [{int(err[1])}, {int(err[2])}]")
+    _handed(stream, q, scale)
     return F8View(q, scale)
 
 
