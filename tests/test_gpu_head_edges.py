@@ -260,3 +260,36 @@ def test_head_rows_of_no_sequence(K, cuda):
     assert n_new.tolist()[1:] == [0, 0] and torch.all(next_ids[4:] == -1) and torch.all(logp[4:].isnan())
     with pytest.raises(K.Error, match="at sequence"):
         h.check_errors()
+
+
+def test_head_captured_with_a_drafter(K, cuda):
+    """A step with the drafter's distributions as a graph, replayed with other batches, padding rows among them: the bits of the same step run at once."""
+    h, buf = head(K, cuda)
+    g = gen(32, cuda)
+    T, B = 12, 3
+    x, y = (torch.zeros((T, 512), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    q, ids, starts = torch.zeros((T, 3000), device=cuda), torch.zeros(T, dtype=torch.int32, device=cuda), torch.tensor([0, 4, 8, 12], dtype=torch.int32, device=cuda)
+    u, u_pick, t = torch.zeros(T, device=cuda), torch.zeros(B, device=cuda), torch.tensor([1.0, 0.6, 0.0], device=cuda)
+    call = (x, y, ids, starts, u, u_pick, q, t)
+    h.forward(*call)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = h.forward(*call)
+    for at in ([0, 4, 8, 12], [1, 11, 11, 12], [0, 2, 5, 9], [3, 3, 3, 3]):
+        x.copy_(torch.randn((T, 512), generator=g, device=cuda))
+        y.copy_(torch.randn((T, 512), generator=g, device=cuda))
+        q.copy_(4 * torch.randn((T, 3000), generator=g, device=cuda))
+        starts.copy_(torch.tensor(at, dtype=torch.int32))
+        ids.copy_(torch.randint(0, 3000, (T,), generator=g, device=cuda))
+        u.copy_(torch.rand(T, generator=g, device=cuda))
+        u_pick.copy_(torch.rand(B, generator=g, device=cuda))
+        graph.replay()
+        torch.cuda.synchronize()
+        h.check_errors()
+        P.check_verified(buf.logits, ids, starts, u, u_pick, q, t, *out)
+        nobody = [r for r in range(T) if not at[0] <= r < at[3]]
+        assert torch.all(out[0][nobody] == -1) and torch.all(out[2][nobody].isnan())
+        graphed = [v.view(torch.int32).clone() for v in out]
+        h.forward(*call)
+        assert all(torch.equal(a, b.view(torch.int32)) for a, b in zip(graphed, out))
