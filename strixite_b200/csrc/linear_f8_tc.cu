@@ -8,8 +8,7 @@
 //   pairs    a cluster of two CTAs has a tile of 256 x 256 (MMAs of cta_group::2: each CTA holds 128 rows of x and half the weight rows, so a stage's bytes feed twice the work);
 //            pairs are persistent, the MMAs run on into the next tile while the sums of the last are stored.
 //            8192 x 8192 x 4096: 230 to 240 us (2.29 to 2.40 PFLOP/s) in bursts, 276 at the power limit, copies and MMAs alone 176; FP32 rows, which leave from registers, 304.  A pair has 448 blocks of
-//            some 890 cycles there (1.64 GHz), of which the tensor pipe is busy for 560: the rest is taken to be the
-//            hand-over (two accumulators, given back when the last of their columns has been read), which has not been measured apart.
+//            some 890 cycles there (1.64 GHz), of which the tensor pipe is busy for 560: the rest is taken to be the hand-over (two accumulators, given back when the last of their columns has been read), not measured apart.
 //   tiles    a CTA has a tile of 128 x 128; where tiles are few, a cluster of up to eight CTAs shares its k, and adds the parts up through distributed shared memory in rank order.
 //            What bounds it is the fill from L2, some 48 bytes a clock and SM, and behind it the parts' way (150 x 2560 x 4096: 11.6 us, of them 4.2 to the first block).
 // Up to 32 rows of x take a form of their own, further down.

@@ -1,9 +1,8 @@
 // Verification of drafted tokens against the target's probabilities, from given random numbers (include/strix_b200.h has the rules).
 //
 // Two launches.  The first reads every row's logits once, a warp a chunk of 4 KB: its largest logit (and, for greedy sequences, the first token that has it) and the sum of 2^(c (x -
-// max)), c = log2(e) / temperature.  A logit takes eight instructions, one of them the exponential, and issue slots, the
-// special-function unit and memory all stand at 55 to 60 %.  The second, a CTA a sequence (a cluster of four or
-// eight where the drafter gives its distribution), joins a row's chunks, tests the drafts, and draws the next token: from the chunks' sums it knows the chunk in which the random number
+// max)), c = log2(e) / temperature.  A logit takes eight instructions, one of them the exponential, and issue slots, the special-function unit and memory all stand at 55 to 60 %.  The second,
+// a CTA a sequence (a cluster of four or eight where the drafter gives its distribution), joins a row's chunks, tests the drafts, and draws the next token: from the chunks' sums it knows the chunk in which the random number
 // falls and reads that one again; only a difference of two distributions takes the whole row of both, once more, shared by the cluster.  It is bound by its chain of loads, of which
 // those that do not wait for the first launch are made ahead of its end.  Nothing is counted or left behind in the workspace: no atomics, and results do not depend on who comes first.
 //
